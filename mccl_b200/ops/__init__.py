@@ -6,3 +6,5 @@ native forward and backward kernels) and has a plain-PyTorch twin in
 """
 from .functional import (adamw_step, causal_attention, embedding, launch_count, linear, linear_cross_entropy, mlp_gelu, mlp_swiglu, native_ops_available, norm,
                          norm_residual, rope_attention, swiglu)  # noqa: F401
+from .paged import copy_pages, paged_append, paged_attention  # noqa: F401
+from .w4 import W4Weight, linear_w4, quantize_w4  # noqa: F401
