@@ -81,8 +81,9 @@ Cache cache_of(const at::Tensor& k, const at::Tensor& v, const at::Tensor& table
   c.table.width = as_int(table.size(1), op);
   c.table.page_size = as_int(k.size(2), op);
   c.table.pages = as_int(k.size(0), op);
-  MCCL_CHECK_TENSOR(static_cast<int64_t>(c.table.width) * c.table.page_size <= std::numeric_limits<int>::max(),
-                    op << ": a row of the page table holds more than 2^31 - 1 positions");
+  // positions are counted in 32 bits, rounded up to whole tiles
+  MCCL_CHECK_TENSOR(static_cast<int64_t>(c.table.width) * c.table.page_size <= std::numeric_limits<int>::max() - 64,
+                    op << ": a row of the page table holds more than 2^31 - 65 positions");
   c.kv_heads = as_int(k.size(1), op);
   c.head_dim = as_int(k.size(3), op);
   return c;
