@@ -3,6 +3,8 @@
 // The formula, for one sequence and head with query q: o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m), s_j = scale q . k_j over the visible
 // positions j and m their maximum.  Sums over any split of the positions join exactly: parts (m, l, o) combine with weights exp(m_part - m).
 #include "../core/launch.hpp"
+#include "../symm/cu_driver.hpp"
+#include "gemm_common.cuh"
 #include "half16.cuh"
 #include "ops.hpp"
 #include "serving.hpp"
@@ -52,6 +54,7 @@ struct Launch {
   long long* plan;              // tiles per warp, then the first tile of every sequence (and behind the last)
   float* part_ml;               // [warps][2][rows][2]
   float* part_o;                // [warps][2][rows][DP]
+  int* err;                     // set when a wait inside the kernel ran out
 };
 
 __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool real) {
@@ -99,33 +102,49 @@ struct Place {
 
 template <int DP, int WARPS, int STAGES>
 struct Shape {
-  static constexpr int kRowBytes = DP * 2;
-  static constexpr int kTileBytes = kTile * kRowBytes;   // of K, and of V
+  static constexpr int kTileBytes = kTile * DP * 2;   // of K, and of V
   static constexpr int kRing = WARPS * STAGES * 2 * kTileBytes;
-  static constexpr int kMasks = WARPS * STAGES * 4;
-  static constexpr int kSmem = kRing + kMasks + kSequences * 4 + (kSequences + 1) * 8 + 64;
+  static constexpr int kBars = WARPS * STAGES * 8, kMasks = WARPS * STAGES * 4;
+  static constexpr int kSmem = kRing + kBars + (kSequences + 1) * 8 + kSequences * 4 + kMasks + 1024;   // the ring starts on 1024 bytes
 };
 
-// Eight 16-byte pieces of neighbouring rows at the same place of their rows lie in eight different groups of banks.
+// A tile is DP / 64 blocks of 16 rows x 128 bytes, the eight 16-byte pieces of a row in the order of the 128-byte swizzle (64: for DP = 32), so that
+// the same piece of eight neighbouring rows lies in eight different groups of banks.
 template <int DP>
 __device__ __forceinline__ uint32_t swizzled(int row, int piece) {
-  const int p = DP >= 64 ? piece ^ (row & 7) : piece ^ ((row >> 1) & 3);
-  return static_cast<uint32_t>(row * (DP * 2) + p * 16);
+  if (DP == 32) return static_cast<uint32_t>(row * 64 + (piece ^ ((row >> 1) & 3)) * 16);
+  return static_cast<uint32_t>((piece >> 3) * (kTile * 128) + row * 128 + ((piece & 7) ^ (row & 7)) * 16);
 }
 
-template <typename H, int DP, int WARPS, int STAGES, int ROWS>
-__global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(Launch p) {
+// Box of 16 positions x 64 (32) columns of one page and head; zero fill outside the tensor, pages among it.
+__device__ __forceinline__ void load_box(uint32_t to, const CUtensorMap* map, uint32_t bar, int col, int at, int head, int page) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(to), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(col), "r"(at), "r"(head), "r"(page)
+      : "memory");
+}
+
+template <typename H, int DP, int WARPS, int STAGES, int ROWS, bool TMA>
+__global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, Launch p) {
   using S = Shape<DP, WARPS, STAGES>;
   using T = typename H::T;
-  extern __shared__ __align__(128) unsigned char smem[];
-  uint32_t* masks = reinterpret_cast<uint32_t*>(smem + S::kRing);
-  long long* first_tile = reinterpret_cast<long long*>(smem + S::kRing + S::kMasks);
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024 - (tc::smem_u32(smem_raw) & 1023)) & 1023);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kRing);
+  long long* first_tile = reinterpret_cast<long long*>(bars + WARPS * STAGES);
   int* length_of = reinterpret_cast<int*>(first_tile + kSequences + 1);
+  uint32_t* masks = reinterpret_cast<uint32_t*>(length_of + kSequences);
   __shared__ long long warp_sum[WARPS];
   const PagedAttentionArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t4 = lane & 3;
   const int room = a.table.width * a.table.page_size;
+  uint64_t* bar = bars + warp * STAGES;   // one per stage: its copies have landed
+  if (TMA && lane == 0) {
+    for (int i = 0; i < STAGES; ++i) tc::mbar_init(bar + i, 1);
+    tc::mbar_init_fence();
+  }
+  __syncwarp();
 
   ::mccl::pdl_wait();
   ::mccl::pdl_trigger();
@@ -215,7 +234,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(Launch p
   const uint32_t ring = tc::smem_u32(smem) + warp * (STAGES * 2 * S::kTileBytes);
   uint32_t* mask_ring = masks + warp * STAGES;
   Place load = begin;
-  int load_item = -1, load_tiles = 0, load_kv = 0;
+  int load_item = -1, load_tiles = 0, load_kv = 0, load_slot = -1, load_page = 0;
+  int ahead = 0;   // tiles that are loaded and not yet used
   Span span = {};
   const int* table = nullptr;
   auto settle = [&](Place& at, int& tiles) {   // past items without tiles and past the end of one
@@ -231,6 +251,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(Launch p
     if (before_end(load)) {
       if (load.item != load_item) {
         load_item = load.item;
+        load_slot = -1;
         const int b = load.item / p.items_per_sequence;
         load_kv = (load.item - b * p.items_per_sequence) / p.blocks_of_heads;
         span = span_of(length_of[b], a.window, a.sinks);
@@ -239,40 +260,59 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(Launch p
       const int tile = load.t + (load.t >= span.head ? span.skip : 0);
       const int r16 = lane & 15, j = tile * kTile + r16;
       const bool seen = j < span.length && (j >= span.first || j < a.sinks);
-      int page = -1, at = 0;
-      if (p.page_tiles > 0) {
-        const int slot = p.page_shift >= 0 ? tile >> p.page_shift : tile / p.page_tiles;
-        page = __ldg(table + slot);
-        at = (tile - slot * p.page_tiles) * kTile + r16;
-      } else if (seen) {
-        const int slot = j / a.table.page_size;
-        page = __ldg(table + slot);
-        at = j - slot * a.table.page_size;
-      }
-      const bool real = seen && page >= 0 && page < a.table.pages;
-      const uint32_t mask = __ballot_sync(0xffffffffu, real) & 0xffffu;
-      if (lane == 0) mask_ring[stage] = mask;
-      constexpr int kPieces = DP / 8, kRowsAtOnce = 32 / kPieces > 0 ? 32 / kPieces : 1;
-      const int piece = lane % kPieces, row0 = lane / kPieces;
       const uint32_t to = ring + stage * (2 * S::kTileBytes);
-      const T* k = static_cast<const T*>(a.k_pages.p) + load_kv * a.k_pages.head + piece * 8;
-      const T* v = static_cast<const T*>(a.v_pages.p) + load_kv * a.v_pages.head + piece * 8;
-      const bool column = piece * 8 < a.head_dim;
+      if (TMA) {   // the tile lies in one page
+        const int slot = p.page_shift >= 0 ? tile >> p.page_shift : tile / p.page_tiles;
+        if (slot != load_slot) {
+          load_slot = slot;
+          load_page = __ldg(table + slot);
+          if (load_page >= a.table.pages) load_page = -1;   // outside the tensor: zeros come back
+        }
+        const uint32_t mask = load_page >= 0 ? __ballot_sync(0xffffffffu, seen) & 0xffffu : 0u;
+        if (tc::elect_one()) {
+          mask_ring[stage] = mask;
+          tc::mbar_expect_tx(bar + stage, 2 * S::kTileBytes);
+          const uint32_t full = tc::smem_u32(bar + stage);
+          const int at = (tile - slot * p.page_tiles) * kTile;
+          constexpr int kBox = DP < 64 ? DP : 64;
 #pragma unroll
-      for (int i = 0; i < kTile / kRowsAtOnce; ++i) {
-        const int row = row0 + i * kRowsAtOnce;
-        const int its_page = __shfl_sync(0xffffffffu, page, row), its_at = __shfl_sync(0xffffffffu, at, row);
-        const bool good = column && ((mask >> row) & 1u);
-        const T* from_k = good ? k + its_page * a.k_pages.page + its_at * a.k_pages.token : static_cast<const T*>(a.k_pages.p);
-        const T* from_v = good ? v + its_page * a.v_pages.page + its_at * a.v_pages.token : static_cast<const T*>(a.v_pages.p);
-        const uint32_t spot = to + swizzled<DP>(row, piece);
-        copy16(spot, from_k, good);
-        copy16(spot + S::kTileBytes, from_v, good);
+          for (int c = 0; c < DP / kBox; ++c) {
+            load_box(to + c * (kTile * kBox * 2), &k_map, full, c * kBox, at, load_kv, load_page);
+            load_box(to + S::kTileBytes + c * (kTile * kBox * 2), &v_map, full, c * kBox, at, load_kv, load_page);
+          }
+        }
+        __syncwarp();
+      } else {
+        int page = -1, at = 0;
+        if (seen) {
+          const int slot = j / a.table.page_size;
+          page = __ldg(table + slot);
+          at = j - slot * a.table.page_size;
+        }
+        const uint32_t mask = __ballot_sync(0xffffffffu, seen && page >= 0 && page < a.table.pages) & 0xffffu;
+        if (lane == 0) mask_ring[stage] = mask;
+        constexpr int kPieces = DP / 8, kRowsAtOnce = 32 / kPieces;
+        const int piece = lane % kPieces, row0 = lane / kPieces;
+        const T* k = static_cast<const T*>(a.k_pages.p) + load_kv * a.k_pages.head + piece * 8;
+        const T* v = static_cast<const T*>(a.v_pages.p) + load_kv * a.v_pages.head + piece * 8;
+        const bool column = piece * 8 < a.head_dim;
+#pragma unroll
+        for (int i = 0; i < kTile / kRowsAtOnce; ++i) {
+          const int row = row0 + i * kRowsAtOnce;
+          const int its_page = __shfl_sync(0xffffffffu, page, row), its_at = __shfl_sync(0xffffffffu, at, row);
+          const bool good = column && ((mask >> row) & 1u);
+          const T* from_k = good ? k + its_page * a.k_pages.page + its_at * a.k_pages.token : static_cast<const T*>(a.k_pages.p);
+          const T* from_v = good ? v + its_page * a.v_pages.page + its_at * a.v_pages.token : static_cast<const T*>(a.v_pages.p);
+          const uint32_t spot = to + swizzled<DP>(row, piece);
+          copy16(spot, from_k, good);
+          copy16(spot + S::kTileBytes, from_v, good);
+        }
       }
       ++load.t;
       settle(load, load_tiles);
+      ++ahead;
     }
-    copy_commit();
+    if (!TMA) copy_commit();
   };
 
 #pragma unroll
@@ -283,8 +323,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(Launch p
   Place at = begin;
   int tiles = tiles_of(at.item);
   settle(at, tiles);
-  bool first_piece = true;
+  bool first_piece = true, ok = true;
   int stage = 0;
+  uint32_t parity = 0;
+  // where in a tile a lane's rows of the fragments are: of K (two groups of eight positions, two pieces) and of V (transposed); the pieces of
+  // step s are the ones of step 0 with s & 3 in the address bits above
+  const uint32_t k_lane = swizzled<DP>((lane >> 4) * 8 + (lane & 7), (lane >> 3) & 1), v_lane = swizzled<DP>(((lane >> 3) & 1) * 8 + (lane & 7), lane >> 4);
   while (before_end(at)) {
     // a new piece of an item: its queries
     const int item = at.item, b = item / p.items_per_sequence, hh = item - b * p.items_per_sequence;
@@ -311,8 +355,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(Launch p
 
     const int stop = item == end.item ? min(tiles, end.t) : tiles;
     for (; at.t < stop; ++at.t) {
-      copy_wait<STAGES - 2>();
-      __syncwarp();
+      if (TMA) {
+        ok = __all_sync(0xffffffffu, tc::mbar_wait(bar + stage, parity));
+        if (!ok) break;
+      } else {
+        copy_wait<STAGES - 2>();
+        __syncwarp();
+      }
+      --ahead;
       issue(stage == 0 ? STAGES - 1 : stage - 1);
       const uint32_t k_tile = ring + stage * (2 * S::kTileBytes), v_tile = k_tile + S::kTileBytes;
       const uint32_t mask = mask_ring[stage];
@@ -321,7 +371,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(Launch p
 #pragma unroll
       for (int step = 0; step < kSteps; ++step) {
         uint32_t r[4];
-        load_matrix(r, k_tile + swizzled<DP>((lane >> 4) * 8 + (lane & 7), step * 2 + ((lane >> 3) & 1)));
+        load_matrix(r, k_tile + (step >> 2) * (kTile * 128) + (k_lane ^ ((step & 3) << 5)));
         mma<H>(s[step & 1][0], q[step], r[0], r[1]);
         mma<H>(s[step & 1][1], q[step], r[2], r[3]);
       }
@@ -369,17 +419,34 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(Launch p
           const float2 back = unpair<H>(hi[i * 2 + h]);
           lo[i * 2 + h] = pair<H>(z[h][2 * i] - back.x, z[h][2 * i + 1] - back.y);
         }
+      // values of positions that are not seen may be anything: they are cleared, for zero times anything need not be zero
+      uint32_t clear[2] = {0xffffffffu, 0xffffffffu};
+      if (TMA && mask != 0xffffu) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          clear[i] = ((mask >> (i * 8 + 2 * t4)) & 1u ? 0x0000ffffu : 0u) | ((mask >> (i * 8 + 2 * t4 + 1)) & 1u ? 0xffff0000u : 0u);
+      }
 #pragma unroll
       for (int c = 0; c < kCols; c += 2) {
         uint32_t r[4];
-        load_matrix_t(r, v_tile + swizzled<DP>(((lane >> 3) & 1) * 8 + (lane & 7), c + (lane >> 4)));
+        load_matrix_t(r, v_tile + (c >> 3) * (kTile * 128) + (v_lane ^ (((c >> 1) & 3) << 5)));
+        if (TMA) {
+          r[0] &= clear[0];
+          r[1] &= clear[1];
+          r[2] &= clear[0];
+          r[3] &= clear[1];
+        }
         mma<H>(o[c], hi, r[0], r[1]);
         mma<H>(o[c + 1], hi, r[2], r[3]);
         mma<H>(o[c], lo, r[0], r[1]);
         mma<H>(o[c + 1], lo, r[2], r[3]);
       }
-      stage = stage == STAGES - 1 ? 0 : stage + 1;
+      if (++stage == STAGES) {
+        stage = 0;
+        parity ^= 1;
+      }
     }
+    if (TMA && !ok) break;
 
     // ---- the end of this piece: the result where it is the whole item, else a part for the join
     const bool complete = from == 0 && at.t == tiles;
@@ -409,7 +476,17 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(Launch p
     first_piece = false;
     settle(at, tiles);
   }
-  copy_wait<0>();
+  if (!TMA) copy_wait<0>();
+  if (TMA && !ok) {
+    if (lane == 0) atomicExch(p.err, 21);
+    for (; ahead > 0; --ahead) {   // copies that were issued must land before the block retires
+      tc::mbar_wait(bar + stage, parity, 1u << 20);
+      if (++stage == STAGES) {
+        stage = 0;
+        parity ^= 1;
+      }
+    }
+  }
 }
 
 // One block per sequence and query head whose tiles were shared out: the parts of its warps in order.
@@ -503,12 +580,27 @@ int rows_of(const PagedAttentionArgs& a) { return a.heads / a.kv_heads <= 8 ? 8 
 
 size_t plan_bytes() { return (kSequences + 2) * sizeof(long long); }
 
-template <typename H, int DP, int WARPS, int STAGES, int ROWS>
-cudaError_t launch(const Launch& p, cudaStream_t stream) {
+// Keys or values as boxes of 16 positions of one page and head.  False where the strides do not fit a tensor map.
+bool encode_pages(CUtensorMap* map, const PagedTensor& t, const PagedAttentionArgs& a, int dp) {
+  const CuDriver& cu = CuDriver::get();
+  if (!cu.loaded || !cu.TensorMapEncodeTiled) return false;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.head_dim), static_cast<cuuint64_t>(a.table.page_size), static_cast<cuuint64_t>(a.kv_heads),
+                              static_cast<cuuint64_t>(a.table.pages)};
+  // the stride of a dimension of one is never used and may be anything
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(t.token * 2), static_cast<cuuint64_t>((a.kv_heads > 1 ? t.head : 8) * 2),
+                                 static_cast<cuuint64_t>((a.table.pages > 1 ? t.page : 8) * 2)};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(dp < 64 ? dp : 64), kTile, 1, 1}, step[4] = {1, 1, 1, 1};
+  return cu.TensorMapEncodeTiled(map, a.type == Half16::bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, t.p, dims, strides, box, step,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, dp < 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename H, int DP, int WARPS, int STAGES, int ROWS, bool TMA>
+cudaError_t launch(const Launch& p, const CUtensorMap (&maps)[2], cudaStream_t stream) {
   constexpr int smem = Shape<DP, WARPS, STAGES>::kSmem;
-  static const cudaError_t rc = cudaFuncSetAttribute(paged_attention_kernel<H, DP, WARPS, STAGES, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static const cudaError_t rc = cudaFuncSetAttribute(paged_attention_kernel<H, DP, WARPS, STAGES, ROWS, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (rc != cudaSuccess) return rc;
-  MCCL_LAUNCH_PDL((paged_attention_kernel<H, DP, WARPS, STAGES, ROWS>), sm_count(), WARPS * 32, smem, stream, p);
+  MCCL_LAUNCH_PDL((paged_attention_kernel<H, DP, WARPS, STAGES, ROWS, TMA>), sm_count(), WARPS * 32, smem, stream, maps[0], maps[1], p);
   count_launch();
   if (!p.whole) {
     MCCL_LAUNCH_PDL((paged_attention_join_kernel<H, DP, ROWS>), dim3(p.a.heads, p.a.batch), 256, 0, stream, p);
@@ -517,14 +609,19 @@ cudaError_t launch(const Launch& p, cudaStream_t stream) {
   return ::mccl::launch_status();
 }
 
-template <typename H, int ROWS>
-cudaError_t by_dim(const Launch& p, cudaStream_t stream) {
+template <typename H, int ROWS, bool TMA>
+cudaError_t by_dim(const Launch& p, const CUtensorMap (&maps)[2], cudaStream_t stream) {
   switch (padded_dim(p.a.head_dim)) {
-    case 32: return launch<H, 32, 8, 8, ROWS>(p, stream);
-    case 64: return launch<H, 64, 8, 6, ROWS>(p, stream);
-    case 128: return launch<H, 128, 8, 3, ROWS>(p, stream);
-    default: return launch<H, 256, 4, 3, ROWS>(p, stream);
+    case 32: return launch<H, 32, 8, 8, ROWS, TMA>(p, maps, stream);
+    case 64: return launch<H, 64, 8, 6, ROWS, TMA>(p, maps, stream);
+    case 128: return launch<H, 128, 8, 3, ROWS, TMA>(p, maps, stream);
+    default: return launch<H, 256, 4, 3, ROWS, TMA>(p, maps, stream);
   }
+}
+template <typename H>
+cudaError_t by_rows(const Launch& p, int rows, bool tma, const CUtensorMap (&maps)[2], cudaStream_t stream) {
+  if (tma) return rows == 8 ? by_dim<H, 8, true>(p, maps, stream) : by_dim<H, 16, true>(p, maps, stream);
+  return rows == 8 ? by_dim<H, 8, false>(p, maps, stream) : by_dim<H, 16, false>(p, maps, stream);
 }
 
 }  // namespace
@@ -552,6 +649,10 @@ cudaError_t paged_attention(const PagedAttentionArgs& args, cudaStream_t stream)
   const size_t slots = static_cast<size_t>(sm_count()) * warps_of(padded_dim(args.head_dim)) * 2 * rows;
   p.part_ml = reinterpret_cast<float*>(static_cast<char*>(args.workspace) + plan_bytes());
   p.part_o = p.part_ml + slots * 2;
+  p.err = gemm_error_device_ptr();
+  CUtensorMap maps[2] = {};
+  const int dp = padded_dim(args.head_dim);
+  const bool tma = p.page_tiles > 0 && encode_pages(&maps[0], args.k_pages, args, dp) && encode_pages(&maps[1], args.v_pages, args, dp);
   for (int b = 0; b < args.batch; b += kSequences) {
     p.a = args;
     p.a.batch = args.batch - b < kSequences ? args.batch - b : kSequences;
@@ -560,11 +661,7 @@ cudaError_t paged_attention(const PagedAttentionArgs& args, cudaStream_t stream)
     p.a.q.p = static_cast<const char*>(args.q.p) + b * args.q.token * 2;
     p.a.o = static_cast<char*>(args.o) + static_cast<long long>(b) * args.heads * args.head_dim * 2;
     p.a.lse = args.lse ? args.lse + static_cast<long long>(b) * args.heads : nullptr;
-    cudaError_t rc;
-    if (args.type == Half16::bf16)
-      rc = rows == 8 ? by_dim<Bf16, 8>(p, stream) : by_dim<Bf16, 16>(p, stream);
-    else
-      rc = rows == 8 ? by_dim<Fp16, 8>(p, stream) : by_dim<Fp16, 16>(p, stream);
+    const cudaError_t rc = args.type == Half16::bf16 ? by_rows<Bf16>(p, rows, tma, maps, stream) : by_rows<Fp16>(p, rows, tma, maps, stream);
     if (rc != cudaSuccess) return rc;
   }
   return cudaSuccess;
