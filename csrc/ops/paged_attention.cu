@@ -17,24 +17,26 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr int kTile = 16;          // positions that a warp takes at a time
+constexpr int kBlock = 16;         // positions of a block: a tile is one or two, and a page that is a multiple of it comes by TMA
+constexpr int kLeast = 2;            // fewest tiles of a warp
 constexpr int kSequences = 1024;   // most sequences of a launch: their lengths and first tiles are kept in shared memory
 
-// What a sequence's visible positions are in tiles: tile t of `tiles` is the one of positions 16 * (t + (t >= head ? skip : 0)) and on.
+// What a sequence's visible positions are in tiles of KT: tile t of `tiles` is the one of positions KT * (t + (t >= head ? skip : 0)) and on.
 struct Span {
   int length, first;   // positions [first, length) and those below `sinks` are seen
   int tiles, head, skip;
 };
+template <int KT>
 __device__ __forceinline__ Span span_of(int length, int window, int sinks) {
   Span s;
   s.length = length;
   s.first = 0;
-  s.tiles = (length + kTile - 1) / kTile;
+  s.tiles = (length + KT - 1) / KT;
   s.head = s.tiles;
   s.skip = 0;
   if (window > 0 && length > window) {
     s.first = length - window;
-    const int head = (min(sinks, s.first) + kTile - 1) / kTile, tail = s.first / kTile;
+    const int head = (min(sinks, s.first) + KT - 1) / KT, tail = s.first / KT;
     if (tail > head) {
       s.head = head;
       s.skip = tail - head;
@@ -48,12 +50,12 @@ struct Launch {
   PagedAttentionArgs a;
   int group, blocks_of_heads;   // query heads per head of keys and values, and blocks of 16 (or 8) that they make
   int items_per_sequence;       // kv_heads * blocks_of_heads
-  int page_tiles, page_shift;   // page_size / 16 where that is whole (else 0), its logarithm where that is whole (else -1)
+  int page_blocks, page_shift;  // page_size / 16 where that is whole (else 0), its logarithm where that is whole (else -1)
   int whole;                    // an item is one warp's
   float scale_log2;
-  long long* plan;              // tiles per warp, then the first tile of every sequence (and behind the last)
-  float* part_ml;               // [warps][2][rows][2]
-  float* part_o;                // [warps][2][rows][DP]
+  unsigned* plan;               // tiles per block, then the first tile of every sequence (and behind the last)
+  float* part_ml;               // [blocks][2][rows][2]
+  float* part_o;                // [blocks][2][rows][DP]
   int* err;                     // set when a wait inside the kernel ran out
 };
 
@@ -100,41 +102,86 @@ struct Place {
   int item, t;
 };
 
-template <int DP, int WARPS, int STAGES>
+// A stage is a tile of K, the same of V, and the queries where the tile is the first of its piece.  A tile is KT / 16 blocks of 16 positions; a block
+// is DP / 64 runs of 16 rows x 128 bytes, the eight 16-byte pieces of a row in the order of the 128-byte swizzle (DP = 32: one run of 64-byte rows with
+// that swizzle), so that the same piece of eight neighbouring rows lies in eight different groups of banks.  Queries are one block of ROWS rows.
+template <int DP, int KT, int WARPS, int STAGES, int ROWS>
 struct Shape {
-  static constexpr int kTileBytes = kTile * DP * 2;   // of K, and of V
-  static constexpr int kRing = WARPS * STAGES * 2 * kTileBytes;
-  static constexpr int kBars = WARPS * STAGES * 8, kMasks = WARPS * STAGES * 4;
-  static constexpr int kSmem = kRing + kBars + (kSequences + 1) * 8 + kSequences * 4 + kMasks + 1024;   // the ring starts on 1024 bytes
+  static constexpr int kBlockBytes = kBlock * DP * 2;
+  static constexpr int kTileBytes = KT * DP * 2;
+  static constexpr int kQueryBytes = ROWS * DP * 2;
+  static constexpr int kStageBytes = 2 * kTileBytes + kQueryBytes;
+  static constexpr int kRing = WARPS * STAGES * kStageBytes;
+  static constexpr int kPiece = ROWS * DP * 4;   // a piece's sums: the first of each warp has a place of its own, the last the warp's part of the ring
+  static constexpr int kBars = WARPS * STAGES * 8;
+  static constexpr int kSmem = kRing + WARPS * kPiece + kBars + (kSequences + 1) * 4 + kSequences * 4 + WARPS * STAGES * 4 + 8 + 1024;   // the ring starts on 1024 bytes
+  static_assert(STAGES * kStageBytes >= kPiece && kStageBytes % (DP < 64 ? 512 : 1024) == 0);   // where the swizzle repeats
+  static constexpr int kBoxes = DP < 64 ? 1 : DP / 64;   // TMA boxes of a block
 };
 
-// A tile is DP / 64 blocks of 16 rows x 128 bytes, the eight 16-byte pieces of a row in the order of the 128-byte swizzle (64: for DP = 32), so that
-// the same piece of eight neighbouring rows lies in eight different groups of banks.
-template <int DP>
+template <int DP, int R>
 __device__ __forceinline__ uint32_t swizzled(int row, int piece) {
   if (DP == 32) return static_cast<uint32_t>(row * 64 + (piece ^ ((row >> 1) & 3)) * 16);
-  return static_cast<uint32_t>((piece >> 3) * (kTile * 128) + row * 128 + ((piece & 7) ^ (row & 7)) * 16);
+  return static_cast<uint32_t>((piece >> 3) * (R * 128) + row * 128 + ((piece & 7) ^ (row & 7)) * 16);
 }
 
-// Box of 16 positions x 64 (32) columns of one page and head; zero fill outside the tensor, pages among it.
-__device__ __forceinline__ void load_box(uint32_t to, const CUtensorMap* map, uint32_t bar, int col, int at, int head, int page) {
+// Box of 16 positions (or ROWS queries) x 64 (32) columns; zero fill outside the tensor, pages among it.
+__device__ __forceinline__ void load_pages(uint32_t to, const CUtensorMap* map, uint32_t bar, int col, int at, int head, int page) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
       ::"r"(to), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(col), "r"(at), "r"(head), "r"(page)
       : "memory");
 }
+__device__ __forceinline__ void load_queries(uint32_t to, const CUtensorMap* map, uint32_t bar, int col, int head, int b) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(to), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(col), "r"(head), "r"(b)
+      : "memory");
+}
 
-template <typename H, int DP, int WARPS, int STAGES, int ROWS, bool TMA>
-__global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, Launch p) {
-  using S = Shape<DP, WARPS, STAGES>;
+// Sums of a split that are joined one after the other, four columns of one row.
+struct Sums {
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  __device__ __forceinline__ void add(float m2, float l2, const float4& o2) {
+    const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.f : top;
+    const float a = exp2f(m - base), b = exp2f(m2 - base);
+    m = top;
+    l = l * a + l2 * b;
+    o.x = o.x * a + o2.x * b;
+    o.y = o.y * a + o2.y * b;
+    o.z = o.z * a + o2.z * b;
+    o.w = o.w * a + o2.w * b;
+  }
+};
+template <typename H>
+__device__ __forceinline__ void store_result(const PagedAttentionArgs& a, long long row, int col, const Sums& s) {
+  if (col < a.head_dim) {
+    const float inv = 1.f / s.l;
+    typename H::T2* to = reinterpret_cast<typename H::T2*>(static_cast<typename H::T*>(a.o) + row * a.head_dim + col);
+    to[0] = H::down(s.o.x * inv, s.o.y * inv);
+    to[1] = H::down(s.o.z * inv, s.o.w * inv);
+  }
+  if (col == 0 && a.lse) a.lse[row] = ((s.m == -INFINITY ? 0.f : s.m) + log2f(s.l)) * kLn2;
+}
+
+template <typename H, int DP, int KT, int WARPS, int STAGES, int ROWS, bool TMA>
+__global__ void __launch_bounds__(WARPS * 32, 1)
+paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap q_map, Launch p) {
+  using S = Shape<DP, KT, WARPS, STAGES, ROWS>;
   using T = typename H::T;
+  constexpr int kSub = KT / kBlock;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024 - (tc::smem_u32(smem_raw) & 1023)) & 1023);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kRing);
-  long long* first_tile = reinterpret_cast<long long*>(bars + WARPS * STAGES);
+  unsigned char* first_pieces = smem + S::kRing;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(first_pieces + WARPS * S::kPiece);
+  unsigned* first_tile = reinterpret_cast<unsigned*>(bars + WARPS * STAGES);   // (a launch has fewer than 2^32 tiles of all its items)
   int* length_of = reinterpret_cast<int*>(first_tile + kSequences + 1);
   uint32_t* masks = reinterpret_cast<uint32_t*>(length_of + kSequences);
-  __shared__ long long warp_sum[WARPS];
+  __shared__ unsigned warp_sum[WARPS];
+  __shared__ int piece_item[WARPS][2];     // -1: none
+  __shared__ int piece_ends[WARPS][2];     // 1: begins its item, 2: ends it
+  __shared__ float2 piece_ml[WARPS][2][ROWS];
   const PagedAttentionArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t4 = lane & 3;
@@ -143,7 +190,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const __
   if (TMA && lane == 0) {
     for (int i = 0; i < STAGES; ++i) tc::mbar_init(bar + i, 1);
     tc::mbar_init_fence();
+    tc::tma_prefetch_desc(&k_map);
+    tc::tma_prefetch_desc(&v_map);
+    tc::tma_prefetch_desc(&q_map);
   }
+  if (lane < 2) piece_item[warp][lane] = -1;
   __syncwarp();
 
   ::mccl::pdl_wait();
@@ -152,8 +203,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const __
   // ---- lengths, and the tiles in front of every sequence
   {
     constexpr int kPer = (kSequences + WARPS * 32 - 1) / (WARPS * 32);
-    int mine[kPer];
-    long long sum = 0;
+    unsigned mine[kPer], sum = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int b = threadIdx.x * kPer + i;
@@ -161,14 +211,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const __
       if (b < a.batch) {
         const int length = min(max(__ldg(a.lengths + b), 0), room);
         length_of[b] = length;
-        mine[i] = span_of(length, a.window, a.sinks).tiles;
+        mine[i] = span_of<KT>(length, a.window, a.sinks).tiles;
       }
       sum += mine[i];
     }
-    long long before = sum;
+    unsigned before = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long other = __shfl_up_sync(0xffffffffu, before, o);
+      const unsigned other = __shfl_up_sync(0xffffffffu, before, o);
       if (lane >= o) before += other;
     }
     if (lane == 31) warp_sum[warp] = before;
@@ -184,6 +234,160 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const __
     }
     __syncthreads();
   }
+
+  // ---- this warp's run of tiles: `left` of them from tile `begin.t` of an item on
+  struct Place {
+    int item, t;   // an item is a head of keys and values of a sequence (and a block of its query heads), t the tile within it
+  };
+  const unsigned items = a.batch * p.items_per_sequence, warps = gridDim.x * WARPS, me = blockIdx.x * WARPS + warp;
+  const unsigned units = first_tile[a.batch] * p.items_per_sequence;
+  Place begin = {0, 0};
+  int left = 0;
+  if (p.whole) {
+    auto unit = [&](unsigned item) {
+      const unsigned b = item / p.items_per_sequence;
+      return b >= a.batch ? units : first_tile[b] * p.items_per_sequence + (item - b * p.items_per_sequence) * (first_tile[b + 1] - first_tile[b]);
+    };
+    begin.item = static_cast<int>(static_cast<unsigned long long>(items) * me / warps);
+    left = static_cast<int>(unit(static_cast<unsigned>(static_cast<unsigned long long>(items) * (me + 1) / warps)) - unit(begin.item));
+  } else {
+    const unsigned per = max((units - 1) / warps + 1, static_cast<unsigned>(kLeast));
+    if (blockIdx.x == 0) {
+      if (threadIdx.x == 0) p.plan[0] = per * WARPS;
+      for (int b = threadIdx.x; b <= a.batch; b += WARPS * 32) p.plan[1 + b] = first_tile[b];
+    }
+    if (units > 0 && me <= (units - 1) / per) {
+      const unsigned u = per * me, tile = u / p.items_per_sequence;   // the sequence is the one that this tile would be in if each had one item
+      left = static_cast<int>(min(per, units - u));
+      int lo = 0, hi = a.batch - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (first_tile[mid] <= tile) lo = mid; else hi = mid - 1;
+      }
+      const unsigned tiles = first_tile[lo + 1] - first_tile[lo], in = u - first_tile[lo] * p.items_per_sequence, k = in / tiles;
+      begin = {static_cast<int>(lo * p.items_per_sequence + k), static_cast<int>(in - k * tiles)};
+    }
+  }
+  auto tiles_of = [&](int item) {
+    const int b = item / p.items_per_sequence;
+    return item < items ? static_cast<int>(first_tile[b + 1] - first_tile[b]) : 1;
+  };
+  auto settle = [&](Place& at, int& tiles) {   // past items without tiles and past the end of one
+    while (at.item < items && at.t >= tiles) {
+      ++at.item;
+      at.t = 0;
+      tiles = tiles_of(at.item);
+    }
+  };
+
+  // ---- the loading side: a tile of K and V into a stage
+  const uint32_t ring = tc::smem_u32(smem) + warp * (STAGES * S::kStageBytes);
+  uint32_t* mask_ring = masks + warp * STAGES;
+  Place load = begin;
+  int to_load = left, load_item = -1, load_tiles = tiles_of(load.item), load_b = 0, load_kv = 0, load_group = 0, load_slot = -1, load_page = 0;
+  int ahead = 0;   // tiles that are loaded and not yet used
+  Span span = {};
+  const int* table = nullptr;
+  if (left > 0) settle(load, load_tiles);
+  auto issue = [&](int stage) {
+    if (to_load > 0) {
+      const bool fresh = load.item != load_item;
+      if (fresh) {
+        load_item = load.item;
+        load_slot = -1;
+        load_b = load.item / p.items_per_sequence;
+        const int hh = load.item - load_b * p.items_per_sequence;
+        load_kv = hh / p.blocks_of_heads;
+        load_group = (hh - load_kv * p.blocks_of_heads) * ROWS;
+        span = span_of<KT>(length_of[load_b], a.window, a.sinks);
+        table = a.table.p + load_b * a.table.stride;
+      }
+      const int head0 = load_kv * p.group + load_group;
+      const int tile = load.t + (load.t >= span.head ? span.skip : 0);
+      const uint32_t to = ring + stage * S::kStageBytes;
+      if (TMA) {   // every block of 16 positions lies in one page
+        const int j = tile * KT + lane;
+        uint32_t mask = __ballot_sync(0xffffffffu, j < span.length && (j >= span.first || j < a.sinks));
+        if (KT < 32) mask &= 0xffffu;
+        int page[kSub], at[kSub];
+#pragma unroll
+        for (int i = 0; i < kSub; ++i) {
+          const int block = tile * kSub + i;
+          const int slot = p.page_shift >= 0 ? block >> p.page_shift : block / p.page_blocks;
+          if (slot != load_slot && (i == 0 || block * kBlock < span.length)) {
+            load_slot = slot;
+            load_page = __ldg(table + slot);
+            if (load_page >= a.table.pages) load_page = -1;   // outside the tensor: zeros come back
+          }
+          page[i] = slot == load_slot ? load_page : -1;
+          at[i] = (block - slot * p.page_blocks) * kBlock;
+          if (page[i] < 0) mask &= ~(0xffffu << (i * kBlock));
+        }
+        if (tc::elect_one()) {
+          mask_ring[stage] = mask;
+          tc::mbar_expect_tx(bar + stage, 2 * S::kTileBytes + (fresh ? S::kQueryBytes : 0));
+          const uint32_t full = tc::smem_u32(bar + stage);
+          constexpr int kBox = DP / S::kBoxes;
+          if (fresh) {
+#pragma unroll
+            for (int c = 0; c < S::kBoxes; ++c) load_queries(to + 2 * S::kTileBytes + c * (ROWS * kBox * 2), &q_map, full, c * kBox, head0, load_b);
+          }
+#pragma unroll
+          for (int i = 0; i < kSub; ++i)
+#pragma unroll
+            for (int c = 0; c < S::kBoxes; ++c) {
+              const uint32_t spot = to + i * S::kBlockBytes + c * (kBlock * kBox * 2);
+              load_pages(spot, &k_map, full, c * kBox, at[i], load_kv, page[i]);
+              load_pages(spot + S::kTileBytes, &v_map, full, c * kBox, at[i], load_kv, page[i]);
+            }
+        }
+        __syncwarp();
+      } else {
+        const int j = tile * KT + lane % KT;
+        const bool seen = j < span.length && (j >= span.first || j < a.sinks);
+        int page = -1, at = 0;
+        if (seen) {
+          const int slot = j / a.table.page_size;
+          page = __ldg(table + slot);
+          at = j - slot * a.table.page_size;
+        }
+        uint32_t mask = __ballot_sync(0xffffffffu, seen && page >= 0 && page < a.table.pages);
+        if (KT < 32) mask &= 0xffffu;
+        if (lane == 0) mask_ring[stage] = mask;
+        constexpr int kPieces = DP / 8, kRowsAtOnce = 32 / kPieces;
+        const int piece = lane % kPieces, row0 = lane / kPieces;
+        const T* k = static_cast<const T*>(a.k_pages.p) + load_kv * a.k_pages.head + piece * 8;
+        const T* v = static_cast<const T*>(a.v_pages.p) + load_kv * a.v_pages.head + piece * 8;
+        const bool column = piece * 8 < a.head_dim;
+#pragma unroll
+        for (int i = 0; i < KT / kRowsAtOnce; ++i) {
+          const int row = row0 + i * kRowsAtOnce;
+          const int its_page = __shfl_sync(0xffffffffu, page, row), its_at = __shfl_sync(0xffffffffu, at, row);
+          const bool good = column && ((mask >> row) & 1u);
+          const T* from_k = good ? k + its_page * a.k_pages.page + its_at * a.k_pages.token : static_cast<const T*>(a.k_pages.p);
+          const T* from_v = good ? v + its_page * a.v_pages.page + its_at * a.v_pages.token : static_cast<const T*>(a.v_pages.p);
+          const uint32_t spot = to + (row / kBlock) * S::kBlockBytes + swizzled<DP, kBlock>(row % kBlock, piece);
+          copy16(spot, from_k, good);
+          copy16(spot + S::kTileBytes, from_v, good);
+        }
+        if (fresh) {
+          const T* q = static_cast<const T*>(a.q.p) + load_b * a.q.token + piece * 8;
+          for (int row = row0; row < ROWS; row += kRowsAtOnce) {
+            const bool good = column && load_group + row < p.group;
+            copy16(to + 2 * S::kTileBytes + swizzled<DP, ROWS>(row, piece), good ? q + (head0 + row) * a.q.head : static_cast<const T*>(a.q.p), good);
+          }
+        }
+      }
+      ++load.t;
+      if (--to_load > 0) settle(load, load_tiles);
+      ++ahead;
+    }
+    if (!TMA) copy_commit();
+  };
+
+#pragma unroll
+  for (int s = 0; s < STAGES; ++s) issue(s);
+
   // sequences that see nothing
   for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
     if (length_of[b] != 0) continue;
@@ -193,201 +397,79 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const __
       for (int i = threadIdx.x; i < a.heads; i += WARPS * 32) a.lse[static_cast<long long>(b) * a.heads + i] = -INFINITY;
   }
 
-  // ---- this warp's run of tiles
-  const int items = a.batch * p.items_per_sequence, warps = gridDim.x * WARPS, me = blockIdx.x * WARPS + warp;
-  const long long units = first_tile[a.batch] * p.items_per_sequence;
-  Place begin, end;   // [begin, end)
-  if (p.whole) {
-    begin = {static_cast<int>(static_cast<long long>(items) * me / warps), 0};
-    end = {static_cast<int>(static_cast<long long>(items) * (me + 1) / warps), 0};
-  } else {
-    const long long per = max((units + warps - 1) / warps, static_cast<long long>(2));
-    if (blockIdx.x == 0) {
-      if (threadIdx.x == 0) p.plan[0] = per;
-      for (int b = threadIdx.x; b <= a.batch; b += WARPS * 32) p.plan[1 + b] = first_tile[b];
-    }
-    const long long u0 = min(per * me, units), u1 = min(u0 + per, units);
-    if (u0 >= u1) return;
-    auto find = [&](long long u) {
-      const long long tile = u / p.items_per_sequence;   // the sequence is the one that this would be in if it had one item
-      int lo = 0, hi = a.batch - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (first_tile[mid] <= tile) lo = mid; else hi = mid - 1;
-      }
-      const int tiles = static_cast<int>(first_tile[lo + 1] - first_tile[lo]);
-      const long long in = u - first_tile[lo] * p.items_per_sequence;
-      const int k = static_cast<int>(in / tiles);
-      return Place{lo * p.items_per_sequence + k, static_cast<int>(in - static_cast<long long>(k) * tiles)};
-    };
-    begin = find(u0);
-    end = find(u1 - 1);
-    ++end.t;
-  }
-  auto before_end = [&](const Place& at) { return at.item < end.item || (at.item == end.item && at.t < end.t); };
-  auto tiles_of = [&](int item) {
-    const int b = item / p.items_per_sequence;
-    return item < items ? static_cast<int>(first_tile[b + 1] - first_tile[b]) : 1;
-  };
-
-  // ---- the loading side: one tile of K and V into a stage
-  const uint32_t ring = tc::smem_u32(smem) + warp * (STAGES * 2 * S::kTileBytes);
-  uint32_t* mask_ring = masks + warp * STAGES;
-  Place load = begin;
-  int load_item = -1, load_tiles = 0, load_kv = 0, load_slot = -1, load_page = 0;
-  int ahead = 0;   // tiles that are loaded and not yet used
-  Span span = {};
-  const int* table = nullptr;
-  auto settle = [&](Place& at, int& tiles) {   // past items without tiles and past the end of one
-    while (at.item < items && at.t >= tiles) {
-      ++at.item;
-      at.t = 0;
-      tiles = tiles_of(at.item);
-    }
-  };
-  load_tiles = tiles_of(load.item);
-  settle(load, load_tiles);
-  auto issue = [&](int stage) {
-    if (before_end(load)) {
-      if (load.item != load_item) {
-        load_item = load.item;
-        load_slot = -1;
-        const int b = load.item / p.items_per_sequence;
-        load_kv = (load.item - b * p.items_per_sequence) / p.blocks_of_heads;
-        span = span_of(length_of[b], a.window, a.sinks);
-        table = a.table.p + b * a.table.stride;
-      }
-      const int tile = load.t + (load.t >= span.head ? span.skip : 0);
-      const int r16 = lane & 15, j = tile * kTile + r16;
-      const bool seen = j < span.length && (j >= span.first || j < a.sinks);
-      const uint32_t to = ring + stage * (2 * S::kTileBytes);
-      if (TMA) {   // the tile lies in one page
-        const int slot = p.page_shift >= 0 ? tile >> p.page_shift : tile / p.page_tiles;
-        if (slot != load_slot) {
-          load_slot = slot;
-          load_page = __ldg(table + slot);
-          if (load_page >= a.table.pages) load_page = -1;   // outside the tensor: zeros come back
-        }
-        const uint32_t mask = load_page >= 0 ? __ballot_sync(0xffffffffu, seen) & 0xffffu : 0u;
-        if (tc::elect_one()) {
-          mask_ring[stage] = mask;
-          tc::mbar_expect_tx(bar + stage, 2 * S::kTileBytes);
-          const uint32_t full = tc::smem_u32(bar + stage);
-          const int at = (tile - slot * p.page_tiles) * kTile;
-          constexpr int kBox = DP < 64 ? DP : 64;
-#pragma unroll
-          for (int c = 0; c < DP / kBox; ++c) {
-            load_box(to + c * (kTile * kBox * 2), &k_map, full, c * kBox, at, load_kv, load_page);
-            load_box(to + S::kTileBytes + c * (kTile * kBox * 2), &v_map, full, c * kBox, at, load_kv, load_page);
-          }
-        }
-        __syncwarp();
-      } else {
-        int page = -1, at = 0;
-        if (seen) {
-          const int slot = j / a.table.page_size;
-          page = __ldg(table + slot);
-          at = j - slot * a.table.page_size;
-        }
-        const uint32_t mask = __ballot_sync(0xffffffffu, seen && page >= 0 && page < a.table.pages) & 0xffffu;
-        if (lane == 0) mask_ring[stage] = mask;
-        constexpr int kPieces = DP / 8, kRowsAtOnce = 32 / kPieces;
-        const int piece = lane % kPieces, row0 = lane / kPieces;
-        const T* k = static_cast<const T*>(a.k_pages.p) + load_kv * a.k_pages.head + piece * 8;
-        const T* v = static_cast<const T*>(a.v_pages.p) + load_kv * a.v_pages.head + piece * 8;
-        const bool column = piece * 8 < a.head_dim;
-#pragma unroll
-        for (int i = 0; i < kTile / kRowsAtOnce; ++i) {
-          const int row = row0 + i * kRowsAtOnce;
-          const int its_page = __shfl_sync(0xffffffffu, page, row), its_at = __shfl_sync(0xffffffffu, at, row);
-          const bool good = column && ((mask >> row) & 1u);
-          const T* from_k = good ? k + its_page * a.k_pages.page + its_at * a.k_pages.token : static_cast<const T*>(a.k_pages.p);
-          const T* from_v = good ? v + its_page * a.v_pages.page + its_at * a.v_pages.token : static_cast<const T*>(a.v_pages.p);
-          const uint32_t spot = to + swizzled<DP>(row, piece);
-          copy16(spot, from_k, good);
-          copy16(spot + S::kTileBytes, from_v, good);
-        }
-      }
-      ++load.t;
-      settle(load, load_tiles);
-      ++ahead;
-    }
-    if (!TMA) copy_commit();
-  };
-
-#pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s) issue(s);
-
   // ---- the computing side
-  constexpr int kSteps = DP / 16, kCols = DP / 8;
+  constexpr int kSteps = DP / 16, kCols = DP / 8, kHalves = ROWS / 8;   // halves: rows g, and rows g + 8
+  constexpr int kChains = KT == 16 ? 2 : 1;
   Place at = begin;
   int tiles = tiles_of(at.item);
-  settle(at, tiles);
+  if (left > 0) settle(at, tiles);
   bool first_piece = true, ok = true;
   int stage = 0;
   uint32_t parity = 0;
-  // where in a tile a lane's rows of the fragments are: of K (two groups of eight positions, two pieces) and of V (transposed); the pieces of
-  // step s are the ones of step 0 with s & 3 in the address bits above
-  const uint32_t k_lane = swizzled<DP>((lane >> 4) * 8 + (lane & 7), (lane >> 3) & 1), v_lane = swizzled<DP>(((lane >> 3) & 1) * 8 + (lane & 7), lane >> 4);
-  while (before_end(at)) {
-    // a new piece of an item: its queries
-    const int item = at.item, b = item / p.items_per_sequence, hh = item - b * p.items_per_sequence;
-    const int kv = hh / p.blocks_of_heads, in_group = (hh - kv * p.blocks_of_heads) * ROWS;
-    const int heads = min(p.group - in_group, ROWS), head0 = kv * p.group + in_group;
-    const int from = at.t;
+  // where in a block a lane's rows of the fragments are: of K (two groups of eight positions, two pieces), of V (transposed) and of the queries; the
+  // pieces of a later step are the ones of the first with the step in the address bits above
+  const uint32_t k_lane = swizzled<DP, kBlock>((lane >> 4) * 8 + (lane & 7), (lane >> 3) & 1), v_lane = swizzled<DP, kBlock>(((lane >> 3) & 1) * 8 + (lane & 7), lane >> 4);
+  while (left > 0) {
+    const int item = at.item, from = at.t, stop = min(tiles, from + left);
+    left -= stop - from;
     uint32_t q[kSteps][4];
-    {
-      const T* base = static_cast<const T*>(a.q.p) + b * a.q.token + head0 * a.q.head;
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = g + (i & 1) * 8, col = s * 16 + (i >> 1) * 8 + 2 * t4;
-          q[s][i] = 0;
-          if ((ROWS == 16 || (i & 1) == 0) && row < heads && col < a.head_dim) q[s][i] = __ldg(reinterpret_cast<const uint32_t*>(base + row * a.q.head + col));
-        }
-    }
     float o[kCols][4];
 #pragma unroll
     for (int c = 0; c < kCols; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
-    constexpr int kHalves = ROWS / 8;   // rows g, and rows g + 8
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
-    const int stop = item == end.item ? min(tiles, end.t) : tiles;
     for (; at.t < stop; ++at.t) {
       if (TMA) {
         ok = __all_sync(0xffffffffu, tc::mbar_wait(bar + stage, parity));
         if (!ok) break;
       } else {
-        copy_wait<STAGES - 2>();
+        copy_wait<STAGES - 1>();
         __syncwarp();
       }
       --ahead;
-      issue(stage == 0 ? STAGES - 1 : stage - 1);
-      const uint32_t k_tile = ring + stage * (2 * S::kTileBytes), v_tile = k_tile + S::kTileBytes;
+      const uint32_t k_tile = ring + stage * S::kStageBytes, v_tile = k_tile + S::kTileBytes;
       const uint32_t mask = mask_ring[stage];
-      // scores of 16 positions: two products side by side over two halves of the head, four chains
-      float s[2][2][4] = {};
+      if (at.t == from) {   // a new piece: its queries
+        const uint32_t q_tile = v_tile + S::kTileBytes;
 #pragma unroll
-      for (int step = 0; step < kSteps; ++step) {
-        uint32_t r[4];
-        load_matrix(r, k_tile + (step >> 2) * (kTile * 128) + (k_lane ^ ((step & 3) << 5)));
-        mma<H>(s[step & 1][0], q[step], r[0], r[1]);
-        mma<H>(s[step & 1][1], q[step], r[2], r[3]);
+        for (int s = 0; s < kSteps; s += 2 / kHalves) {
+          uint32_t r[4];
+          if (ROWS == 8) {
+            load_matrix(r, q_tile + swizzled<DP, ROWS>(lane & 7, 2 * s + (lane >> 3)));
+            q[s][0] = r[0], q[s][1] = 0, q[s][2] = r[1], q[s][3] = 0;
+            q[s + 1][0] = r[2], q[s + 1][1] = 0, q[s + 1][2] = r[3], q[s + 1][3] = 0;
+          } else {
+            load_matrix(q[s], q_tile + swizzled<DP, ROWS>(((lane >> 3) & 1) * 8 + (lane & 7), 2 * s + (lane >> 4)));
+          }
+        }
       }
-      float z[2][4];   // [row half][position: 2 t4, 2 t4 + 1, 8 + 2 t4, 9 + 2 t4]
+      // scores: per 16 positions two products side by side
+      float s[kChains][2 * kSub][4] = {};
+#pragma unroll
+      for (int step = 0; step < kSteps; ++step)
+#pragma unroll
+        for (int i = 0; i < kSub; ++i) {
+          uint32_t r[4];
+          load_matrix(r, k_tile + i * S::kBlockBytes + (step >> 2) * (kBlock * 128) + (k_lane ^ ((step & 3) << 5)));
+          mma<H>(s[step % kChains][2 * i], q[step], r[0], r[1]);
+          mma<H>(s[step % kChains][2 * i + 1], q[step], r[2], r[3]);
+        }
+      float z[2][4 * kSub];   // [row half][8 i + 2 t4, 8 i + 2 t4 + 1 for each i]
 #pragma unroll
       for (int h = 0; h < kHalves; ++h)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float v = (s[0][i >> 1][h * 2 + (i & 1)] + s[1][i >> 1][h * 2 + (i & 1)]) * p.scale_log2;
-          z[h][i] = (mask >> ((i >> 1) * 8 + 2 * t4 + (i & 1))) & 1u ? v : -INFINITY;
+        for (int i = 0; i < 4 * kSub; ++i) {
+          float v = s[0][i >> 1][h * 2 + (i & 1)];
+          if (kChains == 2) v += s[kChains - 1][i >> 1][h * 2 + (i & 1)];
+          z[h][i] = (mask >> ((i >> 1) * 8 + 2 * t4 + (i & 1))) & 1u ? v * p.scale_log2 : -INFINITY;
         }
       float keep[2];
       bool moved = false;
 #pragma unroll
       for (int h = 0; h < kHalves; ++h) {
-        float top = fmaxf(fmaxf(z[h][0], z[h][1]), fmaxf(z[h][2], z[h][3]));
+        float top = fmaxf(z[h][0], z[h][1]);
+#pragma unroll
+        for (int i = 2; i < 4 * kSub; ++i) top = fmaxf(top, z[h][i]);
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const float now = fmaxf(m[h], top), base = now == -INFINITY ? 0.f : now;
@@ -396,7 +478,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const __
         m[h] = now;
         float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 4 * kSub; ++i) {
           z[h][i] = exp2f(z[h][i] - base);
           sum += z[h][i];
         }
@@ -408,39 +490,45 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const __
 #pragma unroll
           for (int i = 0; i < 2 * kHalves; ++i) o[c][i] *= keep[i >> 1];
       }
-      // weights as the sum of two 16-bit values: rounded once to 16 bits they would cost the result as much as its own rounding does,
-      // and the tensor cores have nothing else to do
-      uint32_t hi[4] = {}, lo[4] = {};
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h)
+      for (int i = 0; i < kSub; ++i) {
+        // weights as the sum of two 16-bit values: rounded once to 16 bits they would cost the result as much as its own rounding does,
+        // and the tensor cores have nothing else to do
+        uint32_t hi[4] = {}, lo[4] = {};
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          hi[i * 2 + h] = pair<H>(z[h][2 * i], z[h][2 * i + 1]);
-          const float2 back = unpair<H>(hi[i * 2 + h]);
-          lo[i * 2 + h] = pair<H>(z[h][2 * i] - back.x, z[h][2 * i + 1] - back.y);
+        for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float w0 = z[h][4 * i + 2 * e], w1 = z[h][4 * i + 2 * e + 1];
+            hi[e * 2 + h] = pair<H>(w0, w1);
+            const float2 back = unpair<H>(hi[e * 2 + h]);
+            lo[e * 2 + h] = pair<H>(w0 - back.x, w1 - back.y);
+          }
+        // values of positions that are not seen may be anything: they are cleared, for zero times anything need not be zero
+        uint32_t clear[2] = {0xffffffffu, 0xffffffffu};
+        if (TMA && ((mask >> (16 * i)) & 0xffffu) != 0xffffu) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            clear[e] = ((mask >> (16 * i + e * 8 + 2 * t4)) & 1u ? 0x0000ffffu : 0u) | ((mask >> (16 * i + e * 8 + 2 * t4 + 1)) & 1u ? 0xffff0000u : 0u);
         }
-      // values of positions that are not seen may be anything: they are cleared, for zero times anything need not be zero
-      uint32_t clear[2] = {0xffffffffu, 0xffffffffu};
-      if (TMA && mask != 0xffffu) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          clear[i] = ((mask >> (i * 8 + 2 * t4)) & 1u ? 0x0000ffffu : 0u) | ((mask >> (i * 8 + 2 * t4 + 1)) & 1u ? 0xffff0000u : 0u);
-      }
-#pragma unroll
-      for (int c = 0; c < kCols; c += 2) {
-        uint32_t r[4];
-        load_matrix_t(r, v_tile + (c >> 3) * (kTile * 128) + (v_lane ^ (((c >> 1) & 3) << 5)));
-        if (TMA) {
-          r[0] &= clear[0];
-          r[1] &= clear[1];
-          r[2] &= clear[0];
-          r[3] &= clear[1];
+        for (int c = 0; c < kCols; c += 2) {
+          uint32_t r[4];
+          load_matrix_t(r, v_tile + i * S::kBlockBytes + (c >> 3) * (kBlock * 128) + (v_lane ^ (((c >> 1) & 3) << 5)));
+          if (TMA) {
+            r[0] &= clear[0];
+            r[1] &= clear[1];
+            r[2] &= clear[0];
+            r[3] &= clear[1];
+          }
+          mma<H>(o[c], hi, r[0], r[1]);
+          mma<H>(o[c + 1], hi, r[2], r[3]);
+          mma<H>(o[c], lo, r[0], r[1]);
+          mma<H>(o[c + 1], lo, r[2], r[3]);
         }
-        mma<H>(o[c], hi, r[0], r[1]);
-        mma<H>(o[c + 1], hi, r[2], r[3]);
-        mma<H>(o[c], lo, r[0], r[1]);
-        mma<H>(o[c + 1], lo, r[2], r[3]);
       }
+      __syncwarp();   // every lane has read its fragments
+      issue(stage);
       if (++stage == STAGES) {
         stage = 0;
         parity ^= 1;
@@ -448,9 +536,13 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const __
     }
     if (TMA && !ok) break;
 
-    // ---- the end of this piece: the result where it is the whole item, else a part for the join
+    // ---- the end of this piece: the result where it is the whole item, else its sums for the block
     const bool complete = from == 0 && at.t == tiles;
-    const size_t slot = (static_cast<size_t>(me) * 2 + (first_piece ? 0 : 1)) * ROWS;
+    const int b = item / p.items_per_sequence, hh = item - b * p.items_per_sequence;
+    const int kv = hh / p.blocks_of_heads, in_group = (hh - kv * p.blocks_of_heads) * ROWS;
+    const int heads = min(p.group - in_group, ROWS), head0 = kv * p.group + in_group;
+    const int which = first_piece ? 0 : 1;
+    unsigned char* sums = first_piece ? first_pieces + warp * S::kPiece : smem + warp * (STAGES * S::kStageBytes);
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) {
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
@@ -459,22 +551,27 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const __
       if (row >= heads) continue;
       if (complete) {
         const float inv = 1.f / l[h];
-        T* to = static_cast<T*>(a.o) + (static_cast<long long>(b) * a.heads + head0 + row) * a.head_dim;
+        const long long out = static_cast<long long>(b) * a.heads + head0 + row;
+        T* to = static_cast<T*>(a.o) + out * a.head_dim;
 #pragma unroll
         for (int c = 0; c < kCols; ++c) {
           const int col = c * 8 + 2 * t4;
           if (col < a.head_dim) *reinterpret_cast<typename H::T2*>(to + col) = H::down(o[c][2 * h] * inv, o[c][2 * h + 1] * inv);
         }
-        if (a.lse && t4 == 0) a.lse[static_cast<long long>(b) * a.heads + head0 + row] = ((m[h] == -INFINITY ? 0.f : m[h]) + log2f(l[h])) * kLn2;
+        if (a.lse && t4 == 0) a.lse[out] = ((m[h] == -INFINITY ? 0.f : m[h]) + log2f(l[h])) * kLn2;
       } else {
-        float* to = p.part_o + (slot + row) * DP;
+        float* to = reinterpret_cast<float*>(sums) + row * DP;
 #pragma unroll
         for (int c = 0; c < kCols; ++c) *reinterpret_cast<float2*>(to + c * 8 + 2 * t4) = make_float2(o[c][2 * h], o[c][2 * h + 1]);
-        if (t4 == 0) *reinterpret_cast<float2*>(p.part_ml + (slot + row) * 2) = make_float2(m[h], l[h]);
+        if (t4 == 0) piece_ml[warp][which][row] = make_float2(m[h], l[h]);
       }
     }
+    if (!complete && lane == 0) {
+      piece_item[warp][which] = item;
+      piece_ends[warp][which] = (from == 0 ? 1 : 0) | (at.t == tiles ? 2 : 0);
+    }
     first_piece = false;
-    settle(at, tiles);
+    if (left > 0) settle(at, tiles);
   }
   if (!TMA) copy_wait<0>();
   if (TMA && !ok) {
@@ -487,82 +584,87 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attention_kernel(const __
       }
     }
   }
+  if (p.whole) return;
+
+  // ---- pieces of one item are joined in the order of their positions, a thread per row and four columns.  What lies within the block is a result;
+  // what came from the block before, or goes on in the next, is left for the join.
+  __syncthreads();
+  const int their_item = lane < 2 * WARPS ? piece_item[lane >> 1][lane & 1] : -1, their_ends = lane < 2 * WARPS ? piece_ends[lane >> 1][lane & 1] : 0;
+  const unsigned pieces = __ballot_sync(0xffffffffu, their_item >= 0);
+  for (unsigned rest = pieces; rest != 0;) {
+    // a run of pieces of one item
+    const int item = __shfl_sync(0xffffffffu, their_item, __ffs(rest) - 1);
+    const unsigned run = __ballot_sync(0xffffffffu, their_item == item) & pieces;
+    rest &= ~run;
+    const int begun = __shfl_sync(0xffffffffu, their_ends, __ffs(run) - 1) & 1, ended = __shfl_sync(0xffffffffu, their_ends, 31 - __clz(run)) & 2;
+    const int b = item / p.items_per_sequence, hh = item - b * p.items_per_sequence;
+    const int kv = hh / p.blocks_of_heads, in_group = (hh - kv * p.blocks_of_heads) * ROWS;
+    const int heads = min(p.group - in_group, ROWS);
+    for (int u = threadIdx.x; u < heads * DP / 4; u += WARPS * 32) {
+      const int row = u / (DP / 4), col = u % (DP / 4) * 4;
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 2 * WARPS; ++i)
+        if ((run >> i) & 1u) top = fmaxf(top, piece_ml[i >> 1][i & 1][row].x);
+      Sums sum;
+      sum.m = top;
+      const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int i = 0; i < 2 * WARPS; ++i) {
+        if (!((run >> i) & 1u)) continue;
+        const float2 ml = piece_ml[i >> 1][i & 1][row];
+        const float weight = exp2f(ml.x - base);
+        const float4 o = *reinterpret_cast<const float4*>((i & 1 ? smem + (i >> 1) * (STAGES * S::kStageBytes) : first_pieces + (i >> 1) * S::kPiece) + (row * DP + col) * 4);
+        sum.l += weight * ml.y;
+        sum.o.x += weight * o.x;
+        sum.o.y += weight * o.y;
+        sum.o.z += weight * o.z;
+        sum.o.w += weight * o.w;
+      }
+      if (begun && ended) {
+        store_result<H>(a, static_cast<long long>(b) * a.heads + kv * p.group + in_group + row, col, sum);
+      } else {
+        const size_t slot = (static_cast<size_t>(blockIdx.x) * 2 + begun) * ROWS + row;
+        *reinterpret_cast<float4*>(p.part_o + slot * DP + col) = sum.o;
+        if (col == 0) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(sum.m, sum.l);
+      }
+    }
+  }
 }
 
-// One block per sequence and query head whose tiles were shared out: the parts of its warps in order.
+// One block per sequence and query head: where its tiles were more than one block's, their parts in order.
 template <typename H, int DP, int ROWS>
-__global__ void __launch_bounds__(256) paged_attention_join_kernel(Launch p) {
-  using T = typename H::T;
-  constexpr int kLanes = DP / 4, kGroups = 256 / kLanes;   // four columns per thread, the parts shared out over the groups
-  __shared__ float weight[256];
-  __shared__ float4 sums[256];
-  __shared__ float red[8];
+__global__ void __launch_bounds__(128) paged_attention_join_kernel(Launch p) {
+  constexpr int kLanes = DP / 4, kGroups = 128 / kLanes;   // four columns per thread, the parts shared out over the groups
+  __shared__ __align__(16) unsigned char raw[128 * sizeof(Sums)];
+  Sums* sums = reinterpret_cast<Sums*>(raw);
   const PagedAttentionArgs& a = p.a;
   const int b = blockIdx.y, h = blockIdx.x, kv = h / p.group, in_group = h - kv * p.group;
   const int k = kv * p.blocks_of_heads + in_group / ROWS, row = in_group % ROWS;
+  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   ::mccl::pdl_wait();
   ::mccl::pdl_trigger();
-  const long long per = p.plan[0], first = p.plan[1 + b], tiles = p.plan[2 + b] - first;
-  if (tiles <= 0) return;
-  const long long s = first * p.items_per_sequence + k * tiles, e = s + tiles;
-  const int w0 = static_cast<int>(s / per), w1 = static_cast<int>((e - 1) / per), parts = w1 - w0 + 1;
-  if (parts == 1) return;
-  auto slot = [&](int i) { return (static_cast<size_t>(w0 + i) * 2 + (i == 0 && per * w0 != s ? 1 : 0)) * ROWS + row; };
-  float top = -INFINITY;
-  for (int i = threadIdx.x; i < parts; i += 256) top = fmaxf(top, p.part_ml[slot(i) * 2]);
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
-  __syncthreads();
-  top = red[0];
-  for (int i = 1; i < 8; ++i) top = fmaxf(top, red[i]);
-  const float base = top == -INFINITY ? 0.f : top;
-  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
-  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l = 0.f;
-  for (int i0 = 0; i0 < parts; i0 += 256) {
-    const int n = min(parts - i0, 256);
-    float mine = 0.f;
-    if (threadIdx.x < n) {
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot(i0 + threadIdx.x) * 2);
-      const float w = exp2f(ml.x - base);
-      weight[threadIdx.x] = w;
-      mine = w * ml.y;
-    }
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    __syncthreads();   // red is free
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = mine;
-    __syncthreads();
-    for (int i = 0; i < 8; ++i) l += red[i];
+  const unsigned per = p.plan[0], first = p.plan[1 + b], tiles = p.plan[2 + b] - first;
+  if (tiles == 0) return;
+  const unsigned s = first * p.items_per_sequence + k * tiles;
+  const int c0 = static_cast<int>(s / per), c1 = static_cast<int>((s + tiles - 1) / per);
+  if (c0 == c1) return;
+  Sums sum;
 #pragma unroll 4
-    for (int i = group; i < n; i += kGroups) {
-      const float w = weight[i];
-      const float4 v = *reinterpret_cast<const float4*>(p.part_o + slot(i0 + i) * DP + lane * 4);
-      sum.x += w * v.x;
-      sum.y += w * v.y;
-      sum.z += w * v.z;
-      sum.w += w * v.w;
-    }
-    __syncthreads();
+  for (int c = c0 + group; c <= c1; c += kGroups) {
+    const size_t slot = (static_cast<size_t>(c) * 2 + (c == c0)) * ROWS + row;
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
+    sum.add(ml.x, ml.y, *reinterpret_cast<const float4*>(p.part_o + slot * DP + lane * 4));
   }
   sums[threadIdx.x] = sum;
   __syncthreads();
-  const long long out = static_cast<long long>(b) * a.heads + h;
-  if (group == 0 && lane * 4 < a.head_dim) {
+  if (group == 0) {
     for (int i = 1; i < kGroups; ++i) {
-      const float4 v = sums[i * kLanes + lane];
-      sum.x += v.x;
-      sum.y += v.y;
-      sum.z += v.z;
-      sum.w += v.w;
+      const Sums& other = sums[i * kLanes + lane];
+      sum.add(other.m, other.l, other.o);
     }
-    const float inv = 1.f / l;
-    typename H::T2* to = reinterpret_cast<typename H::T2*>(static_cast<T*>(a.o) + out * a.head_dim + lane * 4);
-    to[0] = H::down(sum.x * inv, sum.y * inv);
-    to[1] = H::down(sum.z * inv, sum.w * inv);
+    store_result<H>(a, static_cast<long long>(b) * a.heads + h, lane * 4, sum);
   }
-  if (threadIdx.x == 0 && a.lse) a.lse[out] = (base + log2f(l)) * kLn2;
 }
 
 int sm_count() {
@@ -575,93 +677,111 @@ int sm_count() {
 }
 
 int padded_dim(int d) { return d <= 32 ? 32 : (d <= 64 ? 64 : (d <= 128 ? 128 : 256)); }
-int warps_of(int dp) { return dp == 256 ? 4 : 8; }
 int rows_of(const PagedAttentionArgs& a) { return a.heads / a.kv_heads <= 8 ? 8 : 16; }
+size_t plan_bytes() { return (kSequences + 4) * sizeof(unsigned); }
+// Whether every item is one warp's: so short that a split would not pay for the join, a launch of its own (longest sequence that the table has room for).
+bool whole(const PagedAttentionArgs& a) { return static_cast<long long>(a.table.width) * a.table.page_size <= 64; }
 
-size_t plan_bytes() { return (kSequences + 2) * sizeof(long long); }
-
-// Keys or values as boxes of 16 positions of one page and head.  False where the strides do not fit a tensor map.
-bool encode_pages(CUtensorMap* map, const PagedTensor& t, const PagedAttentionArgs& a, int dp) {
+bool encode(CUtensorMap* map, Half16 type, int dims, const void* base, const cuuint64_t* size, const cuuint64_t* strides, const cuuint32_t* box) {
   const CuDriver& cu = CuDriver::get();
   if (!cu.loaded || !cu.TensorMapEncodeTiled) return false;
-  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.head_dim), static_cast<cuuint64_t>(a.table.page_size), static_cast<cuuint64_t>(a.kv_heads),
-                              static_cast<cuuint64_t>(a.table.pages)};
-  // the stride of a dimension of one is never used and may be anything
-  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(t.token * 2), static_cast<cuuint64_t>((a.kv_heads > 1 ? t.head : 8) * 2),
-                                 static_cast<cuuint64_t>((a.table.pages > 1 ? t.page : 8) * 2)};
-  const cuuint32_t box[4] = {static_cast<cuuint32_t>(dp < 64 ? dp : 64), kTile, 1, 1}, step[4] = {1, 1, 1, 1};
-  return cu.TensorMapEncodeTiled(map, a.type == Half16::bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, t.p, dims, strides, box, step,
-                                 CU_TENSOR_MAP_INTERLEAVE_NONE, dp < 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+  const cuuint32_t step[4] = {1, 1, 1, 1};
+  return cu.TensorMapEncodeTiled(map, type == Half16::bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, dims, const_cast<void*>(base), size, strides,
+                                 box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, box[0] < 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+// Keys or values as boxes of 16 positions of one page and head, queries as boxes of `rows` heads.  False where the strides do not fit a tensor
+// map.  (The stride of a dimension of one is never used and may be anything.)
+bool encode_pages(CUtensorMap* map, const PagedTensor& t, const PagedAttentionArgs& a, int dp) {
+  const cuuint64_t size[4] = {static_cast<cuuint64_t>(a.head_dim), static_cast<cuuint64_t>(a.table.page_size), static_cast<cuuint64_t>(a.kv_heads),
+                              static_cast<cuuint64_t>(a.table.pages)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(t.token * 2), static_cast<cuuint64_t>((a.kv_heads > 1 ? t.head : 8) * 2),
+                                 static_cast<cuuint64_t>((a.table.pages > 1 ? t.page : 8) * 2)};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(dp < 64 ? dp : 64), kBlock, 1, 1};
+  return encode(map, a.type, 4, t.p, size, strides, box);
+}
+bool encode_queries(CUtensorMap* map, const PagedAttentionArgs& a, int dp, int rows) {
+  const cuuint64_t size[3] = {static_cast<cuuint64_t>(a.head_dim), static_cast<cuuint64_t>(a.heads), static_cast<cuuint64_t>(a.batch)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>((a.heads > 1 ? a.q.head : 8) * 2), static_cast<cuuint64_t>((a.batch > 1 ? a.q.token : 8) * 2)};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(dp < 64 ? dp : 64), static_cast<cuuint32_t>(rows), 1};
+  return encode(map, a.type, 3, a.q.p, size, strides, box);
+}
 
-template <typename H, int DP, int WARPS, int STAGES, int ROWS, bool TMA>
-cudaError_t launch(const Launch& p, const CUtensorMap (&maps)[2], cudaStream_t stream) {
-  constexpr int smem = Shape<DP, WARPS, STAGES>::kSmem;
-  static const cudaError_t rc = cudaFuncSetAttribute(paged_attention_kernel<H, DP, WARPS, STAGES, ROWS, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+template <typename H, int DP, int KT, int WARPS, int STAGES, int ROWS, bool TMA>
+cudaError_t launch(const Launch& p, const CUtensorMap (&maps)[3], cudaStream_t stream) {
+  constexpr int smem = Shape<DP, KT, WARPS, STAGES, ROWS>::kSmem;
+  static const cudaError_t rc = cudaFuncSetAttribute(paged_attention_kernel<H, DP, KT, WARPS, STAGES, ROWS, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (rc != cudaSuccess) return rc;
-  MCCL_LAUNCH_PDL((paged_attention_kernel<H, DP, WARPS, STAGES, ROWS, TMA>), sm_count(), WARPS * 32, smem, stream, maps[0], maps[1], p);
+  MCCL_LAUNCH_PDL((paged_attention_kernel<H, DP, KT, WARPS, STAGES, ROWS, TMA>), sm_count(), WARPS * 32, smem, stream, maps[0], maps[1], maps[2], p);
   count_launch();
   if (!p.whole) {
-    MCCL_LAUNCH_PDL((paged_attention_join_kernel<H, DP, ROWS>), dim3(p.a.heads, p.a.batch), 256, 0, stream, p);
+    MCCL_LAUNCH_PDL((paged_attention_join_kernel<H, DP, ROWS>), dim3(p.a.heads, p.a.batch), 128, 0, stream, p);
     count_launch();
   }
   return ::mccl::launch_status();
 }
 
-template <typename H, int ROWS, bool TMA>
-cudaError_t by_dim(const Launch& p, const CUtensorMap (&maps)[2], cudaStream_t stream) {
-  switch (padded_dim(p.a.head_dim)) {
-    case 32: return launch<H, 32, 8, 8, ROWS, TMA>(p, maps, stream);
-    case 64: return launch<H, 64, 8, 6, ROWS, TMA>(p, maps, stream);
-    case 128: return launch<H, 128, 8, 3, ROWS, TMA>(p, maps, stream);
-    default: return launch<H, 256, 4, 3, ROWS, TMA>(p, maps, stream);
+// Sizes of tile and ring: as many warps as hide the latency of a tile's chain (scores, maximum, weights, products), two stages of 8 KB each.  More bytes in
+// flight are slower (2 x 131009 positions: three stages 181 us, two 172), fewer warps too (4 x 4 stages 191, 6 x 2 182).
+template <typename H, bool TMA>
+cudaError_t by_size(const Launch& p, int rows, const CUtensorMap (&maps)[3], cudaStream_t stream) {
+  const int dp = padded_dim(p.a.head_dim);
+  if (rows == 8) {
+    if (dp == 32) return launch<H, 32, 32, 8, 4, 8, TMA>(p, maps, stream);
+    if (dp == 64) return launch<H, 64, 32, 8, 2, 8, TMA>(p, maps, stream);
+    if (dp == 128) return launch<H, 128, 16, 8, 2, 8, TMA>(p, maps, stream);
+    return launch<H, 256, 16, 4, 2, 8, TMA>(p, maps, stream);
   }
-}
-template <typename H>
-cudaError_t by_rows(const Launch& p, int rows, bool tma, const CUtensorMap (&maps)[2], cudaStream_t stream) {
-  if (tma) return rows == 8 ? by_dim<H, 8, true>(p, maps, stream) : by_dim<H, 16, true>(p, maps, stream);
-  return rows == 8 ? by_dim<H, 8, false>(p, maps, stream) : by_dim<H, 16, false>(p, maps, stream);
+  if (dp == 32) return launch<H, 32, 32, 8, 4, 16, TMA>(p, maps, stream);
+  if (dp == 64) return launch<H, 64, 32, 8, 2, 16, TMA>(p, maps, stream);
+  if (dp == 128) return launch<H, 128, 16, 6, 2, 16, TMA>(p, maps, stream);
+  return launch<H, 256, 16, 3, 2, 16, TMA>(p, maps, stream);
 }
 
 }  // namespace
 
 size_t paged_attention_workspace(const PagedAttentionArgs& a) {
-  const int dp = padded_dim(a.head_dim), rows = rows_of(a);
-  const size_t slots = static_cast<size_t>(sm_count()) * warps_of(dp) * 2 * rows;
-  return plan_bytes() + slots * (2 + dp) * sizeof(float);
+  if (whole(a)) return 0;
+  return plan_bytes() + static_cast<size_t>(sm_count()) * 2 * rows_of(a) * (2 + padded_dim(a.head_dim)) * sizeof(float);
 }
 
 cudaError_t paged_attention(const PagedAttentionArgs& args, cudaStream_t stream) {
   if (args.batch <= 0 || args.heads <= 0) return cudaSuccess;
   Launch p;
   p.group = args.heads / args.kv_heads;
-  const int rows = rows_of(args);
+  const int rows = rows_of(args), dp = padded_dim(args.head_dim);
   p.blocks_of_heads = (p.group + rows - 1) / rows;
   p.items_per_sequence = args.kv_heads * p.blocks_of_heads;
-  p.page_tiles = args.table.page_size % kTile == 0 ? args.table.page_size / kTile : 0;
+  p.page_blocks = args.table.page_size % kBlock == 0 ? args.table.page_size / kBlock : 0;
   p.page_shift = -1;
   for (int s = 0; s < 27; ++s)
-    if (p.page_tiles == 1 << s) p.page_shift = s;
+    if (p.page_blocks == 1 << s) p.page_shift = s;
   p.scale_log2 = args.scale * kLog2e;
-  p.whole = static_cast<long long>(args.table.width) * args.table.page_size <= 64 ? 1 : 0;
-  p.plan = static_cast<long long*>(args.workspace);
-  const size_t slots = static_cast<size_t>(sm_count()) * warps_of(padded_dim(args.head_dim)) * 2 * rows;
+  p.whole = whole(args) ? 1 : 0;
+  p.plan = static_cast<unsigned*>(args.workspace);
   p.part_ml = reinterpret_cast<float*>(static_cast<char*>(args.workspace) + plan_bytes());
-  p.part_o = p.part_ml + slots * 2;
+  p.part_o = p.part_ml + static_cast<size_t>(sm_count()) * 2 * rows * 2;
   p.err = gemm_error_device_ptr();
-  CUtensorMap maps[2] = {};
-  const int dp = padded_dim(args.head_dim);
-  const bool tma = p.page_tiles > 0 && encode_pages(&maps[0], args.k_pages, args, dp) && encode_pages(&maps[1], args.v_pages, args, dp);
-  for (int b = 0; b < args.batch; b += kSequences) {
+  CUtensorMap maps[3] = {};
+  const bool paged = p.page_blocks > 0 && encode_pages(&maps[0], args.k_pages, args, dp) && encode_pages(&maps[1], args.v_pages, args, dp);
+  // tiles of a launch are counted in 32 bits: as many sequences as cannot have more (a product with the blocks' number is among the sums)
+  const long long most = (static_cast<long long>(args.table.width) * args.table.page_size / kBlock + 1) * p.items_per_sequence, room = 0xf0000000ll / most;
+  if (room < 1) return cudaErrorInvalidValue;
+  const int step = room < kSequences ? static_cast<int>(room) : kSequences;
+  for (int b = 0; b < args.batch; b += step) {
     p.a = args;
-    p.a.batch = args.batch - b < kSequences ? args.batch - b : kSequences;
+    p.a.batch = args.batch - b < step ? args.batch - b : step;
     p.a.lengths = args.lengths + b;
     p.a.table.p = args.table.p + b * args.table.stride;
     p.a.q.p = static_cast<const char*>(args.q.p) + b * args.q.token * 2;
     p.a.o = static_cast<char*>(args.o) + static_cast<long long>(b) * args.heads * args.head_dim * 2;
     p.a.lse = args.lse ? args.lse + static_cast<long long>(b) * args.heads : nullptr;
-    const cudaError_t rc = args.type == Half16::bf16 ? by_rows<Bf16>(p, rows, tma, maps, stream) : by_rows<Fp16>(p, rows, tma, maps, stream);
+    const bool tma = paged && encode_queries(&maps[2], p.a, dp, rows);
+    cudaError_t rc;
+    if (args.type == Half16::bf16)
+      rc = tma ? by_size<Bf16, true>(p, rows, maps, stream) : by_size<Bf16, false>(p, rows, maps, stream);
+    else
+      rc = tma ? by_size<Fp16, true>(p, rows, maps, stream) : by_size<Fp16, false>(p, rows, maps, stream);
     if (rc != cudaSuccess) return rc;
   }
   return cudaSuccess;
