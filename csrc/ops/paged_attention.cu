@@ -46,11 +46,21 @@ __device__ __forceinline__ Span span_of(int length, int window, int sinks) {
   return s;
 }
 
+// n / d for n < 2^31 as one multiplication: with 2^s < d <= 2^(s + 1) and m = ceil(2^(32 + s) / d), m d exceeds 2^(32 + s) by less than 2^(s + 1).
+struct Divisor {
+  unsigned d, m, s;
+  __host__ explicit Divisor(unsigned by = 1) : d(by), m(0), s(0) {
+    while ((2ull << s) < by) ++s;
+    if (by > 1) m = static_cast<unsigned>(((1ull << (32 + s)) + by - 1) / by);
+  }
+  __device__ __forceinline__ unsigned of(unsigned n) const { return m == 0 ? n : __umulhi(n, m) >> s; }
+};
+
 struct Launch {
   PagedAttentionArgs a;
-  int group, blocks_of_heads;   // query heads per head of keys and values, and blocks of 16 (or 8) that they make
-  int items_per_sequence;       // kv_heads * blocks_of_heads
-  int page_blocks, page_shift;  // page_size / 16 where that is whole (else 0), its logarithm where that is whole (else -1)
+  int group;                    // query heads per head of keys and values
+  Divisor head_blocks, items;   // blocks of 16 (or 8) that they make; items of a sequence: kv_heads * head_blocks
+  Divisor page_blocks, warps;   // page_size / 16 (1 where that is not whole); warps of the grid
   int whole;                    // an item is one warp's
   float scale_log2;
   unsigned* plan;               // tiles per block, then the first tile of every sequence (and behind the last)
@@ -239,41 +249,41 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   struct Place {
     int item, t;   // an item is a head of keys and values of a sequence (and a block of its query heads), t the tile within it
   };
-  const unsigned items = a.batch * p.items_per_sequence, warps = gridDim.x * WARPS, me = blockIdx.x * WARPS + warp;
-  const unsigned units = first_tile[a.batch] * p.items_per_sequence;
+  const unsigned per_sequence = p.items.d, items = a.batch * per_sequence, me = blockIdx.x * WARPS + warp;
+  const unsigned units = first_tile[a.batch] * per_sequence;
   Place begin = {0, 0};
   int left = 0;
   if (p.whole) {
     auto unit = [&](unsigned item) {
-      const unsigned b = item / p.items_per_sequence;
-      return b >= a.batch ? units : first_tile[b] * p.items_per_sequence + (item - b * p.items_per_sequence) * (first_tile[b + 1] - first_tile[b]);
+      const unsigned b = p.items.of(item);
+      return b >= a.batch ? units : first_tile[b] * per_sequence + (item - b * per_sequence) * (first_tile[b + 1] - first_tile[b]);
     };
-    begin.item = static_cast<int>(static_cast<unsigned long long>(items) * me / warps);
-    left = static_cast<int>(unit(static_cast<unsigned>(static_cast<unsigned long long>(items) * (me + 1) / warps)) - unit(begin.item));
+    const unsigned each = p.warps.of(items), more = items - each * p.warps.d;   // the first `more` warps have one more
+    begin.item = me * each + min(me, more);
+    left = static_cast<int>(unit(begin.item + each + (me < more ? 1 : 0)) - unit(begin.item));
   } else {
-    const unsigned per = max((units - 1) / warps + 1, static_cast<unsigned>(kLeast));
+    const unsigned per = max(p.warps.of(units + p.warps.d - 1), static_cast<unsigned>(kLeast));
     if (blockIdx.x == 0) {
       if (threadIdx.x == 0) p.plan[0] = per * WARPS;
       for (int b = threadIdx.x; b <= a.batch; b += WARPS * 32) p.plan[1 + b] = first_tile[b];
     }
-    if (units > 0 && me <= (units - 1) / per) {
-      const unsigned u = per * me, tile = u / p.items_per_sequence;   // the sequence is the one that this tile would be in if each had one item
+    const unsigned u = per * me;
+    if (u < units) {
+      const unsigned tile = p.items.of(u);   // the sequence is the last that begins at or before this tile
       left = static_cast<int>(min(per, units - u));
-      int lo = 0, hi = a.batch - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (first_tile[mid] <= tile) lo = mid; else hi = mid - 1;
-      }
-      const unsigned tiles = first_tile[lo + 1] - first_tile[lo], in = u - first_tile[lo] * p.items_per_sequence, k = in / tiles;
-      begin = {static_cast<int>(lo * p.items_per_sequence + k), static_cast<int>(in - k * tiles)};
+      static_assert(kSequences <= 32 * 32);
+      const int group = __popc(__ballot_sync(0xffffffffu, lane * 32 < a.batch && first_tile[lane * 32] <= tile)) - 1;
+      const int b = group * 32 + __popc(__ballot_sync(0xffffffffu, group * 32 + lane < a.batch && first_tile[group * 32 + lane] <= tile)) - 1;
+      const unsigned tiles = first_tile[b + 1] - first_tile[b], in = u - first_tile[b] * per_sequence, k = in / tiles;
+      begin = {static_cast<int>(b * per_sequence + k), static_cast<int>(in - k * tiles)};
     }
   }
   auto tiles_of = [&](int item) {
-    const int b = item / p.items_per_sequence;
-    return item < items ? static_cast<int>(first_tile[b + 1] - first_tile[b]) : 1;
+    const int b = p.items.of(item);
+    return static_cast<unsigned>(item) < items ? static_cast<int>(first_tile[b + 1] - first_tile[b]) : 1;
   };
   auto settle = [&](Place& at, int& tiles) {   // past items without tiles and past the end of one
-    while (at.item < items && at.t >= tiles) {
+    while (static_cast<unsigned>(at.item) < items && at.t >= tiles) {
       ++at.item;
       at.t = 0;
       tiles = tiles_of(at.item);
@@ -295,10 +305,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       if (fresh) {
         load_item = load.item;
         load_slot = -1;
-        load_b = load.item / p.items_per_sequence;
-        const int hh = load.item - load_b * p.items_per_sequence;
-        load_kv = hh / p.blocks_of_heads;
-        load_group = (hh - load_kv * p.blocks_of_heads) * ROWS;
+        load_b = p.items.of(load.item);
+        const int hh = load.item - load_b * per_sequence;
+        load_kv = p.head_blocks.of(hh);
+        load_group = (hh - load_kv * p.head_blocks.d) * ROWS;
         span = span_of<KT>(length_of[load_b], a.window, a.sinks);
         table = a.table.p + load_b * a.table.stride;
       }
@@ -313,14 +323,14 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
 #pragma unroll
         for (int i = 0; i < kSub; ++i) {
           const int block = tile * kSub + i;
-          const int slot = p.page_shift >= 0 ? block >> p.page_shift : block / p.page_blocks;
+          const int slot = p.page_blocks.of(block);
           if (slot != load_slot && (i == 0 || block * kBlock < span.length)) {
             load_slot = slot;
             load_page = __ldg(table + slot);
             if (load_page >= a.table.pages) load_page = -1;   // outside the tensor: zeros come back
           }
           page[i] = slot == load_slot ? load_page : -1;
-          at[i] = (block - slot * p.page_blocks) * kBlock;
+          at[i] = (block - slot * p.page_blocks.d) * kBlock;
           if (page[i] < 0) mask &= ~(0xffffu << (i * kBlock));
         }
         if (tc::elect_one()) {
@@ -488,13 +498,13 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
 #pragma unroll
         for (int c = 0; c < kCols; ++c)
 #pragma unroll
-          for (int i = 0; i < 2 * kHalves; ++i) o[c][i] *= keep[i >> 1];
+          for (int i = 0; i < 4; ++i) o[c][i] *= keep[ROWS == 8 ? 0 : i >> 1];
       }
 #pragma unroll
       for (int i = 0; i < kSub; ++i) {
-        // weights as the sum of two 16-bit values: rounded once to 16 bits they would cost the result as much as its own rounding does,
-        // and the tensor cores have nothing else to do
-        uint32_t hi[4] = {}, lo[4] = {};
+        // weights as the sum of two 16-bit values: rounded once to 16 bits they would cost the result as much as its own rounding does.  With
+        // eight queries the rest goes into the eight rows of the product that have none.
+        uint32_t hi[4], lo[4];
 #pragma unroll
         for (int h = 0; h < kHalves; ++h)
 #pragma unroll
@@ -502,7 +512,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             const float w0 = z[h][4 * i + 2 * e], w1 = z[h][4 * i + 2 * e + 1];
             hi[e * 2 + h] = pair<H>(w0, w1);
             const float2 back = unpair<H>(hi[e * 2 + h]);
-            lo[e * 2 + h] = pair<H>(w0 - back.x, w1 - back.y);
+            const uint32_t rest = pair<H>(w0 - back.x, w1 - back.y);
+            if (ROWS == 8) hi[e * 2 + 1] = rest; else lo[e * 2 + h] = rest;
           }
         // values of positions that are not seen may be anything: they are cleared, for zero times anything need not be zero
         uint32_t clear[2] = {0xffffffffu, 0xffffffffu};
@@ -523,8 +534,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
           }
           mma<H>(o[c], hi, r[0], r[1]);
           mma<H>(o[c + 1], hi, r[2], r[3]);
-          mma<H>(o[c], lo, r[0], r[1]);
-          mma<H>(o[c + 1], lo, r[2], r[3]);
+          if (ROWS == 16) {
+            mma<H>(o[c], lo, r[0], r[1]);
+            mma<H>(o[c + 1], lo, r[2], r[3]);
+          }
         }
       }
       __syncwarp();   // every lane has read its fragments
@@ -538,11 +551,15 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
 
     // ---- the end of this piece: the result where it is the whole item, else its sums for the block
     const bool complete = from == 0 && at.t == tiles;
-    const int b = item / p.items_per_sequence, hh = item - b * p.items_per_sequence;
-    const int kv = hh / p.blocks_of_heads, in_group = (hh - kv * p.blocks_of_heads) * ROWS;
+    const int b = p.items.of(item), hh = item - b * per_sequence;
+    const int kv = p.head_blocks.of(hh), in_group = (hh - kv * p.head_blocks.d) * ROWS;
     const int heads = min(p.group - in_group, ROWS), head0 = kv * p.group + in_group;
     const int which = first_piece ? 0 : 1;
     unsigned char* sums = first_piece ? first_pieces + warp * S::kPiece : smem + warp * (STAGES * S::kStageBytes);
+    if (ROWS == 8) {
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) o[c][0] += o[c][2], o[c][1] += o[c][3];
+    }
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) {
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
@@ -597,8 +614,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     const unsigned run = __ballot_sync(0xffffffffu, their_item == item) & pieces;
     rest &= ~run;
     const int begun = __shfl_sync(0xffffffffu, their_ends, __ffs(run) - 1) & 1, ended = __shfl_sync(0xffffffffu, their_ends, 31 - __clz(run)) & 2;
-    const int b = item / p.items_per_sequence, hh = item - b * p.items_per_sequence;
-    const int kv = hh / p.blocks_of_heads, in_group = (hh - kv * p.blocks_of_heads) * ROWS;
+    const int b = p.items.of(item), hh = item - b * per_sequence;
+    const int kv = p.head_blocks.of(hh), in_group = (hh - kv * p.head_blocks.d) * ROWS;
     const int heads = min(p.group - in_group, ROWS);
     for (int u = threadIdx.x; u < heads * DP / 4; u += WARPS * 32) {
       const int row = u / (DP / 4), col = u % (DP / 4) * 4;
@@ -640,13 +657,13 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(Launch p) {
   Sums* sums = reinterpret_cast<Sums*>(raw);
   const PagedAttentionArgs& a = p.a;
   const int b = blockIdx.y, h = blockIdx.x, kv = h / p.group, in_group = h - kv * p.group;
-  const int k = kv * p.blocks_of_heads + in_group / ROWS, row = in_group % ROWS;
+  const int k = kv * p.head_blocks.d + in_group / ROWS, row = in_group % ROWS;
   const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   ::mccl::pdl_wait();
   ::mccl::pdl_trigger();
   const unsigned per = p.plan[0], first = p.plan[1 + b], tiles = p.plan[2 + b] - first;
   if (tiles == 0) return;
-  const unsigned s = first * p.items_per_sequence + k * tiles;
+  const unsigned s = first * p.items.d + k * tiles;
   const int c0 = static_cast<int>(s / per), c1 = static_cast<int>((s + tiles - 1) / per);
   if (c0 == c1) return;
   Sums sum;
@@ -708,10 +725,11 @@ bool encode_queries(CUtensorMap* map, const PagedAttentionArgs& a, int dp, int r
 }
 
 template <typename H, int DP, int KT, int WARPS, int STAGES, int ROWS, bool TMA>
-cudaError_t launch(const Launch& p, const CUtensorMap (&maps)[3], cudaStream_t stream) {
+cudaError_t launch(Launch& p, const CUtensorMap (&maps)[3], cudaStream_t stream) {
   constexpr int smem = Shape<DP, KT, WARPS, STAGES, ROWS>::kSmem;
   static const cudaError_t rc = cudaFuncSetAttribute(paged_attention_kernel<H, DP, KT, WARPS, STAGES, ROWS, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (rc != cudaSuccess) return rc;
+  p.warps = Divisor(sm_count() * WARPS);
   MCCL_LAUNCH_PDL((paged_attention_kernel<H, DP, KT, WARPS, STAGES, ROWS, TMA>), sm_count(), WARPS * 32, smem, stream, maps[0], maps[1], maps[2], p);
   count_launch();
   if (!p.whole) {
@@ -724,7 +742,7 @@ cudaError_t launch(const Launch& p, const CUtensorMap (&maps)[3], cudaStream_t s
 // Sizes of tile and ring: as many warps as hide the latency of a tile's chain (scores, maximum, weights, products), two stages of 8 KB each.  More bytes in
 // flight are slower (2 x 131009 positions: three stages 181 us, two 172), fewer warps too (4 x 4 stages 191, 6 x 2 182).
 template <typename H, bool TMA>
-cudaError_t by_size(const Launch& p, int rows, const CUtensorMap (&maps)[3], cudaStream_t stream) {
+cudaError_t by_size(Launch& p, int rows, const CUtensorMap (&maps)[3], cudaStream_t stream) {
   const int dp = padded_dim(p.a.head_dim);
   if (rows == 8) {
     if (dp == 32) return launch<H, 32, 32, 8, 4, 8, TMA>(p, maps, stream);
@@ -750,12 +768,10 @@ cudaError_t paged_attention(const PagedAttentionArgs& args, cudaStream_t stream)
   Launch p;
   p.group = args.heads / args.kv_heads;
   const int rows = rows_of(args), dp = padded_dim(args.head_dim);
-  p.blocks_of_heads = (p.group + rows - 1) / rows;
-  p.items_per_sequence = args.kv_heads * p.blocks_of_heads;
-  p.page_blocks = args.table.page_size % kBlock == 0 ? args.table.page_size / kBlock : 0;
-  p.page_shift = -1;
-  for (int s = 0; s < 27; ++s)
-    if (p.page_blocks == 1 << s) p.page_shift = s;
+  p.head_blocks = Divisor((p.group + rows - 1) / rows);
+  p.items = Divisor(args.kv_heads * p.head_blocks.d);
+  const bool blocks = args.table.page_size % kBlock == 0;
+  p.page_blocks = Divisor(blocks ? args.table.page_size / kBlock : 1);
   p.scale_log2 = args.scale * kLog2e;
   p.whole = whole(args) ? 1 : 0;
   p.plan = static_cast<unsigned*>(args.workspace);
@@ -763,9 +779,9 @@ cudaError_t paged_attention(const PagedAttentionArgs& args, cudaStream_t stream)
   p.part_o = p.part_ml + static_cast<size_t>(sm_count()) * 2 * rows * 2;
   p.err = gemm_error_device_ptr();
   CUtensorMap maps[3] = {};
-  const bool paged = p.page_blocks > 0 && encode_pages(&maps[0], args.k_pages, args, dp) && encode_pages(&maps[1], args.v_pages, args, dp);
+  const bool paged = blocks && encode_pages(&maps[0], args.k_pages, args, dp) && encode_pages(&maps[1], args.v_pages, args, dp);
   // tiles of a launch are counted in 32 bits: as many sequences as cannot have more (a product with the blocks' number is among the sums)
-  const long long most = (static_cast<long long>(args.table.width) * args.table.page_size / kBlock + 1) * p.items_per_sequence, room = 0xf0000000ll / most;
+  const long long most = (static_cast<long long>(args.table.width) * args.table.page_size / kBlock + 1) * p.items.d, room = 0x7f000000ll / most;
   if (room < 1) return cudaErrorInvalidValue;
   const int step = room < kSequences ? static_cast<int>(room) : kSequences;
   for (int b = 0; b < args.batch; b += step) {
