@@ -78,7 +78,7 @@ cudaError_t paged_attention(const PagedAttentionArgs& a, cudaStream_t stream);
 
 // ---- y[m, n] = act(sum_k x[m, k] scale[n, k / group] (code[n, k] - zero[n, k / group]) + bias[n]) + residual[m, n], bf16.
 // Weights as laid out by mccl_b200/ops/w4.py: tiles of 16 rows and 64 columns, 512 bytes each, [ceil(n / 16), ceil(k / 64)]; a lane's 16
-// bytes are the A fragments of its four m16n8k16 products.  params [ceil(n / 16), k / group, 8, 2]: for rows r and r + 8 of a tile the
+// bytes are the A fragments of four m16n8k16 products.  params [ceil(n / 16), k / group, 8, 2]: for rows r and r + 8 of a tile the
 // scale as bf16 bits and above them those of 128 + zero.  k % 32 == 0, group 32, 64, 128 or 256 and a divisor of k.
 struct W4Args {
   const void* x = nullptr;   // [m, k] bf16, rows ldx elements apart (a multiple of 8), 16-byte aligned

@@ -1,139 +1,469 @@
-// Products of few rows with 4-bit weights.
+// Products with 4-bit weights: y = x W^T, W[n, k] = scale[n, k / g] (code - zero).
 //
-// y = x W^T with W[n, k] = scale[n, k / g] (code - zero): a group's sum is scale * sum x (code - zero), so the codes go into the product as
-// whole numbers and the scale is applied once per group to a sum in fp32.  Nothing but x and y is rounded to 16 bits.
-// The weights are read once, 0.5 bytes each, and bound the time.  They are the A operand of m16n8k16 products (16 weight rows, 8 rows of x
-// as columns): the tensor cores of this generation's own instruction take 64 to 256 rows of x at a time and operands in shared or tensor
-// memory, which single tokens do not fill, while here a code goes from its load through one mask and one subtraction into the product.
+// Two kernels.  For up to 16 rows of x the weights are read once, half a byte each, and bound the time: the narrow kernel multiplies codes as whole
+// numbers and applies a group's scale to its sum in fp32, scale * sum x (code - zero), so nothing but x and y is rounded to 16 bits.  For more rows
+// the wide kernel makes bf16 weights on the way into tensor memory, where they are the left operand of tcgen05 products.
+#include <cuda.h>
+
 #include "../core/launch.hpp"
 #include "bf16x8.cuh"
+#include "gemm_common.cuh"
 #include "ops.hpp"
 #include "serving.hpp"
+#include "tcgen05.cuh"
 
 namespace mccl {
 namespace ops {
 
 namespace {
 
-constexpr int kWarps = 8;
-
 __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
   const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-// Two codes (bits 0-3 and 16-19 of w >> 4 j) as bf16 pair code - zero: 0x4300 is 128, whose last mantissa bit is worth one.
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// Two codes (bits 0-3 and 16-19) as a bf16 pair code - zero: 0x4300 is 128, whose last mantissa bit is worth one.
 __device__ __forceinline__ uint32_t codes2(uint32_t w, uint32_t zero2) { return sub2((w & 0x000f000fu) | 0x43004300u, zero2); }
+// Of a row's parameters (scale, and above it 128 + zero) the scale, and either of them twice.
+__device__ __forceinline__ float scale_of(uint32_t p) { return __uint_as_float(p << 16); }
+__device__ __forceinline__ uint32_t scale2(uint32_t p) { return __byte_perm(p, 0, 0x1010); }
+__device__ __forceinline__ uint32_t zero2(uint32_t p) { return __byte_perm(p, 0, 0x3232); }
 
+template <int kBytes>
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from, bool real = true) {
+  if (kBytes == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(real ? 16 : 0) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(kBytes), "r"(real ? kBytes : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
+__device__ __forceinline__ uint4 shared16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 shared8(uint32_t at) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void load_matrix(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ float finished(const W4Args& a, float v, int m, int n) {
+  if (a.bias) v += __ldg(a.bias + n);
+  if (a.gelu) v = 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
+  if (a.residual) v += __bfloat162float(static_cast<const __nv_bfloat16*>(a.residual)[m * a.ldr + n]);
+  return v;
+}
 
-// A block has kR tiles of 16 weight rows and kN tiles of 8 rows of x; its warps share out K in chunks of 64 and add up at the end.
-template <int kR, int kN, bool kG32>
-__global__ void __launch_bounds__(kWarps * 32) w4_linear_kernel(W4Args a) {
-  extern __shared__ float sums[];   // [warp][token][weight row]
+// ----------------------------------------------------------- up to 16 rows of x --
+constexpr int kNarrowWarps = 8, kNarrowThreads = kNarrowWarps * 32;
+constexpr int kDeep = 4;   // stages of 128 columns that a warp has on their way
+template <int kParams>
+constexpr int kNarrowSlot = 1024 + kParams * 256;
+template <int kN>
+constexpr int kNarrowSums = 2 * kNarrowWarps * kN * 128 * 4;
+template <int kN, int kParams>
+int narrow_smem(int m, int pairs) { return kNarrowWarps * kDeep * kNarrowSlot<kParams> + kNarrowSums<kN> + m * pairs * 256 + 16; }
+
+// A block takes tiles of 16 weight rows, gridDim.x apart; its warps share out K, each a run of stages of 128 columns, and add up at the end of a tile.  A
+// lane's 16 bytes of 64 columns are its own A fragments of four m16n8k16 products: it copies them ahead into its own place and waits for nobody, and so
+// it does with its two rows' parameters (kParams groups in a stage).  x lies in shared memory, 128 bytes of every row per 64 columns, in the order of the
+// 128-byte swizzle; kN is how many times 8 rows it has.
+template <int kN, int kParams>
+__global__ void __launch_bounds__(kNarrowThreads) w4_narrow_kernel(W4Args a, int tiles, int chunks, int group_shift) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  constexpr int kSlot = kNarrowSlot<kParams>, kRows = 8 * kN, kOut = 128 * kN;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int row_tiles = (a.n + 15) / 16, chunks = (a.k + 63) / 64, groups = a.k / a.group;
-  const int tile0 = blockIdx.x * kR, token0 = blockIdx.y * (8 * kN);
-  const uint4* codes = static_cast<const uint4*>(a.codes);
-  const uint2* params = static_cast<const uint2*>(a.params);
-  const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(a.x);
+  const uint32_t ring = tc::smem_u32(smem) + warp * (kDeep * kSlot);
+  float* sums = reinterpret_cast<float*>(smem + kNarrowWarps * kDeep * kSlot);   // [2][warp][row of x][weight row]
+  const int pairs = (chunks + 1) / 2;
+  const uint32_t xs = tc::smem_u32(smem) + kNarrowWarps * kDeep * kSlot + kNarrowSums<kN>, nothing = xs + a.m * pairs * 256;
+  const int c0 = pairs * warp / kNarrowWarps, slice = pairs * (warp + 1) / kNarrowWarps - c0;
+  const int groups = a.k >> group_shift, mine = (tiles - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
   ::mccl::pdl_wait();
   ::mccl::pdl_trigger();
 
-  float total[kR][kN][4] = {};
-  for (int c = warp; c < chunks; c += kWarps) {
-    uint4 w[kR];
+  for (int i = threadIdx.x; i < a.m * pairs * 16; i += kNarrowThreads) {
+    const int row = i / (pairs * 16), piece = i - row * (pairs * 16);
+    const bool real = piece * 8 < a.k;
+    copy_async<16>(xs + (piece >> 3) * (a.m * 128) + row * 128 + (((piece ^ row) & 7) << 4), static_cast<const __nv_bfloat16*>(a.x) + (real ? row * a.ldx + piece * 8 : 0), real);
+  }
+  if (threadIdx.x == 0) *reinterpret_cast<uint4*>(smem + (nothing - tc::smem_u32(smem))) = make_uint4(0, 0, 0, 0);   // rows of x that there are not
+  copy_commit();
+
+  // ---- the loading side
+  int to_load = slice * mine, at = c0;
+  const uint4* codes = static_cast<const uint4*>(a.codes) + (static_cast<size_t>(blockIdx.x) * chunks + 2 * c0) * 32 + lane;
+  const uint2* params = static_cast<const uint2*>(a.params) + static_cast<size_t>(blockIdx.x) * groups * 8 + g;
+  const size_t codes_on = (static_cast<size_t>(gridDim.x) * chunks - 2 * slice) * 32, params_on = static_cast<size_t>(gridDim.x) * groups * 8;
+  auto issue = [&](int slot) {
+    if (to_load > 0) {
+      const uint32_t to = ring + slot * kSlot;
+      copy_async<16>(to + lane * 16, codes);
+      const bool second = 2 * at + 1 < chunks;
+      copy_async<16>(to + 512 + lane * 16, second ? codes + 32 : codes, second);
 #pragma unroll
-    for (int r = 0; r < kR; ++r)
-      w[r] = tile0 + r < row_tiles ? __ldg(codes + (static_cast<size_t>(tile0 + r) * chunks + c) * 32 + lane) : make_uint4(0, 0, 0, 0);
-    uint4 xv[kN][2];
-#pragma unroll
-    for (int n = 0; n < kN; ++n)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int token = token0 + n * 8 + g, k = c * 64 + h * 32 + t * 8;
-        xv[n][h] = token < a.m && k < a.k ? __ldg(reinterpret_cast<const uint4*>(x + token * a.ldx + k)) : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < kParams; ++i) {
+        const int group = kParams == 1 ? at >> (group_shift - 7) : min(kParams * at + i, groups - 1);
+        copy_async<8>(to + 1024 + i * 256 + lane * 8, params + group * 8);
       }
-    constexpr int kParts = kG32 ? 2 : 1;   // groups that a chunk touches
-    uint2 prm[kR][kParts];
-#pragma unroll
-    for (int r = 0; r < kR; ++r)
-#pragma unroll
-      for (int h = 0; h < kParts; ++h) {
-        const int group = min((c * 64 + h * 32) / a.group, groups - 1);
-        prm[r][h] = tile0 + r < row_tiles ? __ldg(params + (static_cast<size_t>(tile0 + r) * groups + group) * 8 + g) : make_uint2(0, 0);
+      --to_load;
+      codes += 64;
+      if (++at == c0 + slice) {
+        at = c0;
+        codes += codes_on;
+        params += params_on;
       }
+    }
+    copy_commit();
+  };
 #pragma unroll
-    for (int r = 0; r < kR; ++r) {
-      float acc[kN][4] = {};
+  for (int i = 0; i < kDeep - 1; ++i) issue(i);
+  copy_wait<kDeep - 1>();   // x
+  __syncthreads();
+
+  const int row = lane & 7;
+  uint32_t x_lane[kN], x_step[kN], x_half[kN];   // pieces 0 to 3 of the first chunk; 4 to 7 are 64 bytes on, the next chunk x_step
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint2 p = prm[r][kG32 ? h : 0];
-        const uint32_t z0 = __byte_perm(p.x, 0, 0x3232), z8 = __byte_perm(p.y, 0, 0x3232);
+  for (int n = 0; n < kN; ++n) {
+    const bool real = n * 8 + row < a.m;
+    x_step[n] = real ? a.m * 128 : 0;
+    x_half[n] = real ? 64 : 0;
+    x_lane[n] = real ? xs + c0 * (a.m * 256) + (n * 8 + row) * 128 + (((lane >> 3) ^ row) << 4) : nothing;
+  }
+  int slot = 0;
+  for (int i = 0; i < mine; ++i) {
+    float total[kN][4] = {};
+    uint32_t x_at[kN];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const uint32_t word = h == 0 ? (s == 0 ? w[r].x : w[r].y) : (s == 0 ? w[r].z : w[r].w);
-          const uint32_t a0 = codes2(word, z0), a1 = codes2(word >> 4, z8), a2 = codes2(word >> 8, z0), a3 = codes2(word >> 12, z8);
+    for (int n = 0; n < kN; ++n) x_at[n] = x_lane[n];
+    for (int c = 0; c < slice; ++c) {
+      copy_wait<kDeep - 2>();
+      const uint32_t from = ring + slot * kSlot;
+      const uint4 w[2] = {shared16(from + lane * 16), shared16(from + 512 + lane * 16)};
+      uint2 p[kParams];
 #pragma unroll
-          for (int n = 0; n < kN; ++n) mma16816(acc[n], a0, a1, a2, a3, s == 0 ? xv[n][h].x : xv[n][h].z, s == 0 ? xv[n][h].y : xv[n][h].w);
+      for (int j = 0; j < kParams; ++j) p[j] = shared8(from + 1024 + j * 256 + lane * 8);
+      issue(slot == 0 ? kDeep - 1 : slot - 1);
+      slot = slot == kDeep - 1 ? 0 : slot + 1;
+      float acc[2][kN][4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t word[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+        uint32_t b[kN][2][4];
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+          load_matrix(b[n][0], x_at[n]);
+          load_matrix(b[n][1], x_at[n] ^ x_half[n]);
+          x_at[n] += x_step[n];
         }
-        if (kG32 || h == 1) {
-          const float s0 = __uint_as_float(p.x << 16), s8 = __uint_as_float(p.y << 16);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const uint2 q = p[kParams == 4 ? 2 * j + (s >> 1) : (kParams == 2 ? j : 0)];
+          const uint32_t z0 = zero2(q.x), z8 = zero2(q.y);
+          const uint32_t a0 = codes2(word[s], z0), a1 = codes2(word[s] >> 4, z8), a2 = codes2(word[s] >> 8, z0), a3 = codes2(word[s] >> 12, z8);
+          const bool begins = kParams == 4 ? (s & 1) == 0 : s == 0, ends = kParams == 4 ? (s & 1) == 1 : s == 3;
 #pragma unroll
           for (int n = 0; n < kN; ++n) {
-            total[r][n][0] += s0 * acc[n][0];
-            total[r][n][1] += s0 * acc[n][1];
-            total[r][n][2] += s8 * acc[n][2];
-            total[r][n][3] += s8 * acc[n][3];
-            acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+            if (begins) acc[j][n][0] = acc[j][n][1] = acc[j][n][2] = acc[j][n][3] = 0.f;
+            mma16816(acc[j][n], a0, a1, a2, a3, b[n][s >> 1][(s & 1) * 2], b[n][s >> 1][(s & 1) * 2 + 1]);
+            if (ends && (kParams > 1 || j == 1)) {
+              if (kParams == 1) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[1][n][e] += acc[0][n][e];
+              }
+              const float s0 = scale_of(q.x), s8 = scale_of(q.y);
+              total[n][0] += s0 * acc[j][n][0];
+              total[n][1] += s0 * acc[j][n][1];
+              total[n][2] += s8 * acc[j][n][2];
+              total[n][3] += s8 * acc[j][n][3];
+            }
           }
         }
       }
     }
-  }
-  constexpr int kRows = kR * 16, kTokens = kN * 8;
-#pragma unroll
-  for (int r = 0; r < kR; ++r)
+    float* to = sums + ((i & 1) * kNarrowWarps + warp) * kOut;
 #pragma unroll
     for (int n = 0; n < kN; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        sums[(warp * kTokens + n * 8 + 2 * t + (i & 1)) * kRows + r * 16 + g + (i >> 1) * 8] = total[r][n][i];
-  __syncthreads();
-  for (int i = threadIdx.x; i < kRows * kTokens; i += kWarps * 32) {
-    const int n = tile0 * 16 + i % kRows, m = token0 + i / kRows;
-    if (n >= a.n || m >= a.m) continue;
-    float v = 0.f;
+      for (int e = 0; e < 4; ++e) to[(n * 8 + 2 * t + (e & 1)) * 16 + g + 8 * (e >> 1)] = total[n][e];
+    __syncthreads();
+    int out = threadIdx.x;
+    if (kN == 1) out -= (i & 1) * 128;   // the two halves of the block take turns
+    if (out >= 0 && out < kOut) {
+      const int m = out >> 4, n = (static_cast<int>(blockIdx.x) + i * static_cast<int>(gridDim.x)) * 16 + (out & 15);
+      if (m < a.m && n < a.n) {
+        float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) v += sums[w * (kRows * kTokens) + i];
-    if (a.bias) v += a.bias[n];
-    if (a.gelu) v = 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
-    if (a.residual) v += __bfloat162float(static_cast<const __nv_bfloat16*>(a.residual)[m * a.ldr + n]);
-    static_cast<__nv_bfloat16*>(a.y)[static_cast<long long>(m) * a.n + n] = __float2bfloat16_rn(v);
+        for (int w = 0; w < kNarrowWarps; ++w) v += sums[((i & 1) * kNarrowWarps + w) * kOut + out];
+        static_cast<__nv_bfloat16*>(a.y)[static_cast<long long>(m) * a.n + n] = __float2bfloat16_rn(finished(a, v, m, n));
+      }
+    }
+  }
+  copy_wait<0>();
+}
+
+// --------------------------------------------------------------- more rows of x --
+constexpr int kWideRows = 128;             // weight rows of a block: the lanes of tensor memory
+constexpr int kWideThreads = 10 * 32;      // warp 0 brings x, warp 1 issues the products, eight make weights and write results
+constexpr int kWideStages = 4;
+constexpr int kCodeDeep = 4;               // chunks that a weight-making warp has on their way
+constexpr int kCodeRing = 8 * kCodeDeep * 2 * 512;
+constexpr int kMostTokens = 128;           // rows of x of a block; twice 256 columns of tensor memory (sums 128, weights 4 x 32) are two blocks per SM
+
+struct Wide {
+  W4Args a;
+  int tokens, chunks, group_shift;   // rows of x per block, a multiple of 16; chunks of 64 columns in K
+  int columns;          // of tensor memory that the sums take; the weights' ring lies behind them
+  int allocated;
+  int splits;           // blocks of a cluster that share out K
+  uint32_t idesc;
+  int* err;
+};
+
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_cols, uint64_t desc_b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a_cols), "l"(desc_b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+      : "memory");
+}
+// 16 lanes x 64 bf16: register 2 i + r of lane 4 g + t is elements 8 i + 2 t and + 1 of row g + 8 r.
+__device__ __forceinline__ void tmem_st_16x64(uint32_t at, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t at, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+                 "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float4 peer_float4(uint32_t at, int rank) {
+  uint32_t there;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(there) : "memory");
+  return v;
+}
+
+// Block (x, y, z): weight rows 128 x and on, rows of x from `tokens` y on, part z of K.  D[weight row, row of x] = W x^T: the weights of a chunk of 64
+// columns go from a lane's 16 bytes through registers into tensor memory (the lanes of an m16n8k16 A fragment are those of a 16x128b store), x comes
+// by TMA.  The weights are rounded to bf16 once, scale times whole number, as a stored bf16 weight would be.
+template <bool kG32>
+__global__ void __launch_bounds__(kWideThreads, 2) w4_wide_kernel(const __grid_constant__ CUtensorMap x_map, Wide p) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024 - (tc::smem_u32(smem_raw) & 1023)) & 1023);
+  __shared__ uint64_t x_full[kWideStages], w_full[kWideStages], empty[kWideStages], done;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int bad;
+  const W4Args& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int first = p.chunks * static_cast<int>(blockIdx.z) / p.splits, last = p.chunks * (static_cast<int>(blockIdx.z) + 1) / p.splits;
+  const int stage_bytes = p.tokens * 128;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kWideStages; ++i) {
+      tc::mbar_init(x_full + i, 1);
+      tc::mbar_init(w_full + i, 4);
+      tc::mbar_init(empty + i, 1);
+    }
+    tc::mbar_init(&done, 1);
+    tc::mbar_init_fence();
+    bad = 0;
+    tc::tma_prefetch_desc(&x_map);
+  }
+  __syncwarp();
+  if (warp == 1) tc::tmem_alloc(&tmem_slot, p.allocated);
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  ::mccl::pdl_wait();
+  ::mccl::pdl_trigger();
+
+  if (warp == 0) {   // ---- x
+    if (tc::elect_one()) {
+      int c = first;
+      for (; c < last; ++c) {
+        const int i = c - first, s = i % kWideStages;
+        if (i >= kWideStages && !tc::mbar_wait(empty + s, ((i / kWideStages) - 1) & 1)) {
+          bad = 1;
+          break;
+        }
+        tc::mbar_expect_tx(x_full + s, stage_bytes);
+        tc::tma_load_2d(smem + s * stage_bytes, &x_map, x_full + s, c * 64, blockIdx.y * p.tokens);
+      }
+      if (bad)   // what was issued must land before the block retires
+        for (int i = max(c - first - kWideStages, 0); i < c - first; ++i) tc::mbar_wait(x_full + i % kWideStages, (i / kWideStages) & 1, 1u << 20);
+    }
+    __syncwarp();
+  } else if (warp == 1) {   // ---- products
+    for (int c = first; c < last; ++c) {
+      const int i = c - first, s = i % kWideStages;
+      bool ok = tc::mbar_wait(x_full + s, (i / kWideStages) & 1);
+      ok = tc::mbar_wait(w_full + s, (i / kWideStages) & 1) && ok;
+      ok = __all_sync(0xffffffffu, ok);
+      tc::fence_after_sync();
+      if (tc::elect_one()) {
+        if (ok) {
+          const uint64_t db = tc::smem_desc_k_sw128(smem + s * stage_bytes);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mma_ts(tmem, tmem + p.columns + s * 32 + k * 8, db + 2 * k, p.idesc, i > 0 || k > 0);
+          tc::mma_commit(empty + s);
+        } else {
+          bad = 1;
+        }
+      }
+      __syncwarp();
+      if (!ok) break;
+    }
+    if (tc::elect_one()) tc::mma_commit(&done);   // also after a failure: it releases the waiters
+    __syncwarp();
+  } else {   // ---- weights: two warps for each 32 rows take chunks in turn
+    const int quarter = warp & 3, turn = (warp - 2) >> 2, g = lane >> 2;
+    const int row_tiles = (a.n + 15) / 16, groups = a.k >> p.group_shift, tile0 = blockIdx.x * (kWideRows / 16) + quarter * 2;
+    const uint32_t ring = tc::smem_u32(smem) + kWideStages * stage_bytes + (warp - 2) * (kCodeDeep * 2 * 512) + lane * 16;
+    auto issue = [&](int c, int slot) {
+      if (c < last) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          copy_async<16>(ring + (slot * 2 + i) * 512, static_cast<const uint4*>(a.codes) + (tile0 + i < row_tiles ? (static_cast<size_t>(tile0 + i) * p.chunks + c) * 32 + lane : 0),
+                         tile0 + i < row_tiles);
+      }
+      copy_commit();
+    };
+    uint2 prm[2][2];
+    auto parameters = [&](int c, uint2 (&to)[2][2]) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int h = 0; h < (kG32 ? 2 : 1); ++h) {
+          const int group = min((c * 64 + h * 32) >> p.group_shift, groups - 1);
+          to[i][h] = c < last && tile0 + i < row_tiles ? __ldg(static_cast<const uint2*>(a.params) + (static_cast<size_t>(tile0 + i) * groups + group) * 8 + g) : make_uint2(0, 0);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < kCodeDeep - 1; ++i) issue(first + turn + 2 * i, i);
+    parameters(first + turn, prm);
+    int slot = 0;
+    for (int c = first + turn; c < last; c += 2) {
+      const int i = c - first, s = i % kWideStages;
+      copy_wait<kCodeDeep - 2>();
+      uint4 w[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) w[k] = shared16(ring + (slot * 2 + k) * 512);
+      issue(c + 2 * (kCodeDeep - 1), slot == 0 ? kCodeDeep - 1 : slot - 1);
+      slot = slot == kCodeDeep - 1 ? 0 : slot + 1;
+      uint2 next[2][2];
+      parameters(c + 2, next);
+      const bool ok = __all_sync(0xffffffffu, i < kWideStages || tc::mbar_wait(empty + s, ((i / kWideStages) - 1) & 1));
+      if (!ok) {
+        if (lane == 0) bad = 1;
+        break;
+      }
+      tc::fence_after_sync();
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t word[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+        uint32_t r[16];
+#pragma unroll
+        for (int step = 0; step < 4; ++step) {
+          const uint2 q = prm[k][kG32 ? step >> 1 : 0];
+          r[4 * step] = mul2(codes2(word[step], zero2(q.x)), scale2(q.x));
+          r[4 * step + 1] = mul2(codes2(word[step] >> 4, zero2(q.y)), scale2(q.y));
+          r[4 * step + 2] = mul2(codes2(word[step] >> 8, zero2(q.x)), scale2(q.x));
+          r[4 * step + 3] = mul2(codes2(word[step] >> 12, zero2(q.y)), scale2(q.y));
+        }
+        tmem_st_16x64(tmem + (static_cast<uint32_t>(quarter * 32 + k * 16) << 16) + p.columns + s * 32, r);
+      }
+      tmem_st_wait();
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(w_full + s);
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) prm[k][h] = next[k][h];
+    }
+    copy_wait<0>();
+  }
+
+  // ---- results
+  __syncwarp();
+  const bool ok = tc::mbar_wait(&done, 0);
+  tc::fence_after_sync();
+  float* sums = reinterpret_cast<float*>(smem);   // [row of x][weight row], where x was
+  const int token0 = blockIdx.y * p.tokens;
+  if (warp >= 2 && ok) {
+    const int quarter = warp & 3, turn = (warp - 2) >> 2, row = quarter * 32 + lane, n = blockIdx.x * kWideRows + row;
+    for (int c = turn; c < p.tokens / 16; c += 2) {
+      uint32_t r[16];
+      tmem_ld_32x16(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + c * 16, r);
+      tc::tmem_ld_wait();
+      if (p.splits > 1) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sums[(c * 16 + i) * kWideRows + row] = __uint_as_float(r[i]);
+      } else if (n < a.n) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int m = token0 + c * 16 + i;
+          if (m < a.m) static_cast<__nv_bfloat16*>(a.y)[static_cast<long long>(m) * a.n + n] = __float2bfloat16_rn(finished(a, __uint_as_float(r[i]), m, n));
+        }
+      }
+    }
+  }
+  __syncwarp();
+  if (p.splits > 1) {
+    cluster_sync();
+    const int from = p.tokens * static_cast<int>(blockIdx.z) / p.splits, to = p.tokens * (static_cast<int>(blockIdx.z) + 1) / p.splits;
+    for (int i = from * 32 + threadIdx.x; i < to * 32; i += kWideThreads) {
+      const int m = token0 + (i >> 5), n = blockIdx.x * kWideRows + (i & 31) * 4;
+      if (m >= a.m) break;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int r = 0; r < p.splits; ++r) {
+        const float4 o = peer_float4(tc::smem_u32(sums + i * 4), r);
+        v.x += o.x;
+        v.y += o.y;
+        v.z += o.z;
+        v.w += o.w;
+      }
+      const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < a.n) static_cast<__nv_bfloat16*>(a.y)[static_cast<long long>(m) * a.n + n + e] = __float2bfloat16_rn(finished(a, f[e], m, n + e));
+    }
+    cluster_sync();   // nobody leaves while its sums may be read
+  }
+  if ((!ok || bad) && threadIdx.x == 0) atomicExch(p.err, 22);
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc(tmem, p.allocated);
   }
 }
 
-template <int kR, int kN>
-cudaError_t launch(const W4Args& a, cudaStream_t stream) {
-  const int smem = kWarps * kR * 16 * kN * 8 * static_cast<int>(sizeof(float));
-  const dim3 grid((a.n + 16 * kR - 1) / (16 * kR), (a.m + 8 * kN - 1) / (8 * kN));
-  if (a.group == 32) {
-    static const cudaError_t rc = cudaFuncSetAttribute(w4_linear_kernel<kR, kN, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (rc != cudaSuccess) return rc;
-    MCCL_LAUNCH_PDL((w4_linear_kernel<kR, kN, true>), grid, kWarps * 32, smem, stream, a);
-  } else {
-    static const cudaError_t rc = cudaFuncSetAttribute(w4_linear_kernel<kR, kN, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (rc != cudaSuccess) return rc;
-    MCCL_LAUNCH_PDL((w4_linear_kernel<kR, kN, false>), grid, kWarps * 32, smem, stream, a);
-  }
-  count_launch();
-  return ::mccl::launch_status();
-}
-
-// A warp per tile of 16 x 64: lane (g, t) writes 8 neighbouring values of rows g and g + 8, in both halves.
+// A warp per tile of 16 x 64: lane (g, t) writes pairs of rows g and g + 8.
 __global__ void __launch_bounds__(256) w4_dequantize_kernel(const uint4* __restrict__ codes, const uint2* __restrict__ params, __nv_bfloat16* __restrict__ w,
                                                             int n, int k, int group) {
   ::mccl::pdl_wait();
@@ -144,36 +474,92 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(const uint4* __restr
   for (long long i = blockIdx.x * 8ll + (threadIdx.x >> 5); i < tiles; i += gridDim.x * 8ll) {
     const int tile = static_cast<int>(i / chunks), c = static_cast<int>(i - static_cast<long long>(tile) * chunks);
     const uint4 raw = __ldg(codes + i * 32 + lane);
+    const uint32_t word[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int at = c * 64 + h * 32 + t * 8;
+    for (int s = 0; s < 4; ++s) {
+      const int at = c * 64 + s * 16 + 2 * t;
       if (at >= k) continue;
       const uint2 p = __ldg(params + (static_cast<size_t>(tile) * groups + at / group) * 8 + g);
-      const uint32_t lo = h == 0 ? raw.x : raw.z, hi = h == 0 ? raw.y : raw.w;
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int row = tile * 16 + r * 8 + g;
-        if (row >= n) continue;
-        const uint32_t prm = r == 0 ? p.x : p.y, z = __byte_perm(prm, 0, 0x3232);
-        const float s = __uint_as_float(prm << 16);
-        const uint32_t v[4] = {codes2(lo >> (4 * r), z), codes2(lo >> (8 + 4 * r), z), codes2(hi >> (4 * r), z), codes2(hi >> (8 + 4 * r), z)};
-        float f[8];
-        unpack8(make_uint4(v[0], v[1], v[2], v[3]), f);
-#pragma unroll
-        for (int q = 0; q < 8; ++q) f[q] *= s;
-        *reinterpret_cast<uint4*>(w + static_cast<size_t>(row) * k + at) = pack8(f);
+      for (int j = 0; j < 4; ++j) {   // nibble j: row g + 8 (j & 1), columns 8 (j >> 1) on
+        const int row = tile * 16 + (j & 1) * 8 + g;
+        const uint32_t prm = j & 1 ? p.y : p.x;
+        if (row < n) *reinterpret_cast<uint32_t*>(w + static_cast<size_t>(row) * k + at + (j >> 1) * 8) = mul2(codes2(word[s] >> (4 * j), zero2(prm)), scale2(prm));
       }
     }
   }
+}
+
+int sm_count() {
+  static const int n = [] {
+    int device = 0, sms = 148;
+    if (cudaGetDevice(&device) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+    return sms;
+  }();
+  return n;
+}
+
+int log2_of(int v) {
+  int s = 0;
+  while ((1 << s) < v) ++s;
+  return s;
+}
+
+template <int kN, int kParams>
+cudaError_t launch_narrow(const W4Args& a, cudaStream_t stream) {
+  static const cudaError_t rc = cudaFuncSetAttribute(w4_narrow_kernel<kN, kParams>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+  if (rc != cudaSuccess) return rc;
+  const int chunks = (a.k + 63) / 64, smem = narrow_smem<kN, kParams>(a.m, (chunks + 1) / 2);
+  const int tiles = (a.n + 15) / 16, blocks = sm_count() * (smem <= 113 * 1024 ? 2 : 1);
+  MCCL_LAUNCH_PDL((w4_narrow_kernel<kN, kParams>), tiles < blocks ? tiles : blocks, kNarrowThreads, smem, stream, a, tiles, chunks, log2_of(a.group));
+  count_launch();
+  return ::mccl::launch_status();
+}
+template <int kN>
+cudaError_t narrow(const W4Args& a, cudaStream_t stream) {
+  return a.group == 32 ? launch_narrow<kN, 4>(a, stream) : (a.group == 64 ? launch_narrow<kN, 2>(a, stream) : launch_narrow<kN, 1>(a, stream));
+}
+
+template <bool kG32>
+cudaError_t launch_wide(const W4Args& a, cudaStream_t stream) {
+  static const cudaError_t rc = cudaFuncSetAttribute(w4_wide_kernel<kG32>, cudaFuncAttributeMaxDynamicSharedMemorySize, 113 * 1024);
+  if (rc != cudaSuccess) return rc;
+  Wide p;
+  p.a = a;
+  p.chunks = (a.k + 63) / 64;
+  p.group_shift = log2_of(a.group);
+  const int tiles = (a.m + kMostTokens - 1) / kMostTokens, blocks = (a.n + kWideRows - 1) / kWideRows;
+  p.tokens = ((a.m + tiles - 1) / tiles + 15) / 16 * 16;
+  p.columns = p.tokens <= 32 ? 32 : (p.tokens <= 64 ? 64 : 128);
+  p.allocated = p.columns + kWideStages * 32 <= 256 ? 256 : 512;
+  // parts of K: as many as fill two blocks per SM, of four chunks at least, for a cluster has to add them up
+  int splits = 2 * sm_count() / (blocks * ((a.m + p.tokens - 1) / p.tokens));
+  if (splits > p.chunks / 4) splits = p.chunks / 4;
+  p.splits = splits < 1 ? 1 : (splits > 8 ? 8 : splits);
+  p.idesc = tc::idesc_bf16(kWideRows, p.tokens);
+  p.err = gemm_error_device_ptr();
+  const CuDriver& cu = CuDriver::get();
+  if (!cu.loaded || !cu.TensorMapEncodeTiled) return cudaErrorNotSupported;
+  CUtensorMap map;
+  const cuuint64_t size[2] = {static_cast<cuuint64_t>(a.k), static_cast<cuuint64_t>(a.m)}, stride[1] = {static_cast<cuuint64_t>((a.m > 1 ? a.ldx : a.k) * 2)};
+  const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(p.tokens)}, step[2] = {1, 1};
+  if (cu.TensorMapEncodeTiled(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(a.x), size, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return cudaErrorNotSupported;
+  const dim3 grid(blocks, (a.m + p.tokens - 1) / p.tokens, p.splits);
+  const int smem = kWideStages * p.tokens * 128 + kCodeRing + 1024;
+  MCCL_LAUNCH_PDL_CLUSTER(w4_wide_kernel<kG32>, grid, kWideThreads, smem, stream, static_cast<unsigned>(p.splits), map, p);
+  count_launch();
+  return ::mccl::launch_status();
 }
 
 }  // namespace
 
 cudaError_t w4_linear(const W4Args& a, cudaStream_t stream) {
   if (a.m <= 0 || a.n <= 0) return cudaSuccess;
-  if (a.m <= 8) return launch<2, 1>(a, stream);
-  if (a.m <= 16) return launch<2, 2>(a, stream);
-  return launch<2, 4>(a, stream);
+  const long long x_bytes = static_cast<long long>(a.m) * ((a.k + 127) / 128) * 256;
+  if (a.m <= 16 && x_bytes <= 128 * 1024) return a.m <= 8 ? narrow<1>(a, stream) : narrow<2>(a, stream);
+  return a.group == 32 ? launch_wide<true>(a, stream) : launch_wide<false>(a, stream);
 }
 
 cudaError_t w4_dequantize(const void* codes, const void* params, void* w, int n, int k, int group, cudaStream_t stream) {

@@ -19,8 +19,8 @@ GROUPS = (32, 64, 128, 256)
 class W4Weight:
     """A weight ``[n, k]`` in 4 bits, laid out once for the kernels.
 
-    ``codes``: uint8 ``[ceil(n / 16), ceil(k / 64), 32, 16]``, tiles of 16 rows and 64 columns.  Lane 4 g + t of a tile has rows g and g + 8 and
-    the columns 8 t .. 8 t + 7 of both halves of 32: the fragments that a warp multiplies with, in the order in which it does.
+    ``codes``: uint8 ``[ceil(n / 16), ceil(k / 64), 32, 16]``, tiles of 16 rows and 64 columns.  Word s of lane 4 g + t has of columns 16 s .. 16 s + 15
+    the codes of rows g and g + 8 in columns 2 t, 2 t + 1, 2 t + 8 and 2 t + 9: what a lane holds of the left operand of a 16 x 8 x 16 product.
     ``params``: int32 ``[ceil(n / 16), k / group, 8, 2]``, rows g and g + 8: the scale's bf16 bits, above them those of 128 + zero."""
 
     def __init__(self, codes: torch.Tensor, params: torch.Tensor, n: int, k: int, group: int):
@@ -60,10 +60,10 @@ class W4Weight:
             raise RuntimeError("W4Weight: codes and zeros are numbers from 0 to 15")
         tiles, chunks = -(-n // 16), -(-k // 64)
         padded = F.pad(codes, (0, chunks * 64 - k, 0, tiles * 16 - n)) if (n % 16 or k % 64) else codes
-        # rows: 8 r + g; columns of a chunk: 32 h + 8 t + 4 p + 2 q + e.  Nibble 4 e + 2 q + r of word 2 h + p.
-        c = padded.reshape(tiles, 2, 8, chunks, 2, 4, 2, 2, 2)
-        packed = c[:, 0] | (c[:, 1] << 4)                                       # [tile, g, chunk, h, t, p, q, e]
-        packed = packed.permute(0, 2, 1, 4, 3, 5, 7, 6).reshape(tiles, chunks, 32, 16).contiguous()
+        # rows: 8 r + g; columns of a chunk: 16 s + 8 q + 2 t + e.  Nibble 4 e + 2 q + r of word s.
+        c = padded.reshape(tiles, 2, 8, chunks, 4, 2, 4, 2)
+        packed = c[:, 0] | (c[:, 1] << 4)                                       # [tile, g, chunk, s, q, t, e]
+        packed = packed.permute(0, 2, 1, 5, 3, 6, 4).reshape(tiles, chunks, 32, 16).contiguous()
         scale = F.pad(scales.to(torch.bfloat16), (0, 0, 0, tiles * 16 - n)).view(torch.int16).to(torch.int32) & 0xffff
         zero = torch.full_like(scale, 8) if zeros is None else F.pad(zeros.to(torch.int32), (0, 0, 0, tiles * 16 - n))
         params = scale | ((zero + 0x4300) << 16)                                # bf16 128 is 0x4300, and its last bit is worth one
@@ -78,9 +78,9 @@ class W4Weight:
 
     def _plain(self) -> torch.Tensor:
         tiles, chunks = self.codes.shape[:2]
-        b = self.codes.view(tiles, chunks, 8, 4, 2, 2, 2, 2)                    # [tile, chunk, g, t, h, p, e, q]
-        c = torch.stack((b & 15, b >> 4), dim=1)                                # [tile, r, chunk, g, t, h, p, e, q]
-        c = c.permute(0, 1, 3, 2, 5, 4, 6, 8, 7).reshape(tiles * 16, chunks * 64)[: self.n, : self.k]
+        b = self.codes.view(tiles, chunks, 8, 4, 4, 2, 2)                       # [tile, chunk, g, t, s, e, q]
+        c = torch.stack((b & 15, b >> 4), dim=1)                                # [tile, r, chunk, g, t, s, e, q]
+        c = c.permute(0, 1, 3, 2, 5, 7, 4, 6).reshape(tiles * 16, chunks * 64)[: self.n, : self.k]
         p = self.params.permute(0, 3, 2, 1).reshape(tiles * 16, -1)[: self.n]
         zero = ((p >> 16) & 0xffff) - 0x4300
         scale = (p & 0xffff).to(torch.int16).view(torch.bfloat16).float() if p.numel() else p.float()
