@@ -17,20 +17,23 @@ namespace ops {
 
 namespace {
 
-__device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
 __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
   const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-// Two codes (bits 0-3 and 16-19) as a bf16 pair code - zero: 0x4300 is 128, whose last mantissa bit is worth one.
-__device__ __forceinline__ uint32_t codes2(uint32_t w, uint32_t zero2) { return sub2((w & 0x000f000fu) | 0x43004300u, zero2); }
+// Two codes (bits 0-3 and 16-19) as a bf16 pair code - zero: 0x4300 is 128, whose last mantissa bit is worth one.  Both steps are written out, one
+// instruction each: the mask and the exponent in one three-input operation, the difference (exact) as a product with one and a sum, on the pipe
+// that does no logic.
+__device__ __forceinline__ uint32_t codes2(uint32_t w, uint32_t minus_zero2) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(0x000f000fu), "r"(0x43004300u));
+  asm("fma.rn.bf16x2 %0, %0, %1, %2;" : "+r"(r) : "r"(0x3f803f80u), "r"(minus_zero2));
+  return r;
+}
 // Of a row's parameters (scale, and above it 128 + zero) the scale, and either of them twice.
 __device__ __forceinline__ float scale_of(uint32_t p) { return __uint_as_float(p << 16); }
 __device__ __forceinline__ uint32_t scale2(uint32_t p) { return __byte_perm(p, 0, 0x1010); }
-__device__ __forceinline__ uint32_t zero2(uint32_t p) { return __byte_perm(p, 0, 0x3232); }
+__device__ __forceinline__ uint32_t minus_zero2(uint32_t p) { return __byte_perm(p, 0, 0x3232) ^ 0x80008000u; }
 
 template <int kBytes>
 __device__ __forceinline__ void copy_async(uint32_t to, const void* from, bool real = true) {
@@ -69,29 +72,32 @@ __device__ __forceinline__ float finished(const W4Args& a, float v, int m, int n
 
 // ----------------------------------------------------------- up to 16 rows of x --
 constexpr int kNarrowWarps = 8, kNarrowThreads = kNarrowWarps * 32;
-constexpr int kDeep = 4;   // stages of 128 columns that a warp has on their way
-template <int kParams>
-constexpr int kNarrowSlot = 1024 + kParams * 256;
-template <int kN>
-constexpr int kNarrowSums = 2 * kNarrowWarps * kN * 128 * 4;
-template <int kN, int kParams>
-int narrow_smem(int m, int pairs) { return kNarrowWarps * kDeep * kNarrowSlot<kParams> + kNarrowSums<kN> + m * pairs * 256 + 16; }
+template <int kR>
+constexpr int kDeep = kR == 2 ? 3 : 4;   // stages of 128 columns that a warp has on their way
+template <int kR, int kParams>
+constexpr int kNarrowSlot = kR * (1024 + kParams * 256);
+template <int kR, int kN>
+constexpr int kNarrowSums = 2 * kNarrowWarps * kR * kN * 128 * 4;
+template <int kR, int kN, int kParams>
+int narrow_smem(int m, int pairs) { return kNarrowWarps * kDeep<kR> * kNarrowSlot<kR, kParams> + kNarrowSums<kR, kN> + m * pairs * 256 + 16; }
 
-// A block takes tiles of 16 weight rows, gridDim.x apart; its warps share out K, each a run of stages of 128 columns, and add up at the end of a tile.  A
-// lane's 16 bytes of 64 columns are its own A fragments of four m16n8k16 products: it copies them ahead into its own place and waits for nobody, and so
+// A warp takes kR tiles of 16 weight rows at a time, a block 8 / along times as many, gridDim.x such groups apart; `along` warps share out K for each, a
+// run of stages of 128 columns, and add up at its end.  A lane's 16 bytes of 64 columns are its own A fragments of four m16n8k16 products: it copies them ahead into its own place and waits for nobody, and so
 // it does with its two rows' parameters (kParams groups in a stage).  x lies in shared memory, 128 bytes of every row per 64 columns, in the order of the
 // 128-byte swizzle; kN is how many times 8 rows it has.
-template <int kN, int kParams>
-__global__ void __launch_bounds__(kNarrowThreads) w4_narrow_kernel(W4Args a, int tiles, int chunks, int group_shift) {
+template <int kR, int kN, int kParams>
+__global__ void __launch_bounds__(kNarrowThreads, 2) w4_narrow_kernel(W4Args a, int tiles, int chunks, int group_shift, int along_shift) {
   extern __shared__ __align__(128) unsigned char smem[];
-  constexpr int kSlot = kNarrowSlot<kParams>, kRows = 8 * kN, kOut = 128 * kN;
+  constexpr int kSlot = kNarrowSlot<kR, kParams>, kTile = 1024 + kParams * 256, kDeep = ops::kDeep<kR>, kOut = kR * kN * 128;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const uint32_t ring = tc::smem_u32(smem) + warp * (kDeep * kSlot);
   float* sums = reinterpret_cast<float*>(smem + kNarrowWarps * kDeep * kSlot);   // [2][warp][row of x][weight row]
   const int pairs = (chunks + 1) / 2;
-  const uint32_t xs = tc::smem_u32(smem) + kNarrowWarps * kDeep * kSlot + kNarrowSums<kN>, nothing = xs + a.m * pairs * 256;
-  const int c0 = pairs * warp / kNarrowWarps, slice = pairs * (warp + 1) / kNarrowWarps - c0;
-  const int groups = a.k >> group_shift, mine = (tiles - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+  const uint32_t xs = tc::smem_u32(smem) + kNarrowWarps * kDeep * kSlot + kNarrowSums<kR, kN>, nothing = xs + a.m * pairs * 256;
+  const int along = 1 << along_shift, at_once = kR * (kNarrowWarps >> along_shift), part = warp & (along - 1);
+  const int c0 = pairs * part >> along_shift, slice = (pairs * (part + 1) >> along_shift) - c0;
+  const int groups = a.k >> group_shift, tile0 = blockIdx.x * at_once + (warp >> along_shift) * kR, step = gridDim.x * at_once;   // this warp's tiles
+  const int rounds = (tiles - static_cast<int>(blockIdx.x) * at_once + step - 1) / step, mine = tile0 < tiles ? (tiles - tile0 + step - 1) / step : 0;
   ::mccl::pdl_wait();
   ::mccl::pdl_trigger();
 
@@ -104,25 +110,32 @@ __global__ void __launch_bounds__(kNarrowThreads) w4_narrow_kernel(W4Args a, int
   copy_commit();
 
   // ---- the loading side
-  int to_load = slice * mine, at = c0;
-  const uint4* codes = static_cast<const uint4*>(a.codes) + (static_cast<size_t>(blockIdx.x) * chunks + 2 * c0) * 32 + lane;
-  const uint2* params = static_cast<const uint2*>(a.params) + static_cast<size_t>(blockIdx.x) * groups * 8 + g;
-  const size_t codes_on = (static_cast<size_t>(gridDim.x) * chunks - 2 * slice) * 32, params_on = static_cast<size_t>(gridDim.x) * groups * 8;
+  int to_load = slice * mine, at = c0, load_tile = tile0;
+  const size_t tile_codes = static_cast<size_t>(chunks) * 32;
+  const uint4* codes = static_cast<const uint4*>(a.codes) + (static_cast<size_t>(tile0) * chunks + 2 * c0) * 32 + lane;
+  const uint2* params = static_cast<const uint2*>(a.params) + static_cast<size_t>(tile0) * groups * 8 + g;
+  const size_t codes_on = (static_cast<size_t>(step) * chunks - 2 * slice) * 32, params_on = static_cast<size_t>(step) * groups * 8;
   auto issue = [&](int slot) {
     if (to_load > 0) {
-      const uint32_t to = ring + slot * kSlot;
-      copy_async<16>(to + lane * 16, codes);
       const bool second = 2 * at + 1 < chunks;
-      copy_async<16>(to + 512 + lane * 16, second ? codes + 32 : codes, second);
 #pragma unroll
-      for (int i = 0; i < kParams; ++i) {
-        const int group = kParams == 1 ? at >> (group_shift - 7) : min(kParams * at + i, groups - 1);
-        copy_async<8>(to + 1024 + i * 256 + lane * 8, params + group * 8);
+      for (int r = 0; r < kR; ++r) {
+        const uint32_t to = ring + slot * kSlot + r * kTile;
+        const bool there = r == 0 || load_tile + r < tiles;
+        const uint4* from = there ? codes + r * tile_codes : codes;
+        copy_async<16>(to + lane * 16, from, there);
+        copy_async<16>(to + 512 + lane * 16, second ? from + 32 : from, second && there);
+#pragma unroll
+        for (int i = 0; i < kParams; ++i) {
+          const int group = kParams == 1 ? at >> (group_shift - 7) : min(kParams * at + i, groups - 1);
+          copy_async<8>(to + 1024 + i * 256 + lane * 8, params + ((there ? r * groups : 0) + group) * 8, there);
+        }
       }
       --to_load;
       codes += 64;
       if (++at == c0 + slice) {
         at = c0;
+        load_tile += step;
         codes += codes_on;
         params += params_on;
       }
@@ -144,24 +157,28 @@ __global__ void __launch_bounds__(kNarrowThreads) w4_narrow_kernel(W4Args a, int
     x_lane[n] = real ? xs + c0 * (a.m * 256) + (n * 8 + row) * 128 + (((lane >> 3) ^ row) << 4) : nothing;
   }
   int slot = 0;
-  for (int i = 0; i < mine; ++i) {
-    float total[kN][4] = {};
+  for (int i = 0; i < rounds; ++i) {
+    float total[kR][kN][4] = {};
     uint32_t x_at[kN];
 #pragma unroll
     for (int n = 0; n < kN; ++n) x_at[n] = x_lane[n];
-    for (int c = 0; c < slice; ++c) {
+    for (int c = i < mine ? slice : 0; c > 0; --c) {
       copy_wait<kDeep - 2>();
       const uint32_t from = ring + slot * kSlot;
-      const uint4 w[2] = {shared16(from + lane * 16), shared16(from + 512 + lane * 16)};
-      uint2 p[kParams];
+      uint4 w[kR][2];
+      uint2 p[kR][kParams];
 #pragma unroll
-      for (int j = 0; j < kParams; ++j) p[j] = shared8(from + 1024 + j * 256 + lane * 8);
+      for (int r = 0; r < kR; ++r) {
+        w[r][0] = shared16(from + r * kTile + lane * 16);
+        w[r][1] = shared16(from + r * kTile + 512 + lane * 16);
+#pragma unroll
+        for (int j = 0; j < kParams; ++j) p[r][j] = shared8(from + r * kTile + 1024 + j * 256 + lane * 8);
+      }
       issue(slot == 0 ? kDeep - 1 : slot - 1);
       slot = slot == kDeep - 1 ? 0 : slot + 1;
-      float acc[2][kN][4];
+      float acc[kR][2][kN][4];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const uint32_t word[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
         uint32_t b[kN][2][4];
 #pragma unroll
         for (int n = 0; n < kN; ++n) {
@@ -170,25 +187,30 @@ __global__ void __launch_bounds__(kNarrowThreads) w4_narrow_kernel(W4Args a, int
           x_at[n] += x_step[n];
         }
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          const uint2 q = p[kParams == 4 ? 2 * j + (s >> 1) : (kParams == 2 ? j : 0)];
-          const uint32_t z0 = zero2(q.x), z8 = zero2(q.y);
-          const uint32_t a0 = codes2(word[s], z0), a1 = codes2(word[s] >> 4, z8), a2 = codes2(word[s] >> 8, z0), a3 = codes2(word[s] >> 12, z8);
-          const bool begins = kParams == 4 ? (s & 1) == 0 : s == 0, ends = kParams == 4 ? (s & 1) == 1 : s == 3;
+        for (int r = 0; r < kR; ++r) {
+          const uint32_t word[4] = {w[r][j].x, w[r][j].y, w[r][j].z, w[r][j].w};
 #pragma unroll
-          for (int n = 0; n < kN; ++n) {
-            if (begins) acc[j][n][0] = acc[j][n][1] = acc[j][n][2] = acc[j][n][3] = 0.f;
-            mma16816(acc[j][n], a0, a1, a2, a3, b[n][s >> 1][(s & 1) * 2], b[n][s >> 1][(s & 1) * 2 + 1]);
-            if (ends && (kParams > 1 || j == 1)) {
-              if (kParams == 1) {
+          for (int s = 0; s < 4; ++s) {
+            const uint2 q = p[r][kParams == 4 ? 2 * j + (s >> 1) : (kParams == 2 ? j : 0)];
+            const uint32_t z0 = minus_zero2(q.x), z8 = minus_zero2(q.y);
+            const uint32_t a0 = codes2(word[s], z0), a1 = codes2(word[s] >> 4, z8), a2 = codes2(word[s] >> 8, z0), a3 = codes2(word[s] >> 12, z8);
+            const bool begins = kParams == 4 ? (s & 1) == 0 : s == 0, ends = kParams == 4 ? (s & 1) == 1 : s == 3;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[1][n][e] += acc[0][n][e];
+            for (int n = 0; n < kN; ++n) {
+              float (&c)[4] = acc[r][j][n];
+              if (begins) c[0] = c[1] = c[2] = c[3] = 0.f;
+              mma16816(c, a0, a1, a2, a3, b[n][s >> 1][(s & 1) * 2], b[n][s >> 1][(s & 1) * 2 + 1]);
+              if (ends && (kParams > 1 || j == 1)) {
+                if (kParams == 1) {
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) c[e] += acc[r][0][n][e];
+                }
+                const float s0 = scale_of(q.x), s8 = scale_of(q.y);
+                total[r][n][0] += s0 * c[0];
+                total[r][n][1] += s0 * c[1];
+                total[r][n][2] += s8 * c[2];
+                total[r][n][3] += s8 * c[3];
               }
-              const float s0 = scale_of(q.x), s8 = scale_of(q.y);
-              total[n][0] += s0 * acc[j][n][0];
-              total[n][1] += s0 * acc[j][n][1];
-              total[n][2] += s8 * acc[j][n][2];
-              total[n][3] += s8 * acc[j][n][3];
             }
           }
         }
@@ -196,18 +218,17 @@ __global__ void __launch_bounds__(kNarrowThreads) w4_narrow_kernel(W4Args a, int
     }
     float* to = sums + ((i & 1) * kNarrowWarps + warp) * kOut;
 #pragma unroll
-    for (int n = 0; n < kN; ++n)
+    for (int r = 0; r < kR; ++r)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) to[(n * 8 + 2 * t + (e & 1)) * 16 + g + 8 * (e >> 1)] = total[n][e];
+      for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) to[(n * 8 + 2 * t + (e & 1)) * (16 * kR) + r * 16 + g + 8 * (e >> 1)] = total[r][n][e];
     __syncthreads();
-    int out = threadIdx.x;
-    if (kN == 1) out -= (i & 1) * 128;   // the two halves of the block take turns
-    if (out >= 0 && out < kOut) {
-      const int m = out >> 4, n = (static_cast<int>(blockIdx.x) + i * static_cast<int>(gridDim.x)) * 16 + (out & 15);
+    for (int o = threadIdx.x; o < (kNarrowWarps >> along_shift) * kOut; o += kNarrowThreads) {
+      const int which = o / kOut, out = o % kOut, m = out / (16 * kR), n = (static_cast<int>(blockIdx.x) * at_once + i * step + which * kR) * 16 + out % (16 * kR);
       if (m < a.m && n < a.n) {
         float v = 0.f;
-#pragma unroll
-        for (int w = 0; w < kNarrowWarps; ++w) v += sums[((i & 1) * kNarrowWarps + w) * kOut + out];
+        for (int w = 0; w < along; ++w) v += sums[((i & 1) * kNarrowWarps + which * along + w) * kOut + out];
         static_cast<__nv_bfloat16*>(a.y)[static_cast<long long>(m) * a.n + n] = __float2bfloat16_rn(finished(a, v, m, n));
       }
     }
@@ -389,10 +410,10 @@ __global__ void __launch_bounds__(kWideThreads, 2) w4_wide_kernel(const __grid_c
 #pragma unroll
         for (int step = 0; step < 4; ++step) {
           const uint2 q = prm[k][kG32 ? step >> 1 : 0];
-          r[4 * step] = mul2(codes2(word[step], zero2(q.x)), scale2(q.x));
-          r[4 * step + 1] = mul2(codes2(word[step] >> 4, zero2(q.y)), scale2(q.y));
-          r[4 * step + 2] = mul2(codes2(word[step] >> 8, zero2(q.x)), scale2(q.x));
-          r[4 * step + 3] = mul2(codes2(word[step] >> 12, zero2(q.y)), scale2(q.y));
+          r[4 * step] = mul2(codes2(word[step], minus_zero2(q.x)), scale2(q.x));
+          r[4 * step + 1] = mul2(codes2(word[step] >> 4, minus_zero2(q.y)), scale2(q.y));
+          r[4 * step + 2] = mul2(codes2(word[step] >> 8, minus_zero2(q.x)), scale2(q.x));
+          r[4 * step + 3] = mul2(codes2(word[step] >> 12, minus_zero2(q.y)), scale2(q.y));
         }
         tmem_st_16x64(tmem + (static_cast<uint32_t>(quarter * 32 + k * 16) << 16) + p.columns + s * 32, r);
       }
@@ -484,7 +505,7 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(const uint4* __restr
       for (int j = 0; j < 4; ++j) {   // nibble j: row g + 8 (j & 1), columns 8 (j >> 1) on
         const int row = tile * 16 + (j & 1) * 8 + g;
         const uint32_t prm = j & 1 ? p.y : p.x;
-        if (row < n) *reinterpret_cast<uint32_t*>(w + static_cast<size_t>(row) * k + at + (j >> 1) * 8) = mul2(codes2(word[s] >> (4 * j), zero2(prm)), scale2(prm));
+        if (row < n) *reinterpret_cast<uint32_t*>(w + static_cast<size_t>(row) * k + at + (j >> 1) * 8) = mul2(codes2(word[s] >> (4 * j), minus_zero2(prm)), scale2(prm));
       }
     }
   }
@@ -505,19 +526,24 @@ int log2_of(int v) {
   return s;
 }
 
-template <int kN, int kParams>
+template <int kR, int kN, int kParams>
 cudaError_t launch_narrow(const W4Args& a, cudaStream_t stream) {
-  static const cudaError_t rc = cudaFuncSetAttribute(w4_narrow_kernel<kN, kParams>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+  static const cudaError_t rc = cudaFuncSetAttribute(w4_narrow_kernel<kR, kN, kParams>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
   if (rc != cudaSuccess) return rc;
-  const int chunks = (a.k + 63) / 64, smem = narrow_smem<kN, kParams>(a.m, (chunks + 1) / 2);
-  const int tiles = (a.n + 15) / 16, blocks = sm_count() * (smem <= 113 * 1024 ? 2 : 1);
-  MCCL_LAUNCH_PDL((w4_narrow_kernel<kN, kParams>), tiles < blocks ? tiles : blocks, kNarrowThreads, smem, stream, a, tiles, chunks, log2_of(a.group));
+  const int chunks = (a.k + 63) / 64, smem = narrow_smem<kR, kN, kParams>(a.m, (chunks + 1) / 2);
+  if (smem > 227 * 1024) return cudaErrorNotSupported;
+  const int tiles = ((a.n + 15) / 16 + kR - 1) / kR, blocks = sm_count() * (smem <= 113 * 1024 ? 2 : 1);
+  // as few warps along K as give every warp a tile: adding up costs a barrier and a pass through shared memory
+  int along = 3;
+  while (along > 0 && tiles << (along - 1) >= blocks * kNarrowWarps * 3 / 4) --along;
+  const int groups = (tiles + (kNarrowWarps >> along) - 1) / (kNarrowWarps >> along);
+  MCCL_LAUNCH_PDL((w4_narrow_kernel<kR, kN, kParams>), groups < blocks ? groups : blocks, kNarrowThreads, smem, stream, a, (a.n + 15) / 16, chunks, log2_of(a.group), along);
   count_launch();
   return ::mccl::launch_status();
 }
-template <int kN>
+template <int kR, int kN>
 cudaError_t narrow(const W4Args& a, cudaStream_t stream) {
-  return a.group == 32 ? launch_narrow<kN, 4>(a, stream) : (a.group == 64 ? launch_narrow<kN, 2>(a, stream) : launch_narrow<kN, 1>(a, stream));
+  return a.group == 32 ? launch_narrow<kR, kN, 4>(a, stream) : (a.group == 64 ? launch_narrow<kR, kN, 2>(a, stream) : launch_narrow<kR, kN, 1>(a, stream));
 }
 
 template <bool kG32>
@@ -558,7 +584,11 @@ cudaError_t launch_wide(const W4Args& a, cudaStream_t stream) {
 cudaError_t w4_linear(const W4Args& a, cudaStream_t stream) {
   if (a.m <= 0 || a.n <= 0) return cudaSuccess;
   const long long x_bytes = static_cast<long long>(a.m) * ((a.k + 127) / 128) * 256;
-  if (a.m <= 16 && x_bytes <= 128 * 1024) return a.m <= 8 ? narrow<1>(a, stream) : narrow<2>(a, stream);
+  if (a.m <= 16 && x_bytes <= 128 * 1024) {
+    const bool two = a.n >= 16 * 3 * sm_count();
+    if (a.m <= 8) return two ? narrow<2, 1>(a, stream) : narrow<1, 1>(a, stream);
+    return narrow<1, 2>(a, stream);
+  }
   return a.group == 32 ? launch_wide<true>(a, stream) : launch_wide<false>(a, stream);
 }
 
