@@ -5,6 +5,8 @@
 // the wide kernel makes bf16 weights on the way into tensor memory, where they are the left operand of tcgen05 products.
 #include <cuda.h>
 
+#include <array>
+
 #include "../core/launch.hpp"
 #include "bf16x8.cuh"
 #include "gemm_common.cuh"
@@ -238,18 +240,26 @@ __global__ void __launch_bounds__(kNarrowThreads, 2) w4_narrow_kernel(W4Args a, 
 
 // --------------------------------------------------------------- more rows of x --
 constexpr int kWideRows = 128;             // weight rows of a block: the lanes of tensor memory
-constexpr int kWideThreads = 10 * 32;      // warp 0 brings x, warp 1 issues the products, eight make weights and write results
+// Warp 0 brings x, warp 1 issues the products, four times kTurns make weights (they take chunks in turn) and write results: a warp of eight needs 1400 clocks
+// for its half of a chunk, most of them latency, so where a block has an SM for itself sixteen do it.
+template <int kTurns>
+constexpr int kWideThreads = (2 + 4 * kTurns) * 32;
 constexpr int kWideStages = 4;
-constexpr int kCodeDeep = 4;               // chunks that a weight-making warp has on their way
-constexpr int kCodeRing = 8 * kCodeDeep * 2 * 512;
-constexpr int kMostTokens = 128;           // rows of x of a block; twice 256 columns of tensor memory (sums 128, weights 4 x 32) are two blocks per SM
+// Chunks that a weight-making warp has on their way.  (Three of them, 32 KB per SM, held 64 rows of x to 2 TB/s.)
+template <int kTurns>
+constexpr int kCodeDeep = kTurns == 2 ? 5 : 6;
+template <int kTurns>
+constexpr int kCodeRing = 4 * kTurns * kCodeDeep<kTurns> * 2 * 512;
+constexpr int kWideSmem = 226 * 1024, kWideSmemOfTwo = 112 * 1024;   // of a block; the rest is for the barriers and what the system takes
+constexpr int kMostTokens = 256;           // rows of x of a block
 
 struct Wide {
   W4Args a;
   int tokens, chunks, group_shift;   // rows of x per block, a multiple of 16; chunks of 64 columns in K
   int columns;          // of tensor memory that the sums take; the weights' ring lies behind them
-  int allocated;
-  int splits;           // blocks of a cluster that share out K
+  int allocated, turns;
+  int splits, share;    // blocks of a cluster that share out K, and rows of x whose sums each of them finishes
+  int vector;           // y and residual can be accessed four elements at a time
   uint32_t idesc;
   int* err;
 };
@@ -276,26 +286,24 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t at, uint32_t (&r)[16]) {
                : "r"(at)
                : "memory");
 }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float4 peer_float4(uint32_t at, int rank) {
+// A store to the same place of shared memory in block `rank` of the cluster.
+__device__ __forceinline__ void store_peer(uint32_t at, int rank, float v) {
   uint32_t there;
-  float4 v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(there) : "memory");
-  return v;
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there), "f"(v) : "memory");
 }
 
 // Block (x, y, z): weight rows 128 x and on, rows of x from `tokens` y on, part z of K.  D[weight row, row of x] = W x^T: the weights of a chunk of 64
 // columns go from a lane's 16 bytes through registers into tensor memory (the lanes of an m16n8k16 A fragment are those of a 16x128b store), x comes
 // by TMA.  The weights are rounded to bf16 once, scale times whole number, as a stored bf16 weight would be.
-template <bool kG32>
-__global__ void __launch_bounds__(kWideThreads, 2) w4_wide_kernel(const __grid_constant__ CUtensorMap x_map, Wide p) {
+// Results go through shared memory so that a row of y leaves in one piece; with K shared out every block of the cluster finishes `share` rows of x, whose
+// sums the others store into it, and adds them in the order of the parts.
+template <int kTurns, bool kG32>
+__global__ void __launch_bounds__(kWideThreads<kTurns>, kTurns == 2 ? 2 : 1) w4_wide_kernel(const __grid_constant__ CUtensorMap x_map, Wide p) {
+  constexpr int kCodeDeep = ops::kCodeDeep<kTurns>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024 - (tc::smem_u32(smem_raw) & 1023)) & 1023);
-  __shared__ uint64_t x_full[kWideStages], w_full[kWideStages], empty[kWideStages], done;
+  __shared__ uint64_t full[kWideStages], empty[kWideStages], done;
   __shared__ uint32_t tmem_slot;
   __shared__ int bad;
   const W4Args& a = p.a;
@@ -304,8 +312,7 @@ __global__ void __launch_bounds__(kWideThreads, 2) w4_wide_kernel(const __grid_c
   const int stage_bytes = p.tokens * 128;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kWideStages; ++i) {
-      tc::mbar_init(x_full + i, 1);
-      tc::mbar_init(w_full + i, 4);
+      tc::mbar_init(full + i, 5);   // x's bytes and their announcement, and the weights of each 32 rows
       tc::mbar_init(empty + i, 1);
     }
     tc::mbar_init(&done, 1);
@@ -319,48 +326,48 @@ __global__ void __launch_bounds__(kWideThreads, 2) w4_wide_kernel(const __grid_c
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = tmem_slot;
+  if (p.splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // this block has started: its memory may be written
   ::mccl::pdl_wait();
   ::mccl::pdl_trigger();
 
   if (warp == 0) {   // ---- x
     if (tc::elect_one()) {
-      int c = first;
+      int c = first, s = 0, round = 0;
       for (; c < last; ++c) {
-        const int i = c - first, s = i % kWideStages;
-        if (i >= kWideStages && !tc::mbar_wait(empty + s, ((i / kWideStages) - 1) & 1)) {
+        if (round > 0 && !tc::mbar_wait(empty + s, (round - 1) & 1)) {
           bad = 1;
           break;
         }
-        tc::mbar_expect_tx(x_full + s, stage_bytes);
-        tc::tma_load_2d(smem + s * stage_bytes, &x_map, x_full + s, c * 64, blockIdx.y * p.tokens);
+        tc::mbar_expect_tx(full + s, stage_bytes);
+        tc::tma_load_2d(smem + s * stage_bytes, &x_map, full + s, c * 64, blockIdx.y * p.tokens);
+        if (++s == kWideStages) s = 0, ++round;
       }
       if (bad)   // what was issued must land before the block retires
-        for (int i = max(c - first - kWideStages, 0); i < c - first; ++i) tc::mbar_wait(x_full + i % kWideStages, (i / kWideStages) & 1, 1u << 20);
+        for (int i = max(c - first - kWideStages, 0); i < c - first; ++i) tc::mbar_wait(full + i % kWideStages, (i / kWideStages) & 1, 1u << 20);
     }
     __syncwarp();
   } else if (warp == 1) {   // ---- products
-    for (int c = first; c < last; ++c) {
-      const int i = c - first, s = i % kWideStages;
-      bool ok = tc::mbar_wait(x_full + s, (i / kWideStages) & 1);
-      ok = tc::mbar_wait(w_full + s, (i / kWideStages) & 1) && ok;
-      ok = __all_sync(0xffffffffu, ok);
-      tc::fence_after_sync();
-      if (tc::elect_one()) {
-        if (ok) {
-          const uint64_t db = tc::smem_desc_k_sw128(smem + s * stage_bytes);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) mma_ts(tmem, tmem + p.columns + s * 32 + k * 8, db + 2 * k, p.idesc, i > 0 || k > 0);
-          tc::mma_commit(empty + s);
-        } else {
+    // One thread from wait to commit: with the warp voting on every wait a chunk took 450 clocks at any number of rows of x.
+    if (tc::elect_one()) {
+      const uint64_t desc = tc::smem_desc_k_sw128(smem);
+      uint32_t weights = tmem + p.columns;
+      int s = 0, parity = 0;
+      for (int c = first; c < last; ++c) {
+        if (!tc::mbar_wait(full + s, parity)) {
           bad = 1;
+          break;
         }
+        tc::fence_after_sync();
+        const uint64_t db = desc + static_cast<uint32_t>(s * stage_bytes >> 4);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mma_ts(tmem, weights + s * 32 + k * 8, db + 2 * k, p.idesc, c > first || k > 0);
+        tc::mma_commit(empty + s);
+        if (++s == kWideStages) s = 0, parity ^= 1;
       }
-      __syncwarp();
-      if (!ok) break;
+      tc::mma_commit(&done);   // also after a failure: it releases the waiters
     }
-    if (tc::elect_one()) tc::mma_commit(&done);   // also after a failure: it releases the waiters
     __syncwarp();
-  } else {   // ---- weights: two warps for each 32 rows take chunks in turn
+  } else {   // ---- weights: kTurns warps for each 32 rows take chunks in turn
     const int quarter = warp & 3, turn = (warp - 2) >> 2, g = lane >> 2;
     const int row_tiles = (a.n + 15) / 16, groups = a.k >> p.group_shift, tile0 = blockIdx.x * (kWideRows / 16) + quarter * 2;
     const uint32_t ring = tc::smem_u32(smem) + kWideStages * stage_bytes + (warp - 2) * (kCodeDeep * 2 * 512) + lane * 16;
@@ -384,19 +391,34 @@ __global__ void __launch_bounds__(kWideThreads, 2) w4_wide_kernel(const __grid_c
         }
     };
 #pragma unroll
-    for (int i = 0; i < kCodeDeep - 1; ++i) issue(first + turn + 2 * i, i);
+    for (int i = 0; i < kCodeDeep - 1; ++i) issue(first + turn + kTurns * i, i);
     parameters(first + turn, prm);
     int slot = 0;
-    for (int c = first + turn; c < last; c += 2) {
+    for (int c = first + turn; c < last; c += kTurns) {
       const int i = c - first, s = i % kWideStages;
       copy_wait<kCodeDeep - 2>();
       uint4 w[2];
 #pragma unroll
       for (int k = 0; k < 2; ++k) w[k] = shared16(ring + (slot * 2 + k) * 512);
-      issue(c + 2 * (kCodeDeep - 1), slot == 0 ? kCodeDeep - 1 : slot - 1);
+      issue(c + kTurns * (kCodeDeep - 1), slot == 0 ? kCodeDeep - 1 : slot - 1);
       slot = slot == kCodeDeep - 1 ? 0 : slot + 1;
       uint2 next[2][2];
-      parameters(c + 2, next);
+      parameters(c + kTurns, next);
+      // the weights are ready in registers before their place in tensor memory is awaited: making them is not part of the loop from one use of a
+      // place to the next (490 clocks per chunk when it was, at any number of rows of x)
+      uint32_t r[2][16];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t word[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+#pragma unroll
+        for (int step = 0; step < 4; ++step) {
+          const uint2 q = prm[k][kG32 ? step >> 1 : 0];
+          r[k][4 * step] = mul2(codes2(word[step], minus_zero2(q.x)), scale2(q.x));
+          r[k][4 * step + 1] = mul2(codes2(word[step] >> 4, minus_zero2(q.y)), scale2(q.y));
+          r[k][4 * step + 2] = mul2(codes2(word[step] >> 8, minus_zero2(q.x)), scale2(q.x));
+          r[k][4 * step + 3] = mul2(codes2(word[step] >> 12, minus_zero2(q.y)), scale2(q.y));
+        }
+      }
       const bool ok = __all_sync(0xffffffffu, i < kWideStages || tc::mbar_wait(empty + s, ((i / kWideStages) - 1) & 1));
       if (!ok) {
         if (lane == 0) bad = 1;
@@ -404,23 +426,11 @@ __global__ void __launch_bounds__(kWideThreads, 2) w4_wide_kernel(const __grid_c
       }
       tc::fence_after_sync();
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const uint32_t word[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
-        uint32_t r[16];
-#pragma unroll
-        for (int step = 0; step < 4; ++step) {
-          const uint2 q = prm[k][kG32 ? step >> 1 : 0];
-          r[4 * step] = mul2(codes2(word[step], minus_zero2(q.x)), scale2(q.x));
-          r[4 * step + 1] = mul2(codes2(word[step] >> 4, minus_zero2(q.y)), scale2(q.y));
-          r[4 * step + 2] = mul2(codes2(word[step] >> 8, minus_zero2(q.x)), scale2(q.x));
-          r[4 * step + 3] = mul2(codes2(word[step] >> 12, minus_zero2(q.y)), scale2(q.y));
-        }
-        tmem_st_16x64(tmem + (static_cast<uint32_t>(quarter * 32 + k * 16) << 16) + p.columns + s * 32, r);
-      }
+      for (int k = 0; k < 2; ++k) tmem_st_16x64(tmem + (static_cast<uint32_t>(quarter * 32 + k * 16) << 16) + p.columns + s * 32, r[k]);
       tmem_st_wait();
       tc::fence_before_sync();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(w_full + s);
+      if (lane == 0) tc::mbar_arrive(full + s);
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -431,49 +441,76 @@ __global__ void __launch_bounds__(kWideThreads, 2) w4_wide_kernel(const __grid_c
 
   // ---- results
   __syncwarp();
+  const int n4 = blockIdx.x * kWideRows + lane * 4, token0 = blockIdx.y * p.tokens;
+  float bias[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) bias[e] = a.bias && n4 + e < a.n ? __ldg(a.bias + n4 + e) : 0.f;
   const bool ok = tc::mbar_wait(&done, 0);
   tc::fence_after_sync();
-  float* sums = reinterpret_cast<float*>(smem);   // [row of x][weight row], where x was
-  const int token0 = blockIdx.y * p.tokens;
+  __syncwarp();
+  // [part][row of x][weight row]: where x was, or behind everything else where other blocks write too
+  float* sums = reinterpret_cast<float*>(smem + (p.splits > 1 ? kWideStages * stage_bytes + kCodeRing<kTurns> : 0));
+  if (p.splits > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (warp >= 2 && ok) {
-    const int quarter = warp & 3, turn = (warp - 2) >> 2, row = quarter * 32 + lane, n = blockIdx.x * kWideRows + row;
-    for (int c = turn; c < p.tokens / 16; c += 2) {
+    const int quarter = warp & 3, turn = (warp - 2) >> 2, row = quarter * 32 + lane;
+    for (int c = turn; c < p.tokens / 16; c += kTurns) {
       uint32_t r[16];
       tmem_ld_32x16(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + c * 16, r);
       tc::tmem_ld_wait();
       if (p.splits > 1) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sums[(c * 16 + i) * kWideRows + row] = __uint_as_float(r[i]);
-      } else if (n < a.n) {
+        int owner = c * 16 / p.share, at = c * 16 - owner * p.share;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int m = token0 + c * 16 + i;
-          if (m < a.m) static_cast<__nv_bfloat16*>(a.y)[static_cast<long long>(m) * a.n + n] = __float2bfloat16_rn(finished(a, __uint_as_float(r[i]), m, n));
+          store_peer(tc::smem_u32(sums + (static_cast<int>(blockIdx.z) * p.share + at) * kWideRows + row), owner, __uint_as_float(r[i]));
+          if (++at == p.share) {
+            at = 0;
+            ++owner;
+          }
         }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sums[(c * 16 + i) * kWideRows + row] = __uint_as_float(r[i]);
       }
     }
   }
   __syncwarp();
   if (p.splits > 1) {
-    cluster_sync();
-    const int from = p.tokens * static_cast<int>(blockIdx.z) / p.splits, to = p.tokens * (static_cast<int>(blockIdx.z) + 1) / p.splits;
-    for (int i = from * 32 + threadIdx.x; i < to * 32; i += kWideThreads) {
-      const int m = token0 + (i >> 5), n = blockIdx.x * kWideRows + (i & 31) * 4;
-      if (m >= a.m) break;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int r = 0; r < p.splits; ++r) {
-        const float4 o = peer_float4(tc::smem_u32(sums + i * 4), r);
-        v.x += o.x;
-        v.y += o.y;
-        v.z += o.z;
-        v.w += o.w;
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  } else {
+    __syncthreads();
+  }
+  const int from = p.splits > 1 ? static_cast<int>(blockIdx.z) * p.share : 0, rows = min(min(p.share, p.tokens - from), a.m - token0 - from);
+  for (int i = warp; i < rows; i += kWideThreads<kTurns> / 32) {
+    const int m = token0 + from + i;
+    float4 v = *reinterpret_cast<const float4*>(sums + i * kWideRows + lane * 4);
+    for (int r = 1; r < p.splits; ++r) {
+      const float4 o = *reinterpret_cast<const float4*>(sums + (r * p.share + i) * kWideRows + lane * 4);
+      v.x += o.x;
+      v.y += o.y;
+      v.z += o.z;
+      v.w += o.w;
+    }
+    float f[4] = {v.x + bias[0], v.y + bias[1], v.z + bias[2], v.w + bias[3]};
+    if (a.gelu) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = 0.5f * f[e] * (1.f + erff(f[e] * 0.70710678118654752f));
+    }
+    __nv_bfloat16* y = static_cast<__nv_bfloat16*>(a.y) + static_cast<long long>(m) * a.n + n4;
+    const __nv_bfloat16* residual = static_cast<const __nv_bfloat16*>(a.residual) + (a.residual ? m * a.ldr + n4 : 0);
+    if (p.vector && n4 + 3 < a.n) {
+      if (a.residual) {
+        const uint2 raw = __ldg(reinterpret_cast<const uint2*>(residual));
+        const float2 lo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.x)), hi = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.y));
+        f[0] += lo.x, f[1] += lo.y, f[2] += hi.x, f[3] += hi.y;
       }
-      const float f[4] = {v.x, v.y, v.z, v.w};
+      __nv_bfloat162 out[2] = {__floats2bfloat162_rn(f[0], f[1]), __floats2bfloat162_rn(f[2], f[3])};
+      *reinterpret_cast<uint2*>(y) = *reinterpret_cast<const uint2*>(out);
+    } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (n + e < a.n) static_cast<__nv_bfloat16*>(a.y)[static_cast<long long>(m) * a.n + n + e] = __float2bfloat16_rn(finished(a, f[e], m, n + e));
+        if (n4 + e < a.n) y[e] = __float2bfloat16_rn(f[e] + (a.residual ? __bfloat162float(residual[e]) : 0.f));
     }
-    cluster_sync();   // nobody leaves while its sums may be read
   }
   if ((!ok || bad) && threadIdx.x == 0) atomicExch(p.err, 22);
   tc::fence_before_sync();
@@ -546,22 +583,87 @@ cudaError_t narrow(const W4Args& a, cudaStream_t stream) {
   return a.group == 32 ? launch_narrow<kR, kN, 4>(a, stream) : (a.group == 64 ? launch_narrow<kR, kN, 2>(a, stream) : launch_narrow<kR, kN, 1>(a, stream));
 }
 
-template <bool kG32>
-cudaError_t launch_wide(const W4Args& a, cudaStream_t stream) {
-  static const cudaError_t rc = cudaFuncSetAttribute(w4_wide_kernel<kG32>, cudaFuncAttributeMaxDynamicSharedMemorySize, 113 * 1024);
+int wide_smem(const Wide& p) { return kWideStages * p.tokens * 128 + (p.turns == 2 ? kCodeRing<2> : kCodeRing<4>) + (p.splits > 1 ? p.splits * p.share * kWideRows * 4 : 0) + 1024; }
+
+// Blocks that the GPU holds at a time, in clusters of `splits`: a cluster lies in one group of SMs, and what is left over in each group stays idle.
+int resident(int turns, int splits) {
+  static const std::array<std::array<int, 9>, 2> counts = [] {
+    std::array<std::array<int, 9>, 2> c = {};
+    for (int t = 0; t < 2; ++t) {
+      const int per_sm = t == 0 ? 2 : 1;
+      for (int n = 1; n <= 8; ++n) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(1, 1, n);
+        cfg.blockDim = dim3(t == 0 ? kWideThreads<2> : kWideThreads<4>);
+        cfg.dynamicSmemBytes = per_sm == 2 ? kWideSmemOfTwo : kWideSmem;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = n;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int clusters = 0;
+        cudaError_t rc = cudaFuncSetAttribute(t == 0 ? w4_wide_kernel<2, false> : w4_wide_kernel<4, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem);
+        if (rc == cudaSuccess)
+          rc = t == 0 ? cudaOccupancyMaxActiveClusters(&clusters, w4_wide_kernel<2, false>, &cfg) : cudaOccupancyMaxActiveClusters(&clusters, w4_wide_kernel<4, false>, &cfg);
+        if (rc != cudaSuccess) cudaGetLastError();
+        c[t][n] = rc == cudaSuccess && clusters > 0 ? clusters * n : sm_count() * per_sm * 3 / 4;
+      }
+    }
+    return c;
+  }();
+  return counts[turns == 2 ? 0 : 1][splits];
+}
+
+// Rows of x per block, parts of K, and whether two blocks share an SM.  A chunk of 64 columns costs an SM the making of its weights (some kMake clocks per
+// block) or its products (two clocks per row of x), a block some 5000 clocks before its first and after its last chunk.
+void choose_wide(int m, int blocks, Wide& p) {
+  constexpr double kMake = 300, kRound = 5000, kSplit = 1500, kToken = 20;
+  double best = 0;
+  Wide w = p;
+  for (int most = 32; most <= kMostTokens; most += 32) {
+    const int tiles = (m + most - 1) / most;
+    w.tokens = ((m + tiles - 1) / tiles + 15) / 16 * 16;
+    for (w.splits = 1; w.splits <= 8 && (w.splits == 1 || w.splits * 2 <= p.chunks); ++w.splits) {
+      w.share = (w.tokens + w.splits - 1) / w.splits;
+      for (w.turns = 2; w.turns <= 4; w.turns += 2) {
+        const int per_sm = w.turns == 2 ? 2 : 1;
+        if (wide_smem(w) > (per_sm == 2 ? kWideSmemOfTwo : kWideSmem) || (per_sm == 2 && w.tokens > 128)) continue;
+        const int all = blocks * ((m + w.tokens - 1) / w.tokens) * w.splits, at_once = resident(w.turns, w.splits), waves = (all + at_once - 1) / at_once;
+        const bool alone = all <= at_once / per_sm;   // no two blocks on an SM
+        const double make = alone && per_sm == 2 ? 1.5 * kMake : per_sm * kMake, products = (alone ? 1 : per_sm) * 2.0 * w.tokens;
+        const double cost = waves * ((p.chunks + w.splits - 1) / w.splits * (make > products ? make : products) + kRound + (w.splits > 1 ? kSplit : 0.0) + kToken * w.tokens);
+        if (best == 0 || cost < best) {
+          best = cost;
+          p.tokens = w.tokens;
+          p.splits = w.splits;
+          p.share = w.share;
+          p.turns = w.turns;
+        }
+      }
+    }
+  }
+}
+
+template <int kTurns, bool kG32>
+cudaError_t start_wide(const Wide& p, dim3 grid, const CUtensorMap& map, cudaStream_t stream) {
+  static const cudaError_t rc = cudaFuncSetAttribute(w4_wide_kernel<kTurns, kG32>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem);
   if (rc != cudaSuccess) return rc;
+  MCCL_LAUNCH_PDL_CLUSTER((w4_wide_kernel<kTurns, kG32>), grid, kWideThreads<kTurns>, wide_smem(p), stream, static_cast<unsigned>(p.splits), map, p);
+  count_launch();
+  return ::mccl::launch_status();
+}
+
+cudaError_t launch_wide(const W4Args& a, cudaStream_t stream) {
   Wide p;
   p.a = a;
   p.chunks = (a.k + 63) / 64;
   p.group_shift = log2_of(a.group);
-  const int tiles = (a.m + kMostTokens - 1) / kMostTokens, blocks = (a.n + kWideRows - 1) / kWideRows;
-  p.tokens = ((a.m + tiles - 1) / tiles + 15) / 16 * 16;
-  p.columns = p.tokens <= 32 ? 32 : (p.tokens <= 64 ? 64 : 128);
+  const int blocks = (a.n + kWideRows - 1) / kWideRows;
+  choose_wide(a.m, blocks, p);
+  p.columns = p.tokens <= 32 ? 32 : (p.tokens <= 64 ? 64 : (p.tokens <= 128 ? 128 : 256));
   p.allocated = p.columns + kWideStages * 32 <= 256 ? 256 : 512;
-  // parts of K: as many as fill two blocks per SM, of four chunks at least, for a cluster has to add them up
-  int splits = 2 * sm_count() / (blocks * ((a.m + p.tokens - 1) / p.tokens));
-  if (splits > p.chunks / 4) splits = p.chunks / 4;
-  p.splits = splits < 1 ? 1 : (splits > 8 ? 8 : splits);
+  p.vector = a.n % 4 == 0 && (a.residual == nullptr || (a.ldr % 4 == 0 && reinterpret_cast<uintptr_t>(a.residual) % 8 == 0));
   p.idesc = tc::idesc_bf16(kWideRows, p.tokens);
   p.err = gemm_error_device_ptr();
   const CuDriver& cu = CuDriver::get();
@@ -573,10 +675,8 @@ cudaError_t launch_wide(const W4Args& a, cudaStream_t stream) {
                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return cudaErrorNotSupported;
   const dim3 grid(blocks, (a.m + p.tokens - 1) / p.tokens, p.splits);
-  const int smem = kWideStages * p.tokens * 128 + kCodeRing + 1024;
-  MCCL_LAUNCH_PDL_CLUSTER(w4_wide_kernel<kG32>, grid, kWideThreads, smem, stream, static_cast<unsigned>(p.splits), map, p);
-  count_launch();
-  return ::mccl::launch_status();
+  if (p.turns == 2) return a.group == 32 ? start_wide<2, true>(p, grid, map, stream) : start_wide<2, false>(p, grid, map, stream);
+  return a.group == 32 ? start_wide<4, true>(p, grid, map, stream) : start_wide<4, false>(p, grid, map, stream);
 }
 
 }  // namespace
@@ -589,7 +689,7 @@ cudaError_t w4_linear(const W4Args& a, cudaStream_t stream) {
     if (a.m <= 8) return two ? narrow<2, 1>(a, stream) : narrow<1, 1>(a, stream);
     return narrow<1, 2>(a, stream);
   }
-  return a.group == 32 ? launch_wide<true>(a, stream) : launch_wide<false>(a, stream);
+  return launch_wide(a, stream);
 }
 
 cudaError_t w4_dequantize(const void* codes, const void* params, void* w, int n, int k, int group, cudaStream_t stream) {
