@@ -240,24 +240,21 @@ __global__ void __launch_bounds__(kNarrowThreads, 2) w4_narrow_kernel(W4Args a, 
 
 // --------------------------------------------------------------- more rows of x --
 constexpr int kWideRows = 128;             // weight rows of a block: the lanes of tensor memory
-// Warp 0 brings x, warp 1 issues the products, four times kTurns make weights (they take chunks in turn) and write results: a warp of eight needs 1400 clocks
-// for its half of a chunk, most of them latency, so where a block has an SM for itself sixteen do it.
-template <int kTurns>
+// Warp 0 brings x, warp 1 issues the products, sixteen make weights and write results.  Four warps share a chunk (32 weight rows each) and take
+// chunks in turn with three other fours: a warp needs some 600 clocks for its part, most of them latency.
+constexpr int kTurns = 4;
 constexpr int kWideThreads = (2 + 4 * kTurns) * 32;
 constexpr int kWideStages = 4;
-// Chunks that a weight-making warp has on their way.  (Three of them, 32 KB per SM, held 64 rows of x to 2 TB/s.)
-template <int kTurns>
-constexpr int kCodeDeep = kTurns == 2 ? 5 : 6;
-template <int kTurns>
-constexpr int kCodeRing = 4 * kTurns * kCodeDeep<kTurns> * 2 * 512;
-constexpr int kWideSmem = 226 * 1024, kWideSmemOfTwo = 112 * 1024;   // of a block; the rest is for the barriers and what the system takes
+constexpr int kCodeDeep = 6;               // chunks that a weight-making warp has on their way
+constexpr int kCodeRing = 4 * kTurns * kCodeDeep * 2 * 512;
+constexpr int kWideSmem = 226 * 1024;      // the rest is for the barriers
 constexpr int kMostTokens = 256;           // rows of x of a block
 
 struct Wide {
   W4Args a;
   int tokens, chunks, group_shift;   // rows of x per block, a multiple of 16; chunks of 64 columns in K
   int columns;          // of tensor memory that the sums take; the weights' ring lies behind them
-  int allocated, turns;
+  int allocated;
   int splits, share;    // blocks of a cluster that share out K, and rows of x whose sums each of them finishes
   int vector;           // y and residual can be accessed four elements at a time
   uint32_t idesc;
@@ -298,9 +295,8 @@ __device__ __forceinline__ void store_peer(uint32_t at, int rank, float v) {
 // by TMA.  The weights are rounded to bf16 once, scale times whole number, as a stored bf16 weight would be.
 // Results go through shared memory so that a row of y leaves in one piece; with K shared out every block of the cluster finishes `share` rows of x, whose
 // sums the others store into it, and adds them in the order of the parts.
-template <int kTurns, bool kG32>
-__global__ void __launch_bounds__(kWideThreads<kTurns>, kTurns == 2 ? 2 : 1) w4_wide_kernel(const __grid_constant__ CUtensorMap x_map, Wide p) {
-  constexpr int kCodeDeep = ops::kCodeDeep<kTurns>;
+template <bool kG32>
+__global__ void __launch_bounds__(kWideThreads, 1) w4_wide_kernel(const __grid_constant__ CUtensorMap x_map, Wide p) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024 - (tc::smem_u32(smem_raw) & 1023)) & 1023);
   __shared__ uint64_t full[kWideStages], empty[kWideStages], done;
@@ -349,20 +345,29 @@ __global__ void __launch_bounds__(kWideThreads<kTurns>, kTurns == 2 ? 2 : 1) w4_
   } else if (warp == 1) {   // ---- products
     // One thread from wait to commit: with the warp voting on every wait a chunk took 450 clocks at any number of rows of x.
     if (tc::elect_one()) {
-      const uint64_t desc = tc::smem_desc_k_sw128(smem);
-      uint32_t weights = tmem + p.columns;
-      int s = 0, parity = 0;
-      for (int c = first; c < last; ++c) {
-        if (!tc::mbar_wait(full + s, parity)) {
-          bad = 1;
-          break;
-        }
-        tc::fence_after_sync();
-        const uint64_t db = desc + static_cast<uint32_t>(s * stage_bytes >> 4);
+      const uint64_t desc = tc::smem_desc_k_sw128(smem), stage_step = static_cast<uint64_t>(stage_bytes >> 4);
+      const uint32_t weights = tmem + p.columns;
+      uint32_t parity = 0;
+      for (int c = first; c < last && !bad; parity ^= 1) {
+        uint64_t db = desc;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mma_ts(tmem, weights + s * 32 + k * 8, db + 2 * k, p.idesc, c > first || k > 0);
-        tc::mma_commit(empty + s);
-        if (++s == kWideStages) s = 0, parity ^= 1;
+        for (int s = 0; s < kWideStages; ++s, db += stage_step) {
+          if (c == last) break;
+          if (!tc::mbar_wait(full + s, parity)) {
+            bad = 1;
+            break;
+          }
+          tc::fence_after_sync();
+          if (s == 0 && c == first) {
+            mma_ts(tmem, weights, db, p.idesc, false);
+          } else {
+            mma_ts(tmem, weights + s * 32, db, p.idesc, true);
+          }
+#pragma unroll
+          for (int k = 1; k < 4; ++k) mma_ts(tmem, weights + s * 32 + k * 8, db + 2 * k, p.idesc, true);
+          tc::mma_commit(empty + s);
+          ++c;
+        }
       }
       tc::mma_commit(&done);   // also after a failure: it releases the waiters
     }
@@ -449,7 +454,7 @@ __global__ void __launch_bounds__(kWideThreads<kTurns>, kTurns == 2 ? 2 : 1) w4_
   tc::fence_after_sync();
   __syncwarp();
   // [part][row of x][weight row]: where x was, or behind everything else where other blocks write too
-  float* sums = reinterpret_cast<float*>(smem + (p.splits > 1 ? kWideStages * stage_bytes + kCodeRing<kTurns> : 0));
+  float* sums = reinterpret_cast<float*>(smem + (p.splits > 1 ? kWideStages * stage_bytes + kCodeRing : 0));
   if (p.splits > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (warp >= 2 && ok) {
     const int quarter = warp & 3, turn = (warp - 2) >> 2, row = quarter * 32 + lane;
@@ -481,7 +486,7 @@ __global__ void __launch_bounds__(kWideThreads<kTurns>, kTurns == 2 ? 2 : 1) w4_
     __syncthreads();
   }
   const int from = p.splits > 1 ? static_cast<int>(blockIdx.z) * p.share : 0, rows = min(min(p.share, p.tokens - from), a.m - token0 - from);
-  for (int i = warp; i < rows; i += kWideThreads<kTurns> / 32) {
+  for (int i = warp; i < rows; i += kWideThreads / 32) {
     const int m = token0 + from + i;
     float4 v = *reinterpret_cast<const float4*>(sums + i * kWideRows + lane * 4);
     for (int r = 1; r < p.splits; ++r) {
@@ -583,42 +588,40 @@ cudaError_t narrow(const W4Args& a, cudaStream_t stream) {
   return a.group == 32 ? launch_narrow<kR, kN, 4>(a, stream) : (a.group == 64 ? launch_narrow<kR, kN, 2>(a, stream) : launch_narrow<kR, kN, 1>(a, stream));
 }
 
-int wide_smem(const Wide& p) { return kWideStages * p.tokens * 128 + (p.turns == 2 ? kCodeRing<2> : kCodeRing<4>) + (p.splits > 1 ? p.splits * p.share * kWideRows * 4 : 0) + 1024; }
+int wide_smem(const Wide& p) { return kWideStages * p.tokens * 128 + kCodeRing + (p.splits > 1 ? p.splits * p.share * kWideRows * 4 : 0) + 1024; }
 
-// Blocks that the GPU holds at a time, in clusters of `splits`: a cluster lies in one group of SMs, and what is left over in each group stays idle.
-int resident(int turns, int splits) {
-  static const std::array<std::array<int, 9>, 2> counts = [] {
-    std::array<std::array<int, 9>, 2> c = {};
-    for (int t = 0; t < 2; ++t) {
-      const int per_sm = t == 0 ? 2 : 1;
-      for (int n = 1; n <= 8; ++n) {
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(1, 1, n);
-        cfg.blockDim = dim3(t == 0 ? kWideThreads<2> : kWideThreads<4>);
-        cfg.dynamicSmemBytes = per_sm == 2 ? kWideSmemOfTwo : kWideSmem;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = 1;
-        attr[0].val.clusterDim.z = n;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        int clusters = 0;
-        cudaError_t rc = cudaFuncSetAttribute(t == 0 ? w4_wide_kernel<2, false> : w4_wide_kernel<4, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem);
-        if (rc == cudaSuccess)
-          rc = t == 0 ? cudaOccupancyMaxActiveClusters(&clusters, w4_wide_kernel<2, false>, &cfg) : cudaOccupancyMaxActiveClusters(&clusters, w4_wide_kernel<4, false>, &cfg);
-        if (rc != cudaSuccess) cudaGetLastError();
-        c[t][n] = rc == cudaSuccess && clusters > 0 ? clusters * n : sm_count() * per_sm * 3 / 4;
-      }
+// Blocks that the GPU holds at a time, in clusters of `splits`: a cluster lies in one group of SMs, and what is left over in each group stays idle (148, 148,
+// 135, 132, 130, 132, 105 and 120 for clusters of one to eight).
+int resident(int splits) {
+  static const std::array<int, 9> counts = [] {
+    std::array<int, 9> c = {};
+    for (int n = 1; n <= 8; ++n) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(1, 1, n);
+      cfg.blockDim = dim3(kWideThreads);
+      cfg.dynamicSmemBytes = kWideSmem;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = n;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      int clusters = 0;
+      cudaError_t rc = cudaFuncSetAttribute(w4_wide_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem);
+      if (rc == cudaSuccess) rc = cudaOccupancyMaxActiveClusters(&clusters, w4_wide_kernel<false>, &cfg);
+      if (rc != cudaSuccess) cudaGetLastError();
+      c[n] = rc == cudaSuccess && clusters > 0 ? clusters * n : sm_count() * 3 / 4;
     }
     return c;
   }();
-  return counts[turns == 2 ? 0 : 1][splits];
+  return counts[splits];
 }
 
-// Rows of x per block, parts of K, and whether two blocks share an SM.  A chunk of 64 columns costs an SM the making of its weights (some kMake clocks per
-// block) or its products (two clocks per row of x), a block some 5000 clocks before its first and after its last chunk.
+// Rows of x per block and parts of K.  A chunk of 64 columns costs the making of its weights (some 400 clocks) or its products (two clocks per row of x), a
+// block some 5000 clocks before its first and after its last chunk.  (Measured beside all other choices for 12 sizes from 24 x 2048 x 2048 to
+// 1537 x 16384 x 2048: within 4 % of the best.)
 void choose_wide(int m, int blocks, Wide& p) {
-  constexpr double kMake = 300, kRound = 5000, kSplit = 1500, kToken = 20;
+  constexpr double kMake = 400, kRound = 5000, kSplit = 1500, kToken = 20;
   double best = 0;
   Wide w = p;
   for (int most = 32; most <= kMostTokens; most += 32) {
@@ -626,30 +629,25 @@ void choose_wide(int m, int blocks, Wide& p) {
     w.tokens = ((m + tiles - 1) / tiles + 15) / 16 * 16;
     for (w.splits = 1; w.splits <= 8 && (w.splits == 1 || w.splits * 2 <= p.chunks); ++w.splits) {
       w.share = (w.tokens + w.splits - 1) / w.splits;
-      for (w.turns = 2; w.turns <= 4; w.turns += 2) {
-        const int per_sm = w.turns == 2 ? 2 : 1;
-        if (wide_smem(w) > (per_sm == 2 ? kWideSmemOfTwo : kWideSmem) || (per_sm == 2 && w.tokens > 128)) continue;
-        const int all = blocks * ((m + w.tokens - 1) / w.tokens) * w.splits, at_once = resident(w.turns, w.splits), waves = (all + at_once - 1) / at_once;
-        const bool alone = all <= at_once / per_sm;   // no two blocks on an SM
-        const double make = alone && per_sm == 2 ? 1.5 * kMake : per_sm * kMake, products = (alone ? 1 : per_sm) * 2.0 * w.tokens;
-        const double cost = waves * ((p.chunks + w.splits - 1) / w.splits * (make > products ? make : products) + kRound + (w.splits > 1 ? kSplit : 0.0) + kToken * w.tokens);
-        if (best == 0 || cost < best) {
-          best = cost;
-          p.tokens = w.tokens;
-          p.splits = w.splits;
-          p.share = w.share;
-          p.turns = w.turns;
-        }
+      if (wide_smem(w) > kWideSmem) continue;
+      const int all = blocks * ((m + w.tokens - 1) / w.tokens) * w.splits, at_once = resident(w.splits), waves = (all + at_once - 1) / at_once;
+      const double products = 2.0 * w.tokens;
+      const double cost = waves * ((p.chunks + w.splits - 1) / w.splits * (kMake > products ? kMake : products) + kRound + (w.splits > 1 ? kSplit : 0.0) + kToken * w.tokens);
+      if (best == 0 || cost < best) {
+        best = cost;
+        p.tokens = w.tokens;
+        p.splits = w.splits;
+        p.share = w.share;
       }
     }
   }
 }
 
-template <int kTurns, bool kG32>
+template <bool kG32>
 cudaError_t start_wide(const Wide& p, dim3 grid, const CUtensorMap& map, cudaStream_t stream) {
-  static const cudaError_t rc = cudaFuncSetAttribute(w4_wide_kernel<kTurns, kG32>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem);
+  static const cudaError_t rc = cudaFuncSetAttribute(w4_wide_kernel<kG32>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem);
   if (rc != cudaSuccess) return rc;
-  MCCL_LAUNCH_PDL_CLUSTER((w4_wide_kernel<kTurns, kG32>), grid, kWideThreads<kTurns>, wide_smem(p), stream, static_cast<unsigned>(p.splits), map, p);
+  MCCL_LAUNCH_PDL_CLUSTER(w4_wide_kernel<kG32>, grid, kWideThreads, wide_smem(p), stream, static_cast<unsigned>(p.splits), map, p);
   count_launch();
   return ::mccl::launch_status();
 }
@@ -675,8 +673,7 @@ cudaError_t launch_wide(const W4Args& a, cudaStream_t stream) {
                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return cudaErrorNotSupported;
   const dim3 grid(blocks, (a.m + p.tokens - 1) / p.tokens, p.splits);
-  if (p.turns == 2) return a.group == 32 ? start_wide<2, true>(p, grid, map, stream) : start_wide<2, false>(p, grid, map, stream);
-  return a.group == 32 ? start_wide<4, true>(p, grid, map, stream) : start_wide<4, false>(p, grid, map, stream);
+  return a.group == 32 ? start_wide<true>(p, grid, map, stream) : start_wide<false>(p, grid, map, stream);
 }
 
 }  // namespace
