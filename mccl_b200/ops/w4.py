@@ -106,10 +106,11 @@ def linear_w4(x: torch.Tensor, weight: W4Weight, bias: Optional[torch.Tensor] = 
     """act(x @ W^T + b) + residual for x bf16 ``[..., k]``; bias fp32 ``[n]``; act "none" or "gelu".  Forward only.
 
     Codes are multiplied as whole numbers and scaled in fp32, so that nothing but x and the result is rounded."""
-    if act not in ("none", "gelu"):
+    gelu = act == "gelu"
+    if not gelu and act != "none":
         raise RuntimeError(f"linear_w4: unknown activation '{act}'")
     if x.is_cuda:
-        return _C.w4_linear(x, weight.codes, weight.params, weight.n, weight.k, weight.group, bias, act == "gelu", residual)
+        return _C.w4_linear(x, weight.codes, weight.params, weight.n, weight.k, weight.group, bias, gelu, residual)
     y = F.linear(x.float(), weight._plain(), None if bias is None else bias.float())
     if act == "gelu":
         y = 0.5 * y * (1.0 + torch.erf(y * math.sqrt(0.5)))
