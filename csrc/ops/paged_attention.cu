@@ -4,6 +4,7 @@
 // positions j and m their maximum.  Sums over any split of the positions join exactly: parts (m, l, o) combine with weights exp(m_part - m).
 #include "../core/launch.hpp"
 #include "../symm/cu_driver.hpp"
+#include "divisor.cuh"
 #include "gemm_common.cuh"
 #include "half16.cuh"
 #include "ops.hpp"
@@ -45,16 +46,6 @@ __device__ __forceinline__ Span span_of(int length, int window, int sinks) {
   }
   return s;
 }
-
-// n / d for n < 2^31 as one multiplication: with 2^s < d <= 2^(s + 1) and m = ceil(2^(32 + s) / d), m d exceeds 2^(32 + s) by less than 2^(s + 1).
-struct Divisor {
-  unsigned d, m, s;
-  __host__ explicit Divisor(unsigned by = 1) : d(by), m(0), s(0) {
-    while ((2ull << s) < by) ++s;
-    if (by > 1) m = static_cast<unsigned>(((1ull << (32 + s)) + by - 1) / by);
-  }
-  __device__ __forceinline__ unsigned of(unsigned n) const { return m == 0 ? n : __umulhi(n, m) >> s; }
-};
 
 struct Launch {
   PagedAttentionArgs a;

@@ -1,6 +1,7 @@
 // Writing into a paged key-value cache and copying its pages.  Both are bound by memory: every value is read once and written once,
 // 16 bytes per thread and access.
 #include "../core/launch.hpp"
+#include "divisor.cuh"
 #include "half16.cuh"
 #include "ops.hpp"
 #include "serving.hpp"
@@ -25,42 +26,53 @@ __device__ __forceinline__ void rotate_pairs(float (&f)[8], const float* cos_row
   }
 }
 
-// A unit is 8 elements of one head of one token.  A block takes `per_block` consecutive tokens, so that the units of a token are
-// counted in 32 bits whatever the number of tokens.
+// A unit is 8 elements of one head of one token: the token's units are k's, v's and, where q is rotated, q's.  A block has one token of many units, or as many
+// tokens as it has threads for, so a thread has one token and follows its place (position, row, page) once; its loads are all under way before the first
+// result.  1537 tokens of 48 heads of 128, 38 MB: 12.4 us with a unit at a time, 11.0 us so (5.8 at the rate of a copy).
 template <typename H>
-__global__ void __launch_bounds__(kThreads) paged_append_kernel(AppendArgs a, int per_block, int units) {
+__global__ void __launch_bounds__(kThreads) paged_append_kernel(AppendArgs a, int per_block, Divisor units, Divisor kv_units, Divisor hd8) {
+  constexpr int kDeep = 4;
   ::mccl::pdl_wait();
   ::mccl::pdl_trigger();
-  const int hd8 = a.head_dim / 8, kv_units = a.kv_heads * hd8;
-  const long long first = static_cast<long long>(blockIdx.x) * per_block;
-  for (int i = threadIdx.x; i < per_block * units; i += kThreads) {
-    const int in_block = i / units, u = i - in_block * units;
-    const long long t = first + in_block;
-    if (t >= a.tokens) break;
-    const int part = u < kv_units ? 0 : (u < 2 * kv_units ? 1 : 2);   // k, v, q
-    const int r = u - part * kv_units;
-    const int h = r / hd8, d8 = r - h * hd8;
+  const int in_block = units.of(threadIdx.x);   // zero where a token's units are more than the threads
+  const long long t = static_cast<long long>(blockIdx.x) * per_block + in_block;
+  if (in_block >= per_block || t >= a.tokens) return;
+  using V = uint4;
+  auto source = [&](int u) -> const V* {
+    const int part = kv_units.of(u), r = u - (part > 2 ? 2 : part) * kv_units.d, h = hd8.of(r);
     const TokenView& from = part == 0 ? a.k : (part == 1 ? a.v : a.q);
-    uint4 raw = __ldg(reinterpret_cast<const uint4*>(static_cast<const typename H::T*>(from.p) + t * from.token + h * from.head) + d8);
-    const int pos = __ldg(a.positions + t), row = a.rows ? __ldg(a.rows + t) : static_cast<int>(t);
-    const int ps = a.table.page_size;
-    int page = -1;
-    if (pos >= 0 && row >= 0 && row < a.table.rows && pos / ps < a.table.width && (a.cos == nullptr || pos < a.rope_rows))
-      page = __ldg(a.table.p + row * a.table.stride + pos / ps);
-    const bool good = page >= 0 && page < a.table.pages;
-    if (a.cos != nullptr && part != 1 && good) {
-      float f[8];
-      unpack8_as<H>(raw, f);
-      const size_t at = (static_cast<size_t>(pos) * hd8 + d8) * 4;
-      rotate_pairs(f, a.cos + at, a.sin + at);
-      raw = pack8_as<H>(f);
-    }
-    if (part == 2) {
-      if (!good) raw = make_uint4(0, 0, 0, 0);
-      reinterpret_cast<uint4*>(static_cast<typename H::T*>(a.q_out) + t * a.heads * a.head_dim)[r] = raw;
-    } else if (good) {
-      const PagedTensor& to = part == 0 ? a.k_pages : a.v_pages;
-      reinterpret_cast<uint4*>(static_cast<typename H::T*>(to.p) + page * to.page + h * to.head + (pos % ps) * to.token)[d8] = raw;
+    return reinterpret_cast<const V*>(static_cast<const typename H::T*>(from.p) + t * from.token + h * from.head) + (r - h * hd8.d);
+  };
+  const int pos = __ldg(a.positions + t), row = a.rows ? __ldg(a.rows + t) : static_cast<int>(t);
+  const int ps = a.table.page_size, slot = pos >= 0 ? pos / ps : 0;
+  const bool inside = pos >= 0 && row >= 0 && row < a.table.rows && slot < a.table.width && (a.cos == nullptr || pos < a.rope_rows);
+  int page = -1;
+  if (inside) page = __ldg(a.table.p + row * a.table.stride + slot);
+  const bool good = page >= 0 && page < a.table.pages;
+  for (int u0 = threadIdx.x - in_block * units.d; u0 < static_cast<int>(units.d); u0 += kThreads * kDeep) {
+    V raw[kDeep];
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i)
+      if (u0 + i * kThreads < static_cast<int>(units.d)) raw[i] = __ldg(source(u0 + i * kThreads));
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i) {
+      const int u = u0 + i * kThreads;
+      if (u >= static_cast<int>(units.d)) break;
+      const int part = min(static_cast<int>(kv_units.of(u)), 2), r = u - part * kv_units.d, h = hd8.of(r), d8 = r - h * hd8.d;
+      if (a.cos != nullptr && part != 1 && good) {
+        float f[8];
+        unpack8_as<H>(raw[i], f);
+        const size_t at = (static_cast<size_t>(pos) * hd8.d + d8) * 4;
+        rotate_pairs(f, a.cos + at, a.sin + at);
+        raw[i] = pack8_as<H>(f);
+      }
+      if (part == 2) {
+        if (!good) raw[i] = make_uint4(0, 0, 0, 0);
+        reinterpret_cast<V*>(static_cast<typename H::T*>(a.q_out) + t * a.heads * a.head_dim)[r] = raw[i];
+      } else if (good) {
+        const PagedTensor& to = part == 0 ? a.k_pages : a.v_pages;
+        reinterpret_cast<V*>(static_cast<typename H::T*>(to.p) + page * to.page + h * to.head + (pos - slot * ps) * to.token)[d8] = raw[i];
+      }
     }
   }
 }
@@ -107,14 +119,14 @@ cudaError_t paged_append(const AppendArgs& a, cudaStream_t stream) {
   if (a.tokens <= 0) return cudaSuccess;
   const int units = (2 * a.kv_heads + (a.q_out ? a.heads : 0)) * (a.head_dim / 8);
   if (units <= 0) return cudaSuccess;
-  int per_block = kThreads / units;
-  if (per_block < 1) per_block = 1;
+  const int per_block = units < kThreads ? kThreads / units : 1;
   const long long blocks = (a.tokens + per_block - 1) / per_block;
   if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
+  const Divisor by_units(units), by_kv(a.kv_heads * (a.head_dim / 8)), by_hd8(a.head_dim / 8);
   if (a.type == Half16::bf16)
-    MCCL_LAUNCH_PDL(paged_append_kernel<Bf16>, static_cast<unsigned>(blocks), kThreads, 0, stream, a, per_block, units);
+    MCCL_LAUNCH_PDL(paged_append_kernel<Bf16>, static_cast<unsigned>(blocks), kThreads, 0, stream, a, per_block, by_units, by_kv, by_hd8);
   else
-    MCCL_LAUNCH_PDL(paged_append_kernel<Fp16>, static_cast<unsigned>(blocks), kThreads, 0, stream, a, per_block, units);
+    MCCL_LAUNCH_PDL(paged_append_kernel<Fp16>, static_cast<unsigned>(blocks), kThreads, 0, stream, a, per_block, by_units, by_kv, by_hd8);
   count_launch();
   return ::mccl::launch_status();
 }
