@@ -65,6 +65,12 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The first product of a sum.
+__device__ __forceinline__ void mma16816_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ float finished(const W4Args& a, float v, int m, int n) {
   if (a.bias) v += __ldg(a.bias + n);
   if (a.gelu) v = 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
@@ -87,7 +93,8 @@ int narrow_smem(int m, int pairs) { return kNarrowWarps * kDeep<kR> * kNarrowSlo
 // run of stages of 128 columns, and add up at its end.  A lane's 16 bytes of 64 columns are its own A fragments of four m16n8k16 products: it copies them ahead into its own place and waits for nobody, and so
 // it does with its two rows' parameters (kParams groups in a stage).  x lies in shared memory, 128 bytes of every row per 64 columns, in the order of the
 // 128-byte swizzle; kN is how many times 8 rows it has.
-template <int kR, int kN, int kParams>
+// kEven: no tile and no half stage is missing at the end of N or K.
+template <int kR, int kN, int kParams, bool kEven>
 __global__ void __launch_bounds__(kNarrowThreads, 2) w4_narrow_kernel(W4Args a, int tiles, int chunks, int group_shift, int along_shift) {
   extern __shared__ __align__(128) unsigned char smem[];
   constexpr int kSlot = kNarrowSlot<kR, kParams>, kTile = 1024 + kParams * 256, kDeep = ops::kDeep<kR>, kOut = kR * kN * 128;
@@ -119,18 +126,19 @@ __global__ void __launch_bounds__(kNarrowThreads, 2) w4_narrow_kernel(W4Args a, 
   const size_t codes_on = (static_cast<size_t>(step) * chunks - 2 * slice) * 32, params_on = static_cast<size_t>(step) * groups * 8;
   auto issue = [&](int slot) {
     if (to_load > 0) {
-      const bool second = 2 * at + 1 < chunks;
+      const bool second = kEven || 2 * at + 1 < chunks;
+      const uint32_t to = ring + slot * kSlot;
 #pragma unroll
       for (int r = 0; r < kR; ++r) {
-        const uint32_t to = ring + slot * kSlot + r * kTile;
-        const bool there = r == 0 || load_tile + r < tiles;
+        const bool there = kEven || r == 0 || load_tile + r < tiles;
         const uint4* from = there ? codes + r * tile_codes : codes;
-        copy_async<16>(to + lane * 16, from, there);
-        copy_async<16>(to + 512 + lane * 16, second ? from + 32 : from, second && there);
+        copy_async<16>(to + r * kTile + lane * 16, from, there);
+        copy_async<16>(to + r * kTile + 512 + lane * 16, second ? from + 32 : from, second && there);
+        const uint2* with = params + (there ? r * groups * 8 : 0);
 #pragma unroll
         for (int i = 0; i < kParams; ++i) {
-          const int group = kParams == 1 ? at >> (group_shift - 7) : min(kParams * at + i, groups - 1);
-          copy_async<8>(to + 1024 + i * 256 + lane * 8, params + ((there ? r * groups : 0) + group) * 8, there);
+          const int group = kParams == 1 ? at >> (group_shift - 7) : (kEven ? kParams * at + i : min(kParams * at + i, groups - 1));
+          copy_async<8>(to + r * kTile + 1024 + i * 256 + lane * 8, with + group * 8, there);
         }
       }
       --to_load;
@@ -200,8 +208,11 @@ __global__ void __launch_bounds__(kNarrowThreads, 2) w4_narrow_kernel(W4Args a, 
 #pragma unroll
             for (int n = 0; n < kN; ++n) {
               float (&c)[4] = acc[r][j][n];
-              if (begins) c[0] = c[1] = c[2] = c[3] = 0.f;
-              mma16816(c, a0, a1, a2, a3, b[n][s >> 1][(s & 1) * 2], b[n][s >> 1][(s & 1) * 2 + 1]);
+              if (begins) {
+                mma16816_first(c, a0, a1, a2, a3, b[n][s >> 1][(s & 1) * 2], b[n][s >> 1][(s & 1) * 2 + 1]);
+              } else {
+                mma16816(c, a0, a1, a2, a3, b[n][s >> 1][(s & 1) * 2], b[n][s >> 1][(s & 1) * 2 + 1]);
+              }
               if (ends && (kParams > 1 || j == 1)) {
                 if (kParams == 1) {
 #pragma unroll
@@ -568,9 +579,9 @@ int log2_of(int v) {
   return s;
 }
 
-template <int kR, int kN, int kParams>
+template <int kR, int kN, int kParams, bool kEven>
 cudaError_t launch_narrow(const W4Args& a, cudaStream_t stream) {
-  static const cudaError_t rc = cudaFuncSetAttribute(w4_narrow_kernel<kR, kN, kParams>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+  static const cudaError_t rc = cudaFuncSetAttribute(w4_narrow_kernel<kR, kN, kParams, kEven>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
   if (rc != cudaSuccess) return rc;
   const int chunks = (a.k + 63) / 64, smem = narrow_smem<kR, kN, kParams>(a.m, (chunks + 1) / 2);
   if (smem > 227 * 1024) return cudaErrorNotSupported;
@@ -579,13 +590,17 @@ cudaError_t launch_narrow(const W4Args& a, cudaStream_t stream) {
   int along = 3;
   while (along > 0 && tiles << (along - 1) >= blocks * kNarrowWarps * 3 / 4) --along;
   const int groups = (tiles + (kNarrowWarps >> along) - 1) / (kNarrowWarps >> along);
-  MCCL_LAUNCH_PDL((w4_narrow_kernel<kR, kN, kParams>), groups < blocks ? groups : blocks, kNarrowThreads, smem, stream, a, (a.n + 15) / 16, chunks, log2_of(a.group), along);
+  MCCL_LAUNCH_PDL((w4_narrow_kernel<kR, kN, kParams, kEven>), groups < blocks ? groups : blocks, kNarrowThreads, smem, stream, a, (a.n + 15) / 16, chunks, log2_of(a.group), along);
   count_launch();
   return ::mccl::launch_status();
 }
+template <int kR, int kN, int kParams>
+cudaError_t narrow_by_size(const W4Args& a, cudaStream_t stream) {
+  return a.k % 128 == 0 && (a.n + 15) / 16 % kR == 0 ? launch_narrow<kR, kN, kParams, true>(a, stream) : launch_narrow<kR, kN, kParams, false>(a, stream);
+}
 template <int kR, int kN>
 cudaError_t narrow(const W4Args& a, cudaStream_t stream) {
-  return a.group == 32 ? launch_narrow<kR, kN, 4>(a, stream) : (a.group == 64 ? launch_narrow<kR, kN, 2>(a, stream) : launch_narrow<kR, kN, 1>(a, stream));
+  return a.group == 32 ? narrow_by_size<kR, kN, 4>(a, stream) : (a.group == 64 ? narrow_by_size<kR, kN, 2>(a, stream) : narrow_by_size<kR, kN, 1>(a, stream));
 }
 
 int wide_smem(const Wide& p) { return kWideStages * p.tokens * 128 + kCodeRing + (p.splits > 1 ? p.splits * p.share * kWideRows * 4 : 0) + 1024; }
