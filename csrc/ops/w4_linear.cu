@@ -384,34 +384,42 @@ __global__ void __launch_bounds__(kWideThreads, 1) w4_wide_kernel(const __grid_c
     }
     __syncwarp();
   } else {   // ---- weights: kTurns warps for each 32 rows take chunks in turn
+    static_assert(kTurns == kWideStages);   // a warp's stage is always the same
     const int quarter = warp & 3, turn = (warp - 2) >> 2, g = lane >> 2;
     const int row_tiles = (a.n + 15) / 16, groups = a.k >> p.group_shift, tile0 = blockIdx.x * (kWideRows / 16) + quarter * 2;
+    const bool there[2] = {tile0 < row_tiles, tile0 + 1 < row_tiles};
     const uint32_t ring = tc::smem_u32(smem) + kWideStages * stage_bytes + (warp - 2) * (kCodeDeep * 2 * 512) + lane * 16;
+    const uint32_t place = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + p.columns + turn * 32;
+    const uint4* codes[2];
+    const uint2* params[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {   // of a tile that there is not, the first one's: nothing of it is used
+      codes[k] = static_cast<const uint4*>(a.codes) + (there[k] ? static_cast<size_t>(tile0 + k) * p.chunks * 32 : 0) + lane;
+      params[k] = static_cast<const uint2*>(a.params) + (there[k] ? static_cast<size_t>(tile0 + k) * groups * 8 : 0) + g;
+    }
     auto issue = [&](int c, int slot) {
       if (c < last) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          copy_async<16>(ring + (slot * 2 + i) * 512, static_cast<const uint4*>(a.codes) + (tile0 + i < row_tiles ? (static_cast<size_t>(tile0 + i) * p.chunks + c) * 32 + lane : 0),
-                         tile0 + i < row_tiles);
+        for (int k = 0; k < 2; ++k) copy_async<16>(ring + (slot * 2 + k) * 512, codes[k] + c * 32, there[k]);
       }
       copy_commit();
     };
     uint2 prm[2][2];
     auto parameters = [&](int c, uint2 (&to)[2][2]) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int h = 0; h < (kG32 ? 2 : 1); ++h) {
-          const int group = min((c * 64 + h * 32) >> p.group_shift, groups - 1);
-          to[i][h] = c < last && tile0 + i < row_tiles ? __ldg(static_cast<const uint2*>(a.params) + (static_cast<size_t>(tile0 + i) * groups + group) * 8 + g) : make_uint2(0, 0);
+          const int group = kG32 ? min(2 * c + h, groups - 1) : c * 64 >> p.group_shift;
+          to[k][h] = there[k] ? __ldg(params[k] + group * 8) : make_uint2(0, 0);
         }
     };
 #pragma unroll
     for (int i = 0; i < kCodeDeep - 1; ++i) issue(first + turn + kTurns * i, i);
-    parameters(first + turn, prm);
+    if (first + turn < last) parameters(first + turn, prm);
     int slot = 0;
-    for (int c = first + turn; c < last; c += kTurns) {
-      const int i = c - first, s = i % kWideStages;
+    uint32_t parity = 1;   // of the use before, once there was one
+    for (int c = first + turn; c < last; c += kTurns, parity ^= 1) {
       copy_wait<kCodeDeep - 2>();
       uint4 w[2];
 #pragma unroll
@@ -419,7 +427,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) w4_wide_kernel(const __grid_c
       issue(c + kTurns * (kCodeDeep - 1), slot == 0 ? kCodeDeep - 1 : slot - 1);
       slot = slot == kCodeDeep - 1 ? 0 : slot + 1;
       uint2 next[2][2];
-      parameters(c + kTurns, next);
+      parameters(min(c + kTurns, last - 1), next);
       // the weights are ready in registers before their place in tensor memory is awaited: making them is not part of the loop from one use of a
       // place to the next (490 clocks per chunk when it was, at any number of rows of x)
       uint32_t r[2][16];
@@ -435,18 +443,18 @@ __global__ void __launch_bounds__(kWideThreads, 1) w4_wide_kernel(const __grid_c
           r[k][4 * step + 3] = mul2(codes2(word[step] >> 12, minus_zero2(q.y)), scale2(q.y));
         }
       }
-      const bool ok = __all_sync(0xffffffffu, i < kWideStages || tc::mbar_wait(empty + s, ((i / kWideStages) - 1) & 1));
-      if (!ok) {
+      const bool ok = c - first < kWideStages || tc::mbar_wait(empty + turn, parity);
+      if (!__all_sync(0xffffffffu, ok)) {
         if (lane == 0) bad = 1;
         break;
       }
       tc::fence_after_sync();
 #pragma unroll
-      for (int k = 0; k < 2; ++k) tmem_st_16x64(tmem + (static_cast<uint32_t>(quarter * 32 + k * 16) << 16) + p.columns + s * 32, r[k]);
+      for (int k = 0; k < 2; ++k) tmem_st_16x64(place + (static_cast<uint32_t>(k * 16) << 16), r[k]);
       tmem_st_wait();
       tc::fence_before_sync();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(full + s);
+      if (lane == 0) tc::mbar_arrive(full + turn);
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
