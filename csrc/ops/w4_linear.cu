@@ -268,6 +268,7 @@ struct Wide {
   int allocated;
   int splits, share;    // blocks of a cluster that share out K, and rows of x whose sums each of them finishes
   int vector;           // y and residual can be accessed four elements at a time
+  int tiles, row_tiles; // of the stream: tiles of weight rows and rows of x, and how many of the latter
   uint32_t idesc;
   int* err;
 };
@@ -299,6 +300,47 @@ __device__ __forceinline__ void store_peer(uint32_t at, int rank, float v) {
   uint32_t there;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there), "f"(v) : "memory");
+}
+
+// A lane's part of 16 x 64 weights for tmem_st_16x64, rounded to bf16 once: scale times whole number.
+template <bool kG32>
+__device__ __forceinline__ void make_weights(uint32_t (&r)[16], const uint4& w, const uint2 (&prm)[2]) {
+  const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int step = 0; step < 4; ++step) {
+    const uint2 q = prm[kG32 ? step >> 1 : 0];
+    r[4 * step] = mul2(codes2(word[step], minus_zero2(q.x)), scale2(q.x));
+    r[4 * step + 1] = mul2(codes2(word[step] >> 4, minus_zero2(q.y)), scale2(q.y));
+    r[4 * step + 2] = mul2(codes2(word[step] >> 8, minus_zero2(q.x)), scale2(q.x));
+    r[4 * step + 3] = mul2(codes2(word[step] >> 12, minus_zero2(q.y)), scale2(q.y));
+  }
+}
+__device__ __forceinline__ void load_bias(float (&bias)[4], const W4Args& a, int n4) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) bias[e] = a.bias && n4 + e < a.n ? __ldg(a.bias + n4 + e) : 0.f;
+}
+// Four neighbouring results of a row; `vector`: y and residual can be accessed four elements at a time.
+__device__ __forceinline__ void finish4(const W4Args& a, const float4& v, const float (&bias)[4], int m, int n4, int vector) {
+  float f[4] = {v.x + bias[0], v.y + bias[1], v.z + bias[2], v.w + bias[3]};
+  if (a.gelu) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = 0.5f * f[e] * (1.f + erff(f[e] * 0.70710678118654752f));
+  }
+  __nv_bfloat16* y = static_cast<__nv_bfloat16*>(a.y) + static_cast<long long>(m) * a.n + n4;
+  const __nv_bfloat16* residual = static_cast<const __nv_bfloat16*>(a.residual) + (a.residual ? m * a.ldr + n4 : 0);
+  if (vector && n4 + 3 < a.n) {
+    if (a.residual) {
+      const uint2 raw = __ldg(reinterpret_cast<const uint2*>(residual));
+      const float2 lo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.x)), hi = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.y));
+      f[0] += lo.x, f[1] += lo.y, f[2] += hi.x, f[3] += hi.y;
+    }
+    __nv_bfloat162 out[2] = {__floats2bfloat162_rn(f[0], f[1]), __floats2bfloat162_rn(f[2], f[3])};
+    *reinterpret_cast<uint2*>(y) = *reinterpret_cast<const uint2*>(out);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n4 + e < a.n) y[e] = __float2bfloat16_rn(f[e] + (a.residual ? __bfloat162float(residual[e]) : 0.f));
+  }
 }
 
 // Block (x, y, z): weight rows 128 x and on, rows of x from `tokens` y on, part z of K.  D[weight row, row of x] = W x^T: the weights of a chunk of 64
@@ -432,17 +474,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) w4_wide_kernel(const __grid_c
       // place to the next (490 clocks per chunk when it was, at any number of rows of x)
       uint32_t r[2][16];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const uint32_t word[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
-#pragma unroll
-        for (int step = 0; step < 4; ++step) {
-          const uint2 q = prm[k][kG32 ? step >> 1 : 0];
-          r[k][4 * step] = mul2(codes2(word[step], minus_zero2(q.x)), scale2(q.x));
-          r[k][4 * step + 1] = mul2(codes2(word[step] >> 4, minus_zero2(q.y)), scale2(q.y));
-          r[k][4 * step + 2] = mul2(codes2(word[step] >> 8, minus_zero2(q.x)), scale2(q.x));
-          r[k][4 * step + 3] = mul2(codes2(word[step] >> 12, minus_zero2(q.y)), scale2(q.y));
-        }
-      }
+      for (int k = 0; k < 2; ++k) make_weights<kG32>(r[k], w[k], prm[k]);
       const bool ok = c - first < kWideStages || tc::mbar_wait(empty + turn, parity);
       if (!__all_sync(0xffffffffu, ok)) {
         if (lane == 0) bad = 1;
@@ -467,8 +499,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) w4_wide_kernel(const __grid_c
   __syncwarp();
   const int n4 = blockIdx.x * kWideRows + lane * 4, token0 = blockIdx.y * p.tokens;
   float bias[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) bias[e] = a.bias && n4 + e < a.n ? __ldg(a.bias + n4 + e) : 0.f;
+  load_bias(bias, a, n4);
   const bool ok = tc::mbar_wait(&done, 0);
   tc::fence_after_sync();
   __syncwarp();
@@ -515,26 +546,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) w4_wide_kernel(const __grid_c
       v.z += o.z;
       v.w += o.w;
     }
-    float f[4] = {v.x + bias[0], v.y + bias[1], v.z + bias[2], v.w + bias[3]};
-    if (a.gelu) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) f[e] = 0.5f * f[e] * (1.f + erff(f[e] * 0.70710678118654752f));
-    }
-    __nv_bfloat16* y = static_cast<__nv_bfloat16*>(a.y) + static_cast<long long>(m) * a.n + n4;
-    const __nv_bfloat16* residual = static_cast<const __nv_bfloat16*>(a.residual) + (a.residual ? m * a.ldr + n4 : 0);
-    if (p.vector && n4 + 3 < a.n) {
-      if (a.residual) {
-        const uint2 raw = __ldg(reinterpret_cast<const uint2*>(residual));
-        const float2 lo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.x)), hi = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.y));
-        f[0] += lo.x, f[1] += lo.y, f[2] += hi.x, f[3] += hi.y;
-      }
-      __nv_bfloat162 out[2] = {__floats2bfloat162_rn(f[0], f[1]), __floats2bfloat162_rn(f[2], f[3])};
-      *reinterpret_cast<uint2*>(y) = *reinterpret_cast<const uint2*>(out);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (n4 + e < a.n) y[e] = __float2bfloat16_rn(f[e] + (a.residual ? __bfloat162float(residual[e]) : 0.f));
-    }
+    finish4(a, v, bias, m, n4, p.vector);
   }
   if ((!ok || bad) && threadIdx.x == 0) atomicExch(p.err, 22);
   tc::fence_before_sync();
@@ -542,6 +554,238 @@ __global__ void __launch_bounds__(kWideThreads, 1) w4_wide_kernel(const __grid_c
   if (warp == 1) {
     tc::fence_after_sync();
     tc::tmem_dealloc(tmem, p.allocated);
+  }
+}
+
+// ------------------------------------------------- tiles for several rounds of SMs --
+// The same products for more tiles than there are SMs: a block takes tiles gridDim.x apart, and its four roles run on from one to the next.  Two sets of
+// sums in tensor memory (up to 192 rows of x each, behind them the weights' ring: 512 columns) let four warps of their own write a tile's results beside
+// the next one's products.  (As one block per tile each round of SMs took 5 us before its first and after its last product.)
+constexpr int kStreamThreads = (2 + 4 * kTurns + 4) * 32;
+constexpr int kStreamTokens = 192;
+constexpr int kStaged = 16 * kWideRows * 4;   // sums of 16 rows of x on their way to a row of y, twice
+int stream_smem(int tokens) { return kWideStages * tokens * 128 + kCodeRing + 2 * kStaged + 1024; }
+
+template <bool kG32>
+__global__ void __launch_bounds__(kStreamThreads, 1) w4_stream_kernel(const __grid_constant__ CUtensorMap x_map, Wide p) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024 - (tc::smem_u32(smem_raw) & 1023)) & 1023);
+  __shared__ uint64_t full[kWideStages], empty[kWideStages], sums_full[2], sums_empty[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int bad;
+  __shared__ volatile int lost;
+  const W4Args& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int stage_bytes = p.tokens * 128;
+  constexpr int kWeights = 2 * kStreamTokens;   // first column of the weights' ring
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kWideStages; ++i) {
+      tc::mbar_init(full + i, 5);
+      tc::mbar_init(empty + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(sums_full + i, 1);
+      tc::mbar_init(sums_empty + i, 4);
+    }
+    tc::mbar_init_fence();
+    bad = 0;
+    lost = 0;
+    tc::tma_prefetch_desc(&x_map);
+  }
+  __syncwarp();
+  if (warp == 1) tc::tmem_alloc(&tmem_slot, 512);
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  ::mccl::pdl_wait();
+  ::mccl::pdl_trigger();
+
+  if (warp == 0) {   // ---- x
+    if (tc::elect_one()) {
+      int s = 0, issued = 0;
+      uint32_t parity = 1;   // of a stage's use before
+      for (int tile = blockIdx.x; tile < p.tiles && !bad; tile += gridDim.x) {
+        const int row0 = tile % p.row_tiles * p.tokens;
+        for (int c = 0; c < p.chunks; ++c, ++issued) {
+          if (issued >= kWideStages && !tc::mbar_wait(empty + s, parity)) {
+            bad = 1;
+            break;
+          }
+          tc::mbar_expect_tx(full + s, stage_bytes);
+          tc::tma_load_2d(smem + s * stage_bytes, &x_map, full + s, c * 64, row0);
+          if (++s == kWideStages) s = 0, parity ^= 1;
+        }
+      }
+      if (bad)   // what was issued must land before the block retires
+        for (int i = max(issued - kWideStages, 0); i < issued; ++i) tc::mbar_wait(full + i % kWideStages, (i / kWideStages) & 1, 1u << 20);
+    }
+    __syncwarp();
+  } else if (warp == 1) {   // ---- products
+    if (tc::elect_one()) {
+      const uint64_t desc = tc::smem_desc_k_sw128(smem), stage_step = static_cast<uint64_t>(stage_bytes >> 4);
+      int s = 0, i = 0;
+      uint32_t parity = 0;
+      for (int tile = blockIdx.x; tile < p.tiles && !bad; tile += gridDim.x, ++i) {
+        if (i >= 2 && !tc::mbar_wait(sums_empty + (i & 1), ((i >> 1) - 1) & 1)) {
+          bad = 1;
+          break;
+        }
+        tc::fence_after_sync();
+        const uint32_t sums = tmem + (i & 1) * kStreamTokens;
+        for (int c = 0; c < p.chunks; ++c) {
+          if (!tc::mbar_wait(full + s, parity)) {
+            bad = 1;
+            break;
+          }
+          tc::fence_after_sync();
+          const uint64_t db = desc + s * stage_step;
+          const uint32_t weights = tmem + kWeights + s * 32;
+          mma_ts(sums, weights, db, p.idesc, c > 0);
+#pragma unroll
+          for (int k = 1; k < 4; ++k) mma_ts(sums, weights + k * 8, db + 2 * k, p.idesc, true);
+          tc::mma_commit(empty + s);
+          if (++s == kWideStages) s = 0, parity ^= 1;
+        }
+        tc::mma_commit(sums_full + (i & 1));   // also after a failure: it releases the waiters
+      }
+    }
+    __syncwarp();
+  } else if (warp < 2 + 4 * kTurns) {   // ---- weights; chunks are counted through all tiles, so that a warp's stage is always the same
+    const int quarter = warp & 3, turn = (warp - 2) >> 2, g = lane >> 2;
+    const int tiles16 = (a.n + 15) / 16, groups = a.k >> p.group_shift;
+    const uint32_t ring = tc::smem_u32(smem) + kWideStages * stage_bytes + (warp - 2) * (kCodeDeep * 2 * 512) + lane * 16;
+    const uint32_t place = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + kWeights + turn * 32;
+    struct Place {   // a chunk of a tile, and where its codes and parameters are
+      int tile, c;
+      const uint4* codes;
+      const uint2* params;
+      bool there[2];
+    };
+    auto at_tile = [&](Place& at) {
+      const int tile0 = at.tile / p.row_tiles * (kWideRows / 16) + quarter * 2;
+      at.there[0] = tile0 < tiles16;
+      at.there[1] = tile0 + 1 < tiles16;
+      at.codes = static_cast<const uint4*>(a.codes) + (at.there[0] ? static_cast<size_t>(tile0) * p.chunks * 32 : 0) + lane;
+      at.params = static_cast<const uint2*>(a.params) + (at.there[0] ? static_cast<size_t>(tile0) * groups * 8 : 0) + g;
+    };
+    auto settle = [&](Place& at) {
+      if (at.c < p.chunks) return;
+      do {
+        at.c -= p.chunks;
+        at.tile += gridDim.x;
+      } while (at.c >= p.chunks);
+      if (at.tile < p.tiles) at_tile(at);
+    };
+    Place now = {static_cast<int>(blockIdx.x), turn, nullptr, nullptr, {false, false}};
+    at_tile(now);
+    settle(now);
+    Place load = now, prm_at = now;
+    auto issue = [&](int slot) {
+      if (load.tile < p.tiles) {
+        copy_async<16>(ring + slot * 1024, load.codes + load.c * 32, load.there[0]);
+        copy_async<16>(ring + slot * 1024 + 512, load.codes + (load.there[1] ? p.chunks * 32 : 0) + load.c * 32, load.there[1]);
+        load.c += kTurns;
+        settle(load);
+      }
+      copy_commit();
+    };
+    auto parameters = [&](uint2 (&to)[2][2]) {
+      if (prm_at.tile >= p.tiles) return;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int h = 0; h < (kG32 ? 2 : 1); ++h) {
+          const int group = kG32 ? min(2 * prm_at.c + h, groups - 1) : prm_at.c * 64 >> p.group_shift;
+          to[k][h] = prm_at.there[k] ? __ldg(prm_at.params + (k * groups + group) * 8) : make_uint2(0, 0);
+        }
+      prm_at.c += kTurns;
+      settle(prm_at);
+    };
+    uint2 prm[2][2] = {}, next[2][2] = {};
+#pragma unroll
+    for (int i = 0; i < kCodeDeep - 1; ++i) issue(i);
+    parameters(prm);
+    int slot = 0;
+    bool used = false;
+    uint32_t parity = 1;
+    for (; now.tile < p.tiles; used = true, parity ^= 1) {
+      copy_wait<kCodeDeep - 2>();
+      uint4 w[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) w[k] = shared16(ring + (slot * 2 + k) * 512);
+      issue(slot == 0 ? kCodeDeep - 1 : slot - 1);
+      slot = slot == kCodeDeep - 1 ? 0 : slot + 1;
+      parameters(next);
+      uint32_t r[2][16];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) make_weights<kG32>(r[k], w[k], prm[k]);
+      const bool ok = !used || tc::mbar_wait(empty + turn, parity);
+      if (!__all_sync(0xffffffffu, ok)) {
+        if (lane == 0) bad = 1;
+        break;
+      }
+      tc::fence_after_sync();
+#pragma unroll
+      for (int k = 0; k < 2; ++k) tmem_st_16x64(place + (static_cast<uint32_t>(k * 16) << 16), r[k]);
+      tmem_st_wait();
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(full + turn);
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) prm[k][h] = next[k][h];
+      now.c += kTurns;
+      while (now.c >= p.chunks) {
+        now.c -= p.chunks;
+        now.tile += gridDim.x;
+      }
+    }
+    copy_wait<0>();
+  } else {   // ---- results
+    const int quarter = warp & 3;
+    float* staged = reinterpret_cast<float*>(smem + kWideStages * stage_bytes + kCodeRing);   // [2][row of x][weight row]
+    int i = 0, half = 0;
+    for (int tile = blockIdx.x; tile < p.tiles; tile += gridDim.x, ++i) {
+      const int block = tile / p.row_tiles, row0 = (tile - block * p.row_tiles) * p.tokens, n4 = block * kWideRows + lane * 4;
+      float bias[4];
+      load_bias(bias, a, n4);
+      if (!__all_sync(0xffffffffu, tc::mbar_wait(sums_full + (i & 1), (i >> 1) & 1)) && lane == 0) lost = 1;
+      asm volatile("bar.sync 1, 128;" ::: "memory");   // these four warps: they leave together or not at all
+      if (lost) {
+        bad = 1;
+        break;
+      }
+      tc::fence_after_sync();
+      const uint32_t sums = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (i & 1) * kStreamTokens;
+      for (int c = 0; c < p.tokens / 16; ++c, half ^= 1) {
+        uint32_t r[16];
+        tmem_ld_32x16(sums + c * 16, r);
+        tc::tmem_ld_wait();
+        if (c == p.tokens / 16 - 1) {   // the products of the tile after next may begin
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(sums_empty + (i & 1));
+        }
+        float* to = staged + half * (kStaged / 4);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) to[e * kWideRows + quarter * 32 + lane] = __uint_as_float(r[e]);
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int m = row0 + c * 16 + quarter * 4 + e;
+          if (m < a.m) finish4(a, *reinterpret_cast<const float4*>(to + (quarter * 4 + e) * kWideRows + lane * 4), bias, m, n4, p.vector);
+        }
+      }
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (bad && threadIdx.x == 0) atomicExch(p.err, 23);
+  if (warp == 1) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc(tmem, 512);
   }
 }
 
@@ -643,7 +887,9 @@ int resident(int splits) {
 // Rows of x per block and parts of K.  A chunk of 64 columns costs the making of its weights (some 400 clocks) or its products (two clocks per row of x), a
 // block some 5000 clocks before its first and after its last chunk.  (Measured beside all other choices for 12 sizes from 24 x 2048 x 2048 to
 // 1537 x 16384 x 2048: within 4 % of the best.)
-void choose_wide(int m, int blocks, Wide& p) {
+// With more tiles than SMs they run on from one to the next (returns true): no round has a beginning and an end of its own, and products hide the making of weights from 190 rows
+// of x on.
+bool choose_wide(int m, int blocks, Wide& p) {
   constexpr double kMake = 400, kRound = 5000, kSplit = 1500, kToken = 20;
   double best = 0;
   Wide w = p;
@@ -664,6 +910,25 @@ void choose_wide(int m, int blocks, Wide& p) {
       }
     }
   }
+  bool stream = false;
+  for (int most = 32; most <= kStreamTokens; most += 32) {
+    const int tiles = (m + most - 1) / most, tokens = ((m + tiles - 1) / tiles + 15) / 16 * 16, row_tiles = (m + tokens - 1) / tokens;
+    if (static_cast<long long>(blocks) * row_tiles > 0x7fffffff) continue;
+    const int all = blocks * row_tiles, rounds = (all + sm_count() - 1) / sm_count();
+    if (rounds < 2) continue;
+    const double products = 2.0 * tokens;
+    const double cost = rounds * (p.chunks * (kMake > products ? kMake : products) + 300.0) + kRound + kToken * tokens;
+    if (cost < best) {
+      best = cost;
+      stream = true;
+      p.tokens = tokens;
+      p.splits = 1;
+      p.share = tokens;
+      p.tiles = all;
+      p.row_tiles = row_tiles;
+    }
+  }
+  return stream;
 }
 
 template <bool kG32>
@@ -675,13 +940,22 @@ cudaError_t start_wide(const Wide& p, dim3 grid, const CUtensorMap& map, cudaStr
   return ::mccl::launch_status();
 }
 
-cudaError_t launch_wide(const W4Args& a, cudaStream_t stream) {
+template <bool kG32>
+cudaError_t start_stream(const Wide& p, const CUtensorMap& map, cudaStream_t stream) {
+  static const cudaError_t rc = cudaFuncSetAttribute(w4_stream_kernel<kG32>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem);
+  if (rc != cudaSuccess) return rc;
+  MCCL_LAUNCH_PDL(w4_stream_kernel<kG32>, p.tiles < sm_count() ? p.tiles : sm_count(), kStreamThreads, stream_smem(p.tokens), stream, map, p);
+  count_launch();
+  return ::mccl::launch_status();
+}
+
+cudaError_t launch_wide(const W4Args& a, cudaStream_t on) {
   Wide p;
   p.a = a;
   p.chunks = (a.k + 63) / 64;
   p.group_shift = log2_of(a.group);
   const int blocks = (a.n + kWideRows - 1) / kWideRows;
-  choose_wide(a.m, blocks, p);
+  const bool stream = choose_wide(a.m, blocks, p);
   p.columns = p.tokens <= 32 ? 32 : (p.tokens <= 64 ? 64 : (p.tokens <= 128 ? 128 : 256));
   p.allocated = p.columns + kWideStages * 32 <= 256 ? 256 : 512;
   p.vector = a.n % 4 == 0 && (a.residual == nullptr || (a.ldr % 4 == 0 && reinterpret_cast<uintptr_t>(a.residual) % 8 == 0));
@@ -695,8 +969,9 @@ cudaError_t launch_wide(const W4Args& a, cudaStream_t stream) {
   if (cu.TensorMapEncodeTiled(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(a.x), size, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return cudaErrorNotSupported;
+  if (stream) return a.group == 32 ? start_stream<true>(p, map, on) : start_stream<false>(p, map, on);
   const dim3 grid(blocks, (a.m + p.tokens - 1) / p.tokens, p.splits);
-  return a.group == 32 ? start_wide<true>(p, grid, map, stream) : start_wide<false>(p, grid, map, stream);
+  return a.group == 32 ? start_wide<true>(p, grid, map, on) : start_wide<false>(p, grid, map, on);
 }
 
 }  // namespace

@@ -67,6 +67,13 @@ def test_epilogues(rows, act, bias, residual):
     check(x_of(rows, 256), weight, w, torch.randn(384, device="cuda") if bias else None, act, x_of(rows, 384, seed=5) if residual else None)
 
 
+@pytest.mark.parametrize("rows,n,k,group", [(600, 4096, 64, 32), (333, 20000, 128, 64), (1025, 4099, 320, 64), (700, 9000, 96, 32), (2049, 2100, 544, 32), (1000, 32000, 192, 64)])
+@pytest.mark.parametrize("act", ["none", "gelu"])
+def test_more_tiles_than_sms(rows, n, k, group, act):
+    weight, w = make(n, k, group, seed=n)
+    check(x_of(rows, k), weight, w, torch.randn(n, device="cuda"), act, x_of(rows, n, seed=3))
+
+
 @pytest.mark.parametrize("rows", [3, 150])
 def test_shapes_and_strides(rows):
     weight, w = make(96, 128, 64)
