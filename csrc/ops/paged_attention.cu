@@ -54,7 +54,7 @@ struct Launch {
   Divisor page_blocks, warps;   // page_size / 16 (1 where that is not whole); warps of the grid
   int whole;                    // an item is one warp's
   float scale_log2;
-  unsigned* plan;               // tiles per block, then the first tile of every sequence (and behind the last)
+  int2* open;                   // [blocks]: the item that begins in a block and goes on behind it (-1: none), and the block where it ends
   float* part_ml;               // [blocks][2][rows][2]
   float* part_o;                // [blocks][2][rows][DP]
   int* err;                     // set when a wait inside the kernel ran out
@@ -244,6 +244,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   const unsigned units = first_tile[a.batch] * per_sequence;
   Place begin = {0, 0};
   int left = 0;
+  unsigned per = 0;
   if (p.whole) {
     auto unit = [&](unsigned item) {
       const unsigned b = p.items.of(item);
@@ -253,11 +254,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     begin.item = me * each + min(me, more);
     left = static_cast<int>(unit(begin.item + each + (me < more ? 1 : 0)) - unit(begin.item));
   } else {
-    const unsigned per = max(p.warps.of(units + p.warps.d - 1), static_cast<unsigned>(kLeast));
-    if (blockIdx.x == 0) {
-      if (threadIdx.x == 0) p.plan[0] = per * WARPS;
-      for (int b = threadIdx.x; b <= a.batch; b += WARPS * 32) p.plan[1 + b] = first_tile[b];
-    }
+    per = max(p.warps.of(units + p.warps.d - 1), static_cast<unsigned>(kLeast));
     const unsigned u = per * me;
     if (u < units) {
       const unsigned tile = p.items.of(u);   // the sequence is the last that begins at or before this tile
@@ -599,6 +596,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   __syncthreads();
   const int their_item = lane < 2 * WARPS ? piece_item[lane >> 1][lane & 1] : -1, their_ends = lane < 2 * WARPS ? piece_ends[lane >> 1][lane & 1] : 0;
   const unsigned pieces = __ballot_sync(0xffffffffu, their_item >= 0);
+  int2 open = make_int2(-1, 0);
   for (unsigned rest = pieces; rest != 0;) {
     // a run of pieces of one item
     const int item = __shfl_sync(0xffffffffu, their_item, __ffs(rest) - 1);
@@ -608,6 +606,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     const int b = p.items.of(item), hh = item - b * per_sequence;
     const int kv = p.head_blocks.of(hh), in_group = (hh - kv * p.head_blocks.d) * ROWS;
     const int heads = min(p.group - in_group, ROWS);
+    if (begun && !ended) open = make_int2(item, (first_tile[b] * per_sequence + (hh + 1) * (first_tile[b + 1] - first_tile[b]) - 1) / (per * WARPS));
     for (int u = threadIdx.x; u < heads * DP / 4; u += WARPS * 32) {
       const int row = u / (DP / 4), col = u % (DP / 4) * 4;
       float top = -INFINITY;
@@ -638,28 +637,26 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       }
     }
   }
+  if (threadIdx.x == 0) p.open[blockIdx.x] = open;
 }
 
-// One block per sequence and query head: where its tiles were more than one block's, their parts in order.
+// Block (c, row): the item that begins in block c and goes on behind it, if there is one, and one of its queries: its parts in order.
 template <typename H, int DP, int ROWS>
 __global__ void __launch_bounds__(128) paged_attention_join_kernel(Launch p) {
   constexpr int kLanes = DP / 4, kGroups = 128 / kLanes;   // four columns per thread, the parts shared out over the groups
   __shared__ __align__(16) unsigned char raw[128 * sizeof(Sums)];
   Sums* sums = reinterpret_cast<Sums*>(raw);
   const PagedAttentionArgs& a = p.a;
-  const int b = blockIdx.y, h = blockIdx.x, kv = h / p.group, in_group = h - kv * p.group;
-  const int k = kv * p.head_blocks.d + in_group / ROWS, row = in_group % ROWS;
-  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes, c0 = blockIdx.x, row = blockIdx.y;
   ::mccl::pdl_wait();
   ::mccl::pdl_trigger();
-  const unsigned per = p.plan[0], first = p.plan[1 + b], tiles = p.plan[2 + b] - first;
-  if (tiles == 0) return;
-  const unsigned s = first * p.items.d + k * tiles;
-  const int c0 = static_cast<int>(s / per), c1 = static_cast<int>((s + tiles - 1) / per);
-  if (c0 == c1) return;
+  const int2 open = p.open[c0];
+  if (open.x < 0) return;
+  const int b = p.items.of(open.x), hh = open.x - b * p.items.d, kv = p.head_blocks.of(hh), in_group = (hh - kv * p.head_blocks.d) * ROWS;
+  if (in_group + row >= p.group) return;
   Sums sum;
 #pragma unroll 4
-  for (int c = c0 + group; c <= c1; c += kGroups) {
+  for (int c = c0 + group; c <= open.y; c += kGroups) {
     const size_t slot = (static_cast<size_t>(c) * 2 + (c == c0)) * ROWS + row;
     const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
     sum.add(ml.x, ml.y, *reinterpret_cast<const float4*>(p.part_o + slot * DP + lane * 4));
@@ -671,7 +668,7 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(Launch p) {
       const Sums& other = sums[i * kLanes + lane];
       sum.add(other.m, other.l, other.o);
     }
-    store_result<H>(a, static_cast<long long>(b) * a.heads + h, lane * 4, sum);
+    store_result<H>(a, static_cast<long long>(b) * a.heads + kv * p.group + in_group + row, lane * 4, sum);
   }
 }
 
@@ -686,7 +683,7 @@ int sm_count() {
 
 int padded_dim(int d) { return d <= 32 ? 32 : (d <= 64 ? 64 : (d <= 128 ? 128 : 256)); }
 int rows_of(const PagedAttentionArgs& a) { return a.heads / a.kv_heads <= 8 ? 8 : 16; }
-size_t plan_bytes() { return (kSequences + 4) * sizeof(unsigned); }
+size_t open_bytes() { return (static_cast<size_t>(sm_count()) * sizeof(int2) + 15) / 16 * 16; }
 // Whether every item is one warp's: so short that a split would not pay for the join, a launch of its own (longest sequence that the table has room for).
 bool whole(const PagedAttentionArgs& a) { return static_cast<long long>(a.table.width) * a.table.page_size <= 64; }
 
@@ -724,7 +721,7 @@ cudaError_t launch(Launch& p, const CUtensorMap (&maps)[3], cudaStream_t stream)
   MCCL_LAUNCH_PDL((paged_attention_kernel<H, DP, KT, WARPS, STAGES, ROWS, TMA>), sm_count(), WARPS * 32, smem, stream, maps[0], maps[1], maps[2], p);
   count_launch();
   if (!p.whole) {
-    MCCL_LAUNCH_PDL((paged_attention_join_kernel<H, DP, ROWS>), dim3(p.a.heads, p.a.batch), 128, 0, stream, p);
+    MCCL_LAUNCH_PDL((paged_attention_join_kernel<H, DP, ROWS>), dim3(sm_count(), p.group < ROWS ? p.group : ROWS), 128, 0, stream, p);
     count_launch();
   }
   return ::mccl::launch_status();
@@ -751,7 +748,7 @@ cudaError_t by_size(Launch& p, int rows, const CUtensorMap (&maps)[3], cudaStrea
 
 size_t paged_attention_workspace(const PagedAttentionArgs& a) {
   if (whole(a)) return 0;
-  return plan_bytes() + static_cast<size_t>(sm_count()) * 2 * rows_of(a) * (2 + padded_dim(a.head_dim)) * sizeof(float);
+  return open_bytes() + static_cast<size_t>(sm_count()) * 2 * rows_of(a) * (2 + padded_dim(a.head_dim)) * sizeof(float);
 }
 
 cudaError_t paged_attention(const PagedAttentionArgs& args, cudaStream_t stream) {
@@ -765,8 +762,8 @@ cudaError_t paged_attention(const PagedAttentionArgs& args, cudaStream_t stream)
   p.page_blocks = Divisor(blocks ? args.table.page_size / kBlock : 1);
   p.scale_log2 = args.scale * kLog2e;
   p.whole = whole(args) ? 1 : 0;
-  p.plan = static_cast<unsigned*>(args.workspace);
-  p.part_ml = reinterpret_cast<float*>(static_cast<char*>(args.workspace) + plan_bytes());
+  p.open = static_cast<int2*>(args.workspace);
+  p.part_ml = reinterpret_cast<float*>(static_cast<char*>(args.workspace) + open_bytes());
   p.part_o = p.part_ml + static_cast<size_t>(sm_count()) * 2 * rows * 2;
   p.err = gemm_error_device_ptr();
   CUtensorMap maps[3] = {};
