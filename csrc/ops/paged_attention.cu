@@ -18,7 +18,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr int kBlock = 16;         // positions of a block: a tile is one or two, and a page that is a multiple of it comes by TMA
+constexpr int kBlock = 16;         // positions of a block: a tile is one or two
 constexpr int kLeast = 2;            // fewest tiles of a warp
 constexpr int kSequences = 1024;   // most sequences of a launch: their lengths and first tiles are kept in shared memory
 
@@ -51,7 +51,7 @@ struct Launch {
   PagedAttentionArgs a;
   int group;                    // query heads per head of keys and values
   Divisor head_blocks, items;   // blocks of 16 (or 8) that they make; items of a sequence: kv_heads * head_blocks
-  Divisor page_blocks, warps;   // page_size / 16 (1 where that is not whole); warps of the grid
+  Divisor page_boxes, warps;    // boxes of a page; warps of the grid
   int whole;                    // an item is one warp's
   float scale_log2;
   int2* open;                   // [blocks]: the item that begins in a block and goes on behind it (-1: none), and the block where it ends
@@ -126,7 +126,7 @@ __device__ __forceinline__ uint32_t swizzled(int row, int piece) {
   return static_cast<uint32_t>((piece >> 3) * (R * 128) + row * 128 + ((piece & 7) ^ (row & 7)) * 16);
 }
 
-// Box of 16 positions (or ROWS queries) x 64 (32) columns; zero fill outside the tensor, pages among it.
+// Box of BOX positions (or ROWS queries) x 64 (32) columns; zero fill outside the tensor, pages among it.
 __device__ __forceinline__ void load_pages(uint32_t to, const CUtensorMap* map, uint32_t bar, int col, int at, int head, int page) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
@@ -166,7 +166,7 @@ __device__ __forceinline__ void store_result(const PagedAttentionArgs& a, long l
   if (col == 0 && a.lse) a.lse[row] = ((s.m == -INFINITY ? 0.f : s.m) + log2f(s.l)) * kLn2;
 }
 
-template <typename H, int DP, int KT, int WARPS, int STAGES, int ROWS, bool TMA>
+template <typename H, int DP, int KT, int WARPS, int STAGES, int ROWS, int BOX>
 __global__ void __launch_bounds__(WARPS * 32, 1)
 paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap q_map, Launch p) {
   using S = Shape<DP, KT, WARPS, STAGES, ROWS>;
@@ -188,7 +188,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   const int g = lane >> 2, t4 = lane & 3;
   const int room = a.table.width * a.table.page_size;
   uint64_t* bar = bars + warp * STAGES;   // one per stage: its copies have landed
-  if (TMA && lane == 0) {
+  if (BOX > 0 && lane == 0) {
     for (int i = 0; i < STAGES; ++i) tc::mbar_init(bar + i, 1);
     tc::mbar_init_fence();
     tc::tma_prefetch_desc(&k_map);
@@ -303,23 +303,23 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       const int head0 = load_kv * p.group + load_group;
       const int tile = load.t + (load.t >= span.head ? span.skip : 0);
       const uint32_t to = ring + stage * S::kStageBytes;
-      if (TMA) {   // every block of 16 positions lies in one page
+      if (BOX > 0) {   // every box of positions lies in one page
         const int j = tile * KT + lane;
         uint32_t mask = __ballot_sync(0xffffffffu, j < span.length && (j >= span.first || j < a.sinks));
         if (KT < 32) mask &= 0xffffu;
-        int page[kSub], at[kSub];
+        constexpr int kBoxes = KT / (BOX > 0 ? BOX : KT);
+        int page[kBoxes], at[kBoxes];
 #pragma unroll
-        for (int i = 0; i < kSub; ++i) {
-          const int block = tile * kSub + i;
-          const int slot = p.page_blocks.of(block);
-          if (slot != load_slot && (i == 0 || block * kBlock < span.length)) {
+        for (int i = 0; i < kBoxes; ++i) {
+          const int box = tile * kBoxes + i, slot = p.page_boxes.of(box);
+          if (slot != load_slot && (i == 0 || box * BOX < span.length)) {
             load_slot = slot;
             load_page = __ldg(table + slot);
             if (load_page >= a.table.pages) load_page = -1;   // outside the tensor: zeros come back
           }
           page[i] = slot == load_slot ? load_page : -1;
-          at[i] = (block - slot * p.page_blocks.d) * kBlock;
-          if (page[i] < 0) mask &= ~(0xffffu << (i * kBlock));
+          at[i] = (box - slot * p.page_boxes.d) * BOX;
+          if (page[i] < 0) mask &= ~(((BOX == 32 ? 0u : 1u << (BOX & 31)) - 1u) << (i * BOX));
         }
         if (tc::elect_one()) {
           mask_ring[stage] = mask;
@@ -331,10 +331,11 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
             for (int c = 0; c < S::kBoxes; ++c) load_queries(to + 2 * S::kTileBytes + c * (ROWS * kBox * 2), &q_map, full, c * kBox, head0, load_b);
           }
 #pragma unroll
-          for (int i = 0; i < kSub; ++i)
+          for (int i = 0; i < kBoxes; ++i)
 #pragma unroll
             for (int c = 0; c < S::kBoxes; ++c) {
-              const uint32_t spot = to + i * S::kBlockBytes + c * (kBlock * kBox * 2);
+              const int row = i * BOX;
+              const uint32_t spot = to + row / kBlock * S::kBlockBytes + c * (kBlock * kBox * 2) + row % kBlock * (kBox * 2);
               load_pages(spot, &k_map, full, c * kBox, at[i], load_kv, page[i]);
               load_pages(spot + S::kTileBytes, &v_map, full, c * kBox, at[i], load_kv, page[i]);
             }
@@ -380,7 +381,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       if (--to_load > 0) settle(load, load_tiles);
       ++ahead;
     }
-    if (!TMA) copy_commit();
+    if (BOX == 0) copy_commit();
   };
 
 #pragma unroll
@@ -417,7 +418,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
     for (; at.t < stop; ++at.t) {
-      if (TMA) {
+      if (BOX > 0) {
         ok = __all_sync(0xffffffffu, tc::mbar_wait(bar + stage, parity));
         if (!ok) break;
       } else {
@@ -505,7 +506,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
           }
         // values of positions that are not seen may be anything: they are cleared, for zero times anything need not be zero
         uint32_t clear[2] = {0xffffffffu, 0xffffffffu};
-        if (TMA && ((mask >> (16 * i)) & 0xffffu) != 0xffffu) {
+        if (BOX > 0 && ((mask >> (16 * i)) & 0xffffu) != 0xffffu) {
 #pragma unroll
           for (int e = 0; e < 2; ++e)
             clear[e] = ((mask >> (16 * i + e * 8 + 2 * t4)) & 1u ? 0x0000ffffu : 0u) | ((mask >> (16 * i + e * 8 + 2 * t4 + 1)) & 1u ? 0xffff0000u : 0u);
@@ -514,7 +515,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         for (int c = 0; c < kCols; c += 2) {
           uint32_t r[4];
           load_matrix_t(r, v_tile + i * S::kBlockBytes + (c >> 3) * (kBlock * 128) + (v_lane ^ (((c >> 1) & 3) << 5)));
-          if (TMA) {
+          if (BOX > 0) {
             r[0] &= clear[0];
             r[1] &= clear[1];
             r[2] &= clear[0];
@@ -535,7 +536,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         parity ^= 1;
       }
     }
-    if (TMA && !ok) break;
+    if (BOX > 0 && !ok) break;
 
     // ---- the end of this piece: the result where it is the whole item, else its sums for the block
     const bool complete = from == 0 && at.t == tiles;
@@ -578,8 +579,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     first_piece = false;
     if (left > 0) settle(at, tiles);
   }
-  if (!TMA) copy_wait<0>();
-  if (TMA && !ok) {
+  if (BOX == 0) copy_wait<0>();
+  if (BOX > 0 && !ok) {
     if (lane == 0) atomicExch(p.err, 21);
     for (; ahead > 0; --ahead) {   // copies that were issued must land before the block retires
       tc::mbar_wait(bar + stage, parity, 1u << 20);
@@ -695,14 +696,14 @@ bool encode(CUtensorMap* map, Half16 type, int dims, const void* base, const cuu
                                  box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, box[0] < 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-// Keys or values as boxes of 16 positions of one page and head, queries as boxes of `rows` heads.  False where the strides do not fit a tensor
+// Keys or values as boxes of positions of one page and head, queries as boxes of `rows` heads.  False where the strides do not fit a tensor
 // map.  (The stride of a dimension of one is never used and may be anything.)
-bool encode_pages(CUtensorMap* map, const PagedTensor& t, const PagedAttentionArgs& a, int dp) {
+bool encode_pages(CUtensorMap* map, const PagedTensor& t, const PagedAttentionArgs& a, int dp, int positions) {
   const cuuint64_t size[4] = {static_cast<cuuint64_t>(a.head_dim), static_cast<cuuint64_t>(a.table.page_size), static_cast<cuuint64_t>(a.kv_heads),
                               static_cast<cuuint64_t>(a.table.pages)};
   const cuuint64_t strides[3] = {static_cast<cuuint64_t>(t.token * 2), static_cast<cuuint64_t>((a.kv_heads > 1 ? t.head : 8) * 2),
                                  static_cast<cuuint64_t>((a.table.pages > 1 ? t.page : 8) * 2)};
-  const cuuint32_t box[4] = {static_cast<cuuint32_t>(dp < 64 ? dp : 64), kBlock, 1, 1};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(dp < 64 ? dp : 64), static_cast<cuuint32_t>(positions), 1, 1};
   return encode(map, a.type, 4, t.p, size, strides, box);
 }
 bool encode_queries(CUtensorMap* map, const PagedAttentionArgs& a, int dp, int rows) {
@@ -712,13 +713,13 @@ bool encode_queries(CUtensorMap* map, const PagedAttentionArgs& a, int dp, int r
   return encode(map, a.type, 3, a.q.p, size, strides, box);
 }
 
-template <typename H, int DP, int KT, int WARPS, int STAGES, int ROWS, bool TMA>
+template <typename H, int DP, int KT, int WARPS, int STAGES, int ROWS, int BOX>
 cudaError_t launch(Launch& p, const CUtensorMap (&maps)[3], cudaStream_t stream) {
   constexpr int smem = Shape<DP, KT, WARPS, STAGES, ROWS>::kSmem;
-  static const cudaError_t rc = cudaFuncSetAttribute(paged_attention_kernel<H, DP, KT, WARPS, STAGES, ROWS, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static const cudaError_t rc = cudaFuncSetAttribute(paged_attention_kernel<H, DP, KT, WARPS, STAGES, ROWS, BOX>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (rc != cudaSuccess) return rc;
   p.warps = Divisor(sm_count() * WARPS);
-  MCCL_LAUNCH_PDL((paged_attention_kernel<H, DP, KT, WARPS, STAGES, ROWS, TMA>), sm_count(), WARPS * 32, smem, stream, maps[0], maps[1], maps[2], p);
+  MCCL_LAUNCH_PDL((paged_attention_kernel<H, DP, KT, WARPS, STAGES, ROWS, BOX>), sm_count(), WARPS * 32, smem, stream, maps[0], maps[1], maps[2], p);
   count_launch();
   if (!p.whole) {
     MCCL_LAUNCH_PDL((paged_attention_join_kernel<H, DP, ROWS>), dim3(sm_count(), p.group < ROWS ? p.group : ROWS), 128, 0, stream, p);
@@ -729,19 +730,24 @@ cudaError_t launch(Launch& p, const CUtensorMap (&maps)[3], cudaStream_t stream)
 
 // Sizes of tile and ring: as many warps as hide the latency of a tile's chain (scores, maximum, weights, products), two stages of 8 KB each.  More bytes in
 // flight are slower (2 x 131009 positions: three stages 181 us, two 172), fewer warps too (4 x 4 stages 191, 6 x 2 182).
-template <typename H, bool TMA>
+template <typename H, int BOX>
 cudaError_t by_size(Launch& p, int rows, const CUtensorMap (&maps)[3], cudaStream_t stream) {
   const int dp = padded_dim(p.a.head_dim);
   if (rows == 8) {
-    if (dp == 32) return launch<H, 32, 32, 8, 4, 8, TMA>(p, maps, stream);
-    if (dp == 64) return launch<H, 64, 32, 8, 2, 8, TMA>(p, maps, stream);
-    if (dp == 128) return launch<H, 128, 16, 8, 2, 8, TMA>(p, maps, stream);
-    return launch<H, 256, 16, 4, 2, 8, TMA>(p, maps, stream);
+    if (dp == 32) return launch<H, 32, 32, 8, 4, 8, BOX>(p, maps, stream);
+    if (dp == 64) return launch<H, 64, 32, 8, 2, 8, BOX>(p, maps, stream);
+    if (dp == 128) return launch<H, 128, 16, 8, 2, 8, BOX>(p, maps, stream);
+    return launch<H, 256, 16, 4, 2, 8, BOX>(p, maps, stream);
   }
-  if (dp == 32) return launch<H, 32, 32, 8, 4, 16, TMA>(p, maps, stream);
-  if (dp == 64) return launch<H, 64, 32, 8, 2, 16, TMA>(p, maps, stream);
-  if (dp == 128) return launch<H, 128, 16, 6, 2, 16, TMA>(p, maps, stream);
-  return launch<H, 256, 16, 3, 2, 16, TMA>(p, maps, stream);
+  if (dp == 32) return launch<H, 32, 32, 8, 4, 16, BOX>(p, maps, stream);
+  if (dp == 64) return launch<H, 64, 32, 8, 2, 16, BOX>(p, maps, stream);
+  if (dp == 128) return launch<H, 128, 16, 6, 2, 16, BOX>(p, maps, stream);
+  return launch<H, 256, 16, 3, 2, 16, BOX>(p, maps, stream);
+}
+
+template <typename H>
+cudaError_t by_box(Launch& p, int box, int rows, const CUtensorMap (&maps)[3], cudaStream_t stream) {
+  return box == 16 ? by_size<H, 16>(p, rows, maps, stream) : (box == 8 ? by_size<H, 8>(p, rows, maps, stream) : by_size<H, 0>(p, rows, maps, stream));
 }
 
 }  // namespace
@@ -758,8 +764,10 @@ cudaError_t paged_attention(const PagedAttentionArgs& args, cudaStream_t stream)
   const int rows = rows_of(args), dp = padded_dim(args.head_dim);
   p.head_blocks = Divisor((p.group + rows - 1) / rows);
   p.items = Divisor(args.kv_heads * p.head_blocks.d);
-  const bool blocks = args.table.page_size % kBlock == 0;
-  p.page_blocks = Divisor(blocks ? args.table.page_size / kBlock : 1);
+  // positions that are certain to lie in one page: what a TMA box may hold.  Pages of any other size come by 16-byte copies, whose addresses cost a warp some 500
+  // instructions per tile (16 ragged sequences, pages of 24: 47 us so, 38 in boxes of 8).
+  const int box = args.table.page_size % 16 == 0 ? 16 : (args.table.page_size % 8 == 0 ? 8 : 0);
+  p.page_boxes = Divisor(box > 0 ? args.table.page_size / box : 1);
   p.scale_log2 = args.scale * kLog2e;
   p.whole = whole(args) ? 1 : 0;
   p.open = static_cast<int2*>(args.workspace);
@@ -767,7 +775,7 @@ cudaError_t paged_attention(const PagedAttentionArgs& args, cudaStream_t stream)
   p.part_o = p.part_ml + static_cast<size_t>(sm_count()) * 2 * rows * 2;
   p.err = gemm_error_device_ptr();
   CUtensorMap maps[3] = {};
-  const bool paged = blocks && encode_pages(&maps[0], args.k_pages, args, dp) && encode_pages(&maps[1], args.v_pages, args, dp);
+  const bool paged = box > 0 && encode_pages(&maps[0], args.k_pages, args, dp, box) && encode_pages(&maps[1], args.v_pages, args, dp, box);
   // tiles of a launch are counted in 32 bits: as many sequences as cannot have more (a product with the blocks' number is among the sums)
   const long long most = (static_cast<long long>(args.table.width) * args.table.page_size / kBlock + 1) * p.items.d, room = 0x7f000000ll / most;
   if (room < 1) return cudaErrorInvalidValue;
@@ -781,11 +789,7 @@ cudaError_t paged_attention(const PagedAttentionArgs& args, cudaStream_t stream)
     p.a.o = static_cast<char*>(args.o) + static_cast<long long>(b) * args.heads * args.head_dim * 2;
     p.a.lse = args.lse ? args.lse + static_cast<long long>(b) * args.heads : nullptr;
     const bool tma = paged && encode_queries(&maps[2], p.a, dp, rows);
-    cudaError_t rc;
-    if (args.type == Half16::bf16)
-      rc = tma ? by_size<Bf16, true>(p, rows, maps, stream) : by_size<Bf16, false>(p, rows, maps, stream);
-    else
-      rc = tma ? by_size<Fp16, true>(p, rows, maps, stream) : by_size<Fp16, false>(p, rows, maps, stream);
+    const cudaError_t rc = args.type == Half16::bf16 ? by_box<Bf16>(p, tma ? box : 0, rows, maps, stream) : by_box<Fp16>(p, tma ? box : 0, rows, maps, stream);
     if (rc != cudaSuccess) return rc;
   }
   return cudaSuccess;
