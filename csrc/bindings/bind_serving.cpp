@@ -298,6 +298,32 @@ void bind_serving(py::module_& m) {
       py::arg("gelu") = false, py::arg("residual") = py::none());
 
   m.def(
+      "w4_pack",
+      [](const at::Tensor& codes, const at::Tensor& scales, const c10::optional<at::Tensor>& zeros) {
+        const char* op = "w4_pack";
+        need_on(codes, codes, op);
+        need_on(scales, codes, op);
+        MCCL_CHECK_TENSOR(codes.scalar_type() == at::kByte && codes.dim() == 2 && codes.is_contiguous(), op << ": codes must be contiguous uint8 [n, k]");
+        const int64_t n = codes.size(0), k = codes.size(1);
+        MCCL_CHECK_TENSOR(scales.scalar_type() == at::kBFloat16 && scales.dim() == 2 && scales.is_contiguous() && scales.size(0) == n && scales.size(1) > 0 && k % scales.size(1) == 0 &&
+                              k / scales.size(1) % 32 == 0,
+                          op << ": scales must be contiguous bf16 [n, groups]");
+        if (zeros.has_value()) {
+          need_on(*zeros, codes, op);
+          MCCL_CHECK_TENSOR(zeros->scalar_type() == at::kByte && zeros->is_contiguous() && zeros->sizes() == scales.sizes(), op << ": zeros must be contiguous uint8 of the scales' shape");
+        }
+        c10::cuda::CUDAGuard guard(codes.device());
+        const int64_t tiles = (n + 15) / 16;
+        at::Tensor packed = empty_on(codes, {tiles, (k + 63) / 64, 32, 16}, at::kByte), params = empty_on(codes, {tiles, scales.size(1), 8, 2}, at::kInt);
+        at::Tensor bad = at::zeros({1}, codes.options().dtype(at::kInt));
+        check_launch(ops::w4_pack(codes.data_ptr<uint8_t>(), scales.data_ptr(), zeros.has_value() ? zeros->data_ptr<uint8_t>() : nullptr, packed.data_ptr(), params.data_ptr(),
+                                  bad.data_ptr<int>(), as_int(n, op), as_int(k, op), as_int(k / scales.size(1), op), stream_of(codes)),
+                     op);
+        return std::make_tuple(packed, params, bad);
+      },
+      py::arg("codes"), py::arg("scales"), py::arg("zeros") = py::none());
+
+  m.def(
       "w4_dequantize",
       [](const at::Tensor& codes, const at::Tensor& params, int64_t n, int64_t k, int64_t group) {
         need_on(codes, codes, "w4_dequantize");

@@ -816,6 +816,48 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(const uint4* __restr
   }
 }
 
+// A warp per tile of 16 x 64, a lane its 16 bytes; behind the tiles, a thread per row and group of the parameters.  (k is even: two neighbouring codes are one access.)
+__global__ void __launch_bounds__(256) w4_pack_kernel(const uint8_t* __restrict__ codes, const uint16_t* __restrict__ scales, const uint8_t* __restrict__ zeros, uint4* __restrict__ packed,
+                                                      uint32_t* __restrict__ params, int* bad, int n, int k, int group) {
+  ::mccl::pdl_wait();
+  ::mccl::pdl_trigger();
+  const int chunks = (k + 63) / 64, groups = k / group, tiles = (n + 15) / 16;
+  const long long pieces = static_cast<long long>(tiles) * chunks * 32, entries = static_cast<long long>(tiles) * groups * 16;
+  uint32_t seen = 0;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < pieces + entries; i += gridDim.x * 256ll) {
+    if (i < pieces) {
+      const int lane = static_cast<int>(i & 31), g = lane >> 2, t = lane & 3;
+      const long long at = i >> 5;
+      const int tile = static_cast<int>(at / chunks), c = static_cast<int>(at - static_cast<long long>(tile) * chunks);
+      uint32_t word[4] = {};
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {   // row g + 8 (j & 1), columns 8 (j >> 1) on
+          const int row = tile * 16 + g + 8 * (j & 1), col = c * 64 + 16 * s + 8 * (j >> 1) + 2 * t;
+          if (row < n && col < k) {
+            const uint32_t two = *reinterpret_cast<const uint16_t*>(codes + static_cast<size_t>(row) * k + col);
+            seen |= two;
+            word[s] |= ((two & 15u) | (two & 0xf00u) << 8) << (4 * j);
+          }
+        }
+      packed[i] = make_uint4(word[0], word[1], word[2], word[3]);
+    } else {
+      const long long e = i - pieces, at = e >> 4;   // [tile][group][8 g][2]
+      const int tile = static_cast<int>(at / groups), group_at = static_cast<int>(at - static_cast<long long>(tile) * groups), row = tile * 16 + static_cast<int>(e >> 1 & 7) + 8 * static_cast<int>(e & 1);
+      uint32_t v = 0x43000000u;
+      if (row < n) {
+        const size_t from = static_cast<size_t>(row) * groups + group_at;
+        const uint32_t zero = zeros ? zeros[from] : 8u;
+        seen |= zero;
+        v = scales[from] | (0x4300u + (zero & 15u)) << 16;
+      }
+      params[e] = v;
+    }
+  }
+  if ((seen & 0xf0f0u) != 0) *bad = 1;
+}
+
 int sm_count() {
   static const int n = [] {
     int device = 0, sms = 148;
@@ -985,6 +1027,15 @@ cudaError_t w4_linear(const W4Args& a, cudaStream_t stream) {
     return narrow<1, 2>(a, stream);
   }
   return launch_wide(a, stream);
+}
+
+cudaError_t w4_pack(const uint8_t* codes, const void* scales, const uint8_t* zeros, void* packed, void* params, int* bad, int n, int k, int group, cudaStream_t stream) {
+  if (n <= 0 || k <= 0) return cudaSuccess;
+  const long long tiles = (n + 15) / 16, all = tiles * ((k + 63) / 64) * 32 + tiles * (k / group) * 16, blocks = (all + 255) / 256;
+  MCCL_LAUNCH_PDL(w4_pack_kernel, static_cast<unsigned>(blocks < 148 * 16 ? blocks : 148 * 16), 256, 0, stream, codes, static_cast<const uint16_t*>(scales), zeros,
+                  static_cast<uint4*>(packed), static_cast<uint32_t*>(params), bad, n, k, group);
+  count_launch();
+  return ::mccl::launch_status();
 }
 
 cudaError_t w4_dequantize(const void* codes, const void* params, void* w, int n, int k, int group, cudaStream_t stream) {

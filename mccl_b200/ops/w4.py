@@ -56,8 +56,14 @@ class W4Weight:
             raise RuntimeError("W4Weight: zeros must be uint8 of the scales' shape")
         if any(t is not None and t.device != codes.device for t in (scales, zeros)):
             raise RuntimeError("W4Weight: codes, scales and zeros on different devices")
-        if codes.numel() and (int(codes.max()) > 15 or (zeros is not None and int(zeros.max()) > 15)):
+        if codes.is_cuda:
+            packed, params, bad = _C.w4_pack(codes.contiguous(), scales.to(torch.bfloat16).contiguous(), None if zeros is None else zeros.contiguous())
+        else:
+            bad = codes.numel() and (int(codes.max()) > 15 or (zeros is not None and int(zeros.max()) > 15))
+        if bad:
             raise RuntimeError("W4Weight: codes and zeros are numbers from 0 to 15")
+        if codes.is_cuda:
+            return cls(packed, params, n, k, group)
         tiles, chunks = -(-n // 16), -(-k // 64)
         padded = F.pad(codes, (0, chunks * 64 - k, 0, tiles * 16 - n)) if (n % 16 or k % 64) else codes
         # rows: 8 r + g; columns of a chunk: 16 s + 8 q + 2 t + e.  Nibble 4 e + 2 q + r of word s.
@@ -65,7 +71,7 @@ class W4Weight:
         packed = c[:, 0] | (c[:, 1] << 4)                                       # [tile, g, chunk, s, q, t, e]
         packed = packed.permute(0, 2, 1, 5, 3, 6, 4).reshape(tiles, chunks, 32, 16).contiguous()
         scale = F.pad(scales.to(torch.bfloat16), (0, 0, 0, tiles * 16 - n)).view(torch.int16).to(torch.int32) & 0xffff
-        zero = torch.full_like(scale, 8) if zeros is None else F.pad(zeros.to(torch.int32), (0, 0, 0, tiles * 16 - n))
+        zero = F.pad(torch.full_like(scale[:n], 8) if zeros is None else zeros.to(torch.int32), (0, 0, 0, tiles * 16 - n))
         params = scale | ((zero + 0x4300) << 16)                                # bf16 128 is 0x4300, and its last bit is worth one
         params = params.view(tiles, 2, 8, groups).permute(0, 3, 2, 1).contiguous()
         return cls(packed, params, n, k, group)

@@ -114,6 +114,22 @@ def test_the_same_bits_again_and_on_another_stream():
         assert all(torch.equal(g, want) for g in got)
 
 
+@pytest.mark.parametrize("n,k,group", [(1, 32, 32), (17, 96, 32), (16, 64, 64), (100, 256, 256), (130, 1088, 64)])
+@pytest.mark.parametrize("zeros", [True, False])
+def test_layout_is_the_same_on_both_devices(n, k, group, zeros):
+    g = torch.Generator().manual_seed(n)
+    codes, scales = torch.randint(0, 16, (n, k), generator=g, dtype=torch.uint8), torch.randn(n, k // group, generator=g)
+    z = torch.randint(0, 16, (n, k // group), generator=g, dtype=torch.uint8) if zeros else None
+    cpu = ops.W4Weight.from_codes(codes, scales, z)
+    gpu = ops.W4Weight.from_codes(codes.cuda(), scales.cuda(), None if z is None else z.cuda())
+    assert torch.equal(cpu.codes, gpu.codes.cpu()) and torch.equal(cpu.params, gpu.params.cpu())
+    apart = ops.W4Weight.from_codes(codes.t().contiguous().cuda().t(), scales.cuda(), None if z is None else z.cuda())
+    assert torch.equal(apart.codes, gpu.codes)
+    for bad_codes, bad_zeros in ((codes.clone().index_fill_(1, torch.tensor([k - 1]), 16), z), (codes, torch.full((n, k // group), 200, dtype=torch.uint8))):
+        with pytest.raises(RuntimeError, match="0 to 15"):
+            ops.W4Weight.from_codes(bad_codes.cuda(), scales.cuda(), None if bad_zeros is None else bad_zeros.cuda())
+
+
 def test_quantize():
     w = torch.randn(130, 256, device="cuda") * 0.02
     w[3] = 0.0
