@@ -9,6 +9,7 @@
 #include "half16.cuh"
 #include "ops.hpp"
 #include "serving.hpp"
+#include "smem_limit.hpp"
 #include "tcgen05.cuh"
 
 namespace mccl {
@@ -729,7 +730,8 @@ bool encode_queries(CUtensorMap* map, const PagedAttentionArgs& a, int dp, int r
 template <typename H, int DP, int KT, int WARPS, int STAGES, int ROWS, int BOX>
 cudaError_t launch(Launch& p, const CUtensorMap (&maps)[3], cudaStream_t stream) {
   constexpr int smem = Shape<DP, KT, WARPS, STAGES, ROWS>::kSmem;
-  static const cudaError_t rc = cudaFuncSetAttribute(paged_attention_kernel<H, DP, KT, WARPS, STAGES, ROWS, BOX>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<uint64_t> allowed{0};
+  const cudaError_t rc = raise_smem_limit(paged_attention_kernel<H, DP, KT, WARPS, STAGES, ROWS, BOX>, smem, allowed);
   if (rc != cudaSuccess) return rc;
   p.warps = Divisor(sm_count() * WARPS);
   MCCL_LAUNCH_PDL((paged_attention_kernel<H, DP, KT, WARPS, STAGES, ROWS, BOX>), sm_count(), WARPS * 32, smem, stream, maps[0], maps[1], maps[2], p);

@@ -12,6 +12,7 @@
 #include "gemm_common.cuh"
 #include "ops.hpp"
 #include "serving.hpp"
+#include "smem_limit.hpp"
 #include "tcgen05.cuh"
 
 namespace mccl {
@@ -875,7 +876,8 @@ int log2_of(int v) {
 
 template <int kR, int kN, int kParams, bool kEven>
 cudaError_t launch_narrow(const W4Args& a, cudaStream_t stream) {
-  static const cudaError_t rc = cudaFuncSetAttribute(w4_narrow_kernel<kR, kN, kParams, kEven>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+  static std::atomic<uint64_t> allowed{0};
+  const cudaError_t rc = raise_smem_limit(w4_narrow_kernel<kR, kN, kParams, kEven>, 227 * 1024, allowed);
   if (rc != cudaSuccess) return rc;
   const int chunks = (a.k + 63) / 64, smem = narrow_smem<kR, kN, kParams>(a.m, (chunks + 1) / 2);
   if (smem > 227 * 1024) return cudaErrorNotSupported;
@@ -975,7 +977,8 @@ bool choose_wide(int m, int blocks, Wide& p) {
 
 template <bool kG32>
 cudaError_t start_wide(const Wide& p, dim3 grid, const CUtensorMap& map, cudaStream_t stream) {
-  static const cudaError_t rc = cudaFuncSetAttribute(w4_wide_kernel<kG32>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem);
+  static std::atomic<uint64_t> allowed{0};
+  const cudaError_t rc = raise_smem_limit(w4_wide_kernel<kG32>, kWideSmem, allowed);
   if (rc != cudaSuccess) return rc;
   MCCL_LAUNCH_PDL_CLUSTER(w4_wide_kernel<kG32>, grid, kWideThreads, wide_smem(p), stream, static_cast<unsigned>(p.splits), map, p);
   count_launch();
@@ -984,7 +987,8 @@ cudaError_t start_wide(const Wide& p, dim3 grid, const CUtensorMap& map, cudaStr
 
 template <bool kG32>
 cudaError_t start_stream(const Wide& p, const CUtensorMap& map, cudaStream_t stream) {
-  static const cudaError_t rc = cudaFuncSetAttribute(w4_stream_kernel<kG32>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem);
+  static std::atomic<uint64_t> allowed{0};
+  const cudaError_t rc = raise_smem_limit(w4_stream_kernel<kG32>, kWideSmem, allowed);
   if (rc != cudaSuccess) return rc;
   MCCL_LAUNCH_PDL(w4_stream_kernel<kG32>, p.tiles < sm_count() ? p.tiles : sm_count(), kStreamThreads, stream_smem(p.tokens), stream, map, p);
   count_launch();

@@ -65,12 +65,13 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     a longer attention can be joined."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
-    if window is not None and window < 1:
+    if window is None:
+        if sinks:
+            raise RuntimeError("paged_attention: sinks without a window")
+    elif window < 1:
         raise RuntimeError(f"paged_attention: window must be positive, got {window}")
-    if sinks and window is None:
-        raise RuntimeError("paged_attention: sinks without a window")
     if q.is_cuda:
-        o, lse = _C.paged_attention(q, k_pages, v_pages, page_table, lengths, scale, window or 0, sinks, return_lse)
+        o, lse = _C.paged_attention(q, k_pages, v_pages, page_table, lengths, scale, 0 if window is None else window, sinks, return_lse)
         return (o, lse) if return_lse else o
     batch, heads, dim = q.shape
     kv_heads, page = k_pages.shape[1], k_pages.shape[2]
