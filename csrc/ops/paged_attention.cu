@@ -2,6 +2,16 @@
 //
 // The formula, for one sequence and head with query q: o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m), s_j = scale q . k_j over the visible
 // positions j and m their maximum.  Sums over any split of the positions join exactly: parts (m, l, o) combine with weights exp(m_part - m).
+//
+// Every key and value is read once and used for the query heads that share it, at most 8 multiply-adds per byte: memory bounds it.  So all tiles of all
+// sequences and heads are counted through and every warp of one block per SM streams an equal run of them, whatever the lengths are, through a ring of its
+// own that no other warp waits for.  The pieces that a run leaves of an item at its two ends are joined in shared memory, what crosses a block's bounds by a
+// second small kernel; everything is added in the order of the positions, so results repeat bit for bit.  Scores and weighted sums are m16n8k16 products:
+// eight heads that share keys fill half of their rows, single ones an eighth, and still they run at a quarter of their rate, while the generation's own
+// instruction would want 64 rows.
+// Measured: 2 x 131009 positions, 32 heads over 8 of 128 (1071 MB): 165 us, 6.5 TB/s; 64 ragged sequences of up to 2048, 16 heads of 128 (540 MB): 87 us, 6.2
+// TB/s; 48 windows of 1024 (101 MB): 25.5 us, of which 15.6 from the first load's issue to the last tile: the rest is finding the run (1.8), joining (1.6) and the second
+// kernel with its start (3.5); one sequence of 37 tokens: 5.0 us, a chain of four dependent loads.
 #include "../core/launch.hpp"
 #include "../symm/cu_driver.hpp"
 #include "divisor.cuh"
@@ -20,7 +30,7 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kBlock = 16;         // positions of a block: a tile is one or two
-constexpr int kLeast = 2;            // fewest tiles of a warp
+constexpr int kLeast = 2;          // fewest tiles of a warp
 constexpr int kSequences = 1024;   // most sequences of a launch: their lengths and first tiles are kept in shared memory
 
 // What a sequence's visible positions are in tiles of KT: tile t of `tiles` is the one of positions KT * (t + (t >= head ? skip : 0)) and on.
@@ -699,8 +709,9 @@ int sm_count() {
 int padded_dim(int d) { return d <= 32 ? 32 : (d <= 64 ? 64 : (d <= 128 ? 128 : 256)); }
 int rows_of(const PagedAttentionArgs& a) { return a.heads / a.kv_heads <= 8 ? 8 : 16; }
 size_t open_bytes() { return (static_cast<size_t>(sm_count()) * sizeof(int2) + 15) / 16 * 16; }
-// Whether every item is one warp's: so short that a split would not pay for the join, a launch of its own (longest sequence that the table has room for).
-bool whole(const PagedAttentionArgs& a) { return static_cast<long long>(a.table.width) * a.table.page_size <= 64; }
+// Whether every item is one warp's: so short that a split would not pay for the join, a launch of its own.  Longest sequences that the table has room for, 64
+// limit / 128 / 256: 16 x 8 heads of 64 up to 128 positions 9.2 / 7.7 / 7.6 us, 32 x 8 up to 256 9.3 / 9.3 / 12.2, 256 x 12 up to 256 28.7 / 28.5 / 33.5.
+bool whole(const PagedAttentionArgs& a) { return static_cast<long long>(a.table.width) * a.table.page_size <= 128; }
 
 bool encode(CUtensorMap* map, Half16 type, int dims, const void* base, const cuuint64_t* size, const cuuint64_t* strides, const cuuint32_t* box) {
   const CuDriver& cu = CuDriver::get();
