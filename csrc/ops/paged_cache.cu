@@ -15,8 +15,7 @@ constexpr int kThreads = 256;
 
 // Four (even, odd) pairs rotated.  Products are rounded before they are added, as the training path's rotation does, so a key in the
 // cache has the bits of the key that scoring the whole text would use.
-__device__ __forceinline__ void rotate_pairs(float (&f)[8], const float* cos_row, const float* sin_row) {
-  const float4 c = __ldg(reinterpret_cast<const float4*>(cos_row)), s = __ldg(reinterpret_cast<const float4*>(sin_row));
+__device__ __forceinline__ void rotate_pairs(float (&f)[8], const float4& c, const float4& s) {
   const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -26,58 +25,70 @@ __device__ __forceinline__ void rotate_pairs(float (&f)[8], const float* cos_row
   }
 }
 
-// A unit is 8 elements of one head of one token: the token's units are k's, v's and, where q is rotated, q's.  A block has one token of many units, or as many
-// tokens as it has threads for, so a thread has one token and follows its place (position, row, page) once; its loads are all under way before the first
-// result.  1537 tokens of 48 heads of 128, 38 MB: 12.4 us with a unit at a time, 11.0 us so (5.8 at the rate of a copy).
+// A token's heads are k's, v's and, where q is rotated, q's.  A thread has eight elements of a head, the same eight of every `rows`-th head of one token: it
+// follows the token's place (position, row, page), takes its part of the rotation and works out addresses once, and its loads are all under way before
+// the first result.  A block has one token, or as many as it has threads for.  64 tokens of 48 heads of 128: 2.6 us (3.2 with a place per 16 bytes), 1537 of
+// them, 38 MB: 11.0 us (12.4), of which 2.5 are the launch: 4.5 TB/s.  (Blocks that go from token to token and look two places ahead: 2.9 and 10.8 us.)
 template <typename H>
-__global__ void __launch_bounds__(kThreads) paged_append_kernel(AppendArgs a, int per_block, Divisor units, Divisor kv_units, Divisor hd8) {
+__global__ void __launch_bounds__(kThreads) paged_append_kernel(AppendArgs a, int per_block, int rows, int all_heads, Divisor by_heads, Divisor by_hd8) {
   constexpr int kDeep = 4;
   ::mccl::pdl_wait();
   ::mccl::pdl_trigger();
-  const int in_block = units.of(threadIdx.x);   // zero where a token's units are more than the threads
+  const int at_row = by_hd8.of(threadIdx.x), d8 = threadIdx.x - at_row * by_hd8.d;
+  const int in_block = per_block > 1 ? by_heads.of(at_row) : 0;
   const long long t = static_cast<long long>(blockIdx.x) * per_block + in_block;
-  if (in_block >= per_block || t >= a.tokens) return;
-  using V = uint4;
-  auto source = [&](int u) -> const V* {
-    const int part = kv_units.of(u), r = u - (part > 2 ? 2 : part) * kv_units.d, h = hd8.of(r);
-    const TokenView& from = part == 0 ? a.k : (part == 1 ? a.v : a.q);
-    return reinterpret_cast<const V*>(static_cast<const typename H::T*>(from.p) + t * from.token + h * from.head) + (r - h * hd8.d);
-  };
+  if (at_row >= rows || in_block >= per_block || t >= a.tokens) return;
+  using T = typename H::T;
+  const int kv = a.kv_heads;
+  const T* k = static_cast<const T*>(a.k.p) + t * a.k.token + d8 * 8;
+  const T* v = static_cast<const T*>(a.v.p) + t * a.v.token + d8 * 8;
+  const T* q = static_cast<const T*>(a.q.p) + t * a.q.token + d8 * 8;
   const int pos = __ldg(a.positions + t), row = a.rows ? __ldg(a.rows + t) : static_cast<int>(t);
   const int ps = a.table.page_size, slot = pos >= 0 ? pos / ps : 0;
   const bool inside = pos >= 0 && row >= 0 && row < a.table.rows && slot < a.table.width && (a.cos == nullptr || pos < a.rope_rows);
   int page = -1;
-  if (inside) page = __ldg(a.table.p + row * a.table.stride + slot);
+  float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (inside) {
+    page = __ldg(a.table.p + row * a.table.stride + slot);
+    if (a.cos != nullptr) {
+      const size_t at = (static_cast<size_t>(pos) * by_hd8.d + d8) * 4;
+      c = __ldg(reinterpret_cast<const float4*>(a.cos + at));
+      s = __ldg(reinterpret_cast<const float4*>(a.sin + at));
+    }
+  }
   const bool good = page >= 0 && page < a.table.pages;
-  for (int u0 = threadIdx.x - in_block * units.d; u0 < static_cast<int>(units.d); u0 += kThreads * kDeep) {
-    V raw[kDeep];
-#pragma unroll
-    for (int i = 0; i < kDeep; ++i)
-      if (u0 + i * kThreads < static_cast<int>(units.d)) raw[i] = __ldg(source(u0 + i * kThreads));
+  const long long place = static_cast<long long>(good ? page : 0), at = good ? pos - slot * ps : 0;
+  T* to_k = static_cast<T*>(a.k_pages.p) + place * a.k_pages.page + at * a.k_pages.token + d8 * 8;
+  T* to_v = static_cast<T*>(a.v_pages.p) + place * a.v_pages.page + at * a.v_pages.token + d8 * 8;
+  T* to_q = static_cast<T*>(a.q_out) + t * a.heads * a.head_dim + d8 * 8;
+  for (int h0 = at_row - in_block * all_heads; h0 < all_heads; h0 += kDeep * rows) {
+    uint4 raw[kDeep];
 #pragma unroll
     for (int i = 0; i < kDeep; ++i) {
-      const int u = u0 + i * kThreads;
-      if (u >= static_cast<int>(units.d)) break;
-      const int part = min(static_cast<int>(kv_units.of(u)), 2), r = u - part * kv_units.d, h = hd8.of(r), d8 = r - h * hd8.d;
-      if (a.cos != nullptr && part != 1 && good) {
+      const int h = h0 + i * rows;
+      if (h < all_heads) raw[i] = __ldg(reinterpret_cast<const uint4*>(h < kv ? k + h * a.k.head : (h < 2 * kv ? v + (h - kv) * a.v.head : q + (h - 2 * kv) * a.q.head)));
+    }
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i) {
+      const int h = h0 + i * rows;
+      if (h >= all_heads) break;
+      const bool value = h >= kv && h < 2 * kv;
+      if (a.cos != nullptr && !value) {
         float f[8];
         unpack8_as<H>(raw[i], f);
-        const size_t at = (static_cast<size_t>(pos) * hd8.d + d8) * 4;
-        rotate_pairs(f, a.cos + at, a.sin + at);
+        rotate_pairs(f, c, s);
         raw[i] = pack8_as<H>(f);
       }
-      if (part == 2) {
-        if (!good) raw[i] = make_uint4(0, 0, 0, 0);
-        reinterpret_cast<V*>(static_cast<typename H::T*>(a.q_out) + t * a.heads * a.head_dim)[r] = raw[i];
-      } else if (good) {
-        const PagedTensor& to = part == 0 ? a.k_pages : a.v_pages;
-        reinterpret_cast<V*>(static_cast<typename H::T*>(to.p) + page * to.page + h * to.head + (pos - slot * ps) * to.token)[d8] = raw[i];
-      }
+      if (h >= 2 * kv)
+        *reinterpret_cast<uint4*>(to_q + (h - 2 * kv) * static_cast<long long>(a.head_dim)) = good ? raw[i] : make_uint4(0, 0, 0, 0);
+      else if (good)
+        *reinterpret_cast<uint4*>(value ? to_v + (h - kv) * a.v_pages.head : to_k + h * a.k_pages.head) = raw[i];
     }
   }
 }
 
-// Block (x, y): piece x of the pages, pairs y, y + gridDim.y, ... of outer index and copy.  Four accesses in flight per thread.
+// Block (x, y): piece x of the pages, pairs y, y + gridDim.y, ... of outer index and copy.  Four accesses in flight per thread.  61 pages of 12 layers of 16 heads
+// of 128 (384 MB read and written): 115 us, 6.7 TB/s, the rate of a plain copy.
 template <typename V>
 __global__ void __launch_bounds__(kThreads) copy_pages_kernel(char* base, long long outer_stride, long long page_stride, long long words, int pages,
                                                               const int* __restrict__ src, const int* __restrict__ dst, long long count, long long pairs) {
@@ -117,16 +128,16 @@ cudaError_t launch_copy(void* base, long long outer, long long outer_stride, lon
 
 cudaError_t paged_append(const AppendArgs& a, cudaStream_t stream) {
   if (a.tokens <= 0) return cudaSuccess;
-  const int units = (2 * a.kv_heads + (a.q_out ? a.heads : 0)) * (a.head_dim / 8);
-  if (units <= 0) return cudaSuccess;
-  const int per_block = units < kThreads ? kThreads / units : 1;
+  const int hd8 = a.head_dim / 8, all_heads = 2 * a.kv_heads + (a.q_out ? a.heads : 0);
+  if (hd8 <= 0 || all_heads <= 0) return cudaSuccess;
+  if (hd8 > kThreads) return cudaErrorNotSupported;
+  const int rows = kThreads / hd8, per_block = all_heads < rows ? rows / all_heads : 1;
   const long long blocks = (a.tokens + per_block - 1) / per_block;
   if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
-  const Divisor by_units(units), by_kv(a.kv_heads * (a.head_dim / 8)), by_hd8(a.head_dim / 8);
   if (a.type == Half16::bf16)
-    MCCL_LAUNCH_PDL(paged_append_kernel<Bf16>, static_cast<unsigned>(blocks), kThreads, 0, stream, a, per_block, by_units, by_kv, by_hd8);
+    MCCL_LAUNCH_PDL(paged_append_kernel<Bf16>, static_cast<unsigned>(blocks), kThreads, 0, stream, a, per_block, rows, all_heads, Divisor(all_heads), Divisor(hd8));
   else
-    MCCL_LAUNCH_PDL(paged_append_kernel<Fp16>, static_cast<unsigned>(blocks), kThreads, 0, stream, a, per_block, by_units, by_kv, by_hd8);
+    MCCL_LAUNCH_PDL(paged_append_kernel<Fp16>, static_cast<unsigned>(blocks), kThreads, 0, stream, a, per_block, rows, all_heads, Divisor(all_heads), Divisor(hd8));
   count_launch();
   return ::mccl::launch_status();
 }
