@@ -274,6 +274,23 @@ struct Wide {
   int* err;
 };
 
+// Bounded wait that leaves the issue slots to others: a poll may sleep for two microseconds, or until the phase ends (a third of the stream kernel's instructions were
+// polls without that).  Some two seconds in all.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity) {
+  const uint32_t at = tc::smem_u32(bar);
+  for (int i = 0; i < (1 << 20); ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(at), "r"(parity), "r"(2000)
+        : "memory");
+    if (done) return true;
+  }
+  return false;
+}
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_cols, uint64_t desc_b, uint32_t idesc, bool accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
@@ -384,7 +401,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) w4_wide_kernel(const __grid_c
     if (tc::elect_one()) {
       int c = first, s = 0, round = 0;
       for (; c < last; ++c) {
-        if (round > 0 && !tc::mbar_wait(empty + s, (round - 1) & 1)) {
+        if (round > 0 && !wait_for(empty + s, (round - 1) & 1)) {
           bad = 1;
           break;
         }
@@ -407,7 +424,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) w4_wide_kernel(const __grid_c
 #pragma unroll
         for (int s = 0; s < kWideStages; ++s, db += stage_step) {
           if (c == last) break;
-          if (!tc::mbar_wait(full + s, parity)) {
+          if (!wait_for(full + s, parity)) {
             bad = 1;
             break;
           }
@@ -476,7 +493,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) w4_wide_kernel(const __grid_c
       uint32_t r[2][16];
 #pragma unroll
       for (int k = 0; k < 2; ++k) make_weights<kG32>(r[k], w[k], prm[k]);
-      const bool ok = c - first < kWideStages || tc::mbar_wait(empty + turn, parity);
+      const bool ok = c - first < kWideStages || wait_for(empty + turn, parity);
       if (!__all_sync(0xffffffffu, ok)) {
         if (lane == 0) bad = 1;
         break;
@@ -501,7 +518,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) w4_wide_kernel(const __grid_c
   const int n4 = blockIdx.x * kWideRows + lane * 4, token0 = blockIdx.y * p.tokens;
   float bias[4];
   load_bias(bias, a, n4);
-  const bool ok = tc::mbar_wait(&done, 0);
+  const bool ok = wait_for(&done, 0);
   tc::fence_after_sync();
   __syncwarp();
   // [part][row of x][weight row]: where x was, or behind everything else where other blocks write too
@@ -609,7 +626,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) w4_stream_kernel(const __gr
       for (int tile = blockIdx.x; tile < p.tiles && !bad; tile += gridDim.x) {
         const int row0 = tile % p.row_tiles * p.tokens;
         for (int c = 0; c < p.chunks; ++c, ++issued) {
-          if (issued >= kWideStages && !tc::mbar_wait(empty + s, parity)) {
+          if (issued >= kWideStages && !wait_for(empty + s, parity)) {
             bad = 1;
             break;
           }
@@ -628,14 +645,14 @@ __global__ void __launch_bounds__(kStreamThreads, 1) w4_stream_kernel(const __gr
       int s = 0, i = 0;
       uint32_t parity = 0;
       for (int tile = blockIdx.x; tile < p.tiles && !bad; tile += gridDim.x, ++i) {
-        if (i >= 2 && !tc::mbar_wait(sums_empty + (i & 1), ((i >> 1) - 1) & 1)) {
+        if (i >= 2 && !wait_for(sums_empty + (i & 1), ((i >> 1) - 1) & 1)) {
           bad = 1;
           break;
         }
         tc::fence_after_sync();
         const uint32_t sums = tmem + (i & 1) * kStreamTokens;
         for (int c = 0; c < p.chunks; ++c) {
-          if (!tc::mbar_wait(full + s, parity)) {
+          if (!wait_for(full + s, parity)) {
             bad = 1;
             break;
           }
@@ -721,7 +738,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) w4_stream_kernel(const __gr
       uint32_t r[2][16];
 #pragma unroll
       for (int k = 0; k < 2; ++k) make_weights<kG32>(r[k], w[k], prm[k]);
-      const bool ok = !used || tc::mbar_wait(empty + turn, parity);
+      const bool ok = !used || wait_for(empty + turn, parity);
       if (!__all_sync(0xffffffffu, ok)) {
         if (lane == 0) bad = 1;
         break;
@@ -752,7 +769,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) w4_stream_kernel(const __gr
       const int block = tile / p.row_tiles, row0 = (tile - block * p.row_tiles) * p.tokens, n4 = block * kWideRows + lane * 4;
       float bias[4];
       load_bias(bias, a, n4);
-      if (!__all_sync(0xffffffffu, tc::mbar_wait(sums_full + (i & 1), (i >> 1) & 1)) && lane == 0) lost = 1;
+      if (!__all_sync(0xffffffffu, wait_for(sums_full + (i & 1), (i >> 1) & 1)) && lane == 0) lost = 1;
       asm volatile("bar.sync 1, 128;" ::: "memory");   // these four warps: they leave together or not at all
       if (lost) {
         bad = 1;
