@@ -257,8 +257,13 @@ constexpr int kWideRows = 128;             // weight rows of a block: the lanes 
 constexpr int kTurns = 4;
 constexpr int kWideThreads = (2 + 4 * kTurns) * 32;
 constexpr int kWideStages = 4;
-constexpr int kCodeDeep = 6;               // chunks that a weight-making warp has on their way
-constexpr int kCodeRing = 4 * kTurns * kCodeDeep * 2 * 512;
+// A weight-making warp copies the codes and parameters of its two tiles ahead, each lane its own: so many chunks are on their way (3 KB or 4 KB each, 96 KB of all).
+template <bool kG32>
+constexpr int kCodeTile = 512 + (kG32 ? 512 : 256);
+template <bool kG32>
+constexpr int kCodeDeep = kG32 ? 3 : 4;
+constexpr int kCodeRing = 4 * kTurns * 2 * kCodeDeep<false> * kCodeTile<false>;
+static_assert(kCodeRing == 4 * kTurns * 2 * kCodeDeep<true> * kCodeTile<true>);
 constexpr int kWideSmem = 226 * 1024;      // the rest is for the barriers
 constexpr int kMostTokens = 256;           // rows of x of a block
 
@@ -320,6 +325,28 @@ __device__ __forceinline__ void store_peer(uint32_t at, int rank, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there), "f"(v) : "memory");
 }
 
+// A lane's codes and parameters of chunk c of a tile to `to` and 512 bytes on; zeros of a tile that there is not.
+template <bool kG32>
+__device__ __forceinline__ void copy_tile(uint32_t to, int lane, const uint4* codes, const uint2* params, int c, int group_shift, int groups, bool there) {
+  copy_async<16>(to + lane * 16, codes + c * 32, there);
+  if (kG32) {
+    copy_async<8>(to + 512 + lane * 16, params + 2 * c * 8, there);
+    copy_async<8>(to + 520 + lane * 16, params + min(2 * c + 1, groups - 1) * 8, there);
+  } else {
+    copy_async<8>(to + 512 + lane * 8, params + (c * 64 >> group_shift) * 8, there);
+  }
+}
+template <bool kG32>
+__device__ __forceinline__ void take_tile(uint32_t from, int lane, uint4& codes, uint2 (&params)[2]) {
+  codes = shared16(from + lane * 16);
+  if (kG32) {
+    const uint4 both = shared16(from + 512 + lane * 16);
+    params[0] = make_uint2(both.x, both.y);
+    params[1] = make_uint2(both.z, both.w);
+  } else {
+    params[0] = shared8(from + 512 + lane * 8);
+  }
+}
 // A lane's part of 16 x 64 weights for tmem_st_16x64, rounded to bf16 once: scale times whole number.
 template <bool kG32>
 __device__ __forceinline__ void make_weights(uint32_t (&r)[16], const uint4& w, const uint2 (&prm)[2]) {
@@ -448,7 +475,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) w4_wide_kernel(const __grid_c
     const int quarter = warp & 3, turn = (warp - 2) >> 2, g = lane >> 2;
     const int row_tiles = (a.n + 15) / 16, groups = a.k >> p.group_shift, tile0 = blockIdx.x * (kWideRows / 16) + quarter * 2;
     const bool there[2] = {tile0 < row_tiles, tile0 + 1 < row_tiles};
-    const uint32_t ring = tc::smem_u32(smem) + kWideStages * stage_bytes + (warp - 2) * (kCodeDeep * 2 * 512) + lane * 16;
+    constexpr int kDeep = kCodeDeep<kG32>, kTile = kCodeTile<kG32>;
+    const uint32_t ring = tc::smem_u32(smem) + kWideStages * stage_bytes + (warp - 2) * (kDeep * 2 * kTile);
     const uint32_t place = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + p.columns + turn * 32;
     const uint4* codes[2];
     const uint2* params[2];
@@ -460,34 +488,22 @@ __global__ void __launch_bounds__(kWideThreads, 1) w4_wide_kernel(const __grid_c
     auto issue = [&](int c, int slot) {
       if (c < last) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) copy_async<16>(ring + (slot * 2 + k) * 512, codes[k] + c * 32, there[k]);
+        for (int k = 0; k < 2; ++k) copy_tile<kG32>(ring + (slot * 2 + k) * kTile, lane, codes[k], params[k], c, p.group_shift, groups, there[k]);
       }
       copy_commit();
     };
-    uint2 prm[2][2];
-    auto parameters = [&](int c, uint2 (&to)[2][2]) {
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int h = 0; h < (kG32 ? 2 : 1); ++h) {
-          const int group = kG32 ? min(2 * c + h, groups - 1) : c * 64 >> p.group_shift;
-          to[k][h] = there[k] ? __ldg(params[k] + group * 8) : make_uint2(0, 0);
-        }
-    };
-#pragma unroll
-    for (int i = 0; i < kCodeDeep - 1; ++i) issue(first + turn + kTurns * i, i);
-    if (first + turn < last) parameters(first + turn, prm);
+    for (int i = 0; i < kDeep - 1; ++i) issue(first + turn + kTurns * i, i);
     int slot = 0;
     uint32_t parity = 1;   // of the use before, once there was one
     for (int c = first + turn; c < last; c += kTurns, parity ^= 1) {
-      copy_wait<kCodeDeep - 2>();
+      copy_wait<kDeep - 2>();
       uint4 w[2];
+      uint2 prm[2][2];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) w[k] = shared16(ring + (slot * 2 + k) * 512);
-      issue(c + kTurns * (kCodeDeep - 1), slot == 0 ? kCodeDeep - 1 : slot - 1);
-      slot = slot == kCodeDeep - 1 ? 0 : slot + 1;
-      uint2 next[2][2];
-      parameters(min(c + kTurns, last - 1), next);
+      for (int k = 0; k < 2; ++k) take_tile<kG32>(ring + (slot * 2 + k) * kTile, lane, w[k], prm[k]);
+      issue(c + kTurns * (kDeep - 1), slot == 0 ? kDeep - 1 : slot - 1);
+      slot = slot == kDeep - 1 ? 0 : slot + 1;
       // the weights are ready in registers before their place in tensor memory is awaited: making them is not part of the loop from one use of a
       // place to the next (490 clocks per chunk when it was, at any number of rows of x)
       uint32_t r[2][16];
@@ -505,10 +521,6 @@ __global__ void __launch_bounds__(kWideThreads, 1) w4_wide_kernel(const __grid_c
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(full + turn);
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) prm[k][h] = next[k][h];
     }
     copy_wait<0>();
   }
@@ -672,69 +684,56 @@ __global__ void __launch_bounds__(kStreamThreads, 1) w4_stream_kernel(const __gr
   } else if (warp < 2 + 4 * kTurns) {   // ---- weights; chunks are counted through all tiles, so that a warp's stage is always the same
     const int quarter = warp & 3, turn = (warp - 2) >> 2, g = lane >> 2;
     const int tiles16 = (a.n + 15) / 16, groups = a.k >> p.group_shift;
-    const uint32_t ring = tc::smem_u32(smem) + kWideStages * stage_bytes + (warp - 2) * (kCodeDeep * 2 * 512) + lane * 16;
+    constexpr int kDeep = kCodeDeep<kG32>, kTile = kCodeTile<kG32>;
+    const uint32_t ring = tc::smem_u32(smem) + kWideStages * stage_bytes + (warp - 2) * (kDeep * 2 * kTile);
     const uint32_t place = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + kWeights + turn * 32;
-    struct Place {   // a chunk of a tile, and where its codes and parameters are
-      int tile, c;
-      const uint4* codes;
-      const uint2* params;
-      bool there[2];
+    // the loading side: a chunk of a tile, and where its codes and parameters are
+    int tile = blockIdx.x, c = turn;
+    bool there[2];
+    const uint4* codes;
+    const uint2* params;
+    auto at_tile = [&]() {
+      const int tile0 = tile / p.row_tiles * (kWideRows / 16) + quarter * 2;
+      there[0] = tile0 < tiles16;
+      there[1] = tile0 + 1 < tiles16;
+      codes = static_cast<const uint4*>(a.codes) + (there[0] ? static_cast<size_t>(tile0) * p.chunks * 32 : 0) + lane;
+      params = static_cast<const uint2*>(a.params) + (there[0] ? static_cast<size_t>(tile0) * groups * 8 : 0) + g;
     };
-    auto at_tile = [&](Place& at) {
-      const int tile0 = at.tile / p.row_tiles * (kWideRows / 16) + quarter * 2;
-      at.there[0] = tile0 < tiles16;
-      at.there[1] = tile0 + 1 < tiles16;
-      at.codes = static_cast<const uint4*>(a.codes) + (at.there[0] ? static_cast<size_t>(tile0) * p.chunks * 32 : 0) + lane;
-      at.params = static_cast<const uint2*>(a.params) + (at.there[0] ? static_cast<size_t>(tile0) * groups * 8 : 0) + g;
-    };
-    auto settle = [&](Place& at) {
-      if (at.c < p.chunks) return;
+    auto settle = [&]() {
+      if (c < p.chunks) return;
       do {
-        at.c -= p.chunks;
-        at.tile += gridDim.x;
-      } while (at.c >= p.chunks);
-      if (at.tile < p.tiles) at_tile(at);
+        c -= p.chunks;
+        tile += gridDim.x;
+      } while (c >= p.chunks);
+      if (tile < p.tiles) at_tile();
     };
-    Place now = {static_cast<int>(blockIdx.x), turn, nullptr, nullptr, {false, false}};
-    at_tile(now);
-    settle(now);
-    Place load = now, prm_at = now;
+    // this warp's chunks among those of all the block's tiles
+    const int mine = (p.tiles - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x) * p.chunks;
+    at_tile();
+    settle();
     auto issue = [&](int slot) {
-      if (load.tile < p.tiles) {
-        copy_async<16>(ring + slot * 1024, load.codes + load.c * 32, load.there[0]);
-        copy_async<16>(ring + slot * 1024 + 512, load.codes + (load.there[1] ? p.chunks * 32 : 0) + load.c * 32, load.there[1]);
-        load.c += kTurns;
-        settle(load);
+      if (tile < p.tiles) {
+        const uint32_t to = ring + slot * (2 * kTile);
+        copy_tile<kG32>(to, lane, codes, params, c, p.group_shift, groups, there[0]);
+        copy_tile<kG32>(to + kTile, lane, codes + (there[1] ? p.chunks * 32 : 0), params + (there[1] ? groups * 8 : 0), c, p.group_shift, groups, there[1]);
+        c += kTurns;
+        settle();
       }
       copy_commit();
     };
-    auto parameters = [&](uint2 (&to)[2][2]) {
-      if (prm_at.tile >= p.tiles) return;
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int h = 0; h < (kG32 ? 2 : 1); ++h) {
-          const int group = kG32 ? min(2 * prm_at.c + h, groups - 1) : prm_at.c * 64 >> p.group_shift;
-          to[k][h] = prm_at.there[k] ? __ldg(prm_at.params + (k * groups + group) * 8) : make_uint2(0, 0);
-        }
-      prm_at.c += kTurns;
-      settle(prm_at);
-    };
-    uint2 prm[2][2] = {}, next[2][2] = {};
-#pragma unroll
-    for (int i = 0; i < kCodeDeep - 1; ++i) issue(i);
-    parameters(prm);
+    for (int i = 0; i < kDeep - 1; ++i) issue(i);
     int slot = 0;
     bool used = false;
     uint32_t parity = 1;
-    for (; now.tile < p.tiles; used = true, parity ^= 1) {
-      copy_wait<kCodeDeep - 2>();
+    for (int n = turn; n < mine; n += kTurns, used = true, parity ^= 1) {
+      copy_wait<kDeep - 2>();
       uint4 w[2];
+      uint2 prm[2][2];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) w[k] = shared16(ring + (slot * 2 + k) * 512);
-      issue(slot == 0 ? kCodeDeep - 1 : slot - 1);
-      slot = slot == kCodeDeep - 1 ? 0 : slot + 1;
-      parameters(next);
+      for (int k = 0; k < 2; ++k) take_tile<kG32>(ring + (slot * 2 + k) * kTile, lane, w[k], prm[k]);
+      issue(slot == 0 ? kDeep - 1 : slot - 1);
+      slot = slot == kDeep - 1 ? 0 : slot + 1;
       uint32_t r[2][16];
 #pragma unroll
       for (int k = 0; k < 2; ++k) make_weights<kG32>(r[k], w[k], prm[k]);
@@ -750,15 +749,6 @@ __global__ void __launch_bounds__(kStreamThreads, 1) w4_stream_kernel(const __gr
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(full + turn);
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) prm[k][h] = next[k][h];
-      now.c += kTurns;
-      while (now.c >= p.chunks) {
-        now.c -= p.chunks;
-        now.tile += gridDim.x;
-      }
     }
     copy_wait<0>();
   } else {   // ---- results
