@@ -1,8 +1,13 @@
 // Products with 4-bit weights: y = x W^T, W[n, k] = scale[n, k / g] (code - zero).
 //
-// Two kernels.  For up to 16 rows of x the weights are read once, half a byte each, and bound the time: the narrow kernel multiplies codes as whole
-// numbers and applies a group's scale to its sum in fp32, scale * sum x (code - zero), so nothing but x and y is rounded to 16 bits.  For more rows
-// the wide kernel makes bf16 weights on the way into tensor memory, where they are the left operand of tcgen05 products.
+// Three kernels.  For up to 16 rows of x that fit shared memory the weights are read once, half a byte each: the narrow kernel multiplies codes as whole
+// numbers (bf16 holds -15 to 15 exactly) and applies a group's scale to its sum in fp32, scale * sum x (code - zero), so nothing but x and y is rounded to
+// 16 bits.  Its time is that of taking the codes apart: some 190 instructions per KB.  For more rows bf16 weights, scale * (code - zero) rounded once, are
+// made on the way into tensor memory, where they are the left operand of tcgen05 products: a block per tile and part of K where that fills the SMs (the wide
+// kernel), a block per SM that runs on from tile to tile where there are several for each (the stream kernel).  For 16384 x 2048 the
+// narrow kernel takes 7.4 us for 8 rows and 10.2 for 16, the wide one 9.9 for up to 32: where they meet the narrow one stays, which rounds no weights.
+// Measured (codes from memory): 4 x 32000 x 2048, 36 MB: 12.8 us, 2.8 TB/s; 1 x 16384 x 2048: 6.5 us; 1 x 2048 x 2048: 2.6 us, a launch and one chain of loads;
+// 48 x 3072 x 768: 5.1 us; 128 x 16384 x 2048: 12.3 us, 0.70 PFLOP/s; 256: 17.4 us; 1537: 90 us, 1.15 PFLOP/s.
 #include <cuda.h>
 
 #include <array>
@@ -91,9 +96,10 @@ template <int kR, int kN, int kParams>
 int narrow_smem(int m, int pairs) { return kNarrowWarps * kDeep<kR> * kNarrowSlot<kR, kParams> + kNarrowSums<kR, kN> + m * pairs * 256 + 16; }
 
 // A warp takes kR tiles of 16 weight rows at a time, a block 8 / along times as many, gridDim.x such groups apart; `along` warps share out K for each, a
-// run of stages of 128 columns, and add up at its end.  A lane's 16 bytes of 64 columns are its own A fragments of four m16n8k16 products: it copies them ahead into its own place and waits for nobody, and so
-// it does with its two rows' parameters (kParams groups in a stage).  x lies in shared memory, 128 bytes of every row per 64 columns, in the order of the
-// 128-byte swizzle; kN is how many times 8 rows it has.
+// run of stages of 128 columns, and add up at its end.  A lane's 16 bytes of 64 columns are its own A fragments of four m16n8k16 products: it copies them
+// ahead into its own place and waits for nobody, and so it does with its two rows' parameters (kParams groups in a stage).  x lies in shared memory, 128
+// bytes of every row per 64 columns, in the order of the 128-byte swizzle; kN is how many times 8 rows it has.
+// Two blocks of 8 warps per SM: one of 16 warps took 14.2 us for 4 x 32000 x 2048 and 6.1 for a small product, whose next launch then finds no room.
 // kEven: no tile and no half stage is missing at the end of N or K.
 template <int kR, int kN, int kParams, bool kEven>
 __global__ void __launch_bounds__(kNarrowThreads, 2) w4_narrow_kernel(W4Args a, int tiles, int chunks, int group_shift, int along_shift) {
@@ -253,7 +259,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 2) w4_narrow_kernel(W4Args a, 
 // --------------------------------------------------------------- more rows of x --
 constexpr int kWideRows = 128;             // weight rows of a block: the lanes of tensor memory
 // Warp 0 brings x, warp 1 issues the products, sixteen make weights and write results.  Four warps share a chunk (32 weight rows each) and take
-// chunks in turn with three other fours: a warp needs some 600 clocks for its part, most of them latency.
+// chunks in turn with three other fours: a warp's part is mostly latency (copy, shared memory, arithmetic, tensor memory, barrier), and four under way hide it.
 constexpr int kTurns = 4;
 constexpr int kWideThreads = (2 + 4 * kTurns) * 32;
 constexpr int kWideStages = 4;
@@ -938,8 +944,8 @@ int resident(int splits) {
 // Rows of x per block and parts of K.  A chunk of 64 columns costs the making of its weights (some 400 clocks) or its products (two clocks per row of x), a
 // block some 5000 clocks before its first and after its last chunk.  (Measured beside all other choices for 12 sizes from 24 x 2048 x 2048 to
 // 1537 x 16384 x 2048: within 4 % of the best.)
-// With more tiles than SMs they run on from one to the next (returns true): no round has a beginning and an end of its own, and products hide the making of weights from 190 rows
-// of x on.
+// With more tiles than SMs they run on from one to the next (returns true), so that no round has a beginning and an end of its own: 1537 x 16384 x 2048 took
+// 103 us in rounds.  Its limit stays the making of weights: the products of 176 rows are 350 of a chunk's some 570 clocks.
 bool choose_wide(int m, int blocks, Wide& p) {
   constexpr double kMake = 400, kRound = 5000, kSplit = 1500, kToken = 20;
   double best = 0;
@@ -1033,6 +1039,8 @@ cudaError_t w4_linear(const W4Args& a, cudaStream_t stream) {
   if (a.m <= 0 || a.n <= 0) return cudaSuccess;
   const long long x_bytes = static_cast<long long>(a.m) * ((a.k + 127) / 128) * 256;
   if (a.m <= 16 && x_bytes <= 128 * 1024) {
+    // two tiles of weights per warp share what is read of x (1 x 16384 x 2048 6.5 us, 7.9 with one; 4 x 32000 x 2048 12.8 and 14.3), if that leaves every SM some
+    // warps' work (1 x 2048 x 2048: 2.6 with one); 16 rows' sums leave no registers for it
     const bool two = a.n >= 16 * 3 * sm_count();
     if (a.m <= 8) return two ? narrow<2, 1>(a, stream) : narrow<1, 1>(a, stream);
     return narrow<1, 2>(a, stream);

@@ -111,7 +111,9 @@ def quantize_w4(weight: torch.Tensor, group: int = 128) -> W4Weight:
 def linear_w4(x: torch.Tensor, weight: W4Weight, bias: Optional[torch.Tensor] = None, act: str = "none", residual: Optional[torch.Tensor] = None):
     """act(x @ W^T + b) + residual for x bf16 ``[..., k]``; bias fp32 ``[n]``; act "none" or "gelu".  Forward only.
 
-    Codes are multiplied as whole numbers and scaled in fp32, so that nothing but x and the result is rounded."""
+    With up to 16 rows of x (fewer where 256 bytes per row and 128 columns pass 128 KB) codes are multiplied as whole numbers and scaled in fp32, so that
+    nothing but x and the result is rounded; with more rows ``scale * (code - zero)`` is rounded to bf16 first, as :meth:`W4Weight.dequantize` has it.
+    Sums are fp32 either way, and added in an order that depends on the sizes only."""
     gelu = act == "gelu"
     if not gelu and act != "none":
         raise RuntimeError(f"linear_w4: unknown activation '{act}'")
