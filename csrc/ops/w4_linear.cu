@@ -597,10 +597,18 @@ __global__ void __launch_bounds__(kWideThreads, 1) w4_wide_kernel(const __grid_c
 // The same products for more tiles than there are SMs: a block takes tiles gridDim.x apart, and its four roles run on from one to the next.  Two sets of
 // sums in tensor memory (up to 192 rows of x each, behind them the weights' ring: 512 columns) let four warps of their own write a tile's results beside
 // the next one's products.  (As one block per tile each round of SMs took 5 us before its first and after its last product.)
-constexpr int kStreamThreads = (2 + 4 * kTurns + 4) * 32;
+constexpr int kResultWarps = 8;   // in two fours that take 16 rows of x in turn
+constexpr int kStreamThreads = (2 + 4 * kTurns + kResultWarps) * 32;
 constexpr int kStreamTokens = 192;
-constexpr int kStaged = 16 * kWideRows * 4;   // sums of 16 rows of x on their way to a row of y, twice
-int stream_smem(int tokens) { return kWideStages * tokens * 128 + kCodeRing + 2 * kStaged + 1024; }
+constexpr int kStaged = 16 * kWideRows * 2;   // 16 rows of y on their way to memory, twice for each four warps
+int stream_smem(int tokens) { return kWideStages * tokens * 128 + kCodeRing + 4 * kStaged + 1024; }
+
+// Whether any of the 128 threads at a barrier says so.
+__device__ __forceinline__ bool any_of_128(int barrier, bool mine) {
+  uint32_t any;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbarrier.cta.red.or.pred p, %2, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(any) : "r"(mine ? 1u : 0u), "r"(barrier) : "memory");
+  return any != 0;
+}
 
 template <bool kG32>
 __global__ void __launch_bounds__(kStreamThreads, 1) w4_stream_kernel(const __grid_constant__ CUtensorMap x_map, Wide p) {
@@ -609,7 +617,6 @@ __global__ void __launch_bounds__(kStreamThreads, 1) w4_stream_kernel(const __gr
   __shared__ uint64_t full[kWideStages], empty[kWideStages], sums_full[2], sums_empty[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int bad;
-  __shared__ volatile int lost;
   const W4Args& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int stage_bytes = p.tokens * 128;
@@ -621,11 +628,10 @@ __global__ void __launch_bounds__(kStreamThreads, 1) w4_stream_kernel(const __gr
     }
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(sums_full + i, 1);
-      tc::mbar_init(sums_empty + i, 4);
+      tc::mbar_init(sums_empty + i, kResultWarps);
     }
     tc::mbar_init_fence();
     bad = 0;
-    lost = 0;
     tc::tma_prefetch_desc(&x_map);
   }
   __syncwarp();
@@ -658,33 +664,44 @@ __global__ void __launch_bounds__(kStreamThreads, 1) w4_stream_kernel(const __gr
     }
     __syncwarp();
   } else if (warp == 1) {   // ---- products
+    // Chunks are counted through all tiles, and the loop is written out stage by stage: barriers and operands that are known when it is compiled leave
+    // the thread some 140 clocks per chunk, a stage that is a variable 360 (and more beside warps that compute).
     if (tc::elect_one()) {
       const uint64_t desc = tc::smem_desc_k_sw128(smem), stage_step = static_cast<uint64_t>(stage_bytes >> 4);
-      int s = 0, i = 0;
-      uint32_t parity = 0;
-      for (int tile = blockIdx.x; tile < p.tiles && !bad; tile += gridDim.x, ++i) {
-        if (i >= 2 && !wait_for(sums_empty + (i & 1), ((i >> 1) - 1) & 1)) {
-          bad = 1;
-          break;
-        }
-        tc::fence_after_sync();
-        const uint32_t sums = tmem + (i & 1) * kStreamTokens;
-        for (int c = 0; c < p.chunks; ++c) {
+      int left = (p.tiles - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), c = 0;
+      uint32_t parity = 0, set = 0, sums = tmem, used = 0, set_parity = 1;   // set_parity: of a set's use before
+      while (left > 0 && !bad) {
+        uint64_t db = desc;
+#pragma unroll
+        for (int s = 0; s < kWideStages; ++s, db += stage_step) {
+          if (left == 0) break;
+          if (c == 0 && used >= 2 && !wait_for(sums_empty + set, set_parity)) {
+            bad = 1;
+            break;
+          }
           if (!wait_for(full + s, parity)) {
             bad = 1;
             break;
           }
           tc::fence_after_sync();
-          const uint64_t db = desc + s * stage_step;
-          const uint32_t weights = tmem + kWeights + s * 32;
-          mma_ts(sums, weights, db, p.idesc, c > 0);
+          mma_ts(sums, tmem + kWeights + s * 32, db, p.idesc, c > 0);
 #pragma unroll
-          for (int k = 1; k < 4; ++k) mma_ts(sums, weights + k * 8, db + 2 * k, p.idesc, true);
+          for (int k = 1; k < 4; ++k) mma_ts(sums, tmem + kWeights + s * 32 + k * 8, db + 2 * k, p.idesc, true);
           tc::mma_commit(empty + s);
-          if (++s == kWideStages) s = 0, parity ^= 1;
+          if (++c == p.chunks) {
+            tc::mma_commit(sums_full + set);
+            c = 0;
+            --left;
+            ++used;
+            set ^= 1;
+            set_parity ^= set ^ 1;
+            sums = tmem + set * kStreamTokens;
+          }
         }
-        tc::mma_commit(sums_full + (i & 1));   // also after a failure: it releases the waiters
+        parity ^= 1;
       }
+      if (bad)   // releases the waiters
+        for (int i = 0; i < 2; ++i) tc::mma_commit(sums_full + i);
     }
     __syncwarp();
   } else if (warp < 2 + 4 * kTurns) {   // ---- weights; chunks are counted through all tiles, so that a warp's stage is always the same
@@ -758,40 +775,58 @@ __global__ void __launch_bounds__(kStreamThreads, 1) w4_stream_kernel(const __gr
     }
     copy_wait<0>();
   } else {   // ---- results
-    const int quarter = warp & 3;
-    float* staged = reinterpret_cast<float*>(smem + kWideStages * stage_bytes + kCodeRing);   // [2][row of x][weight row]
+    const int quarter = warp & 3, four = (warp - 2 - 4 * kTurns) >> 2, thread = threadIdx.x & 127;
+    unsigned char* staged = smem + kWideStages * stage_bytes + kCodeRing + four * (2 * kStaged);   // [2][row of x][weight row]
+    __nv_bfloat16* y = static_cast<__nv_bfloat16*>(a.y);
+    const __nv_bfloat16* residual = static_cast<const __nv_bfloat16*>(a.residual);
     int i = 0, half = 0;
     for (int tile = blockIdx.x; tile < p.tiles; tile += gridDim.x, ++i) {
-      const int block = tile / p.row_tiles, row0 = (tile - block * p.row_tiles) * p.tokens, n4 = block * kWideRows + lane * 4;
-      float bias[4];
-      load_bias(bias, a, n4);
-      if (!__all_sync(0xffffffffu, wait_for(sums_full + (i & 1), (i >> 1) & 1)) && lane == 0) lost = 1;
-      asm volatile("bar.sync 1, 128;" ::: "memory");   // these four warps: they leave together or not at all
-      if (lost) {
+      const int block = tile / p.row_tiles, row0 = (tile - block * p.row_tiles) * p.tokens, n0 = block * kWideRows, n = n0 + quarter * 32 + lane;
+      const float bias = a.bias && n < a.n ? __ldg(a.bias + n) : 0.f;
+      if (any_of_128(1 + four, !wait_for(sums_full + (i & 1), (i >> 1) & 1))) {   // these four warps leave together or not at all
         bad = 1;
         break;
       }
       tc::fence_after_sync();
       const uint32_t sums = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (i & 1) * kStreamTokens;
-      for (int c = 0; c < p.tokens / 16; ++c, half ^= 1) {
+      for (int c = four; c < p.tokens / 16; c += 2, half ^= 1) {
         uint32_t r[16];
         tmem_ld_32x16(sums + c * 16, r);
         tc::tmem_ld_wait();
-        if (c == p.tokens / 16 - 1) {   // the products of the tile after next may begin
-          tc::fence_before_sync();
-          __syncwarp();
-          if (lane == 0) tc::mbar_arrive(sums_empty + (i & 1));
+        __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(staged + half * kStaged);
+        float v[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(r[e]) + bias;
+        if (a.gelu) {   // (the branches once and not for every element: 1100 clocks less)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) v[e] = 0.5f * v[e] * (1.f + erff(v[e] * 0.70710678118654752f));
         }
-        float* to = staged + half * (kStaged / 4);
+        if (a.residual && n < a.n) {
+          const int m0 = row0 + c * 16;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) to[e * kWideRows + quarter * 32 + lane] = __uint_as_float(r[e]);
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+          for (int e = 0; e < 16; ++e) v[e] += __bfloat162float(residual[min(m0 + e, a.m - 1) * a.ldr + n]);
+        }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int m = row0 + c * 16 + quarter * 4 + e;
-          if (m < a.m) finish4(a, *reinterpret_cast<const float4*>(to + (quarter * 4 + e) * kWideRows + lane * 4), bias, m, n4, p.vector);
+        for (int e = 0; e < 16; ++e) to[e * kWideRows + quarter * 32 + lane] = __float2bfloat16_rn(v[e]);
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + four) : "memory");
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {   // 8 rows at a time, 8 elements per thread
+          const int row = e * 8 + (thread >> 4), m = row0 + c * 16 + row, n8 = n0 + (thread & 15) * 8;
+          if (m < a.m && n8 < a.n) {
+            const __nv_bfloat16* from = to + row * kWideRows + (thread & 15) * 8;
+            __nv_bfloat16* out = y + static_cast<long long>(m) * a.n + n8;
+            if (p.vector) {
+              *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(from);
+            } else {
+              for (int k = 0; k < min(8, a.n - n8); ++k) out[k] = from[k];
+            }
+          }
         }
       }
+      // the products of the tile after next may begin
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(sums_empty + (i & 1));
     }
   }
   tc::fence_before_sync();
@@ -1018,6 +1053,7 @@ cudaError_t launch_wide(const W4Args& a, cudaStream_t on) {
   p.columns = p.tokens <= 32 ? 32 : (p.tokens <= 64 ? 64 : (p.tokens <= 128 ? 128 : 256));
   p.allocated = p.columns + kWideStages * 32 <= 256 ? 256 : 512;
   p.vector = a.n % 4 == 0 && (a.residual == nullptr || (a.ldr % 4 == 0 && reinterpret_cast<uintptr_t>(a.residual) % 8 == 0));
+  if (stream) p.vector = a.n % 8 == 0;   // of y alone
   p.idesc = tc::idesc_bf16(kWideRows, p.tokens);
   p.err = gemm_error_device_ptr();
   const CuDriver& cu = CuDriver::get();
