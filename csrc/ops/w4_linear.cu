@@ -7,7 +7,7 @@
 // kernel), a block per SM that runs on from tile to tile where there are several for each (the stream kernel).  For 16384 x 2048 the
 // narrow kernel takes 7.4 us for 8 rows and 10.2 for 16, the wide one 9.9 for up to 32: where they meet the narrow one stays, which rounds no weights.
 // Measured (codes from memory): 4 x 32000 x 2048, 36 MB: 12.8 us, 2.8 TB/s; 1 x 16384 x 2048: 6.5 us; 1 x 2048 x 2048: 2.6 us, a launch and one chain of loads;
-// 48 x 3072 x 768: 5.1 us; 128 x 16384 x 2048: 12.3 us, 0.70 PFLOP/s; 256: 17.4 us; 1537: 90 us, 1.15 PFLOP/s.
+// 48 x 3072 x 768: 5.1 us; 128 x 16384 x 2048: 12.3 us, 0.70 PFLOP/s; 256: 17.4 us; 1537: 81 us, 1.27 PFLOP/s.
 #include <cuda.h>
 
 #include <array>
@@ -595,13 +595,21 @@ __global__ void __launch_bounds__(kWideThreads, 1) w4_wide_kernel(const __grid_c
 
 // ------------------------------------------------- tiles for several rounds of SMs --
 // The same products for more tiles than there are SMs: a block takes tiles gridDim.x apart, and its four roles run on from one to the next.  Two sets of
-// sums in tensor memory (up to 192 rows of x each, behind them the weights' ring: 512 columns) let four warps of their own write a tile's results beside
-// the next one's products.  (As one block per tile each round of SMs took 5 us before its first and after its last product.)
+// sums in tensor memory (up to 176 rows of x each, behind them five chunks of weights: 512 columns) let eight warps of their own write a tile's results beside
+// the next one's products.  1537 x 16384 x 2048 takes 81 us, 1.27 PFLOP/s (89 when it goes on for seconds and the power limit lowers the clock): 500 clocks per
+// chunk, of which the products want 352.  No role alone is the rest: with a quarter of the products it takes 69 us, with weights that cost no arithmetic 71,
+// with x that need not come 73.  (As one block per tile each round of SMs took 5 us before its first and after its last product: 103 us; four stages 83, six and
+// fewer rows 87; rings of their own for x and weights, whose stages are then variables to the issuing thread, 99.)
 constexpr int kResultWarps = 8;   // in two fours that take 16 rows of x in turn
 constexpr int kStreamThreads = (2 + 4 * kTurns + kResultWarps) * 32;
-constexpr int kStreamTokens = 192;
+constexpr int kStages = 5;   // of x and weights
+constexpr int kStreamTokens = (512 - 32 * kStages) / 2;
+constexpr int kStreamDeep = 3;   // chunks of codes of a warp
+template <bool kG32>
+constexpr int kStreamCodes = 4 * kTurns * 2 * kStreamDeep * kCodeTile<kG32>;
 constexpr int kStaged = 16 * kWideRows * 2;   // 16 rows of y on their way to memory, twice for each four warps
-int stream_smem(int tokens) { return kWideStages * tokens * 128 + kCodeRing + 4 * kStaged + 1024; }
+template <bool kG32>
+int stream_smem(int tokens) { return kStages * tokens * 128 + kStreamCodes<kG32> + 4 * kStaged + 1024; }
 
 // Whether any of the 128 threads at a barrier says so.
 __device__ __forceinline__ bool any_of_128(int barrier, bool mine) {
@@ -614,7 +622,7 @@ template <bool kG32>
 __global__ void __launch_bounds__(kStreamThreads, 1) w4_stream_kernel(const __grid_constant__ CUtensorMap x_map, Wide p) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024 - (tc::smem_u32(smem_raw) & 1023)) & 1023);
-  __shared__ uint64_t full[kWideStages], empty[kWideStages], sums_full[2], sums_empty[2];
+  __shared__ uint64_t full[kStages], empty[kStages], sums_full[2], sums_empty[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int bad;
   const W4Args& a = p.a;
@@ -622,7 +630,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) w4_stream_kernel(const __gr
   const int stage_bytes = p.tokens * 128;
   constexpr int kWeights = 2 * kStreamTokens;   // first column of the weights' ring
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kWideStages; ++i) {
+    for (int i = 0; i < kStages; ++i) {
       tc::mbar_init(full + i, 5);
       tc::mbar_init(empty + i, 1);
     }
@@ -650,17 +658,17 @@ __global__ void __launch_bounds__(kStreamThreads, 1) w4_stream_kernel(const __gr
       for (int tile = blockIdx.x; tile < p.tiles && !bad; tile += gridDim.x) {
         const int row0 = tile % p.row_tiles * p.tokens;
         for (int c = 0; c < p.chunks; ++c, ++issued) {
-          if (issued >= kWideStages && !wait_for(empty + s, parity)) {
+          if (issued >= kStages && !wait_for(empty + s, parity)) {
             bad = 1;
             break;
           }
           tc::mbar_expect_tx(full + s, stage_bytes);
           tc::tma_load_2d(smem + s * stage_bytes, &x_map, full + s, c * 64, row0);
-          if (++s == kWideStages) s = 0, parity ^= 1;
+          if (++s == kStages) s = 0, parity ^= 1;
         }
       }
       if (bad)   // what was issued must land before the block retires
-        for (int i = max(issued - kWideStages, 0); i < issued; ++i) tc::mbar_wait(full + i % kWideStages, (i / kWideStages) & 1, 1u << 20);
+        for (int i = max(issued - kStages, 0); i < issued; ++i) tc::mbar_wait(full + i % kStages, (i / kStages) & 1, 1u << 20);
     }
     __syncwarp();
   } else if (warp == 1) {   // ---- products
@@ -673,7 +681,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) w4_stream_kernel(const __gr
       while (left > 0 && !bad) {
         uint64_t db = desc;
 #pragma unroll
-        for (int s = 0; s < kWideStages; ++s, db += stage_step) {
+        for (int s = 0; s < kStages; ++s, db += stage_step) {
           if (left == 0) break;
           if (c == 0 && used >= 2 && !wait_for(sums_empty + set, set_parity)) {
             bad = 1;
@@ -707,9 +715,9 @@ __global__ void __launch_bounds__(kStreamThreads, 1) w4_stream_kernel(const __gr
   } else if (warp < 2 + 4 * kTurns) {   // ---- weights; chunks are counted through all tiles, so that a warp's stage is always the same
     const int quarter = warp & 3, turn = (warp - 2) >> 2, g = lane >> 2;
     const int tiles16 = (a.n + 15) / 16, groups = a.k >> p.group_shift;
-    constexpr int kDeep = kCodeDeep<kG32>, kTile = kCodeTile<kG32>;
-    const uint32_t ring = tc::smem_u32(smem) + kWideStages * stage_bytes + (warp - 2) * (kDeep * 2 * kTile);
-    const uint32_t place = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + kWeights + turn * 32;
+    constexpr int kDeep = kStreamDeep, kTile = kCodeTile<kG32>;
+    const uint32_t ring = tc::smem_u32(smem) + kStages * stage_bytes + (warp - 2) * (kDeep * 2 * kTile);
+    const uint32_t place = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + kWeights;
     // the loading side: a chunk of a tile, and where its codes and parameters are
     int tile = blockIdx.x, c = turn;
     bool there[2];
@@ -747,9 +755,9 @@ __global__ void __launch_bounds__(kStreamThreads, 1) w4_stream_kernel(const __gr
 #pragma unroll
     for (int i = 0; i < kDeep - 1; ++i) issue(i);
     int slot = 0;
-    bool used = false;
-    uint32_t parity = 1;
-    for (int n = turn; n < mine; n += kTurns, used = true, parity ^= 1) {
+    int s = turn;
+    uint32_t parity = 1;   // of a stage's use before
+    for (int n = turn; n < mine; n += kTurns) {
       copy_wait<kDeep - 2>();
       uint4 w[2];
       uint2 prm[2][2];
@@ -760,23 +768,25 @@ __global__ void __launch_bounds__(kStreamThreads, 1) w4_stream_kernel(const __gr
       uint32_t r[2][16];
 #pragma unroll
       for (int k = 0; k < 2; ++k) make_weights<kG32>(r[k], w[k], prm[k]);
-      const bool ok = !used || wait_for(empty + turn, parity);
+      const bool ok = n < kStages || wait_for(empty + s, parity);
       if (!__all_sync(0xffffffffu, ok)) {
         if (lane == 0) bad = 1;
         break;
       }
       tc::fence_after_sync();
 #pragma unroll
-      for (int k = 0; k < 2; ++k) tmem_st_16x64(place + (static_cast<uint32_t>(k * 16) << 16), r[k]);
+      for (int k = 0; k < 2; ++k) tmem_st_16x64(place + s * 32 + (static_cast<uint32_t>(k * 16) << 16), r[k]);
       tmem_st_wait();
       tc::fence_before_sync();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(full + turn);
+      if (lane == 0) tc::mbar_arrive(full + s);
+      s += kTurns;
+      if (s >= kStages) s -= kStages, parity ^= 1;
     }
     copy_wait<0>();
   } else {   // ---- results
     const int quarter = warp & 3, four = (warp - 2 - 4 * kTurns) >> 2, thread = threadIdx.x & 127;
-    unsigned char* staged = smem + kWideStages * stage_bytes + kCodeRing + four * (2 * kStaged);   // [2][row of x][weight row]
+    unsigned char* staged = smem + kStages * stage_bytes + kStreamCodes<kG32> + four * (2 * kStaged);   // [2][row of x][weight row]
     __nv_bfloat16* y = static_cast<__nv_bfloat16*>(a.y);
     const __nv_bfloat16* residual = static_cast<const __nv_bfloat16*>(a.residual);
     int i = 0, half = 0;
@@ -980,7 +990,7 @@ int resident(int splits) {
 // block some 5000 clocks before its first and after its last chunk.  (Measured beside all other choices for 12 sizes from 24 x 2048 x 2048 to
 // 1537 x 16384 x 2048: within 4 % of the best.)
 // With more tiles than SMs they run on from one to the next (returns true), so that no round has a beginning and an end of its own: 1537 x 16384 x 2048 took
-// 103 us in rounds.  Its limit stays the making of weights: the products of 176 rows are 350 of a chunk's some 570 clocks.
+// 103 us in rounds.
 bool choose_wide(int m, int blocks, Wide& p) {
   constexpr double kMake = 400, kRound = 5000, kSplit = 1500, kToken = 20;
   double best = 0;
@@ -1003,9 +1013,9 @@ bool choose_wide(int m, int blocks, Wide& p) {
     }
   }
   bool stream = false;
-  for (int most = 32; most <= kStreamTokens; most += 32) {
+  for (int most = 32; most <= kStreamTokens; most += 16) {
     const int tiles = (m + most - 1) / most, tokens = ((m + tiles - 1) / tiles + 15) / 16 * 16, row_tiles = (m + tokens - 1) / tokens;
-    if (static_cast<long long>(blocks) * row_tiles > 0x7fffffff) continue;
+    if (tokens > kStreamTokens || static_cast<long long>(blocks) * row_tiles > 0x7fffffff || (p.a.group == 32 ? stream_smem<true>(tokens) : stream_smem<false>(tokens)) > kWideSmem) continue;
     const int all = blocks * row_tiles, rounds = (all + sm_count() - 1) / sm_count();
     if (rounds < 2) continue;
     const double products = 2.0 * tokens;
@@ -1038,7 +1048,7 @@ cudaError_t start_stream(const Wide& p, const CUtensorMap& map, cudaStream_t str
   static std::atomic<uint64_t> allowed{0};
   const cudaError_t rc = raise_smem_limit(w4_stream_kernel<kG32>, kWideSmem, allowed);
   if (rc != cudaSuccess) return rc;
-  MCCL_LAUNCH_PDL(w4_stream_kernel<kG32>, p.tiles < sm_count() ? p.tiles : sm_count(), kStreamThreads, stream_smem(p.tokens), stream, map, p);
+  MCCL_LAUNCH_PDL(w4_stream_kernel<kG32>, p.tiles < sm_count() ? p.tiles : sm_count(), kStreamThreads, stream_smem<kG32>(p.tokens), stream, map, p);
   count_launch();
   return ::mccl::launch_status();
 }
