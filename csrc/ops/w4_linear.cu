@@ -279,7 +279,7 @@ struct Wide {
   int columns;          // of tensor memory that the sums take; the weights' ring lies behind them
   int allocated;
   int splits, share;    // blocks of a cluster that share out K, and rows of x whose sums each of them finishes
-  int vector;           // y and residual can be accessed four elements at a time
+  int vector, rows8;    // y and residual can be accessed four elements at a time, y eight
   int tiles, row_tiles; // of the stream: tiles of weight rows and rows of x, and how many of the latter
   uint32_t idesc;
   int* err;
@@ -391,6 +391,51 @@ __device__ __forceinline__ void finish4(const W4Args& a, const float4& v, const 
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (n4 + e < a.n) y[e] = __float2bfloat16_rn(f[e] + (a.residual ? __bfloat162float(residual[e]) : 0.f));
+  }
+}
+
+// Whether any of the 128 threads at a barrier says so.
+__device__ __forceinline__ bool any_of_128(int barrier, bool mine) {
+  uint32_t any;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbarrier.cta.red.or.pred p, %2, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(any) : "r"(mine ? 1u : 0u), "r"(barrier) : "memory");
+  return any != 0;
+}
+
+// Sums of 128 weight rows and 16 rows of x, from tensor memory to y, by four warps: a lane has a weight row, and through shared memory (`to`, [row of x][weight
+// row]) a row of y leaves in one piece.  rows8: rows of y are made of eights.  Branches stand around all sixteen values: around each of them they cost 1100 clocks.
+constexpr int kStaged = 16 * kWideRows * 2;
+__device__ __forceinline__ void finish16(const W4Args& a, int rows8, uint32_t sums, __nv_bfloat16* to, int barrier, int m0, int n0, int quarter, int lane, float bias) {
+  uint32_t r[16];
+  tmem_ld_32x16(sums, r);
+  tc::tmem_ld_wait();
+  float v[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(r[e]) + bias;
+  if (a.gelu) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = 0.5f * v[e] * (1.f + erff(v[e] * 0.70710678118654752f));
+  }
+  const int n = n0 + quarter * 32 + lane;
+  if (a.residual && n < a.n) {
+    const __nv_bfloat16* residual = static_cast<const __nv_bfloat16*>(a.residual) + n;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] += __bfloat162float(residual[min(m0 + e, a.m - 1) * a.ldr]);
+  }
+#pragma unroll
+  for (int e = 0; e < 16; ++e) to[e * kWideRows + quarter * 32 + lane] = __float2bfloat16_rn(v[e]);
+  asm volatile("bar.sync %0, 128;" ::"r"(barrier) : "memory");
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {   // 8 rows at a time, 8 elements per thread
+    const int row = e * 8 + quarter * 2 + (lane >> 4), m = m0 + row, n8 = n0 + (lane & 15) * 8;
+    if (m < a.m && n8 < a.n) {
+      const __nv_bfloat16* from = to + row * kWideRows + (lane & 15) * 8;
+      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.y) + static_cast<long long>(m) * a.n + n8;
+      if (rows8) {
+        *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(from);
+      } else {
+        for (int k = 0; k < min(8, a.n - n8); ++k) out[k] = from[k];
+      }
+    }
   }
 }
 
@@ -533,22 +578,29 @@ __global__ void __launch_bounds__(kWideThreads, 1) w4_wide_kernel(const __grid_c
 
   // ---- results
   __syncwarp();
-  const int n4 = blockIdx.x * kWideRows + lane * 4, token0 = blockIdx.y * p.tokens;
-  float bias[4];
-  load_bias(bias, a, n4);
+  const int n0 = blockIdx.x * kWideRows, token0 = blockIdx.y * p.tokens, quarter = warp & 3, turn = (warp - 2) >> 2, row = quarter * 32 + lane;
+  float bias[4] = {};
+  if (p.splits > 1) {
+    load_bias(bias, a, n0 + lane * 4);
+  } else {
+    bias[0] = a.bias && n0 + row < a.n ? __ldg(a.bias + n0 + row) : 0.f;
+  }
   const bool ok = wait_for(&done, 0);
   tc::fence_after_sync();
   __syncwarp();
-  // [part][row of x][weight row]: where x was, or behind everything else where other blocks write too
-  float* sums = reinterpret_cast<float*>(smem + (p.splits > 1 ? kWideStages * stage_bytes + kCodeRing : 0));
-  if (p.splits > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  if (warp >= 2 && ok) {
-    const int quarter = warp & 3, turn = (warp - 2) >> 2, row = quarter * 32 + lane;
-    for (int c = turn; c < p.tokens / 16; c += kTurns) {
-      uint32_t r[16];
-      tmem_ld_32x16(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + c * 16, r);
-      tc::tmem_ld_wait();
-      if (p.splits > 1) {
+  const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+  if (p.splits == 1) {
+    if (warp >= 2 && !any_of_128(1 + turn, !ok))   // four warps leave together or not at all
+      for (int c = turn; c < p.tokens / 16; c += kTurns)   // through where x was
+        finish16(a, p.rows8, lanes + c * 16, reinterpret_cast<__nv_bfloat16*>(smem + c * kStaged), 1 + turn, token0 + c * 16, n0, quarter, lane, bias[0]);
+  } else {
+    float* sums = reinterpret_cast<float*>(smem + kWideStages * stage_bytes + kCodeRing);   // [part][row of x][weight row], behind everything else: other blocks write too
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (warp >= 2 && ok) {
+      for (int c = turn; c < p.tokens / 16; c += kTurns) {
+        uint32_t r[16];
+        tmem_ld_32x16(lanes + c * 16, r);
+        tc::tmem_ld_wait();
         int owner = c * 16 / p.share, at = c * 16 - owner * p.share;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -558,31 +610,23 @@ __global__ void __launch_bounds__(kWideThreads, 1) w4_wide_kernel(const __grid_c
             ++owner;
           }
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sums[(c * 16 + i) * kWideRows + row] = __uint_as_float(r[i]);
       }
     }
-  }
-  __syncwarp();
-  if (p.splits > 1) {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  } else {
-    __syncthreads();
-  }
-  const int from = p.splits > 1 ? static_cast<int>(blockIdx.z) * p.share : 0, rows = min(min(p.share, p.tokens - from), a.m - token0 - from);
-  for (int i = warp; i < rows; i += kWideThreads / 32) {
-    const int m = token0 + from + i;
-    float4 v = *reinterpret_cast<const float4*>(sums + i * kWideRows + lane * 4);
-    for (int r = 1; r < p.splits; ++r) {
-      const float4 o = *reinterpret_cast<const float4*>(sums + (r * p.share + i) * kWideRows + lane * 4);
-      v.x += o.x;
-      v.y += o.y;
-      v.z += o.z;
-      v.w += o.w;
+    const int from = static_cast<int>(blockIdx.z) * p.share, rows = min(min(p.share, p.tokens - from), a.m - token0 - from);
+    for (int i = warp; i < rows; i += kWideThreads / 32) {
+      float4 v = *reinterpret_cast<const float4*>(sums + i * kWideRows + lane * 4);
+      for (int r = 1; r < p.splits; ++r) {
+        const float4 o = *reinterpret_cast<const float4*>(sums + (r * p.share + i) * kWideRows + lane * 4);
+        v.x += o.x;
+        v.y += o.y;
+        v.z += o.z;
+        v.w += o.w;
+      }
+      finish4(a, v, bias, token0 + from + i, n0 + lane * 4, p.vector);
     }
-    finish4(a, v, bias, m, n4, p.vector);
   }
   if ((!ok || bad) && threadIdx.x == 0) atomicExch(p.err, 22);
   tc::fence_before_sync();
@@ -607,16 +651,8 @@ constexpr int kStreamTokens = (512 - 32 * kStages) / 2;
 constexpr int kStreamDeep = 3;   // chunks of codes of a warp
 template <bool kG32>
 constexpr int kStreamCodes = 4 * kTurns * 2 * kStreamDeep * kCodeTile<kG32>;
-constexpr int kStaged = 16 * kWideRows * 2;   // 16 rows of y on their way to memory, twice for each four warps
 template <bool kG32>
 int stream_smem(int tokens) { return kStages * tokens * 128 + kStreamCodes<kG32> + 4 * kStaged + 1024; }
-
-// Whether any of the 128 threads at a barrier says so.
-__device__ __forceinline__ bool any_of_128(int barrier, bool mine) {
-  uint32_t any;
-  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbarrier.cta.red.or.pred p, %2, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(any) : "r"(mine ? 1u : 0u), "r"(barrier) : "memory");
-  return any != 0;
-}
 
 template <bool kG32>
 __global__ void __launch_bounds__(kStreamThreads, 1) w4_stream_kernel(const __grid_constant__ CUtensorMap x_map, Wide p) {
@@ -785,10 +821,8 @@ __global__ void __launch_bounds__(kStreamThreads, 1) w4_stream_kernel(const __gr
     }
     copy_wait<0>();
   } else {   // ---- results
-    const int quarter = warp & 3, four = (warp - 2 - 4 * kTurns) >> 2, thread = threadIdx.x & 127;
+    const int quarter = warp & 3, four = (warp - 2 - 4 * kTurns) >> 2;
     unsigned char* staged = smem + kStages * stage_bytes + kStreamCodes<kG32> + four * (2 * kStaged);   // [2][row of x][weight row]
-    __nv_bfloat16* y = static_cast<__nv_bfloat16*>(a.y);
-    const __nv_bfloat16* residual = static_cast<const __nv_bfloat16*>(a.residual);
     int i = 0, half = 0;
     for (int tile = blockIdx.x; tile < p.tiles; tile += gridDim.x, ++i) {
       const int block = tile / p.row_tiles, row0 = (tile - block * p.row_tiles) * p.tokens, n0 = block * kWideRows, n = n0 + quarter * 32 + lane;
@@ -799,40 +833,8 @@ __global__ void __launch_bounds__(kStreamThreads, 1) w4_stream_kernel(const __gr
       }
       tc::fence_after_sync();
       const uint32_t sums = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (i & 1) * kStreamTokens;
-      for (int c = four; c < p.tokens / 16; c += 2, half ^= 1) {
-        uint32_t r[16];
-        tmem_ld_32x16(sums + c * 16, r);
-        tc::tmem_ld_wait();
-        __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(staged + half * kStaged);
-        float v[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(r[e]) + bias;
-        if (a.gelu) {   // (the branches once and not for every element: 1100 clocks less)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) v[e] = 0.5f * v[e] * (1.f + erff(v[e] * 0.70710678118654752f));
-        }
-        if (a.residual && n < a.n) {
-          const int m0 = row0 + c * 16;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) v[e] += __bfloat162float(residual[min(m0 + e, a.m - 1) * a.ldr + n]);
-        }
-#pragma unroll
-        for (int e = 0; e < 16; ++e) to[e * kWideRows + quarter * 32 + lane] = __float2bfloat16_rn(v[e]);
-        asm volatile("bar.sync %0, 128;" ::"r"(1 + four) : "memory");
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {   // 8 rows at a time, 8 elements per thread
-          const int row = e * 8 + (thread >> 4), m = row0 + c * 16 + row, n8 = n0 + (thread & 15) * 8;
-          if (m < a.m && n8 < a.n) {
-            const __nv_bfloat16* from = to + row * kWideRows + (thread & 15) * 8;
-            __nv_bfloat16* out = y + static_cast<long long>(m) * a.n + n8;
-            if (p.vector) {
-              *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(from);
-            } else {
-              for (int k = 0; k < min(8, a.n - n8); ++k) out[k] = from[k];
-            }
-          }
-        }
-      }
+      for (int c = four; c < p.tokens / 16; c += 2, half ^= 1)
+        finish16(a, p.rows8, sums + c * 16, reinterpret_cast<__nv_bfloat16*>(staged + half * kStaged), 1 + four, row0 + c * 16, n0, quarter, lane, bias);
       // the products of the tile after next may begin
       tc::fence_before_sync();
       __syncwarp();
@@ -1063,7 +1065,7 @@ cudaError_t launch_wide(const W4Args& a, cudaStream_t on) {
   p.columns = p.tokens <= 32 ? 32 : (p.tokens <= 64 ? 64 : (p.tokens <= 128 ? 128 : 256));
   p.allocated = p.columns + kWideStages * 32 <= 256 ? 256 : 512;
   p.vector = a.n % 4 == 0 && (a.residual == nullptr || (a.ldr % 4 == 0 && reinterpret_cast<uintptr_t>(a.residual) % 8 == 0));
-  if (stream) p.vector = a.n % 8 == 0;   // of y alone
+  p.rows8 = a.n % 8 == 0;
   p.idesc = tc::idesc_bf16(kWideRows, p.tokens);
   p.err = gemm_error_device_ptr();
   const CuDriver& cu = CuDriver::get();
