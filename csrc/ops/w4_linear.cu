@@ -38,9 +38,17 @@ __device__ __forceinline__ uint32_t codes2(uint32_t w, uint32_t minus_zero2) {
   asm("fma.rn.bf16x2 %0, %0, %1, %2;" : "+r"(r) : "r"(0x3f803f80u), "r"(minus_zero2));
   return r;
 }
+// The same from 128 + zero itself.
+__device__ __forceinline__ uint32_t codes2_less(uint32_t w, uint32_t zero2) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(0x000f000fu), "r"(0x43004300u));
+  asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(r) : "r"(zero2), "r"(0xbf80bf80u));
+  return r;
+}
 // Of a row's parameters (scale, and above it 128 + zero) the scale, and either of them twice.
 __device__ __forceinline__ float scale_of(uint32_t p) { return __uint_as_float(p << 16); }
 __device__ __forceinline__ uint32_t scale2(uint32_t p) { return __byte_perm(p, 0, 0x1010); }
+__device__ __forceinline__ uint32_t zero2(uint32_t p) { return __byte_perm(p, 0, 0x3232); }
 __device__ __forceinline__ uint32_t minus_zero2(uint32_t p) { return __byte_perm(p, 0, 0x3232) ^ 0x80008000u; }
 
 template <int kBytes>
@@ -331,16 +339,39 @@ __device__ __forceinline__ void store_peer(uint32_t at, int rank, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there), "f"(v) : "memory");
 }
 
-// A lane's codes and parameters of chunk c of a tile to `to` and 512 bytes on; zeros of a tile that there is not.
+// Where a lane's codes and parameters of a chunk of a tile are.  The next chunk of the same warp is kTurns, 256 columns, on: a step that is the same for all.
+struct Ahead {
+  const uint4* codes;
+  const uint2* params;
+  uint32_t size;   // 16, or 0 for a tile that there is not: zeros
+};
+__device__ __forceinline__ void copy_sized16(uint32_t to, const void* from, uint32_t size) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(size) : "memory");
+}
+__device__ __forceinline__ void copy_sized8(uint32_t to, const void* from, uint32_t size) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(size) : "memory");
+}
 template <bool kG32>
-__device__ __forceinline__ void copy_tile(uint32_t to, int lane, const uint4* codes, const uint2* params, int c, int group_shift, int groups, bool there) {
-  copy_async<16>(to + lane * 16, codes + c * 32, there);
+__device__ __forceinline__ Ahead ahead_of(const W4Args& a, int chunks, int groups, int group_shift, int tile, int tiles, int c, int lane) {
+  Ahead at;
+  const bool there = tile < tiles;
+  at.codes = static_cast<const uint4*>(a.codes) + (static_cast<size_t>(there ? tile : 0) * chunks + c) * 32 + lane;
+  at.params = static_cast<const uint2*>(a.params) + (static_cast<size_t>(there ? tile : 0) * groups + (kG32 ? 2 * c : c * 64 >> group_shift)) * 8 + (lane >> 2);
+  at.size = there ? 16 : 0;
+  return at;
+}
+// A chunk's to `to` and 512 bytes on; `both`: with groups of 32, whether there is a second one.
+template <bool kG32>
+__device__ __forceinline__ void copy_tile(uint32_t to, int lane, Ahead& at, int params_step, bool both) {
+  copy_sized16(to + lane * 16, at.codes, at.size);
   if (kG32) {
-    copy_async<8>(to + 512 + lane * 16, params + 2 * c * 8, there);
-    copy_async<8>(to + 520 + lane * 16, params + min(2 * c + 1, groups - 1) * 8, there);
+    copy_sized8(to + 512 + lane * 16, at.params, at.size >> 1);
+    copy_sized8(to + 520 + lane * 16, at.params + (both ? 8 : 0), both ? at.size >> 1 : 0);
   } else {
-    copy_async<8>(to + 512 + lane * 8, params + (c * 64 >> group_shift) * 8, there);
+    copy_sized8(to + 512 + lane * 8, at.params, at.size >> 1);
   }
+  at.codes += kTurns * 32;
+  at.params += params_step;
 }
 template <bool kG32>
 __device__ __forceinline__ void take_tile(uint32_t from, int lane, uint4& codes, uint2 (&params)[2]) {
@@ -360,10 +391,10 @@ __device__ __forceinline__ void make_weights(uint32_t (&r)[16], const uint4& w, 
 #pragma unroll
   for (int step = 0; step < 4; ++step) {
     const uint2 q = prm[kG32 ? step >> 1 : 0];
-    r[4 * step] = mul2(codes2(word[step], minus_zero2(q.x)), scale2(q.x));
-    r[4 * step + 1] = mul2(codes2(word[step] >> 4, minus_zero2(q.y)), scale2(q.y));
-    r[4 * step + 2] = mul2(codes2(word[step] >> 8, minus_zero2(q.x)), scale2(q.x));
-    r[4 * step + 3] = mul2(codes2(word[step] >> 12, minus_zero2(q.y)), scale2(q.y));
+    r[4 * step] = mul2(codes2_less(word[step], zero2(q.x)), scale2(q.x));
+    r[4 * step + 1] = mul2(codes2_less(word[step] >> 4, zero2(q.y)), scale2(q.y));
+    r[4 * step + 2] = mul2(codes2_less(word[step] >> 8, zero2(q.x)), scale2(q.x));
+    r[4 * step + 3] = mul2(codes2_less(word[step] >> 12, zero2(q.y)), scale2(q.y));
   }
 }
 __device__ __forceinline__ void load_bias(float (&bias)[4], const W4Args& a, int n4) {
@@ -523,23 +554,19 @@ __global__ void __launch_bounds__(kWideThreads, 1) w4_wide_kernel(const __grid_c
     __syncwarp();
   } else {   // ---- weights: kTurns warps for each 32 rows take chunks in turn
     static_assert(kTurns == kWideStages);   // a warp's stage is always the same
-    const int quarter = warp & 3, turn = (warp - 2) >> 2, g = lane >> 2;
+    const int quarter = warp & 3, turn = (warp - 2) >> 2;
     const int row_tiles = (a.n + 15) / 16, groups = a.k >> p.group_shift, tile0 = blockIdx.x * (kWideRows / 16) + quarter * 2;
-    const bool there[2] = {tile0 < row_tiles, tile0 + 1 < row_tiles};
     constexpr int kDeep = kCodeDeep<kG32>, kTile = kCodeTile<kG32>;
     const uint32_t ring = tc::smem_u32(smem) + kWideStages * stage_bytes + (warp - 2) * (kDeep * 2 * kTile);
     const uint32_t place = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + p.columns + turn * 32;
-    const uint4* codes[2];
-    const uint2* params[2];
+    const int params_step = kTurns * 64 >> p.group_shift << 3;
+    Ahead at[2];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {   // of a tile that there is not, the first one's: nothing of it is used
-      codes[k] = static_cast<const uint4*>(a.codes) + (there[k] ? static_cast<size_t>(tile0 + k) * p.chunks * 32 : 0) + lane;
-      params[k] = static_cast<const uint2*>(a.params) + (there[k] ? static_cast<size_t>(tile0 + k) * groups * 8 : 0) + g;
-    }
+    for (int k = 0; k < 2; ++k) at[k] = ahead_of<kG32>(a, p.chunks, groups, p.group_shift, tile0 + k, row_tiles, first + turn, lane);
     auto issue = [&](int c, int slot) {
       if (c < last) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) copy_tile<kG32>(ring + (slot * 2 + k) * kTile, lane, codes[k], params[k], c, p.group_shift, groups, there[k]);
+        for (int k = 0; k < 2; ++k) copy_tile<kG32>(ring + (slot * 2 + k) * kTile, lane, at[k], params_step, 2 * c + 1 < groups);
       }
       copy_commit();
     };
@@ -749,42 +776,36 @@ __global__ void __launch_bounds__(kStreamThreads, 1) w4_stream_kernel(const __gr
     }
     __syncwarp();
   } else if (warp < 2 + 4 * kTurns) {   // ---- weights; chunks are counted through all tiles, so that a warp's stage is always the same
-    const int quarter = warp & 3, turn = (warp - 2) >> 2, g = lane >> 2;
+    const int quarter = warp & 3, turn = (warp - 2) >> 2;
     const int tiles16 = (a.n + 15) / 16, groups = a.k >> p.group_shift;
     constexpr int kDeep = kStreamDeep, kTile = kCodeTile<kG32>;
     const uint32_t ring = tc::smem_u32(smem) + kStages * stage_bytes + (warp - 2) * (kDeep * 2 * kTile);
     const uint32_t place = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + kWeights;
     // the loading side: a chunk of a tile, and where its codes and parameters are
     int tile = blockIdx.x, c = turn;
-    bool there[2];
-    const uint4* codes;
-    const uint2* params;
-    auto at_tile = [&]() {
-      const int tile0 = tile / p.row_tiles * (kWideRows / 16) + quarter * 2;
-      there[0] = tile0 < tiles16;
-      there[1] = tile0 + 1 < tiles16;
-      codes = static_cast<const uint4*>(a.codes) + (there[0] ? static_cast<size_t>(tile0) * p.chunks * 32 : 0) + lane;
-      params = static_cast<const uint2*>(a.params) + (there[0] ? static_cast<size_t>(tile0) * groups * 8 : 0) + g;
-    };
-    auto settle = [&]() {
-      if (c < p.chunks) return;
-      do {
+    const int params_step = kTurns * 64 >> p.group_shift << 3;
+    Ahead at[2];
+    auto settle = [&]() {   // after a tile's end: on to the tile that chunk c is one of
+      while (c >= p.chunks) {
         c -= p.chunks;
         tile += gridDim.x;
-      } while (c >= p.chunks);
-      if (tile < p.tiles) at_tile();
+      }
+      if (tile < p.tiles) {
+        const int tile0 = tile / p.row_tiles * (kWideRows / 16) + quarter * 2;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) at[k] = ahead_of<kG32>(a, p.chunks, groups, p.group_shift, tile0 + k, tiles16, c, lane);
+      }
     };
     // this warp's chunks among those of all the block's tiles
     const int mine = (p.tiles - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x) * p.chunks;
-    at_tile();
     settle();
     auto issue = [&](int slot) {
       if (tile < p.tiles) {
         const uint32_t to = ring + slot * (2 * kTile);
-        copy_tile<kG32>(to, lane, codes, params, c, p.group_shift, groups, there[0]);
-        copy_tile<kG32>(to + kTile, lane, codes + (there[1] ? p.chunks * 32 : 0), params + (there[1] ? groups * 8 : 0), c, p.group_shift, groups, there[1]);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) copy_tile<kG32>(to + k * kTile, lane, at[k], params_step, 2 * c + 1 < groups);
         c += kTurns;
-        settle();
+        if (c >= p.chunks) settle();
       }
       copy_commit();
     };
