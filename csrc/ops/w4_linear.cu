@@ -29,17 +29,10 @@ __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
   const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-// Two codes (bits 0-3 and 16-19) as a bf16 pair code - zero: 0x4300 is 128, whose last mantissa bit is worth one.  Both steps are written out, one
-// instruction each: the mask and the exponent in one three-input operation, the difference (exact) as a product with one and a sum, on the pipe
-// that does no logic.
-__device__ __forceinline__ uint32_t codes2(uint32_t w, uint32_t minus_zero2) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(0x000f000fu), "r"(0x43004300u));
-  asm("fma.rn.bf16x2 %0, %0, %1, %2;" : "+r"(r) : "r"(0x3f803f80u), "r"(minus_zero2));
-  return r;
-}
-// The same from 128 + zero itself.
-__device__ __forceinline__ uint32_t codes2_less(uint32_t w, uint32_t zero2) {
+// Two codes (bits 0-3 and 16-19) as a bf16 pair code - zero, from 128 + zero: 0x4300 is 128, whose last mantissa bit is worth one.  Both steps are written
+// out, one instruction each: the mask and the exponent in one three-input operation, the difference (exact) as a product with minus one and a sum, on the
+// pipe that does no logic.
+__device__ __forceinline__ uint32_t codes2(uint32_t w, uint32_t zero2) {
   uint32_t r;
   asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(0x000f000fu), "r"(0x43004300u));
   asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(r) : "r"(zero2), "r"(0xbf80bf80u));
@@ -49,7 +42,6 @@ __device__ __forceinline__ uint32_t codes2_less(uint32_t w, uint32_t zero2) {
 __device__ __forceinline__ float scale_of(uint32_t p) { return __uint_as_float(p << 16); }
 __device__ __forceinline__ uint32_t scale2(uint32_t p) { return __byte_perm(p, 0, 0x1010); }
 __device__ __forceinline__ uint32_t zero2(uint32_t p) { return __byte_perm(p, 0, 0x3232); }
-__device__ __forceinline__ uint32_t minus_zero2(uint32_t p) { return __byte_perm(p, 0, 0x3232) ^ 0x80008000u; }
 
 template <int kBytes>
 __device__ __forceinline__ void copy_async(uint32_t to, const void* from, bool real = true) {
@@ -217,7 +209,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 2) w4_narrow_kernel(W4Args a, 
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
             const uint2 q = p[r][kParams == 4 ? 2 * j + (s >> 1) : (kParams == 2 ? j : 0)];
-            const uint32_t z0 = minus_zero2(q.x), z8 = minus_zero2(q.y);
+            const uint32_t z0 = zero2(q.x), z8 = zero2(q.y);
             const uint32_t a0 = codes2(word[s], z0), a1 = codes2(word[s] >> 4, z8), a2 = codes2(word[s] >> 8, z0), a3 = codes2(word[s] >> 12, z8);
             const bool begins = kParams == 4 ? (s & 1) == 0 : s == 0, ends = kParams == 4 ? (s & 1) == 1 : s == 3;
 #pragma unroll
@@ -391,10 +383,10 @@ __device__ __forceinline__ void make_weights(uint32_t (&r)[16], const uint4& w, 
 #pragma unroll
   for (int step = 0; step < 4; ++step) {
     const uint2 q = prm[kG32 ? step >> 1 : 0];
-    r[4 * step] = mul2(codes2_less(word[step], zero2(q.x)), scale2(q.x));
-    r[4 * step + 1] = mul2(codes2_less(word[step] >> 4, zero2(q.y)), scale2(q.y));
-    r[4 * step + 2] = mul2(codes2_less(word[step] >> 8, zero2(q.x)), scale2(q.x));
-    r[4 * step + 3] = mul2(codes2_less(word[step] >> 12, zero2(q.y)), scale2(q.y));
+    r[4 * step] = mul2(codes2(word[step], zero2(q.x)), scale2(q.x));
+    r[4 * step + 1] = mul2(codes2(word[step] >> 4, zero2(q.y)), scale2(q.y));
+    r[4 * step + 2] = mul2(codes2(word[step] >> 8, zero2(q.x)), scale2(q.x));
+    r[4 * step + 3] = mul2(codes2(word[step] >> 12, zero2(q.y)), scale2(q.y));
   }
 }
 __device__ __forceinline__ void load_bias(float (&bias)[4], const W4Args& a, int n4) {
@@ -892,7 +884,7 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(const uint4* __restr
       for (int j = 0; j < 4; ++j) {   // nibble j: row g + 8 (j & 1), columns 8 (j >> 1) on
         const int row = tile * 16 + (j & 1) * 8 + g;
         const uint32_t prm = j & 1 ? p.y : p.x;
-        if (row < n) *reinterpret_cast<uint32_t*>(w + static_cast<size_t>(row) * k + at + (j >> 1) * 8) = mul2(codes2(word[s] >> (4 * j), minus_zero2(prm)), scale2(prm));
+        if (row < n) *reinterpret_cast<uint32_t*>(w + static_cast<size_t>(row) * k + at + (j >> 1) * 8) = mul2(codes2(word[s] >> (4 * j), zero2(prm)), scale2(prm));
       }
     }
   }
