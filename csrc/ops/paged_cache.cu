@@ -43,6 +43,16 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(AppendArgs a, in
   const T* k = static_cast<const T*>(a.k.p) + t * a.k.token + d8 * 8;
   const T* v = static_cast<const T*>(a.v.p) + t * a.v.token + d8 * 8;
   const T* q = static_cast<const T*>(a.q.p) + t * a.q.token + d8 * 8;
+  int h0 = at_row - in_block * all_heads;
+  uint4 raw[kDeep];
+  auto load = [&]() {
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i) {
+      const int h = h0 + i * rows;
+      if (h < all_heads) raw[i] = __ldg(reinterpret_cast<const uint4*>(h < kv ? k + h * a.k.head : (h < 2 * kv ? v + (h - kv) * a.v.head : q + (h - 2 * kv) * a.q.head)));
+    }
+  };
+  load();   // before anything is waited for
   const int pos = __ldg(a.positions + t), row = a.rows ? __ldg(a.rows + t) : static_cast<int>(t);
   const int ps = a.table.page_size, slot = pos >= 0 ? pos / ps : 0;
   const bool inside = pos >= 0 && row >= 0 && row < a.table.rows && slot < a.table.width && (a.cos == nullptr || pos < a.rope_rows);
@@ -61,13 +71,7 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(AppendArgs a, in
   T* to_k = static_cast<T*>(a.k_pages.p) + place * a.k_pages.page + at * a.k_pages.token + d8 * 8;
   T* to_v = static_cast<T*>(a.v_pages.p) + place * a.v_pages.page + at * a.v_pages.token + d8 * 8;
   T* to_q = static_cast<T*>(a.q_out) + t * a.heads * a.head_dim + d8 * 8;
-  for (int h0 = at_row - in_block * all_heads; h0 < all_heads; h0 += kDeep * rows) {
-    uint4 raw[kDeep];
-#pragma unroll
-    for (int i = 0; i < kDeep; ++i) {
-      const int h = h0 + i * rows;
-      if (h < all_heads) raw[i] = __ldg(reinterpret_cast<const uint4*>(h < kv ? k + h * a.k.head : (h < 2 * kv ? v + (h - kv) * a.v.head : q + (h - 2 * kv) * a.q.head)));
-    }
+  while (true) {
 #pragma unroll
     for (int i = 0; i < kDeep; ++i) {
       const int h = h0 + i * rows;
@@ -84,6 +88,9 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(AppendArgs a, in
       else if (good)
         *reinterpret_cast<uint4*>(value ? to_v + (h - kv) * a.v_pages.head : to_k + h * a.k_pages.head) = raw[i];
     }
+    h0 += kDeep * rows;
+    if (h0 >= all_heads) break;
+    load();
   }
 }
 
