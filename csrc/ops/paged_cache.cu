@@ -27,11 +27,12 @@ __device__ __forceinline__ void rotate_pairs(float (&f)[8], const float4& c, con
 
 // A token's heads are k's, v's and, where q is rotated, q's.  A thread has eight elements of a head, the same eight of every `rows`-th head of one token: it
 // follows the token's place (position, row, page), takes its part of the rotation and works out addresses once, and its loads are all under way before
-// the first result.  A block has one token, or as many as it has threads for.  64 tokens of 48 heads of 128: 2.6 us (3.2 with a place per 16 bytes), 1537 of
-// them, 38 MB: 11.0 us (12.4), of which 2.5 are the launch: 4.5 TB/s.  (Blocks that go from token to token and look two places ahead: 2.9 and 10.8 us.)
+// that and the first result.  A block has one token, or as many as it has threads for.  64 tokens of 48 heads of 128: 2.5 us (3.2 with a place per 16 bytes),
+// 1537 of them, 38 MB: 9.2 us, of which 2.5 are the launch: 5.6 TB/s.  (Four loads ahead 9.4; loads behind the position's 11.0; blocks that go from token to token and
+// look two places ahead 10.8, and 2.9 for the 64.)
 template <typename H>
 __global__ void __launch_bounds__(kThreads) paged_append_kernel(AppendArgs a, int per_block, int rows, int all_heads, Divisor by_heads, Divisor by_hd8) {
-  constexpr int kDeep = 4;
+  constexpr int kDeep = 3;
   ::mccl::pdl_wait();
   ::mccl::pdl_trigger();
   const int at_row = by_hd8.of(threadIdx.x), d8 = threadIdx.x - at_row * by_hd8.d;
@@ -138,13 +139,16 @@ cudaError_t paged_append(const AppendArgs& a, cudaStream_t stream) {
   const int hd8 = a.head_dim / 8, all_heads = 2 * a.kv_heads + (a.q_out ? a.heads : 0);
   if (hd8 <= 0 || all_heads <= 0) return cudaSuccess;
   if (hd8 > kThreads) return cudaErrorNotSupported;
-  const int rows = kThreads / hd8, per_block = all_heads < rows ? rows / all_heads : 1;
+  // Tokens for several rounds of SMs take half as many threads each, whose blocks come and go more evenly (1537 tokens of 48 heads of 128 9.2 us, 9.8 with
+  // all; 2048 of 36 heads of 64 5.1 and 7.5); fewer tokens finish sooner with all (64 tokens 2.5 and 3.2 us, 600 4.4 and 4.7).
+  const int threads = a.tokens >= 5 * 148 && hd8 <= kThreads / 2 ? kThreads / 2 : kThreads;
+  const int rows = threads / hd8, per_block = all_heads < rows ? rows / all_heads : 1;
   const long long blocks = (a.tokens + per_block - 1) / per_block;
   if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
   if (a.type == Half16::bf16)
-    MCCL_LAUNCH_PDL(paged_append_kernel<Bf16>, static_cast<unsigned>(blocks), kThreads, 0, stream, a, per_block, rows, all_heads, Divisor(all_heads), Divisor(hd8));
+    MCCL_LAUNCH_PDL(paged_append_kernel<Bf16>, static_cast<unsigned>(blocks), threads, 0, stream, a, per_block, rows, all_heads, Divisor(all_heads), Divisor(hd8));
   else
-    MCCL_LAUNCH_PDL(paged_append_kernel<Fp16>, static_cast<unsigned>(blocks), kThreads, 0, stream, a, per_block, rows, all_heads, Divisor(all_heads), Divisor(hd8));
+    MCCL_LAUNCH_PDL(paged_append_kernel<Fp16>, static_cast<unsigned>(blocks), threads, 0, stream, a, per_block, rows, all_heads, Divisor(all_heads), Divisor(hd8));
   count_launch();
   return ::mccl::launch_status();
 }
