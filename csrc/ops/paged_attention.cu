@@ -675,14 +675,19 @@ __global__ void __launch_bounds__(128) paged_attention_join_kernel(Launch p) {
   const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes, c0 = blockIdx.x, row = blockIdx.y;
   ::mccl::pdl_wait();
   ::mccl::pdl_trigger();
+  // a thread's first part is on its way before it is known whether there is one (there is room for it)
+  const size_t first = (static_cast<size_t>(min(c0 + group, static_cast<int>(gridDim.x) - 1)) * 2 + (group == 0)) * ROWS + row;
+  const float2 first_ml = *reinterpret_cast<const float2*>(p.part_ml + first * 2);
+  const float4 first_o = *reinterpret_cast<const float4*>(p.part_o + first * DP + lane * 4);
   const int2 open = p.open[c0];
   if (open.x < 0) return;
   const int b = p.items.of(open.x), hh = open.x - b * p.items.d, kv = p.head_blocks.of(hh), in_group = (hh - kv * p.head_blocks.d) * ROWS;
   if (in_group + row >= p.group) return;
   Sums sum;
+  if (c0 + group <= open.y) sum.add(first_ml.x, first_ml.y, first_o);
 #pragma unroll 4
-  for (int c = c0 + group; c <= open.y; c += kGroups) {
-    const size_t slot = (static_cast<size_t>(c) * 2 + (c == c0)) * ROWS + row;
+  for (int c = c0 + group + kGroups; c <= open.y; c += kGroups) {
+    const size_t slot = static_cast<size_t>(c) * 2 * ROWS + row;
     const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
     sum.add(ml.x, ml.y, *reinterpret_cast<const float4*>(p.part_o + slot * DP + lane * 4));
   }
