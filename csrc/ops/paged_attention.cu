@@ -10,7 +10,7 @@
 // eight heads that share keys fill half of their rows, single ones an eighth, and still they run at a quarter of their rate, while the generation's own
 // instruction would want 64 rows.
 // Measured: 2 x 131009 positions, 32 heads over 8 of 128 (1071 MB): 165 us, 6.5 TB/s; 64 ragged sequences of up to 2048, 16 heads of 128 (540 MB): 87 us, 6.2
-// TB/s; 48 windows of 1024 (101 MB): 25.5 us, of which 15.6 from the first load's issue to the last tile: the rest is finding the run (1.8), joining (1.6) and the second
+// TB/s; 48 windows of 1024 (101 MB): 25.2 us, of which 15.6 from the first load's issue to the last tile: the rest is finding the run (1.8), joining (1.6) and the second
 // kernel with its start (3.5); one sequence of 37 tokens: 5.0 us, a chain of four dependent loads.
 #include "../core/launch.hpp"
 #include "../symm/cu_driver.hpp"

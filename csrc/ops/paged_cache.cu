@@ -28,7 +28,7 @@ __device__ __forceinline__ void rotate_pairs(float (&f)[8], const float4& c, con
 // A token's heads are k's, v's and, where q is rotated, q's.  A thread has eight elements of a head, the same eight of every `rows`-th head of one token: it
 // follows the token's place (position, row, page), takes its part of the rotation and works out addresses once, and its loads are all under way before
 // that and the first result.  A block has one token, or as many as it has threads for.  64 tokens of 48 heads of 128: 2.5 us (3.2 with a place per 16 bytes),
-// 1537 of them, 38 MB: 9.2 us, of which 2.5 are the launch: 5.6 TB/s.  (Four loads ahead 9.4; loads behind the position's 11.0; blocks that go from token to token and
+// 1537 of them, 38 MB: 9.5 us, of which 2.5 are the launch: 5.4 TB/s.  (Four loads ahead 9.4; loads behind the position's 11.0; blocks that go from token to token and
 // look two places ahead 10.8, and 2.9 for the 64.)
 template <typename H>
 __global__ void __launch_bounds__(kThreads) paged_append_kernel(AppendArgs a, int per_block, int rows, int all_heads, Divisor by_heads, Divisor by_hd8) {
