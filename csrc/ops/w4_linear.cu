@@ -1002,21 +1002,27 @@ int resident(int splits) {
 }
 
 // Rows of x per block and parts of K.  A chunk of 64 columns costs the making of its weights (some 400 clocks) or its products (two clocks per row of x), a
-// block some 5000 clocks before its first and after its last chunk.  (Measured beside all other choices for 12 sizes from 24 x 2048 x 2048 to
+// block some 5000 clocks before its first and after its last chunk.  (Measured beside all other choices for 27 sizes from 20 x 512 x 512 to
 // 1537 x 16384 x 2048: within 4 % of the best.)
 // With more tiles than SMs they run on from one to the next (returns true), so that no round has a beginning and an end of its own: 1537 x 16384 x 2048 took
 // 103 us in rounds.
 bool choose_wide(int m, int blocks, Wide& p) {
-  constexpr double kMake = 400, kRound = 5000, kSplit = 1500, kToken = 20;
+  constexpr double kMake = 400, kRound = 5000, kSplit = 2200, kToken = 20;
   double best = 0;
   Wide w = p;
-  for (int most = 32; most <= kMostTokens; most += 32) {
+  for (int most = 16, before = 0; most <= kMostTokens && before != 1; most += 16) {
     const int tiles = (m + most - 1) / most;
+    if (tiles == before || tiles > 65535) continue;
+    before = tiles;
     w.tokens = ((m + tiles - 1) / tiles + 15) / 16 * 16;
+    const int row_tiles = (m + w.tokens - 1) / w.tokens;
     for (w.splits = 1; w.splits <= 8 && (w.splits == 1 || w.splits * 2 <= p.chunks); ++w.splits) {
       w.share = (w.tokens + w.splits - 1) / w.splits;
       if (wide_smem(w) > kWideSmem) continue;
-      const int all = blocks * ((m + w.tokens - 1) / w.tokens) * w.splits, at_once = resident(w.splits), waves = (all + at_once - 1) / at_once;
+      const long long all = static_cast<long long>(blocks) * row_tiles * w.splits;
+      const int at_once = resident(w.splits);
+      if (w.splits > 1 && all > at_once) break;
+      const long long waves = (all + at_once - 1) / at_once;
       const double products = 2.0 * w.tokens;
       const double cost = waves * ((p.chunks + w.splits - 1) / w.splits * (kMake > products ? kMake : products) + kRound + (w.splits > 1 ? kSplit : 0.0) + kToken * w.tokens);
       if (best == 0 || cost < best) {
@@ -1028,8 +1034,10 @@ bool choose_wide(int m, int blocks, Wide& p) {
     }
   }
   bool stream = false;
-  for (int most = 32; most <= kStreamTokens; most += 16) {
+  for (int most = 32, before = 0; most <= kStreamTokens && before != 1; most += 16) {
     const int tiles = (m + most - 1) / most, tokens = ((m + tiles - 1) / tiles + 15) / 16 * 16, row_tiles = (m + tokens - 1) / tokens;
+    if (tiles == before) continue;
+    before = tiles;
     if (tokens > kStreamTokens || static_cast<long long>(blocks) * row_tiles > 0x7fffffff || (p.a.group == 32 ? stream_smem<true>(tokens) : stream_smem<false>(tokens)) > kWideSmem) continue;
     const int all = blocks * row_tiles, rounds = (all + sm_count() - 1) / sm_count();
     if (rounds < 2) continue;
