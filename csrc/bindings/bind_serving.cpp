@@ -99,6 +99,16 @@ ops::TokenView tokens_of(const at::Tensor& t, const char* what) {
   return {t.data_ptr(), t.stride(0), t.stride(1)};
 }
 
+// A 4-bit weight as the kernels read it: 16 bytes of codes and 8 of parameters at a time.
+void need_w4(const at::Tensor& codes, const at::Tensor& params, int64_t n, int64_t k, int64_t group, const char* op) {
+  MCCL_CHECK_TENSOR((group == 32 || group == 64 || group == 128 || group == 256) && n >= 0 && k >= 0 && k % group == 0 && codes.is_contiguous() && params.is_contiguous() &&
+                        codes.numel() * static_cast<int64_t>(codes.element_size()) == (n + 15) / 16 * ((k + 63) / 64) * 512 && params.scalar_type() == at::kInt &&
+                        params.numel() == (n + 15) / 16 * (k / group) * 16,
+                    op << ": the weight is not laid out for [" << n << ", " << k << "]");
+  MCCL_CHECK_TENSOR(reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(params.data_ptr()) % 8 == 0,
+                    op << ": codes must begin on a 16-byte boundary, parameters on one of 8 bytes");
+}
+
 }  // namespace
 
 void bind_serving(py::module_& m) {
@@ -253,9 +263,7 @@ void bind_serving(py::module_& m) {
         need_forward_only(x, op);
         MCCL_CHECK_TENSOR(x.scalar_type() == at::kBFloat16, op << ": expected bf16, got " << c10::toString(x.scalar_type()));
         MCCL_CHECK_TENSOR(x.dim() >= 1 && x.size(-1) == k, op << ": x must have " << k << " columns");
-        MCCL_CHECK_TENSOR(codes.is_contiguous() && params.is_contiguous() && codes.numel() * static_cast<int64_t>(codes.element_size()) == (n + 15) / 16 * ((k + 63) / 64) * 512 &&
-                              params.scalar_type() == at::kInt && group > 0 && params.numel() == (n + 15) / 16 * (k / group) * 16,
-                          op << ": the weight is not laid out for [" << n << ", " << k << "]");
+        need_w4(codes, params, n, k, group, op);
         c10::cuda::CUDAGuard guard(x.device());
         at::Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, k});
         if (!vector_rows(x2)) x2 = x2.clone(at::MemoryFormat::Contiguous);
@@ -328,9 +336,7 @@ void bind_serving(py::module_& m) {
       [](const at::Tensor& codes, const at::Tensor& params, int64_t n, int64_t k, int64_t group) {
         need_on(codes, codes, "w4_dequantize");
         need_on(params, codes, "w4_dequantize");
-        MCCL_CHECK_TENSOR(codes.is_contiguous() && params.is_contiguous() && codes.numel() * static_cast<int64_t>(codes.element_size()) == (n + 15) / 16 * ((k + 63) / 64) * 512 &&
-                              params.scalar_type() == at::kInt && group > 0 && params.numel() == (n + 15) / 16 * (k / group) * 16,
-                          "w4_dequantize: the weight is not laid out for [" << n << ", " << k << "]");
+        need_w4(codes, params, n, k, group, "w4_dequantize");
         c10::cuda::CUDAGuard guard(codes.device());
         at::Tensor w = empty_on(codes, {n, k}, at::kBFloat16);
         check_launch(ops::w4_dequantize(codes.data_ptr(), params.data_ptr(), w.data_ptr(), as_int(n, "w4_dequantize"), as_int(k, "w4_dequantize"),

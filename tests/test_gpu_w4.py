@@ -170,3 +170,19 @@ def test_refusals():
     for args in ((torch.zeros(4, 100), 64), (torch.zeros(4, 96), 48), (torch.zeros(64), 64)):
         with pytest.raises(RuntimeError, match="quantize_w4"):
             ops.quantize_w4(*args)
+
+
+def test_refuses_weights_off_their_boundaries():
+    weight, w = make(64, 128, 64)
+    x = x_of(2, 128)
+    shifted = torch.zeros(weight.codes.numel() + 8, dtype=torch.uint8, device="cuda")[8:].view(weight.codes.shape)
+    odd = torch.zeros(weight.params.numel() + 1, dtype=torch.int32, device="cuda")[1:].view(weight.params.shape)
+    for codes, params in ((shifted, weight.params), (weight.codes, odd)):
+        moved = ops.W4Weight(codes, params, 64, 128, 64)
+        with pytest.raises(RuntimeError, match="boundary"):
+            ops.linear_w4(x, moved)
+        with pytest.raises(RuntimeError, match="boundary"):
+            moved.dequantize()
+    for group in (48, 16, 512):
+        with pytest.raises(RuntimeError, match="laid out"):
+            ops.linear_w4(x, ops.W4Weight(weight.codes, weight.params, 64, 128, group))
