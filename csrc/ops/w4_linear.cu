@@ -5,9 +5,9 @@
 // 16 bits.  Its time is that of taking the codes apart: some 190 instructions per KB.  For more rows bf16 weights, scale * (code - zero) rounded once, are
 // made on the way into tensor memory, where they are the left operand of tcgen05 products: a block per tile and part of K where that fills the SMs (the wide
 // kernel), a block per SM that runs on from tile to tile where there are several for each (the stream kernel).  For 16384 x 2048 the
-// narrow kernel takes 7.4 us for 8 rows and 10.2 for 16, the wide one 9.9 for up to 32: where they meet the narrow one stays, which rounds no weights.
-// Measured (codes from memory): 4 x 32000 x 2048, 36 MB: 12.8 us, 2.8 TB/s; 1 x 16384 x 2048: 6.5 us; 1 x 2048 x 2048: 2.6 us, a launch and one chain of loads;
-// 48 x 3072 x 768: 5.1 us; 128 x 16384 x 2048: 12.3 us, 0.70 PFLOP/s; 256: 17.4 us; 1537: 81 us, 1.27 PFLOP/s.
+// narrow kernel takes 7.4 us for 8 rows and 10.3 for 16, the wide one 9.6 for up to 32: where they meet the narrow one stays, which rounds no weights.
+// Measured (codes from memory): 4 x 32000 x 2048, 36 MB: 12.7 us, 2.8 TB/s; 1 x 16384 x 2048: 6.5 us; 1 x 2048 x 2048: 2.6 us, a launch and one chain of loads;
+// 48 x 3072 x 768: 5.0 us; 128 x 16384 x 2048: 11.3 us, 0.76 PFLOP/s; 256: 16.0 us; 1537: 80 us, 1.29 PFLOP/s.
 #include <cuda.h>
 
 #include <array>
@@ -659,7 +659,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) w4_wide_kernel(const __grid_c
 // ------------------------------------------------- tiles for several rounds of SMs --
 // The same products for more tiles than there are SMs: a block takes tiles gridDim.x apart, and its four roles run on from one to the next.  Two sets of
 // sums in tensor memory (up to 176 rows of x each, behind them five chunks of weights: 512 columns) let eight warps of their own write a tile's results beside
-// the next one's products.  1537 x 16384 x 2048 takes 81 us, 1.27 PFLOP/s (89 when it goes on for seconds and the power limit lowers the clock): 500 clocks per
+// the next one's products.  1537 x 16384 x 2048 takes 80 us, 1.29 PFLOP/s (89 and more when it goes on for seconds and the power limit lowers the clock): 500 clocks per
 // chunk, of which the products want 352.  No role alone is the rest: with a quarter of the products it takes 69 us, with weights that cost no arithmetic 71,
 // with x that need not come 73.  (As one block per tile each round of SMs took 5 us before its first and after its last product: 103 us; four stages 83, six and
 // fewer rows 87; rings of their own for x and weights, whose stages are then variables to the issuing thread, 99.)
@@ -1108,7 +1108,7 @@ cudaError_t w4_linear(const W4Args& a, cudaStream_t stream) {
   if (a.m <= 0 || a.n <= 0) return cudaSuccess;
   const long long x_bytes = static_cast<long long>(a.m) * ((a.k + 127) / 128) * 256;
   if (a.m <= 16 && x_bytes <= 128 * 1024) {
-    // two tiles of weights per warp share what is read of x (1 x 16384 x 2048 6.5 us, 7.9 with one; 4 x 32000 x 2048 12.8 and 14.3), if that leaves every SM some
+    // two tiles of weights per warp share what is read of x (1 x 16384 x 2048 6.5 us, 7.9 with one; 4 x 32000 x 2048 12.7 and 14.3), if that leaves every SM some
     // warps' work (1 x 2048 x 2048: 2.6 with one); 16 rows' sums leave no registers for it
     const bool two = a.n >= 16 * 3 * sm_count();
     if (a.m <= 8) return two ? narrow<2, 1>(a, stream) : narrow<1, 1>(a, stream);
