@@ -80,16 +80,16 @@ class PagedKVCache:
 
     def reserve(self, rows: Sequence[int], lengths: Sequence[int]) -> None:
         """Pages for the first ``lengths[i]`` positions of each sequence.  Nothing changes when there are not enough."""
-        need = []
+        need: Dict[int, int] = {}
         for row, length in zip(rows, lengths):
             self._known(row)
             if length > self.max_positions:
                 raise RuntimeError(f"PagedKVCache: {length} positions, at most {self.max_positions} were asked for")
-            need.append(max(0, -(-length // self.page_size) - len(self._rows[row])))
-        if sum(need) > len(self._free):
-            raise RuntimeError(f"PagedKVCache: {sum(need)} pages needed, {len(self._free)} of {len(self._owners)} free")
+            need[row] = max(need.get(row, 0), -(-length // self.page_size) - len(self._rows[row]))   # a row may be named more than once
+        if sum(need.values()) > len(self._free):
+            raise RuntimeError(f"PagedKVCache: {sum(need.values())} pages needed, {len(self._free)} of {len(self._owners)} free")
         at, new = [], []
-        for row, n in zip(rows, need):
+        for row, n in need.items():
             for _ in range(n):
                 page = self._free.pop()
                 self._owners[page] = 1
