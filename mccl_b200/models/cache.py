@@ -100,6 +100,8 @@ class PagedKVCache:
 
     def advance(self, rows: Sequence[int], count: int) -> None:
         """Notes on the host that each sequence has `count` more positions (``lengths`` is the caller's: kernels that append know it first)."""
+        if count < 0:
+            raise RuntimeError(f"PagedKVCache: {count} more positions; set_length() makes a sequence shorter")
         for row in rows:
             self._known(row)
             if -(-(self._length[row] + count) // self.page_size) > len(self._rows[row]):
@@ -108,10 +110,13 @@ class PagedKVCache:
             self._length[row] += count
 
     def set_length(self, row: int, length: int) -> None:
-        """The sequence's length, on the host and on the device."""
+        """The sequence's length, on the host and on the device.  A sequence that goes back among pages it shares keeps the whole ones before its new
+        end; of the one that holds the end it gets a copy, and those behind it are the others' from then on (``reserve`` gives new ones)."""
         self._known(row)
         if length < 0 or -(-length // self.page_size) > len(self._rows[row]):
             raise RuntimeError(f"PagedKVCache: row {row} has no pages for {length} positions")
+        if length < self._length[row]:
+            self._go_back(row, length)
         self._length[row] = length
         self.lengths[row] = length
 
@@ -188,6 +193,29 @@ class PagedKVCache:
         return used
 
     # -------------------------------------------------------------------------------------------------------------- inside --
+    def _go_back(self, row: int, length: int) -> None:
+        """No page that the sequence will write from position `length` on has another owner.  (``fork`` shares pages in front of both sequences'
+        ends only, so this is where such a page can come to lie behind one.)"""
+        pages = self._rows[row]
+        full, end = length // self.page_size, -(-length // self.page_size)
+        own = [page for page in pages[end:] if page >= 0 and self._owners[page] == 1]
+        cut = pages[full] if end > full and pages[full] >= 0 and self._owners[pages[full]] > 1 else None
+        if cut is None and len(own) == len(pages) - end:
+            return
+        if cut is not None:
+            if not own and not self._free:
+                raise RuntimeError(f"PagedKVCache: 1 page needed, 0 of {len(self._owners)} free")
+            copy = own.pop(0) if own else self._free.pop()
+            ops.copy_pages(self.pages, self._numbers([cut]), self._numbers([copy]), dim=2)
+        kept = pages[:full] + ([] if end == full else [pages[full] if cut is None else copy]) + own
+        for page in pages[full:]:
+            if page >= 0 and self._owners[page] > 1:
+                self._owners[page] -= 1
+        if cut is not None:
+            self._owners[copy] = 1
+        self._rows[row] = kept
+        self._write([(row, i) for i in range(full, len(pages))], kept[full:] + [-1] * (len(pages) - len(kept)))
+
     def _drop(self, page: int) -> int:
         if page < 0:
             return 0

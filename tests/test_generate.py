@@ -221,3 +221,20 @@ def test_refusals():
             call()
     assert gen.cache.rows == [row] and gen.cache.length(row) == 2 and gen.cache.free_pages == 2
     assert gen.step([], []).shape == (0, 512)
+
+
+def test_a_fork_that_goes_back():
+    torch.manual_seed(4)
+    model = sharpen(build_decoder("tiny"))
+    prompt = list(range(16))
+    gen, alone = Generator(model, max_sequences=3, page_size=8), Generator(model, max_sequences=3, page_size=8)
+    a, _ = gen.prefill(prompt)
+    (b,) = gen.fork(a)
+    gen.cache.set_length(b, 13)
+    for tokens in ((40, 50), (41, 51), (42, 52), (43, 53)):
+        got = gen.step([a, b], tokens)
+    one, _ = alone.prefill(prompt)
+    two, _ = alone.prefill(prompt[:13])
+    for tokens in ((40, 50), (41, 51), (42, 52), (43, 53)):
+        want = torch.cat([alone.step([r], [t]) for r, t in zip((one, two), tokens)])
+    assert torch.allclose(got.float(), want.float(), atol=0.03)

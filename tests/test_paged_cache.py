@@ -35,3 +35,73 @@ def test_a_row_that_is_named_twice_gets_its_pages_once():
         cache.reserve([row, row, row], [8, 5, 8])
         sound(cache)
         assert len(cache.row_pages(row)) == 2 and cache.free_pages == 6
+
+
+def test_a_shortened_fork_leaves_the_others_alone():
+    for back in (6, 4, 3, 1, 0):
+        cache = cache_of(pages=12)
+        a = cache.add()
+        kv = fill(cache, a, 8, 1)
+        b, c = cache.fork(a, 2)
+        cache.set_length(b, back)
+        sound(cache)
+        assert torch.equal(read(cache, b), kv[:, :, :back]) if back else True
+        cache.reserve([b], [11])
+        for i in range(back, 11):
+            append(cache, b, i, float(i))
+        cache.set_length(b, 11)
+        sound(cache)
+        assert torch.equal(read(cache, a), kv) and torch.equal(read(cache, c), kv)
+        assert torch.equal(read(cache, b)[:, :, :back], kv[:, :, :back])
+        assert all((read(cache, b)[:, :, i] == i).all() for i in range(back, 11))
+        assert len(set(cache.row_pages(b)) & set(cache.row_pages(a))) == back // 4
+
+
+def test_the_first_one_of_a_fork_may_go_back_too():
+    cache = cache_of(pages=12)
+    a = cache.add()
+    kv = fill(cache, a, 10, 2)
+    (b,) = cache.fork(a)
+    cache.reserve([a], [16])
+    cache.set_length(a, 2)      # a page that is shared in part, one that is shared behind, and two of its own
+    sound(cache)
+    cache.reserve([a], [16])
+    for i in range(2, 16):
+        append(cache, a, i, 1.0)
+    cache.set_length(a, 16)
+    sound(cache)
+    assert torch.equal(read(cache, b), kv) and torch.equal(read(cache, a)[:, :, :2], kv[:, :, :2]) and (read(cache, a)[:, :, 2:] == 1).all()
+
+
+def test_pages_of_its_own_stay_where_a_sequence_goes_back():
+    cache = cache_of(pages=4)
+    a = cache.add()
+    kv = fill(cache, a, 16, 3)
+    pages = cache.row_pages(a)
+    cache.set_length(a, 5)
+    assert cache.row_pages(a) == pages and cache.free_pages == 0 and torch.equal(read(cache, a), kv[:, :, :5])
+    sound(cache)
+
+
+def test_going_back_without_a_page_to_copy_to_changes_nothing():
+    cache = cache_of(pages=2)
+    a = cache.add()
+    kv = fill(cache, a, 8, 4)
+    (b,) = cache.fork(a)
+    with pytest.raises(RuntimeError, match="PagedKVCache"):
+        cache.set_length(b, 6)
+    sound(cache)
+    assert cache.length(b) == 8 and torch.equal(read(cache, a), kv) and torch.equal(read(cache, b), kv)
+    cache.set_length(b, 4)      # whole pages need no copy
+    sound(cache)
+    cache.free(a)
+    assert torch.equal(read(cache, b), kv[:, :, :4])
+
+
+def test_the_host_count_goes_forward_only():
+    cache = cache_of()
+    a = cache.add()
+    fill(cache, a, 8, 5)
+    with pytest.raises(RuntimeError, match="set_length"):
+        cache.advance([a], -2)
+    assert cache.length(a) == 8
