@@ -32,6 +32,7 @@ class PagedKVCache:
         self._free = list(range(pages - 1, -1, -1))      # the lowest page is taken first
         self._rows: Dict[int, List[int]] = {}            # row -> its pages in order, -1 where one was dropped
         self._length: Dict[int, int] = {}
+        self._window: Dict[int, int] = {}                # row -> the window that pages were dropped for
 
     # ------------------------------------------------------------------------------------------------------- what there is --
     @property
@@ -111,7 +112,8 @@ class PagedKVCache:
 
     def set_length(self, row: int, length: int) -> None:
         """The sequence's length, on the host and on the device.  A sequence that goes back among pages it shares keeps the whole ones before its new
-        end; of the one that holds the end it gets a copy, and those behind it are the others' from then on (``reserve`` gives new ones)."""
+        end; of the one that holds the end it gets a copy, and those behind it are the others' from then on (``reserve`` gives new ones).  It cannot
+        go back to where ``drop_unseen`` has given back some of its window's last positions."""
         self._known(row)
         if length < 0 or -(-length // self.page_size) > len(self._rows[row]):
             raise RuntimeError(f"PagedKVCache: row {row} has no pages for {length} positions")
@@ -141,6 +143,8 @@ class PagedKVCache:
                 copies.append(page)
                 pages = pages + [page]
             self._rows[r], self._length[r] = pages, length
+            if row in self._window:
+                self._window[r] = self._window[row]
         self._write([(r, i) for r in new for i in range(len(self._rows[r]))], [page for r in new for page in self._rows[r]])
         self.lengths[self._indices(new)] = length
         if copies:
@@ -153,6 +157,7 @@ class PagedKVCache:
         for page in self._rows[row]:
             self._drop(page)
         del self._rows[row], self._length[row]
+        self._window.pop(row, None)
         self.table[row] = -1
         self.lengths[row] = 0
 
@@ -167,6 +172,7 @@ class PagedKVCache:
                 if page >= 0:
                     dropped += self._drop(page)
                     self._rows[row][i] = -1
+                    self._window[row] = window
                     at.append((row, i))
         self._write(at, [-1] * len(at))
         return dropped
@@ -194,9 +200,11 @@ class PagedKVCache:
 
     # -------------------------------------------------------------------------------------------------------------- inside --
     def _go_back(self, row: int, length: int) -> None:
-        """No page that the sequence will write from position `length` on has another owner.  (``fork`` shares pages in front of both sequences'
-        ends only, so this is where such a page can come to lie behind one.)"""
+        """No page that the sequence will write from position `length` on has another owner or was dropped.  (``fork`` shares pages in front of both
+        sequences' ends only, and those that are dropped lie there too, so this is where such a page can come to lie behind one.)"""
         pages = self._rows[row]
+        if row in self._window and any(page < 0 for page in pages[max(0, length - self._window[row]) // self.page_size:-(-length // self.page_size)]):
+            raise RuntimeError(f"PagedKVCache: row {row} cannot go back to {length} positions, pages of its last {self._window[row]} were given back")
         full, end = length // self.page_size, -(-length // self.page_size)
         own = [page for page in pages[end:] if page >= 0 and self._owners[page] == 1]
         cut = pages[full] if end > full and pages[full] >= 0 and self._owners[pages[full]] > 1 else None

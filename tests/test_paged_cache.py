@@ -105,3 +105,51 @@ def test_the_host_count_goes_forward_only():
     with pytest.raises(RuntimeError, match="set_length"):
         cache.advance([a], -2)
     assert cache.length(a) == 8
+
+
+def windowed():
+    """27 positions in pages of 4, of which a window of 10 and one first position have left the pages 0 and 4 to 6."""
+    cache = cache_of(pages=12, rows=2)
+    a = cache.add()
+    kv = fill(cache, a, 27, 6)
+    assert cache.drop_unseen([a], 10, 1) == 3 and cache.row_pages(a)[1:4] == [-1] * 3
+    return cache, a, kv
+
+
+@pytest.mark.parametrize("length", [25, 24, 17, 16, 15, 9, 6, 5])
+def test_no_way_back_to_where_a_window_is_gone(length):
+    cache, a, _ = windowed()
+    before = cache.row_pages(a)
+    with pytest.raises(RuntimeError, match="given back"):
+        cache.set_length(a, length)
+    assert cache.length(a) == 27 and cache.row_pages(a) == before
+    sound(cache)
+
+
+@pytest.mark.parametrize("length", [26, 4, 2, 0])
+def test_back_to_where_everything_is_there(length):
+    cache, a, kv = windowed()
+    cache.set_length(a, length)
+    sound(cache)
+    end = min(length + 13, 32)
+    cache.reserve([a], [end])
+    for i in range(length, end):
+        append(cache, a, i, float(i))
+    cache.set_length(a, end)
+    sound(cache)
+    for i in list(range(min(length, 4))) + list(range(16 if length > 4 else length, end)):
+        page = int(cache.table[a, i // 4])
+        assert page >= 0
+        held = cache.pages[:, :, page, :, i % 4]
+        assert torch.equal(held, kv[:, :, i]) if i < length else (held == i).all()
+    (b,) = cache.fork(a)
+    sound(cache)
+
+
+def test_a_fork_knows_what_its_window_is():
+    cache, a, _ = windowed()
+    (b,) = cache.fork(a)
+    with pytest.raises(RuntimeError, match="given back"):
+        cache.set_length(b, 20)
+    cache.set_length(b, 3)
+    sound(cache)
