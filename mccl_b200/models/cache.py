@@ -125,6 +125,8 @@ class PagedKVCache:
     def fork(self, row: int, count: int = 1) -> List[int]:
         """`count` new sequences that begin as this one.  Full pages are shared; the last one, which will be written, is copied."""
         self._known(row)
+        if count < 0:
+            raise RuntimeError(f"PagedKVCache: {count} forks")
         length, old = self._length[row], self._rows[row]
         full = length // self.page_size
         partial = old[full] if length % self.page_size else None
@@ -163,6 +165,8 @@ class PagedKVCache:
 
     def drop_unseen(self, rows: Sequence[int], window: int, sinks: int = 0) -> int:
         """Gives back pages none of whose positions a window of the last `window` positions and the first `sinks` sees, now or later; returns how many."""
+        if window < 1 or sinks < 0:
+            raise RuntimeError(f"PagedKVCache: no window of {window} with {sinks} first positions")
         at, dropped = [], 0
         for row in rows:
             self._known(row)

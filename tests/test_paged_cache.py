@@ -153,3 +153,15 @@ def test_a_fork_knows_what_its_window_is():
         cache.set_length(b, 20)
     cache.set_length(b, 3)
     sound(cache)
+
+
+def test_counts_and_windows_that_make_no_sense():
+    cache = cache_of(rows=4)
+    a = cache.add()
+    kv = fill(cache, a, 16, 7)
+    for call in (lambda: cache.fork(a, -1), lambda: cache.drop_unseen([a], 0), lambda: cache.drop_unseen([a], -4), lambda: cache.drop_unseen([a], 2, -5)):
+        with pytest.raises(RuntimeError, match="PagedKVCache"):
+            call()
+        sound(cache)
+        assert cache.rows == [a] and torch.equal(read(cache, a), kv)
+    assert cache.fork(a, 0) == []
