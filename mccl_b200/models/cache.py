@@ -33,6 +33,7 @@ class PagedKVCache:
         self._rows: Dict[int, List[int]] = {}            # row -> its pages in order, -1 where one was dropped
         self._length: Dict[int, int] = {}
         self._window: Dict[int, int] = {}                # row -> the window that pages were dropped for
+        self._dropped: Dict[int, tuple] = {}             # row -> (i, j): nothing is left to drop among its pages i to j - 1
 
     # ------------------------------------------------------------------------------------------------------- what there is --
     @property
@@ -147,6 +148,8 @@ class PagedKVCache:
             self._rows[r], self._length[r] = pages, length
             if row in self._window:
                 self._window[r] = self._window[row]
+            if row in self._dropped:
+                self._dropped[r] = self._dropped[row]
         self._write([(r, i) for r in new for i in range(len(self._rows[r]))], [page for r in new for page in self._rows[r]])
         self.lengths[self._indices(new)] = length
         if copies:
@@ -160,6 +163,7 @@ class PagedKVCache:
             self._drop(page)
         del self._rows[row], self._length[row]
         self._window.pop(row, None)
+        self._dropped.pop(row, None)
         self.table[row] = -1
         self.lengths[row] = 0
 
@@ -171,7 +175,13 @@ class PagedKVCache:
         for row in rows:
             self._known(row)
             first = self._length[row] - window   # the next token's window begins one later
-            for i in range(-(-sinks // self.page_size), max(0, first) // self.page_size):
+            start, stop = -(-sinks // self.page_size), max(0, first) // self.page_size
+            done, until = self._dropped.get(row, (start, start))   # what the steps before have walked over
+            if done <= start <= until:
+                look, self._dropped[row] = range(until, stop), (done, max(until, stop))
+            else:
+                look, self._dropped[row] = range(start, stop), (start, max(start, stop))
+            for i in look:
                 page = self._rows[row][i]
                 if page >= 0:
                     dropped += self._drop(page)
@@ -210,6 +220,8 @@ class PagedKVCache:
         if row in self._window and any(page < 0 for page in pages[max(0, length - self._window[row]) // self.page_size:-(-length // self.page_size)]):
             raise RuntimeError(f"PagedKVCache: row {row} cannot go back to {length} positions, pages of its last {self._window[row]} were given back")
         full, end = length // self.page_size, -(-length // self.page_size)
+        if row in self._dropped:
+            self._dropped[row] = tuple(min(i, full) for i in self._dropped[row])
         own = [page for page in pages[end:] if page >= 0 and self._owners[page] == 1]
         cut = pages[full] if end > full and pages[full] >= 0 and self._owners[pages[full]] > 1 else None
         if cut is None and len(own) == len(pages) - end:

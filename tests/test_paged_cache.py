@@ -165,3 +165,62 @@ def test_counts_and_windows_that_make_no_sense():
         sound(cache)
         assert cache.rows == [a] and torch.equal(read(cache, a), kv)
     assert cache.fork(a, 0) == []
+
+
+class Counted(list):
+    looks = 0
+
+    def __getitem__(self, i):
+        Counted.looks += 1
+        return super().__getitem__(i)
+
+
+def test_pages_out_of_sight_are_looked_at_once():
+    cache = PagedKVCache(1, 1, 8, pages=600, max_sequences=2, max_positions=2400, page_size=4, device="cpu")
+    a = cache.add()
+    cache.reserve([a], [2000])
+    cache.set_length(a, 2000)
+    cache._rows[a] = Counted(cache._rows[a])
+    assert cache.drop_unseen([a], 100, 5) == 475 - 2      # positions below 1900, without the first two pages
+    Counted.looks = 0
+    for n in range(2001, 2101):
+        cache.reserve([a], [n])
+        cache.set_length(a, n)
+        cache.drop_unseen([a], 100, 5)
+    assert cache.row_pages(a).count(-1) == 500 - 2 and Counted.looks <= 3 * 100
+    sound(cache)
+
+
+def test_what_is_out_of_sight_is_given_back_whatever_was_asked_before():
+    """A walk that begins where the last one ended gives back what a walk over everything does."""
+    def unseen(pages, length, window, sinks):
+        return [p for i, p in enumerate(pages) if p >= 0 and -(-sinks // 4) <= i < max(0, length - window) // 4]
+
+    for seed in range(20):
+        g = torch.Generator().manual_seed(seed)
+        cache = PagedKVCache(1, 1, 8, pages=200, max_sequences=3, max_positions=200, page_size=4, device="cpu")
+        rows = [cache.add()]
+        for _ in range(60):
+            row = rows[int(torch.randint(0, len(rows), (1,), generator=g))]
+            kind = int(torch.randint(0, 8, (1,), generator=g))
+            length = cache.length(row)
+            if kind == 0 and len(rows) < 3:
+                rows += cache.fork(row)
+            elif kind == 1 and length:
+                to = int(torch.randint(0, length, (1,), generator=g))
+                try:
+                    cache.set_length(row, to)
+                except RuntimeError:
+                    pass
+            elif kind <= 4 and length < 190:
+                to = length + int(torch.randint(1, 10, (1,), generator=g))
+                cache.reserve([row], [to])
+                cache.set_length(row, to)
+            else:
+                window, sinks = int(torch.randint(1, 40, (1,), generator=g)), int(torch.randint(0, 30, (1,), generator=g)) * int(torch.randint(0, 2, (1,), generator=g))
+                want = unseen(cache.row_pages(row), cache.length(row), window, sinks)
+                free = cache.free_pages
+                got = cache.drop_unseen([row], window, sinks)
+                assert not unseen(cache.row_pages(row), cache.length(row), window, sinks)
+                assert got == cache.free_pages - free <= len(want)
+            sound(cache)
