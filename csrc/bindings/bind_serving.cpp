@@ -307,7 +307,7 @@ void bind_serving(py::module_& m) {
 
   m.def(
       "w4_pack",
-      [](const at::Tensor& codes, const at::Tensor& scales, const c10::optional<at::Tensor>& zeros) {
+      [](at::Tensor codes, const at::Tensor& scales, const c10::optional<at::Tensor>& zeros) {
         const char* op = "w4_pack";
         need_on(codes, codes, op);
         need_on(scales, codes, op);
@@ -321,6 +321,8 @@ void bind_serving(py::module_& m) {
           MCCL_CHECK_TENSOR(zeros->scalar_type() == at::kByte && zeros->is_contiguous() && zeros->sizes() == scales.sizes(), op << ": zeros must be contiguous uint8 of the scales' shape");
         }
         c10::cuda::CUDAGuard guard(codes.device());
+        // the kernel reads two codes at a time: k is even, and codes that begin on an odd byte (a part of a buffer) are moved first
+        if (reinterpret_cast<uintptr_t>(codes.data_ptr()) % 2 != 0) codes = codes.clone();
         const int64_t tiles = (n + 15) / 16;
         at::Tensor packed = empty_on(codes, {tiles, (k + 63) / 64, 32, 16}, at::kByte), params = empty_on(codes, {tiles, scales.size(1), 8, 2}, at::kInt);
         at::Tensor bad = at::zeros({1}, codes.options().dtype(at::kInt));

@@ -93,7 +93,7 @@ struct W4Args {
   bool gelu = false;
 };
 cudaError_t w4_linear(const W4Args& a, cudaStream_t stream);
-// Lays out codes [n, k] (one per byte), scales [n, k / group] bf16 and zeros (bytes, may be null: 8); *bad becomes nonzero when one is above 15.
+// Lays out codes [n, k] (one per byte, from an even address on), scales [n, k / group] bf16 and zeros (bytes, may be null: 8); *bad becomes nonzero when one is above 15.
 cudaError_t w4_pack(const uint8_t* codes, const void* scales, const uint8_t* zeros, void* packed, void* params, int* bad, int n, int k, int group, cudaStream_t stream);
 // w [n, k] bf16 = scale (code - zero), rounded once.
 cudaError_t w4_dequantize(const void* codes, const void* params, void* w, int n, int k, int group, cudaStream_t stream);

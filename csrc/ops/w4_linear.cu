@@ -890,7 +890,7 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(const uint4* __restr
   }
 }
 
-// A warp per tile of 16 x 64, a lane its 16 bytes; behind the tiles, a thread per row and group of the parameters.  (k is even: two neighbouring codes are one access.)
+// A warp per tile of 16 x 64, a lane its 16 bytes; behind the tiles, a thread per row and group of the parameters.  (k and the address of the codes are even: two neighbouring codes are one access.)
 __global__ void __launch_bounds__(256) w4_pack_kernel(const uint8_t* __restrict__ codes, const uint16_t* __restrict__ scales, const uint8_t* __restrict__ zeros, uint4* __restrict__ packed,
                                                       uint32_t* __restrict__ params, int* bad, int n, int k, int group) {
   ::mccl::pdl_wait();
