@@ -92,8 +92,11 @@ template <int kR, int kParams>
 constexpr int kNarrowSlot = kR * (1024 + kParams * 256);
 template <int kR, int kN>
 constexpr int kNarrowSums = 2 * kNarrowWarps * kR * kN * 128 * 4;
+constexpr int kNarrowX = 128 * 1024;   // most bytes of x: m rows of 256 per 128 columns
 template <int kR, int kN, int kParams>
-int narrow_smem(int m, int pairs) { return kNarrowWarps * kDeep<kR> * kNarrowSlot<kR, kParams> + kNarrowSums<kR, kN> + m * pairs * 256 + 16; }
+constexpr int narrow_smem(int x_bytes) { return kNarrowWarps * kDeep<kR> * kNarrowSlot<kR, kParams> + kNarrowSums<kR, kN> + x_bytes + 16; }
+constexpr int kSmemLimit = 227 * 1024;
+static_assert(narrow_smem<1, 1, 4>(kNarrowX) <= kSmemLimit && narrow_smem<1, 2, 4>(kNarrowX) <= kSmemLimit);   // one tile per warp always fits
 
 // A warp takes kR tiles of 16 weight rows at a time, a block 8 / along times as many, gridDim.x such groups apart; `along` warps share out K for each, a
 // run of stages of 128 columns, and add up at its end.  A lane's 16 bytes of 64 columns are its own A fragments of four m16n8k16 products: it copies them
@@ -950,10 +953,10 @@ int log2_of(int v) {
 template <int kR, int kN, int kParams, bool kEven>
 cudaError_t launch_narrow(const W4Args& a, cudaStream_t stream) {
   static std::atomic<uint64_t> allowed{0};
-  const cudaError_t rc = raise_smem_limit(w4_narrow_kernel<kR, kN, kParams, kEven>, 227 * 1024, allowed);
+  const cudaError_t rc = raise_smem_limit(w4_narrow_kernel<kR, kN, kParams, kEven>, kSmemLimit, allowed);
   if (rc != cudaSuccess) return rc;
-  const int chunks = (a.k + 63) / 64, smem = narrow_smem<kR, kN, kParams>(a.m, (chunks + 1) / 2);
-  if (smem > 227 * 1024) return cudaErrorNotSupported;
+  const int chunks = (a.k + 63) / 64, smem = narrow_smem<kR, kN, kParams>(a.m * ((chunks + 1) / 2) * 256);
+  if (smem > kSmemLimit) return cudaErrorNotSupported;
   const int tiles = ((a.n + 15) / 16 + kR - 1) / kR, blocks = sm_count() * (smem <= 113 * 1024 ? 2 : 1);
   // as few warps along K as give every warp a tile: adding up costs a barrier and a pass through shared memory
   int along = 3;
@@ -1107,10 +1110,11 @@ cudaError_t launch_wide(const W4Args& a, cudaStream_t on) {
 cudaError_t w4_linear(const W4Args& a, cudaStream_t stream) {
   if (a.m <= 0 || a.n <= 0) return cudaSuccess;
   const long long x_bytes = static_cast<long long>(a.m) * ((a.k + 127) / 128) * 256;
-  if (a.m <= 16 && x_bytes <= 128 * 1024) {
+  if (a.m <= 16 && x_bytes <= kNarrowX) {
     // two tiles of weights per warp share what is read of x (1 x 16384 x 2048 6.5 us, 7.9 with one; 4 x 32000 x 2048 12.7 and 14.3), if that leaves every SM some
-    // warps' work (1 x 2048 x 2048: 2.6 with one); 16 rows' sums leave no registers for it
-    const bool two = a.n >= 16 * 3 * sm_count();
+    // warps' work (1 x 2048 x 2048: 2.6 with one) and x its room (with groups of 32 the parameters leave 115 KB); 16 rows' sums leave no registers for it
+    const int bytes = static_cast<int>(x_bytes), smem = a.group == 32 ? narrow_smem<2, 1, 4>(bytes) : (a.group == 64 ? narrow_smem<2, 1, 2>(bytes) : narrow_smem<2, 1, 1>(bytes));
+    const bool two = a.n >= 16 * 3 * sm_count() && smem <= kSmemLimit;
     if (a.m <= 8) return two ? narrow<2, 1>(a, stream) : narrow<1, 1>(a, stream);
     return narrow<1, 2>(a, stream);
   }
