@@ -11,6 +11,7 @@
 #include <cuda.h>
 
 #include <array>
+#include <limits>
 
 #include "../core/launch.hpp"
 #include "bf16x8.cuh"
@@ -275,10 +276,11 @@ constexpr int kCodeRing = 4 * kTurns * 2 * kCodeDeep<false> * kCodeTile<false>;
 static_assert(kCodeRing == 4 * kTurns * 2 * kCodeDeep<true> * kCodeTile<true>);
 constexpr int kWideSmem = 226 * 1024;      // the rest is for the barriers
 constexpr int kMostTokens = 256;           // rows of x of a block
+constexpr int kMostRows = 0x7fffffff - kMostTokens;   // of x: a tile's last row is counted in 32 bits
 
 struct Wide {
   W4Args a;
-  int tokens, chunks, group_shift;   // rows of x per block, a multiple of 16; chunks of 64 columns in K
+  int tokens = 0, chunks, group_shift;   // rows of x per block, a multiple of 16; chunks of 64 columns in K
   int columns;          // of tensor memory that the sums take; the weights' ring lies behind them
   int allocated;
   int splits, share;    // blocks of a cluster that share out K, and rows of x whose sums each of them finishes
@@ -1008,10 +1010,10 @@ int resident(int splits) {
 // block some 5000 clocks before its first and after its last chunk.  (Measured beside all other choices for 27 sizes from 20 x 512 x 512 to
 // 1537 x 16384 x 2048: within 4 % of the best.)
 // With more tiles than SMs they run on from one to the next (returns true), so that no round has a beginning and an end of its own: 1537 x 16384 x 2048 took
-// 103 us in rounds.
+// 103 us in rounds.  More rows than a grid has blocks for, 256 x 65535, always run on: they are enough for several rounds.  (p.tokens stays 0 where nothing fits.)
 bool choose_wide(int m, int blocks, Wide& p) {
   constexpr double kMake = 400, kRound = 5000, kSplit = 2200, kToken = 20;
-  double best = 0;
+  double best = std::numeric_limits<double>::infinity();
   Wide w = p;
   for (int most = 16, before = 0; most <= kMostTokens && before != 1; most += 16) {
     const int tiles = (m + most - 1) / most;
@@ -1028,7 +1030,7 @@ bool choose_wide(int m, int blocks, Wide& p) {
       const long long waves = (all + at_once - 1) / at_once;
       const double products = 2.0 * w.tokens;
       const double cost = waves * ((p.chunks + w.splits - 1) / w.splits * (kMake > products ? kMake : products) + kRound + (w.splits > 1 ? kSplit : 0.0) + kToken * w.tokens);
-      if (best == 0 || cost < best) {
+      if (cost < best) {
         best = cost;
         p.tokens = w.tokens;
         p.splits = w.splits;
@@ -1085,7 +1087,9 @@ cudaError_t launch_wide(const W4Args& a, cudaStream_t on) {
   p.chunks = (a.k + 63) / 64;
   p.group_shift = log2_of(a.group);
   const int blocks = (a.n + kWideRows - 1) / kWideRows;
+  if (a.m > kMostRows) return cudaErrorInvalidValue;
   const bool stream = choose_wide(a.m, blocks, p);
+  if (p.tokens == 0) return cudaErrorInvalidValue;
   p.columns = p.tokens <= 32 ? 32 : (p.tokens <= 64 ? 64 : (p.tokens <= 128 ? 128 : 256));
   p.allocated = p.columns + kWideStages * 32 <= 256 ? 256 : 512;
   p.vector = a.n % 4 == 0 && (a.residual == nullptr || (a.ldr % 4 == 0 && reinterpret_cast<uintptr_t>(a.residual) % 8 == 0));

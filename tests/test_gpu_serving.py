@@ -44,3 +44,17 @@ def test_few_rows_of_many_columns(rows, n, k, group):
         w = w.view(-1, k)
         want[:, part], size[:, part] = x.double() @ w.t(), x.double().abs() @ w.abs().t()
     assert ((y - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -19 * size).all()
+
+
+def test_more_rows_than_a_grid_has_in_a_column():
+    # 256 rows of x per block and 65535 blocks along them are 16776960; x and y are 1.1 and 0.3 GB
+    rows, n, k = 65535 * 256 + 1345, 9, 32
+    g = torch.Generator(device="cuda").manual_seed(3)
+    weight = ops.W4Weight.from_codes(torch.randint(0, 16, (n, k), generator=g, device="cuda", dtype=torch.uint8), torch.rand(n, 1, generator=g, device="cuda"))
+    w = weight.dequantize().float()   # what many rows are multiplied with
+    x = torch.randn(rows, k, generator=g, device="cuda", dtype=torch.bfloat16)
+    y = ops.linear_w4(x, weight)
+    for at in range(0, rows, 1 << 21):
+        part = x[at:at + (1 << 21)].float()
+        want, size = part @ w.t(), part.abs() @ w.abs().t()
+        assert ((y[at:at + (1 << 21)].float() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -18 * size).all()   # 32 products each, in fp32 on both sides
