@@ -99,6 +99,13 @@ __device__ __forceinline__ void mma<Fp16>(float (&c)[4], const uint32_t (&a)[4],
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Weights, and with them their sums, are kept times 2^kLift: fp16 has steps of 2^-24 at its low end, and what many positions have that are far below the largest
+// would be lost in the products while the sum of weights counts it.  The largest stays below fp16's limit, and bf16 needs no factor.
+template <typename H>
+constexpr float kLift = 0.f;
+template <>
+constexpr float kLift<Fp16> = 15.f;
+
 template <typename H>
 __device__ __forceinline__ uint32_t pair(float a, float b) {
   const typename H::T2 v = H::down(a, b);
@@ -167,6 +174,8 @@ struct Sums {
   }
 };
 template <typename H>
+__device__ __forceinline__ float log_of_sum(float m, float l) { return ((m == -INFINITY ? 0.f : m) + (log2f(l) - kLift<H>)) * kLn2; }
+template <typename H>
 __device__ __forceinline__ void store_result(const PagedAttentionArgs& a, long long row, int col, const Sums& s) {
   if (col < a.head_dim) {
     const float inv = 1.f / s.l;
@@ -174,7 +183,7 @@ __device__ __forceinline__ void store_result(const PagedAttentionArgs& a, long l
     to[0] = H::down(s.o.x * inv, s.o.y * inv);
     to[1] = H::down(s.o.z * inv, s.o.w * inv);
   }
-  if (col == 0 && a.lse) a.lse[row] = ((s.m == -INFINITY ? 0.f : s.m) + log2f(s.l)) * kLn2;
+  if (col == 0 && a.lse) a.lse[row] = log_of_sum<H>(s.m, s.l);
 }
 
 template <typename H, int DP, int KT, int WARPS, int STAGES, int ROWS, int BOX>
@@ -487,9 +496,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         keep[h] = exp2f(m[h] - base);
         m[h] = now;
         float sum = 0.f;
+        const float lifted = base - kLift<H>;
 #pragma unroll
         for (int i = 0; i < 4 * kSub; ++i) {
-          z[h][i] = exp2f(z[h][i] - base);
+          z[h][i] = exp2f(z[h][i] - lifted);
           sum += z[h][i];
         }
         l[h] = l[h] * keep[h] + sum;
@@ -575,7 +585,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
           const int col = c * 8 + 2 * t4;
           if (col < a.head_dim) *reinterpret_cast<typename H::T2*>(to + col) = H::down(o[c][2 * h] * inv, o[c][2 * h + 1] * inv);
         }
-        if (a.lse && t4 == 0) a.lse[out] = ((m[h] == -INFINITY ? 0.f : m[h]) + log2f(l[h])) * kLn2;
+        if (a.lse && t4 == 0) a.lse[out] = log_of_sum<H>(m[h], l[h]);
       } else {
         float* to = reinterpret_cast<float*>(sums) + row * DP;
 #pragma unroll
