@@ -104,6 +104,7 @@ def apply_rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.T
 
 # What applies to every module of the process (torch.nn.modules.module.register_module_forward_hook and friends).
 _GLOBAL_HOOKS = tuple(getattr(nn.modules.module, f"_global_{kind}_hooks") for kind in ("forward", "forward_pre", "backward", "backward_pre"))
+_GLOBAL_FORWARD_HOOKS = _GLOBAL_HOOKS[:2]
 
 
 def _stock(m: nn.Module) -> bool:

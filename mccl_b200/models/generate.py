@@ -16,11 +16,12 @@ import torch.nn.functional as F
 
 from .. import ops
 from .cache import PagedKVCache
-from .decoder import Block, Decoder, Linear, Norm, _rope_tables
+from .decoder import _GLOBAL_FORWARD_HOOKS, Block, Decoder, Linear, Norm, _rope_tables, _stock
 
 
 class Generator:
-    """A snapshot of a decoder's weights with a cache for `max_sequences` sequences.
+    """A snapshot of a decoder's weights with a cache for `max_sequences` sequences.  A decoder whose modules compute something else than this package's
+    (derived ones with a forward of their own, forward hooks) is refused.
 
     weights: "bf16", or "w4" for the layers' matrices in 4 bits (`group` columns per scale; the vocabulary projection stays bf16).
     pages: of `page_size` positions; by default enough for every sequence to be `max_positions` long (by default the model's).
@@ -33,11 +34,18 @@ class Generator:
             raise RuntimeError(f"Generator: weights are 'bf16' or 'w4', not '{weights}'")
         if window is not None and window < 1 or sinks < 0 or (sinks and window is None):
             raise RuntimeError(f"Generator: no window of {window} with {sinks} first positions")
-        if not isinstance(model, Decoder) or type(model).forward is not Decoder.forward or type(model).hidden is not Decoder.hidden:
+        if (not isinstance(model, Decoder) or type(model).__call__ is not torch.nn.Module.__call__
+                or any(getattr(type(model), name) is not getattr(Decoder, name) or name in model.__dict__ for name in ("forward", "hidden", "head_weight"))):
             raise RuntimeError("Generator: a Decoder whose forward is its own")
         for blk in model.blocks:
-            if type(blk).forward is not Block.forward or any(not isinstance(m, (Linear, Norm)) for m in blk.children()):
+            if not isinstance(blk, Block) or blk.cfg != model.cfg or any(not isinstance(m, (Linear, Norm)) for m in blk.children()):
                 raise RuntimeError("Generator: the decoder's layers were replaced or wrapped")
+        called = [model.tok, model.ln_f, *(m for blk in model.blocks for m in (blk, *blk.children()))]
+        if not isinstance(model.tok, torch.nn.Embedding) or not isinstance(model.ln_f, Norm) or not all(
+                _stock(m) and "forward" not in m.__dict__ and "with_residual" not in m.__dict__ for m in called):
+            raise RuntimeError("Generator: modules of the decoder have a forward of their own")
+        if any(_GLOBAL_FORWARD_HOOKS) or any(m._forward_hooks or m._forward_pre_hooks for m in (model, *called)):
+            raise RuntimeError("Generator: forward hooks, which a step would not call")
         cfg = self.cfg = model.cfg
         self.max_positions = max_positions or cfg.max_seq
         if cfg.pos == "learned" and self.max_positions > cfg.max_seq:
@@ -55,7 +63,7 @@ class Generator:
                 return (ops.quantize_w4(w, group) if quantize else w.to(torch.bfloat16).clone()), None if m.bias is None else m.bias.detach().clone()
 
             def norm(m: Norm):
-                return m.weight.detach().clone(), None if m.bias is None else m.bias.detach().clone()
+                return m.weight.detach().clone(), None if m.bias is None else m.bias.detach().clone(), m.eps
 
             w4 = weights == "w4"
             self._layers = [{"ln1": norm(b.ln1), "qkv": matrix(b.qkv, w4), "proj": matrix(b.proj, w4), "ln2": norm(b.ln2),
@@ -74,7 +82,7 @@ class Generator:
         return f(x, w, b, act=act, residual=residual)
 
     def _mlp(self, x, layer):
-        h = ops.norm(x, *layer["ln2"], self.cfg.eps)
+        h = ops.norm(x, *layer["ln2"])
         if self.cfg.act == "swiglu":
             h = ops.swiglu(self._linear(h, layer["up"]))
         else:
@@ -88,7 +96,7 @@ class Generator:
         return qkv[:, 0] if q is None else q
 
     def _logits(self, x):
-        return ops.linear(ops.norm(x, *self._ln_f, self.cfg.eps), self._head)
+        return ops.linear(ops.norm(x, *self._ln_f), self._head)
 
     # --------------------------------------------------------------------------------------------------------- prompts ----
     @torch.no_grad()
@@ -118,7 +126,7 @@ class Generator:
         rows = torch.full_like(positions, row)
         x = ops.embedding(ids[None], self._tok, self._pos)
         for i, layer in enumerate(self._layers):
-            qkv = self._linear(ops.norm(x, *layer["ln1"], cfg.eps), layer["qkv"])
+            qkv = self._linear(ops.norm(x, *layer["ln1"]), layer["qkv"])
             self._append(i, qkv.view(count, 3, cfg.n_heads, cfg.head_dim), self.cache.table, positions, rows, False)
             a = ops.causal_attention(qkv, cfg.n_heads) if self._rope is None else ops.rope_attention(qkv, cfg.n_heads, *self._rope)
             x = self._mlp(self._linear(a, layer["proj"], residual=x), layer)
@@ -180,7 +188,7 @@ class Generator:
             x = x + F.embedding(positions.long(), self._pos)
         x = x.to(torch.bfloat16)
         for i, layer in enumerate(self._layers):
-            qkv = self._linear(ops.norm(x, *layer["ln1"], cfg.eps), layer["qkv"]).view(count, 3, cfg.n_heads, cfg.head_dim)
+            qkv = self._linear(ops.norm(x, *layer["ln1"]), layer["qkv"]).view(count, 3, cfg.n_heads, cfg.head_dim)
             q = self._append(i, qkv, table, positions, None, True)
             a = ops.paged_attention(q, cache.keys(i), cache.values(i), table, lengths, window=self.window, sinks=self.sinks).view(count, cfg.d_model)
             x = self._mlp(self._linear(a, layer["proj"], residual=x), layer)

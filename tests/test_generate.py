@@ -2,6 +2,8 @@
 
 Logits of the generator and of the model's own forward over the whole text are both computed with bf16 activations; neither is nearer to the model in 32
 bits by construction, so the generator may be off by at most twice as much (root mean square) as that forward."""
+import dataclasses
+
 import pytest
 import torch
 
@@ -238,3 +240,92 @@ def test_a_fork_that_goes_back():
     for tokens in ((40, 50), (41, 51), (42, 52), (43, 53)):
         want = torch.cat([alone.step([r], [t]) for r, t in zip((one, two), tokens)])
     assert torch.allclose(got.float(), want.float(), atol=0.03)
+
+
+class Adapted(type(build_decoder("tiny").blocks[0].up)):
+    def forward(self, x, native, act="none", residual=None):
+        return super().forward(x, native, act, residual) * 1.5
+
+
+class Scaled(torch.nn.Embedding):
+    def forward(self, ids):
+        return super().forward(ids) * 2.0
+
+
+def _adapter(model):
+    model.blocks[1].up.__class__ = Adapted
+
+
+def _embedding(model):
+    model.tok.__class__ = Scaled
+
+
+def _own_forward(model):
+    first = model.blocks[0].proj
+    stock = first.forward
+    first.forward = lambda *a, **k: stock(*a, **k) * 1.5
+
+
+def _own_head(model):
+    model.head_weight = lambda: model.tok.weight * 2.0
+
+
+def _other_heads(model):
+    model.blocks[0].cfg = dataclasses.replace(model.cfg, n_heads=2)
+
+
+CHANGES = {"adapter": _adapter, "embedding": _embedding, "forward": _own_forward, "head": _own_head, "heads": _other_heads,
+           "hook-block": lambda m: m.blocks[0].register_forward_hook(lambda mod, args, out: out * 1.5),
+           "hook-projection": lambda m: m.blocks[1].qkv.register_forward_pre_hook(lambda mod, args: (args[0] * 1.5, *args[1:])),
+           "hook-norm": lambda m: m.ln_f.register_forward_hook(lambda mod, args, out: out * 1.5),
+           "hook-embedding": lambda m: m.tok.register_forward_hook(lambda mod, args, out: out * 1.5),
+           "hook-model": lambda m: m.register_forward_hook(lambda mod, args, out: out * 1.5)}
+
+
+@pytest.mark.parametrize("change", list(CHANGES))
+def test_a_changed_model_is_refused(change):
+    model = build_decoder("tiny")
+    CHANGES[change](model)
+    with pytest.raises(RuntimeError, match="Generator"):
+        Generator(model)
+
+
+def test_hooks_of_all_modules_are_refused():
+    model = build_decoder("tiny")
+    handle = torch.nn.modules.module.register_module_forward_hook(lambda mod, args, out: None)
+    try:
+        with pytest.raises(RuntimeError, match="Generator"):
+            Generator(model)
+    finally:
+        handle.remove()
+    Generator(model)
+
+
+def _norms(model):
+    for i, m in enumerate(m for m in model.modules() if hasattr(m, "eps") and hasattr(m, "kind")):
+        m.eps = (0.02, 0.1, 0.5)[i % 3]
+
+
+def _parametrized(model):
+    class Half(torch.nn.Module):
+        def forward(self, w):
+            return w * 0.5
+    torch.nn.utils.parametrize.register_parametrization(model.blocks[0].up, "weight", Half())
+
+
+@pytest.mark.parametrize("change", [_norms, _parametrized])
+@pytest.mark.parametrize("family", list(FAMILIES))
+def test_a_changed_model_that_can_be_answered_for(family, change):
+    """What a norm adds under its root, and a weight that is computed, are the module's own."""
+    if family == "swiglu" and change is _parametrized:
+        pytest.skip("one family shows it")
+    torch.manual_seed(5)
+    model = sharpen(build_decoder("tiny", **FAMILIES[family]))
+    before = Generator(model).prefill(range(10))[1].float()
+    change(model)
+    gen = Generator(model)
+    row, first = gen.prefill(range(10))
+    got = torch.stack([first, gen.step([row], [10])[0]]).float()
+    with torch.no_grad():
+        want = model(torch.arange(11)[None])[0, 9:].float()
+    assert rms(got[0] - before) > 10 * rms(got - want) and torch.allclose(got, want, atol=0.05)
