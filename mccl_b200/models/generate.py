@@ -9,6 +9,7 @@ sequences.  On a CPU the same math runs on the operators' plain forms.
 """
 from __future__ import annotations
 
+import contextlib
 from typing import Dict, List, Optional, Sequence
 
 import torch
@@ -98,10 +99,18 @@ class Generator:
     def _logits(self, x):
         return ops.linear(ops.norm(x, *self._ln_f), self._head)
 
+    def _here(self):
+        """The model's device as the current one: kernels, captures and replays go to its streams, whichever device the caller is on."""
+        return torch.cuda.device(self.device) if self.device.type == "cuda" else contextlib.nullcontext()
+
     # --------------------------------------------------------------------------------------------------------- prompts ----
     @torch.no_grad()
     def prefill(self, tokens: Sequence[int]):
         """A new sequence that begins with these tokens: (its row, the logits ``[vocab]`` behind the last one)."""
+        with self._here():
+            return self._prefill(tokens)
+
+    def _prefill(self, tokens):
         ids = torch.as_tensor(tokens, dtype=torch.int64).reshape(-1).to(self.device)
         count = ids.numel()
         if count < 1 or count > self.max_positions:
@@ -136,7 +145,10 @@ class Generator:
     @torch.no_grad()
     def step(self, rows: Sequence[int], tokens) -> torch.Tensor:
         """One more token for each of these sequences (different ones); returns the logits ``[len(rows), vocab]`` behind it."""
-        rows = list(rows)
+        with self._here():
+            return self._step(list(rows), tokens)
+
+    def _step(self, rows, tokens):
         if len(set(rows)) != len(rows):
             raise RuntimeError("Generator: a sequence twice in one step")
         ids = torch.as_tensor(tokens, dtype=torch.int64).to(self.device)
@@ -173,7 +185,7 @@ class Generator:
             self.cache.lengths.copy_(before)     # the replay writes the same places again
         torch.cuda.current_stream(self.device).wait_stream(side)
         graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph):
+        with torch.cuda.graph(graph, stream=side):   # its own default is a stream of the device that captured first
             out = self._one(static_rows, static_ids)
         return graph, static_rows, static_ids, out
 

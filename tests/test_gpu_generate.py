@@ -104,3 +104,40 @@ def test_generate():
     texts = gen.generate([[5], list(range(20)), [9, 8, 7]], 6)
     assert [len(t) for t in texts] == [6, 6, 6] and gen.cache.rows == []
     assert texts == gen.generate([[5], list(range(20)), [9, 8, 7]], 6)
+
+
+def test_a_step_is_captured_on_a_stream_of_the_models_device(monkeypatch):
+    """Without a stream of its own a capture takes one of the device that was current at the process's first capture."""
+    model = build_decoder("tiny").cuda()
+    gen = Generator(model, max_sequences=2)
+    row, _ = gen.prefill([1, 2, 3])
+    seen, stock = [], torch.cuda.graph
+
+    class Graph(stock):
+        def __init__(self, graph, pool=None, stream=None, **kw):
+            seen.append((stream, torch.cuda.current_device()))
+            super().__init__(graph, pool=pool, stream=stream, **kw)
+
+    monkeypatch.setattr(torch.cuda, "graph", Graph)
+    gen.step([row], [4])
+    (stream, current), = seen
+    assert stream is not None and stream.device == gen.device and current == gen.device.index
+
+
+def test_prompts_and_steps_run_with_the_models_device_current(monkeypatch):
+    model = build_decoder("tiny").cuda()
+    gen = Generator(model, max_sequences=2)
+    entered, stock = [], torch.cuda.device
+
+    class Device(stock):
+        def __enter__(self):
+            entered.append(self.idx)
+            return super().__enter__()
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    row, _ = gen.prefill([1, 2, 3])
+    assert entered[:1] == [gen.device.index]
+    for _ in range(2):      # captured, replayed
+        entered.clear()
+        gen.step([row], [4])
+        assert entered[:1] == [gen.device.index]
