@@ -10,6 +10,7 @@ sequences.  On a CPU the same math runs on the operators' plain forms.
 from __future__ import annotations
 
 import contextlib
+import gc
 from typing import Dict, List, Optional, Sequence
 
 import torch
@@ -185,8 +186,14 @@ class Generator:
             self.cache.lengths.copy_(before)     # the replay writes the same places again
         torch.cuda.current_stream(self.device).wait_stream(side)
         graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph, stream=side):   # its own default is a stream of the device that captured first
-            out = self._one(static_rows, static_ids)
+        collecting = gc.isenabled()
+        gc.disable()   # a graph that the collector destroys meanwhile, another generator's, would invalidate the capture
+        try:
+            with torch.cuda.graph(graph, stream=side):   # its own default is a stream of the device that captured first
+                out = self._one(static_rows, static_ids)
+        finally:
+            if collecting:
+                gc.enable()
         return graph, static_rows, static_ids, out
 
     def _one(self, rows, ids):

@@ -1,4 +1,6 @@
 """Answering token by token on the native operators, see test_generate.py for the bound."""
+import gc
+
 import pytest
 import torch
 
@@ -141,3 +143,37 @@ def test_prompts_and_steps_run_with_the_models_device_current(monkeypatch):
         entered.clear()
         gen.step([row], [4])
         assert entered[:1] == [gen.device.index]
+
+
+def test_garbage_with_graphs_does_not_break_a_capture():
+    """A generator in a reference cycle, with its graph, that nobody has collected when another one captures."""
+    model = build_decoder("tiny").cuda()
+    gen = Generator(model, max_sequences=2)
+    row, _ = gen.prefill([1, 2, 3])
+    stock, calls, kept = gen._one, [], []
+
+    def one(rows, ids):
+        calls.append(gc.isenabled())
+        if torch.cuda.is_current_stream_capturing():
+            kept.pop()
+            for _ in range(3):
+                [[] for _ in range(3 * gc.get_threshold()[0])]      # allocations enough for the collector to run by itself
+        return stock(rows, ids)
+
+    gen._one = one
+    other = Generator(model, max_sequences=2)
+    other.step([other.prefill([1, 2])[0]], [3])
+    other.me = other
+    kept.append(other)
+    threshold = gc.get_threshold()
+    gc.collect()
+    del other
+    try:
+        gc.set_threshold(50, 1, 1)
+        logits = gen.step([row], [4])
+    finally:
+        gc.set_threshold(*threshold)
+        gen._one = stock
+    assert calls == [True, False] and gc.isenabled()
+    again = Generator(model, max_sequences=2)
+    assert torch.equal(logits, again.step([again.prefill([1, 2, 3])[0]], [4]))
