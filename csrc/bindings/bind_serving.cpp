@@ -2,6 +2,7 @@
 // workspaces through torch and launches on the current CUDA stream of the operands' device, so the calls can be captured in a CUDA graph.
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -32,6 +33,7 @@ void need_on(const at::Tensor& t, const at::Tensor& like, const char* what) {
 }
 void need_forward_only(const at::Tensor& t, const char* what) {
   MCCL_CHECK_TENSOR(!(at::GradMode::is_enabled() && t.requires_grad()), what << ": has no backward pass; call it under torch.no_grad()");
+  MCCL_CHECK_TENSOR(!(c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined()), what << ": has no forward-mode derivative; a tangent would be lost");
 }
 ops::Half16 half16(const at::Tensor& t, const char* what) {
   MCCL_CHECK_TENSOR(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf,
@@ -142,6 +144,7 @@ void bind_serving(py::module_& m) {
         if (cos_t.has_value()) {
           for (const auto* t : {&*cos_t, &*sin_t}) {
             need_on(*t, k, "paged_append(rope)");
+            need_forward_only(*t, op);
             MCCL_CHECK_TENSOR(t->scalar_type() == at::kFloat && t->dim() == 2 && t->is_contiguous() && t->size(1) * 2 == c.head_dim &&
                                   reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
                               "paged_append(rope): cos and sin must be contiguous fp32 [positions, head_dim / 2]");

@@ -58,3 +58,39 @@ def test_more_rows_than_a_grid_has_in_a_column():
         part = x[at:at + (1 << 21)].float()
         want, size = part @ w.t(), part.abs() @ w.abs().t()
         assert ((y[at:at + (1 << 21)].float() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -18 * size).all()   # 32 products each, in fp32 on both sides
+
+
+def _calls():
+    """Every operator as a call of its floating operands, and those."""
+    def r(*shape, dtype=torch.bfloat16):
+        return torch.randn(*shape, device="cuda", dtype=dtype)
+    table, one = torch.arange(4, dtype=torch.int32, device="cuda").view(2, 2), torch.ones(2, dtype=torch.int32, device="cuda")
+    weight = ops.quantize_w4(r(16, 64), 64)
+    return {
+        "attention": (lambda q, k, v: ops.paged_attention(q, k, v, table, one), [r(2, 4, 16), r(4, 2, 8, 16), r(4, 2, 8, 16)]),
+        "append": (lambda k, v, kp, vp, q, cos, sin: ops.paged_append(k, v, kp, vp, table, one, q=q, rope=(cos, sin)),
+                   [r(2, 2, 16), r(2, 2, 16), r(4, 2, 8, 16), r(4, 2, 8, 16), r(2, 4, 16), r(9, 8, dtype=torch.float32), r(9, 8, dtype=torch.float32)]),
+        "copy": (lambda p: ops.copy_pages(p, one[:1], one[:1] * 2), [r(4, 2, 8, 16)]),
+        "w4": (lambda x, b, y: ops.linear_w4(x, weight, b, residual=y), [r(3, 64), r(16, dtype=torch.float32), r(3, 16)]),
+    }
+
+
+@pytest.mark.parametrize("op", ["attention", "append", "copy", "w4"])
+def test_operands_whose_derivative_would_be_lost(op):
+    import torch.autograd.forward_ad as forward
+    call, operands = _calls()[op]
+    call(*operands)
+    for i, t in enumerate(operands):
+        rest = operands[:i], operands[i + 1:]
+        leaf = t.clone().requires_grad_()
+        with pytest.raises(RuntimeError, match="no_grad"):
+            call(*rest[0], leaf, *rest[1])
+        with torch.no_grad():
+            call(*rest[0], leaf, *rest[1])
+        with forward.dual_level():
+            dual = forward.make_dual(t.clone(), torch.ones_like(t))
+            with pytest.raises(RuntimeError, match="tangent"):
+                call(*rest[0], dual, *rest[1])
+            call(*rest[0], forward.unpack_dual(dual).primal, *rest[1])
+            with torch.inference_mode():
+                call(*operands)
