@@ -100,6 +100,14 @@ class Generator:
     def _logits(self, x):
         return ops.linear(ops.norm(x, *self._ln_f), self._head)
 
+    def _ids(self, tokens):
+        """Tokens on the model's device.  Those on the host are looked at first; one on the device that is outside the vocabulary counts as token 0."""
+        ids = torch.as_tensor(tokens, dtype=torch.int64)
+        vocab = self._tok.shape[0]
+        if not ids.is_cuda and ids.numel() and not (0 <= int(ids.min()) and int(ids.max()) < vocab):
+            raise RuntimeError(f"Generator: tokens outside the vocabulary of {vocab}")
+        return ids.to(self.device)
+
     def _here(self):
         """The model's device as the current one: kernels, captures and replays go to its streams, whichever device the caller is on."""
         return torch.cuda.device(self.device) if self.device.type == "cuda" else contextlib.nullcontext()
@@ -112,7 +120,7 @@ class Generator:
             return self._prefill(tokens)
 
     def _prefill(self, tokens):
-        ids = torch.as_tensor(tokens, dtype=torch.int64).reshape(-1).to(self.device)
+        ids = self._ids(tokens).reshape(-1)
         count = ids.numel()
         if count < 1 or count > self.max_positions:
             raise RuntimeError(f"Generator: a prompt of {count} tokens, 1 to {self.max_positions} are possible")
@@ -152,7 +160,7 @@ class Generator:
     def _step(self, rows, tokens):
         if len(set(rows)) != len(rows):
             raise RuntimeError("Generator: a sequence twice in one step")
-        ids = torch.as_tensor(tokens, dtype=torch.int64).to(self.device)
+        ids = self._ids(tokens)
         if ids.shape != (len(rows),):
             raise RuntimeError(f"Generator: {tuple(ids.shape)} tokens for {len(rows)} sequences")
         if not rows:
@@ -202,10 +210,7 @@ class Generator:
         positions = cache.lengths.index_select(0, rows)
         lengths = positions + 1
         table = cache.table.index_select(0, rows)
-        x = F.embedding(ids, self._tok)
-        if self._pos is not None:
-            x = x + F.embedding(positions.long(), self._pos)
-        x = x.to(torch.bfloat16)
+        x = ops.embedding(ids, self._tok, None if self._pos is None else F.embedding(positions.long(), self._pos))
         for i, layer in enumerate(self._layers):
             qkv = self._linear(ops.norm(x, *layer["ln1"]), layer["qkv"]).view(count, 3, cfg.n_heads, cfg.head_dim)
             q = self._append(i, qkv, table, positions, None, True)

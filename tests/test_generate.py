@@ -329,3 +329,15 @@ def test_a_changed_model_that_can_be_answered_for(family, change):
     with torch.no_grad():
         want = model(torch.arange(11)[None])[0, 9:].float()
     assert rms(got[0] - before) > 10 * rms(got - want) and torch.allclose(got, want, atol=0.05)
+
+
+def test_tokens_outside_the_vocabulary():
+    gen = Generator(build_decoder("tiny"), max_sequences=2)
+    row, _ = gen.prefill([1, 2])
+    free = gen.cache.free_pages
+    for bad in (512, -1, 2 ** 40):
+        for call in (lambda: gen.prefill([1, bad]), lambda: gen.step([row], [bad]), lambda: gen.step([row], torch.tensor([bad])), lambda: gen.generate([[1], [bad]], 2)):
+            with pytest.raises(RuntimeError, match="vocabulary"):
+                call()
+            assert gen.cache.rows == [row] and gen.cache.length(row) == 2 and gen.cache.free_pages == free
+    gen.step([row], [511])

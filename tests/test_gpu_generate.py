@@ -177,3 +177,21 @@ def test_garbage_with_graphs_does_not_break_a_capture():
     assert calls == [True, False] and gc.isenabled()
     again = Generator(model, max_sequences=2)
     assert torch.equal(logits, again.step([again.prefill([1, 2, 3])[0]], [4]))
+
+
+@pytest.mark.parametrize("preset,changes", [("tiny", {}), ("1.3b", dict(n_layers=1, vocab=500, d_model=128, n_heads=2, d_ff=256, max_seq=64))])
+def test_tokens_outside_the_vocabulary(preset, changes):
+    """On the host they are refused; on the device, where looking would mean waiting, they count as token 0, as they do where whole texts are scored."""
+    torch.manual_seed(6)
+    model = build_decoder(preset, **changes).cuda()
+    gen = Generator(model, max_sequences=4, page_size=16)
+    with pytest.raises(RuntimeError, match="vocabulary"):
+        gen.prefill([1, model.cfg.vocab])
+    rows = [gen.prefill([1, 2])[0] for _ in range(3)]
+    with pytest.raises(RuntimeError, match="vocabulary"):
+        gen.step(rows, [0, -1, 3])
+    got = gen.step(rows, torch.tensor([0, -1, 2 ** 40], device="cuda"))
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+    first = gen.prefill(torch.tensor([1, model.cfg.vocab], device="cuda"))
+    again = Generator(model, max_sequences=1, page_size=16)
+    assert torch.equal(first[1], again.prefill([1, 0])[1])
