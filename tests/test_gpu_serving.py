@@ -94,3 +94,37 @@ def test_operands_whose_derivative_would_be_lost(op):
             call(*rest[0], forward.unpack_dual(dual).primal, *rest[1])
             with torch.inference_mode():
                 call(*operands)
+
+
+@pytest.mark.parametrize("dim", [0, 1, 2])
+def test_copies_are_made_in_place(dim):
+    pages = torch.randn(4, 6, 8, device="cuda")
+    want = pages.clone()
+    if dim < 2:
+        want.select(dim, 2).copy_(pages.select(dim, 1))
+    else:
+        want[..., 2] = pages[..., 1]
+    one = torch.ones(1, dtype=torch.int32, device="cuda")
+    assert ops.copy_pages(pages, one, one * 2, dim=dim) is pages
+    assert torch.equal(pages, want)
+
+
+# A result of many rows: rounding of the result, sums of k products in fp32, weights rounded to bf16 once (six standard deviations of 2^-8 of each, evenly
+# spread), all at the GELU's largest slope; and the GELU itself in fp32, whose erf is off by up to two units in the last place: 2^-23 |z|, twice that here.
+@pytest.mark.parametrize("rows,n,k,group", [(1, 512, 512, 128), (7, 7200, 256, 64), (16, 300, 96, 32), (20, 512, 512, 128), (48, 3072, 768, 128), (130, 1000, 1088, 64), (300, 2048, 64, 32),
+                                            (600, 8192, 256, 128), (1025, 4099, 320, 64)])
+@pytest.mark.parametrize("residual", [False, True])
+def test_gelu_has_no_error_of_its_own(rows, n, k, group, residual):
+    g = torch.Generator(device="cuda").manual_seed(n + rows)
+    weight = ops.W4Weight.from_codes(torch.randint(0, 16, (n, k), generator=g, device="cuda", dtype=torch.uint8), torch.rand(n, k // group, generator=g, device="cuda") * 0.04)
+    w = weight._plain().double()
+    x = torch.randn(rows, k, generator=g, device="cuda").to(torch.bfloat16)
+    bias = torch.randn(n, generator=g, device="cuda")
+    add = torch.randn(rows, n, generator=g, device="cuda").to(torch.bfloat16) if residual else None
+    y = ops.linear_w4(x, weight, bias, act="gelu", residual=add).double()
+    z = x.double() @ w.t() + bias.double()
+    want = 0.5 * z * torch.special.erfc(-z * 0.5 ** 0.5) + (add.double() if residual else 0.0)
+    before = 2.0 ** -19 * (x.double().abs() @ w.abs().t() + bias.double().abs())
+    if rows > 16:
+        before = before + 6 * 2.0 ** -8 * ((x.double() ** 2) @ (w.t() ** 2) / 3).sqrt()
+    assert ((y - want).abs() <= 2.0 ** -8 * want.abs() + 1.13 * before + 2.0 ** -22 * z.abs()).all()
