@@ -3,14 +3,15 @@
 // The formula, for one sequence and head with query q: o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m), s_j = scale q . k_j over the visible
 // positions j and m their maximum.  Sums over any split of the positions join exactly: parts (m, l, o) combine with weights exp(m_part - m).
 //
-// Every key and value is read once and used for the query heads that share it, at most 8 multiply-adds per byte: memory bounds it.  So all tiles of all
+// Every key and value is read once and used for up to 16 query heads that share it (more of them: once per 16), at most 8 multiply-adds per byte: memory bounds
+// it.  So all tiles of all
 // sequences and heads are counted through and every warp of one block per SM streams an equal run of them, whatever the lengths are, through a ring of its
 // own that no other warp waits for.  The pieces that a run leaves of an item at its two ends are joined in shared memory, what crosses a block's bounds by a
 // second small kernel; everything is added in the order of the positions, so results repeat bit for bit.  Scores and weighted sums are m16n8k16 products:
 // eight heads that share keys fill half of their rows, single ones an eighth, and still they run at a quarter of their rate, while the generation's own
 // instruction would want 64 rows.
 // Measured: 2 x 131009 positions, 32 heads over 8 of 128 (1071 MB): 165 us, 6.5 TB/s; 64 ragged sequences of up to 2048, 16 heads of 128 (540 MB): 87 us, 6.2
-// TB/s; 48 windows of 1024 (101 MB): 25.2 us, of which 15.6 from the first load's issue to the last tile: the rest is finding the run (1.8), joining (1.6) and the second
+// TB/s (by the lengths that are drawn up to 96); 48 windows of 1024 (101 MB): 25.2 us, of which 15.6 from the first load's issue to the last tile: the rest is finding the run (1.8), joining (1.6) and the second
 // kernel with its start (3.5); one sequence of 37 tokens: 5.0 us, a chain of four dependent loads.
 #include "../core/launch.hpp"
 #include "../symm/cu_driver.hpp"
@@ -115,11 +116,6 @@ template <typename H>
 __device__ __forceinline__ float2 unpair(uint32_t v) {
   return H::up(*reinterpret_cast<const typename H::T2*>(&v));
 }
-
-// Where a warp is: an item is a head of keys and values of a sequence (and a block of its query heads), t the tile within it.
-struct Place {
-  int item, t;
-};
 
 // A stage is a tile of K, the same of V, and the queries where the tile is the first of its piece.  A tile is KT / 16 blocks of 16 positions; a block
 // is DP / 64 runs of 16 rows x 128 bytes, the eight 16-byte pieces of a row in the order of the 128-byte swizzle (DP = 32: one run of 64-byte rows with

@@ -2,12 +2,14 @@
 //
 // Three kernels.  For up to 16 rows of x that fit shared memory the weights are read once, half a byte each: the narrow kernel multiplies codes as whole
 // numbers (bf16 holds -15 to 15 exactly) and applies a group's scale to its sum in fp32, scale * sum x (code - zero), so nothing but x and y is rounded to
-// 16 bits.  Its time is that of taking the codes apart: some 190 instructions per KB.  For more rows bf16 weights, scale * (code - zero) rounded once, are
+// 16 bits.  Neither memory (28 % of its rate under the profiler) nor issue (53 % of the slots, 49 % of the ALU pipe: some 190 instructions per KB, most of
+// them to take codes apart) is full: four warps per scheduler wait for their own chains as much as for slots.  For more rows bf16 weights, scale * (code - zero) rounded once, are
 // made on the way into tensor memory, where they are the left operand of tcgen05 products: a block per tile and part of K where that fills the SMs (the wide
 // kernel), a block per SM that runs on from tile to tile where there are several for each (the stream kernel).  For 16384 x 2048 the
 // narrow kernel takes 7.4 us for 8 rows and 10.3 for 16, the wide one 9.6 for up to 32: where they meet the narrow one stays, which rounds no weights.
 // Measured (codes from memory): 4 x 32000 x 2048, 36 MB: 12.7 us, 2.8 TB/s; 1 x 16384 x 2048: 6.5 us; 1 x 2048 x 2048: 2.6 us, a launch and one chain of loads;
-// 48 x 3072 x 768: 5.0 us; 128 x 16384 x 2048: 11.3 us, 0.76 PFLOP/s; 256: 16.0 us; 1537: 80 us, 1.29 PFLOP/s.
+// 48 x 3072 x 768: 5.0 us; 128 x 16384 x 2048: 11.3 us, 0.76 PFLOP/s; 256: 16.0 us; 1537: 95 us, 1.09 PFLOP/s, among calls that go on for seconds (80 us, 1.29
+// PFLOP/s, in a burst, before the power limit lowers the clock).
 #include <cuda.h>
 
 #include <array>
@@ -664,7 +666,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) w4_wide_kernel(const __grid_c
 // ------------------------------------------------- tiles for several rounds of SMs --
 // The same products for more tiles than there are SMs: a block takes tiles gridDim.x apart, and its four roles run on from one to the next.  Two sets of
 // sums in tensor memory (up to 176 rows of x each, behind them five chunks of weights: 512 columns) let eight warps of their own write a tile's results beside
-// the next one's products.  1537 x 16384 x 2048 takes 80 us, 1.29 PFLOP/s (89 and more when it goes on for seconds and the power limit lowers the clock): 500 clocks per
+// the next one's products.  1537 x 16384 x 2048 takes 80 us in a burst, 1.29 PFLOP/s (95, 1.09, when calls go on for seconds and the power limit lowers the clock): 500 clocks per
 // chunk, of which the products want 352.  No role alone is the rest: with a quarter of the products it takes 69 us, with weights that cost no arithmetic 71,
 // with x that need not come 73.  (As one block per tile each round of SMs took 5 us before its first and after its last product: 103 us; four stages 83, six and
 // fewer rows 87; rings of their own for x and weights, whose stages are then variables to the issuing thread, 99.)

@@ -59,7 +59,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     heads is a multiple of the cache's kv_heads: neighbouring query heads share keys and values.  With `window`, only the last `window`
     positions and the first `sinks` are seen; pages without a visible position are not looked at (their table entries may be -1).
     A sequence of length zero gives zeros.  A length beyond the table's row counts as the row's; a visible position whose page
-    lies outside the cache is left out (NaN where none is left).
+    lies outside the cache is left out (NaN where none is left).  What lies at positions that are not seen may be anything; an infinite value at
+    one that is seen makes its column NaN (weights are kept in two parts, of which one may be zero).
 
     return_lse: also the logarithm of the sum of exponentials, fp32 ``[sequences, heads]`` (-inf for an empty sequence), with which parts of
     a longer attention can be joined."""
