@@ -243,7 +243,11 @@ class Generator:
                 rows = list(active)
                 last = torch.stack([logits[r] for r in rows]).float()
                 if temperature > 0:
-                    tokens = torch.multinomial(torch.softmax(last / temperature, dim=-1), 1, generator=generator)[:, 0]
+                    # (a temperature so low that logits / temperature overflows is that of the likeliest token)
+                    chances = torch.softmax(last / max(temperature, 1e-30), dim=-1)
+                    if not bool(torch.isfinite(chances).all()):
+                        raise RuntimeError("Generator: the logits are not finite, there is nothing to draw from")
+                    tokens = torch.multinomial(chances, 1, generator=generator)[:, 0]
                 else:
                     tokens = last.argmax(-1)
                 for row, token in zip(rows, tokens.tolist()):

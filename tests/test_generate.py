@@ -341,3 +341,22 @@ def test_tokens_outside_the_vocabulary():
                 call()
             assert gen.cache.rows == [row] and gen.cache.length(row) == 2 and gen.cache.free_pages == free
     gen.step([row], [511])
+
+
+def test_temperatures_near_zero():
+    torch.manual_seed(7)
+    gen = Generator(sharpen(build_decoder("tiny")), max_sequences=2)
+    likeliest = gen.generate([[1, 2], [3]], 4)
+    for temperature in (1e-20, 1e-39, 1e-46):
+        assert gen.generate([[1, 2], [3]], 4, temperature=temperature) == likeliest
+    assert gen.cache.rows == []
+
+
+def test_no_token_is_drawn_from_logits_that_are_no_numbers():
+    model = build_decoder("tiny")
+    with torch.no_grad():
+        model.ln_f.weight[3] = float("nan")
+    gen = Generator(model, max_sequences=2)
+    with pytest.raises(RuntimeError, match="Generator"):
+        gen.generate([[1, 2]], 3, temperature=1.0)
+    assert gen.cache.rows == []
