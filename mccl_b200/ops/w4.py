@@ -102,6 +102,8 @@ def quantize_w4(weight: torch.Tensor, group: int = 128) -> W4Weight:
     w = weight.detach().float().view(n, k // group, group)
     low, high = w.amin(-1).clamp(max=0.0), w.amax(-1).clamp(min=0.0)
     scale = ((high - low) / 15.0).to(torch.bfloat16).float()
+    if not bool(torch.isfinite(scale).all()):
+        raise RuntimeError("quantize_w4: weights that are not finite, or that no scale spans")
     scale = torch.where(scale > 0, scale, torch.ones_like(scale))
     zero = (-low / scale).round().clamp(0, 15)
     codes = (w / scale[..., None]).round().add(zero[..., None]).clamp(0, 15).to(torch.uint8).view(n, k)

@@ -366,3 +366,16 @@ def test_no_token_is_drawn_from_logits_that_are_no_numbers():
     with pytest.raises(RuntimeError, match="Generator"):
         gen.generate([[1, 2]], 3, temperature=1.0)
     assert gen.cache.rows == []
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_weights_that_are_no_numbers_are_not_quantized(value):
+    w = torch.randn(20, 128)
+    w[17, 100] = value
+    with pytest.raises(RuntimeError, match="quantize_w4"):
+        ops.quantize_w4(w, 64)
+    w[17, 100] = 0.0
+    ops.quantize_w4(w, 64)
+    with pytest.raises(RuntimeError, match="quantize_w4"):
+        ops.quantize_w4(torch.tensor([3e38, -3e38]).repeat(1, 16), 32)     # a range that no scale spans
+    assert ops.quantize_w4(w[:0], 64).shape == (0, 128)
