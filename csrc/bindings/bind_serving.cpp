@@ -197,7 +197,11 @@ void bind_serving(py::module_& m) {
           MCCL_CHECK_TENSOR(pages.stride(i) == outer_stride * outer, op << ": the dimensions before the pages must have one common stride");
           outer *= pages.size(i);
         }
-        MCCL_CHECK_TENSOR((pages.size(dim) <= 1 || pages.stride(dim) >= page) && (outer == 1 || outer_stride != 0), op << ": pages that overlap in memory");
+        // pages of one outer index lie one after the other and the outer indices behind them, or the outer indices within a page's stride
+        const int64_t many = pages.size(dim), stride = pages.stride(dim);
+        MCCL_CHECK_TENSOR((many <= 1 || stride >= page) && (outer <= 1 || (outer_stride >= page && (many <= 1 || outer_stride >= (many - 1) * stride + page ||
+                                                                                                   stride >= (outer - 1) * outer_stride + page))),
+                          op << ": pages that overlap in memory");
         const int count = as_int(pages.size(dim), op);
         c10::cuda::CUDAGuard guard(pages.device());
         if (pages.numel() > 0)

@@ -128,3 +128,17 @@ def test_gelu_has_no_error_of_its_own(rows, n, k, group, residual):
     if rows > 16:
         before = before + 6 * 2.0 ** -8 * ((x.double() ** 2) @ (w.t() ** 2) / 3).sqrt()
     assert ((y - want).abs() <= 2.0 ** -8 * want.abs() + 1.13 * before + 2.0 ** -22 * z.abs()).all()
+
+
+def test_copies_into_pages_that_overlap_are_refused():
+    memory = torch.arange(64, dtype=torch.float32, device="cuda")
+    one = torch.ones(1, dtype=torch.int32, device="cuda")
+    for size, stride in (((2, 4, 8), (8, 8, 1)), ((3, 3, 8), (16, 8, 1)), ((2, 3, 8), (12, 8, 1)), ((2, 4, 8), (4, 16, 1)), ((1, 4, 8), (0, 4, 1))):
+        with pytest.raises(RuntimeError, match="overlap"):
+            ops.copy_pages(memory.as_strided(size, stride), one, one * 2, dim=1)
+    for size, stride in (((2, 4, 8), (32, 8, 1)), ((2, 4, 8), (8, 16, 1)), ((1, 4, 8), (1, 8, 1)), ((2, 1, 8), (8, 1, 1))):     # pages of two layers in turn, too
+        pages = memory.clone().as_strided(size, stride)
+        want = pages.clone()
+        if size[1] > 2:
+            want[:, 2] = want[:, 1]
+        assert torch.equal(ops.copy_pages(pages, one, one * 2, dim=1), want)
