@@ -54,6 +54,19 @@ bool vector_rows(const at::Tensor& t) {
     if (t.size(i) > 1 && t.stride(i) % 8 != 0) return false;
   return true;
 }
+// Whether a tensor has elements that are one place in memory (a dimension that was expanded), and whether two of the same sizes are the same places, all or, where
+// both are without gaps, some.  (at::get_overlap_status and its like cost a small call a quarter of a microsecond.)
+bool repeated(const at::Tensor& t) {
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1 && t.stride(i) == 0) return true;
+  return false;
+}
+bool same_memory(const at::Tensor& a, const at::Tensor& b) {
+  if (a.numel() == 0) return false;
+  const uintptr_t at_a = reinterpret_cast<uintptr_t>(a.data_ptr()), at_b = reinterpret_cast<uintptr_t>(b.data_ptr());
+  const uintptr_t apart = at_a > at_b ? at_a - at_b : at_b - at_a;
+  return apart == 0 || (apart < static_cast<uintptr_t>(a.nbytes()) && a.is_non_overlapping_and_dense() && b.is_non_overlapping_and_dense());
+}
 const int* need_int32(const at::Tensor& t, const at::Tensor& like, int64_t count, const char* what) {
   need_on(t, like, what);
   MCCL_CHECK_TENSOR(t.scalar_type() == at::kInt && t.dim() == 1 && t.is_contiguous(), what << ": expected a contiguous one-dimensional int32 tensor");
@@ -127,6 +140,7 @@ void bind_serving(py::module_& m) {
         a.type = half16(k, op);
         MCCL_CHECK_TENSOR(v.scalar_type() == k.scalar_type() && v.sizes() == k.sizes(), op << ": k and v differ in dtype or sizes");
         const Cache c = cache_of(k_pages, v_pages, table, k, op);
+        MCCL_CHECK_TENSOR(!repeated(k_pages) && !repeated(v_pages) && !same_memory(k_pages, v_pages), op << ": pages that overlap in memory");
         a.k = tokens_of(k, "paged_append(k)");
         a.v = tokens_of(v, "paged_append(v)");
         a.k_pages = c.k;

@@ -142,3 +142,18 @@ def test_copies_into_pages_that_overlap_are_refused():
         if size[1] > 2:
             want[:, 2] = want[:, 1]
         assert torch.equal(ops.copy_pages(pages, one, one * 2, dim=1), want)
+
+
+def test_tokens_into_pages_that_overlap_are_refused():
+    k, v = torch.randn(2, 2, 2, 16, device="cuda").to(torch.bfloat16)
+    table, at = torch.arange(4, dtype=torch.int32, device="cuda").view(2, 2), torch.ones(2, dtype=torch.int32, device="cuda")
+    pages = torch.zeros(2, 4, 2, 8, 16, dtype=torch.bfloat16, device="cuda")
+    for k_pages, v_pages in ((pages[0, :1].expand(4, -1, -1, -1), pages[1]), (pages[0], pages[1, :, :1].expand(-1, 2, -1, -1)), (pages[0], pages[0]),
+                             (pages.view(8, 2, 8, 16)[:4], pages.view(8, 2, 8, 16)[3:7])):
+        with pytest.raises(RuntimeError, match="paged_append"):
+            ops.paged_append(k, v, k_pages, v_pages, table, at)
+    assert not pages.any()
+    ops.paged_append(k, v, pages[0], pages[1], table, at)
+    both = torch.zeros(4, 2, 2, 8, 16, dtype=torch.bfloat16, device="cuda")     # keys and values of a page side by side
+    ops.paged_append(k, v, both[:, 0], both[:, 1], table, at)
+    assert torch.equal(both.transpose(0, 1), pages)
