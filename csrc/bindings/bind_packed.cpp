@@ -1,0 +1,166 @@
+// Python bindings of the operators around whole prompts and packed texts (csrc/ops/packed.hpp).  As in bind_serving.cpp every function checks its operands,
+// allocates through torch and launches on the current stream of the operands' device.  Those that models train with are autograd nodes of their own here: a
+// Python node costs more host time than the kernels of a few thousand tokens take.
+#include "../ops/ops.hpp"
+#include "../ops/packed.hpp"
+#include "bind.hpp"
+#include "operand_checks.hpp"
+
+#include <cmath>
+
+namespace py = pybind11;
+
+namespace mccl {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+namespace {
+
+void need_no_tangent(const at::Tensor& t, const char* what) {
+  MCCL_CHECK_TENSOR(!(c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined()), what << ": has no forward-mode derivative; a tangent would be lost");
+}
+// A backward pass that would itself be differentiated.
+void need_first_order(const char* what) { MCCL_CHECK_TENSOR(!at::GradMode::is_enabled(), what << ": has no second derivative (create_graph)"); }
+
+// As tensor maps and 16-byte accesses take them: gradients and expanded tensors come in any strides.
+at::Tensor rows_of_heads(const at::Tensor& t) { return vector_rows(t) && !repeated(t) ? t : t.contiguous(); }
+
+// The operands of a call as the kernels take them.
+struct Attention {
+  at::Tensor q, k, v, offsets, k_offsets;
+  double scale;
+  int64_t window, sinks;
+
+  ops::PackedAttentionArgs args(const char* op) const {
+    ops::PackedAttentionArgs a;
+    a.type = half16(q, op);
+    a.q = tokens_of(q, "packed_attention(q)");
+    a.k = tokens_of(k, "packed_attention(k)");
+    a.v = tokens_of(v, "packed_attention(v)");
+    a.offsets = offsets.data_ptr<int>();
+    a.k_offsets = k_offsets.data_ptr<int>();
+    a.tokens = as_int(q.size(0), op);
+    a.k_tokens = as_int(k.size(0), op);
+    a.sequences = as_int(offsets.numel() - 1, op);
+    a.heads = as_int(q.size(1), op);
+    a.kv_heads = as_int(k.size(1), op);
+    a.head_dim = as_int(q.size(2), op);
+    a.scale = static_cast<float>(scale);
+    const int64_t most = std::numeric_limits<int>::max();
+    a.window = static_cast<int>(std::min(window, most));
+    a.sinks = static_cast<int>(std::min(sinks, most));
+    return a;
+  }
+};
+
+// (o, lse [heads, tokens] or undefined)
+std::pair<at::Tensor, at::Tensor> attention_forward(const Attention& x, bool lse) {
+  const char* op = "packed_attention";
+  ops::PackedAttentionArgs a = x.args(op);
+  c10::cuda::CUDAGuard guard(x.q.device());
+  at::Tensor o = empty_on(x.q, {x.q.size(0), x.q.size(1), x.q.size(2)}, x.q.scalar_type()), l;
+  a.o = o.data_ptr();
+  if (lse) {
+    l = empty_on(x.q, {x.q.size(1), x.q.size(0)}, at::kFloat);
+    a.lse = l.data_ptr<float>();
+  }
+  if (a.k_tokens == 0 || a.sequences == 0) {   // nothing to see
+    o.zero_();
+    if (lse) l.fill_(-std::numeric_limits<float>::infinity());
+  } else {
+    check_launch(ops::packed_attention(a, stream_of(x.q)), op);
+  }
+  return {o, l};
+}
+
+struct AttentionNode : torch::autograd::Function<AttentionNode> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& offsets, const at::Tensor& k_offsets, double scale,
+                               int64_t window, int64_t sinks) {
+    const auto [o, lse] = attention_forward({q, k, v, offsets, k_offsets, scale, window, sinks}, true);
+    ctx->save_for_backward({q, k, v, offsets, k_offsets, o, lse});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["window"] = window;
+    ctx->saved_data["sinks"] = sinks;
+    ctx->mark_non_differentiable({lse});
+    return {o, lse};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const char* op = "packed_attention";
+    need_first_order(op);
+    const auto s = ctx->get_saved_variables();
+    const Attention x{s[0], s[1], s[2], s[3], s[4], ctx->saved_data["scale"].toDouble(), ctx->saved_data["window"].toInt(), ctx->saved_data["sinks"].toInt()};
+    const at::Tensor &o = s[5], &lse = s[6], d_o = rows_of_heads(grads[0]);
+    c10::cuda::CUDAGuard guard(x.q.device());
+    at::Tensor dq = empty_on(x.q, x.q.sizes(), at::kBFloat16), dk = empty_on(x.q, x.k.sizes(), at::kBFloat16), dv = empty_on(x.q, x.v.sizes(), at::kBFloat16);
+    if (x.k.size(0) == 0 || x.q.size(0) == 0 || x.offsets.numel() == 1) {
+      dq.zero_();
+      dk.zero_();
+      dv.zero_();
+    } else {
+      ops::PackedAttentionGradArgs a;
+      a.f = x.args(op);
+      a.f.lse = lse.data_ptr<float>();
+      a.o = tokens_of(o, op);
+      a.d_o = tokens_of(d_o, "packed_attention(gradient)");
+      a.dq = dq.data_ptr();
+      a.dk = dk.data_ptr();
+      a.dv = dv.data_ptr();
+      at::Tensor delta = empty_on(x.q, lse.sizes(), at::kFloat);
+      a.delta = delta.data_ptr<float>();
+      check_launch(ops::packed_attention_grad(a, stream_of(x.q)), "packed_attention backward");
+    }
+    return {dq, dk, dv, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+}  // namespace
+
+void bind_packed(py::module_& m) {
+  m.def(
+      "packed_attention",
+      [](const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& offsets, const c10::optional<at::Tensor>& k_offsets, double scale, int64_t window,
+         int64_t sinks, bool return_lse) -> std::pair<at::Tensor, c10::optional<at::Tensor>> {
+        const char* op = "packed_attention";
+        bool train = false;
+        for (const auto* t : {&q, &k, &v}) {
+          need_on(*t, q, op);
+          need_no_tangent(*t, op);
+          MCCL_CHECK_TENSOR(t->dim() == 3, op << ": expected [tokens, heads, head_dim]");
+          MCCL_CHECK_TENSOR(t->scalar_type() == q.scalar_type(), op << ": q, k and v differ in dtype");
+          train = train || t->requires_grad();
+        }
+        train = train && at::GradMode::is_enabled();
+        half16(q, op);
+        MCCL_CHECK_TENSOR(!train || q.scalar_type() == at::kBFloat16, op << ": gradients are computed in bf16 only (in fp16 the gradients of scores fall below its smallest numbers)");
+        MCCL_CHECK_TENSOR(k.sizes() == v.sizes(), op << ": keys and values of different sizes");
+        MCCL_CHECK_TENSOR(q.size(2) == k.size(2), op << ": q has head_dim " << q.size(2) << ", k " << k.size(2));
+        MCCL_CHECK_TENSOR(q.size(2) > 0 && q.size(2) % 8 == 0 && q.size(2) <= 128, op << ": head_dim must be a multiple of 8 up to 128");
+        MCCL_CHECK_TENSOR(k.size(1) > 0 && q.size(1) % k.size(1) == 0, op << ": " << q.size(1) << " query heads over " << k.size(1) << " heads of keys and values");
+        MCCL_CHECK_TENSOR(std::max(q.size(0), k.size(0)) < (1 << 30), op << ": 2^30 tokens or more");
+        MCCL_CHECK_TENSOR(offsets.dim() == 1 && offsets.numel() >= 1, op << ": offsets must be int32 [sequences + 1]");
+        need_int32(offsets, q, offsets.numel(), "packed_attention(offsets)");
+        if (k_offsets.has_value()) need_int32(*k_offsets, q, offsets.numel(), "packed_attention(k_offsets)");
+        MCCL_CHECK_TENSOR(k_offsets.has_value() || q.size(0) == k.size(0), op << ": " << q.size(0) << " queries and " << k.size(0) << " keys without offsets of their own");
+        MCCL_CHECK_TENSOR(std::isfinite(scale) && scale > 0 && static_cast<float>(scale) > 0, op << ": scale must be a positive number");
+        MCCL_CHECK_TENSOR(window >= 0 && sinks >= 0, op << ": window and sinks must not be negative");
+        // expanded tensors are copied; other strides than the kernels' are refused
+        auto dense = [](const at::Tensor& t) { return repeated(t) ? t.contiguous() : t; };
+        const at::Tensor q_ = dense(q), k_ = dense(k), v_ = dense(v), ko = k_offsets.value_or(offsets);
+        for (const auto* t : {&q_, &k_, &v_}) tokens_of(*t, op);
+        at::Tensor o, lse;
+        if (train) {
+          const variable_list r = AttentionNode::apply(q_, k_, v_, offsets, ko, scale, window, sinks);
+          o = r[0];
+          lse = r[1];
+        } else {
+          std::tie(o, lse) = attention_forward({q_, k_, v_, offsets, ko, scale, window, sinks}, return_lse);
+        }
+        if (!return_lse) return {o, c10::nullopt};
+        return {o, lse.t()};
+      },
+      py::arg("q"), py::arg("k"), py::arg("v"), py::arg("offsets"), py::arg("k_offsets") = py::none(), py::arg("scale"), py::arg("window") = 0, py::arg("sinks") = 0,
+      py::arg("return_lse") = false);
+}
+
+}  // namespace mccl

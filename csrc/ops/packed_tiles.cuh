@@ -1,0 +1,183 @@
+// What the kernels of packed attention share: which tile a block works on, which keys its rows see, tiles in shared memory and tensor memory.
+#pragma once
+
+#include "../core/launch.hpp"
+#include "../symm/cu_driver.hpp"
+#include "half16.cuh"
+#include "ops.hpp"
+#include "packed.hpp"
+#include "tcgen05.cuh"
+
+#include <type_traits>
+
+namespace mccl {
+namespace ops {
+
+int* gemm_error_device_ptr();
+
+namespace packed {
+
+constexpr int kRows = 128;                 // queries of a tile, and keys of a block
+constexpr int kSub = kRows * 64 * 2;       // a tile's 64 columns: rows of 128 bytes with the 128-byte swizzle, 16 KB
+constexpr float kLog2e = 1.4426950408889634f;
+
+// What all kernels know of the problem.
+struct Problem {
+  const int* offsets;
+  const int* k_offsets;
+  int tokens, k_tokens, sequences, heads, kv_heads, group, head_dim;
+  int window, sinks;   // window: 2^30 without one
+  float scale, scale_log2;
+  int* err;
+};
+
+// A sequence's rows among the queries and among the keys.
+struct Sequence {
+  int q0, n, k0, m;
+};
+__device__ __forceinline__ int clamp(int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); }
+__device__ __forceinline__ Sequence sequence_of(const Problem& p, int s) {
+  Sequence r;
+  r.q0 = clamp(p.offsets[s], 0, p.tokens);
+  r.n = clamp(p.offsets[s + 1], r.q0, p.tokens) - r.q0;
+  r.k0 = clamp(p.k_offsets[s], 0, p.k_tokens);
+  r.m = clamp(p.k_offsets[s + 1], r.k0, p.k_tokens) - r.k0;
+  return r;
+}
+
+// Slots of `rows` rows: sequence s begins at slot offsets[s] / rows + s, which leaves it enough of them (floor(a + n) - floor(a) + 1 >= ceil(n)) and needs no sums
+// over the sequences before it.  Whole-warp call: the sequence whose slots `slot` belongs to (-1: none) by probing 32 places at a time.
+__device__ __forceinline__ int find_sequence(const int* offsets, int sequences, int tokens, int slot, int rows) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = sequences;
+  bool first = true;
+  while (n > 1 || first) {
+    first = false;
+    const int step = (n + 31) / 32, at = lo + lane * step;
+    const bool below = lane * step < n && clamp(offsets[at], 0, tokens) / rows + at <= slot;
+    const int count = __popc(__ballot_sync(0xffffffffu, below));
+    if (count == 0) return -1;
+    lo += (count - 1) * step;
+    n = min(step, n - (count - 1) * step);
+  }
+  return lo;
+}
+__host__ __device__ __forceinline__ long long slots_of(long long tokens, int sequences, int rows) { return tokens / rows + sequences; }
+
+// Blocks of keys that a tile of queries sees: [0, sink) and [lo, hi).
+struct Blocks {
+  int sink, lo, hi;
+  __device__ __forceinline__ bool has(int b) const { return b < sink || (b >= lo && b < hi); }
+  __device__ __forceinline__ int next(int b) const {   // the next one after b
+    ++b;
+    return b >= sink && b < lo ? lo : b;
+  }
+};
+// rows: positions first .. last
+__device__ __forceinline__ Blocks blocks_of(const Problem& p, int first, int last) {
+  Blocks r;
+  r.hi = last < 0 ? 0 : last / kRows + 1;
+  r.lo = min(max(0, first - p.window + 1) / kRows, r.hi);
+  r.sink = min((min(p.sinks, 1 << 30) + kRows - 1) / kRows, r.lo);
+  return r;
+}
+// Whether every one of the positions first .. last sees all keys of block b.
+__device__ __forceinline__ bool all_seen(const Problem& p, int b, int first, int last) {
+  const int k0 = b * kRows, k1 = k0 + kRows - 1;
+  return k1 <= first && (k0 > last - p.window || k1 < p.sinks);
+}
+
+// --------------------------------------------------------------------------------------------------- memory ----
+// Byte offset of 16-byte chunk c (0..7) of row r in a [rows x 64] tile as TMA stores it with the 128-byte swizzle.
+__device__ __forceinline__ uint32_t sw128(int r, int c) { return static_cast<uint32_t>(r * 128 + ((c ^ (r & 7)) << 4)); }
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// 64 columns from `col` of `head` in rows row .. row + 127; zeros behind the tensor's end and its head_dim.
+__device__ __forceinline__ void load_box(void* dst, const CUtensorMap* map, uint64_t* bar, int col, int head, int row) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(tc::smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(tc::smem_u32(bar)), "r"(col), "r"(head), "r"(row)
+      : "memory");
+}
+template <int DP>
+__device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int head, int row) {
+#pragma unroll
+  for (int c = 0; c < DP / 64; ++c) load_box(dst + c * kSub, map, bar, c * 64, head, row);
+}
+
+// Instruction descriptor of 16-bit operands with fp32 sums.
+template <typename H>
+__host__ __device__ constexpr uint32_t idesc16(int m, int n, bool a_mn, bool b_mn) {
+  constexpr uint32_t type = std::is_same<H, Bf16>::value ? 1u : 0u;
+  return (1u << 4) | (type << 7) | (type << 10) | (a_mn ? (1u << 15) : 0u) | (b_mn ? (1u << 16) : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(m >> 4) << 24);
+}
+// D[tmem] (+)= A[tmem] B[smem]; issued by one thread.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t desc_b, uint32_t idesc, bool accumulate) {
+  const uint32_t acc = accumulate ? 1u : 0u;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(desc_b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// Products over K-major tiles: D[128 x 128 keys] = A B^T over `steps` steps of 16 columns.
+__device__ __forceinline__ void mma_rows(uint32_t d, const uint8_t* a, const uint8_t* b, uint32_t idesc, int steps) {
+  const uint64_t da = tc::smem_desc_k_sw128(a), db = tc::smem_desc_k_sw128(b);
+#pragma unroll 4
+  for (int k = 0; k < steps; ++k) {
+    const uint64_t off = static_cast<uint64_t>((k >> 2) * (kSub >> 4) + (k & 3) * 2);
+    tc::mma_bf16(d, da + off, db + off, idesc, k != 0);
+  }
+}
+// D[128 x n] (+)= A[tmem, 128 x 128] B with B's rows along the sum: 128 rows of a tile.
+__device__ __forceinline__ void mma_weights(uint32_t d, uint32_t a, const uint8_t* b, uint32_t idesc, bool accumulate) {
+  const uint64_t db = tc::smem_desc_mn_sw128(b, kSub);
+#pragma unroll
+  for (int k = 0; k < kRows / 16; ++k) mma_ts(d, a + 8 * k, db + 128 * k, idesc, k != 0 || accumulate);
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+      "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// A wait that gives up, and at once when another role of the block has: the first to give up says so in *bad.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* bad) {
+  for (uint32_t i = 0; i < (1u << 22); ++i) {
+    if (tc::mbar_try_wait(bar, parity)) return true;
+    if ((i & 15) == 15 && *bad) return false;
+  }
+  *bad = 1;
+  return false;
+}
+
+// [tokens, heads, head_dim] as boxes of 64 columns of 128 rows of a head.  (The stride of a dimension of one is never used and may be anything.)
+inline bool encode_rows(CUtensorMap* map, Half16 type, const TokenView& t, int tokens, int heads, int head_dim) {
+  const CuDriver& cu = CuDriver::get();
+  if (!cu.loaded || !cu.TensorMapEncodeTiled) return false;
+  const cuuint64_t size[3] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>((heads > 1 ? t.head : head_dim) * 2), static_cast<cuuint64_t>((tokens > 1 ? t.token : head_dim) * 2)};
+  const cuuint32_t box[3] = {64, 1, kRows}, step[3] = {1, 1, 1};
+  return cu.TensorMapEncodeTiled(map, type == Half16::bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(t.p), size,
+                                 strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace packed
+}  // namespace ops
+}  // namespace mccl

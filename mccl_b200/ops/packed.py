@@ -1,0 +1,71 @@
+"""Whole prompts and packed texts: causal attention of texts of different lengths that lie one behind the other, without padding between them, and
+rotary positions of any tokens.
+
+Queries, keys and values are ``[tokens, heads, head_dim]``; ``offsets``, int32 ``[texts + 1]`` on the device, says where each text begins (and the
+last one ends).  Nothing of a call depends on numbers the host would have to wait for, so it can be captured in a CUDA graph.
+
+CUDA tensors run this package's kernels; CPU tensors run the plain forms below (tests without a GPU).
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+
+from .. import _C
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor, k_offsets: Optional[torch.Tensor] = None, *, scale: Optional[float] = None,
+                     window: Optional[int] = None, sinks: int = 0, return_lse: bool = False):
+    """Causal attention within each of the texts: softmax(scale q.K) V for q ``[tokens, heads, head_dim]`` and k, v ``[tokens, kv_heads, head_dim]``;
+    scale defaults to ``head_dim ** -0.5``.  bf16 and fp16, head dimensions of up to 128 (multiples of 8); gradients of q, k and v in bf16.
+
+    Text s has the tokens ``offsets[s]`` to ``offsets[s + 1] - 1``; offsets do not decrease, a text may be empty.  With `k_offsets` its keys are
+    ``k_offsets[s]`` to ``k_offsets[s + 1] - 1`` instead: those in front of its queries are from before (a prompt that goes on behind what a cache
+    holds), the last query stands at the last key.  heads is a multiple of kv_heads: neighbouring query heads share keys and values.
+    With `window`, only the last `window` positions and the first `sinks` of the text are seen.
+
+    Rows of no text, and queries that see nothing (more queries than keys), give zeros, and zero gradients.  What lies at positions that a query does not
+    see has no influence on its result, whatever it is; an infinite or NaN value at one that is seen makes its column infinite or NaN.  In the gradients
+    such numbers may reach other positions of the same text, but no other text.
+
+    return_lse: also the logarithm of the sum of exponentials, fp32 ``[tokens, heads]`` (-inf where nothing is seen; no gradient)."""
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    if window is None:
+        if sinks:
+            raise RuntimeError("packed_attention: sinks without a window")
+    elif window < 1:
+        raise RuntimeError(f"packed_attention: window must be positive, got {window}")
+    if q.is_cuda:
+        o, lse = _C.packed_attention(q, k, v, offsets, k_offsets, scale, 0 if window is None else window, sinks, return_lse)
+        return (o, lse) if return_lse else o
+    starts = offsets.tolist()
+    key_starts = starts if k_offsets is None else k_offsets.tolist()
+    group = q.shape[1] // k.shape[1]
+    parts, sums, at = [], [], 0
+    nothing = q.new_zeros((0, *q.shape[1:])), torch.zeros(0, q.shape[1])
+
+    def rows_without(n):
+        parts.append(q.new_zeros((n, *q.shape[1:])))
+        sums.append(torch.full((n, q.shape[1]), -math.inf))
+
+    for first, last, key, key_end in zip(starts, starts[1:], key_starts, key_starts[1:]):
+        rows_without(first - at)
+        n, m, at = last - first, key_end - key, last
+        blind = min(n, max(0, n - m))   # these stand in front of the first key
+        rows_without(blind)
+        if n == blind:
+            continue
+        i, j = torch.arange(m - (n - blind), m)[:, None], torch.arange(m)[None]
+        seen = j <= i
+        if window is not None:
+            seen = seen & ((j > i - window) | (j < sinks))
+        qq, kk, vv = q[first + blind:last].float(), *(t[key:key_end].float().repeat_interleave(group, dim=1) for t in (k, v))
+        score = torch.where(seen, torch.einsum("ihd,jhd->hij", qq, kk) * scale, -math.inf)
+        sums.append(torch.logsumexp(score, -1).t())
+        parts.append(torch.einsum("hij,jhd->ihd", torch.softmax(score, -1), vv).to(q.dtype))
+    rows_without(q.shape[0] - at)
+    o = torch.cat([nothing[0], *parts])
+    return (o, torch.cat([nothing[1], *sums]).detach()) if return_lse else o
