@@ -137,7 +137,7 @@ void bind_packed(py::module_& m) {
         MCCL_CHECK_TENSOR(q.size(2) == k.size(2), op << ": q has head_dim " << q.size(2) << ", k " << k.size(2));
         MCCL_CHECK_TENSOR(q.size(2) > 0 && q.size(2) % 8 == 0 && q.size(2) <= 128, op << ": head_dim must be a multiple of 8 up to 128");
         MCCL_CHECK_TENSOR(k.size(1) > 0 && q.size(1) % k.size(1) == 0, op << ": " << q.size(1) << " query heads over " << k.size(1) << " heads of keys and values");
-        MCCL_CHECK_TENSOR(std::max(q.size(0), k.size(0)) < (1 << 30), op << ": 2^30 tokens or more");
+        MCCL_CHECK_TENSOR(std::max(q.size(0), k.size(0)) < (1 << 29), op << ": 2^29 tokens or more");
         MCCL_CHECK_TENSOR(offsets.dim() == 1 && offsets.numel() >= 1, op << ": offsets must be int32 [sequences + 1]");
         need_int32(offsets, q, offsets.numel(), "packed_attention(offsets)");
         if (k_offsets.has_value()) need_int32(*k_offsets, q, offsets.numel(), "packed_attention(k_offsets)");

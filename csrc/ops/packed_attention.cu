@@ -415,23 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint4 raw;
-          typename H::T2* h = reinterpret_cast<typename H::T2*>(&raw);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) h[e] = H::down(f[8 * c + 2 * e], f[8 * c + 2 * e + 1]);
-          *reinterpret_cast<uint4*>(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = raw;
-        }
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = i * 8 + (lane >> 2), c = lane & 3;
-          if (u.row[t] + (warp & 3) * 32 + r < u.s.n && c0 + c * 8 < p.head_dim)
-            *reinterpret_cast<uint4*>(o_base + static_cast<long long>(r) * p.heads * p.head_dim + c0 + c * 8) =
-                *reinterpret_cast<const uint4*>(stage + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
-        }
-        __syncwarp();
+        rows_out<H>(stage, f, o_base, static_cast<long long>(p.heads) * p.head_dim, u.s.n - u.row[t] - (warp & 3) * 32, c0, p.head_dim);
       }
     }
     tc::fence_before_sync();
@@ -442,35 +426,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc::fence_after_sync();
     tc::tmem_dealloc(tmem, 512);
   }
-  // rows of no sequence: zeros
-  const int begin = clamp(p.offsets[0], 0, p.tokens), end = max(begin, clamp(p.offsets[p.sequences], 0, p.tokens));
-  const long long outside = static_cast<long long>(begin) + p.tokens - end;
-  for (long long i = blockIdx.x; i < outside; i += gridDim.x) {
-    const long long r = i < begin ? i : end + (i - begin);
-    uint4* to = reinterpret_cast<uint4*>(static_cast<typename H::T*>(a.o) + r * p.heads * p.head_dim);
-    for (int c = tid; c < p.heads * p.head_dim / 8; c += kThreads) to[c] = make_uint4(0u, 0u, 0u, 0u);
-    if (a.lse != nullptr)
-      for (int h = tid; h < p.heads; h += kThreads) a.lse[static_cast<long long>(h) * p.tokens + r] = -INFINITY;
-  }
-}
-
-Problem problem_of(const PackedAttentionArgs& a) {
-  Problem p;
-  p.offsets = a.offsets;
-  p.k_offsets = a.k_offsets;
-  p.tokens = a.tokens;
-  p.k_tokens = a.k_tokens;
-  p.sequences = a.sequences;
-  p.heads = a.heads;
-  p.kv_heads = a.kv_heads;
-  p.group = a.heads / a.kv_heads;
-  p.head_dim = a.head_dim;
-  p.window = a.window > 0 && a.window < (1 << 30) ? a.window : 1 << 30;
-  p.sinks = a.sinks;
-  p.scale = a.scale;
-  p.scale_log2 = a.scale * kLog2e;
-  p.err = gemm_error_device_ptr();
-  return p;
+  zero_outside<typename H::T>(a.o, p.heads * p.head_dim, a.lse, p.heads, p.offsets, p.sequences, p.tokens);
 }
 
 template <typename H, int DP>

@@ -131,11 +131,12 @@ __device__ __forceinline__ void mma_rows(uint32_t d, const uint8_t* a, const uin
     tc::mma_bf16(d, da + off, db + off, idesc, k != 0);
   }
 }
-// D[128 x n] (+)= A[tmem, 128 x 128] B with B's rows along the sum: 128 rows of a tile.
+// D[128 x n] (+)= A[tmem, 128 x 128] B with B's rows along the sum: 128 rows of a tile.  The second half of A is `kApart` columns behind the first.
+template <int kApart = 32>
 __device__ __forceinline__ void mma_weights(uint32_t d, uint32_t a, const uint8_t* b, uint32_t idesc, bool accumulate) {
   const uint64_t db = tc::smem_desc_mn_sw128(b, kSub);
 #pragma unroll
-  for (int k = 0; k < kRows / 16; ++k) mma_ts(d, a + 8 * k, db + 128 * k, idesc, k != 0 || accumulate);
+  for (int k = 0; k < kRows / 16; ++k) mma_ts(d, a + (k >> 2) * kApart + 8 * (k & 3), db + 128 * k, idesc, k != 0 || accumulate);
 }
 
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
@@ -156,6 +157,40 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// 32 rows (a lane's each) of 32 columns from c0 on leave through 2 KB of the warp's own: 64 bytes of a row from four neighbouring lanes.  `rows` of them exist.
+template <typename H>
+__device__ __forceinline__ void rows_out(uint8_t* stage, const float (&f)[32], typename H::T* to, long long stride, int rows, int c0, int head_dim) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint4 raw;
+    typename H::T2* h = reinterpret_cast<typename H::T2*>(&raw);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[e] = H::down(f[8 * c + 2 * e], f[8 * c + 2 * e + 1]);
+    *reinterpret_cast<uint4*>(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = raw;
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 8 + (lane >> 2), c = lane & 3;
+    if (r < rows && c0 + c * 8 < head_dim) *reinterpret_cast<uint4*>(to + r * stride + c0 + c * 8) = *reinterpret_cast<const uint4*>(stage + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+  }
+  __syncwarp();
+}
+
+// Rows of no sequence, shared out over the grid's blocks: zeros in x [tokens, width], minus infinity in lse [heads, tokens] (may be null).
+template <typename T>
+__device__ __forceinline__ void zero_outside(void* x, int width, float* lse, int heads, const int* offsets, int sequences, int tokens) {
+  const int begin = clamp(offsets[0], 0, tokens), end = max(begin, clamp(offsets[sequences], 0, tokens)), outside = begin + tokens - end;
+  for (int i = blockIdx.x; i < outside; i += gridDim.x) {
+    const long long r = i < begin ? i : end + (i - begin);
+    uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(x) + r * width);
+    for (int c = threadIdx.x; c < width / 8; c += blockDim.x) to[c] = make_uint4(0u, 0u, 0u, 0u);
+    if (lse != nullptr)
+      for (int h = threadIdx.x; h < heads; h += blockDim.x) lse[static_cast<long long>(h) * tokens + r] = -INFINITY;
+  }
+}
+
 // A wait that gives up, and at once when another role of the block has: the first to give up says so in *bad.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* bad) {
   for (uint32_t i = 0; i < (1u << 22); ++i) {
@@ -164,6 +199,25 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
   }
   *bad = 1;
   return false;
+}
+
+inline Problem problem_of(const PackedAttentionArgs& a) {
+  Problem p;
+  p.offsets = a.offsets;
+  p.k_offsets = a.k_offsets;
+  p.tokens = a.tokens;
+  p.k_tokens = a.k_tokens;
+  p.sequences = a.sequences;
+  p.heads = a.heads;
+  p.kv_heads = a.kv_heads;
+  p.group = a.heads / a.kv_heads;
+  p.head_dim = a.head_dim;
+  p.window = a.window > 0 && a.window < (1 << 30) ? a.window : 1 << 30;
+  p.sinks = a.sinks;
+  p.scale = a.scale;
+  p.scale_log2 = a.scale * kLog2e;
+  p.err = gemm_error_device_ptr();
+  return p;
 }
 
 // [tokens, heads, head_dim] as boxes of 64 columns of 128 rows of a head.  (The stride of a dimension of one is never used and may be anything.)
