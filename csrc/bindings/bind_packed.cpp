@@ -114,9 +114,163 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
   }
 };
 
+// Rotation tables and positions of a call.
+struct Turn {
+  at::Tensor cos, sin, positions;   // positions may be undefined
+  bool halves;
+
+  // (q, k or undefined) turned; with `inverse` the other way
+  std::pair<at::Tensor, at::Tensor> operator()(const at::Tensor& q, const at::Tensor& k, bool inverse) const {
+    const char* op = "rotary";
+    ops::RotaryArgs a;
+    a.type = half16(q, op);
+    a.cos = cos.data_ptr<float>();
+    a.sin = sin.data_ptr<float>();
+    a.rope_rows = as_int(cos.size(0), op);
+    a.width = as_int(cos.size(1), op);
+    a.positions = positions.defined() ? positions.data_ptr<int>() : nullptr;
+    a.tokens = as_int(q.size(0), op);
+    a.head_dim = as_int(q.size(2), op);
+    a.halves = halves;
+    a.inverse = inverse;
+    c10::cuda::CUDAGuard guard(q.device());
+    at::Tensor out[2];
+    const at::Tensor* in[2] = {&q, &k};
+    ops::RotaryPart* part[2] = {&a.q, &a.k};
+    for (int i = 0; i < 2; ++i) {
+      if (!in[i]->defined()) continue;
+      out[i] = empty_on(q, in[i]->sizes(), q.scalar_type());
+      part[i]->x = tokens_of(*in[i], i == 0 ? "rotary(q)" : "rotary(k)");
+      part[i]->out = out[i].data_ptr();
+      part[i]->heads = as_int(in[i]->size(1), op);
+    }
+    check_launch(ops::rotary(a, stream_of(q)), op);
+    return {out[0], out[1]};
+  }
+};
+
+struct RotaryNode : torch::autograd::Function<RotaryNode> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const c10::optional<at::Tensor>& k, const at::Tensor& cos, const at::Tensor& sin,
+                               const c10::optional<at::Tensor>& positions, bool halves) {
+    const at::Tensor at = positions.value_or(at::Tensor());
+    ctx->save_for_backward({cos, sin, at});
+    ctx->saved_data["halves"] = halves;
+    ctx->saved_data["both"] = k.has_value();
+    const auto [a, b] = Turn{cos, sin, at, halves}(q, k.value_or(at::Tensor()), false);
+    return k.has_value() ? variable_list{a, b} : variable_list{a};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    need_first_order("rotary");
+    const auto s = ctx->get_saved_variables();
+    const bool both = ctx->saved_data["both"].toBool();
+    const auto [a, b] = Turn{s[0], s[1], s[2], ctx->saved_data["halves"].toBool()}(rows_of_heads(grads[0]), both ? rows_of_heads(grads[1]) : at::Tensor(), true);
+    return {a, b, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+// A setting of a sampler: a number, or one per row.
+template <typename T>
+ops::RowSetting<T> row_setting(const py::object& value, const at::Tensor& logits, at::ScalarType dtype, const char* what, double low, double high) {
+  ops::RowSetting<T> s;
+  if (THPVariable_Check(value.ptr())) {
+    const at::Tensor& t = THPVariable_Unpack(value.ptr());
+    need_on(t, logits, what);
+    MCCL_CHECK_TENSOR(t.scalar_type() == dtype && t.dim() == 1 && t.numel() == logits.size(0) && t.is_contiguous(),
+                      what << ": expected a number or contiguous " << c10::toString(dtype) << " [" << logits.size(0) << "]");
+    s.each = t.data_ptr<T>();
+    return s;
+  }
+  const double v = value.cast<double>();
+  MCCL_CHECK_TENSOR(v >= low && v <= high, what << ": " << v << " is out of range");
+  s.all = static_cast<T>(v);
+  return s;
+}
+
 }  // namespace
 
 void bind_packed(py::module_& m) {
+  m.def(
+      "rotary",
+      [](const at::Tensor& q, const c10::optional<at::Tensor>& k, const at::Tensor& cos_t, const at::Tensor& sin_t, const c10::optional<at::Tensor>& positions,
+         bool halves) -> std::pair<at::Tensor, c10::optional<at::Tensor>> {
+        const char* op = "rotary";
+        need_on(q, q, op);
+        half16(q, op);
+        MCCL_CHECK_TENSOR(q.dim() == 3 && q.size(2) > 0 && q.size(2) % 8 == 0, op << ": expected [tokens, heads, head_dim] with a head_dim that is a multiple of 8");
+        MCCL_CHECK_TENSOR(q.size(0) < std::numeric_limits<int>::max(), op << ": 2^31 - 1 tokens or more");
+        need_no_tangent(q, op);
+        bool train = q.requires_grad();
+        if (k.has_value()) {
+          need_on(*k, q, "rotary(k)");
+          need_no_tangent(*k, op);
+          MCCL_CHECK_TENSOR(k->scalar_type() == q.scalar_type() && k->dim() == 3 && k->size(0) == q.size(0) && k->size(2) == q.size(2),
+                            "rotary(k): another dtype, other tokens or another head_dim than q");
+          train = train || k->requires_grad();
+        }
+        train = train && at::GradMode::is_enabled();
+        for (const auto* t : {&cos_t, &sin_t}) {
+          need_on(*t, q, "rotary(rope)");
+          need_forward_only(*t, "rotary(rope)");
+          MCCL_CHECK_TENSOR(t->scalar_type() == at::kFloat && t->dim() == 2 && t->is_contiguous() && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
+                            "rotary(rope): cos and sin must be contiguous fp32 [positions, pairs] on a 16-byte boundary");
+        }
+        MCCL_CHECK_TENSOR(cos_t.sizes() == sin_t.sizes(), "rotary(rope): cos and sin of different sizes");
+        MCCL_CHECK_TENSOR(cos_t.size(1) > 0 && cos_t.size(1) % 4 == 0 && 2 * cos_t.size(1) <= q.size(2),
+                          "rotary(rope): " << cos_t.size(1) << " pairs for heads of " << q.size(2) << "; multiples of 4 up to half a head are possible");
+        if (positions.has_value()) need_int32(*positions, q, q.size(0), "rotary(positions)");
+        auto dense = [](const at::Tensor& t) { return repeated(t) ? t.contiguous() : t; };
+        const at::Tensor q_ = dense(q);
+        tokens_of(q_, "rotary(q)");
+        c10::optional<at::Tensor> k_;
+        if (k.has_value()) {
+          k_ = dense(*k);
+          tokens_of(*k_, "rotary(k)");
+        }
+        at::Tensor a, b;
+        if (train) {
+          const variable_list r = RotaryNode::apply(q_, k_, cos_t, sin_t, positions, halves);
+          a = r[0];
+          if (k_.has_value()) b = r[1];
+        } else {
+          std::tie(a, b) = Turn{cos_t, sin_t, positions.value_or(at::Tensor()), halves}(q_, k_.value_or(at::Tensor()), false);
+        }
+        if (!b.defined()) return {a, c10::nullopt};
+        return {a, b};
+      },
+      py::arg("q"), py::arg("k"), py::arg("cos"), py::arg("sin"), py::arg("positions") = py::none(), py::arg("halves") = false);
+
+  m.def(
+      "sample",
+      [](const at::Tensor& logits, const at::Tensor& uniform, const py::object& temperature, const py::object& top_k, const py::object& top_p, const py::object& min_p) {
+        const char* op = "sample";
+        need_on(logits, logits, op);
+        const at::ScalarType type = logits.scalar_type();
+        MCCL_CHECK_TENSOR(type == at::kBFloat16 || type == at::kHalf || type == at::kFloat, op << ": expected bf16, fp16 or fp32, got " << c10::toString(type));
+        MCCL_CHECK_TENSOR(logits.dim() == 2 && logits.size(1) >= 1 && logits.size(1) <= (1 << 20), op << ": expected [rows, vocab] with 1 to 2^20 tokens");
+        MCCL_CHECK_TENSOR(logits.size(1) == 1 || logits.stride(1) == 1, op << ": the logits of a row must be contiguous");
+        need_on(uniform, logits, "sample(uniform)");
+        MCCL_CHECK_TENSOR((uniform.scalar_type() == at::kFloat || uniform.scalar_type() == at::kDouble) && uniform.dim() == 1 && uniform.numel() == logits.size(0) && uniform.is_contiguous(),
+                          "sample(uniform): expected contiguous fp32 or fp64 [" << logits.size(0) << "]");
+        ops::SampleArgs a;
+        a.logits = logits.data_ptr();
+        a.stride = logits.stride(0);
+        a.type = type == at::kBFloat16 ? ops::Logits::bf16 : (type == at::kHalf ? ops::Logits::fp16 : ops::Logits::fp32);
+        a.rows = as_int(logits.size(0), op);
+        a.vocab = as_int(logits.size(1), op);
+        a.uniform = uniform.data_ptr();
+        a.uniform64 = uniform.scalar_type() == at::kDouble;
+        a.temperature = row_setting<float>(temperature, logits, at::kFloat, "sample(temperature)", 0.0, 3.4e38);
+        a.top_k = row_setting<int>(top_k, logits, at::kInt, "sample(top_k)", 0.0, std::numeric_limits<int>::max());
+        a.top_p = row_setting<float>(top_p, logits, at::kFloat, "sample(top_p)", 0.0, 1.0);
+        a.min_p = row_setting<float>(min_p, logits, at::kFloat, "sample(min_p)", 0.0, 1.0);
+        c10::cuda::CUDAGuard guard(logits.device());
+        at::Tensor tokens = empty_on(logits, {logits.size(0)}, at::kLong);
+        a.tokens = reinterpret_cast<long long*>(tokens.data_ptr<int64_t>());
+        check_launch(ops::sample(a, stream_of(logits)), op);
+        return tokens;
+      },
+      py::arg("logits"), py::arg("uniform"), py::arg("temperature"), py::arg("top_k"), py::arg("top_p"), py::arg("min_p"));
+
   m.def(
       "packed_attention",
       [](const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& offsets, const c10::optional<at::Tensor>& k_offsets, double scale, int64_t window,

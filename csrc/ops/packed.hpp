@@ -41,5 +41,48 @@ struct PackedAttentionGradArgs {
 };
 cudaError_t packed_attention_grad(const PackedAttentionGradArgs& a, cudaStream_t stream);
 
+// ---- rotary positions.  x [tokens, heads, head_dim] and, where its `heads` is not zero, k of the same tokens: the first 2 * width elements of every head are
+// turned by row positions[t] (null: t) of cos / sin (fp32 [rope_rows, width]) into contiguous out; the others are copied.  Pairs are neighbours or, with `halves`,
+// `width` apart; `inverse` turns the other way.  A token whose position lies outside the tables becomes zeros.  head_dim % 8 == 0, width % 4 == 0.
+struct RotaryPart {
+  TokenView x;
+  void* out = nullptr;
+  int heads = 0;
+};
+struct RotaryArgs {
+  RotaryPart q, k;
+  const float* cos = nullptr;
+  const float* sin = nullptr;
+  const int* positions = nullptr;
+  int rope_rows = 0, width = 0;
+  int tokens = 0, head_dim = 0;
+  bool halves = false, inverse = false;
+  Half16 type = Half16::bf16;
+};
+cudaError_t rotary(const RotaryArgs& a, cudaStream_t stream);
+
+// ---- one token per row of logits [rows, vocab] (stride elements apart).  With w_i = exp((l_i - max) / temperature): the top_k likeliest (<= 0: all; the lowest
+// numbers among equals), of these the fewest likeliest whose weights reach top_p times the sum of these (>= 1: all), of these the ones with w >= min_p; then the
+// lowest i for which the sum of the kept w_j, j <= i, exceeds uniform[row] times their whole sum.  temperature 0: the likeliest.  -1 for a row that holds a NaN
+// or +inf or nothing finite, or whose temperature is negative or NaN.  vocab <= 2^20.
+enum class Logits : int { bf16 = 0, fp16 = 1, fp32 = 2 };
+template <typename T>
+struct RowSetting {
+  const T* each = nullptr;   // one per row, or
+  T all = T(0);              // one for all
+};
+struct SampleArgs {
+  const void* logits = nullptr;
+  long long stride = 0;
+  Logits type = Logits::bf16;
+  int rows = 0, vocab = 0;
+  const void* uniform = nullptr;   // fp32, or fp64
+  bool uniform64 = false;
+  RowSetting<float> temperature, top_p, min_p;
+  RowSetting<int> top_k;
+  long long* tokens = nullptr;
+};
+cudaError_t sample(const SampleArgs& a, cudaStream_t stream);
+
 }  // namespace ops
 }  // namespace mccl

@@ -9,7 +9,7 @@ CUDA tensors run this package's kernels; CPU tensors run the plain forms below (
 from __future__ import annotations
 
 import math
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
@@ -69,3 +69,62 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     rows_without(q.shape[0] - at)
     o = torch.cat([nothing[0], *parts])
     return (o, torch.cat([nothing[1], *sums]).detach()) if return_lse else o
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor] = None, *, rope: Tuple[torch.Tensor, torch.Tensor], positions: Optional[torch.Tensor] = None, layout: str = "interleaved"):
+    """Queries and keys turned by their positions: new tensors (q, k), or q alone without `k`.  q ``[tokens, heads, head_dim]``, k of the same tokens; bf16 or
+    fp16, differentiable.
+
+    rope: (cos, sin), fp32 ``[positions, pairs]`` (:func:`rotary_tables`).  The first ``2 * pairs`` elements of each head are turned, what is behind them stays.
+    Pairs are neighbours in the layout "interleaved" (that of :func:`paged_append` and of this package's models) and `pairs` apart in the layout "half".
+    positions: int32 ``[tokens]`` (without it, token t stands at t).  A token whose position lies outside the tables becomes zeros."""
+    if layout not in ("interleaved", "half"):
+        raise RuntimeError(f"rotary: layouts are 'interleaved' and 'half', not '{layout}'")
+    cos, sin = rope
+    if q.is_cuda:
+        a, b = _C.rotary(q, k, cos, sin, positions, layout == "half")
+        return a if k is None else (a, b)
+    pairs = cos.shape[1]
+    at = torch.arange(q.shape[0]) if positions is None else positions.long()
+    inside = (at >= 0) & (at < cos.shape[0])
+    c, s = (t[at.clamp(0, max(0, cos.shape[0] - 1))][:, None] if cos.shape[0] else t.new_zeros(len(at), 1, pairs) for t in (cos, sin))
+
+    def turn(x):
+        part = x[..., :2 * pairs].float()
+        a, b = (part[..., 0::2], part[..., 1::2]) if layout == "interleaved" else (part[..., :pairs], part[..., pairs:])
+        a, b = a * c - b * s, a * s + b * c
+        part = torch.stack((a, b), dim=-1).flatten(-2) if layout == "interleaved" else torch.cat((a, b), dim=-1)
+        return torch.where(inside[:, None, None], torch.cat((part.to(x.dtype), x[..., 2 * pairs:]), dim=-1), 0)
+
+    return turn(q) if k is None else (turn(q), turn(k))
+
+
+def rotary_tables(positions: int, dim: int, *, theta: float = 10000.0, scaling: Optional[str] = None, factor: float = 1.0, original: Optional[int] = None,
+                  magnitude: float = 1.0, device="cuda") -> Tuple[torch.Tensor, torch.Tensor]:
+    """(cos, sin), fp32 ``[positions, dim / 2]``, of position times ``theta ** (-2 i / dim)``, from angles in 64 bits (far positions keep their angle).
+
+    scaling, for texts `factor` times longer than a model was trained on:
+      "linear"  all angles are divided by the factor
+      "base"    theta grows so that the slowest pair's angle is divided by the factor and the fastest stays
+      "bands"   pairs that turn 32 times or more within `original` positions stay, those that turn once or less are divided by the factor, those in between go
+                from one to the other evenly with the number of turns
+    magnitude: both tables times this."""
+    if positions < 0 or dim < 2 or dim % 2 or not theta > 0 or not factor > 0:
+        raise RuntimeError(f"rotary_tables: no tables of {positions} positions, {dim} elements, theta {theta} and factor {factor}")
+    step = torch.arange(0, dim, 2, dtype=torch.float64) / dim
+    if scaling == "base":
+        if dim < 4:
+            raise RuntimeError("rotary_tables: one pair has no slowest and fastest")
+        theta = theta * factor ** (dim / (dim - 2))
+    speed = theta ** -step
+    if scaling == "linear":
+        speed = speed / factor
+    elif scaling == "bands":
+        if original is None or original < 1:
+            raise RuntimeError("rotary_tables: scaling 'bands' needs the original number of positions")
+        share = ((original * speed / (2 * math.pi) - 1.0) / 31.0).clamp(0.0, 1.0)   # how much of the pair stays as it was
+        speed = speed * share + speed / factor * (1.0 - share)
+    elif scaling not in (None, "base"):
+        raise RuntimeError(f"rotary_tables: scalings are 'linear', 'base' and 'bands', not '{scaling}'")
+    angle = torch.outer(torch.arange(positions, dtype=torch.float64, device=device), speed.to(device))
+    return (angle.cos() * magnitude).float(), (angle.sin() * magnitude).float()
