@@ -29,12 +29,18 @@ using u64 = unsigned long long;
 constexpr int kThreads = 512, kWarps = kThreads / 32, kMost = 8;   // blocks per row at most
 constexpr int kBins = 2048, kList = 1024;
 constexpr int kOne = 43;             // a weight of one is 2^43: the sum of 2^20 of them stays below 2^63
-constexpr float kReach = 30.6f;      // exp(-30.6) 2^43 is below one half
+constexpr float kReach = 30.6f;      // exp(-30.6) 2^43 is below one half (44 powers of two are 30.5)
 constexpr double kLog2e = 1.4426950408889634;
 
 struct Histogram {
   unsigned count[kBins];
   u64 sum[kBins];
+};
+// A block's own: sums in three parts of 15 bits, whose 32-bit words hold those of 2^17 weights (one 64-bit addition in shared memory is a loop of exchanges).
+constexpr int kPart = 15, kBlockTokens = 1 << 17;
+struct Parts {
+  unsigned count[kBins];
+  unsigned sum[3][kBins];
 };
 // Where a border lies: the interval, what is in front of it, how many are in it.
 struct Border {
@@ -44,8 +50,8 @@ struct Border {
   int found;
 };
 struct Shared {
-  Histogram mine, merged;              // merged: in the first block, sums over the row; of the first level
-  Histogram deeper;                    // ... and of the others
+  Parts mine;
+  Histogram merged;                    // in the first block: over the whole row
   u64 list[kList];
   u64 weights[kList];
   u64 best[kMost];                     // per block: the likeliest (composite key)
@@ -57,9 +63,11 @@ struct Shared {
   unsigned scan_count[kWarps];
   u64 warp_sum[kWarps];
   Border border;
-  u64 result, result_sum;
+  u64 result;
+  int place;
   unsigned listed;
-  double power[64];                    // 2^(j / 64)
+  double enough;                       // in the first block: the sum of weights that top-p asks for
+  int power[64];                       // 2^(j / 64) 2^30
 };
 
 template <typename T>
@@ -71,34 +79,41 @@ __device__ __forceinline__ float value_of(__nv_bfloat16 x) { return __bfloat162f
 template <>
 __device__ __forceinline__ float value_of(__half x) { return __half2float(x); }
 
-// Ascending order of this number is descending order of values, then ascending of token numbers.  (-0 counts as +0.)
-__device__ __forceinline__ u64 composite(float x, int i) {
+// A number whose order is that of values.  (-0 counts as +0; below that of -inf and above that of +inf are NaNs.)
+__device__ __forceinline__ unsigned rising(float x) {
   unsigned b = __float_as_uint(x);
   if (b == 0x80000000u) b = 0;
-  const unsigned up = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-  return (static_cast<u64>(~up) << 32) | static_cast<unsigned>(i);
+  return b ^ (static_cast<unsigned>(static_cast<int>(b) >> 31) | 0x80000000u);
 }
+constexpr unsigned kPlusInfinity = 0xff800000u, kMinusInfinity = 0x007fffffu;
+// Ascending order of this number is descending order of values, then ascending of token numbers.
+__device__ __forceinline__ u64 composite(float x, int i) { return (static_cast<u64>(~rising(x)) << 32) | static_cast<unsigned>(i); }
 __device__ __forceinline__ float value_of_key(u64 c) {
   const unsigned up = ~static_cast<unsigned>(c >> 32);
   return __uint_as_float((up & 0x80000000u) ? (up & 0x7fffffffu) : ~up);
 }
 
-// Weights of a row.
+// Weights of a row, 2^(t / 64) 2^43 rounded for t = (x - max) 64 / (T ln 2), in 32-bit arithmetic (in fp64 a pass over 64 x 128000 logits took 82 us).
 struct Scale {
-  double max, per;   // 64 / (T ln 2)
-  const double* power;
-  // 2^(t / 64) 2^43 for t = (x - max) per, rounded: t = 64 n + j + f with |f| <= 1/2, 2^(f / 64) by its series up to the fourth power (the next term is 2^-47)
+  float max, per, per_low;    // the factor in two parts
+  const int* power;           // 2^(j / 64) 2^30, 64 of them
+  __device__ __forceinline__ bool some(float x) const { return __fmul_rn(__fsub_rn(x, max), per) > -64.f * 44.f; }
+  // x for which some() holds
   __device__ __forceinline__ u64 weight(float x) const {
-    const double t = (static_cast<double>(x) - max) * per;
-    if (!(t > -64.0 * 44.5)) return 0;
-    const double round = 6755399441055744.0;   // 1.5 2^52: the sum's last bit is worth one
-    const double r = t + round;
-    const int whole = __double2loint(r);
-    const double z = (t - (r - round)) * (0.6931471805599453 / 64.0);
-    const double q = z * (1.0 + z * (0.5 + z * (1.0 / 6.0 + z * (1.0 / 24.0))));
-    double p = power[whole & 63];
-    p = p + p * q;
-    return __double2ull_rn(__hiloint2double(__double2hiint(p) + (((whole >> 6) + kOne) << 20), __double2loint(p)));
+    // x - max and its product with the factor, each with what rounding leaves: t is off by less than 2^-25
+    const float d = __fsub_rn(x, max), back = __fsub_rn(d, x);
+    const float d_low = __fsub_rn(__fsub_rn(x, __fsub_rn(d, back)), __fadd_rn(max, back));
+    const float t = __fmul_rn(d, per);
+    const float t_low = fmaf(d_low, per, fmaf(d, per_low, fmaf(d, per, -t)));
+    // t = 64 n + j + f with |f| <= 1/2 and a little; 2^(f / 64) - 1 by its series up to the third power (the next term is below 2^-34)
+    const float r = __fadd_rn(t, 12582912.f);   // 1.5 2^23: the sum's last bit is worth one
+    const int whole = __float_as_int(r) - 0x4b400000;
+    const float z = __fadd_rn(__fsub_rn(t, __fsub_rn(r, 12582912.f)), t_low) * static_cast<float>(0.6931471805599453 / 64.0);
+    const float more = fmaf(z * fmaf(z, 1.f / 6.f, 0.5f), z, z);
+    const int p = power[whole & 63];
+    const unsigned w = static_cast<unsigned>(p + __mulhi(p, __float2int_rn(more * 4294967296.f)));
+    // w / 2^30 2^kOne 2^n, rounded
+    return ((static_cast<u64>(w) << (kOne - 30 + 1) >> -(whole >> 6)) + 1) >> 1;
   }
 };
 
@@ -113,56 +128,117 @@ __device__ __forceinline__ u64 warp_min(u64 v) {
   return v;
 }
 
-// A warp's part [lo, hi) of the row, in order: f(value, number, valid) by whole warps, V neighbouring tokens per lane and step.
+// A warp's part [lo, hi) of the row, in order: f(value, number, valid) by whole warps, V neighbouring tokens per lane and step.  Several steps' loads are under
+// way together (one at a time 17 us for the maximum of 64 x 128000).
 template <typename T, int V, typename F>
 __device__ __forceinline__ void walk(const T* row, int lo, int hi, F f) {
+  constexpr int kSteps = V == 1 ? 4 : 16 / V;
   const int lane = threadIdx.x & 31;
-  for (int base = lo; base < hi; base += 32 * V) {
-    const int i = base + lane * V;
+  for (int base = lo; base < hi; base += 32 * V * kSteps) {
+    const int i0 = base + lane * V;
     if constexpr (V == 1) {
-      f(i < hi ? value_of<T>(row[i]) : 0.f, i, i < hi);
-    } else {
-      uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-      T* x = reinterpret_cast<T*>(&raw);
-      if (i + V <= hi) {
-        raw = *reinterpret_cast<const uint4*>(row + i);
-      } else {
+      T x[kSteps];
 #pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (i + e < hi) x[e] = row[i + e];
+      for (int k = 0; k < kSteps; ++k)
+        if (i0 + 32 * k < hi) x[k] = row[i0 + 32 * k];
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) f(value_of<T>(x[k]), i0 + 32 * k, i0 + 32 * k < hi);
+    } else {
+      uint4 raw[kSteps];
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) {
+        const int i = i0 + 32 * V * k;
+        if (i + V <= hi) {
+          raw[k] = *reinterpret_cast<const uint4*>(row + i);
+        } else {
+          raw[k] = make_uint4(0u, 0u, 0u, 0u);
+          T* x = reinterpret_cast<T*>(&raw[k]);
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            if (i + e < hi) x[e] = row[i + e];
+        }
       }
 #pragma unroll
-      for (int e = 0; e < V; ++e) f(value_of<T>(x[e]), i + e, i + e < hi);
+      for (int k = 0; k < kSteps; ++k) {
+        const int i = i0 + 32 * V * k;
+        const T* x = reinterpret_cast<const T*>(&raw[k]);
+#pragma unroll
+        for (int e = 0; e < V; ++e) f(value_of<T>(x[e]), i + e, i + e < hi);
+      }
     }
   }
 }
 
-// Adds a warp's weights to bins: at once where all lanes have the same bin (rows of equal logits).  bin < 0: nothing.
-__device__ __forceinline__ void add(Histogram& h, int bin, u64 w) {
-  int same = 0;
-  __match_all_sync(0xffffffffu, bin, &same);
-  if (same) {
-    if (bin < 0) return;
-    const u64 sum = warp_sum(w);
-    if ((threadIdx.x & 31) == 0) {
-      atomicAdd(&h.count[bin], 32u);
-      atomicAdd(&h.sum[bin], sum);
+template <bool WEIGHTS>
+__device__ __forceinline__ void add(Parts& h, int bin, u64 w) {
+  atomicAdd(&h.count[bin], 1u);
+  if (WEIGHTS) {
+    atomicAdd(&h.sum[0][bin], static_cast<unsigned>(w) & ((1u << kPart) - 1));
+    atomicAdd(&h.sum[1][bin], static_cast<unsigned>(w >> kPart) & ((1u << kPart) - 1));
+    atomicAdd(&h.sum[2][bin], static_cast<unsigned>(w >> 2 * kPart));
+  }
+}
+__device__ __forceinline__ void clear(Parts& h) {
+  for (int b = threadIdx.x; b < kBins; b += kThreads) h.count[b] = h.sum[0][b] = h.sum[1][b] = h.sum[2][b] = 0;
+}
+
+// list[0 .. n) in ascending order, n a power of two from 32 on; by a block.
+__device__ __forceinline__ void sort(u64* list, int n) {
+  for (int k = 2; k <= n; k <<= 1) {   // bitonic
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      for (int i = threadIdx.x; i < n / 2; i += kThreads) {
+        const int a = 2 * i - (i & (j - 1)), o = a + j;
+        const u64 x = list[a], y = list[o];
+        if ((x > y) == ((a & k) == 0)) {
+          list[a] = y;
+          list[o] = x;
+        }
+      }
+      __syncthreads();
     }
-  } else if (bin >= 0) {
-    atomicAdd(&h.count[bin], 1u);
-    atomicAdd(&h.sum[bin], w);
   }
 }
-
-__device__ __forceinline__ void clear(Histogram& h) {
-  for (int b = threadIdx.x; b < kBins; b += kThreads) {
-    h.count[b] = 0;
-    h.sum[b] = 0;
-  }
+__device__ __forceinline__ int power_of_two(int n) {
+  int p = 32;
+  while (p < n) p <<= 1;
+  return p;
 }
 
-// The blocks' bins added up in the first block's `to`.  Ends with a barrier of the cluster.
-__device__ __forceinline__ void merge(cg::cluster_group& cluster, Shared& s, Histogram Shared::*to) {
+// The first i < n whose running sum of w[0 .. i] is `aim` or more (n without one); by a block, and the whole sum.
+__device__ __forceinline__ int first_at(Shared& s, const u64* w, int n, u64 aim, u64& whole) {
+  constexpr int kEach = kList / kThreads;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, base = static_cast<int>(threadIdx.x) * kEach;
+  u64 v[kEach], in = 0;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) in += v[e] = base + e < n ? w[base + e] : 0;
+  const u64 mine = in;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 x = __shfl_up_sync(0xffffffffu, in, o);
+    if (lane >= o) in += x;
+  }
+  if (lane == 31) s.scan[warp] = in;
+  if (threadIdx.x == 0) s.place = n;
+  __syncthreads();
+  u64 before = in - mine;
+  whole = 0;
+  for (int i = 0; i < kWarps; ++i) {
+    if (i < warp) before += s.scan[i];
+    whole += s.scan[i];
+  }
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    if (base + e < n && before < aim && before + v[e] >= aim) s.place = base + e;   // one thread's
+    before += v[e];
+  }
+  __syncthreads();
+  const int at = s.place;
+  __syncthreads();
+  return at;
+}
+
+// The blocks' bins added up in the first block's `merged`.  Begins and ends with a barrier of the cluster.
+__device__ __forceinline__ void merge(cg::cluster_group& cluster, Shared& s) {
   const int blocks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   cluster.sync();
   Shared* first = cluster.map_shared_rank(&s, 0);
@@ -173,64 +249,12 @@ __device__ __forceinline__ void merge(cg::cluster_group& cluster, Shared& s, His
     for (int r = 0; r < blocks; ++r) {
       const Shared* other = cluster.map_shared_rank(&s, r);
       count += other->mine.count[b];
-      sum += other->mine.sum[b];
+      sum += other->mine.sum[0][b] + (static_cast<u64>(other->mine.sum[1][b]) << kPart) + (static_cast<u64>(other->mine.sum[2][b]) << 2 * kPart);
     }
-    (first->*to).count[b] = count;
-    (first->*to).sum[b] = sum;
+    first->merged.count[b] = count;
+    first->merged.sum[b] = sum;
   }
   cluster.sync();
-}
-
-// First block only, all threads: the first bin at whose end `reached` is true of (tokens, weights) up to there; s.border has it, or found = 0.
-template <typename F>
-__device__ __forceinline__ void find_bin(Shared& s, const Histogram& h, int count0, u64 sum0, F reached) {
-  constexpr int kEach = kBins / kThreads;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  unsigned c[kEach], count = 0;
-  u64 w[kEach], sum = 0;
-#pragma unroll
-  for (int e = 0; e < kEach; ++e) {
-    c[e] = h.count[threadIdx.x * kEach + e];
-    w[e] = h.sum[threadIdx.x * kEach + e];
-    count += c[e];
-    sum += w[e];
-  }
-  unsigned in_count = count;
-  u64 in_sum = sum;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const unsigned a = __shfl_up_sync(0xffffffffu, in_count, o);
-    const u64 b = __shfl_up_sync(0xffffffffu, in_sum, o);
-    if (lane >= o) {
-      in_count += a;
-      in_sum += b;
-    }
-  }
-  if (lane == 31) {
-    s.scan_count[warp] = in_count;
-    s.scan[warp] = in_sum;
-  }
-  if (threadIdx.x == 0) s.border.found = 0;
-  __syncthreads();
-  unsigned before = static_cast<unsigned>(count0) + in_count - count;
-  u64 before_sum = sum0 + in_sum - sum;
-  for (int i = 0; i < warp; ++i) {
-    before += s.scan_count[i];
-    before_sum += s.scan[i];
-  }
-#pragma unroll
-  for (int e = 0; e < kEach; ++e) {
-    if (c[e] > 0 && !reached(before, before_sum) && reached(before + c[e], before_sum + w[e])) {   // one thread's at most: both grow
-      s.border.bin = threadIdx.x * kEach + e;
-      s.border.count = static_cast<int>(before);
-      s.border.sum = before_sum;
-      s.border.inside = static_cast<int>(c[e]);
-      s.border.found = 1;
-    }
-    before += c[e];
-    before_sum += w[e];
-  }
-  __syncthreads();
 }
 
 template <typename T, int V>
@@ -245,10 +269,114 @@ struct Row {
     return b < 0 ? 0 : (b < kBins ? b : kBins - 1);
   }
 
-  // The composite key of the border token and the sum of weights up to and with it, for all blocks.  Called with s.border of the first block (found) from
-  // the first level; `reached` as in find_bin.
-  template <typename F>
-  __device__ void resolve(cg::cluster_group& cluster, Shared& s, F reached, u64& key, u64& sum) const {
+  // First block only, all threads: the first bin at whose end `need` tokens (with WEIGHTS: share of all weights, or s.enough of them) have been passed, behind
+  // count0 tokens and weights of sum0; s.border has it, or found = 0.
+  template <bool WEIGHTS>
+  __device__ __forceinline__ static void find_bin(Shared& s, int count0, u64 sum0, unsigned need, float share) {
+    constexpr int kEach = kBins / kThreads;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    unsigned c[kEach], count = 0;
+    u64 w[kEach], sum = 0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      c[e] = s.merged.count[threadIdx.x * kEach + e];
+      w[e] = WEIGHTS ? s.merged.sum[threadIdx.x * kEach + e] : 0;
+      count += c[e];
+      sum += w[e];
+    }
+    unsigned in_count = count;
+    u64 in_sum = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned a = __shfl_up_sync(0xffffffffu, in_count, o);
+      const u64 b = WEIGHTS ? __shfl_up_sync(0xffffffffu, in_sum, o) : 0;
+      if (lane >= o) {
+        in_count += a;
+        in_sum += b;
+      }
+    }
+    if (lane == 31) {
+      s.scan_count[warp] = in_count;
+      s.scan[warp] = in_sum;
+    }
+    if (threadIdx.x == 0) s.border.found = 0;
+    __syncthreads();
+    if (WEIGHTS && share >= 0.f) {   // a token is kept while the weights in front of it are below the share of all: the border is where they are reached
+      u64 all = 0;
+      for (int i = 0; i < kWarps; ++i) all += s.scan[i];
+      if (threadIdx.x == 0) s.enough = static_cast<double>(share) * static_cast<double>(all);
+      __syncthreads();
+    }
+    unsigned before = static_cast<unsigned>(count0) + in_count - count;
+    u64 before_sum = sum0 + in_sum - sum;
+    for (int i = 0; i < warp; ++i) {
+      before += s.scan_count[i];
+      before_sum += s.scan[i];
+    }
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      if (c[e] > 0 && !reached<WEIGHTS>(s, before, before_sum, need) && reached<WEIGHTS>(s, before + c[e], before_sum + w[e], need)) {   // one thread's at most: both grow
+        s.border.bin = threadIdx.x * kEach + e;
+        s.border.count = static_cast<int>(before);
+        s.border.sum = before_sum;
+        s.border.inside = static_cast<int>(c[e]);
+        s.border.found = 1;
+      }
+      before += c[e];
+      before_sum += w[e];
+    }
+    __syncthreads();
+  }
+  template <bool WEIGHTS>
+  __device__ __forceinline__ static bool reached(const Shared& s, unsigned count, u64 sum, unsigned need) {
+    return WEIGHTS ? count > 0 && static_cast<double>(sum) >= s.enough : count >= need;
+  }
+
+  // The first block has all candidates in its list: the choice among them.  need: top-k (0: none); share: top-p of the sum of these (1: none, below 0: s.enough);
+  // weights below `least` do not count.
+  __device__ long long choose(Shared& s, int n, unsigned need, float share, u64 least, double u) const {
+    const int all = power_of_two(n);
+    for (int i = n + threadIdx.x; i < all; i += kThreads) s.list[i] = ~0ull;
+    __syncthreads();
+    sort(s.list, all);
+    int kept = need > 0 ? min(n, static_cast<int>(need)) : n;
+    for (int i = threadIdx.x; i < kept; i += kThreads) s.weights[i] = scale.weight(value_of_key(s.list[i]));
+    __syncthreads();
+    u64 whole;
+    if (share < 1.f) {
+      double enough = s.enough;
+      if (share >= 0.f) {
+        first_at(s, s.weights, kept, 0, whole);
+        enough = static_cast<double>(share) * static_cast<double>(whole);
+      }
+      // the first that reaches it stays, whatever it asks for
+      kept = min(kept, first_at(s, s.weights, kept, static_cast<u64>(max(1ll, static_cast<long long>(ceil(enough)))), whole) + 1);
+    }
+    // by number
+    for (int i = threadIdx.x; i < all; i += kThreads) s.list[i] = i < kept ? (s.list[i] << 32) | static_cast<unsigned>(i) : ~0ull;
+    __syncthreads();
+    sort(s.list, all);
+    u64 mine[kList / kThreads];
+#pragma unroll
+    for (int e = 0; e < kList / kThreads; ++e) {
+      const int i = static_cast<int>(threadIdx.x) + e * kThreads;
+      mine[e] = i < kept ? s.weights[s.list[i] & 0xffffffffu] : 0;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kList / kThreads; ++e) s.weights[threadIdx.x + e * kThreads] = mine[e] < least ? 0 : mine[e];
+    __syncthreads();
+    first_at(s, s.weights, kept, 0, whole);
+    const double at = u * static_cast<double>(whole);
+    const u64 aim = at > 0.0 ? min(static_cast<u64>(at), whole - 1) : 0;
+    return static_cast<long long>(s.list[first_at(s, s.weights, kept, aim + 1, whole)] >> 32);
+  }
+
+  // The composite key of the last token kept: the need-th (fewer tokens: none, ~0), or with WEIGHTS the one that reaches `share` of the weights, among those
+  // up to `limit`.  The same in all blocks.  `few` is called instead, in all blocks, where the first one can have all candidates up to it in its list; it has
+  // then been told how many there are.
+  template <bool WEIGHTS, typename F>
+  __device__ u64 find(cg::cluster_group& cluster, Shared& s, u64 limit, unsigned need, float share, bool& done, F few) const {
     const int blocks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     Shared* first = cluster.map_shared_rank(&s, 0);
@@ -257,14 +385,35 @@ struct Row {
       if (rank == 0 && threadIdx.x == 0) s.listed = 0;
       cluster.sync();
     };
+    const bool limited = limit != ~0ull;
+    clear(s.mine);
+    __syncthreads();
+    walk<T, V>(row, lo, hi, [&](float x, int i, bool valid) {
+      if (valid && scale.some(x) && (!limited || composite(x, i) <= limit)) add<WEIGHTS>(s.mine, bin(x), WEIGHTS ? scale.weight(x) : 0);
+    });
+    merge(cluster, s);
+    if (rank == 0) find_bin<WEIGHTS>(s, 0, 0, need, share);
     tell();
+    if (!s.border.found) return ~0ull;
     bool level = true;   // still the first
-    while (s.border.inside > kList) {
-      const Border b = s.border;
-      auto member = [&](float x, int i, u64& c) {
-        c = composite(x, i);
-        return level ? (bin(x) == b.bin && scale.weight(x) > 0) : (c >= b.lo && c <= b.hi);
-      };
+    Border b = s.border;
+    if (!limited && b.count + b.inside <= kList) {
+      walk<T, V>(row, lo, hi, [&](float x, int i, bool valid) {
+        if (valid && scale.some(x) && bin(x) <= b.bin) {
+          const unsigned at = atomicAdd(&first->listed, 1u);
+          if (at < kList) first->list[at] = composite(x, i);
+        }
+      });
+      cluster.sync();
+      if (rank == 0) few(b.count + b.inside);
+      done = true;
+      return 0;
+    }
+    auto member = [&](float x, int i, u64& c) {
+      c = composite(x, i);
+      return level ? scale.some(x) && bin(x) == b.bin && c <= limit : c >= b.lo && c <= b.hi;
+    };
+    while (b.inside > kList) {
       u64 low = ~0ull, high = 0;
       walk<T, V>(row, lo, hi, [&](float x, int i, bool valid) {
         u64 c;
@@ -292,91 +441,65 @@ struct Row {
         other->high[rank] = h;
       }
       cluster.sync();
-      for (int i = 0; i < blocks; ++i) {
-        low = min(i == 0 ? ~0ull : low, s.low[i]);
-        high = max(i == 0 ? 0ull : high, s.high[i]);
+      low = s.low[0];
+      high = s.high[0];
+      for (int i = 1; i < blocks; ++i) {
+        low = min(low, s.low[i]);
+        high = max(high, s.high[i]);
       }
       int shift = 0;
       while (((high - low) >> shift) >= kBins) ++shift;
       walk<T, V>(row, lo, hi, [&](float x, int i, bool valid) {
-        u64 c = 0;
-        const bool in = valid && member(x, i, c);
-        add(s.mine, in ? static_cast<int>((c - low) >> shift) : -1, in ? scale.weight(x) : 0);
+        u64 c;
+        if (valid && member(x, i, c)) add<WEIGHTS>(s.mine, static_cast<int>((c - low) >> shift), WEIGHTS ? scale.weight(x) : 0);
       });
-      merge(cluster, s, &Shared::deeper);
+      merge(cluster, s);
       if (rank == 0) {
-        find_bin(s, s.deeper, b.count, b.sum, reached);
+        find_bin<WEIGHTS>(s, b.count, b.sum, need, -1.f);
         if (threadIdx.x == 0) {
           s.border.lo = low + (static_cast<u64>(s.border.bin) << shift);
           s.border.hi = min(high, s.border.lo + ((1ull << shift) - 1));
         }
         __syncthreads();
       }
-      level = false;
       tell();
+      level = false;
+      b = s.border;
     }
-    const Border b = s.border;
     walk<T, V>(row, lo, hi, [&](float x, int i, bool valid) {
-      if (!valid) return;
-      const u64 c = composite(x, i);
-      if (level ? (bin(x) == b.bin && scale.weight(x) > 0) : (c >= b.lo && c <= b.hi)) {
+      u64 c;
+      if (valid && member(x, i, c)) {
         const unsigned at = atomicAdd(&first->listed, 1u);
         if (at < kList) first->list[at] = c;
       }
     });
     cluster.sync();
     if (rank == 0) {
-      int n = 32;
-      while (n < b.inside) n <<= 1;
+      const int n = power_of_two(b.inside);
       for (int i = b.inside + threadIdx.x; i < n; i += kThreads) s.list[i] = ~0ull;
       __syncthreads();
-      for (int k = 2; k <= n; k <<= 1) {   // bitonic
-        for (int j = k >> 1; j > 0; j >>= 1) {
-          for (int i = threadIdx.x; i < n / 2; i += kThreads) {
-            const int a = 2 * i - (i & (j - 1)), o = a + j;
-            const u64 x = s.list[a], y = s.list[o];
-            if ((x > y) == ((a & k) == 0)) {
-              s.list[a] = y;
-              s.list[o] = x;
-            }
-          }
-          __syncthreads();
-        }
-      }
-      for (int i = threadIdx.x; i < b.inside; i += kThreads) s.weights[i] = scale.weight(value_of_key(s.list[i]));
-      __syncthreads();
+      sort(s.list, n);
       if (threadIdx.x < 32) {
         u64 sum = b.sum;
         for (int base = 0; base < b.inside; base += 32) {
           const int i = base + lane;
-          u64 in = i < b.inside ? s.weights[i] : 0;
+          u64 in = WEIGHTS && i < b.inside ? scale.weight(value_of_key(s.list[i])) : 0;
 #pragma unroll
           for (int o = 1; o < 32; o <<= 1) {
             const u64 x = __shfl_up_sync(0xffffffffu, in, o);
             if (lane >= o) in += x;
           }
-          const unsigned there = __ballot_sync(0xffffffffu, i < b.inside && reached(static_cast<unsigned>(b.count + i + 1), sum + in));
+          const unsigned there = __ballot_sync(0xffffffffu, i < b.inside && reached<WEIGHTS>(s, static_cast<unsigned>(b.count + i + 1), sum + in, need));
           if (there) {
-            const int at = __ffs(there) - 1;
-            if (lane == at) {
-              s.result = s.list[i];
-              s.result_sum = sum + in;
-            }
+            if (lane < blocks) cluster.map_shared_rank(&s, lane)->result = s.list[base + __ffs(there) - 1];
             break;
           }
           sum += __shfl_sync(0xffffffffu, in, 31);
         }
       }
-      __syncthreads();
-      if (threadIdx.x > 0 && static_cast<int>(threadIdx.x) < blocks) {
-        Shared* other = cluster.map_shared_rank(&s, threadIdx.x);
-        other->result = s.result;
-        other->result_sum = s.result_sum;
-      }
     }
     cluster.sync();
-    key = s.result;
-    sum = s.result_sum;
+    return s.result;
   }
 };
 
@@ -384,13 +507,13 @@ template <typename T>
 __device__ __forceinline__ T setting(const RowSetting<T>& s, int row) { return s.each != nullptr ? s.each[row] : s.all; }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& s = *reinterpret_cast<Shared*>(smem);
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = static_cast<int>(gridDim.z), rank = static_cast<int>(blockIdx.z), line = static_cast<int>(blockIdx.x);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (threadIdx.x < 64) s.power[threadIdx.x] = exp2(static_cast<double>(threadIdx.x) / 64.0);
+  if (threadIdx.x < 64) s.power[threadIdx.x] = __double2int_rn(exp2(static_cast<double>(threadIdx.x) / 64.0) * 1073741824.0);
   cluster.sync();   // all blocks are there: their memory may be written
   pdl_wait();
   pdl_trigger();
@@ -401,14 +524,19 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
   r.hi = min(a.vocab, r.lo + part);
 
   // ---- the likeliest, and the range
-  u64 best = ~0ull;
-  bool strange = false;
+  unsigned top = 0, bottom = ~0u;
+  int top_at = 0;
   walk<T, V>(r.row, r.lo, r.hi, [&](float x, int i, bool valid) {
     if (!valid) return;
-    best = min(best, composite(x, i));
-    const unsigned b = __float_as_uint(x);
-    strange |= (b & 0x7fffffffu) > 0x7f800000u || b == 0x7f800000u;
+    const unsigned up = rising(x);
+    bottom = min(bottom, up);
+    if (up > top) {   // a lane's numbers ascend: the first of equals stays
+      top = up;
+      top_at = i;
+    }
   });
+  u64 best = (static_cast<u64>(~top) << 32) | static_cast<unsigned>(top_at);   // (a warp without tokens: a NaN's, behind all values)
+  bool strange = top >= kPlusInfinity || bottom < kMinusInfinity;
   best = warp_min(best);
   strange = __any_sync(0xffffffffu, strange);
   if (lane == 0) {
@@ -444,63 +572,39 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
     return;
   }
   r.most = most;
-  r.scale = {static_cast<double>(most), 64.0 * kLog2e / static_cast<double>(temperature), s.power};
+  const double per = 64.0 * kLog2e / static_cast<double>(temperature);
+  r.scale = {most, static_cast<float>(per), static_cast<float>(per - static_cast<double>(static_cast<float>(per))), s.power};
   r.steps = static_cast<float>(kBins) / (kReach * temperature);
 
   // ---- the border
   const int k = setting(a.top_k, line);
   const float top_p = setting(a.top_p, line);
+  const float min_p = setting(a.min_p, line);
+  const u64 least = min_p > 0.f ? static_cast<u64>(ceil(static_cast<double>(min(min_p, 1.f)) * static_cast<double>(1ull << kOne))) : 0;
+  const double u = a.uniform64 ? static_cast<const double*>(a.uniform)[line] : static_cast<double>(static_cast<const float*>(a.uniform)[line]);
   u64 border = ~0ull;
-  const bool some_k = k > 0 && k < a.vocab, some_p = top_p < 1.f;
-  if (some_k || some_p) {
-    clear(s.mine);
-    __syncthreads();
-    walk<T, V>(r.row, r.lo, r.hi, [&](float x, int i, bool valid) {
-      const u64 w = valid ? r.scale.weight(x) : 0;
-      add(s.mine, w > 0 ? r.bin(x) : -1, w);
+  bool done = false;
+  if (k > 0 && k < a.vocab) {
+    border = r.template find<false>(cluster, s, border, static_cast<unsigned>(k), 0.f, done, [&](int n) {
+      const long long token = r.choose(s, n, static_cast<unsigned>(k), top_p < 1.f ? fmaxf(top_p, 0.f) : 1.f, least, u);
+      if (threadIdx.x == 0) a.tokens[line] = token;
     });
-    merge(cluster, s, &Shared::merged);
-    u64 sum = 0;
-    bool limited = false;
-    if (some_k) {
-      auto reached = [&](unsigned count, u64) { return count >= static_cast<unsigned>(k); };
-      if (rank == 0) {
-        find_bin(s, s.merged, 0, 0, reached);
-        if (static_cast<int>(threadIdx.x) < blocks && threadIdx.x > 0) cluster.map_shared_rank(&s, threadIdx.x)->border.found = s.border.found;
-      }
-      cluster.sync();
-      limited = s.border.found != 0;   // otherwise fewer than k have a weight at all
-      if (limited) r.resolve(cluster, s, reached, border, sum);
-    }
-    if (some_p) {
-      if (!limited) {   // all weights
-        if (rank == 0) {
-          find_bin(s, s.merged, 0, 0, [](unsigned, u64) { return false; });
-          if (threadIdx.x == 0) {
-            u64 all = 0;
-            for (int i = 0; i < kWarps; ++i) all += s.scan[i];
-            s.result_sum = all;
-          }
-          __syncthreads();
-        }
-      }
-      // a token is kept while the weights in front of it are below top_p times the sum: the border is where they are reached
-      const double enough = static_cast<double>(top_p) * static_cast<double>(rank == 0 ? s.result_sum : 0);
-      auto reached = [&](unsigned count, u64 w) { return count > 0 && static_cast<double>(w) >= enough; };
-      if (rank == 0) find_bin(s, s.merged, 0, 0, reached);
-      u64 key, ignored;
-      r.resolve(cluster, s, reached, key, ignored);
-      border = min(border, key);
-    }
   }
+  if (top_p < 1.f && !done) {
+    const u64 limit = border;
+    border = min(limit, r.template find<true>(cluster, s, limit, 0, fmaxf(top_p, 0.f), done, [&](int n) {
+      const long long token = r.choose(s, n, 0, -1.f, least, u);
+      if (threadIdx.x == 0) a.tokens[line] = token;
+    }));
+  }
+  if (done) return;
 
   // ---- the choice
-  const float min_p = setting(a.min_p, line);
-  const double least = static_cast<double>(min(min_p, 1.f)) * static_cast<double>(1ull << kOne);
+  const bool limited = border != ~0ull;
   auto kept = [&](float x, int i) -> u64 {
-    if (composite(x, i) > border) return 0;
+    if (!r.scale.some(x) || (limited && composite(x, i) > border)) return 0;
     const u64 w = r.scale.weight(x);
-    return min_p > 0.f && static_cast<double>(w) < least ? 0 : w;
+    return w < least ? 0 : w;
   };
   u64 sum = 0;
   walk<T, V>(r.row, r.lo, r.hi, [&](float x, int i, bool valid) { sum += valid ? kept(x, i) : 0; });
@@ -518,33 +622,42 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs a)
     if (i < rank) before += s.total[i];
     total += s.total[i];
   }
-  const double u = a.uniform64 ? static_cast<const double*>(a.uniform)[line] : static_cast<double>(static_cast<const float*>(a.uniform)[line]);
   // the first token at whose end the running sum is above this
   const double at = u * static_cast<double>(total);
   const u64 aim = at > 0.0 ? min(static_cast<u64>(at), total - 1) : 0;
-  for (int i = 0; i < warp; ++i) before += s.warp_sum[i];
-  if (!(aim >= before && aim < before + s.warp_sum[warp])) return;   // whole warps
-  int token = -1;
-  for (int base = r.lo; base < r.hi && token < 0; base += 32) {
-    const int i = base + lane;
-    const u64 w = i < r.hi ? kept(value_of<T>(r.row[i]), i) : 0;
-    u64 in = w;
+  if (!(aim >= before && aim < before + s.total[rank])) return;   // whole blocks
+  // the warp whose part it falls into; all threads take a few neighbouring tokens of that part
+  int owner = 0;
+  while (aim >= before + s.warp_sum[owner]) before += s.warp_sum[owner++];
+  const int begin = min(a.vocab, (rank * kWarps + owner) * part), end = min(a.vocab, begin + part), each = (end - begin + kThreads - 1) / kThreads;
+  const int lo = min(end, begin + static_cast<int>(threadIdx.x) * each), hi = min(end, lo + each);
+  u64 mine = 0;
+  for (int i = lo; i < hi; ++i) mine += kept(value_of<T>(r.row[i]), i);
+  u64 in = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const u64 x = __shfl_up_sync(0xffffffffu, in, o);
-      if (lane >= o) in += x;
-    }
-    const unsigned there = __ballot_sync(0xffffffffu, before + in > aim);
-    if (there) token = base + __ffs(there) - 1;
-    before += __shfl_sync(0xffffffffu, in, 31);
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 x = __shfl_up_sync(0xffffffffu, in, o);
+    if (lane >= o) in += x;
   }
-  if (lane == 0) a.tokens[line] = token;
+  if (lane == 31) s.scan[warp] = in;
+  __syncthreads();
+  before += in - mine;
+  for (int i = 0; i < warp; ++i) before += s.scan[i];
+  if (aim >= before && aim < before + mine) {
+    int i = lo;
+    for (;; ++i) {
+      before += kept(value_of<T>(r.row[i]), i);
+      if (before > aim) break;
+    }
+    a.tokens[line] = i;
+  }
 }
 
 template <typename T, int V>
 cudaError_t launch(const SampleArgs& a, cudaStream_t stream) {
-  // blocks per row: as many as leave no SM idle, with some 2000 tokens each
+  // blocks per row: as many as leave no SM idle, with some 2000 tokens each and no more than a block may add up
   int blocks = 1;
+  while (a.vocab > blocks * kBlockTokens) blocks *= 2;
   while (blocks < kMost && static_cast<long long>(a.rows) * blocks * 2 <= 2 * 148 && a.vocab / blocks > 4096) blocks *= 2;
   static std::atomic<uint64_t> allowed{0};
   const cudaError_t rc = raise_smem_limit(sample_kernel<T, V>, sizeof(Shared), allowed);
