@@ -54,16 +54,20 @@ struct Attention {
   }
 };
 
-// (o, lse [heads, tokens] or undefined)
-std::pair<at::Tensor, at::Tensor> attention_forward(const Attention& x, bool lse) {
+// (o, lse [heads, tokens] or undefined, what rounding o left or undefined)
+std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_forward(const Attention& x, bool lse, bool rest) {
   const char* op = "packed_attention";
   ops::PackedAttentionArgs a = x.args(op);
   c10::cuda::CUDAGuard guard(x.q.device());
-  at::Tensor o = empty_on(x.q, {x.q.size(0), x.q.size(1), x.q.size(2)}, x.q.scalar_type()), l;
+  at::Tensor o = empty_on(x.q, {x.q.size(0), x.q.size(1), x.q.size(2)}, x.q.scalar_type()), l, r;
   a.o = o.data_ptr();
   if (lse) {
     l = empty_on(x.q, {x.q.size(1), x.q.size(0)}, at::kFloat);
     a.lse = l.data_ptr<float>();
+  }
+  if (rest) {
+    r = empty_on(x.q, o.sizes(), x.q.scalar_type());
+    a.o_rest = r.data_ptr();
   }
   if (a.k_tokens == 0 || a.sequences == 0) {   // nothing to see
     o.zero_();
@@ -71,14 +75,14 @@ std::pair<at::Tensor, at::Tensor> attention_forward(const Attention& x, bool lse
   } else {
     check_launch(ops::packed_attention(a, stream_of(x.q)), op);
   }
-  return {o, l};
+  return {o, l, r};
 }
 
 struct AttentionNode : torch::autograd::Function<AttentionNode> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& offsets, const at::Tensor& k_offsets, double scale,
                                int64_t window, int64_t sinks) {
-    const auto [o, lse] = attention_forward({q, k, v, offsets, k_offsets, scale, window, sinks}, true);
-    ctx->save_for_backward({q, k, v, offsets, k_offsets, o, lse});
+    const auto [o, lse, rest] = attention_forward({q, k, v, offsets, k_offsets, scale, window, sinks}, true, true);
+    ctx->save_for_backward({q, k, v, offsets, k_offsets, o, lse, rest});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["window"] = window;
     ctx->saved_data["sinks"] = sinks;
@@ -90,7 +94,7 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
     need_first_order(op);
     const auto s = ctx->get_saved_variables();
     const Attention x{s[0], s[1], s[2], s[3], s[4], ctx->saved_data["scale"].toDouble(), ctx->saved_data["window"].toInt(), ctx->saved_data["sinks"].toInt()};
-    const at::Tensor &o = s[5], &lse = s[6], d_o = rows_of_heads(grads[0]);
+    const at::Tensor &o = s[5], &lse = s[6], &rest = s[7], d_o = rows_of_heads(grads[0]);
     c10::cuda::CUDAGuard guard(x.q.device());
     at::Tensor dq = empty_on(x.q, x.q.sizes(), at::kBFloat16), dk = empty_on(x.q, x.k.sizes(), at::kBFloat16), dv = empty_on(x.q, x.v.sizes(), at::kBFloat16);
     if (x.k.size(0) == 0 || x.q.size(0) == 0 || x.offsets.numel() == 1) {
@@ -101,7 +105,8 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
       ops::PackedAttentionGradArgs a;
       a.f = x.args(op);
       a.f.lse = lse.data_ptr<float>();
-      a.o = tokens_of(o, op);
+      a.f.o = o.data_ptr();
+      a.f.o_rest = rest.data_ptr();
       a.d_o = tokens_of(d_o, "packed_attention(gradient)");
       a.dq = dq.data_ptr();
       a.dk = dk.data_ptr();
@@ -308,7 +313,7 @@ void bind_packed(py::module_& m) {
           o = r[0];
           lse = r[1];
         } else {
-          std::tie(o, lse) = attention_forward({q_, k_, v_, offsets, ko, scale, window, sinks}, return_lse);
+          std::tie(o, lse, std::ignore) = attention_forward({q_, k_, v_, offsets, ko, scale, window, sinks}, return_lse, false);
         }
         if (!return_lse) return {o, c10::nullopt};
         return {o, lse.t()};

@@ -21,6 +21,7 @@ struct PackedAttentionArgs {
   const int* k_offsets = nullptr;
   void* o = nullptr;
   float* lse = nullptr;
+  void* o_rest = nullptr;   // [tokens, heads, head_dim], may be null: what rounding o to 16 bits left, rounded to 16 bits (zero in rows of no sequence or not written)
   int tokens = 0, k_tokens = 0, sequences = 0;
   int heads = 0, kv_heads = 0, head_dim = 0;
   float scale = 1.f;
@@ -29,11 +30,11 @@ struct PackedAttentionArgs {
 };
 cudaError_t packed_attention(const PackedAttentionArgs& a, cudaStream_t stream);
 
-// ---- its gradients, bf16.  o and lse are what the forward call left (f.o is not written), d_o [tokens, heads, head_dim]; dq, dk and dv are contiguous and
+// ---- its gradients, bf16.  f.o, f.o_rest and f.lse are what the forward call left, d_o [tokens, heads, head_dim]; dq, dk and dv are contiguous and
 // zero in rows of no sequence.  delta: [heads, tokens] fp32 of room.  Every sum is taken in an order that depends on the sizes only.
 struct PackedAttentionGradArgs {
   PackedAttentionArgs f;
-  TokenView o, d_o;
+  TokenView d_o;
   void* dq = nullptr;
   void* dk = nullptr;
   void* dv = nullptr;

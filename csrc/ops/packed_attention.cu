@@ -29,6 +29,7 @@ constexpr int kStage = 8 * 2048;           // results on their way out, 32 rows 
 struct Forward {
   Problem p;
   void* o;
+  void* o_rest;      // may be null
   float* lse;
   TokenView v;       // for values that are not finite
   int pair_heads;    // a block's tiles are two heads, otherwise two times 128 rows
@@ -391,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (a.lse != nullptr && mine)
         a.lse[static_cast<long long>(u.head[t]) * p.tokens + u.s.q0 + u.row[t] + row] = none ? -INFINITY : (m * p.scale_log2 + log2f(l) - Weights<H>::kBias) / kLog2e;
       uint8_t* stage = s_out + warp * 2048;
-      typename H::T* o_base = static_cast<typename H::T*>(a.o) + (static_cast<long long>(u.s.q0 + u.row[t] + (warp & 3) * 32) * p.heads + u.head[t]) * p.head_dim;
+      const long long o_at = (static_cast<long long>(u.s.q0 + u.row[t] + (warp & 3) * 32) * p.heads + u.head[t]) * p.head_dim;
       const bool odd = *odd_values != 0;
       for (int c0 = 0; c0 < p.head_dim; c0 += 32) {
         uint32_t o[32] = {};
@@ -415,7 +416,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        rows_out<H>(stage, f, o_base, static_cast<long long>(p.heads) * p.head_dim, u.s.n - u.row[t] - (warp & 3) * 32, c0, p.head_dim);
+        const long long stride = static_cast<long long>(p.heads) * p.head_dim;
+        const int rows = u.s.n - u.row[t] - (warp & 3) * 32;
+        rows_out<H>(stage, f, static_cast<typename H::T*>(a.o) + o_at, stride, rows, c0, p.head_dim);
+        if (a.o_rest != nullptr) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) f[e] -= H::up(H::down(f[e]));
+          rows_out<H>(stage, f, static_cast<typename H::T*>(a.o_rest) + o_at, stride, rows, c0, p.head_dim);
+        }
       }
     }
     tc::fence_before_sync();
@@ -434,6 +442,7 @@ cudaError_t launch(const PackedAttentionArgs& args, cudaStream_t stream) {
   Forward f;
   f.p = problem_of(args);
   f.o = args.o;
+  f.o_rest = args.o_rest;
   f.lse = args.lse;
   f.v = args.v;
   f.pair_heads = f.p.group % 2 == 0 ? 1 : 0;

@@ -49,8 +49,9 @@ __device__ __forceinline__ void zero_rows(uint8_t* tile, int row) {
 }
 
 // ----------------------------------------------------------------------------------------------------- delta ----
-// delta[h, t] = sum_d dO[t, h, d] O[t, h, d]: a warp per 32 rows of a head, a half-warp per row at a time.
-__global__ void __launch_bounds__(256) packed_delta_kernel(TokenView o, TokenView d_o, float* delta, int tokens, int heads, int head_dim) {
+// delta[h, t] = sum_d dO[t, h, d] O[t, h, d], with O as it was before it was rounded (its rounding would be the same for all of a row's scores: dQ and dK were off
+// by 1.5 to 1.6 times what their own rounding leaves, now by 1.4).  A warp per 32 rows of a head, a half-warp per row at a time.
+__global__ void __launch_bounds__(256) packed_delta_kernel(const H::T* o, const H::T* o_rest, TokenView d_o, float* delta, int tokens, int heads, int head_dim) {
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = lane >> 4, c = (lane & 15) * 8;
@@ -62,11 +63,13 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(TokenView o, TokenVie
     const int t = t0 + 2 * i + half;
     float sum = 0.f;
     if (t < tokens && c < head_dim) {
-      float x[8], y[8];
-      unpack8_as<H>(__ldg(reinterpret_cast<const uint4*>(static_cast<const H::T*>(o.p) + t * o.token + h * o.head + c)), x);
+      const long long at = (static_cast<long long>(t) * heads + h) * head_dim + c;
+      float x[8], rest[8], y[8];
+      unpack8_as<H>(__ldg(reinterpret_cast<const uint4*>(o + at)), x);
+      unpack8_as<H>(__ldg(reinterpret_cast<const uint4*>(o_rest + at)), rest);
       unpack8_as<H>(__ldg(reinterpret_cast<const uint4*>(static_cast<const H::T*>(d_o.p) + t * d_o.token + h * d_o.head + c)), y);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum = fmaf(x[e], y[e], sum);
+      for (int e = 0; e < 8; ++e) sum = fmaf(x[e] + rest[e], y[e], sum);
     }
 #pragma unroll
     for (int s = 8; s >= 1; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
@@ -701,7 +704,8 @@ cudaError_t launch(const PackedAttentionGradArgs& args, cudaStream_t stream) {
   cudaError_t rc = raise_smem_limit(packed_grad_keys_kernel<DP>, key_smem<DP>(), allowed_keys);
   if (rc == cudaSuccess) rc = raise_smem_limit(packed_grad_queries_kernel<DP>, query_smem<DP>(), allowed_queries);
   if (rc != cudaSuccess) return rc;
-  MCCL_LAUNCH_PDL(packed_delta_kernel, dim3((f.tokens + 31) / 32, (f.heads + 7) / 8), 256, 0, stream, args.o, args.d_o, args.delta, f.tokens, f.heads, f.head_dim);
+  MCCL_LAUNCH_PDL(packed_delta_kernel, dim3((f.tokens + 31) / 32, (f.heads + 7) / 8), 256, 0, stream, static_cast<const H::T*>(f.o), static_cast<const H::T*>(f.o_rest),
+                  args.d_o, args.delta, f.tokens, f.heads, f.head_dim);
   g.units = static_cast<int>(keys);
   MCCL_LAUNCH_PDL(packed_grad_keys_kernel<DP>, g.units, kThreads, key_smem<DP>(), stream, q, k, v, d_o, g);
   g.units = static_cast<int>(queries);
