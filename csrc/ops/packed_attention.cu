@@ -20,10 +20,11 @@ namespace {
 
 using namespace packed;
 
-constexpr int kStages = 4;                 // tiles of keys and values under way
-constexpr int kThreads = 12 * 32;          // warps 0-3 and 4-7: rows of tiles 0 and 1; 8: products; 9: loads; 10: blocks seen in part; 11: nothing
+constexpr int kStages = 2;                 // pairs of tiles under way: values of a block and keys of the next one, which are used together
+constexpr int kThreads = 12 * 32;          // warps 0-3 and 4-7: rows of tiles 0 and 1; 8: products; 9: loads; 10: blocks seen in part; 11: what comes next
 // A row's scores need more registers than an even share: 256 x 208 + 128 x 80 of the launch's 384 x 168.
 constexpr int kRowRegisters = 208, kOtherRegisters = 80;
+constexpr int kRoles = 8 + 3;              // warps that take a unit from the planning one
 constexpr int kStage = 8 * 2048;           // results on their way out, 32 rows x 64 bytes per warp
 
 struct Forward {
@@ -38,7 +39,7 @@ struct Forward {
 };
 
 template <int DP>
-constexpr int smem_bytes() { return (2 + kStages) * (DP / 64) * kSub + kStage + 512 + 1024; }
+constexpr int smem_bytes() { return (2 + 2 * kStages) * (DP / 64) * kSub + kStage + 512 + 1024; }
 
 // Weights are kept 2^kBias times larger in fp16, whose smallest normal number is 2^-14; the running maximum may be exceeded by 2^kSlack before sums are
 // rescaled (exact in fp32 either way), so that the largest weight is 2^8 in bf16 and 2^15 in fp16.
@@ -57,11 +58,11 @@ struct Unit {
   int row[2], head[2];       // first row within the sequence; row >= s.n: nothing
   int first[2], last[2];     // positions of the tile's rows
   Blocks b[2], all;
-  bool any;
-  // Whether all rows of the unit that have block b see all of its keys.
-  __device__ __forceinline__ bool whole(const Problem& p, int block) const {
-    return (!b[0].has(block) || all_seen(p, block, first[0], last[0])) && (!b[1].has(block) || all_seen(p, block, first[1], last[1]));
-  }
+  int seen_from, seen_below, seen_first;
+  bool any, end;
+  int odd;                   // values that are not finite were met
+  // Whether all rows of the unit see all keys of a block.
+  __device__ __forceinline__ bool whole(int block) const { return block < seen_below && (block >= seen_from || block < seen_first); }
 };
 __device__ __forceinline__ Unit unit_of(const Forward& a, int u) {
   const Problem& p = a.p;
@@ -69,7 +70,8 @@ __device__ __forceinline__ Unit unit_of(const Forward& a, int u) {
   const int slots = a.units / a.head_units;
   const int in = u % a.head_units, slot = slots - 1 - u / a.head_units;   // long rows first
   Unit r;
-  r.any = false;
+  r.any = r.end = false;
+  r.odd = 0;
   const int s = find_sequence(p.offsets, p.sequences, p.tokens, slot, rows);
   if (s < 0) return r;
   r.s = sequence_of(p, s);
@@ -93,6 +95,11 @@ __device__ __forceinline__ Unit unit_of(const Forward& a, int u) {
   r.all.lo = r.b[1].hi == 0 ? r.b[0].lo : (r.b[0].hi == 0 ? r.b[1].lo : min(r.b[0].lo, r.b[1].lo));
   r.all.sink = max(r.b[0].sink, r.b[1].sink);
   if (r.all.sink >= r.all.lo) r.all.sink = r.all.lo = 0;   // one run
+  const bool both = r.b[1].hi > 0, only = r.b[0].hi == 0;   // tiles that have blocks: the last one always does if any
+  const int from = only ? r.first[1] : r.first[0], to = both ? r.last[1] : r.last[0];
+  r.seen_below = from < 0 ? 0 : (from + 1) / kRows;                                      // keys up to the first position
+  r.seen_from = to < p.window ? 0 : (to - p.window) / kRows + 1;                         // keys within the last position's window
+  r.seen_first = min(p.sinks, 1 << 30) / kRows;
   return r;
 }
 
@@ -103,20 +110,25 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* s_q = smem;                        // [2] tiles
-  uint8_t* s_kv = s_q + 2 * kTile;            // [kStages] tiles
-  uint8_t* s_out = s_kv + kStages * kTile;
+  uint8_t* s_kv = s_q + 2 * kTile;            // [kStages][2] tiles: values, keys
+  uint8_t* s_out = s_kv + 2 * kStages * kTile;
   uint64_t* q_full = reinterpret_cast<uint64_t*>(s_out + kStage);   // [2]
   uint64_t* kv_full = q_full + 2;             // [kStages]
   uint64_t* kv_empty = kv_full + kStages;     // [kStages]
   uint64_t* raw_full = kv_empty + kStages;    // [kStages]: values that are looked at before they are used are here, ...
   uint64_t* looked = raw_full + kStages;      // [kStages]: ... and have been
   uint64_t* s_full = looked + kStages;        // [2]
-  uint64_t* p_full = s_full + 2;              // [2]
-  uint64_t* o_full = p_full + 2;              // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
+  uint64_t* p_full = s_full + 2;              // [2][2]: tile, half of a block's keys
+  uint64_t* o_full = p_full + 4;              // [2]
+  uint64_t* q_empty = o_full + 2;
+  uint64_t* unit_full = q_empty + 1;          // [2]
+  uint64_t* unit_empty = unit_full + 2;       // [2]
+  uint64_t* next_full = unit_empty + 2;
+  uint64_t* loads_done = next_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(loads_done + 1);
   volatile int* bad = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* odd_values = bad + 1;
-  Unit* s_unit = reinterpret_cast<Unit*>(tmem_slot + 4);
+  uint4* s_next = reinterpret_cast<uint4*>((reinterpret_cast<uintptr_t>(tmem_slot + 2) + 15) & ~static_cast<uintptr_t>(15));
+  Unit* s_unit = reinterpret_cast<Unit*>(s_next + 1);   // [2]
 
   const Problem& p = a.p;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -124,7 +136,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int t = 0; t < 2; ++t) {
       tc::mbar_init(&q_full[t], 1);
       tc::mbar_init(&s_full[t], 1);
-      tc::mbar_init(&p_full[t], 128);
+      for (int h = 0; h < 2; ++h) tc::mbar_init(&p_full[2 * t + h], 4);
       tc::mbar_init(&o_full[t], 1);
     }
     for (int i = 0; i < kStages; ++i) {
@@ -133,77 +145,163 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::mbar_init(&raw_full[i], 1);
       tc::mbar_init(&looked[i], 1);
     }
+    tc::mbar_init(q_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&unit_full[i], 1);
+      tc::mbar_init(&unit_empty[i], kRoles);
+    }
+    tc::mbar_init(next_full, 1);
+    tc::mbar_init(loads_done, 1);
     *bad = 0;
-    *odd_values = 0;
     tc::mbar_init_fence();
   }
   if (warp == 8) tc::tmem_alloc(tmem_slot, 512);
   pdl_wait();
-  if (warp == 0) {
-    const Unit found = unit_of(a, static_cast<int>(blockIdx.x));
-    if (lane == 0) *s_unit = found;
-  }
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = *tmem_slot;
-  const Unit& u = *s_unit;
   pdl_trigger();
   // tensor memory: S of tile t in columns 128 t .. 128 t + 127 (P in the first 64 of them), O in 256 + DP t ..
-  const int kv = u.any ? u.head[0] / p.group : 0;
+  // Each role takes the units as they come; what they share in stages and phases goes on from one to the next, so that the loads and first products of a unit
+  // are under way while the results of the one before are on their way out.
+  auto take = [&](int k) {   // unit k of this block is described
+    const bool ok = wait(&unit_full[k & 1], (k >> 1) & 1, bad);
+    return __all_sync(0xffffffffu, ok) && !s_unit[k & 1].end;
+  };
+  auto give_back = [&](int k) {
+    __syncwarp();
+    if (lane == 0) tc::mbar_arrive(&unit_empty[k & 1]);
+  };
 
-  if (u.any && warp >= 8) {
+  if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
-  if (warp == 9) {
-    // ------------------------------------------------------------------------------------------- loads ----
-    if (tc::elect_one()) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-        if (u.b[t].hi > 0) {
-          tc::mbar_expect_tx(&q_full[t], kTile);
-          load_tile<DP>(s_q + t * kTile, &tm_q, &q_full[t], u.head[t], u.s.q0 + u.row[t]);
+  if (warp == 11) {
+    // ----------------------------------------------------------------------------------- what comes next ----
+    // A block that is done with its unit takes the next one of the grid that no block has begun (the launch's order: long ones first).
+    int id = static_cast<int>(blockIdx.x), asked = 0;
+    bool more = true;
+    for (int k = 0; more;) {
+      const Unit found = unit_of(a, id);
+      zero_outside<typename H::T>(a.o, p.heads * p.head_dim, a.lse, p.heads, p.offsets, p.sequences, p.tokens, id, a.units, lane, 32);
+      if (found.any) {
+        const bool ok = k < 2 || wait(&unit_empty[k & 1], ((k >> 1) - 1) & 1, bad);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        if (lane == 0) {
+          s_unit[k & 1] = found;
+          tc::mbar_arrive(&unit_full[k & 1]);
         }
-      int n = 0;   // tiles so far
-      uint32_t raw = 0, uses = 0, raw_uses = 0;   // a bit per stage: which barrier its last load is on, phases of both kinds
-      bool ok = true;
-      for (int b = u.all.next(-1); ok && b < u.all.hi; b = u.all.next(b)) {
-        const bool look = !u.whole(p, b);
-        for (int v = 0; v < 2 && ok; ++v) {
-          const int st = n % kStages;
-          if (n >= kStages) ok = wait(&kv_empty[st], (n / kStages - 1) & 1, bad);
-          if (!ok) break;
-          const bool r = look && v == 1;
-          uint64_t* full = r ? &raw_full[st] : &kv_full[st];
-          (r ? raw_uses : uses) ^= 1u << st;
-          raw = (raw & ~(1u << st)) | (r ? 1u << st : 0u);
-          tc::mbar_expect_tx(full, kTile);
-          load_tile<DP>(s_kv + st * kTile, v == 0 ? &tm_k : &tm_v, full, kv, u.s.k0 + b * kRows);
-          ++n;
-        }
+        __syncwarp();
+        ++k;
+        // asked for no earlier than the unit's last loads are under way: another block may be free sooner
+        const bool near = wait(loads_done, (k - 1) & 1, bad);
+        if (!__all_sync(0xffffffffu, near)) break;
       }
-      if (!ok) {   // loads that were issued must land before the block retires
-        for (int t = 0; t < 2; ++t)
-          if (u.b[t].hi > 0) tc::mbar_wait(&q_full[t], 0, 1u << 18);
-        for (int st = 0; st < min(n, kStages); ++st) {
-          const bool r = (raw >> st) & 1;
-          tc::mbar_wait(r ? &raw_full[st] : &kv_full[st], (((r ? raw_uses : uses) >> st) & 1) ^ 1, 1u << 18);
+      if (lane == 0) {
+        fence_async_smem();
+        tc::mbar_expect_tx(next_full, 16);
+        asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(tc::smem_u32(s_next)), "r"(tc::smem_u32(next_full))
+                     : "memory");
+      }
+      __syncwarp();
+      bool ok = wait(next_full, asked & 1, bad);
+      if (!__all_sync(0xffffffffu, ok)) {
+        tc::mbar_wait(next_full, asked & 1, 1u << 16);   // the answer must land before the block retires
+        break;
+      }
+      ++asked;
+      uint32_t got, x;
+      asm volatile(
+          "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"
+          "ld.shared.b128 h, [%2];\n\t"
+          "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+          "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
+          : "=r"(got), "=r"(x)
+          : "r"(tc::smem_u32(s_next))
+          : "memory");
+      __syncwarp();
+      more = got != 0;
+      id = static_cast<int>(x);
+      if (!more) {
+        const bool free = k < 2 || wait(&unit_empty[k & 1], ((k >> 1) - 1) & 1, bad);
+        if (!__all_sync(0xffffffffu, free)) break;
+        if (lane == 0) {
+          s_unit[k & 1].end = true;
+          tc::mbar_arrive(&unit_full[k & 1]);
         }
+        __syncwarp();
       }
     }
-    __syncwarp();
+  } else if (warp == 9) {
+    // ------------------------------------------------------------------------------------------- loads ----
+    uint32_t raw_uses = 0, q_uses = 0;   // a bit per stage, a bit per tile
+    int i = 0, units = 0;                // steps, and units with keys, so far
+    bool ok = true;
+    for (int k = 0; ok && take(k); ++k) {
+      const Unit& u = s_unit[k & 1];
+      if (tc::elect_one()) {
+        const int kv = u.head[0] / p.group;
+        if (u.all.hi > 0) {
+          if (units > 0) ok = wait(q_empty, (units - 1) & 1, bad);
+          ++units;
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (ok && u.b[t].hi > 0) {
+            tc::mbar_expect_tx(&q_full[t], kTile);
+            load_tile<DP>(s_q + t * kTile, &tm_q, &q_full[t], u.head[t], u.s.q0 + u.row[t]);
+            q_uses ^= 1u << t;
+          }
+        // a step brings the values of the block before and the keys of the next one
+        for (int before = -1, b = u.all.next(-1); ok && (b < u.all.hi || before >= 0); ++i) {
+          const int st = i % kStages;
+          const bool more = b < u.all.hi, look = before >= 0 && !u.whole(before);
+          if (i >= kStages) ok = wait(&kv_empty[st], (i / kStages - 1) & 1, bad);
+          if (!ok) break;
+          tc::mbar_expect_tx(&kv_full[st], (more ? kTile : 0) + (before >= 0 && !look ? kTile : 0));
+          if (before >= 0) {
+            if (look) {
+              tc::mbar_expect_tx(&raw_full[st], kTile);
+              raw_uses ^= 1u << st;
+            }
+            load_tile<DP>(s_kv + 2 * st * kTile, &tm_v, look ? &raw_full[st] : &kv_full[st], kv, u.s.k0 + before * kRows);
+          }
+          if (more) load_tile<DP>(s_kv + (2 * st + 1) * kTile, &tm_k, &kv_full[st], kv, u.s.k0 + b * kRows);
+          before = more ? b : -1;
+          if (more) b = u.all.next(b);
+        }
+        if (!ok) {   // loads that were issued must land before the block retires
+          for (int t = 0; t < 2; ++t) tc::mbar_wait(&q_full[t], ((q_uses >> t) & 1) ^ 1, 1u << 16);
+          for (int j = max(0, i - kStages); j < i; ++j) {
+            const int st = j % kStages;
+            tc::mbar_wait(&kv_full[st], (j / kStages) & 1, 1u << 16);
+            tc::mbar_wait(&raw_full[st], ((raw_uses >> st) & 1) ^ 1, 1u << 16);
+          }
+        }
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      if (lane == 0) tc::mbar_arrive(loads_done);
+      give_back(k);
+    }
   } else if (warp == 10) {
     // --------------------------------------------------------- blocks of keys that not every row sees ----
     // A weight of zero times a value that is not finite would be NaN in rows that do not see the value: such values become zeros, and rows that do see
     // them are put right at the end.  Rows behind the sequence are another sequence's.
-    int n = 1;
+    int steps = 0;
     uint32_t phase = 0;   // a bit per stage
-    for (int b = u.all.next(-1); b < u.all.hi; b = u.all.next(b), n += 2) {
-      if (u.whole(p, b)) continue;
-      const int st = n % kStages, rows = min(kRows, u.s.m - b * kRows);
-      const bool ok = wait(&raw_full[st], (phase >> st) & 1, bad);
-      if (!__all_sync(0xffffffffu, ok)) break;
+    bool ok = true;
+    for (int k = 0; ok && take(k); ++k) {
+    const Unit& u = s_unit[k & 1];
+    int i = steps + 1;
+    for (int b = u.all.next(-1); b < u.all.hi; b = u.all.next(b), ++i) {
+      if (u.whole(b)) continue;
+      const int st = i % kStages, rows = min(kRows, u.s.m - b * kRows);
+      ok = wait(&raw_full[st], (phase >> st) & 1, bad);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
       phase ^= 1u << st;
-      uint8_t* tile = s_kv + st * kTile;
+      uint8_t* tile = s_kv + 2 * st * kTile;
       using T2 = typename H::T2;
       const T2 zero = H::down(0.f, 0.f);
       T2 sum = zero;   // products with zero add up to zero, or to NaN
@@ -232,90 +330,97 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int k = 0; k < 8; ++k) e[k] = (e[k] & kExponent) == kExponent ? static_cast<uint16_t>(0) : e[k];
           *at = x;
         }
-        if (lane == 0) *odd_values = 1;
+        if (lane == 0) *reinterpret_cast<volatile int*>(&s_unit[k & 1].odd) = 1;
       }
       fence_async_smem();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&looked[st]);
     }
+    if (u.all.hi > 0) steps = i;   // a step more than blocks
+    give_back(k);
+    }
   } else if (warp == 8) {
     // ---------------------------------------------------------------------------------------- products ----
+    // One thread.  What it does between the last product of one tile and the first of the other has some 500 clocks, the time of those under way; a barrier's
+    // state takes 250 while the products read shared memory.  Hence one barrier for values and keys of a step, and nothing else on the way.
     constexpr uint32_t idesc_s = idesc16<H>(kRows, kRows, false, false);
     const uint32_t idesc_o = idesc16<H>(kRows, (p.head_dim + 15) / 16 * 16, false, true);
     const int steps = (p.head_dim + 15) / 16;
-    int n = 0, before = -1;
-    bool begun[2] = {false, false}, have_q[2] = {false, false};
-    uint32_t p_phase[2] = {0, 0}, full_phase = 0, looked_phase = 0;   // the last two: a bit per stage
+    uint32_t q_phase = 0, p_phase = 0, looked_phase = 0;   // a bit per tile; the last: per stage
+    int i = 0;                                             // steps so far
     bool ok = true;
-    auto all_wait = [&](uint64_t* bar, uint32_t parity) {
-      const bool w = ok && wait(bar, parity, bad);
-      ok = __all_sync(0xffffffffu, w);
-      return ok;
-    };
-    int b = u.all.next(-1);
-    while (ok && (b < u.all.hi || before >= 0)) {
-      const bool more = b < u.all.hi;
-      const int sk = n % kStages, sv = (n - 1 + kStages) % kStages;   // keys of b, values of `before`
-      if (more) {
-        if (!all_wait(&kv_full[sk], (full_phase >> sk) & 1)) break;
-        full_phase ^= 1u << sk;
-      }
-      if (before >= 0) {
-        const bool look = !u.whole(p, before);
-        if (!all_wait(look ? &looked[sv] : &kv_full[sv], ((look ? looked_phase : full_phase) >> sv) & 1)) break;
-        (look ? looked_phase : full_phase) ^= 1u << sv;
-      }
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if (ok && before >= 0 && u.b[t].has(before) && all_wait(&p_full[t], p_phase[t])) {
-          p_phase[t] ^= 1;
-          tc::fence_after_sync();
-          if (tc::elect_one()) {
-            mma_weights(tmem + 256 + t * DP, tmem + t * 128, s_kv + sv * kTile, idesc_o, begun[t]);
-            tc::mma_commit(&o_full[t]);
-          }
-          __syncwarp();
-          begun[t] = true;
-        }
-        if (ok && more && u.b[t].has(b) && (have_q[t] || all_wait(&q_full[t], 0))) {
-          have_q[t] = true;
-          tc::fence_after_sync();
-          if (tc::elect_one()) {
-            mma_rows(tmem + t * 128, s_q + t * kTile, s_kv + sk * kTile, idesc_s, steps);
-            tc::mma_commit(&s_full[t]);
-          }
-          __syncwarp();
-        }
-      }
+    for (int k = 0; ok && take(k); ++k) {
+      const Unit m = s_unit[k & 1];
       if (tc::elect_one()) {
-        if (before >= 0) tc::mma_commit(&kv_empty[sv]);
-        if (more) tc::mma_commit(&kv_empty[sk]);
+        uint32_t begun = 0;
+        bool look = false;
+        for (int before = -1, b = m.all.next(-1); b < m.all.hi || before >= 0; ++i) {
+          const int st = i % kStages;
+          const bool more = b < m.all.hi;
+          ok = wait(&kv_full[st], (i / kStages) & 1, bad);
+          if (look) {
+            ok = ok && wait(&looked[st], (looked_phase >> st) & 1, bad);
+            looked_phase ^= 1u << st;
+          }
+          if (!ok) break;
+#pragma unroll 1
+          for (int t = 0; t < 2; ++t) {
+            const Blocks mine = t == 0 ? m.b[0] : m.b[1];
+            const uint32_t t_s = tmem + t * 128;
+            if (before >= 0 && mine.has(before)) {
+#pragma unroll 1
+              for (int h = 0; h < 2; ++h) {   // the first half of the weights is multiplied while the second is made
+                ok = ok && wait(&p_full[2 * t + h], (p_phase >> t) & 1, bad);
+                if (!ok) break;
+                tc::fence_after_sync();
+                mma_weights<64>(tmem + 256 + t * DP, t_s + 32 * h, s_kv + 2 * st * kTile + h * 64 * 128, idesc_o, h != 0 || ((begun >> t) & 1));
+              }
+              p_phase ^= 1u << t;
+              begun |= 1u << t;
+            } else if (more && mine.has(b) && ((begun >> t) & 1) == 0) {
+              ok = ok && wait(&q_full[t], (q_phase >> t) & 1, bad);
+              q_phase ^= 1u << t;
+            }
+            if (!ok) break;
+            if (more && mine.has(b)) {
+              tc::fence_after_sync();
+              mma_rows(t_s, s_q + t * kTile, s_kv + (2 * st + 1) * kTile, idesc_s, steps);
+              tc::mma_commit(&s_full[t]);
+            }
+            if (before >= 0 && mine.has(before)) tc::mma_commit(&o_full[t]);
+          }
+          if (!ok) break;
+          tc::mma_commit(&kv_empty[st]);
+          look = more && !m.whole(b);
+          before = more ? b : -1;
+          if (more) b = m.all.next(b);
+          if (more && b >= m.all.hi) tc::mma_commit(q_empty);   // those were the last scores
+        }
       }
-      __syncwarp();
-      before = more ? b : -1;
-      if (more) b = u.all.next(b);
-      n += 2;
+      ok = __all_sync(0xffffffffu, ok);
+      give_back(k);
     }
   }
-  } else if (u.any) {
+  } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowRegisters));
     // ------------------------------------------------------------------------------------------ a row per thread ----
     const int t = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t t_s = lane_base + t * 128, t_o = lane_base + 256 + t * DP;
+    const F2 scale2 = f2(p.scale_log2, p.scale_log2);
+    uint32_t phase = 0;   // of the next S
+    int total = 0;        // blocks so far, of all units
+    bool ok = true;
+    for (int k = 0; ok && take(k); ++k) {
+    const Unit& u = s_unit[k & 1];
     const int pos = u.first[t] + row, first = u.first[t], last = u.last[t];
     const Blocks blocks = u.b[t];
     float m = -INFINITY, l = 0.f;
-    uint32_t phase = 0;   // of the next S
     int done = 0;         // blocks so far
-    bool ok = true;
-    for (int b = blocks.next(-1); b < blocks.hi; b = blocks.next(b)) {
+    for (int b = blocks.next(-1); b < blocks.hi; b = blocks.next(b), phase ^= 1) {
       ok = wait(&s_full[t], phase, bad);
-      if (!__all_sync(0xffffffffu, ok)) {
-        ok = false;
-        break;
-      }
-      phase ^= 1;
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
       tc::fence_after_sync();
       float s[128];
       {
@@ -331,56 +436,67 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int c = 0; c < 128; ++c) s[c] = c <= high && (c > low || c < sink) ? s[c] : -INFINITY;
       }
-      float mx = fmaxf(s[0], s[1]);
+      float m8[8];
 #pragma unroll
-      for (int c = 2; c < 128; c += 2) mx = fmaxf(mx, fmaxf(s[c], s[c + 1]));
+      for (int i = 0; i < 8; ++i) m8[i] = fmaxf(s[2 * i], s[2 * i + 1]);
+#pragma unroll
+      for (int c = 16; c < 128; c += 16) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m8[i] = max3(m8[i], s[c + 2 * i], s[c + 2 * i + 1]);
+      }
+      const float mx = max3(max3(m8[0], m8[1], m8[2]), max3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]));
       // a row's maximum stays until it is passed by 2^kSlack.  (Each row's own: its bits do not depend on what else is in the tile.)
       const bool raise = (mx - m) * p.scale_log2 > Weights<H>::kSlack || (m == -INFINITY && mx > m);
       if (__any_sync(0xffffffffu, raise)) {
         const float next = raise ? mx : m, f = raise ? (m == -INFINITY ? 0.f : exp2f((m - next) * p.scale_log2)) : 1.f;
         if (done > 0) {
-          ok = wait(&o_full[t], (done - 1) & 1, bad);
-          if (!__all_sync(0xffffffffu, ok)) {
-            ok = false;
-            break;
-          }
+          ok = wait(&o_full[t], (total - 1) & 1, bad);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
           tc::fence_after_sync();
-#pragma unroll
-          for (int c = 0; c < DP / 32; ++c) {
-            uint32_t o[32];
-            tc::tmem_ld_32x32(t_o + 32 * c, o);
+#pragma unroll 1
+          for (int c = 0; c < DP / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld16(t_o + 16 * c, o);
             tc::tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tmem_st32(t_o + 32 * c, o);
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tmem_st16(t_o + 16 * c, o);
           }
         }
         l *= f;
         m = next;
       }
       const float base = (m == -INFINITY ? 0.f : m * p.scale_log2) - Weights<H>::kBias;
-      float sum0 = 0.f, sum1 = 0.f;
+      const F2 base2 = f2(-base, -base);
+      F2 sums[4] = {f2(0.f, 0.f), f2(0.f, 0.f), f2(0.f, 0.f), f2(0.f, 0.f)};
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int h = 0; h < 2; ++h) {
         uint32_t w[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
-          const float x = exp2f(fmaf(s[64 * c + 2 * e], p.scale_log2, -base)), y = exp2f(fmaf(s[64 * c + 2 * e + 1], p.scale_log2, -base));
-          sum0 += x;
-          sum1 += y;
-          const typename H::T2 h = H::down(x, y);
-          w[e] = *reinterpret_cast<const uint32_t*>(&h);
+          float lo, hi;
+          split(fma2(f2(s[64 * h + 2 * e], s[64 * h + 2 * e + 1]), scale2, base2), lo, hi);
+          lo = exp2f(lo);
+          hi = exp2f(hi);
+          sums[e & 3] = add2(sums[e & 3], f2(lo, hi));
+          const typename H::T2 h2 = H::down(lo, hi);
+          w[e] = *reinterpret_cast<const uint32_t*>(&h2);
         }
-        tmem_st32(t_s + 32 * c, w);
+        tmem_st32(t_s + 32 * h, w);
+        tmem_st_wait();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&p_full[2 * t + h]);
       }
-      l += sum0 + sum1;
-      tmem_st_wait();
-      tc::fence_before_sync();
-      tc::mbar_arrive(&p_full[t]);
+      float sum, other;
+      split(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])), sum, other);
+      l += sum + other;
       ++done;
+      ++total;
     }
     if (ok && done > 0) {
-      ok = wait(&o_full[t], (done - 1) & 1, bad);
+      ok = wait(&o_full[t], (total - 1) & 1, bad);
       ok = __all_sync(0xffffffffu, ok);
       tc::fence_after_sync();
     }
@@ -393,7 +509,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         a.lse[static_cast<long long>(u.head[t]) * p.tokens + u.s.q0 + u.row[t] + row] = none ? -INFINITY : (m * p.scale_log2 + log2f(l) - Weights<H>::kBias) / kLog2e;
       uint8_t* stage = s_out + warp * 2048;
       const long long o_at = (static_cast<long long>(u.s.q0 + u.row[t] + (warp & 3) * 32) * p.heads + u.head[t]) * p.head_dim;
-      const bool odd = *odd_values != 0;
+      const bool odd = *reinterpret_cast<const volatile int*>(&u.odd) != 0;
+      const int kv = u.head[t] / p.group;
       for (int c0 = 0; c0 < p.head_dim; c0 += 32) {
         uint32_t o[32] = {};
         if (done > 0) {
@@ -407,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           // values that are not finite in blocks that were looked at, seen by this row
           const typename H::T* v = static_cast<const typename H::T*>(a.v.p) + kv * a.v.head + static_cast<long long>(u.s.k0) * a.v.token + c0;
           for (int b = blocks.next(-1); b < blocks.hi; b = blocks.next(b)) {
-            if (u.whole(p, b)) continue;
+            if (u.whole(b)) continue;
             for (int j = b * kRows; j < min(b * kRows + kRows, pos + 1); ++j) {
               if (j <= pos - p.window && j >= p.sinks) continue;
 #pragma unroll
@@ -426,6 +543,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
+    tc::fence_before_sync();   // the next unit's first product with V writes O
+    give_back(k);
+    }
     tc::fence_before_sync();
   }
   __syncthreads();
@@ -434,7 +554,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc::fence_after_sync();
     tc::tmem_dealloc(tmem, 512);
   }
-  zero_outside<typename H::T>(a.o, p.heads * p.head_dim, a.lse, p.heads, p.offsets, p.sequences, p.tokens);
 }
 
 template <typename H, int DP>

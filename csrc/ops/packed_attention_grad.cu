@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int st = n & 1, next = st ^ 1;
         const bool more = n + 1 < items;
         if (!all_wait(p_full, n & 1)) break;
-        if (tc::elect_one()) mma_weights<64>(t_dv, t_s, s_do + st * kTile, idesc_g, n > 0);
+        if (tc::elect_one()) mma_weights<128, 64>(t_dv, t_s, s_do + st * kTile, idesc_g, n > 0);
         __syncwarp();
         if (more) {
           if (!all_wait(&q_full[next], ((n + 1) / 2) & 1)) break;
@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (!all_wait(ds_full, n & 1)) break;
         if (tc::elect_one()) {
-          mma_weights<64>(t_dk, t_dp, s_q + st * kTile, idesc_g, n > 0);
+          mma_weights<128, 64>(t_dk, t_dp, s_q + st * kTile, idesc_g, n > 0);
           tc::mma_commit(&empty[st]);
           if (more) {
             mma_rows(t_dp, s_v, s_do + next * kTile, idesc_s, steps);
@@ -408,8 +408,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc::fence_after_sync();
     tc::tmem_dealloc(tmem, 512);
   }
-  zero_outside<H::T>(a.dk, p.kv_heads * p.head_dim, nullptr, 0, p.k_offsets, p.sequences, p.k_tokens);
-  zero_outside<H::T>(a.dv, p.kv_heads * p.head_dim, nullptr, 0, p.k_offsets, p.sequences, p.k_tokens);
+  zero_outside<H::T>(a.dk, p.kv_heads * p.head_dim, nullptr, 0, p.k_offsets, p.sequences, p.k_tokens, blockIdx.x, gridDim.x, tid, kThreads);
+  zero_outside<H::T>(a.dv, p.kv_heads * p.head_dim, nullptr, 0, p.k_offsets, p.sequences, p.k_tokens, blockIdx.x, gridDim.x, tid, kThreads);
 }
 
 // --------------------------------------------------------------------------------------------------- queries ----
@@ -577,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (more) scores(n + 1);
         if (!all_wait(ds_full, n & 1)) break;
         if (tc::elect_one()) {
-          mma_weights<64>(t_dq, t_dp, s_k + st * kTile, idesc_g, n > 0);
+          mma_weights<128, 64>(t_dq, t_dp, s_k + st * kTile, idesc_g, n > 0);
           tc::mma_commit(&k_empty[st]);
           if (!more) tc::mma_commit(done);
         }
@@ -681,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc::fence_after_sync();
     tc::tmem_dealloc(tmem, 512);
   }
-  zero_outside<H::T>(a.dq, p.heads * p.head_dim, nullptr, 0, p.offsets, p.sequences, p.tokens);
+  zero_outside<H::T>(a.dq, p.heads * p.head_dim, nullptr, 0, p.offsets, p.sequences, p.tokens, blockIdx.x, gridDim.x, tid, kThreads);
 }
 
 template <int DP>

@@ -131,12 +131,12 @@ __device__ __forceinline__ void mma_rows(uint32_t d, const uint8_t* a, const uin
     tc::mma_bf16(d, da + off, db + off, idesc, k != 0);
   }
 }
-// D[128 x n] (+)= A[tmem, 128 x 128] B with B's rows along the sum: 128 rows of a tile.  The second half of A is `kApart` columns behind the first.
-template <int kApart = 32>
+// D[128 x n] (+)= A[tmem, 128 x kKeys] B with B's rows along the sum: kKeys rows of a tile.  A's second 64 columns are `kApart` columns behind the first.
+template <int kKeys, int kApart = 0>
 __device__ __forceinline__ void mma_weights(uint32_t d, uint32_t a, const uint8_t* b, uint32_t idesc, bool accumulate) {
   const uint64_t db = tc::smem_desc_mn_sw128(b, kSub);
 #pragma unroll
-  for (int k = 0; k < kRows / 16; ++k) mma_ts(d, a + (k >> 2) * kApart + 8 * (k & 3), db + 128 * k, idesc, k != 0 || accumulate);
+  for (int k = 0; k < kKeys / 16; ++k) mma_ts(d, a + (k >> 2) * kApart + 8 * (k & 3), db + 128 * k, idesc, k != 0 || accumulate);
 }
 
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
@@ -147,6 +147,13 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
       "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
       "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+                 "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr)
+               : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
@@ -178,22 +185,48 @@ __device__ __forceinline__ void rows_out(uint8_t* stage, const float (&f)[32], t
   __syncwarp();
 }
 
-// Rows of no sequence, shared out over the grid's blocks: zeros in x [tokens, width], minus infinity in lse [heads, tokens] (may be null).
+// Rows of no sequence: zeros in x [tokens, width], minus infinity in lse [heads, tokens] (may be null).  Share `share` of `shares`, by `threads` threads.
 template <typename T>
-__device__ __forceinline__ void zero_outside(void* x, int width, float* lse, int heads, const int* offsets, int sequences, int tokens) {
+__device__ __forceinline__ void zero_outside(void* x, int width, float* lse, int heads, const int* offsets, int sequences, int tokens, int share, int shares, int thread,
+                                             int threads) {
   const int begin = clamp(offsets[0], 0, tokens), end = max(begin, clamp(offsets[sequences], 0, tokens)), outside = begin + tokens - end;
-  for (int i = blockIdx.x; i < outside; i += gridDim.x) {
+  for (int i = share; i < outside; i += shares) {
     const long long r = i < begin ? i : end + (i - begin);
     uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(x) + r * width);
-    for (int c = threadIdx.x; c < width / 8; c += blockDim.x) to[c] = make_uint4(0u, 0u, 0u, 0u);
+    for (int c = thread; c < width / 8; c += threads) to[c] = make_uint4(0u, 0u, 0u, 0u);
     if (lse != nullptr)
-      for (int h = threadIdx.x; h < heads; h += blockDim.x) lse[static_cast<long long>(h) * tokens + r] = -INFINITY;
+      for (int h = thread; h < heads; h += threads) lse[static_cast<long long>(h) * tokens + r] = -INFINITY;
   }
 }
 
+// Two fp32 numbers in one register pair and instruction.
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void split(F2 a, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a.v)); }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 // A wait that gives up, and at once when another role of the block has: the first to give up says so in *bad.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* bad) {
-  for (uint32_t i = 0; i < (1u << 22); ++i) {
+  for (uint32_t i = 0; i < (1u << 17); ++i) {   // a second or so: the instruction itself waits for some microseconds
     if (tc::mbar_try_wait(bar, parity)) return true;
     if ((i & 15) == 15 && *bad) return false;
   }
