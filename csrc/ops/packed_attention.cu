@@ -107,6 +107,7 @@ template <typename H, int DP>
 __global__ void __launch_bounds__(kThreads, 1)
     packed_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Forward a) {
   constexpr int kTile = (DP / 64) * kSub;
+  constexpr uint32_t kP = DP == 64 ? 384 : 0, kPStep = DP == 64 ? 64 : 128;   // columns of the weights
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* s_q = smem;                        // [2] tiles
@@ -162,7 +163,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc::fence_after_sync();
   const uint32_t tmem = *tmem_slot;
   pdl_trigger();
-  // tensor memory: S of tile t in columns 128 t .. 128 t + 127 (P in the first 64 of them), O in 256 + DP t ..
+  // tensor memory: S of tile t in columns 128 t .. 128 t + 127, O in 256 + DP t .., P in 384 + 64 t .. where O leaves room for it.  Otherwise P is in the first 64
+  // columns of S, and the next scores are written behind its product: products of one shape (both 128 x 128 x 16) are carried out in the order they were issued
+  // in.  (Of different shapes they are not: 128 x 64 behind 128 x 128 overwrote weights that were still to be read.)
   // Each role takes the units as they come; what they share in stages and phases goes on from one to the next, so that the loads and first products of a unit
   // are under way while the results of the one before are on their way out.
   auto take = [&](int k) {   // unit k of this block is described
@@ -344,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // One thread.  What it does between the last product of one tile and the first of the other has some 500 clocks, the time of those under way; a barrier's
     // state takes 250 while the products read shared memory.  Hence one barrier for values and keys of a step, and nothing else on the way.
     constexpr uint32_t idesc_s = idesc16<H>(kRows, kRows, false, false);
-    const uint32_t idesc_o = idesc16<H>(kRows, (p.head_dim + 15) / 16 * 16, false, true);
+    constexpr uint32_t idesc_o = idesc16<H>(kRows, DP, false, true);   // (columns behind head_dim are zeros: TMA fills them in)
     const int steps = (p.head_dim + 15) / 16;
     uint32_t q_phase = 0, p_phase = 0, looked_phase = 0;   // a bit per tile; the last: per stage
     int i = 0;                                             // steps so far
@@ -366,14 +369,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
           for (int t = 0; t < 2; ++t) {
             const Blocks mine = t == 0 ? m.b[0] : m.b[1];
-            const uint32_t t_s = tmem + t * 128;
             if (before >= 0 && mine.has(before)) {
 #pragma unroll 1
               for (int h = 0; h < 2; ++h) {   // the first half of the weights is multiplied while the second is made
                 ok = ok && wait(&p_full[2 * t + h], (p_phase >> t) & 1, bad);
                 if (!ok) break;
                 tc::fence_after_sync();
-                mma_weights<64>(tmem + 256 + t * DP, t_s + 32 * h, s_kv + 2 * st * kTile + h * 64 * 128, idesc_o, h != 0 || ((begun >> t) & 1));
+                mma_weights<64>(tmem + 256 + t * DP, tmem + kP + kPStep * t + 32 * h, s_kv + 2 * st * kTile + h * 64 * 128, idesc_o, h != 0 || ((begun >> t) & 1));
               }
               p_phase ^= 1u << t;
               begun |= 1u << t;
@@ -384,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) break;
             if (more && mine.has(b)) {
               tc::fence_after_sync();
-              mma_rows(t_s, s_q + t * kTile, s_kv + (2 * st + 1) * kTile, idesc_s, steps);
+              mma_rows(tmem + t * 128, s_q + t * kTile, s_kv + (2 * st + 1) * kTile, idesc_s, steps);
               tc::mma_commit(&s_full[t]);
             }
             if (before >= 0 && mine.has(before)) tc::mma_commit(&o_full[t]);
@@ -406,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------------------------------------ a row per thread ----
     const int t = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const uint32_t t_s = lane_base + t * 128, t_o = lane_base + 256 + t * DP;
+    const uint32_t t_s = lane_base + t * 128, t_o = lane_base + 256 + t * DP, t_p = lane_base + kP + kPStep * t;
     const F2 scale2 = f2(p.scale_log2, p.scale_log2);
     uint32_t phase = 0;   // of the next S
     int total = 0;        // blocks so far, of all units
@@ -483,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const typename H::T2 h2 = H::down(lo, hi);
           w[e] = *reinterpret_cast<const uint32_t*>(&h2);
         }
-        tmem_st32(t_s + 32 * h, w);
+        tmem_st32(t_p + 32 * h, w);
         tmem_st_wait();
         tc::fence_before_sync();
         __syncwarp();
