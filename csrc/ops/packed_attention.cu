@@ -122,14 +122,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* p_full = s_full + 2;              // [2][2]: tile, half of a block's keys
   uint64_t* o_full = p_full + 4;              // [2]
   uint64_t* q_empty = o_full + 2;
-  uint64_t* unit_full = q_empty + 1;          // [2]
-  uint64_t* unit_empty = unit_full + 2;       // [2]
-  uint64_t* next_full = unit_empty + 2;
-  uint64_t* loads_done = next_full + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(loads_done + 1);
+  uint64_t* plan_barriers = q_empty + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(plan_barriers + Plan::kBarriers);
   volatile int* bad = reinterpret_cast<volatile int*>(tmem_slot + 1);
   uint4* s_next = reinterpret_cast<uint4*>((reinterpret_cast<uintptr_t>(tmem_slot + 2) + 15) & ~static_cast<uintptr_t>(15));
   Unit* s_unit = reinterpret_cast<Unit*>(s_next + 1);   // [2]
+  const Plan plan = Plan::at(plan_barriers, s_next, bad);
 
   const Problem& p = a.p;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -147,12 +145,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::mbar_init(&looked[i], 1);
     }
     tc::mbar_init(q_empty, 1);
-    for (int i = 0; i < 2; ++i) {
-      tc::mbar_init(&unit_full[i], 1);
-      tc::mbar_init(&unit_empty[i], kRoles);
-    }
-    tc::mbar_init(next_full, 1);
-    tc::mbar_init(loads_done, 1);
+    plan.init(kRoles);
     *bad = 0;
     tc::mbar_init_fence();
   }
@@ -168,80 +161,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   // in.  (Of different shapes they are not: 128 x 64 behind 128 x 128 overwrote weights that were still to be read.)
   // Each role takes the units as they come; what they share in stages and phases goes on from one to the next, so that the loads and first products of a unit
   // are under way while the results of the one before are on their way out.
-  auto take = [&](int k) {   // unit k of this block is described
-    const bool ok = wait(&unit_full[k & 1], (k >> 1) & 1, bad);
-    return __all_sync(0xffffffffu, ok) && !s_unit[k & 1].end;
-  };
-  auto give_back = [&](int k) {
-    __syncwarp();
-    if (lane == 0) tc::mbar_arrive(&unit_empty[k & 1]);
-  };
-
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
   if (warp == 11) {
     // ----------------------------------------------------------------------------------- what comes next ----
-    // A block that is done with its unit takes the next one of the grid that no block has begun (the launch's order: long ones first).
-    int id = static_cast<int>(blockIdx.x), asked = 0;
-    bool more = true;
-    for (int k = 0; more;) {
-      const Unit found = unit_of(a, id);
+    plan.run(s_unit, [&](int id) {
       zero_outside<typename H::T>(a.o, p.heads * p.head_dim, a.lse, p.heads, p.offsets, p.sequences, p.tokens, id, a.units, lane, 32);
-      if (found.any) {
-        const bool ok = k < 2 || wait(&unit_empty[k & 1], ((k >> 1) - 1) & 1, bad);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        if (lane == 0) {
-          s_unit[k & 1] = found;
-          tc::mbar_arrive(&unit_full[k & 1]);
-        }
-        __syncwarp();
-        ++k;
-        // asked for no earlier than the unit's last loads are under way: another block may be free sooner
-        const bool near = wait(loads_done, (k - 1) & 1, bad);
-        if (!__all_sync(0xffffffffu, near)) break;
-      }
-      if (lane == 0) {
-        fence_async_smem();
-        tc::mbar_expect_tx(next_full, 16);
-        asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(tc::smem_u32(s_next)), "r"(tc::smem_u32(next_full))
-                     : "memory");
-      }
-      __syncwarp();
-      bool ok = wait(next_full, asked & 1, bad);
-      if (!__all_sync(0xffffffffu, ok)) {
-        tc::mbar_wait(next_full, asked & 1, 1u << 16);   // the answer must land before the block retires
-        break;
-      }
-      ++asked;
-      uint32_t got, x;
-      asm volatile(
-          "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"
-          "ld.shared.b128 h, [%2];\n\t"
-          "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
-          "selp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
-          "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
-          : "=r"(got), "=r"(x)
-          : "r"(tc::smem_u32(s_next))
-          : "memory");
-      __syncwarp();
-      more = got != 0;
-      id = static_cast<int>(x);
-      if (!more) {
-        const bool free = k < 2 || wait(&unit_empty[k & 1], ((k >> 1) - 1) & 1, bad);
-        if (!__all_sync(0xffffffffu, free)) break;
-        if (lane == 0) {
-          s_unit[k & 1].end = true;
-          tc::mbar_arrive(&unit_full[k & 1]);
-        }
-        __syncwarp();
-      }
-    }
+      return unit_of(a, id);
+    });
   } else if (warp == 9) {
     // ------------------------------------------------------------------------------------------- loads ----
     uint32_t raw_uses = 0, q_uses = 0;   // a bit per stage, a bit per tile
     int i = 0, units = 0;                // steps, and units with keys, so far
     bool ok = true;
-    for (int k = 0; ok && take(k); ++k) {
+    for (int k = 0; ok && plan.take(s_unit, k); ++k) {
       const Unit& u = s_unit[k & 1];
       if (tc::elect_one()) {
         const int kv = u.head[0] / p.group;
@@ -284,8 +217,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       ok = __all_sync(0xffffffffu, ok);
-      if (lane == 0) tc::mbar_arrive(loads_done);
-      give_back(k);
+      if (lane == 0) tc::mbar_arrive(plan.loads_done);
+      plan.give_back(k);
     }
   } else if (warp == 10) {
     // --------------------------------------------------------- blocks of keys that not every row sees ----
@@ -294,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int steps = 0;
     uint32_t phase = 0;   // a bit per stage
     bool ok = true;
-    for (int k = 0; ok && take(k); ++k) {
+    for (int k = 0; ok && plan.take(s_unit, k); ++k) {
     const Unit& u = s_unit[k & 1];
     int i = steps + 1;
     for (int b = u.all.next(-1); b < u.all.hi; b = u.all.next(b), ++i) {
@@ -340,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) tc::mbar_arrive(&looked[st]);
     }
     if (u.all.hi > 0) steps = i;   // a step more than blocks
-    give_back(k);
+    plan.give_back(k);
     }
   } else if (warp == 8) {
     // ---------------------------------------------------------------------------------------- products ----
@@ -352,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t q_phase = 0, p_phase = 0, looked_phase = 0;   // a bit per tile; the last: per stage
     int i = 0;                                             // steps so far
     bool ok = true;
-    for (int k = 0; ok && take(k); ++k) {
+    for (int k = 0; ok && plan.take(s_unit, k); ++k) {
       const Unit m = s_unit[k & 1];
       if (tc::elect_one()) {
         uint32_t begun = 0;
@@ -400,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       ok = __all_sync(0xffffffffu, ok);
-      give_back(k);
+      plan.give_back(k);
     }
   }
   } else {
@@ -413,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t phase = 0;   // of the next S
     int total = 0;        // blocks so far, of all units
     bool ok = true;
-    for (int k = 0; ok && take(k); ++k) {
+    for (int k = 0; ok && plan.take(s_unit, k); ++k) {
     const Unit& u = s_unit[k & 1];
     const int pos = u.first[t] + row, first = u.first[t], last = u.last[t];
     const Blocks blocks = u.b[t];
@@ -546,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     tc::fence_before_sync();   // the next unit's first product with V writes O
-    give_back(k);
+    plan.give_back(k);
     }
     tc::fence_before_sync();
   }

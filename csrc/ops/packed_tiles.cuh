@@ -139,6 +139,17 @@ __device__ __forceinline__ void mma_weights(uint32_t d, uint32_t a, const uint8_
   for (int k = 0; k < kKeys / 16; ++k) mma_ts(d, a + (k >> 2) * kApart + 8 * (k & 3), db + 128 * k, idesc, k != 0 || accumulate);
 }
 
+// The same with A and B in halves: of each 64 columns (two times, `kApart` columns of tensor memory apart) the 32 from 32 h on.
+template <int kApart>
+__device__ __forceinline__ void mma_half(uint32_t d, uint32_t a, const uint8_t* b, int h, uint32_t idesc, bool accumulate) {
+  const uint64_t db = tc::smem_desc_mn_sw128(b, kSub);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int w = i >> 1, k = 4 * w + 2 * h + (i & 1);
+    mma_ts(d, a + w * kApart + 8 * (k & 3), db + 128 * k, idesc, i != 0 || accumulate);
+  }
+}
+
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
@@ -252,6 +263,93 @@ inline Problem problem_of(const PackedAttentionArgs& a) {
   p.err = gemm_error_device_ptr();
   return p;
 }
+
+// ------------------------------------------------------------------------------------------------ units of work ----
+// A block goes on from unit to unit: one warp plans, the others take what it describes.  The first unit is the block's own, the next ones are blocks of the grid
+// that have not begun, which it asks the hardware for (the launch's order: long ones first).
+struct Plan {
+  uint64_t* full;        // [2]: a unit is described
+  uint64_t* empty;       // [2]: all roles are done with it
+  uint64_t* answer;      // of the request for the next one
+  uint64_t* loads_done;  // the unit's last loads are under way: no earlier is the next one asked for, another block may be free sooner
+  uint4* next;
+  volatile int* bad;
+  static constexpr int kBarriers = 6;
+  __device__ __forceinline__ static Plan at(uint64_t* barriers, uint4* next, volatile int* bad) { return {barriers, barriers + 2, barriers + 4, barriers + 5, next, bad}; }
+  __device__ __forceinline__ void init(int roles) const {   // one thread
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&full[i], 1);
+      tc::mbar_init(&empty[i], roles);
+    }
+    tc::mbar_init(answer, 1);
+    tc::mbar_init(loads_done, 1);
+  }
+  // Unit k of this block is described (false: there is none).  Whole warps.
+  template <typename Unit>
+  __device__ __forceinline__ bool take(const Unit* units, int k) const {
+    const bool ok = wait(&full[k & 1], (k >> 1) & 1, bad);
+    return __all_sync(0xffffffffu, ok) && !units[k & 1].end;
+  }
+  __device__ __forceinline__ void give_back(int k) const {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) tc::mbar_arrive(&empty[k & 1]);
+  }
+  // The planning warp.  find(id): the unit of block `id` (any: whether there is work for the others).
+  template <typename Unit, typename Find>
+  __device__ __forceinline__ void run(Unit* units, Find find) const {
+    const int lane = threadIdx.x & 31;
+    int id = static_cast<int>(blockIdx.x), asked = 0;
+    auto free = [&](int k) { return __all_sync(0xffffffffu, k < 2 || wait(&empty[k & 1], ((k >> 1) - 1) & 1, bad)); };
+    for (int k = 0;;) {
+      const Unit found = find(id);
+      if (found.any) {
+        if (!free(k)) return;
+        if (lane == 0) {
+          units[k & 1] = found;
+          tc::mbar_arrive(&full[k & 1]);
+        }
+        __syncwarp();
+        const bool near = wait(loads_done, k & 1, bad);
+        if (!__all_sync(0xffffffffu, near)) return;
+        ++k;
+      }
+      if (lane == 0) {
+        fence_async_smem();   // the last answer has been read
+        tc::mbar_expect_tx(answer, 16);
+        asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(tc::smem_u32(next)), "r"(tc::smem_u32(answer))
+                     : "memory");
+      }
+      __syncwarp();
+      const bool ok = wait(answer, asked & 1, bad);
+      if (!__all_sync(0xffffffffu, ok)) {
+        tc::mbar_wait(answer, asked & 1, 1u << 16);   // it must land before the block retires
+        return;
+      }
+      ++asked;
+      uint32_t got, x;
+      asm volatile(
+          "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"
+          "ld.shared.b128 h, [%2];\n\t"
+          "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+          "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
+          : "=r"(got), "=r"(x)
+          : "r"(tc::smem_u32(next))
+          : "memory");
+      __syncwarp();
+      if (got == 0) {
+        if (!free(k)) return;
+        if (lane == 0) {
+          units[k & 1].end = true;
+          tc::mbar_arrive(&full[k & 1]);
+        }
+        __syncwarp();
+        return;
+      }
+      id = static_cast<int>(x);
+    }
+  }
+};
 
 // [tokens, heads, head_dim] as boxes of 64 columns of 128 rows of a head.  (The stride of a dimension of one is never used and may be anything.)
 inline bool encode_rows(CUtensorMap* map, Half16 type, const TokenView& t, int tokens, int heads, int head_dim) {
