@@ -24,33 +24,42 @@ struct Rotary {
   int turned;               // the first of them turn pairs
 };
 
+// N values of one access.
+template <int N>
+struct Access;
+template <>
+struct Access<8> {
+  using V = uint4;
+};
+template <>
+struct Access<4> {
+  using V = uint2;
+};
 template <typename H, int N>
-struct Vector;
-template <typename H>
-struct Vector<H, 8> {
-  uint4 raw;
-  __device__ __forceinline__ void up(float (&f)[8]) const { unpack8_as<H>(raw, f); }
-  __device__ __forceinline__ void down(const float (&f)[8]) { raw = pack8_as<H>(f); }
-};
-template <typename H>
-struct Vector<H, 4> {
-  uint2 raw;
-  __device__ __forceinline__ void up(float (&f)[4]) const {
-    const typename H::T2* h = reinterpret_cast<const typename H::T2*>(&raw);
-    const float2 a = H::up(h[0]), b = H::up(h[1]);
-    f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y;
+__device__ __forceinline__ void up(const typename Access<N>::V& raw, float (&f)[N]) {
+  const typename H::T2* h = reinterpret_cast<const typename H::T2*>(&raw);
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) {
+    const float2 t = H::up(h[i]);
+    f[2 * i] = t.x;
+    f[2 * i + 1] = t.y;
   }
-  __device__ __forceinline__ void down(const float (&f)[4]) {
-    typename H::T2* h = reinterpret_cast<typename H::T2*>(&raw);
-    h[0] = H::down(f[0], f[1]);
-    h[1] = H::down(f[2], f[3]);
-  }
-};
+}
+template <typename H, int N>
+__device__ __forceinline__ typename Access<N>::V down(const float (&f)[N]) {
+  typename Access<N>::V raw;
+  typename H::T2* h = reinterpret_cast<typename H::T2*>(&raw);
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) h[i] = H::down(f[2 * i], f[2 * i + 1]);
+  return raw;
+}
 
-// HALVES: N elements and the N of the other half per place; otherwise 8 elements, four pairs.  Behind the turned places 8 elements each are copied.
-template <typename H, bool HALVES, int N>
+// HALVES: N elements and the N of the other half per place; otherwise 8 elements, four pairs.  Behind the turned places 8 elements each are copied.  HEADS heads per
+// thread, all of whose loads are under way together.
+template <typename H, bool HALVES, int N, int HEADS>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const Rotary r, int total) {
   using T = typename H::T;
+  using V = typename Access<N>::V;
   const RotaryArgs& a = r.a;
   pdl_wait();
   pdl_trigger();
@@ -59,68 +68,85 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Rotary r, int to
   const int rest = r.places.of(i), place = i - rest * r.places.d, t = r.groups.of(rest), group = rest - t * r.groups.d;
   const int pos = a.positions != nullptr ? __ldg(a.positions + t) : t;
   const bool inside = pos >= 0 && pos < a.rope_rows, turn = place < r.turned;
-  constexpr int kPairs = HALVES ? N : 4;
-  float c[kPairs], s[kPairs];
-  if (turn && inside) {
-    const float* at_c = a.cos + static_cast<long long>(pos) * a.width + place * kPairs;
-    const float* at_s = a.sin + static_cast<long long>(pos) * a.width + place * kPairs;
-#pragma unroll
-    for (int e = 0; e < kPairs; e += 4) {
-      const float4 x = __ldg(reinterpret_cast<const float4*>(at_c + e)), y = __ldg(reinterpret_cast<const float4*>(at_s + e));
-      c[e] = x.x, c[e + 1] = x.y, c[e + 2] = x.z, c[e + 3] = x.w;
-      s[e] = y.x, s[e + 1] = y.y, s[e + 2] = y.z, s[e + 3] = y.w;
-    }
-    if (a.inverse) {
-#pragma unroll
-      for (int e = 0; e < kPairs; ++e) s[e] = -s[e];
-    }
-  }
   const int column = turn ? place * (HALVES ? N : 8) : 2 * a.width + (place - r.turned) * 8;
-#pragma unroll 4
-  for (int h = group; h < a.q.heads + a.k.heads; h += r.groups.d) {
-    const bool is_q = h < a.q.heads;
+  const T* from[HEADS];
+  T* to[HEADS];
+#pragma unroll
+  for (int j = 0; j < HEADS; ++j) {
+    const int h = group + j * r.groups.d;
+    const bool is_q = h < a.q.heads, any = h < a.q.heads + a.k.heads;
     const RotaryPart& part = is_q ? a.q : a.k;
     const int hh = is_q ? h : h - a.q.heads;
-    const T* x = static_cast<const T*>(part.x.p) + t * part.x.token + hh * part.x.head + column;
-    T* y = static_cast<T*>(part.out) + (static_cast<long long>(t) * part.heads + hh) * a.head_dim + column;
-    if (!turn) {
-      *reinterpret_cast<uint4*>(y) = inside ? __ldg(reinterpret_cast<const uint4*>(x)) : make_uint4(0u, 0u, 0u, 0u);
-    } else if constexpr (HALVES) {
-      using V = decltype(Vector<H, N>::raw);
-      Vector<H, N> lo{}, hi{};
-      if (inside) {
-        lo.raw = __ldg(reinterpret_cast<const V*>(x));
-        hi.raw = __ldg(reinterpret_cast<const V*>(x + a.width));
-        float f[N], g[N];
-        lo.up(f);
-        hi.up(g);
+    from[j] = any && inside ? static_cast<const T*>(part.x.p) + t * part.x.token + hh * part.x.head + column : nullptr;
+    to[j] = any ? static_cast<T*>(part.out) + (static_cast<long long>(t) * part.heads + hh) * a.head_dim + column : nullptr;
+  }
+  if (!turn) {
+    uint4 x[HEADS];
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float u = f[e], v = g[e];
-          f[e] = u * c[e] - v * s[e];
-          g[e] = u * s[e] + v * c[e];
-        }
-        lo.down(f);
-        hi.down(g);
-      }
-      *reinterpret_cast<V*>(y) = lo.raw;
-      *reinterpret_cast<V*>(y + a.width) = hi.raw;
-    } else {
-      uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-      if (inside) {
-        float f[8];
-        unpack8_as<H>(__ldg(reinterpret_cast<const uint4*>(x)), f);
+    for (int j = 0; j < HEADS; ++j) x[j] = from[j] != nullptr ? __ldg(reinterpret_cast<const uint4*>(from[j])) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float u = f[2 * e], v = f[2 * e + 1];
-          f[2 * e] = u * c[e] - v * s[e];
-          f[2 * e + 1] = u * s[e] + v * c[e];
-        }
-        raw = pack8_as<H>(f);
-      }
-      *reinterpret_cast<uint4*>(y) = raw;
+    for (int j = 0; j < HEADS; ++j)
+      if (to[j] != nullptr) *reinterpret_cast<uint4*>(to[j]) = x[j];
+    return;
+  }
+  constexpr int kPairs = HALVES ? N : 4;
+  V lo[HEADS], hi[HEADS];
+#pragma unroll
+  for (int j = 0; j < HEADS; ++j) {
+    lo[j] = hi[j] = V{};
+    if (from[j] != nullptr) {
+      lo[j] = __ldg(reinterpret_cast<const V*>(from[j]));
+      if (HALVES) hi[j] = __ldg(reinterpret_cast<const V*>(from[j] + a.width));
     }
   }
+  float c[kPairs], s[kPairs];
+#pragma unroll
+  for (int e = 0; e < kPairs; e += 4) {
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+    if (inside) {
+      x = __ldg(reinterpret_cast<const float4*>(a.cos + static_cast<long long>(pos) * a.width + place * kPairs + e));
+      y = __ldg(reinterpret_cast<const float4*>(a.sin + static_cast<long long>(pos) * a.width + place * kPairs + e));
+    }
+    c[e] = x.x, c[e + 1] = x.y, c[e + 2] = x.z, c[e + 3] = x.w;
+    s[e] = y.x, s[e + 1] = y.y, s[e + 2] = y.z, s[e + 3] = y.w;
+  }
+  if (a.inverse) {
+#pragma unroll
+    for (int e = 0; e < kPairs; ++e) s[e] = -s[e];
+  }
+#pragma unroll
+  for (int j = 0; j < HEADS; ++j) {
+    if (to[j] == nullptr) continue;
+    float f[N];
+    up<H, N>(lo[j], f);
+    if constexpr (HALVES) {
+      float g[N];
+      up<H, N>(hi[j], g);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float u = f[e], v = g[e];
+        f[e] = u * c[e] - v * s[e];
+        g[e] = u * s[e] + v * c[e];
+      }
+      *reinterpret_cast<V*>(to[j]) = down<H, N>(f);
+      *reinterpret_cast<V*>(to[j] + a.width) = down<H, N>(g);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float u = f[2 * e], v = f[2 * e + 1];
+        f[2 * e] = u * c[e] - v * s[e];
+        f[2 * e + 1] = u * s[e] + v * c[e];
+      }
+      *reinterpret_cast<V*>(to[j]) = down<H, N>(f);
+    }
+  }
+}
+
+template <typename H, bool HALVES, int N>
+void enqueue(const Rotary& r, int total, int per_thread, cudaStream_t stream) {
+  const int blocks = (total + kThreads - 1) / kThreads;
+  if (per_thread == 1) MCCL_LAUNCH_PDL((rotary_kernel<H, HALVES, N, 1>), blocks, kThreads, 0, stream, r, total);
+  else MCCL_LAUNCH_PDL((rotary_kernel<H, HALVES, N, 4>), blocks, kThreads, 0, stream, r, total);
 }
 
 template <typename H>
@@ -128,10 +154,9 @@ cudaError_t launch(const RotaryArgs& args, cudaStream_t stream) {
   const int wide = args.halves && args.width % 8 != 0 ? 4 : 8;
   const int turned = args.halves ? args.width / wide : args.width / 4, heads = args.q.heads + args.k.heads;
   const int places = turned + (args.head_dim - 2 * args.width) / 8;
-  // a thread takes as many heads as leave every SM its threads, up to 4: more of them share what it holds
+  // a thread takes four heads where that leaves every SM its threads
   const long long one = static_cast<long long>(args.tokens) * places * heads;
-  int per_thread = static_cast<int>(one / (148ll * 2048));
-  per_thread = per_thread < 1 ? 1 : (per_thread > 4 ? 4 : per_thread);
+  const int per_thread = one / 4 < 148ll * 2048 ? 1 : 4;
   const int groups = (heads + per_thread - 1) / per_thread;
   const long long per_token = static_cast<long long>(groups) * places;
   if (per_token > INT_MAX / 2) return cudaErrorInvalidValue;
@@ -157,14 +182,9 @@ cudaError_t launch(const RotaryArgs& args, cudaStream_t stream) {
     r.groups = Divisor(groups);
     r.turned = turned;
     const int total = static_cast<int>(tokens * per_token);
-    const int blocks = (total + kThreads - 1) / kThreads;
-    if (!args.halves) {
-      MCCL_LAUNCH_PDL((rotary_kernel<H, false, 8>), blocks, kThreads, 0, stream, r, total);
-    } else if (wide == 8) {
-      MCCL_LAUNCH_PDL((rotary_kernel<H, true, 8>), blocks, kThreads, 0, stream, r, total);
-    } else {
-      MCCL_LAUNCH_PDL((rotary_kernel<H, true, 4>), blocks, kThreads, 0, stream, r, total);
-    }
+    if (!args.halves) enqueue<H, false, 8>(r, total, per_thread, stream);
+    else if (wide == 8) enqueue<H, true, 8>(r, total, per_thread, stream);
+    else enqueue<H, true, 4>(r, total, per_thread, stream);
     count_launch();
   }
   return ::mccl::launch_status();
