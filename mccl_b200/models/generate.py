@@ -3,7 +3,8 @@
     generator = Generator(model, max_sequences=8, weights="w4")
     texts = generator.generate([[1, 2, 3], [4, 5]], max_new_tokens=20)
 
-On a CUDA device a prompt goes through the operators that score whole texts, which also fill the cache; a step is ``ops.paged_append`` (with the
+On a CUDA device a prompt goes through the operators that score whole texts, which also fill the cache, or several prompts of different lengths at once through
+those of packed texts (``ops.rotary``, ``ops.packed_attention``); a step is ``ops.paged_append`` (with the
 rotation of the models that have one), ``ops.paged_attention`` and, with 4-bit weights, ``ops.linear_w4``, captured as a CUDA graph per number of
 sequences.  On a CPU the same math runs on the operators' plain forms.
 """
@@ -11,7 +12,7 @@ from __future__ import annotations
 
 import contextlib
 import gc
-from typing import Dict, List, Optional, Sequence
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 import torch.nn.functional as F
@@ -150,6 +151,53 @@ class Generator:
             x = self._mlp(self._linear(a, layer["proj"], residual=x), layer)
         return self._logits(x[0, -1:])[0]
 
+    @torch.no_grad()
+    def prefill_together(self, prompts: Sequence[Sequence[int]]) -> Tuple[List[int], torch.Tensor]:
+        """New sequences that begin with these prompts, all of them in one pass: (their rows, the logits ``[len(prompts), vocab]`` behind each one's last token).
+
+        With a window too: a prompt longer than it needs pages for all its positions until the pass is over (``prefill`` goes on token by token instead)."""
+        with self._here():
+            return self._prefill_together(prompts)
+
+    def _prefill_together(self, prompts):
+        ids = [self._ids(tokens).reshape(-1) for tokens in prompts]
+        counts = [t.numel() for t in ids]
+        for count in counts:
+            if count < 1 or count > self.max_positions:
+                raise RuntimeError(f"Generator: a prompt of {count} tokens, 1 to {self.max_positions} are possible")
+        if not counts:
+            return [], torch.empty(0, self._head.shape[0], dtype=torch.bfloat16, device=self.device)
+        rows: List[int] = []
+        try:
+            for _ in counts:
+                rows.append(self.cache.add())
+            self.cache.reserve(rows, counts)
+            logits = self._packed(torch.cat(ids), rows, counts)
+            for row, count in zip(rows, counts):
+                self.cache.set_length(row, count)
+            if self.window is not None:
+                self.cache.drop_unseen(rows, self.window, self.sinks)
+        except BaseException:
+            for row in rows:
+                self.cache.free(row)
+            raise
+        return rows, logits
+
+    def _packed(self, ids, rows, counts):
+        cfg, cache, total = self.cfg, self.cache, ids.numel()
+        positions = torch.cat([torch.arange(n, dtype=torch.int32) for n in counts]).to(self.device)
+        owners = torch.repeat_interleave(torch.tensor(rows, dtype=torch.int32), torch.tensor(counts)).to(self.device)
+        offsets = torch.cumsum(torch.tensor([0] + counts), 0).to(torch.int32).to(self.device)
+        x = ops.embedding(ids, self._tok, None if self._pos is None else F.embedding(positions.long(), self._pos))
+        for i, layer in enumerate(self._layers):
+            q, k, v = self._linear(ops.norm(x, *layer["ln1"]), layer["qkv"]).view(total, 3, cfg.n_heads, cfg.head_dim).unbind(1)
+            if self._rope is not None:
+                q, k = ops.rotary(q, k, rope=self._rope, positions=positions)
+            ops.paged_append(k, v, cache.keys(i), cache.values(i), cache.table, positions, rows=owners)
+            a = ops.packed_attention(q, k, v, offsets, window=self.window, sinks=self.sinks).view(total, cfg.d_model)
+            x = self._mlp(self._linear(a, layer["proj"], residual=x), layer)
+        return self._logits(x.index_select(0, offsets[1:].long() - 1))
+
     # ----------------------------------------------------------------------------------------------------------- steps ----
     @torch.no_grad()
     def step(self, rows: Sequence[int], tokens) -> torch.Tensor:
@@ -229,20 +277,34 @@ class Generator:
 
     @torch.no_grad()
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: int, temperature: float = 0.0, generator: Optional[torch.Generator] = None,
-                 stop: Optional[int] = None) -> List[List[int]]:
-        """New tokens for each prompt: the likeliest ones (the lowest number among equals), or drawn at a temperature.  A sequence ends with the token
-        `stop`, after `max_new_tokens`, or at the last position; its pages are free afterwards."""
+                 stop: Optional[int] = None, *, top_k: Optional[int] = None, top_p: Optional[float] = None, min_p: Optional[float] = None,
+                 together: bool = False) -> List[List[int]]:
+        """New tokens for each prompt: the likeliest ones (the lowest number among equals), or drawn at a temperature, with any of top_k, top_p and min_p by
+        ``ops.sample``.  A sequence ends with the token `stop`, after `max_new_tokens`, or at the last position; its pages are free afterwards.
+        together: all prompts go through the model in one pass (``prefill_together``)."""
+        settings = {"top_k": top_k, "top_p": top_p, "min_p": min_p}
         out: List[List[int]] = [[] for _ in prompts]
         active: Dict[int, int] = {}   # row -> prompt
         logits = {}
         try:
-            for i, prompt in enumerate(prompts):
-                row, last = self.prefill(prompt)
-                active[row], logits[row] = i, last
+            if together:
+                rows, first = self.prefill_together(prompts)
+                active = {row: i for i, row in enumerate(rows)}
+                logits = dict(zip(rows, first))
+            else:
+                for i, prompt in enumerate(prompts):
+                    row, last = self.prefill(prompt)
+                    active[row], logits[row] = i, last
             while active and max_new_tokens > 0:
                 rows = list(active)
                 last = torch.stack([logits[r] for r in rows]).float()
-                if temperature > 0:
+                if temperature > 0 and any(v is not None for v in settings.values()):
+                    uniform = torch.rand(len(rows), generator=generator, device=self.device if generator is None else generator.device).to(self.device)
+                    with self._here():
+                        tokens = ops.sample(last, uniform, temperature=temperature, **settings)
+                    if bool((tokens < 0).any()):
+                        raise RuntimeError("Generator: the logits are not finite, there is nothing to draw from")
+                elif temperature > 0:
                     # (a temperature so low that logits / temperature overflows is that of the likeliest token)
                     chances = torch.softmax(last / max(temperature, 1e-30), dim=-1)
                     if not bool(torch.isfinite(chances).all()):
