@@ -73,6 +73,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_forward(const Attention
     o.zero_();
     if (lse) l.fill_(-std::numeric_limits<float>::infinity());
   } else {
+    at::Tensor workspace;
+    if (const size_t bytes = ops::packed_attention_workspace(a)) {
+      workspace = empty_on(x.q, {static_cast<int64_t>(bytes)}, at::kByte);
+      a.workspace = workspace.data_ptr();
+    }
     check_launch(ops::packed_attention(a, stream_of(x.q)), op);
   }
   return {o, l, r};

@@ -27,7 +27,9 @@ struct PackedAttentionArgs {
   float scale = 1.f;
   int window = 0, sinks = 0;
   Half16 type = Half16::bf16;
+  void* workspace = nullptr;   // packed_attention_workspace() bytes, on a 16-byte boundary
 };
+size_t packed_attention_workspace(const PackedAttentionArgs& a);
 cudaError_t packed_attention(const PackedAttentionArgs& a, cudaStream_t stream);
 
 // ---- its gradients, bf16.  f.o, f.o_rest and f.lse are what the forward call left, d_o [tokens, heads, head_dim]; dq, dk and dv are contiguous and

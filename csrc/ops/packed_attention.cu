@@ -36,6 +36,9 @@ struct Forward {
   int pair_heads;    // a block's tiles are two heads, otherwise two times 128 rows
   int head_units;    // blocks per slot
   int units;
+  int parts;         // blocks that share out a unit's keys; with more than one, results go here:
+  float* part_o;     // [parts, tokens, heads, head_dim]
+  float* part_lse;   // [parts, heads, tokens]
 };
 
 template <int DP>
@@ -59,6 +62,7 @@ struct Unit {
   int first[2], last[2];     // positions of the tile's rows
   Blocks b[2], all;
   int seen_from, seen_below, seen_first;
+  int part;
   bool any, end;
   int odd;                   // values that are not finite were met
   // Whether all rows of the unit see all keys of a block.
@@ -67,7 +71,8 @@ struct Unit {
 __device__ __forceinline__ Unit unit_of(const Forward& a, int u) {
   const Problem& p = a.p;
   const int rows = a.pair_heads ? kRows : 2 * kRows;
-  const int slots = a.units / a.head_units;
+  const int slots = a.units / a.parts / a.head_units, part = u % a.parts;
+  u /= a.parts;
   const int in = u % a.head_units, slot = slots - 1 - u / a.head_units;   // long rows first
   Unit r;
   r.any = r.end = false;
@@ -81,8 +86,9 @@ __device__ __forceinline__ Unit unit_of(const Forward& a, int u) {
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     if (a.pair_heads) {
-      r.row[t] = row;
-      r.head[t] = 2 * in + t;   // an even number of heads shares keys and values
+      const int pairs = (p.group + 1) / 2, kv = in / pairs, head = 2 * (in - kv * pairs) + t;
+      r.row[t] = head < p.group ? row : r.s.n;   // (of an odd number the last one is alone)
+      r.head[t] = kv * p.group + head;
     } else {
       r.row[t] = row + t * kRows;
       r.head[t] = in;
@@ -90,6 +96,20 @@ __device__ __forceinline__ Unit unit_of(const Forward& a, int u) {
     r.first[t] = r.s.m - r.s.n + r.row[t];
     r.last[t] = min(r.first[t] + kRows, r.s.m) - 1;
     r.b[t] = r.row[t] < r.s.n ? blocks_of(p, r.first[t], r.last[t]) : Blocks{0, 0, 0};
+  }
+  r.part = part;
+  if (a.parts > 1) {
+    // an even share of the blocks from the first one that either tile's last positions see on; the first positions' blocks go with the first share
+    const int lo = r.b[1].hi == 0 ? r.b[0].lo : (r.b[0].hi == 0 ? r.b[1].lo : min(r.b[0].lo, r.b[1].lo)), hi = max(r.b[0].hi, r.b[1].hi), count = hi - lo;
+    const int from = lo + static_cast<int>(static_cast<long long>(count) * part / a.parts), to = lo + static_cast<int>(static_cast<long long>(count) * (part + 1) / a.parts);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      Blocks& b = r.b[t];
+      const int first = max(b.lo, from), last = min(b.hi, to);
+      if (part > 0) b.sink = 0;
+      if (first < last) b = {min(b.sink, first), first, last};
+      else b = {0, 0, b.sink};   // none but the first positions'
+    }
   }
   r.all.hi = max(r.b[0].hi, r.b[1].hi);
   r.all.lo = r.b[1].hi == 0 ? r.b[0].lo : (r.b[0].hi == 0 ? r.b[1].lo : min(r.b[0].lo, r.b[1].lo));
@@ -145,6 +165,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::mbar_init(&looked[i], 1);
     }
     tc::mbar_init(q_empty, 1);
+    tc::tma_prefetch_desc(&tm_q);
+    tc::tma_prefetch_desc(&tm_k);
+    tc::tma_prefetch_desc(&tm_v);
     plan.init(kRoles);
     *bad = 0;
     tc::mbar_init_fence();
@@ -166,7 +189,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 11) {
     // ----------------------------------------------------------------------------------- what comes next ----
     plan.run(s_unit, [&](int id) {
-      zero_outside<typename H::T>(a.o, p.heads * p.head_dim, a.lse, p.heads, p.offsets, p.sequences, p.tokens, id, a.units, lane, 32);
+      if (a.parts == 1) {
+        zero_outside<typename H::T>(a.o, p.heads * p.head_dim, a.lse, p.heads, p.offsets, p.sequences, p.tokens, id, a.units, lane, 32);
+      } else {
+        const int width = p.heads * p.head_dim;   // (of floats: two 16-bit numbers each)
+        for (int i = 0; i < a.parts; ++i)
+          zero_outside<uint16_t>(a.part_o + static_cast<long long>(i) * p.tokens * width, 2 * width, a.part_lse + static_cast<long long>(i) * p.tokens * p.heads, p.heads, p.offsets,
+                                 p.sequences, p.tokens, id, a.units, lane, 32);
+      }
       return unit_of(a, id);
     });
   } else if (warp == 9) {
@@ -351,6 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int pos = u.first[t] + row, first = u.first[t], last = u.last[t];
     const Blocks blocks = u.b[t];
     float m = -INFINITY, l = 0.f;
+    bool sees = false;
     int done = 0;         // blocks so far
     for (int b = blocks.next(-1); b < blocks.hi; b = blocks.next(b), phase ^= 1) {
       ok = wait(&s_full[t], phase, bad);
@@ -366,8 +397,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int c = 0; c < 128; ++c) s[c] = __uint_as_float(r[c / 32][c % 32]);
       }
-      if (!all_seen(p, b, first, last)) {
+      if (all_seen(p, b, first, last)) {
+        sees = true;
+      } else {
         const int high = pos - b * kRows, low = high - p.window, sink = p.sinks - b * kRows;   // columns seen: c <= high and (c > low or c < sink)
+        sees = sees || (high >= 0 && (low < min(high, kRows - 1) || sink > 0));
 #pragma unroll
         for (int c = 0; c < 128; ++c) s[c] = c <= high && (c > low || c < sink) ? s[c] : -INFINITY;
       }
@@ -437,11 +471,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (ok && u.row[t] < u.s.n) {
       const bool mine = u.row[t] + row < u.s.n;
-      // nothing seen: no key up to the position, or none within the window and no first ones
-      const bool none = pos < 0;
+      const bool none = !sees || pos < 0;
       const float inv = none ? 0.f : 1.f / l;
-      if (a.lse != nullptr && mine)
-        a.lse[static_cast<long long>(u.head[t]) * p.tokens + u.s.q0 + u.row[t] + row] = none ? -INFINITY : (m * p.scale_log2 + log2f(l) - Weights<H>::kBias) / kLog2e;
+      float* to_lse = a.parts > 1 ? a.part_lse + static_cast<long long>(u.part) * p.heads * p.tokens : a.lse;
+      if (to_lse != nullptr && mine)
+        to_lse[static_cast<long long>(u.head[t]) * p.tokens + u.s.q0 + u.row[t] + row] = none ? -INFINITY : (m * p.scale_log2 + log2f(l) - Weights<H>::kBias) / kLog2e;
       uint8_t* stage = s_out + warp * 2048;
       const long long o_at = (static_cast<long long>(u.s.q0 + u.row[t] + (warp & 3) * 32) * p.heads + u.head[t]) * p.head_dim;
       const bool odd = *reinterpret_cast<const volatile int*>(&u.odd) != 0;
@@ -468,6 +502,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
+        if (a.parts > 1) {
+          if (mine) {
+            float* to = a.part_o + static_cast<long long>(u.part) * p.tokens * p.heads * p.head_dim + o_at + static_cast<long long>(lane) * p.heads * p.head_dim + c0;
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              if (c0 + e < p.head_dim) *reinterpret_cast<float4*>(to + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+          }
+          continue;
+        }
         const long long stride = static_cast<long long>(p.heads) * p.head_dim;
         const int rows = u.s.n - u.row[t] - (warp & 3) * 32;
         rows_out<H>(stage, f, static_cast<typename H::T*>(a.o) + o_at, stride, rows, c0, p.head_dim);
@@ -491,6 +534,76 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// The parts' results joined: each counts with its share of the sum of exponentials.  Four elements of a head per thread.
+template <typename H>
+__global__ void __launch_bounds__(256) packed_join_kernel(const Forward a) {
+  pdl_wait();
+  pdl_trigger();
+  const Problem& p = a.p;
+  const long long rows = static_cast<long long>(p.tokens) * p.heads;
+  const int lanes = p.head_dim / 4, per_block = 256 / lanes, in = threadIdx.x / lanes, c = threadIdx.x % lanes * 4;
+  if (in >= per_block) return;
+  for (long long r = blockIdx.x * static_cast<long long>(per_block) + in; r < rows; r += static_cast<long long>(gridDim.x) * per_block) {
+    const long long t = r / p.heads;
+    const int h = static_cast<int>(r - t * p.heads);
+    const float* lse = a.part_lse + static_cast<long long>(h) * p.tokens + t;
+    const long long part = static_cast<long long>(p.heads) * p.tokens;
+    float top = -INFINITY;
+    for (int i = 0; i < a.parts; ++i) top = fmaxf(top, lse[i * part]);
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    float whole = 0.f;
+    for (int i = 0; i < a.parts; ++i) {
+      const float l = lse[i * part];
+      // parts that saw nothing are left out; where none saw anything, and where scores were all minus infinity, theirs are the zeros and the NaN
+      if (l == -INFINITY && top != -INFINITY) continue;
+      const float w = top == -INFINITY ? 1.f : exp2f((l - top) * kLog2e);
+      const float4 x = *reinterpret_cast<const float4*>(a.part_o + (i * part + r) * p.head_dim + c);
+      sum.x = fmaf(w, x.x, sum.x), sum.y = fmaf(w, x.y, sum.y), sum.z = fmaf(w, x.z, sum.z), sum.w = fmaf(w, x.w, sum.w);
+      whole += w;
+    }
+    const float inv = 1.f / whole;
+    const float f[4] = {sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv};
+    typename H::T2 out[2] = {H::down(f[0], f[1]), H::down(f[2], f[3])};
+    *reinterpret_cast<uint2*>(static_cast<typename H::T*>(a.o) + r * p.head_dim + c) = *reinterpret_cast<const uint2*>(out);
+    if (a.o_rest != nullptr) {
+      const float2 u = H::up(out[0]), v = H::up(out[1]);
+      typename H::T2 rest[2] = {H::down(f[0] - u.x, f[1] - u.y), H::down(f[2] - v.x, f[3] - v.y)};
+      *reinterpret_cast<uint2*>(static_cast<typename H::T*>(a.o_rest) + r * p.head_dim + c) = *reinterpret_cast<const uint2*>(rest);
+    }
+    if (a.lse != nullptr && c == 0) a.lse[static_cast<long long>(h) * p.tokens + t] = top == -INFINITY ? -INFINITY : top + logf(whole);
+  }
+}
+
+constexpr int kSms = 148;
+// Two heads that share keys and values make a unit, or else 256 rows of one: an odd number of heads leaves one alone, sequences of up to 128 rows the second tile
+// of rows empty.  (8 texts of up to 130 rows behind up to 4096 keys, 12 heads over 4 of 64: 54 us with rows, XX with heads.)
+bool pairs_heads(const PackedAttentionArgs& a) {
+  const int group = a.heads / a.kv_heads;
+  return group % 2 == 0 || (group > 1 && a.tokens / a.sequences <= kRows);
+}
+int head_units_of(const PackedAttentionArgs& a) { return pairs_heads(a) ? a.kv_heads * ((a.heads / a.kv_heads + 1) / 2) : a.heads; }
+long long units_of(const PackedAttentionArgs& a) { return slots_of(a.tokens, a.sequences, pairs_heads(a) ? kRows : 2 * kRows) * head_units_of(a); }
+// How many blocks share out the keys of a unit, by what it costs in microseconds: a step of a unit 2, its beginning and end 5, results in parts 4 and 0.45 per MB (12 heads
+// over 4 of 64, 8 texts of some 100 rows behind 3072 keys: 59 / 43 / 52 / 50 us in 1 / 2 / 3 / 4 parts; 16 heads of 128, 2048 rows: 47 / 61 / 73 / 81; one row over
+// 16384 keys 228 in one, 36 in 16).  The host knows no lengths: an average sequence, whose last tile is half full.
+int parts_of(const PackedAttentionArgs& a) {
+  const int rows = pairs_heads(a) ? kRows : 2 * kRows;
+  const float slots = fminf(static_cast<float>(slots_of(a.tokens, a.sequences, rows)), static_cast<float>(a.tokens) / rows + 0.5f * (a.sequences + 1));
+  const float units = slots * head_units_of(a), megabytes = static_cast<float>(a.tokens) * a.heads * a.head_dim * 4e-6f;
+  if (units >= kSms) return 1;
+  const float steps = fmaxf(1.f, (a.k_tokens - 0.5f * a.tokens) / a.sequences / kRows);
+  int best = 1;
+  float least = INFINITY;
+  for (int parts = 1; parts <= 16 && parts * megabytes <= 64.f; ++parts) {
+    const float cost = fmaxf(1.f, units * parts / kSms + (parts > 1 ? 0.3f : 0.f)) * (2.f * steps / parts + 5.f) + (parts > 1 ? 4.f + 0.45f * parts * megabytes : 0.f);
+    if (cost < least) {
+      least = cost;
+      best = parts;
+    }
+  }
+  return best;
+}
+
 template <typename H, int DP>
 cudaError_t launch(const PackedAttentionArgs& args, cudaStream_t stream) {
   Forward f;
@@ -499,9 +612,12 @@ cudaError_t launch(const PackedAttentionArgs& args, cudaStream_t stream) {
   f.o_rest = args.o_rest;
   f.lse = args.lse;
   f.v = args.v;
-  f.pair_heads = f.p.group % 2 == 0 ? 1 : 0;
-  f.head_units = f.pair_heads ? args.heads / 2 : args.heads;
-  const long long units = slots_of(args.tokens, args.sequences, f.pair_heads ? kRows : 2 * kRows) * f.head_units;
+  f.pair_heads = pairs_heads(args) ? 1 : 0;
+  f.head_units = head_units_of(args);
+  f.parts = args.workspace != nullptr ? parts_of(args) : 1;
+  f.part_o = static_cast<float*>(args.workspace);
+  f.part_lse = f.part_o + static_cast<size_t>(f.parts) * args.tokens * args.heads * args.head_dim;
+  const long long units = units_of(args) * f.parts;
   if (f.p.err == nullptr || units > INT_MAX) return cudaErrorInvalidValue;
   f.units = static_cast<int>(units);
   CUtensorMap q, k, v;
@@ -513,10 +629,22 @@ cudaError_t launch(const PackedAttentionArgs& args, cudaStream_t stream) {
   if (rc != cudaSuccess) return rc;
   MCCL_LAUNCH_PDL((packed_attention_kernel<H, DP>), f.units, kThreads, smem_bytes<DP>(), stream, q, k, v, f);
   count_launch();
+  if (f.parts > 1) {
+    const int per_block = 256 / (args.head_dim / 4);
+    const long long blocks = (static_cast<long long>(args.tokens) * args.heads + per_block - 1) / per_block;
+    MCCL_LAUNCH_PDL(packed_join_kernel<H>, static_cast<int>(blocks < 16 * kSms ? blocks : 16 * kSms), 256, 0, stream, f);
+    count_launch();
+  }
   return ::mccl::launch_status();
 }
 
 }  // namespace
+
+size_t packed_attention_workspace(const PackedAttentionArgs& a) {
+  if (a.tokens <= 0 || a.heads <= 0 || a.sequences <= 0) return 0;
+  const int parts = parts_of(a);
+  return parts == 1 ? 0 : static_cast<size_t>(parts) * a.tokens * a.heads * (a.head_dim + 1) * sizeof(float);
+}
 
 cudaError_t packed_attention(const PackedAttentionArgs& a, cudaStream_t stream) {
   if (a.tokens <= 0 || a.heads <= 0) return cudaSuccess;

@@ -106,6 +106,35 @@ def test_keys_from_before(heads, kv_heads, dim, window, sinks):
     check(*make([1, 130, 64, 0, 257], heads, kv_heads, dim, before=[900, 77, 128, 40, 0], seed=3), window=window, sinks=sinks)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (1500, 0), (1500, 9), (3, 300)])
+@pytest.mark.parametrize("lengths,before,heads,kv_heads,dim", [([1], [5000], 3, 1, 128), ([37, 0, 130], [3000, 10, 2500], 4, 2, 64), ([2100], None, 2, 2, 72), ([200], [1100], 8, 8, 32)])
+def test_few_rows_over_many_keys(lengths, before, heads, kv_heads, dim, window, sinks, dtype):
+    """Keys are shared out over several blocks and their results joined."""
+    check(*make(lengths, heads, kv_heads, dim, dtype, before=before, begin=3, spare=5, seed=8), window=window, sinks=sinks)
+
+
+def test_infinite_numbers_where_keys_are_shared_out():
+    q, k, v, offsets, k_offsets = make([30, 20], 2, 2, 64, before=[2500, 1800], seed=6)
+    good = ops.packed_attention(q, k, v, offsets, k_offsets)
+    bad_v, bad_k = v.clone(), k.clone()
+    bad_v[2520, 0, 5] = math.inf       # the 21st new position of the first text, ...
+    bad_k[2520, 1, 7] = math.nan
+    bad_v[2530 + 7, 1, 3] = math.nan   # ... and an early one of the second
+    o = ops.packed_attention(q, bad_k, bad_v, offsets, k_offsets)
+    assert torch.equal(o[:20], good[:20]) and torch.equal(o[30:, 0], good[30:, 0])
+    assert not torch.isfinite(o[20:30, 0, 5]).any() and torch.isnan(o[20:30, 1]).all() and torch.isnan(o[30:, 1, 3]).all()
+    keep = torch.arange(64, device="cuda")
+    assert torch.equal(o[20:30, 0][:, keep != 5], good[20:30, 0][:, keep != 5]) and torch.equal(o[30:, 1][:, keep != 3], good[30:, 1][:, keep != 3])
+    # scores that are all minus infinity have no softmax; where some are finite, those count
+    low_k = k.clone()
+    low_k[:2530] = -math.inf
+    assert torch.isnan(ops.packed_attention(q.abs() + 0.1, low_k, v, offsets, k_offsets)[:30]).all()
+    low_k[2529] = k[2529]
+    o = ops.packed_attention(q.abs() + 0.1, low_k, v, offsets, k_offsets)
+    assert torch.isnan(o[:29]).all() and torch.allclose(o[29].float(), v[2529].float(), rtol=2 ** -7)
+
+
 def test_more_queries_than_keys():
     # the first 60, 300 and all of the queries stand in front of their first key
     o = check(*make([100, 500, 70], 4, 2, 64, before=[-60, -300, -70]))

@@ -95,6 +95,12 @@ def test_keys_from_before(heads, kv_heads, dim, window, sinks):
     check(*make([1, 130, 64, 0, 257], heads, kv_heads, dim, before=[900, 77, 128, 40, 0], seed=3), window=window, sinks=sinks)
 
 
+def test_few_rows_over_many_keys():
+    """The forward pass shares the keys out there."""
+    check(*make([37, 130], 4, 2, 64, before=[3000, 2500], begin=3, spare=5, seed=8))
+    check(*make([2100], 2, 2, 128, seed=9), window=1500, sinks=9)
+
+
 def test_more_queries_than_keys():
     dq, _, _ = check(*make([100, 500, 70], 4, 2, 64, before=[-60, -300, -70]))
     assert not dq[:60].any() and not dq[100:400].any() and not dq[600:].any()
