@@ -25,7 +25,6 @@ constexpr int kThreads = 12 * 32;          // warps 0-3 and 4-7: rows of tiles 0
 // A row's scores need more registers than an even share: 256 x 208 + 128 x 80 of the launch's 384 x 168.
 constexpr int kRowRegisters = 208, kOtherRegisters = 80;
 constexpr int kRoles = 8 + 3;              // warps that take a unit from the planning one
-constexpr int kStage = 8 * 2048;           // results on their way out, 32 rows x 64 bytes per warp
 
 struct Forward {
   Problem p;
@@ -42,7 +41,7 @@ struct Forward {
 };
 
 template <int DP>
-constexpr int smem_bytes() { return (2 + 2 * kStages) * (DP / 64) * kSub + kStage + 512 + 1024; }
+constexpr int smem_bytes() { return (2 + 2 * kStages) * (DP / 64) * kSub + 8 * kOut + 512 + 1024; }
 
 // Weights are kept 2^kBias times larger in fp16, whose smallest normal number is 2^-14; the running maximum may be exceeded by 2^kSlack before sums are
 // rescaled (exact in fp32 either way), so that the largest weight is 2^8 in bf16 and 2^15 in fp16.
@@ -123,17 +122,34 @@ __device__ __forceinline__ Unit unit_of(const Forward& a, int u) {
   return r;
 }
 
+// The columns, of 64 from c0 on, in which a value that a row sees in one of the blocks that were looked at is not finite.
+template <typename H>
+__device__ __noinline__ unsigned long long odd_columns(const Problem& p, const TokenView& v, const Unit& u, const Blocks& blocks, int pos, int c0) {
+  unsigned long long marks = 0;
+  const typename H::T* from = static_cast<const typename H::T*>(v.p) + u.head[0] / p.group * v.head + static_cast<long long>(u.s.k0) * v.token + c0;
+  for (int b = blocks.next(-1); b < blocks.hi; b = blocks.next(b)) {
+    if (u.whole(b)) continue;
+    for (int j = b * kRows; j < min(b * kRows + kRows, pos + 1); ++j) {
+      if (j <= pos - p.window && j >= p.sinks) continue;
+      for (int e = 0; e < 64 && c0 + e < p.head_dim; ++e)
+        if (!(fabsf(H::up(from[j * v.token + e])) < INFINITY)) marks |= 1ull << e;
+    }
+  }
+  return marks;
+}
+
 template <typename H, int DP>
 __global__ void __launch_bounds__(kThreads, 1)
-    packed_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Forward a) {
+    packed_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                            const __grid_constant__ CUtensorMap tm_o, const __grid_constant__ CUtensorMap tm_rest, const Forward a) {
   constexpr int kTile = (DP / 64) * kSub;
   constexpr uint32_t kP = DP == 64 ? 384 : 0, kPStep = DP == 64 ? 64 : 128;   // columns of the weights
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* s_q = smem;                        // [2] tiles
   uint8_t* s_kv = s_q + 2 * kTile;            // [kStages][2] tiles: values, keys
-  uint8_t* s_out = s_kv + 2 * kStages * kTile;
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(s_out + kStage);   // [2]
+  uint8_t* s_out = s_kv + 2 * kStages * kTile;   // a warp's rows on their way out
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(s_out + 8 * kOut);   // [2]
   uint64_t* kv_full = q_full + 2;             // [kStages]
   uint64_t* kv_empty = kv_full + kStages;     // [kStages]
   uint64_t* raw_full = kv_empty + kStages;    // [kStages]: values that are looked at before they are used are here, ...
@@ -168,6 +184,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc::tma_prefetch_desc(&tm_q);
     tc::tma_prefetch_desc(&tm_k);
     tc::tma_prefetch_desc(&tm_v);
+    tc::tma_prefetch_desc(&tm_o);
     plan.init(kRoles);
     *bad = 0;
     tc::mbar_init_fence();
@@ -476,54 +493,43 @@ __global__ void __launch_bounds__(kThreads, 1)
       float* to_lse = a.parts > 1 ? a.part_lse + static_cast<long long>(u.part) * p.heads * p.tokens : a.lse;
       if (to_lse != nullptr && mine)
         to_lse[static_cast<long long>(u.head[t]) * p.tokens + u.s.q0 + u.row[t] + row] = none ? -INFINITY : (m * p.scale_log2 + log2f(l) - Weights<H>::kBias) / kLog2e;
-      uint8_t* stage = s_out + warp * 2048;
-      const long long o_at = (static_cast<long long>(u.s.q0 + u.row[t] + (warp & 3) * 32) * p.heads + u.head[t]) * p.head_dim;
+      const int first_row = u.s.q0 + u.row[t] + (warp & 3) * 32, rows = u.s.n - u.row[t] - (warp & 3) * 32, head = u.head[t];
       const bool odd = *reinterpret_cast<const volatile int*>(&u.odd) != 0;
-      const int kv = u.head[t] / p.group;
-      for (int c0 = 0; c0 < p.head_dim; c0 += 32) {
-        uint32_t o[32] = {};
+#pragma unroll 1
+      for (int c0 = 0; c0 < p.head_dim; c0 += 64) {
+        uint32_t o[2][32] = {};
         if (done > 0) {
-          tc::tmem_ld_32x32(t_o + c0, o);
+          tc::tmem_ld_32x32(t_o + c0, o[0]);
+          tc::tmem_ld_32x32(t_o + c0 + 32, o[1]);
           tc::tmem_ld_wait();
         }
-        float f[32];
+        float f[64];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) f[e] = none ? 0.f : __uint_as_float(o[e]) * inv;
+        for (int e = 0; e < 64; ++e) f[e] = none ? 0.f : __uint_as_float(o[e / 32][e % 32]) * inv;
         if (odd) {
-          // values that are not finite in blocks that were looked at, seen by this row
-          const typename H::T* v = static_cast<const typename H::T*>(a.v.p) + kv * a.v.head + static_cast<long long>(u.s.k0) * a.v.token + c0;
-          for (int b = blocks.next(-1); b < blocks.hi; b = blocks.next(b)) {
-            if (u.whole(b)) continue;
-            for (int j = b * kRows; j < min(b * kRows + kRows, pos + 1); ++j) {
-              if (j <= pos - p.window && j >= p.sinks) continue;
+          const unsigned long long marks = odd_columns<H>(p, a.v, u, blocks, pos, c0);
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (c0 + e < p.head_dim && !(fabsf(H::up(v[j * a.v.token + e])) < INFINITY)) f[e] = NAN;
-            }
-          }
+          for (int e = 0; e < 64; ++e) f[e] = (marks >> e) & 1 ? NAN : f[e];
         }
         if (a.parts > 1) {
-          if (mine) {
-            float* to = a.part_o + static_cast<long long>(u.part) * p.tokens * p.heads * p.head_dim + o_at + static_cast<long long>(lane) * p.heads * p.head_dim + c0;
+          float* to = a.part_o + ((static_cast<long long>(u.part) * p.tokens + first_row + lane) * p.heads + head) * p.head_dim + c0;
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              if (c0 + e < p.head_dim) *reinterpret_cast<float4*>(to + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
-          }
+          for (int e = 0; e < 64; e += 4)
+            if (mine && c0 + e < p.head_dim) *reinterpret_cast<float4*>(to + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
           continue;
         }
-        const long long stride = static_cast<long long>(p.heads) * p.head_dim;
-        const int rows = u.s.n - u.row[t] - (warp & 3) * 32;
-        rows_out<H>(stage, f, static_cast<typename H::T*>(a.o) + o_at, stride, rows, c0, p.head_dim);
+        rows_out<H>(s_out + warp * kOut, &tm_o, f, a.o, p.heads, p.head_dim, head, first_row, rows, c0);
         if (a.o_rest != nullptr) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) f[e] -= H::up(H::down(f[e]));
-          rows_out<H>(stage, f, static_cast<typename H::T*>(a.o_rest) + o_at, stride, rows, c0, p.head_dim);
+          for (int e = 0; e < 64; ++e) f[e] -= H::up(H::down(f[e]));
+          rows_out<H>(s_out + warp * kOut, &tm_rest, f, a.o_rest, p.heads, p.head_dim, head, first_row, rows, c0);
         }
       }
     }
     tc::fence_before_sync();   // the next unit's first product with V writes O
     plan.give_back(k);
     }
+    rows_sent();
     tc::fence_before_sync();
   }
   __syncthreads();
@@ -620,14 +626,15 @@ cudaError_t launch(const PackedAttentionArgs& args, cudaStream_t stream) {
   const long long units = units_of(args) * f.parts;
   if (f.p.err == nullptr || units > INT_MAX) return cudaErrorInvalidValue;
   f.units = static_cast<int>(units);
-  CUtensorMap q, k, v;
+  CUtensorMap q, k, v, o, rest = {};
   if (!encode_rows(&q, args.type, args.q, args.tokens, args.heads, args.head_dim) || !encode_rows(&k, args.type, args.k, args.k_tokens, args.kv_heads, args.head_dim) ||
-      !encode_rows(&v, args.type, args.v, args.k_tokens, args.kv_heads, args.head_dim))
+      !encode_rows(&v, args.type, args.v, args.k_tokens, args.kv_heads, args.head_dim) || !encode_result(&o, args.type, args.o, args.tokens, args.heads, args.head_dim) ||
+      (args.o_rest != nullptr && !encode_result(&rest, args.type, args.o_rest, args.tokens, args.heads, args.head_dim)))
     return cudaErrorInvalidValue;
   static std::atomic<uint64_t> allowed{0};
   const cudaError_t rc = raise_smem_limit(packed_attention_kernel<H, DP>, smem_bytes<DP>(), allowed);
   if (rc != cudaSuccess) return rc;
-  MCCL_LAUNCH_PDL((packed_attention_kernel<H, DP>), f.units, kThreads, smem_bytes<DP>(), stream, q, k, v, f);
+  MCCL_LAUNCH_PDL((packed_attention_kernel<H, DP>), f.units, kThreads, smem_bytes<DP>(), stream, q, k, v, o, rest, f);
   count_launch();
   if (f.parts > 1) {
     const int per_block = 256 / (args.head_dim / 4);

@@ -28,7 +28,6 @@ constexpr int kThreads = 12 * 32;   // warps 0-3 and 4-7: rows, half of the colu
 // 256 x 208 + 128 x 80 of the launch's 384 x 168 registers.
 constexpr int kRowRegisters = 208, kOtherRegisters = 80;
 constexpr int kRoles = 8 + 3;       // warps that take a unit from the planning one
-constexpr int kStage = 8 * 2048;    // results on their way out, 32 rows x 64 bytes per warp
 
 // Where the 16-bit weights (or score gradients) of a tile are in tensor memory: in columns of their own where head_dim leaves room, otherwise in those of the scores,
 // each half of the threads in its own.  In the latter case the next scores are written behind the product that reads them: products of one shape, here 128 x 128
@@ -127,21 +126,20 @@ __device__ __forceinline__ KeyUnit key_unit(const Grad& a, int u) {
 }
 
 template <int DP>
-constexpr int key_smem() { return 6 * (DP / 64) * kSub + kStage + 2 * 2 * kRows * 4 + 512 + 1024; }
+constexpr int key_smem() { return 6 * (DP / 64) * kSub + 8 * kOut + 2 * 2 * kRows * 4 + 512; }
 
 template <int DP>
 __global__ void __launch_bounds__(kThreads, 1)
     packed_grad_keys_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                            const __grid_constant__ CUtensorMap tm_do, const Grad a) {
+                            const __grid_constant__ CUtensorMap tm_do, const __grid_constant__ CUtensorMap tm_out, const __grid_constant__ CUtensorMap tm_out2, const Grad a) {
   constexpr int kTile = (DP / 64) * kSub;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* s_k = smem;
+  extern __shared__ __align__(1024) uint8_t smem_aligned[];   // (no room to move the beginning: all but 512 bytes are in use)
+  uint8_t* s_k = smem_aligned;
   uint8_t* s_v = s_k + kTile;
   uint8_t* s_q = s_v + kTile;        // [2]
   uint8_t* s_do = s_q + 2 * kTile;   // [2]
-  uint8_t* s_out = s_do + 2 * kTile;
-  float* s_lse = reinterpret_cast<float*>(s_out + kStage);   // [2][128], times log2 e
+  uint8_t* s_out = s_do + 2 * kTile;   // a warp's rows on their way out
+  float* s_lse = reinterpret_cast<float*>(s_out + 8 * kOut);   // [2][128], times log2 e
   float* s_delta = s_lse + 2 * kRows;                        // [2][128]
   uint64_t* k_full = reinterpret_cast<uint64_t*>(s_delta + 2 * kRows);
   uint64_t* v_full = k_full + 1;
@@ -455,22 +453,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok) {   // one half takes dV out, the other dK
         const uint32_t from = (half == 0 ? t_dv : t_dk) + lanes;
         const float scale = half == 0 ? 1.f : p.scale;
-        const long long stride = static_cast<long long>(p.kv_heads) * p.head_dim;
         const int first_row = first_key + (warp & 3) * 32;
-        H::T* to = static_cast<H::T*>(half == 0 ? a.dv : a.dk) + (u.s.k0 + first_row) * stride + u.kv * p.head_dim;
-        for (int c0 = 0; c0 < p.head_dim; c0 += 32) {
-          uint32_t r[32];
-          tc::tmem_ld_32x32(from + c0, r);
+#pragma unroll 1
+        for (int c0 = 0; c0 < p.head_dim; c0 += 64) {
+          uint32_t r[2][32];
+          tc::tmem_ld_32x32(from + c0, r[0]);
+          tc::tmem_ld_32x32(from + c0 + 32, r[1]);
           tc::tmem_ld_wait();
-          float f[32];
+          float f[64];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) f[e] = __uint_as_float(r[e]) * scale;
-          rows_out<H>(s_out + warp * 2048, f, to, stride, u.s.m - first_row, c0, p.head_dim);
+          for (int e = 0; e < 64; ++e) f[e] = __uint_as_float(r[e / 32][e % 32]) * scale;
+          rows_out<H>(s_out + warp * kOut, half == 0 ? &tm_out2 : &tm_out, f, half == 0 ? a.dv : a.dk, p.kv_heads, p.head_dim, u.kv, u.s.k0 + first_row, u.s.m - first_row, c0);
         }
       }
       tc::fence_before_sync();   // the next unit's first products overwrite the sums
       plan.give_back(k);
     }
+    rows_sent();
     tc::fence_before_sync();
   }
   __syncthreads();
@@ -512,13 +511,15 @@ __device__ __forceinline__ QueryUnit query_unit(const Grad& a, int u) {
   return r;
 }
 
+static_assert(key_smem<128>() <= 227 * 1024, "shared memory of a block");
+
 template <int DP>
-constexpr int query_smem() { return 6 * (DP / 64) * kSub + kStage + 512 + 1024; }
+constexpr int query_smem() { return 6 * (DP / 64) * kSub + 8 * kOut + 512 + 1024; }
 
 template <int DP>
 __global__ void __launch_bounds__(kThreads, 1)
     packed_grad_queries_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                               const __grid_constant__ CUtensorMap tm_do, const Grad a) {
+                               const __grid_constant__ CUtensorMap tm_do, const __grid_constant__ CUtensorMap tm_out, const Grad a) {
   constexpr int kTile = (DP / 64) * kSub;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -526,8 +527,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* s_do = s_q + kTile;
   uint8_t* s_k = s_do + kTile;      // [2]
   uint8_t* s_v = s_k + 2 * kTile;   // [2]
-  uint8_t* s_out = s_v + 2 * kTile;
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(s_out + kStage);
+  uint8_t* s_out = s_v + 2 * kTile;   // a warp's rows on their way out
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(s_out + 8 * kOut);
   uint64_t* do_full = q_full + 1;
   uint64_t* q_empty = do_full + 1;  // the unit's last products are done: so are its sums
   uint64_t* raw = q_empty + 1;      // [2]: keys of a block that ends behind the sequence: here, to be cleared there
@@ -757,22 +758,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::fence_after_sync();
       }
       if (ok) {   // each half takes half of the columns out
-        const long long stride = static_cast<long long>(p.heads) * p.head_dim;
-        const int first_row = u.row + (warp & 3) * 32;
-        H::T* to = static_cast<H::T*>(a.dq) + (u.s.q0 + first_row) * stride + u.head * p.head_dim;
-        for (int c0 = half * 32; c0 < p.head_dim; c0 += 64) {
-          uint32_t r[32];
-          tc::tmem_ld_32x32(t_dq + lanes + c0, r);
+        const int first_row = u.row + (warp & 3) * 32, c0 = 64 * half;
+        if (c0 < p.head_dim) {
+          uint32_t r[2][32];
+          tc::tmem_ld_32x32(t_dq + lanes + c0, r[0]);
+          tc::tmem_ld_32x32(t_dq + lanes + c0 + 32, r[1]);
           tc::tmem_ld_wait();
-          float f[32];
+          float f[64];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) f[e] = pos < 0 ? 0.f : __uint_as_float(r[e]) * p.scale;
-          rows_out<H>(s_out + warp * 2048, f, to, stride, u.s.n - first_row, c0, p.head_dim);
+          for (int e = 0; e < 64; ++e) f[e] = pos < 0 ? 0.f : __uint_as_float(r[e / 32][e % 32]) * p.scale;
+          rows_out<H>(s_out + warp * kOut, &tm_out, f, a.dq, p.heads, p.head_dim, u.head, u.s.q0 + first_row, u.s.n - first_row, c0);
         }
       }
       tc::fence_before_sync();   // the next unit's first products overwrite the sums
       plan.give_back(k);
     }
+    rows_sent();
     tc::fence_before_sync();
   }
   __syncthreads();
@@ -795,9 +796,11 @@ cudaError_t launch(const PackedAttentionGradArgs& args, cudaStream_t stream) {
   g.dv = args.dv;
   const long long keys = slots_of(f.k_tokens, f.sequences, kRows) * f.kv_heads, queries = slots_of(f.tokens, f.sequences, kRows) * f.heads;
   if (g.p.err == nullptr || keys > INT_MAX || queries > INT_MAX) return cudaErrorInvalidValue;
-  CUtensorMap q, k, v, d_o;
+  CUtensorMap q, k, v, d_o, dq, dk, dv;
   if (!encode_rows(&q, f.type, f.q, f.tokens, f.heads, f.head_dim) || !encode_rows(&k, f.type, f.k, f.k_tokens, f.kv_heads, f.head_dim) ||
-      !encode_rows(&v, f.type, f.v, f.k_tokens, f.kv_heads, f.head_dim) || !encode_rows(&d_o, f.type, args.d_o, f.tokens, f.heads, f.head_dim))
+      !encode_rows(&v, f.type, f.v, f.k_tokens, f.kv_heads, f.head_dim) || !encode_rows(&d_o, f.type, args.d_o, f.tokens, f.heads, f.head_dim) ||
+      !encode_result(&dq, f.type, args.dq, f.tokens, f.heads, f.head_dim) || !encode_result(&dk, f.type, args.dk, f.k_tokens, f.kv_heads, f.head_dim) ||
+      !encode_result(&dv, f.type, args.dv, f.k_tokens, f.kv_heads, f.head_dim))
     return cudaErrorInvalidValue;
   static std::atomic<uint64_t> allowed_keys{0}, allowed_queries{0};
   cudaError_t rc = raise_smem_limit(packed_grad_keys_kernel<DP>, key_smem<DP>(), allowed_keys);
@@ -806,9 +809,9 @@ cudaError_t launch(const PackedAttentionGradArgs& args, cudaStream_t stream) {
   MCCL_LAUNCH_PDL(packed_delta_kernel<DP / 8>, dim3((f.tokens + 31) / 32, (f.heads + 7) / 8), 256, 0, stream, static_cast<const H::T*>(f.o),
                   static_cast<const H::T*>(f.o_rest), args.d_o, args.delta, f.tokens, f.heads, f.head_dim);
   g.units = static_cast<int>(keys);
-  MCCL_LAUNCH_PDL(packed_grad_keys_kernel<DP>, g.units, kThreads, key_smem<DP>(), stream, q, k, v, d_o, g);
+  MCCL_LAUNCH_PDL(packed_grad_keys_kernel<DP>, g.units, kThreads, key_smem<DP>(), stream, q, k, v, d_o, dk, dv, g);
   g.units = static_cast<int>(queries);
-  MCCL_LAUNCH_PDL(packed_grad_queries_kernel<DP>, g.units, kThreads, query_smem<DP>(), stream, q, k, v, d_o, g);
+  MCCL_LAUNCH_PDL(packed_grad_queries_kernel<DP>, g.units, kThreads, query_smem<DP>(), stream, q, k, v, d_o, dq, g);
   count_launch(3);
   return ::mccl::launch_status();
 }

@@ -175,24 +175,44 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// 32 rows (a lane's each) of 32 columns from c0 on leave through 2 KB of the warp's own: 64 bytes of a row from four neighbouring lanes.  `rows` of them exist.
+// A warp's 32 rows (a lane's each) of 64 columns from c0 on leave through 4 KB of its own as one TMA store (rows from `row` on of `head`; columns behind head_dim are
+// cut off), or, where not all of the rows are the sequence's, row by row.  f: this lane's columns.  (Stores of registers, each lane to a row of its own, and stores
+// through shared memory, four lanes to a row, both took a tile of 128 columns some 5000 clocks.)
+constexpr int kOut = 4096;
 template <typename H>
-__device__ __forceinline__ void rows_out(uint8_t* stage, const float (&f)[32], typename H::T* to, long long stride, int rows, int c0, int head_dim) {
+__device__ __forceinline__ void rows_out(uint8_t* stage, const CUtensorMap* map, const float (&f)[64], void* base, int heads, int head_dim, int head, int row, int rows, int c0) {
   const int lane = threadIdx.x & 31;
+  uint4 x[8];
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    uint4 raw;
-    typename H::T2* h = reinterpret_cast<typename H::T2*>(&raw);
+  for (int c = 0; c < 8; ++c) {
+    typename H::T2* h = reinterpret_cast<typename H::T2*>(&x[c]);
 #pragma unroll
     for (int e = 0; e < 4; ++e) h[e] = H::down(f[8 * c + 2 * e], f[8 * c + 2 * e + 1]);
-    *reinterpret_cast<uint4*>(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = raw;
   }
+  if (rows < 32) {
+    typename H::T* to = static_cast<typename H::T*>(base) + (static_cast<long long>(row + lane) * heads + head) * head_dim + c0;
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (lane < rows && c0 + 8 * c < head_dim) *reinterpret_cast<uint4*>(to + 8 * c) = x[c];
+    return;
+  }
+  if (tc::elect_one()) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // what was here before has been read
   __syncwarp();
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = i * 8 + (lane >> 2), c = lane & 3;
-    if (r < rows && c0 + c * 8 < head_dim) *reinterpret_cast<uint4*>(to + r * stride + c0 + c * 8) = *reinterpret_cast<const uint4*>(stage + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+  for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(stage + sw128(lane, c)) = x[c];
+  fence_async_smem();
+  __syncwarp();
+  if (tc::elect_one()) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(tc::smem_u32(stage)), "r"(c0), "r"(head),
+                 "r"(row)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
   }
+  __syncwarp();
+}
+// The thread that sent a warp's rows waits until they have been read; by the whole warp, before the block retires.
+__device__ __forceinline__ void rows_sent() {
+  if (tc::elect_one()) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   __syncwarp();
 }
 
@@ -351,16 +371,21 @@ struct Plan {
   }
 };
 
-// [tokens, heads, head_dim] as boxes of 64 columns of 128 rows of a head.  (The stride of a dimension of one is never used and may be anything.)
-inline bool encode_rows(CUtensorMap* map, Half16 type, const TokenView& t, int tokens, int heads, int head_dim) {
+// [tokens, heads, head_dim] as boxes of 64 columns of `rows` rows of a head.  (The stride of a dimension of one is never used and may be anything.)
+inline bool encode_rows(CUtensorMap* map, Half16 type, const TokenView& t, int tokens, int heads, int head_dim, int rows = kRows) {
   const CuDriver& cu = CuDriver::get();
   if (!cu.loaded || !cu.TensorMapEncodeTiled) return false;
   const cuuint64_t size[3] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens)};
   const cuuint64_t strides[2] = {static_cast<cuuint64_t>((heads > 1 ? t.head : head_dim) * 2), static_cast<cuuint64_t>((tokens > 1 ? t.token : head_dim) * 2)};
-  const cuuint32_t box[3] = {64, 1, kRows}, step[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {64, 1, static_cast<cuuint32_t>(rows)}, step[3] = {1, 1, 1};
   return cu.TensorMapEncodeTiled(map, type == Half16::bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(t.p), size,
                                  strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// A contiguous result, as the 32 rows that a warp stores.
+inline bool encode_result(CUtensorMap* map, Half16 type, const void* p, int tokens, int heads, int head_dim) {
+  return encode_rows(map, type, {p, static_cast<long long>(heads) * head_dim, head_dim}, tokens, heads, head_dim, 32);
 }
 
 }  // namespace packed
