@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) break;
             if (more && mine.has(b)) {
               tc::fence_after_sync();
-              mma_rows(tmem + t * 128, s_q + t * kTile, s_kv + (2 * st + 1) * kTile, idesc_s, steps);
+              mma_rows<DP>(tmem + t * 128, s_q + t * kTile, s_kv + (2 * st + 1) * kTile, idesc_s, steps);
               tc::mma_commit(&s_full[t]);
             }
             if (before >= 0 && mine.has(before)) tc::mma_commit(&o_full[t]);

@@ -301,12 +301,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (tc::elect_one()) {
           ok = wait(k_full, k & 1, bad) && wait(&q_full[n & 1], (n / 2) & 1, bad);
           if (ok) {
-            mma_rows(t_s, s_k, s_q + (n & 1) * kTile, idesc_s, steps);
+            mma_rows<DP>(t_s, s_k, s_q + (n & 1) * kTile, idesc_s, steps);
             tc::mma_commit(&s_full[n & 1]);
             ok = wait(v_full, k & 1, bad) && wait(&do_full[n & 1], (n / 2) & 1, bad);
           }
           if (ok) {
-            mma_rows(t_dp, s_v, s_do + (n & 1) * kTile, idesc_s, steps);
+            mma_rows<DP>(t_dp, s_v, s_do + (n & 1) * kTile, idesc_s, steps);
             tc::mma_commit(dp_full);
           }
           for (int i = 0; i < items && ok; ++i, ++n) {
@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (ok && more) ok = wait(&q_full[next], ((n + 1) / 2) & 1, bad);
             if (!ok) break;
             if (more) {
-              mma_rows(t_s, s_k, s_q + next * kTile, idesc_s, steps);
+              mma_rows<DP>(t_s, s_k, s_q + next * kTile, idesc_s, steps);
               tc::mma_commit(&s_full[next]);
             }
 #pragma unroll 1
@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (ok && more) ok = wait(&do_full[next], ((n + 1) / 2) & 1, bad);
             if (!ok) break;
             if (more) {
-              mma_rows(t_dp, s_v, s_do + next * kTile, idesc_s, steps);
+              mma_rows<DP>(t_dp, s_v, s_do + next * kTile, idesc_s, steps);
               tc::mma_commit(dp_full);
             } else {
               tc::mma_commit(kv_empty);
@@ -649,7 +649,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           auto scores = [&](int n) {
             ok = ok && wait(&k_full[n & 1], (n / 2) & 1, bad);
             if (!ok) return;
-            mma_rows(tmem + (n & 1) * 128, s_q, s_k + (n & 1) * kTile, idesc_s, steps);
+            mma_rows<DP>(tmem + (n & 1) * 128, s_q, s_k + (n & 1) * kTile, idesc_s, steps);
             tc::mma_commit(&s_full[n & 1]);
           };
           ok = wait(q_full, k & 1, bad);
@@ -663,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = wait(&v_full[st], (n / 2) & 1, bad);
             if (!ok) break;
             tc::fence_after_sync();
-            mma_rows(t_dp, s_do, s_v + st * kTile, idesc_s, steps);
+            mma_rows<DP>(t_dp, s_do, s_v + st * kTile, idesc_s, steps);
             tc::mma_commit(dp_full);
             tc::mma_commit(&v_empty[st]);
             if (more) scores(n + 1);

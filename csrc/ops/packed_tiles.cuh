@@ -112,23 +112,38 @@ __host__ __device__ constexpr uint32_t idesc16(int m, int n, bool a_mn, bool b_m
   return (1u << 4) | (type << 7) | (type << 10) | (a_mn ? (1u << 15) : 0u) | (b_mn ? (1u << 16) : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
          (static_cast<uint32_t>(m >> 4) << 24);
 }
-// D[tmem] (+)= A[tmem] B[smem]; issued by one thread.
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t desc_b, uint32_t idesc, bool accumulate) {
-  const uint32_t acc = accumulate ? 1u : 0u;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(d), "r"(a), "l"(desc_b), "r"(idesc), "r"(acc)
-      : "memory");
+// D[tmem] (+)= A B[smem]; issued by one thread.  A in tensor memory or (a descriptor) in shared memory.  Adding is told apart from overwriting while compiling where it can
+// be: every instruction of that thread counts.
+__device__ __forceinline__ void mma_add(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.eq.u32 p, 0, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc) : "memory");
 }
-// Products over K-major tiles: D[128 x 128 keys] = A B^T over `steps` steps of 16 columns.
+__device__ __forceinline__ void mma_add(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.eq.u32 p, 0, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc) : "memory");
+}
+__device__ __forceinline__ void mma_new(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, 0, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc) : "memory");
+}
+__device__ __forceinline__ void mma_either(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+               : "memory");
+}
+// Products over K-major tiles: D[128 x 128 keys] = A B^T over `steps` steps of 16 columns (all DP columns, where they are that many, without counting).
+template <int DP>
 __device__ __forceinline__ void mma_rows(uint32_t d, const uint8_t* a, const uint8_t* b, uint32_t idesc, int steps) {
   const uint64_t da = tc::smem_desc_k_sw128(a), db = tc::smem_desc_k_sw128(b);
-#pragma unroll 4
-  for (int k = 0; k < steps; ++k) {
-    const uint64_t off = static_cast<uint64_t>((k >> 2) * (kSub >> 4) + (k & 3) * 2);
-    tc::mma_bf16(d, da + off, db + off, idesc, k != 0);
+  if (steps == DP / 16) {
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k) {
+      const uint64_t off = static_cast<uint64_t>((k >> 2) * (kSub >> 4) + (k & 3) * 2);
+      k == 0 ? mma_new(d, da, db, idesc) : mma_add(d, da + off, db + off, idesc);
+    }
+  } else {
+#pragma unroll 1
+    for (int k = 0; k < steps; ++k) {
+      const uint64_t off = static_cast<uint64_t>((k >> 2) * (kSub >> 4) + (k & 3) * 2);
+      k == 0 ? mma_new(d, da, db, idesc) : mma_add(d, da + off, db + off, idesc);
+    }
   }
 }
 // D[128 x n] (+)= A[tmem, 128 x kKeys] B with B's rows along the sum: kKeys rows of a tile.  A's second 64 columns are `kApart` columns behind the first.
@@ -136,7 +151,10 @@ template <int kKeys, int kApart = 0>
 __device__ __forceinline__ void mma_weights(uint32_t d, uint32_t a, const uint8_t* b, uint32_t idesc, bool accumulate) {
   const uint64_t db = tc::smem_desc_mn_sw128(b, kSub);
 #pragma unroll
-  for (int k = 0; k < kKeys / 16; ++k) mma_ts(d, a + (k >> 2) * kApart + 8 * (k & 3), db + 128 * k, idesc, k != 0 || accumulate);
+  for (int k = 0; k < kKeys / 16; ++k) {
+    const uint32_t at = a + (k >> 2) * kApart + 8 * (k & 3);
+    k == 0 ? mma_either(d, at, db, idesc, accumulate) : mma_add(d, at, db + 128 * k, idesc);
+  }
 }
 
 // The same with A and B in halves: of each 64 columns (two times, `kApart` columns of tensor memory apart) the 32 from 32 h on.
@@ -146,7 +164,8 @@ __device__ __forceinline__ void mma_half(uint32_t d, uint32_t a, const uint8_t* 
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int w = i >> 1, k = 4 * w + 2 * h + (i & 1);
-    mma_ts(d, a + w * kApart + 8 * (k & 3), db + 128 * k, idesc, i != 0 || accumulate);
+    const uint32_t at = a + w * kApart + 8 * (k & 3);
+    i == 0 ? mma_either(d, at, db + 128 * k, idesc, accumulate) : mma_add(d, at, db + 128 * k, idesc);
   }
 }
 
