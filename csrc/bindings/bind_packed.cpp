@@ -192,6 +192,7 @@ ops::RowSetting<T> row_setting(const py::object& value, const at::Tensor& logits
   }
   const double v = value.cast<double>();
   MCCL_CHECK_TENSOR(v >= low && v <= high, what << ": " << v << " is out of range");
+  MCCL_CHECK_TENSOR(std::is_floating_point<T>::value || v == std::floor(v), what << ": " << v << " is not a whole number");
   s.all = static_cast<T>(v);
   return s;
 }

@@ -31,7 +31,7 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: Setting 
         return _C.sample(logits, uniform, *settings)
     rows, vocab = logits.shape
     for name, value, high in zip(("temperature", "top_k", "top_p", "min_p"), settings, (3.4e38, 2 ** 31 - 1, 1.0, 1.0)):
-        if not torch.is_tensor(value) and not 0 <= value <= high:
+        if not torch.is_tensor(value) and not (0 <= value <= high and (name != "top_k" or value == int(value))):
             raise RuntimeError(f"sample({name}): {value} is out of range")
     t, k, p, low = (torch.as_tensor(v, dtype=torch.float32).double().expand(rows)[:, None] for v in settings)
     x = logits.double()

@@ -64,6 +64,12 @@ def exact(q, k, v, offsets, k_offsets, scale, window=None, sinks=0):
     return o, spread, lse
 
 
+def close(o, lse, want, dtype):
+    (want, spread, want_lse), u = want, UNIT[dtype]
+    assert ((o.double() - want).abs() <= u * want.abs() + (u + 2e-4) * spread + 1e-7).all()
+    assert (lse.double() - want_lse).abs().max().item() < 2e-4
+
+
 def check(q, k, v, offsets, k_offsets=None, scale=None, window=None, sinks=0):
     scale_ = q.shape[-1] ** -0.5 if scale is None else scale
     o, lse = ops.packed_attention(q, k, v, offsets, k_offsets, scale=scale, window=window, sinks=sinks, return_lse=True)
@@ -240,6 +246,45 @@ def test_offsets_that_do_not_fit_stay_within_the_tensors():
         o = ops.packed_attention(q, k, v, torch.tensor(bad, dtype=torch.int32).cuda())
         assert o.shape == q.shape
     torch.cuda.synchronize()
+
+
+def test_offsets_beyond_32_bits():
+    """Keys and values, and then queries and results, whose elements are numbered past 2^31."""
+    many = 1_070_000   # x 16 heads of 128: 2.19e9 elements
+    k, v = (torch.empty(many, 16, 128, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    for t in (k, v):
+        t[-5000:].normal_()
+    q = torch.randn(70, 32, 128, device="cuda").to(torch.bfloat16)
+    o, lse = ops.packed_attention(q, k, v, offsets_of([70]), offsets_of([5000], many - 5000), return_lse=True)
+    close(o, lse, exact(q, k[-5000:], v[-5000:], offsets_of([70]), offsets_of([5000]), 128 ** -0.5), torch.bfloat16)
+    del k, v
+    rows = 135_000     # x 128 heads of 128: 2.21e9 elements
+    q = torch.empty(rows, 128, 128, dtype=torch.bfloat16, device="cuda")
+    q[-300:].normal_()
+    k, v = (torch.randn(300, 2, 128, device="cuda").to(torch.bfloat16) for _ in range(2))
+    o, lse = ops.packed_attention(q, k, v, offsets_of([300], rows - 300), offsets_of([300]), return_lse=True)
+    close(o[-300:], lse[-300:], exact(q[-300:], k, v, offsets_of([300]), None, 128 ** -0.5), torch.bfloat16)
+    assert not o[:-300].any() and torch.isneginf(lse[:-300]).all()
+
+
+def test_two_graphs_and_two_streams_at_once():
+    """Each call has its own workspace (keys are shared out here)."""
+    sets = [make([40, 60], 4, 2, 64, before=[3000, 2000], seed=s, poison=False) for s in (1, 2)]
+    want = [ops.packed_attention(*x) for x in sets]
+    graphs, outs = [], []
+    for x in sets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(ops.packed_attention(*x))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
 
 
 def test_refusals():

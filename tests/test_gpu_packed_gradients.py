@@ -11,6 +11,7 @@ import pytest
 import torch
 
 from mccl_b200 import ops
+from tests.test_gpu_packed_attention import exact as exact_results
 from tests.test_gpu_packed_attention import make, offsets_of
 
 pytestmark = pytest.mark.gpu
@@ -160,30 +161,27 @@ def test_only_some_inputs_and_the_logarithm():
 
 
 def test_against_differences():
-    """A step of h in one direction moves a sum of results by h times the gradient along it.  In fp64 the plain form itself has the gradient of the formula
-    above; here: sum of o g, from results rounded to bf16.  Both results are off by at most b = sum |g| (u |o| + (u + w) sum p |v|), their difference over 2 h
-    by b / h, and the third derivative along unit directions stays below its size times h^2, which is put at a tenth of that."""
+    """Central differences of sum o g along the signs of the gradient.  They leave the slope by the truncation, which the formula in 64 bits gives for the same
+    two points, by the results' roundings at both, sum |g| (u |o| + (u + w) sum p |v|) over 2 h each, and by the gradient's own bound along the step."""
     q, k, v, offsets, _ = make([200], 2, 1, 64, poison=False)
-    gen = torch.Generator().manual_seed(3)
-    g = torch.randn(q.shape, generator=gen).to(q.dtype).cuda()
+    g = torch.randn(q.shape, generator=torch.Generator().manual_seed(3)).to(q.dtype).cuda()
     _, grads = run(q, k, v, g, offsets)
+    exact_grads, bounds = exact(q, k, v, g, offsets, None, 0.125)
     h = 0.25
-    for i, t in enumerate((q, k, v)):
-        d = torch.randn(t.shape, generator=gen).cuda()
-        up, down = ([x if j != i else (x.float() + s * h * d).to(x.dtype) for j, x in enumerate((q, k, v))] for s in (1, -1))
+    for i in range(3):
+        up, down = ([x if j != i else (x + s * h * grads[i].sign()).to(x.dtype) for j, x in enumerate((q, k, v))] for s in (1, -1))
         step = (up[i].double() - down[i].double()) / (2 * h)   # as it is after rounding
-        values = [(ops.packed_attention(*x, offsets).double() * g.double()).sum().item() for x in (up, down)]
+        got, want, off = [], [], 0.0
+        for x in (up, down):
+            got.append((ops.packed_attention(*x, offsets).double() * g.double()).sum().item())
+            o, spread, _ = exact_results(*x, offsets, None, 0.125)
+            want.append((o * g.double()).sum().item())
+            off += (g.double().abs() * (U * o.abs() + (U + W) * spread + 1e-7)).sum().item() / (2 * h)
         slope = (grads[i].double() * step).sum().item()
-        # exact slope by the formula in 64 bits
-        leaves = [x.double().requires_grad_() for x in (q, k, v)]
-        score = torch.einsum("ihd,jd->hij", leaves[0], leaves[1][:, 0]) / 8.0
-        mask = torch.ones(200, 200, dtype=torch.bool, device="cuda").tril()
-        p = torch.softmax(score.masked_fill(~mask, -math.inf), -1)
-        o = torch.einsum("hij,jd->ihd", p, leaves[2][:, 0])
-        spread = torch.einsum("hij,jd->ihd", p, leaves[2][:, 0].abs())
-        noise = (g.double().abs() * (U * o.abs() + (U + W) * spread)).pow(2).sum().sqrt().item() * 6 / h   # independent roundings: six of their deviations
-        third = 0.1 * abs(slope) + noise
-        assert abs((values[0] - values[1]) / (2 * h) - slope) <= third + noise, (i, values, slope, noise)
+        truncation = abs((want[0] - want[1]) / (2 * h) - (exact_grads[i] * step).sum().item())
+        bound = truncation + off + (bounds[i] * step.abs()).sum().item()
+        assert abs((got[0] - got[1]) / (2 * h) - slope) <= bound, (i, got, slope, bound)
+        assert bound < 0.6 * abs(slope), (i, slope, bound)   # a missing or doubled part would show
 
 
 def test_other_texts_are_other_texts():

@@ -192,7 +192,7 @@ def test_refusals():
     f = ops.sample
     calls = [
         lambda: f(x.double(), u), lambda: f(x[0], u), lambda: f(x[:, :0], u), lambda: f(x.t().contiguous().t(), u), lambda: f(x, u.half()), lambda: f(x, u[:1]), lambda: f(x, u.cpu()),
-        lambda: f(x, u, temperature=-1.0), lambda: f(x, u, temperature=math.nan), lambda: f(x, u, top_k=-1), lambda: f(x, u, top_p=1.5), lambda: f(x, u, top_p=-0.1), lambda: f(x, u, min_p=2.0),
+        lambda: f(x, u, temperature=-1.0), lambda: f(x, u, temperature=math.nan), lambda: f(x, u, top_k=-1), lambda: f(x, u, top_k=2.5), lambda: f(x, u, top_k=1 << 31), lambda: f(x, u, top_p=1.5), lambda: f(x, u, top_p=-0.1), lambda: f(x, u, min_p=2.0),
         lambda: f(x, u, temperature=u.double()), lambda: f(x, u, top_k=u), lambda: f(x, u, top_p=u[:1]), lambda: f(x, u, min_p=u.cpu()), lambda: f(x, u, temperature=math.inf),
         lambda: f(torch.zeros(1, (1 << 20) + 1, device="cuda"), u[:1]),
     ]
