@@ -1,6 +1,6 @@
 // Rotary positions of queries and keys: (a, b) -> (a cos - b sin, a sin + b cos) for the pairs of a head's first elements, the rest copied.
 //
-// Bound by memory: every element is read and written once.  A thread holds the cosines and sines of one place within the head and goes over several heads of
+// Bound by memory: every element is read and written once (16384 tokens of 32 + 8 heads of 128: 51 us, 6.6 TB/s; a device-to-device copy of as much takes 58).  A thread holds the cosines and sines of one place within the head and goes over several heads of
 // its token with them, so that the tables cost a fraction of the rest.  Pairs are neighbours within 16 bytes, or half a turned part apart: two accesses of 16
 // bytes then (8 where the half is an odd number of 4).  Products and sums are fp32, rounded once.
 #include "../core/launch.hpp"
@@ -21,7 +21,8 @@ constexpr int kThreads = 256;
 struct Rotary {
   RotaryArgs a;
   Divisor places, groups;   // places within a head that a thread may have; threads that share out a token's heads
-  int turned;               // the first of them turn pairs
+  int turned;               // the first of them turn pairs, ...
+  int apart, lone;          // ... the others copy N elements and, with halves, the N `apart` behind them; place `lone` has no second ones
 };
 
 // N values of one access.
@@ -54,8 +55,9 @@ __device__ __forceinline__ typename Access<N>::V down(const float (&f)[N]) {
   return raw;
 }
 
-// HALVES: N elements and the N of the other half per place; otherwise 8 elements, four pairs.  Behind the turned places 8 elements each are copied.  HEADS heads per
-// thread, all of whose loads are under way together.
+// HALVES: N elements and the N of the other half per place; otherwise 8 elements, four pairs.  Behind the turned places as many elements per place are copied, in
+// the same accesses (with a way of their own for copies, halves of 64 of 128 elements took 71 us where they take 51, of 16384 tokens with 32 + 8 heads).  HEADS heads per thread, all of whose loads are
+// under way together.
 template <typename H, bool HALVES, int N, int HEADS>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const Rotary r, int total) {
   using T = typename H::T;
@@ -68,7 +70,9 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Rotary r, int to
   const int rest = r.places.of(i), place = i - rest * r.places.d, t = r.groups.of(rest), group = rest - t * r.groups.d;
   const int pos = a.positions != nullptr ? __ldg(a.positions + t) : t;
   const bool inside = pos >= 0 && pos < a.rope_rows, turn = place < r.turned;
-  const int column = turn ? place * (HALVES ? N : 8) : 2 * a.width + (place - r.turned) * 8;
+  const int second = turn ? a.width : r.apart;
+  const bool two = HALVES && place != r.lone;
+  const int column = turn ? place * N : 2 * a.width + (place - r.turned) * N;
   const T* from[HEADS];
   T* to[HEADS];
 #pragma unroll
@@ -80,15 +84,6 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Rotary r, int to
     from[j] = any && inside ? static_cast<const T*>(part.x.p) + t * part.x.token + hh * part.x.head + column : nullptr;
     to[j] = any ? static_cast<T*>(part.out) + (static_cast<long long>(t) * part.heads + hh) * a.head_dim + column : nullptr;
   }
-  if (!turn) {
-    uint4 x[HEADS];
-#pragma unroll
-    for (int j = 0; j < HEADS; ++j) x[j] = from[j] != nullptr ? __ldg(reinterpret_cast<const uint4*>(from[j])) : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-    for (int j = 0; j < HEADS; ++j)
-      if (to[j] != nullptr) *reinterpret_cast<uint4*>(to[j]) = x[j];
-    return;
-  }
   constexpr int kPairs = HALVES ? N : 4;
   V lo[HEADS], hi[HEADS];
 #pragma unroll
@@ -96,14 +91,14 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Rotary r, int to
     lo[j] = hi[j] = V{};
     if (from[j] != nullptr) {
       lo[j] = __ldg(reinterpret_cast<const V*>(from[j]));
-      if (HALVES) hi[j] = __ldg(reinterpret_cast<const V*>(from[j] + a.width));
+      if (two) hi[j] = __ldg(reinterpret_cast<const V*>(from[j] + second));
     }
   }
   float c[kPairs], s[kPairs];
 #pragma unroll
   for (int e = 0; e < kPairs; e += 4) {
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-    if (inside) {
+    if (inside && turn) {
       x = __ldg(reinterpret_cast<const float4*>(a.cos + static_cast<long long>(pos) * a.width + place * kPairs + e));
       y = __ldg(reinterpret_cast<const float4*>(a.sin + static_cast<long long>(pos) * a.width + place * kPairs + e));
     }
@@ -117,6 +112,11 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Rotary r, int to
 #pragma unroll
   for (int j = 0; j < HEADS; ++j) {
     if (to[j] == nullptr) continue;
+    if (!turn) {
+      *reinterpret_cast<V*>(to[j]) = lo[j];
+      if (two) *reinterpret_cast<V*>(to[j] + second) = hi[j];
+      continue;
+    }
     float f[N];
     up<H, N>(lo[j], f);
     if constexpr (HALVES) {
@@ -146,17 +146,17 @@ template <typename H, bool HALVES, int N>
 void enqueue(const Rotary& r, int total, int per_thread, cudaStream_t stream) {
   const int blocks = (total + kThreads - 1) / kThreads;
   if (per_thread == 1) MCCL_LAUNCH_PDL((rotary_kernel<H, HALVES, N, 1>), blocks, kThreads, 0, stream, r, total);
-  else MCCL_LAUNCH_PDL((rotary_kernel<H, HALVES, N, 4>), blocks, kThreads, 0, stream, r, total);
+  else MCCL_LAUNCH_PDL((rotary_kernel<H, HALVES, N, 2>), blocks, kThreads, 0, stream, r, total);
 }
 
 template <typename H>
 cudaError_t launch(const RotaryArgs& args, cudaStream_t stream) {
   const int wide = args.halves && args.width % 8 != 0 ? 4 : 8;
   const int turned = args.halves ? args.width / wide : args.width / 4, heads = args.q.heads + args.k.heads;
-  const int places = turned + (args.head_dim - 2 * args.width) / 8;
-  // a thread takes four heads where that leaves every SM its threads
+  const int copied = (args.head_dim - 2 * args.width) / wide, pieces = args.halves ? 2 : 1, places = turned + (copied + pieces - 1) / pieces;
+  // a thread takes two heads where that leaves every SM its threads (16384 tokens of 32 + 8 heads: 51.1 us with two, 52.3 with four)
   const long long one = static_cast<long long>(args.tokens) * places * heads;
-  const int per_thread = one / 4 < 148ll * 2048 ? 1 : 4;
+  const int per_thread = one / 2 < 148ll * 2048 ? 1 : 2;
   const int groups = (heads + per_thread - 1) / per_thread;
   const long long per_token = static_cast<long long>(groups) * places;
   if (per_token > INT_MAX / 2) return cudaErrorInvalidValue;
@@ -181,6 +181,8 @@ cudaError_t launch(const RotaryArgs& args, cudaStream_t stream) {
     r.places = Divisor(places);
     r.groups = Divisor(groups);
     r.turned = turned;
+    r.apart = (copied + 1) / 2 * wide;
+    r.lone = args.halves && copied % 2 != 0 ? places - 1 : -1;
     const int total = static_cast<int>(tokens * per_token);
     if (!args.halves) enqueue<H, false, 8>(r, total, per_thread, stream);
     else if (wide == 8) enqueue<H, true, 8>(r, total, per_thread, stream);
