@@ -6,7 +6,15 @@
 //   m' = max(m, rowmax S),  P = exp2((S - m') c),  l = l 2^((m - m') c) + sum P,  O = O 2^((m - m') c) + P V
 // P goes back to the columns of S in 16 bits and is the left operand of the second product from there, so no weight passes through shared memory.
 // One warpgroup per tile has a row per thread; one warp issues the products of both tiles in turn, so that the tensor cores work on one
-// tile while the other's exponentials are computed; one warp brings tiles by TMA; one looks after blocks that not every row sees in whole.
+// tile while the other's exponentials are computed; one warp brings tiles by TMA; one looks after blocks that not every row sees in whole;
+// one finds out what the block does next: a block stays, and takes units of two tiles as long as there are any, the long ones first.
+//
+// What bounds it: a block of 128 x 128 scores of 128 columns takes the tensor cores some 1024 clocks in both products, and its 16384 exponentials take the special
+// function units as long, behind which the threads of a tile have maxima, differences and conversions to do; two tiles in turn fill the tensor cores to three quarters
+// (16381 tokens of 32 heads over 8 of 128: 1.73 ms, 1270 TFLOP/s; 2.0 ms where calls follow one another and the card's power is drawn).  Measured on the way there:
+// the first version, two threads with products and a unit per block, 2.54 ms; products by one thread that waits once a step, and blocks that stay, 1.71; 8 texts of
+// 2048 tokens, 16 heads of 128: 190 us, with results by TMA 171.  Tried and slower: exponentials partly as polynomials, a second thread for the second tile's products
+// (both tiles then wait in step), the next unit's first scores ahead of the last products of the one before (1.75 -> 1.82 ms).
 #include "packed_tiles.cuh"
 
 #include "smem_limit.hpp"
@@ -203,186 +211,186 @@ __global__ void __launch_bounds__(kThreads, 1)
   // are under way while the results of the one before are on their way out.
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
-  if (warp == 11) {
-    // ----------------------------------------------------------------------------------- what comes next ----
-    plan.run(s_unit, [&](int id) {
-      if (a.parts == 1) {
-        zero_outside<typename H::T>(a.o, p.heads * p.head_dim, a.lse, p.heads, p.offsets, p.sequences, p.tokens, id, a.units, lane, 32);
-      } else {
-        const int width = p.heads * p.head_dim;   // (of floats: two 16-bit numbers each)
-        for (int i = 0; i < a.parts; ++i)
-          zero_outside<uint16_t>(a.part_o + static_cast<long long>(i) * p.tokens * width, 2 * width, a.part_lse + static_cast<long long>(i) * p.tokens * p.heads, p.heads, p.offsets,
-                                 p.sequences, p.tokens, id, a.units, lane, 32);
-      }
-      return unit_of(a, id);
-    });
-  } else if (warp == 9) {
-    // ------------------------------------------------------------------------------------------- loads ----
-    uint32_t raw_uses = 0, q_uses = 0;   // a bit per stage, a bit per tile
-    int i = 0, units = 0;                // steps, and units with keys, so far
-    bool ok = true;
-    for (int k = 0; ok && plan.take(s_unit, k); ++k) {
-      const Unit& u = s_unit[k & 1];
-      if (tc::elect_one()) {
-        const int kv = u.head[0] / p.group;
-        if (u.all.hi > 0) {
-          if (units > 0) ok = wait(q_empty, (units - 1) & 1, bad);
-          ++units;
-        }
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-          if (ok && u.b[t].hi > 0) {
-            tc::mbar_expect_tx(&q_full[t], kTile);
-            load_tile<DP>(s_q + t * kTile, &tm_q, &q_full[t], u.head[t], u.s.q0 + u.row[t]);
-            q_uses ^= 1u << t;
-          }
-        // a step brings the values of the block before and the keys of the next one
-        for (int before = -1, b = u.all.next(-1); ok && (b < u.all.hi || before >= 0); ++i) {
-          const int st = i % kStages;
-          const bool more = b < u.all.hi, look = before >= 0 && !u.whole(before);
-          if (i >= kStages) ok = wait(&kv_empty[st], (i / kStages - 1) & 1, bad);
-          if (!ok) break;
-          tc::mbar_expect_tx(&kv_full[st], (more ? kTile : 0) + (before >= 0 && !look ? kTile : 0));
-          if (before >= 0) {
-            if (look) {
-              tc::mbar_expect_tx(&raw_full[st], kTile);
-              raw_uses ^= 1u << st;
-            }
-            load_tile<DP>(s_kv + 2 * st * kTile, &tm_v, look ? &raw_full[st] : &kv_full[st], kv, u.s.k0 + before * kRows);
-          }
-          if (more) load_tile<DP>(s_kv + (2 * st + 1) * kTile, &tm_k, &kv_full[st], kv, u.s.k0 + b * kRows);
-          before = more ? b : -1;
-          if (more) b = u.all.next(b);
-        }
-        if (!ok) {   // loads that were issued must land before the block retires
-          for (int t = 0; t < 2; ++t) tc::mbar_wait(&q_full[t], ((q_uses >> t) & 1) ^ 1, 1u << 16);
-          for (int j = max(0, i - kStages); j < i; ++j) {
-            const int st = j % kStages;
-            tc::mbar_wait(&kv_full[st], (j / kStages) & 1, 1u << 16);
-            tc::mbar_wait(&raw_full[st], ((raw_uses >> st) & 1) ^ 1, 1u << 16);
-          }
-        }
-      }
-      ok = __all_sync(0xffffffffu, ok);
-      if (lane == 0) tc::mbar_arrive(plan.loads_done);
-      plan.give_back(k);
-    }
-  } else if (warp == 10) {
-    // --------------------------------------------------------- blocks of keys that not every row sees ----
-    // A weight of zero times a value that is not finite would be NaN in rows that do not see the value: such values become zeros, and rows that do see
-    // them are put right at the end.  Rows behind the sequence are another sequence's.
-    int steps = 0;
-    uint32_t phase = 0;   // a bit per stage
-    bool ok = true;
-    for (int k = 0; ok && plan.take(s_unit, k); ++k) {
-    const Unit& u = s_unit[k & 1];
-    int i = steps + 1;
-    for (int b = u.all.next(-1); b < u.all.hi; b = u.all.next(b), ++i) {
-      if (u.whole(b)) continue;
-      const int st = i % kStages, rows = min(kRows, u.s.m - b * kRows);
-      ok = wait(&raw_full[st], (phase >> st) & 1, bad);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      phase ^= 1u << st;
-      uint8_t* tile = s_kv + 2 * st * kTile;
-      using T2 = typename H::T2;
-      const T2 zero = H::down(0.f, 0.f);
-      T2 sum = zero;   // products with zero add up to zero, or to NaN
-#pragma unroll 4
-      for (int i = lane; i < kTile / 16; i += 32) {
-        const int r = (i / 8) % kRows;
-        uint4* at = reinterpret_cast<uint4*>(tile + i * 16);
-        if (r < rows) {
-          const uint4 x = *at;
-          const T2* h = reinterpret_cast<const T2*>(&x);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sum = __hfma2(h[e], zero, sum);
+    if (warp == 11) {
+      // ----------------------------------------------------------------------------------- what comes next ----
+      plan.run(s_unit, [&](int id) {
+        if (a.parts == 1) {
+          zero_outside<typename H::T>(a.o, p.heads * p.head_dim, a.lse, p.heads, p.offsets, p.sequences, p.tokens, id, a.units, lane, 32);
         } else {
-          *at = make_uint4(0u, 0u, 0u, 0u);
+          const int width = p.heads * p.head_dim;   // (of floats: two 16-bit numbers each)
+          for (int i = 0; i < a.parts; ++i)
+            zero_outside<uint16_t>(a.part_o + static_cast<long long>(i) * p.tokens * width, 2 * width, a.part_lse + static_cast<long long>(i) * p.tokens * p.heads, p.heads, p.offsets,
+                                   p.sequences, p.tokens, id, a.units, lane, 32);
         }
-      }
-      const float2 s2 = H::up(sum);
-      if (__any_sync(0xffffffffu, !(s2.x == 0.f && s2.y == 0.f))) {
-        for (int i = lane; i < kTile / 16; i += 32) {
-          if ((i / 8) % kRows >= rows) continue;
-          uint4* at = reinterpret_cast<uint4*>(tile + i * 16);
-          uint4 x = *at;
-          uint16_t* e = reinterpret_cast<uint16_t*>(&x);
-          constexpr uint16_t kExponent = std::is_same<H, Bf16>::value ? 0x7f80 : 0x7c00;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) e[k] = (e[k] & kExponent) == kExponent ? static_cast<uint16_t>(0) : e[k];
-          *at = x;
-        }
-        if (lane == 0) *reinterpret_cast<volatile int*>(&s_unit[k & 1].odd) = 1;
-      }
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&looked[st]);
-    }
-    if (u.all.hi > 0) steps = i;   // a step more than blocks
-    plan.give_back(k);
-    }
-  } else if (warp == 8) {
-    // ---------------------------------------------------------------------------------------- products ----
-    // One thread.  What it does between the last product of one tile and the first of the other has some 500 clocks, the time of those under way; a barrier's
-    // state takes 250 while the products read shared memory.  Hence one barrier for values and keys of a step, and nothing else on the way.
-    constexpr uint32_t idesc_s = idesc16<H>(kRows, kRows, false, false);
-    constexpr uint32_t idesc_o = idesc16<H>(kRows, DP, false, true);   // (columns behind head_dim are zeros: TMA fills them in)
-    const int steps = (p.head_dim + 15) / 16;
-    uint32_t q_phase = 0, p_phase = 0, looked_phase = 0;   // a bit per tile; the last: per stage
-    int i = 0;                                             // steps so far
-    bool ok = true;
-    for (int k = 0; ok && plan.take(s_unit, k); ++k) {
-      const Unit m = s_unit[k & 1];
-      if (tc::elect_one()) {
-        uint32_t begun = 0;
-        bool look = false;
-        for (int before = -1, b = m.all.next(-1); b < m.all.hi || before >= 0; ++i) {
-          const int st = i % kStages;
-          const bool more = b < m.all.hi;
-          ok = wait(&kv_full[st], (i / kStages) & 1, bad);
-          if (look) {
-            ok = ok && wait(&looked[st], (looked_phase >> st) & 1, bad);
-            looked_phase ^= 1u << st;
+        return unit_of(a, id);
+      });
+    } else if (warp == 9) {
+      // ------------------------------------------------------------------------------------------- loads ----
+      uint32_t raw_uses = 0, q_uses = 0;   // a bit per stage, a bit per tile
+      int i = 0, units = 0;                // steps, and units with keys, so far
+      bool ok = true;
+      for (int k = 0; ok && plan.take(s_unit, k); ++k) {
+        const Unit& u = s_unit[k & 1];
+        if (tc::elect_one()) {
+          const int kv = u.head[0] / p.group;
+          if (u.all.hi > 0) {
+            if (units > 0) ok = wait(q_empty, (units - 1) & 1, bad);
+            ++units;
           }
-          if (!ok) break;
-#pragma unroll 1
-          for (int t = 0; t < 2; ++t) {
-            const Blocks mine = t == 0 ? m.b[0] : m.b[1];
-            if (before >= 0 && mine.has(before)) {
-#pragma unroll 1
-              for (int h = 0; h < 2; ++h) {   // the first half of the weights is multiplied while the second is made
-                ok = ok && wait(&p_full[2 * t + h], (p_phase >> t) & 1, bad);
-                if (!ok) break;
-                tc::fence_after_sync();
-                mma_weights<64>(tmem + 256 + t * DP, tmem + kP + kPStep * t + 32 * h, s_kv + 2 * st * kTile + h * 64 * 128, idesc_o, h != 0 || ((begun >> t) & 1));
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            if (ok && u.b[t].hi > 0) {
+              tc::mbar_expect_tx(&q_full[t], kTile);
+              load_tile<DP>(s_q + t * kTile, &tm_q, &q_full[t], u.head[t], u.s.q0 + u.row[t]);
+              q_uses ^= 1u << t;
+            }
+          // a step brings the values of the block before and the keys of the next one
+          for (int before = -1, b = u.all.next(-1); ok && (b < u.all.hi || before >= 0); ++i) {
+            const int st = i % kStages;
+            const bool more = b < u.all.hi, look = before >= 0 && !u.whole(before);
+            if (i >= kStages) ok = wait(&kv_empty[st], (i / kStages - 1) & 1, bad);
+            if (!ok) break;
+            tc::mbar_expect_tx(&kv_full[st], (more ? kTile : 0) + (before >= 0 && !look ? kTile : 0));
+            if (before >= 0) {
+              if (look) {
+                tc::mbar_expect_tx(&raw_full[st], kTile);
+                raw_uses ^= 1u << st;
               }
-              p_phase ^= 1u << t;
-              begun |= 1u << t;
-            } else if (more && mine.has(b) && ((begun >> t) & 1) == 0) {
-              ok = ok && wait(&q_full[t], (q_phase >> t) & 1, bad);
-              q_phase ^= 1u << t;
+              load_tile<DP>(s_kv + 2 * st * kTile, &tm_v, look ? &raw_full[st] : &kv_full[st], kv, u.s.k0 + before * kRows);
+            }
+            if (more) load_tile<DP>(s_kv + (2 * st + 1) * kTile, &tm_k, &kv_full[st], kv, u.s.k0 + b * kRows);
+            before = more ? b : -1;
+            if (more) b = u.all.next(b);
+          }
+          if (!ok) {   // loads that were issued must land before the block retires
+            for (int t = 0; t < 2; ++t) tc::mbar_wait(&q_full[t], ((q_uses >> t) & 1) ^ 1, 1u << 16);
+            for (int j = max(0, i - kStages); j < i; ++j) {
+              const int st = j % kStages;
+              tc::mbar_wait(&kv_full[st], (j / kStages) & 1, 1u << 16);
+              tc::mbar_wait(&raw_full[st], ((raw_uses >> st) & 1) ^ 1, 1u << 16);
+            }
+          }
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (lane == 0) tc::mbar_arrive(plan.loads_done);
+        plan.give_back(k);
+      }
+    } else if (warp == 10) {
+      // --------------------------------------------------------- blocks of keys that not every row sees ----
+      // A weight of zero times a value that is not finite would be NaN in rows that do not see the value: such values become zeros, and rows that do see
+      // them are put right at the end.  Rows behind the sequence are another sequence's.
+      int steps = 0;
+      uint32_t phase = 0;   // a bit per stage
+      bool ok = true;
+      for (int k = 0; ok && plan.take(s_unit, k); ++k) {
+        const Unit& u = s_unit[k & 1];
+        int i = steps + 1;
+        for (int b = u.all.next(-1); b < u.all.hi; b = u.all.next(b), ++i) {
+          if (u.whole(b)) continue;
+          const int st = i % kStages, rows = min(kRows, u.s.m - b * kRows);
+          ok = wait(&raw_full[st], (phase >> st) & 1, bad);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          phase ^= 1u << st;
+          uint8_t* tile = s_kv + 2 * st * kTile;
+          using T2 = typename H::T2;
+          const T2 zero = H::down(0.f, 0.f);
+          T2 sum = zero;   // products with zero add up to zero, or to NaN
+#pragma unroll 4
+          for (int i = lane; i < kTile / 16; i += 32) {
+            const int r = (i / 8) % kRows;
+            uint4* at = reinterpret_cast<uint4*>(tile + i * 16);
+            if (r < rows) {
+              const uint4 x = *at;
+              const T2* h = reinterpret_cast<const T2*>(&x);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sum = __hfma2(h[e], zero, sum);
+            } else {
+              *at = make_uint4(0u, 0u, 0u, 0u);
+            }
+          }
+          const float2 s2 = H::up(sum);
+          if (__any_sync(0xffffffffu, !(s2.x == 0.f && s2.y == 0.f))) {
+            for (int i = lane; i < kTile / 16; i += 32) {
+              if ((i / 8) % kRows >= rows) continue;
+              uint4* at = reinterpret_cast<uint4*>(tile + i * 16);
+              uint4 x = *at;
+              uint16_t* e = reinterpret_cast<uint16_t*>(&x);
+              constexpr uint16_t kExponent = std::is_same<H, Bf16>::value ? 0x7f80 : 0x7c00;
+#pragma unroll
+              for (int k = 0; k < 8; ++k) e[k] = (e[k] & kExponent) == kExponent ? static_cast<uint16_t>(0) : e[k];
+              *at = x;
+            }
+            if (lane == 0) *reinterpret_cast<volatile int*>(&s_unit[k & 1].odd) = 1;
+          }
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&looked[st]);
+        }
+        if (u.all.hi > 0) steps = i;   // a step more than blocks
+        plan.give_back(k);
+      }
+    } else if (warp == 8) {
+      // ---------------------------------------------------------------------------------------- products ----
+      // One thread.  What it does between the last product of one tile and the first of the other has some 500 clocks, the time of those under way; a barrier's
+      // state takes 250 while the products read shared memory.  Hence one barrier for values and keys of a step, and nothing else on the way.
+      constexpr uint32_t idesc_s = idesc16<H>(kRows, kRows, false, false);
+      constexpr uint32_t idesc_o = idesc16<H>(kRows, DP, false, true);   // (columns behind head_dim are zeros: TMA fills them in)
+      const int steps = (p.head_dim + 15) / 16;
+      uint32_t q_phase = 0, p_phase = 0, looked_phase = 0;   // a bit per tile; the last: per stage
+      int i = 0;                                             // steps so far
+      bool ok = true;
+      for (int k = 0; ok && plan.take(s_unit, k); ++k) {
+        const Unit m = s_unit[k & 1];
+        if (tc::elect_one()) {
+          uint32_t begun = 0;
+          bool look = false;
+          for (int before = -1, b = m.all.next(-1); b < m.all.hi || before >= 0; ++i) {
+            const int st = i % kStages;
+            const bool more = b < m.all.hi;
+            ok = wait(&kv_full[st], (i / kStages) & 1, bad);
+            if (look) {
+              ok = ok && wait(&looked[st], (looked_phase >> st) & 1, bad);
+              looked_phase ^= 1u << st;
             }
             if (!ok) break;
-            if (more && mine.has(b)) {
-              tc::fence_after_sync();
-              mma_rows<DP>(tmem + t * 128, s_q + t * kTile, s_kv + (2 * st + 1) * kTile, idesc_s, steps);
-              tc::mma_commit(&s_full[t]);
+#pragma unroll 1
+            for (int t = 0; t < 2; ++t) {
+              const Blocks mine = t == 0 ? m.b[0] : m.b[1];
+              if (before >= 0 && mine.has(before)) {
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h) {   // the first half of the weights is multiplied while the second is made
+                  ok = ok && wait(&p_full[2 * t + h], (p_phase >> t) & 1, bad);
+                  if (!ok) break;
+                  tc::fence_after_sync();
+                  mma_weights<64>(tmem + 256 + t * DP, tmem + kP + kPStep * t + 32 * h, s_kv + 2 * st * kTile + h * 64 * 128, idesc_o, h != 0 || ((begun >> t) & 1));
+                }
+                p_phase ^= 1u << t;
+                begun |= 1u << t;
+              } else if (more && mine.has(b) && ((begun >> t) & 1) == 0) {
+                ok = ok && wait(&q_full[t], (q_phase >> t) & 1, bad);
+                q_phase ^= 1u << t;
+              }
+              if (!ok) break;
+              if (more && mine.has(b)) {
+                tc::fence_after_sync();
+                mma_rows<DP>(tmem + t * 128, s_q + t * kTile, s_kv + (2 * st + 1) * kTile, idesc_s, steps);
+                tc::mma_commit(&s_full[t]);
+              }
+              if (before >= 0 && mine.has(before)) tc::mma_commit(&o_full[t]);
             }
-            if (before >= 0 && mine.has(before)) tc::mma_commit(&o_full[t]);
+            if (!ok) break;
+            tc::mma_commit(&kv_empty[st]);
+            look = more && !m.whole(b);
+            before = more ? b : -1;
+            if (more) b = m.all.next(b);
+            if (more && b >= m.all.hi) tc::mma_commit(q_empty);   // those were the last scores
           }
-          if (!ok) break;
-          tc::mma_commit(&kv_empty[st]);
-          look = more && !m.whole(b);
-          before = more ? b : -1;
-          if (more) b = m.all.next(b);
-          if (more && b >= m.all.hi) tc::mma_commit(q_empty);   // those were the last scores
         }
+        ok = __all_sync(0xffffffffu, ok);
+        plan.give_back(k);
       }
-      ok = __all_sync(0xffffffffu, ok);
-      plan.give_back(k);
     }
-  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowRegisters));
     // ------------------------------------------------------------------------------------------ a row per thread ----
@@ -394,140 +402,140 @@ __global__ void __launch_bounds__(kThreads, 1)
     int total = 0;        // blocks so far, of all units
     bool ok = true;
     for (int k = 0; ok && plan.take(s_unit, k); ++k) {
-    const Unit& u = s_unit[k & 1];
-    const int pos = u.first[t] + row, first = u.first[t], last = u.last[t];
-    const Blocks blocks = u.b[t];
-    float m = -INFINITY, l = 0.f;
-    bool sees = false;
-    int done = 0;         // blocks so far
-    for (int b = blocks.next(-1); b < blocks.hi; b = blocks.next(b), phase ^= 1) {
-      ok = wait(&s_full[t], phase, bad);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      tc::fence_after_sync();
-      float s[128];
-      {
-        uint32_t r[4][32];
+      const Unit& u = s_unit[k & 1];
+      const int pos = u.first[t] + row, first = u.first[t], last = u.last[t];
+      const Blocks blocks = u.b[t];
+      float m = -INFINITY, l = 0.f;
+      bool sees = false;
+      int done = 0;         // blocks so far
+      for (int b = blocks.next(-1); b < blocks.hi; b = blocks.next(b), phase ^= 1) {
+        ok = wait(&s_full[t], phase, bad);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc::fence_after_sync();
+        float s[128];
+        {
+          uint32_t r[4][32];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tc::tmem_ld_32x32(t_s + 32 * c, r[c]);
-        tc::tmem_ld_wait();
+          for (int c = 0; c < 4; ++c) tc::tmem_ld_32x32(t_s + 32 * c, r[c]);
+          tc::tmem_ld_wait();
 #pragma unroll
-        for (int c = 0; c < 128; ++c) s[c] = __uint_as_float(r[c / 32][c % 32]);
-      }
-      if (all_seen(p, b, first, last)) {
-        sees = true;
-      } else {
-        const int high = pos - b * kRows, low = high - p.window, sink = p.sinks - b * kRows;   // columns seen: c <= high and (c > low or c < sink)
-        sees = sees || (high >= 0 && (low < min(high, kRows - 1) || sink > 0));
+          for (int c = 0; c < 128; ++c) s[c] = __uint_as_float(r[c / 32][c % 32]);
+        }
+        if (all_seen(p, b, first, last)) {
+          sees = true;
+        } else {
+          const int high = pos - b * kRows, low = high - p.window, sink = p.sinks - b * kRows;   // columns seen: c <= high and (c > low or c < sink)
+          sees = sees || (high >= 0 && (low < min(high, kRows - 1) || sink > 0));
 #pragma unroll
-        for (int c = 0; c < 128; ++c) s[c] = c <= high && (c > low || c < sink) ? s[c] : -INFINITY;
-      }
-      float m8[8];
+          for (int c = 0; c < 128; ++c) s[c] = c <= high && (c > low || c < sink) ? s[c] : -INFINITY;
+        }
+        float m8[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) m8[i] = fmaxf(s[2 * i], s[2 * i + 1]);
+        for (int i = 0; i < 8; ++i) m8[i] = fmaxf(s[2 * i], s[2 * i + 1]);
 #pragma unroll
-      for (int c = 16; c < 128; c += 16) {
+        for (int c = 16; c < 128; c += 16) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m8[i] = max3(m8[i], s[c + 2 * i], s[c + 2 * i + 1]);
-      }
-      const float mx = max3(max3(m8[0], m8[1], m8[2]), max3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]));
-      // a row's maximum stays until it is passed by 2^kSlack.  (Each row's own: its bits do not depend on what else is in the tile.)
-      const bool raise = (mx - m) * p.scale_log2 > Weights<H>::kSlack || (m == -INFINITY && mx > m);
-      if (__any_sync(0xffffffffu, raise)) {
-        const float next = raise ? mx : m, f = raise ? (m == -INFINITY ? 0.f : exp2f((m - next) * p.scale_log2)) : 1.f;
-        if (done > 0) {
-          ok = wait(&o_full[t], (total - 1) & 1, bad);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          tc::fence_after_sync();
+          for (int i = 0; i < 8; ++i) m8[i] = max3(m8[i], s[c + 2 * i], s[c + 2 * i + 1]);
+        }
+        const float mx = max3(max3(m8[0], m8[1], m8[2]), max3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]));
+        // a row's maximum stays until it is passed by 2^kSlack.  (Each row's own: its bits do not depend on what else is in the tile.)
+        const bool raise = (mx - m) * p.scale_log2 > Weights<H>::kSlack || (m == -INFINITY && mx > m);
+        if (__any_sync(0xffffffffu, raise)) {
+          const float next = raise ? mx : m, f = raise ? (m == -INFINITY ? 0.f : exp2f((m - next) * p.scale_log2)) : 1.f;
+          if (done > 0) {
+            ok = wait(&o_full[t], (total - 1) & 1, bad);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc::fence_after_sync();
 #pragma unroll 1
-          for (int c = 0; c < DP / 16; ++c) {
-            uint32_t o[16];
-            tmem_ld16(t_o + 16 * c, o);
-            tc::tmem_ld_wait();
+            for (int c = 0; c < DP / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld16(t_o + 16 * c, o);
+              tc::tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tmem_st16(t_o + 16 * c, o);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st16(t_o + 16 * c, o);
+            }
+          }
+          l *= f;
+          m = next;
+        }
+        const float base = (m == -INFINITY ? 0.f : m * p.scale_log2) - Weights<H>::kBias;
+        const F2 base2 = f2(-base, -base);
+        F2 sums[4] = {f2(0.f, 0.f), f2(0.f, 0.f), f2(0.f, 0.f), f2(0.f, 0.f)};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t w[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            float lo, hi;
+            split(fma2(f2(s[64 * h + 2 * e], s[64 * h + 2 * e + 1]), scale2, base2), lo, hi);
+            lo = exp2f(lo);
+            hi = exp2f(hi);
+            sums[e & 3] = add2(sums[e & 3], f2(lo, hi));
+            const typename H::T2 h2 = H::down(lo, hi);
+            w[e] = *reinterpret_cast<const uint32_t*>(&h2);
+          }
+          tmem_st32(t_p + 32 * h, w);
+          tmem_st_wait();
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&p_full[2 * t + h]);
+        }
+        float sum, other;
+        split(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])), sum, other);
+        l += sum + other;
+        ++done;
+        ++total;
+      }
+      if (ok && done > 0) {
+        ok = wait(&o_full[t], (total - 1) & 1, bad);
+        ok = __all_sync(0xffffffffu, ok);
+        tc::fence_after_sync();
+      }
+      if (ok && u.row[t] < u.s.n) {
+        const bool mine = u.row[t] + row < u.s.n;
+        const bool none = !sees || pos < 0;
+        const float inv = none ? 0.f : 1.f / l;
+        float* to_lse = a.parts > 1 ? a.part_lse + static_cast<long long>(u.part) * p.heads * p.tokens : a.lse;
+        if (to_lse != nullptr && mine)
+          to_lse[static_cast<long long>(u.head[t]) * p.tokens + u.s.q0 + u.row[t] + row] = none ? -INFINITY : (m * p.scale_log2 + log2f(l) - Weights<H>::kBias) / kLog2e;
+        const int first_row = u.s.q0 + u.row[t] + (warp & 3) * 32, rows = u.s.n - u.row[t] - (warp & 3) * 32, head = u.head[t];
+        const bool odd = *reinterpret_cast<const volatile int*>(&u.odd) != 0;
+#pragma unroll 1
+        for (int c0 = 0; c0 < p.head_dim; c0 += 64) {
+          uint32_t o[2][32] = {};
+          if (done > 0) {
+            tc::tmem_ld_32x32(t_o + c0, o[0]);
+            tc::tmem_ld_32x32(t_o + c0 + 32, o[1]);
+            tc::tmem_ld_wait();
+          }
+          float f[64];
+#pragma unroll
+          for (int e = 0; e < 64; ++e) f[e] = none ? 0.f : __uint_as_float(o[e / 32][e % 32]) * inv;
+          if (odd) {
+            const unsigned long long marks = odd_columns<H>(p, a.v, u, blocks, pos, c0);
+#pragma unroll
+            for (int e = 0; e < 64; ++e) f[e] = (marks >> e) & 1 ? NAN : f[e];
+          }
+          if (a.parts > 1) {
+            float* to = a.part_o + ((static_cast<long long>(u.part) * p.tokens + first_row + lane) * p.heads + head) * p.head_dim + c0;
+#pragma unroll
+            for (int e = 0; e < 64; e += 4)
+              if (mine && c0 + e < p.head_dim) *reinterpret_cast<float4*>(to + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+            continue;
+          }
+          rows_out<H>(s_out + warp * kOut, &tm_o, f, a.o, p.heads, p.head_dim, head, first_row, rows, c0);
+          if (a.o_rest != nullptr) {
+#pragma unroll
+            for (int e = 0; e < 64; ++e) f[e] -= H::up(H::down(f[e]));
+            rows_out<H>(s_out + warp * kOut, &tm_rest, f, a.o_rest, p.heads, p.head_dim, head, first_row, rows, c0);
           }
         }
-        l *= f;
-        m = next;
       }
-      const float base = (m == -INFINITY ? 0.f : m * p.scale_log2) - Weights<H>::kBias;
-      const F2 base2 = f2(-base, -base);
-      F2 sums[4] = {f2(0.f, 0.f), f2(0.f, 0.f), f2(0.f, 0.f), f2(0.f, 0.f)};
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t w[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          float lo, hi;
-          split(fma2(f2(s[64 * h + 2 * e], s[64 * h + 2 * e + 1]), scale2, base2), lo, hi);
-          lo = exp2f(lo);
-          hi = exp2f(hi);
-          sums[e & 3] = add2(sums[e & 3], f2(lo, hi));
-          const typename H::T2 h2 = H::down(lo, hi);
-          w[e] = *reinterpret_cast<const uint32_t*>(&h2);
-        }
-        tmem_st32(t_p + 32 * h, w);
-        tmem_st_wait();
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&p_full[2 * t + h]);
-      }
-      float sum, other;
-      split(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])), sum, other);
-      l += sum + other;
-      ++done;
-      ++total;
-    }
-    if (ok && done > 0) {
-      ok = wait(&o_full[t], (total - 1) & 1, bad);
-      ok = __all_sync(0xffffffffu, ok);
-      tc::fence_after_sync();
-    }
-    if (ok && u.row[t] < u.s.n) {
-      const bool mine = u.row[t] + row < u.s.n;
-      const bool none = !sees || pos < 0;
-      const float inv = none ? 0.f : 1.f / l;
-      float* to_lse = a.parts > 1 ? a.part_lse + static_cast<long long>(u.part) * p.heads * p.tokens : a.lse;
-      if (to_lse != nullptr && mine)
-        to_lse[static_cast<long long>(u.head[t]) * p.tokens + u.s.q0 + u.row[t] + row] = none ? -INFINITY : (m * p.scale_log2 + log2f(l) - Weights<H>::kBias) / kLog2e;
-      const int first_row = u.s.q0 + u.row[t] + (warp & 3) * 32, rows = u.s.n - u.row[t] - (warp & 3) * 32, head = u.head[t];
-      const bool odd = *reinterpret_cast<const volatile int*>(&u.odd) != 0;
-#pragma unroll 1
-      for (int c0 = 0; c0 < p.head_dim; c0 += 64) {
-        uint32_t o[2][32] = {};
-        if (done > 0) {
-          tc::tmem_ld_32x32(t_o + c0, o[0]);
-          tc::tmem_ld_32x32(t_o + c0 + 32, o[1]);
-          tc::tmem_ld_wait();
-        }
-        float f[64];
-#pragma unroll
-        for (int e = 0; e < 64; ++e) f[e] = none ? 0.f : __uint_as_float(o[e / 32][e % 32]) * inv;
-        if (odd) {
-          const unsigned long long marks = odd_columns<H>(p, a.v, u, blocks, pos, c0);
-#pragma unroll
-          for (int e = 0; e < 64; ++e) f[e] = (marks >> e) & 1 ? NAN : f[e];
-        }
-        if (a.parts > 1) {
-          float* to = a.part_o + ((static_cast<long long>(u.part) * p.tokens + first_row + lane) * p.heads + head) * p.head_dim + c0;
-#pragma unroll
-          for (int e = 0; e < 64; e += 4)
-            if (mine && c0 + e < p.head_dim) *reinterpret_cast<float4*>(to + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
-          continue;
-        }
-        rows_out<H>(s_out + warp * kOut, &tm_o, f, a.o, p.heads, p.head_dim, head, first_row, rows, c0);
-        if (a.o_rest != nullptr) {
-#pragma unroll
-          for (int e = 0; e < 64; ++e) f[e] -= H::up(H::down(f[e]));
-          rows_out<H>(s_out + warp * kOut, &tm_rest, f, a.o_rest, p.heads, p.head_dim, head, first_row, rows, c0);
-        }
-      }
-    }
-    tc::fence_before_sync();   // the next unit's first product with V writes O
-    plan.give_back(k);
+      tc::fence_before_sync();   // the next unit's first product with V writes O
+      plan.give_back(k);
     }
     rows_sent();
     tc::fence_before_sync();
@@ -582,7 +590,7 @@ __global__ void __launch_bounds__(256) packed_join_kernel(const Forward a) {
 
 constexpr int kSms = 148;
 // Two heads that share keys and values make a unit, or else 256 rows of one: an odd number of heads leaves one alone, sequences of up to 128 rows the second tile
-// of rows empty.  (8 texts of up to 130 rows behind up to 4096 keys, 12 heads over 4 of 64: 54 us with rows, XX with heads.)
+// of rows empty.  (8 texts of up to 130 rows behind up to 4096 keys, 12 heads over 4 of 64: 60 us with rows, 42 with heads.)
 bool pairs_heads(const PackedAttentionArgs& a) {
   const int group = a.heads / a.kv_heads;
   return group % 2 == 0 || (group > 1 && a.tokens / a.sequences <= kRows);
