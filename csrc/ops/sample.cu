@@ -567,7 +567,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     if (rank == 0 && threadIdx.x == 0) a.tokens[line] = -1;
     return;
   }
-  if (temperature < 1.2e-38f) {   // zero, or too small to divide by
+  if (temperature < 1e-36f) {   // zero, or so small that the factor of the logits is no number of 32 bits (from 2.7e-37 down)
     if (rank == 0 && threadIdx.x == 0) a.tokens[line] = static_cast<long long>(best & 0xffffffffu);
     return;
   }

@@ -187,6 +187,14 @@ def test_agrees_with_the_plain_form():
         assert torch.equal(ops.sample(x, u.cuda(), **options).cpu(), ops.sample(x.cpu(), u, **options))
 
 
+@pytest.mark.parametrize("temperature", [0.0, 1e-45, 1e-38, 1.3e-38, 2e-37, 1e-36, 1e-30])
+def test_temperatures_next_to_zero(temperature):
+    x = torch.randn(5, 1000, generator=torch.Generator().manual_seed(1)).cuda()
+    u = torch.full((5,), 0.999, device="cuda")
+    for settings in ({}, {"top_k": 7}, {"top_p": 0.5, "min_p": 0.1}):
+        assert torch.equal(ops.sample(x, u, temperature=temperature, **settings), x.argmax(1))
+
+
 def test_refusals():
     x, u = logits_of(2, 100, torch.float32), torch.rand(2, device="cuda")
     f = ops.sample
