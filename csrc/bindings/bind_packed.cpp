@@ -102,7 +102,7 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
     const at::Tensor &o = s[5], &lse = s[6], &rest = s[7], d_o = rows_of_heads(grads[0]);
     c10::cuda::CUDAGuard guard(x.q.device());
     at::Tensor dq = empty_on(x.q, x.q.sizes(), at::kBFloat16), dk = empty_on(x.q, x.k.sizes(), at::kBFloat16), dv = empty_on(x.q, x.v.sizes(), at::kBFloat16);
-    if (x.k.size(0) == 0 || x.q.size(0) == 0 || x.offsets.numel() == 1) {
+    if (x.k.size(0) == 0 || x.q.numel() == 0 || x.offsets.numel() == 1) {
       dq.zero_();
       dk.zero_();
       dv.zero_();

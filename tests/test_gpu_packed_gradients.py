@@ -128,6 +128,14 @@ def test_no_texts_and_no_tokens():
     assert not any(t.any() for t in run(q[:0], k, v, q[:0], both[1], both[0])[1])
 
 
+def test_no_query_heads():
+    """Their keys' gradients are zeros, not what was in the memory before."""
+    q, k, v, offsets, _ = make([50], 4, 2, 64, poison=False)
+    run(q, k, v, torch.ones_like(q), offsets)
+    o, grads = run(q[:, :0], k, v, q[:, :0], offsets)
+    assert o.shape == (50, 0, 64) and grads[0].shape == (50, 0, 64) and not grads[1].any() and not grads[2].any()
+
+
 def test_many_texts():
     g = torch.Generator().manual_seed(1)
     check(*make(torch.randint(0, 30, (1500,), generator=g).tolist(), 2, 2, 64))
