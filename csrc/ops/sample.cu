@@ -175,7 +175,7 @@ __device__ __forceinline__ void add(Parts& h, int bin, u64 w) {
   if (WEIGHTS) {
     atomicAdd(&h.sum[0][bin], static_cast<unsigned>(w) & ((1u << kPart) - 1));
     atomicAdd(&h.sum[1][bin], static_cast<unsigned>(w >> kPart) & ((1u << kPart) - 1));
-    atomicAdd(&h.sum[2][bin], static_cast<unsigned>(w >> 2 * kPart));
+    if (w >> 2 * kPart) atomicAdd(&h.sum[2][bin], static_cast<unsigned>(w >> 2 * kPart));   // (seldom: 1e-4 of the likeliest token's weight and more)
   }
 }
 __device__ __forceinline__ void clear(Parts& h) {
@@ -263,16 +263,23 @@ struct Row {
   int lo, hi;   // this warp's part
   Scale scale;
   float steps, most;   // bins of the first level per unit of logit, and the maximum
+  float temperature;
+  int vocab;
 
   __device__ __forceinline__ int bin(float x) const {
     const int b = static_cast<int>((most - x) * steps);   // both grow together: rounding keeps the order
     return b < 0 ? 0 : (b < kBins ? b : kBins - 1);
   }
 
-  // First block only, all threads: the first bin at whose end `need` tokens (with WEIGHTS: share of all weights, or s.enough of them) have been passed, behind
+  // A logit from which on all weights are (1 - share) / 2 / vocab or more (rounded down: it may lie below).
+  __device__ __forceinline__ float deep_below(float share) const {
+    return __fsub_rd(most, __fmul_ru(temperature, logf(2.f * static_cast<float>(vocab) / (1.f - share))));
+  }
+
+  // First block only, all threads: the first bin at whose end `need` tokens (with WEIGHTS: share of all blocks' weights, or s.enough of them) have been passed, behind
   // count0 tokens and weights of sum0; s.border has it, or found = 0.
   template <bool WEIGHTS>
-  __device__ __forceinline__ static void find_bin(Shared& s, int count0, u64 sum0, unsigned need, float share) {
+  __device__ __forceinline__ static void find_bin(Shared& s, int blocks, int count0, u64 sum0, unsigned need, float share) {
     constexpr int kEach = kBins / kThreads;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     unsigned c[kEach], count = 0;
@@ -303,7 +310,7 @@ struct Row {
     __syncthreads();
     if (WEIGHTS && share >= 0.f) {   // a token is kept while the weights in front of it are below the share of all: the border is where they are reached
       u64 all = 0;
-      for (int i = 0; i < kWarps; ++i) all += s.scan[i];
+      for (int i = 0; i < blocks; ++i) all += s.total[i];
       if (threadIdx.x == 0) s.enough = static_cast<double>(share) * static_cast<double>(all);
       __syncthreads();
     }
@@ -388,11 +395,29 @@ struct Row {
     const bool limited = limit != ~0ull;
     clear(s.mine);
     __syncthreads();
+    // All tokens with weights below (1 - share) / 2 / vocab together are less than half of what lies behind the border: they count in the sum of all, but it is not
+    // among them, and they are not counted in their bins.
+    const int deep = WEIGHTS ? bin(deep_below(share)) : kBins - 1;   // (whole bins: what is counted is what is found again)
+    u64 all = 0;
     walk<T, V>(row, lo, hi, [&](float x, int i, bool valid) {
-      if (valid && scale.some(x) && (!limited || composite(x, i) <= limit)) add<WEIGHTS>(s.mine, bin(x), WEIGHTS ? scale.weight(x) : 0);
+      if (valid && scale.some(x) && (!limited || composite(x, i) <= limit)) {
+        const u64 w = WEIGHTS ? scale.weight(x) : 0;
+        if (WEIGHTS) all += w;
+        const int at = bin(x);
+        if (at <= deep) add<WEIGHTS>(s.mine, at, w);
+      }
     });
+    if (WEIGHTS) {
+      all = warp_sum(all);
+      if (lane == 0) s.warp_sum[warp] = all;
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        for (int i = 1; i < kWarps; ++i) all += s.warp_sum[i];
+        first->total[rank] = all;
+      }
+    }
     merge(cluster, s);
-    if (rank == 0) find_bin<WEIGHTS>(s, 0, 0, need, share);
+    if (rank == 0) find_bin<WEIGHTS>(s, blocks, 0, 0, need, share);
     tell();
     if (!s.border.found) return ~0ull;
     bool level = true;   // still the first
@@ -455,7 +480,7 @@ struct Row {
       });
       merge(cluster, s);
       if (rank == 0) {
-        find_bin<WEIGHTS>(s, b.count, b.sum, need, -1.f);
+        find_bin<WEIGHTS>(s, blocks, b.count, b.sum, need, -1.f);
         if (threadIdx.x == 0) {
           s.border.lo = low + (static_cast<u64>(s.border.bin) << shift);
           s.border.hi = min(high, s.border.lo + ((1ull << shift) - 1));
@@ -572,6 +597,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     return;
   }
   r.most = most;
+  r.temperature = temperature;
+  r.vocab = a.vocab;
   const double per = 64.0 * kLog2e / static_cast<double>(temperature);
   r.scale = {most, static_cast<float>(per), static_cast<float>(per - static_cast<double>(static_cast<float>(per))), s.power};
   r.steps = static_cast<float>(kBins) / (kReach * temperature);
@@ -601,8 +628,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
 
   // ---- the choice
   const bool limited = border != ~0ull;
+  // logits below this are none of the kept ones: the border's, or half of min_p (which the weights below decide on)
+  const float low = fmaxf(limited ? value_of_key(border) : -INFINITY, min_p > 0.f ? __fadd_rd(most, __fmul_rd(temperature, logf(0.5f * fminf(min_p, 1.f)))) : -INFINITY);
   auto kept = [&](float x, int i) -> u64 {
-    if (!r.scale.some(x) || (limited && composite(x, i) > border)) return 0;
+    if (!(x >= low) || !r.scale.some(x) || (limited && composite(x, i) > border)) return 0;
     const u64 w = r.scale.weight(x);
     return w < least ? 0 : w;
   };
