@@ -3,6 +3,7 @@
 // Python node costs more host time than the kernels of a few thousand tokens take.
 #include "../ops/ops.hpp"
 #include "../ops/packed.hpp"
+#include "../symm/cu_driver.hpp"
 #include "bind.hpp"
 #include "operand_checks.hpp"
 
@@ -78,6 +79,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_forward(const Attention
       workspace = empty_on(x.q, {static_cast<int64_t>(bytes)}, at::kByte);
       a.workspace = workspace.data_ptr();
     }
+    CuDriver::get().ensure_context(x.q.get_device());   // (tensor maps)
     check_launch(ops::packed_attention(a, stream_of(x.q)), op);
   }
   return {o, l, r};
@@ -92,11 +94,13 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
     ctx->saved_data["window"] = window;
     ctx->saved_data["sinks"] = sinks;
     ctx->mark_non_differentiable({lse});
+    ctx->set_materialize_grads(false);   // (zeros for lse would be a launch of their own)
     return {o, lse};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const char* op = "packed_attention";
     need_first_order(op);
+    if (!grads[0].defined()) return variable_list(8);
     const auto s = ctx->get_saved_variables();
     const Attention x{s[0], s[1], s[2], s[3], s[4], ctx->saved_data["scale"].toDouble(), ctx->saved_data["window"].toInt(), ctx->saved_data["sinks"].toInt()};
     const at::Tensor &o = s[5], &lse = s[6], &rest = s[7], d_o = rows_of_heads(grads[0]);
@@ -118,6 +122,7 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
       a.dv = dv.data_ptr();
       at::Tensor delta = empty_on(x.q, lse.sizes(), at::kFloat);
       a.delta = delta.data_ptr<float>();
+      CuDriver::get().ensure_context(x.q.get_device());
       check_launch(ops::packed_attention_grad(a, stream_of(x.q)), "packed_attention backward");
     }
     return {dq, dk, dv, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};

@@ -192,6 +192,24 @@ def test_against_differences():
         assert bound < 0.6 * abs(slope), (i, slope, bound)   # a missing or doubled part would show
 
 
+def test_threads_that_have_done_nothing_yet():
+    """Tensor maps need a context; a thread whose memory all comes from the cache may have none."""
+    import threading
+    q, k, v, offsets, _ = make([300, 40], 4, 2, 64, poison=False)
+    g = torch.ones_like(q)
+    want = run(q, k, v, g, offsets)
+    got = []
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    thread = threading.Thread(target=lambda: got.append(ops.packed_attention(*leaves, offsets)))
+    thread.start()
+    thread.join()
+    assert torch.equal(got[0], want[0])
+    thread = threading.Thread(target=lambda: got.extend(torch.autograd.grad(got[0], leaves, g)))
+    thread.start()
+    thread.join()
+    assert all(torch.equal(a, b) for a, b in zip(got[1:], want[1])) and len(got) == 4
+
+
 def test_other_texts_are_other_texts():
     q, k, v, offsets, _ = make([70, 200, 65], 4, 2, 128)
     g = torch.ones_like(q)
