@@ -51,15 +51,17 @@ struct Forward {
 template <int DP>
 constexpr int smem_bytes() { return (2 + 2 * kStages) * (DP / 64) * kSub + 8 * kOut + 512 + 1024; }
 
-// Weights are kept 2^kBias times larger in fp16, whose smallest normal number is 2^-14; the running maximum may be exceeded by 2^kSlack before sums are
-// rescaled (exact in fp32 either way), so that the largest weight is 2^8 in bf16 and 2^15 in fp16.
+// Weights are kept 2^kBias times larger in fp16: below 2^-21 they are subnormal there and off by 2^-32 at most, which over 2^17 keys is 2^-15 of the sum.  The running
+// maximum may be exceeded by 2^kSlack before sums are rescaled (exact in fp32 either way), so that the largest weight is 2^8 in bf16 and 2^15 in fp16.  (With 2^11 and
+// 2^4, windows of 1024 and 4 first positions, 4 texts up to 8192 of 16 heads over 4 of 128, took 317 us in fp16: a window's first block is seen in part, and its maximum
+// is soon passed.  With 2^7 and 2^8 251.)
 template <typename H>
 struct Weights {
   static constexpr float kBias = 0.f, kSlack = 8.f;
 };
 template <>
 struct Weights<Fp16> {
-  static constexpr float kBias = 11.f, kSlack = 4.f;
+  static constexpr float kBias = 7.f, kSlack = 8.f;
 };
 
 // The tiles of a unit.

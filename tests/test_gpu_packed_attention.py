@@ -248,6 +248,19 @@ def test_offsets_that_do_not_fit_stay_within_the_tensors():
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_weights_of_all_sizes(dtype):
+    """One key that outweighs the others by up to 2^30, first, in the middle or last, and thousands whose weights count together."""
+    n = 4000
+    for place in (0, 1900, n - 1):
+        q, k, v, offsets, _ = make([n], 2, 1, 64, dtype, poison=False, seed=place)
+        q, k, v = (t.contiguous() for t in (q, k, v))
+        q[..., 0], k[..., 0] = 8.0, 0.0
+        k[place, :, 0] = 20.0   # a score of 20 more
+        v.abs_()
+        check(q, k, v, offsets)
+
+
 def test_offsets_beyond_32_bits():
     """Keys and values, and then queries and results, whose elements are numbered past 2^31."""
     many = 1_070_000   # x 16 heads of 128: 2.19e9 elements
