@@ -4,17 +4,19 @@
 // neighbouring rows of one head.  Per tile and block of 128 keys:
 //   S = Q K^T (tcgen05, operands in shared memory, sums in tensor memory)
 //   m' = max(m, rowmax S),  P = exp2((S - m') c),  l = l 2^((m - m') c) + sum P,  O = O 2^((m - m') c) + P V
-// P goes back to the columns of S in 16 bits and is the left operand of the second product from there, so no weight passes through shared memory.
+// P goes to tensor memory in 16 bits (columns of S, or its own where there are some) and is the left operand of the second product from there, so no weight passes through shared memory.
 // One warpgroup per tile has a row per thread; one warp issues the products of both tiles in turn, so that the tensor cores work on one
 // tile while the other's exponentials are computed; one warp brings tiles by TMA; one looks after blocks that not every row sees in whole;
 // one finds out what the block does next: a block stays, and takes units of two tiles as long as there are any, the long ones first.
 //
 // What bounds it: a block of 128 x 128 scores of 128 columns takes the tensor cores some 1024 clocks in both products, and its 16384 exponentials take the special
-// function units as long, behind which the threads of a tile have maxima, differences and conversions to do; two tiles in turn fill the tensor cores to three quarters
-// (16381 tokens of 32 heads over 8 of 128: 1.73 ms, 1270 TFLOP/s; 2.0 ms where calls follow one another and the card's power is drawn).  Measured on the way there:
+// function units as long, behind which the threads of a tile have maxima, differences and conversions to do; two tiles in turn reach three quarters of the rate of a library
+// product (16381 tokens of 32 heads over 8 of 128: 1.73 ms, 1270 TFLOP/s; 2.0 ms where calls follow one another and the card's power is drawn).  A step of both tiles takes
+// 3400 clocks; per tile 200 until the scores are in registers, 500 for the maximum, 720 for each half of the exponentials, 1250 for the product with V and the next scores.  Measured on the way there:
 // the first version, two threads with products and a unit per block, 2.54 ms; products by one thread that waits once a step, and blocks that stay, 1.71; 8 texts of
 // 2048 tokens, 16 heads of 128: 190 us, with results by TMA 171.  Tried and slower: exponentials partly as polynomials, a second thread for the second tile's products
-// (both tiles then wait in step), the next unit's first scores ahead of the last products of the one before (1.75 -> 1.82 ms).
+// (both tiles then wait in step), the next unit's first scores ahead of the last products of the one before (1.75 -> 1.82 ms), two warps per row with half of the keys each (1.97 ms), the first half's
+// exponentials with the maximum so far while the block's own is found (1.76 ms).
 #include "packed_tiles.cuh"
 
 #include "smem_limit.hpp"
