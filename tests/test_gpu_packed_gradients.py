@@ -192,6 +192,19 @@ def test_against_differences():
         assert bound < 0.6 * abs(slope), (i, slope, bound)   # a missing or doubled part would show
 
 
+@pytest.mark.parametrize("lengths,before,window,sinks", [([3] * 100, None, None, 0), ([8] * 60, None, None, 0), ([20] * 30, None, None, 0), ([300, 77], None, 2, 0), ([300, 77], None, 5, 3),
+                                                         ([4] * 90, [2] * 90, 3, 1), ([500], None, None, 0)])
+def test_two_roundings_and_no_more(lengths, before, window, sinks):
+    """dQ and dK are rounded themselves and are sums of gradients of scores that were rounded, each time by as much (root mean square): 2^0.5 times what rounding the exact ones
+    leaves.  Everything else is a sixth of that at most, 1.5 times in all."""
+    q, k, v, offsets, k_offsets = make(lengths, 4, 2, 64, before=before, poison=False, seed=len(lengths))
+    g = torch.randn(q.shape, generator=torch.Generator().manual_seed(7)).to(q.dtype).cuda()
+    want, _ = exact(q, k, v, g, offsets, k_offsets, 0.125, window, sinks)
+    _, got = run(q, k, v, g, offsets, k_offsets, window=window, sinks=sinks)
+    for name, a, b in list(zip("qkv", got, want))[:2]:
+        assert (a.double() - b).norm() <= 1.5 * (b.to(torch.bfloat16).double() - b).norm(), name
+
+
 def test_threads_that_have_done_nothing_yet():
     """Tensor maps need a context; a thread whose memory all comes from the cache may have none."""
     import threading
