@@ -8,6 +8,10 @@
 //   3. sums of the kept weights per warp; the warp in whose part the random number falls goes through it once more
 // Weights are whole numbers, exp((l - max) / T) 2^43 rounded, and their sums are exact: nothing depends on the order in which they are added, and the running
 // sum of 100000 tokens is off by 1e-11 of itself where sums of fp32 would be off by more than a token's weight.
+//
+// What bounds it: for one row the chain of passes and barriers (32000 tokens under top-k 50 and top-p 0.9: 11.5 us; maximum 1.1, barrier 0.6, counts 2.1, their sum over 8
+// blocks 1.5, border 0.9, list 1.7, the choice among 50 3), for many the instructions: some 60 per token with its weight, 10 us of 64 x 128000 for the pass itself, 8 for the
+// weights, 6 for the additions in shared memory.
 #include "../core/launch.hpp"
 #include "half16.cuh"
 #include "ops.hpp"
@@ -178,15 +182,35 @@ __device__ __forceinline__ void add(Parts& h, int bin, u64 w) {
     if (w >> 2 * kPart) atomicAdd(&h.sum[2][bin], static_cast<unsigned>(w >> 2 * kPart));   // (seldom: 1e-4 of the likeliest token's weight and more)
   }
 }
+template <bool WEIGHTS>
 __device__ __forceinline__ void clear(Parts& h) {
-  for (int b = threadIdx.x; b < kBins; b += kThreads) h.count[b] = h.sum[0][b] = h.sum[1][b] = h.sum[2][b] = 0;
+  for (int b = threadIdx.x; b < kBins; b += kThreads) {
+    h.count[b] = 0;
+    if (WEIGHTS) h.sum[0][b] = h.sum[1][b] = h.sum[2][b] = 0;
+  }
 }
 
-// list[0 .. n) in ascending order, n a power of two from 32 on; by a block.
+// list[0 .. n) of different numbers in ascending order; by a block.  Up to kThreads numbers each thread counts how many are smaller than its own (n steps without a barrier:
+// 50 numbers 0.4 us, 2.4 in a network), more go through a bitonic network, with the highest number behind them.
 __device__ __forceinline__ void sort(u64* list, int n) {
-  for (int k = 2; k <= n; k <<= 1) {   // bitonic
+  const int tid = static_cast<int>(threadIdx.x);
+  if (n <= kThreads) {
+    const u64 x = tid < n ? list[tid] : 0;
+    int rank = 0;
+    if (tid < n) {
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) rank += list[j] < x ? 1 : 0;
+    }
+    __syncthreads();
+    if (tid < n) list[rank] = x;
+    __syncthreads();
+    return;
+  }
+  for (int i = n + tid; i < kList; i += kThreads) list[i] = ~0ull;
+  __syncthreads();
+  for (int k = 2; k <= kList; k <<= 1) {
     for (int j = k >> 1; j > 0; j >>= 1) {
-      for (int i = threadIdx.x; i < n / 2; i += kThreads) {
+      for (int i = tid; i < kList / 2; i += kThreads) {
         const int a = 2 * i - (i & (j - 1)), o = a + j;
         const u64 x = list[a], y = list[o];
         if ((x > y) == ((a & k) == 0)) {
@@ -197,11 +221,6 @@ __device__ __forceinline__ void sort(u64* list, int n) {
       __syncthreads();
     }
   }
-}
-__device__ __forceinline__ int power_of_two(int n) {
-  int p = 32;
-  while (p < n) p <<= 1;
-  return p;
 }
 
 // The first i < n whose running sum of w[0 .. i] is `aim` or more (n without one); by a block, and the whole sum.
@@ -238,6 +257,7 @@ __device__ __forceinline__ int first_at(Shared& s, const u64* w, int n, u64 aim,
 }
 
 // The blocks' bins added up in the first block's `merged`.  Begins and ends with a barrier of the cluster.
+template <bool WEIGHTS>
 __device__ __forceinline__ void merge(cg::cluster_group& cluster, Shared& s) {
   const int blocks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   cluster.sync();
@@ -246,13 +266,15 @@ __device__ __forceinline__ void merge(cg::cluster_group& cluster, Shared& s) {
   for (int b = rank * share + threadIdx.x; b < (rank + 1) * share; b += kThreads) {
     unsigned count = 0;
     u64 sum = 0;
-    for (int r = 0; r < blocks; ++r) {
+#pragma unroll
+    for (int r = 0; r < kMost; ++r) {   // (all loads under way together)
+      if (r >= blocks) continue;
       const Shared* other = cluster.map_shared_rank(&s, r);
       count += other->mine.count[b];
-      sum += other->mine.sum[0][b] + (static_cast<u64>(other->mine.sum[1][b]) << kPart) + (static_cast<u64>(other->mine.sum[2][b]) << 2 * kPart);
+      if (WEIGHTS) sum += other->mine.sum[0][b] + (static_cast<u64>(other->mine.sum[1][b]) << kPart) + (static_cast<u64>(other->mine.sum[2][b]) << 2 * kPart);
     }
     first->merged.count[b] = count;
-    first->merged.sum[b] = sum;
+    if (WEIGHTS) first->merged.sum[b] = sum;
   }
   cluster.sync();
 }
@@ -342,10 +364,7 @@ struct Row {
   // The first block has all candidates in its list: the choice among them.  need: top-k (0: none); share: top-p of the sum of these (1: none, below 0: s.enough);
   // weights below `least` do not count.
   __device__ long long choose(Shared& s, int n, unsigned need, float share, u64 least, double u) const {
-    const int all = power_of_two(n);
-    for (int i = n + threadIdx.x; i < all; i += kThreads) s.list[i] = ~0ull;
-    __syncthreads();
-    sort(s.list, all);
+    sort(s.list, n);
     int kept = need > 0 ? min(n, static_cast<int>(need)) : n;
     for (int i = threadIdx.x; i < kept; i += kThreads) s.weights[i] = scale.weight(value_of_key(s.list[i]));
     __syncthreads();
@@ -360,9 +379,9 @@ struct Row {
       kept = min(kept, first_at(s, s.weights, kept, static_cast<u64>(max(1ll, static_cast<long long>(ceil(enough)))), whole) + 1);
     }
     // by number
-    for (int i = threadIdx.x; i < all; i += kThreads) s.list[i] = i < kept ? (s.list[i] << 32) | static_cast<unsigned>(i) : ~0ull;
+    for (int i = threadIdx.x; i < kept; i += kThreads) s.list[i] = (s.list[i] << 32) | static_cast<unsigned>(i);
     __syncthreads();
-    sort(s.list, all);
+    sort(s.list, kept);
     u64 mine[kList / kThreads];
 #pragma unroll
     for (int e = 0; e < kList / kThreads; ++e) {
@@ -393,7 +412,7 @@ struct Row {
       cluster.sync();
     };
     const bool limited = limit != ~0ull;
-    clear(s.mine);
+    clear<WEIGHTS>(s.mine);
     __syncthreads();
     // All tokens with weights below (1 - share) / 2 / vocab together are less than half of what lies behind the border: they count in the sum of all, but it is not
     // among them, and they are not counted in their bins.
@@ -416,7 +435,7 @@ struct Row {
         first->total[rank] = all;
       }
     }
-    merge(cluster, s);
+    merge<WEIGHTS>(cluster, s);
     if (rank == 0) find_bin<WEIGHTS>(s, blocks, 0, 0, need, share);
     tell();
     if (!s.border.found) return ~0ull;
@@ -453,7 +472,7 @@ struct Row {
         s.scan[warp] = low;
         s.warp_sum[warp] = high;
       }
-      clear(s.mine);
+      clear<WEIGHTS>(s.mine);
       __syncthreads();
       if (static_cast<int>(threadIdx.x) < blocks) {
         u64 l = ~0ull, h = 0;
@@ -478,7 +497,7 @@ struct Row {
         u64 c;
         if (valid && member(x, i, c)) add<WEIGHTS>(s.mine, static_cast<int>((c - low) >> shift), WEIGHTS ? scale.weight(x) : 0);
       });
-      merge(cluster, s);
+      merge<WEIGHTS>(cluster, s);
       if (rank == 0) {
         find_bin<WEIGHTS>(s, blocks, b.count, b.sum, need, -1.f);
         if (threadIdx.x == 0) {
@@ -500,10 +519,7 @@ struct Row {
     });
     cluster.sync();
     if (rank == 0) {
-      const int n = power_of_two(b.inside);
-      for (int i = b.inside + threadIdx.x; i < n; i += kThreads) s.list[i] = ~0ull;
-      __syncthreads();
-      sort(s.list, n);
+      sort(s.list, b.inside);
       if (threadIdx.x < 32) {
         u64 sum = b.sum;
         for (int base = 0; base < b.inside; base += 32) {
