@@ -30,6 +30,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     see has no influence on its result, whatever it is; an infinite or NaN value at one that is seen makes its column infinite or NaN.  In the gradients
     such numbers may reach other positions of the same text, but no other text.
 
+    For the gradients a call keeps q, k and v, its result with what its rounding left (so twice the result's memory), and the logarithms below.
+
     return_lse: also the logarithm of the sum of exponentials, fp32 ``[tokens, heads]`` (-inf where nothing is seen; no gradient)."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
