@@ -134,6 +134,17 @@ def test_rows_that_nothing_can_be_drawn_from(dtype):
     assert ops.sample(x, torch.full((8,), 0.25, device="cuda"), temperature=0.0).tolist()[1:5] == [-1] * 4
 
 
+@pytest.mark.parametrize("k", [0, 2500])
+@pytest.mark.parametrize("low", [0.3, 0.9, 1.0, 0.01, 1e-6])
+@pytest.mark.parametrize("off", [-1e-2, -1e-5, 1e-5, 1e-2])
+def test_min_p_next_to_top_p(k, low, off):
+    """What min_p keeps is a share of the weights that is a little above or below top_p."""
+    x = torch.cat([torch.zeros(7), torch.full((40,), -1.0), torch.full((3000,), -4.0), torch.full((30000,), -9.0)])[torch.randperm(33047, generator=torch.Generator().manual_seed(3))]
+    w = np.sort(np.exp(x.double().numpy()))[::-1][:k or None]
+    p = min(0.9999, w[w >= low].sum() / w.sum() * (1 + off))
+    check(x[None].expand(9, -1).cuda(), k=k, p=p, low=low)
+
+
 def test_settings_of_each_row():
     rng = np.random.default_rng(13)
     rows = 90
