@@ -45,6 +45,9 @@ struct Grad {
   int units;
 };
 
+// Every query sees one key: weights of one, no gradient of any score.
+__device__ __forceinline__ bool one_key(const Problem& p) { return p.window == 1 && p.sinks == 0; }
+
 // Rows row .. 127 of a tile: zeros.  Whole-warp call.
 template <int DP>
 __device__ __forceinline__ void zero_rows(uint8_t* tile, int row) {
@@ -335,6 +338,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               d[i] = r < rows ? a.delta[at + r] : 0.f;
               if (l[i] == -INFINITY) l[i] = INFINITY;   // sees nothing
             }
+            // A text's first query sees one key: its weight is one and its scores have no gradient, of which dP - delta would leave rounding.  Its row becomes zeros, and so do its
+            // scores and what it adds to dK.  (In tiles that are looked at, which those of texts of few tokens are; elsewhere 1e-6 of it stays.)
+            const bool lone = rows < kRows && u.block == 0 && t == 0 && row + u.place == 0;
+            if (lone && lane == 0 && fabsf(l[0]) < INFINITY) l[0] = 0.f;
             ok = n < 2 || wait(&q_empty[st], (n / 2 - 1) & 1, bad);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
@@ -352,6 +359,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               looked ^= 1u << st;
               zero_rows<DP>(s_q + st * kTile, rows);
               zero_rows<DP>(s_do + st * kTile, rows);
+              if (lone && lane < DP / 8) *reinterpret_cast<uint4*>(s_q + st * kTile + lane / 8 * kSub + lane % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
               fence_async_smem();
               __syncwarp();
               if (lane == 0) {
@@ -525,7 +533,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (ok) {   // one half takes dV out, the other dK
         const uint32_t from = (half == 0 ? t_dv : t_dk) + lanes;
-        const float scale = half == 0 ? 1.f : p.scale;
+        const float scale = half == 0 ? 1.f : (one_key(p) ? 0.f : p.scale);
         const int first_row = first_key + (warp & 3) * 32;
 #pragma unroll 1
         for (int c0 = 0; c0 < p.head_dim; c0 += 64) {
@@ -776,7 +784,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool mine = u.row + row < u.s.n;
       const long long at = static_cast<long long>(u.head) * p.tokens + u.s.q0 + u.row + row;
       float lse = mine ? a.lse[at] * kLog2e : INFINITY;
-      if (lse == -INFINITY) lse = INFINITY;   // sees nothing
+      if (lse == -INFINITY || ((pos == 0 || one_key(p)) && lse == lse)) lse = INFINITY;   // sees nothing, or one key, whose score has no gradient
       const float delta = mine ? a.delta[at] : 0.f;
       const F2 lse2 = f2(-lse, -lse);
       for (int b = blocks.next(-1); b < blocks.hi; b = blocks.next(b), ++n) {

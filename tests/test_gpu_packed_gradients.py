@@ -192,6 +192,26 @@ def test_against_differences():
         assert bound < 0.6 * abs(slope), (i, slope, bound)   # a missing or doubled part would show
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim", [(3, 3, 128), (4, 2, 64)])
+@pytest.mark.parametrize("lengths,before,window", [([1], None, None), ([1] * 40, None, None), ([1, 0, 5, 1, 100], None, None), ([300, 77, 1], None, 1), ([20, 1, 60], [700, 5, 0], 1),
+                                                   ([3, 9], [-2, -9], None)])
+def test_rows_of_one_key(lengths, before, window, heads, kv_heads, dim):
+    """Their weight is one whatever the score is: no gradient of it, not even a rounded one."""
+    dq, dk, _ = check(*make(lengths, heads, kv_heads, dim, before=before, seed=4), window=window)
+    keys = lengths if before is None else [max(0, n + m) for n, m in zip(lengths, before)]
+    row = key = 0
+    for n, m in zip(lengths, keys):
+        blind = max(0, n - m)
+        assert not dq[row:row + blind].any()
+        if window == 1:
+            assert not dq[row:row + n].any() and not dk[key:key + m].any()
+        elif m <= n and m > 0:
+            assert not dq[row + blind].any()
+            if m == 1:
+                assert not dk[key].any()
+        row, key = row + n, key + m
+
+
 @pytest.mark.parametrize("lengths,before,window,sinks", [([3] * 100, None, None, 0), ([8] * 60, None, None, 0), ([20] * 30, None, None, 0), ([300, 77], None, 2, 0), ([300, 77], None, 5, 3),
                                                          ([4] * 90, [2] * 90, 3, 1), ([500], None, None, 0)])
 def test_two_roundings_and_no_more(lengths, before, window, sinks):
