@@ -602,7 +602,7 @@ bool pairs_heads(const PackedAttentionArgs& a) {
 int head_units_of(const PackedAttentionArgs& a) { return pairs_heads(a) ? a.kv_heads * ((a.heads / a.kv_heads + 1) / 2) : a.heads; }
 long long units_of(const PackedAttentionArgs& a) { return slots_of(a.tokens, a.sequences, pairs_heads(a) ? kRows : 2 * kRows) * head_units_of(a); }
 // How many blocks share out the keys of a unit, by what it costs in microseconds: a step of a unit 2, its beginning and end 5, results in parts 4 and 0.45 per MB (12 heads
-// over 4 of 64, 8 texts of some 100 rows behind 3072 keys: 59 / 43 / 52 / 50 us in 1 / 2 / 3 / 4 parts; 16 heads of 128, 2048 rows: 47 / 61 / 73 / 81; one row over
+// over 4 of 64, 8 texts of some 100 rows behind some 3000 keys: 59 / 43 / 52 / 50 us in 1 / 2 / 3 / 4 parts; 16 heads of 128, 2048 rows: 47 / 61 / 73 / 81; one row over
 // 16384 keys 228 in one, 36 in 16).  The host knows no lengths: an average sequence, whose last tile is half full.
 int parts_of(const PackedAttentionArgs& a) {
   const int rows = pairs_heads(a) ? kRows : 2 * kRows;
