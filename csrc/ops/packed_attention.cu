@@ -134,14 +134,15 @@ __device__ __forceinline__ Unit unit_of(const Forward& a, int u) {
   return r;
 }
 
-// The columns, of 64 from c0 on, in which a value that a row sees in one of the blocks that were looked at is not finite.
+// The columns, of 64 from c0 on, in which a value that a row of the text sees in one of the blocks that were looked at is not finite.
 template <typename H>
 __device__ __noinline__ unsigned long long odd_columns(const Problem& p, const TokenView& v, const Unit& u, const Blocks& blocks, int pos, int c0) {
   unsigned long long marks = 0;
   const typename H::T* from = static_cast<const typename H::T*>(v.p) + u.head[0] / p.group * v.head + static_cast<long long>(u.s.k0) * v.token + c0;
   for (int b = blocks.next(-1); b < blocks.hi; b = blocks.next(b)) {
     if (u.whole(b)) continue;
-    for (int j = b * kRows; j < min(b * kRows + kRows, pos + 1); ++j) {
+    const BlockKeys keys = block_keys(b, pos, u.s.m);
+    for (int j = keys.first; j < keys.end; ++j) {
       if (j <= pos - p.window && j >= p.sinks) continue;
       for (int e = 0; e < 64 && c0 + e < p.head_dim; ++e)
         if (!(fabsf(H::up(from[j * v.token + e])) < INFINITY)) marks |= 1ull << e;
@@ -518,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           float f[64];
 #pragma unroll
           for (int e = 0; e < 64; ++e) f[e] = none ? 0.f : __uint_as_float(o[e / 32][e % 32]) * inv;
-          if (odd) {
+          if (odd && mine) {   // (rows behind the text are another's, or none)
             const unsigned long long marks = odd_columns<H>(p, a.v, u, blocks, pos, c0);
 #pragma unroll
             for (int e = 0; e < 64; ++e) f[e] = (marks >> e) & 1 ? NAN : f[e];

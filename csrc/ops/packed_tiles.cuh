@@ -6,6 +6,7 @@
 #include "half16.cuh"
 #include "ops.hpp"
 #include "packed.hpp"
+#include "packed_keys.hpp"
 #include "tcgen05.cuh"
 
 #include <type_traits>
@@ -17,7 +18,6 @@ int* gemm_error_device_ptr();
 
 namespace packed {
 
-constexpr int kRows = 128;                 // queries of a tile, and keys of a block
 constexpr int kSub = kRows * 64 * 2;       // a tile's 64 columns: rows of 128 bytes with the 128-byte swizzle, 16 KB
 constexpr float kLog2e = 1.4426950408889634f;
 
