@@ -24,8 +24,8 @@ void need_no_tangent(const at::Tensor& t, const char* what) {
 // A backward pass that would itself be differentiated.
 void need_first_order(const char* what) { MCCL_CHECK_TENSOR(!at::GradMode::is_enabled(), what << ": has no second derivative (create_graph)"); }
 
-// As tensor maps and 16-byte accesses take them: gradients and expanded tensors come in any strides.
-at::Tensor rows_of_heads(const at::Tensor& t) { return vector_rows(t) && !repeated(t) ? t : t.contiguous(); }
+// As tensor maps and 16-byte accesses take them: gradients come in any strides and from any place on (contiguous() would leave one that only begins off a 16-byte boundary as it is).
+at::Tensor rows_of_heads(const at::Tensor& t) { return vector_rows(t) && !repeated(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
 
 // The operands of a call as the kernels take them.
 struct Attention {

@@ -30,3 +30,24 @@ def test_values_of_the_last_text_that_are_not_finite(lengths, before, heads, kv_
         columns = torch.arange(dim, device="cuda") != 5
         assert not torch.isfinite(o[sees][:, :group, 5]).any()
         assert torch.equal(o[~sees], good[~sees]) and torch.equal(o[:, group:], good[:, group:]) and torch.equal(o[:, :group][..., columns], good[:, :group][..., columns])
+
+
+@pytest.mark.parametrize("elements", [1, 3, 4])
+def test_gradients_that_begin_off_a_boundary(elements):
+    """What the gradient of a concatenation hands on is contiguous and begins anywhere."""
+    q, k, v, offsets, _ = make([300], 4, 2, 64, poison=False)
+    front = torch.zeros(elements, dtype=q.dtype, device="cuda")
+    g = torch.randn(q.shape, generator=torch.Generator().manual_seed(1)).to(q.dtype).cuda()
+    shifted = torch.cat([front, g.flatten()])[elements:].view(q.shape)
+    assert shifted.is_contiguous() and shifted.data_ptr() % 16
+
+    def gradients(f, leaves, grad):
+        leaves = [t.detach().requires_grad_() for t in leaves]
+        return torch.autograd.grad(f(*leaves), leaves, grad)
+
+    rope = ops.rotary_tables(300, 64)
+    for f, inputs in ((lambda *x: ops.packed_attention(*x, offsets), (q, k, v)), (lambda x: ops.rotary(x, rope=rope), (q,)),
+                      (lambda x, y: ops.rotary(x, y, rope=rope, layout="half")[0], (q, k))):
+        want = gradients(f, inputs, g)
+        for got in (gradients(f, inputs, shifted), gradients(lambda *x: torch.cat([front, f(*x).flatten()]), inputs, torch.cat([front, g.flatten()]))):
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
