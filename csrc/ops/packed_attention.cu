@@ -173,8 +173,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* q_empty = o_full + 2;
   uint64_t* plan_barriers = q_empty + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(plan_barriers + Plan::kBarriers);
-  volatile int* bad = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  uint4* s_next = reinterpret_cast<uint4*>((reinterpret_cast<uintptr_t>(tmem_slot + 2) + 15) & ~static_cast<uintptr_t>(15));
+  volatile int* bad = reinterpret_cast<volatile int*>(tmem_slot + 1);   // [2]
+  uint4* s_next = reinterpret_cast<uint4*>((reinterpret_cast<uintptr_t>(tmem_slot + 3) + 15) & ~static_cast<uintptr_t>(15));
   Unit* s_unit = reinterpret_cast<Unit*>(s_next + 1);   // [2]
   const Plan plan = Plan::at(plan_barriers, s_next, bad);
 
@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc::tma_prefetch_desc(&tm_v);
     tc::tma_prefetch_desc(&tm_o);
     plan.init(kRoles);
-    *bad = 0;
+    bad[0] = bad[1] = 0;
     tc::mbar_init_fence();
   }
   if (warp == 8) tc::tmem_alloc(tmem_slot, 512);
@@ -264,6 +264,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               load_tile<DP>(s_kv + 2 * st * kTile, &tm_v, look ? &raw_full[st] : &kv_full[st], kv, u.s.k0 + before * kRows);
             }
             if (more) load_tile<DP>(s_kv + (2 * st + 1) * kTile, &tm_k, &kv_full[st], kv, u.s.k0 + b * kRows);
+            if ((i & 15) == 0) goes_on(bad);
             before = more ? b : -1;
             if (more) b = u.all.next(b);
           }
@@ -293,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int b = u.all.next(-1); b < u.all.hi; b = u.all.next(b), ++i) {
           if (u.whole(b)) continue;
           const int st = i % kStages, rows = min(kRows, u.s.m - b * kRows);
-          ok = wait(&raw_full[st], (phase >> st) & 1, bad);
+          ok = wait_unit(&raw_full[st], (phase >> st) & 1, bad);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           phase ^= 1u << st;

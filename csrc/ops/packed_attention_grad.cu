@@ -231,8 +231,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* ds_full = p_full + 2;    // [2]
   uint64_t* plan_barriers = ds_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(plan_barriers + Plan::kBarriers);
-  volatile int* bad = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  uint4* s_next = reinterpret_cast<uint4*>((reinterpret_cast<uintptr_t>(tmem_slot + 2) + 15) & ~static_cast<uintptr_t>(15));
+  volatile int* bad = reinterpret_cast<volatile int*>(tmem_slot + 1);   // [2]
+  uint4* s_next = reinterpret_cast<uint4*>((reinterpret_cast<uintptr_t>(tmem_slot + 3) + 15) & ~static_cast<uintptr_t>(15));
   KeyUnit* s_unit = reinterpret_cast<KeyUnit*>(s_next + 1);   // [2]
   const Plan plan = Plan::at(plan_barriers, s_next, bad);
 
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tid == 0) {
     for (uint64_t* b = k_full; b < plan_barriers; ++b) tc::mbar_init(b, b >= p_full ? 8 : (b == s_full || b == s_full + 1 ? 2 : 1));
     plan.init(kRoles);
-    *bad = 0;
+    bad[0] = bad[1] = 0;
     tc::mbar_init_fence();
   }
   if (warp == 8) tc::tmem_alloc(tmem_slot, 512);
@@ -305,6 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!ok) break;
                 bring(s_q, &tm_q, &q_full[st]);
               }
+              if ((n & 15) == 0) goes_on(bad);
             }
           }
           if (!ok) {   // loads that were issued must land before the block retires
@@ -622,8 +623,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* ds_full = dp_full + 1;  // [2]: halves of each half's columns
   uint64_t* plan_barriers = ds_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(plan_barriers + Plan::kBarriers);
-  volatile int* bad = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  uint4* s_next = reinterpret_cast<uint4*>((reinterpret_cast<uintptr_t>(tmem_slot + 2) + 15) & ~static_cast<uintptr_t>(15));
+  volatile int* bad = reinterpret_cast<volatile int*>(tmem_slot + 1);   // [2]
+  uint4* s_next = reinterpret_cast<uint4*>((reinterpret_cast<uintptr_t>(tmem_slot + 3) + 15) & ~static_cast<uintptr_t>(15));
   QueryUnit* s_unit = reinterpret_cast<QueryUnit*>(s_next + 1);   // [2]
   const Plan plan = Plan::at(plan_barriers, s_next, bad);
 
@@ -632,7 +633,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tid == 0) {
     for (uint64_t* b = q_full; b < plan_barriers; ++b) tc::mbar_init(b, b >= ds_full ? 8 : 1);
     plan.init(kRoles);
-    *bad = 0;
+    bad[0] = bad[1] = 0;
     tc::mbar_init_fence();
   }
   if (warp == 8) tc::tmem_alloc(tmem_slot, 512);
@@ -687,6 +688,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) break;
             tc::mbar_expect_tx(&v_full[st], kTile);
             load_tile<DP>(s_v + st * kTile, &tm_v, &v_full[st], kv, row);
+            if ((n & 15) == 0) goes_on(bad);
           }
           if (!ok) {   // loads that were issued must land before the block retires
             for (uint64_t* b = q_full; b < s_full; ++b) {
@@ -710,7 +712,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int b = u.b.next(-1); b < u.b.hi; b = u.b.next(b), ++n) {
           const int st = n & 1, rows = u.s.m - b * kRows;
           if (rows >= kRows) continue;
-          ok = wait(&raw[st], (looked >> st) & 1, bad);
+          ok = wait_unit(&raw[st], (looked >> st) & 1, bad);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           looked ^= 1u << st;

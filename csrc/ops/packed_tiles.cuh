@@ -274,11 +274,27 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// A wait that gives up, and at once when another role of the block has: the first to give up says so in *bad.
+// A block's two words on its waits: [0] a role has given up, [1] counts what goes on: units looked for, and every 16th step of loads.
+__device__ __forceinline__ void goes_on(volatile int* bad) { atomicAdd(const_cast<int*>(bad) + 1, 1); }
+// A wait for another role's part of a step that gives up, and at once when another role of the block has: the first to give up says so in *bad.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* bad) {
-  for (uint32_t i = 0; i < (1u << 17); ++i) {   // a second or so: the instruction itself waits for some microseconds
+  for (uint32_t i = 0; i < (1u << 17); ++i) {   // 0.2 s: the instruction itself waits for 1.5 us
     if (tc::mbar_try_wait(bar, parity)) return true;
     if ((i & 15) == 15 && *bad) return false;
+  }
+  *bad = 1;
+  return false;
+}
+// A wait that may be for a whole unit, of any number of steps (a block of keys that a million rows of 128 heads see takes 2 s): gives up where nothing goes on for as long as above.
+__device__ __forceinline__ bool wait_unit(uint64_t* bar, uint32_t parity, volatile int* bad) {
+  for (int steps = bad[1];;) {
+    for (uint32_t i = 0; i < (1u << 17); ++i) {
+      if (tc::mbar_try_wait(bar, parity)) return true;
+      if ((i & 15) == 15 && *bad) return false;
+    }
+    const int now = bad[1];
+    if (now == steps) break;
+    steps = now;
   }
   *bad = 1;
   return false;
@@ -312,7 +328,7 @@ struct Plan {
   uint64_t* answer;      // of the request for the next one
   uint64_t* loads_done;  // the unit's last loads are under way: no earlier is the next one asked for, another block may be free sooner
   uint4* next;
-  volatile int* bad;
+  volatile int* bad;     // [2]
   static constexpr int kBarriers = 6;
   __device__ __forceinline__ static Plan at(uint64_t* barriers, uint4* next, volatile int* bad) { return {barriers, barriers + 2, barriers + 4, barriers + 5, next, bad}; }
   __device__ __forceinline__ void init(int roles) const {   // one thread
@@ -326,7 +342,7 @@ struct Plan {
   // Unit k of this block is described (false: there is none).  Whole warps.
   template <typename Unit>
   __device__ __forceinline__ bool take(const Unit* units, int k) const {
-    const bool ok = wait(&full[k & 1], (k >> 1) & 1, bad);
+    const bool ok = wait_unit(&full[k & 1], (k >> 1) & 1, bad);
     return __all_sync(0xffffffffu, ok) && !units[k & 1].end;
   }
   __device__ __forceinline__ void give_back(int k) const {
@@ -341,6 +357,7 @@ struct Plan {
     auto free = [&](int k) { return __all_sync(0xffffffffu, k < 2 || wait(&empty[k & 1], ((k >> 1) - 1) & 1, bad)); };
     for (int k = 0;;) {
       const Unit found = find(id);
+      if (lane == 0) goes_on(bad);   // (there may be many without work)
       if (found.any) {
         if (!free(k)) return;
         if (lane == 0) {
@@ -348,7 +365,7 @@ struct Plan {
           tc::mbar_arrive(&full[k & 1]);
         }
         __syncwarp();
-        const bool near = wait(loads_done, k & 1, bad);
+        const bool near = wait_unit(loads_done, k & 1, bad);
         if (!__all_sync(0xffffffffu, near)) return;
         ++k;
       }

@@ -51,3 +51,33 @@ def test_gradients_that_begin_off_a_boundary(elements):
         want = gradients(f, inputs, g)
         for got in (gradients(f, inputs, shifted), gradients(lambda *x: torch.cat([front, f(*x).flatten()]), inputs, torch.cat([front, g.flatten()]))):
             assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_units_of_work_that_take_seconds():
+    """A block of keys that all rows of 128 heads see: a million steps of one block of the grid, more than a second, in which others of its warps wait for the next unit.
+
+    Every row but the first sees the first position and itself, with scores of zero and so weights of one half; the numbers are small and whole, so every sum is exact."""
+    tokens, heads, dim, scale = 1_000_000, 128, 8, 0.25
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    whole = lambda *sizes: torch.randint(-1, 2, sizes, generator=gen, device="cuda", dtype=torch.int8).to(torch.bfloat16)
+    q = torch.zeros(tokens, heads, dim, dtype=torch.bfloat16, device="cuda").requires_grad_()
+    k, v = (whole(tokens, 1, dim).requires_grad_() for _ in range(2))
+    g = whole(tokens, heads, dim)
+    o = ops.packed_attention(q, k, v, offsets_of([tokens]), window=1, sinks=1, scale=scale)
+    dq, dk, dv = torch.autograd.grad(o, (q, k, v), g)
+    k, v = k.detach().float()[:, 0], v.detach().float()[:, 0]
+    assert not dk.any()   # (of queries that are zeros)
+    first = torch.zeros(dim, dtype=torch.float64, device="cuda")
+    for a in range(0, tokens, 100_000):
+        part, kk, vv = slice(a, a + 100_000), k[a:a + 100_000], v[a:a + 100_000]
+        gg = g[part].float()
+        assert torch.equal(o[part].float(), ((v[0] + vv) / 2)[:, None].expand(-1, heads, -1))
+        own = gg.sum(1, dtype=torch.float64) / 2
+        first += own.sum(0)
+        if a == 0:
+            first += own[0]   # the first row sees one key, with a weight of one
+        seen = slice(1 if a == 0 else 0, None)
+        assert torch.equal(dv[part][seen, 0], own[seen].to(torch.bfloat16))
+        ds = ((gg @ v[0])[..., None] - (gg * vv[:, None]).sum(-1, keepdim=True)) / 4   # of the first position's score; the own one's is the opposite
+        assert torch.equal(dq[part], (scale * (ds * k[0] - ds * kk[:, None])).to(torch.bfloat16))
+    assert torch.equal(dv[0, 0], first.to(torch.bfloat16))
