@@ -61,10 +61,10 @@ __device__ __forceinline__ void zero_rows(uint8_t* tile, int row) {
 // delta[h, t] = sum_d dO[t, h, d] O[t, h, d], with O as it was before it was rounded (its rounding would be the same for all of a row's scores: dQ and dK were off
 // by 1.5 to 1.6 times what their own rounding leaves, now by 1.4).  A warp per 32 rows of a head, LANES lanes per row.
 // Rows that see up to kFew keys: O's weights were rounded to 16 bits, which few keys do not even out (gradients off by 1.53 times their own rounding where rows see 2 to 4
-// keys); delta is the sum of p dP itself there, from q, k and v (1.42).  Only where the sizes let expect many of them (FEW): finding a row's text costs every warp a chain of loads
-// (32 texts up to 256 of 8 heads of 64, forward and gradients, 86 -> 93 us).
+// keys); delta is the sum of p dP itself there, from q, k and v (1.42).  Each row's own number of keys decides, not what else is in the batch; a warp finds its rows' texts by 32 probes at
+// a time, the first of which are under way beside the rows.
 constexpr int kFew = 8;
-template <int LANES, bool FEW>
+template <int LANES>
 __global__ void __launch_bounds__(256) packed_delta_kernel(const Problem p, const H::T* o, const H::T* o_rest, TokenView q, TokenView k, TokenView v, TokenView d_o, float* delta) {
   pdl_wait();
   pdl_trigger();
@@ -72,6 +72,8 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(const Problem p, cons
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, in = lane / LANES, c = (lane % LANES) * 8;
   const int h = blockIdx.y * 8 + warp, t0 = blockIdx.x * 32, tokens = p.tokens, heads = p.heads, head_dim = p.head_dim;
   if (h >= heads) return;
+  int text = 0, texts = p.sequences, step = (texts + 31) / 32;   // the last text that begins at t0 or before is one of `texts` from `text` on
+  int begins = lane * step < texts ? __ldg(p.offsets + lane * step) : INT_MAX;
   float mine = 0.f;
 #pragma unroll 8
   for (int i = 0; i < LANES; ++i) {
@@ -91,73 +93,108 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(const Problem p, cons
     sum = __shfl_sync(0xffffffffu, sum, (lane % kAtOnce) * LANES);
     if (lane / kAtOnce == i) mine = sum;
   }
-  if (!FEW) {
-    if (t0 + lane < tokens) delta[static_cast<long long>(h) * tokens + t0 + lane] = mine;
-    return;
+  for (;;) {
+    const int before = max(1, __popc(__ballot_sync(0xffffffffu, begins <= t0)));   // (offsets do not decrease)
+    text += (before - 1) * step;
+    texts = min(step, texts - (before - 1) * step);
+    if (texts <= 1) break;
+    step = (texts + 31) / 32;
+    begins = lane * step < texts ? __ldg(p.offsets + text + lane * step) : INT_MAX;
   }
-  // this lane's row: its text is the last one that begins at it or before; keys first[0 .. head) and from[0 .. count - head)
+  // this lane's row: its text is the last one that begins at it or before, one of the 31 from here on or else (texts without tokens) looked for; keys first[0 .. head) and
+  // from[0 .. count - head)
   int count = 0, head = 0, from = 0, first = 0;
-  if (t0 + lane < tokens) {
-    int lo = 0, n = p.sequences;
-    while (n > 1) {
-      const int half = n >> 1;
-      if (__ldg(p.offsets + lo + half) <= t0 + lane) lo += half, n -= half;
-      else n = half;
+  {
+    const int t = t0 + lane, here = min(text + lane, p.sequences), begin = __ldg(p.offsets + here), k_begin = __ldg(p.k_offsets + here);
+    const int later = text + lane < p.sequences ? begin : INT_MAX;
+    int s = 0;
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1)
+      if (__shfl_sync(0xffffffffu, later, s + o) <= t) s += o;
+    Sequence x;
+    x.q0 = clamp(__shfl_sync(0xffffffffu, begin, s), 0, tokens);
+    x.n = clamp(__shfl_sync(0xffffffffu, begin, s + 1), x.q0, tokens) - x.q0;
+    x.k0 = clamp(__shfl_sync(0xffffffffu, k_begin, s), 0, p.k_tokens);
+    x.m = clamp(__shfl_sync(0xffffffffu, k_begin, s + 1), x.k0, p.k_tokens) - x.k0;
+    if (s == 31) {
+      int lo = text + s, n = p.sequences - lo;
+      while (n > 1) {
+        const int half = n >> 1;
+        if (__ldg(p.offsets + lo + half) <= t) lo += half, n -= half;
+        else n = half;
+      }
+      x = sequence_of(p, lo);
     }
-    const Sequence s = sequence_of(p, lo);
-    const int row = t0 + lane - s.q0, pos = s.m - s.n + row;
-    if (row >= 0 && row < s.n && pos >= 0) {
+    const int row = t - x.q0, pos = x.m - x.n + row;
+    if (t < tokens && row >= 0 && row < x.n && pos >= 0) {
       from = max(0, pos - p.window + 1);
       head = min(p.sinks, from);
       count = pos - from + 1 <= kFew && pos - from + 1 + head <= kFew ? pos - from + 1 + head : 0;
-      first = s.k0;
+      first = x.k0;
     }
   }
-  if (__any_sync(0xffffffffu, count > 0)) {
-#pragma unroll 1
-    for (int i = 0; i < LANES; ++i) {
-      const int r = kAtOnce * i + in;
-      const int n = __shfl_sync(0xffffffffu, count, r), n_head = __shfl_sync(0xffffffffu, head, r), n_from = __shfl_sync(0xffffffffu, from, r), n_first = __shfl_sync(0xffffffffu, first, r);
-      if (!__any_sync(0xffffffffu, n > 0)) continue;
-      const bool mine_too = n > 0 && c < head_dim;
+  // kAtOnce of these rows at a time (one key has a weight of one, and its score no gradient)
+  for (unsigned rows = __ballot_sync(0xffffffffu, count > 1); rows != 0;) {
+    int of[kAtOnce], r = -1;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      of[i] = __ffs(rows) - 1;
+      rows &= rows - 1;
+      if (i == in) r = of[i];
+    }
+    const int n_ = __shfl_sync(0xffffffffu, count, max(r, 0)), n_head = __shfl_sync(0xffffffffu, head, max(r, 0)), n_from = __shfl_sync(0xffffffffu, from, max(r, 0)),
+              n_first = __shfl_sync(0xffffffffu, first, max(r, 0)), n = r < 0 ? 0 : n_;
+    float score[kFew] = {}, dp[kFew] = {};
+    if (n > 0 && c < head_dim) {   // (all loads under way together: those of keys behind the last one are of that one again)
       const long long t = t0 + r;
-      float x[8] = {}, y[8] = {}, score[kFew], dp[kFew];
-      if (mine_too) {
-        unpack8_as<H>(__ldg(reinterpret_cast<const uint4*>(static_cast<const H::T*>(q.p) + t * q.token + h * q.head + c)), x);
-        unpack8_as<H>(__ldg(reinterpret_cast<const uint4*>(static_cast<const H::T*>(d_o.p) + t * d_o.token + h * d_o.head + c)), y);
-      }
-      float top = -INFINITY;
+      const uint4 q_raw = __ldg(reinterpret_cast<const uint4*>(static_cast<const H::T*>(q.p) + t * q.token + h * q.head + c));
+      const uint4 d_raw = __ldg(reinterpret_cast<const uint4*>(static_cast<const H::T*>(d_o.p) + t * d_o.token + h * d_o.head + c));
+      uint4 k_raw[kFew], v_raw[kFew];
 #pragma unroll
       for (int j = 0; j < kFew; ++j) {
-        score[j] = dp[j] = 0.f;
-        if (mine_too && j < n) {
-          const long long key = n_first + (j < n_head ? j : n_from + j - n_head);
-          float a[8], b[8];
-          unpack8_as<H>(__ldg(reinterpret_cast<const uint4*>(static_cast<const H::T*>(k.p) + key * k.token + h / p.group * k.head + c)), a);
-          unpack8_as<H>(__ldg(reinterpret_cast<const uint4*>(static_cast<const H::T*>(v.p) + key * v.token + h / p.group * v.head + c)), b);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            score[j] = fmaf(x[e], a[e], score[j]);
-            dp[j] = fmaf(y[e], b[e], dp[j]);
-          }
-        }
-#pragma unroll
-        for (int s = LANES / 2; s >= 1; s >>= 1) {
-          score[j] += __shfl_xor_sync(0xffffffffu, score[j], s);
-          dp[j] += __shfl_xor_sync(0xffffffffu, dp[j], s);
-        }
-        if (j < n) top = fmaxf(top, score[j]);
+        const int at = min(j, n - 1);
+        const long long key = n_first + (at < n_head ? at : n_from + at - n_head);
+        k_raw[j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const H::T*>(k.p) + key * k.token + h / p.group * k.head + c));
+        v_raw[j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const H::T*>(v.p) + key * v.token + h / p.group * v.head + c));
       }
-      float sum = 0.f, all = 0.f;
+      float x[8], y[8];
+      unpack8_as<H>(q_raw, x);
+      unpack8_as<H>(d_raw, y);
 #pragma unroll
       for (int j = 0; j < kFew; ++j) {
-        if (j >= n) continue;
-        const float w = exp2f((score[j] - top) * p.scale_log2);
-        sum = fmaf(w, dp[j], sum);
-        all += w;
+        float a[8], b[8];
+        unpack8_as<H>(k_raw[j], a);
+        unpack8_as<H>(v_raw[j], b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          score[j] = fmaf(x[e], a[e], score[j]);
+          dp[j] = fmaf(y[e], b[e], dp[j]);
+        }
       }
-      sum = __shfl_sync(0xffffffffu, sum / all, (lane % kAtOnce) * LANES);
-      if (lane / kAtOnce == i && count > 0) mine = sum;
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < kFew; ++j) {
+#pragma unroll
+      for (int s = LANES / 2; s >= 1; s >>= 1) {
+        score[j] += __shfl_xor_sync(0xffffffffu, score[j], s);
+        dp[j] += __shfl_xor_sync(0xffffffffu, dp[j], s);
+      }
+      if (j < n) top = fmaxf(top, score[j]);
+    }
+    float sum = 0.f, all = 0.f;
+#pragma unroll
+    for (int j = 0; j < kFew; ++j) {
+      if (j >= n) continue;
+      const float w = exp2f((score[j] - top) * p.scale_log2);
+      sum = fmaf(w, dp[j], sum);
+      all += w;
+    }
+    sum /= all;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const float its = __shfl_sync(0xffffffffu, sum, i * LANES);
+      if (lane == of[i]) mine = its;
     }
   }
   if (t0 + lane < tokens) delta[static_cast<long long>(h) * tokens + t0 + lane] = mine;
@@ -893,14 +930,8 @@ cudaError_t launch(const PackedAttentionGradArgs& args, cudaStream_t stream) {
   cudaError_t rc = raise_smem_limit(packed_grad_keys_kernel<DP>, key_smem<DP>(), allowed_keys);
   if (rc == cudaSuccess) rc = raise_smem_limit(packed_grad_queries_kernel<DP>, query_smem<DP>(), allowed_queries);
   if (rc != cudaSuccess) return rc;
-  // windows of a few positions, or texts of a few tokens on average (from 24 on most rows see more than kFew keys, and dQ and dK are off by less than 1.47 times their rounding)
-  const bool few = static_cast<long long>(g.p.window) + g.p.sinks <= kFew || f.tokens / f.sequences < 24;
   const dim3 groups((f.tokens + 31) / 32, (f.heads + 7) / 8);
-  if (few) {
-    MCCL_LAUNCH_PDL((packed_delta_kernel<DP / 8, true>), groups, 256, 0, stream, g.p, static_cast<const H::T*>(f.o), static_cast<const H::T*>(f.o_rest), f.q, f.k, f.v, args.d_o, args.delta);
-  } else {
-    MCCL_LAUNCH_PDL((packed_delta_kernel<DP / 8, false>), groups, 256, 0, stream, g.p, static_cast<const H::T*>(f.o), static_cast<const H::T*>(f.o_rest), f.q, f.k, f.v, args.d_o, args.delta);
-  }
+  MCCL_LAUNCH_PDL(packed_delta_kernel<DP / 8>, groups, 256, 0, stream, g.p, static_cast<const H::T*>(f.o), static_cast<const H::T*>(f.o_rest), f.q, f.k, f.v, args.d_o, args.delta);
   g.units = static_cast<int>(keys);
   MCCL_LAUNCH_PDL(packed_grad_keys_kernel<DP>, g.units, kThreads, key_smem<DP>(), stream, q, k, v, d_o, dk, dv, g);
   g.units = static_cast<int>(queries);

@@ -7,6 +7,7 @@ import torch
 
 from mccl_b200 import ops
 from tests.test_gpu_packed_attention import make, offsets_of
+from tests.test_gpu_packed_gradients import exact, run
 
 pytestmark = pytest.mark.gpu
 
@@ -81,3 +82,24 @@ def test_units_of_work_that_take_seconds():
         ds = ((gg @ v[0])[..., None] - (gg * vv[:, None]).sum(-1, keepdim=True)) / 4   # of the first position's score; the own one's is the opposite
         assert torch.equal(dq[part], (scale * (ds * k[0] - ds * kk[:, None])).to(torch.bfloat16))
     assert torch.equal(dv[0, 0], first.to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("short,long,window,sinks", [([3] * 160, [5000], None, 0), ([8] * 160, [5000, 0, 3000], None, 0), ([2, 0, 0, 5] * 80, [6000], None, 0), ([1, 4, 7] * 60, [5000], 400, 2)])
+def test_gradients_of_short_texts_do_not_depend_on_the_batch(short, long, window, sinks):
+    """dQ and dK of short texts beside long ones: rounded themselves, and sums of gradients of scores that were rounded (2^0.5 times what rounding the exact ones leaves, everything else
+    a sixth of that at most: 1.5 times), as where they are alone, and the same bits."""
+    lengths, rows = short + long, sum(short)
+    q, k, v, offsets, _ = make(lengths, 4, 4, 64, poison=False, seed=len(lengths))
+    g = torch.randn(q.shape, generator=torch.Generator().manual_seed(7)).to(q.dtype).cuda()
+    _, got = run(q, k, v, g, offsets, window=window, sinks=sinks)
+    alone = offsets_of(short)
+    want, _ = exact(q[:rows], k[:rows], v[:rows], g[:rows], alone, None, 0.125, window, sinks)
+    for name, a, b in list(zip("qkv", got, want))[:2]:
+        assert (a[:rows].double() - b).norm() <= 1.5 * (b.to(torch.bfloat16).double() - b).norm(), name
+    _, again = run(*(t[:rows] for t in (q, k, v, g)), alone, window=window, sinks=sinks)
+    assert all(torch.equal(a[:rows], b) for a, b in zip(got, again))
+    # and behind the long ones, where they begin at other places of a tile
+    behind = offsets_of(long + short)
+    moved = [torch.cat((t[rows:], t[:rows])) for t in (q, k, v, g)]
+    _, last = run(*moved, behind, window=window, sinks=sinks)
+    assert all(torch.equal(a[-rows:], b) for a, b in zip(last, again))
