@@ -376,10 +376,6 @@ __global__ void __launch_bounds__(kThreads, 1)
               d[i] = r < rows ? a.delta[at + r] : 0.f;
               if (l[i] == -INFINITY) l[i] = INFINITY;   // sees nothing
             }
-            // A text's first query sees one key: its weight is one and its scores have no gradient, of which dP - delta would leave rounding.  Its row becomes zeros, and so do its
-            // scores and what it adds to dK.  (In tiles that are looked at, which those of texts of few tokens are; elsewhere 1e-6 of it stays.)
-            const bool lone = rows < kRows && u.block == 0 && t == 0 && row + u.place == 0;
-            if (lone && lane == 0 && fabsf(l[0]) < INFINITY) l[0] = 0.f;
             ok = n < 2 || wait(&q_empty[st], (n / 2 - 1) & 1, bad);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
@@ -397,7 +393,6 @@ __global__ void __launch_bounds__(kThreads, 1)
               looked ^= 1u << st;
               zero_rows<DP>(s_q + st * kTile, rows);
               zero_rows<DP>(s_do + st * kTile, rows);
-              if (lone && lane < DP / 8) *reinterpret_cast<uint4*>(s_q + st * kTile + lane / 8 * kSub + lane % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
               fence_async_smem();
               __syncwarp();
               if (lane == 0) {
@@ -488,6 +483,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         // the columns that see my key: low <= c < high
         const bool partly = !(first >= first_key + kRows - 1 && (first + 63 - p.window < first_key || all_sinks));
         const int low = key - first, high = sink ? 64 : min(64, far - first);
+        // (the first position sees one key, with a weight of one: its score has no gradient, of which dP - delta would leave rounding)
+        const int low_ds = key == 0 ? low + 1 : low;
         ok = wait(&s_full[st], (n / 2) & 1, bad);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
@@ -549,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (partly) {
 #pragma unroll
-            for (int c = 0; c < 32; ++c) f[c] = 32 * h + c >= low && 32 * h + c < high ? f[c] : 0.f;
+            for (int c = 0; c < 32; ++c) f[c] = 32 * h + c >= low_ds && 32 * h + c < high ? f[c] : 0.f;
           }
           uint32_t x[16];
 #pragma unroll

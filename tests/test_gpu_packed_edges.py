@@ -103,3 +103,19 @@ def test_gradients_of_short_texts_do_not_depend_on_the_batch(short, long, window
     moved = [torch.cat((t[rows:], t[:rows])) for t in (q, k, v, g)]
     _, last = run(*moved, behind, window=window, sinks=sinks)
     assert all(torch.equal(a[-rows:], b) for a, b in zip(last, again))
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(3, 3, 128), (4, 2, 64)])
+@pytest.mark.parametrize("lengths,before", [([128, 256], None), ([129, 700], None), ([1, 127, 1000], None), ([300, 260], [-44, -132])])
+def test_first_positions_have_no_gradient_of_their_score(lengths, before, heads, kv_heads, dim):
+    """A first position sees one key: its weight is one whatever the score is.  With gradients in the rows of first positions alone dQ and dK are zeros, whatever else is in their tiles."""
+    q, k, v, offsets, k_offsets = make(lengths, heads, kv_heads, dim, before=before, poison=False, seed=5)
+    firsts = torch.tensor([a + max(0, -m) for a, m in zip(offsets.tolist(), before or [0] * len(lengths))], device="cuda")
+    g = torch.zeros_like(q)
+    g[firsts] = torch.randn((len(lengths), heads, dim), generator=torch.Generator().manual_seed(2)).to(q.dtype).cuda()
+    _, (dq, dk, dv) = run(q, k, v, g, offsets, k_offsets)
+    assert not dq.any() and not dk.any()
+    want = g[firsts].float().view(len(lengths), kv_heads, -1, dim).sum(2)
+    got = dv[(offsets if k_offsets is None else k_offsets)[:-1].long()].float()
+    # sums of up to three numbers of 8 bits in fp32, rounded once; products with a weight that rounds to one are exact
+    assert torch.allclose(got, want, rtol=2.0 ** -8, atol=1e-6)
