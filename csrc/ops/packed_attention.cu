@@ -119,7 +119,8 @@ __device__ __forceinline__ Unit unit_of(const Forward& a, int u) {
       const int first = max(b.lo, from), last = min(b.hi, to);
       if (part > 0) b.sink = 0;
       if (first < last) b = {min(b.sink, first), first, last};
-      else b = {0, 0, b.sink};   // none but the first positions'
+      else if (b.sink > 0) b = {b.sink, max(b.sink, from), max(b.sink, from)};   // none but the first positions' (and no run of blocks up to the other tile's)
+      else b = {0, 0, 0};
     }
   }
   r.all.hi = max(r.b[0].hi, r.b[1].hi);

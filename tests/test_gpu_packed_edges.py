@@ -6,7 +6,8 @@ import pytest
 import torch
 
 from mccl_b200 import ops
-from tests.test_gpu_packed_attention import make, offsets_of
+from tests.test_gpu_packed_attention import close, make, offsets_of
+from tests.test_gpu_packed_attention import exact as exact_results
 from tests.test_gpu_packed_gradients import exact, run
 
 pytestmark = pytest.mark.gpu
@@ -119,3 +120,32 @@ def test_first_positions_have_no_gradient_of_their_score(lengths, before, heads,
     got = dv[(offsets if k_offsets is None else k_offsets)[:-1].long()].float()
     # sums of up to three numbers of 8 bits in fp32, rounded once; products with a weight that rounds to one are exact
     assert torch.allclose(got, want, rtol=2.0 ** -8, atol=1e-6)
+
+
+def test_windows_behind_a_long_cache_take_as_long_as_behind_a_short_one():
+    """Where keys are shared out, one tile's share may be the first positions alone while the other has blocks of the window: what lies between (800 blocks here, of which nothing is
+    seen) is not walked through."""
+    rows, heads, dim, window, sinks = 512, 16, 128, 2048, 4
+
+    def call(keys):
+        g = torch.Generator().manual_seed(keys)
+        q = torch.randn((rows, heads, dim), generator=g).to(torch.bfloat16).cuda()
+        k, v = (torch.randn((keys, heads, dim), generator=g).to(torch.bfloat16).cuda() for _ in range(2))
+        at = offsets_of([rows]), offsets_of([keys])
+        best = math.inf
+        for _ in range(10):
+            begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            begin.record()
+            for _ in range(5):
+                ops.packed_attention(q, k, v, *at, window=window, sinks=sinks)
+            end.record()
+            end.synchronize()
+            best = min(best, begin.elapsed_time(end))
+        # what the window and the first positions are: a text of those keys alone, whose first positions stand right in front
+        near = torch.cat((torch.arange(sinks), torch.arange(keys - rows - window + 1, keys))).cuda()
+        o, lse = ops.packed_attention(q, k, v, *at, window=window, sinks=sinks, return_lse=True)
+        close(o, lse, exact_results(q, k[near], v[near], at[0], offsets_of([len(near)]), dim ** -0.5, window, sinks), torch.bfloat16)
+        return best
+
+    short, long = call(8000), call(100_000)
+    assert long < 5 * short, (short, long)   # twice as long: an average over more shares; 30 times with the blocks between
