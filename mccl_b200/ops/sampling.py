@@ -23,7 +23,8 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: Setting 
       top_p  of these keeps the fewest likeliest whose w add up to `top_p` of the sum over these (1 or None: all; at least one stays)
       min_p  of these keeps those whose w is `min_p` or more (0 or None: all)
     The token is the lowest one at which the running sum of the kept w exceeds its row's uniform number times their whole sum.  Temperature 0: the likeliest
-    token.  Each setting is a number, or one per row (fp32 ``[rows]``; int32 for top_k); numbers count as fp32.  Sums are exact to 2^-43.
+    token.  Each setting is a number, or one per row (fp32 ``[rows]``; int32 for top_k); numbers count as fp32.  A w is off by less
+    than 2^-36 of itself and 2^-44, sums of them are exact.
 
     A row with a NaN or +inf, or with nothing finite, gives -1, and so does one whose temperature is negative or NaN."""
     settings = (temperature, 0 if top_k is None else top_k, 1.0 if top_p is None else top_p, 0.0 if min_p is None else min_p)

@@ -31,7 +31,7 @@ def pytest_collection_modifyitems(config, items):
 
 #: modules whose kernels give up a wait that runs out with an error word and incomplete results
 _STATUS = ("test_gpu_paged_attention", "test_gpu_paged_cache", "test_gpu_w4", "test_gpu_generate", "test_gpu_serving", "test_gpu_attention_weights",
-           "test_gpu_packed_attention", "test_gpu_packed_edges", "test_gpu_packed_gradients", "test_gpu_rotary", "test_gpu_sample", "test_gpu_prompts")
+           "test_gpu_packed_attention", "test_gpu_packed_edges", "test_gpu_packed_gradients", "test_gpu_rotary", "test_gpu_sample", "test_gpu_sample_weights", "test_gpu_prompts")
 
 
 @pytest.fixture(autouse=True)
