@@ -35,6 +35,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     return_lse: also the logarithm of the sum of exponentials, fp32 ``[tokens, heads]`` (-inf where nothing is seen; no gradient)."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
+    if not 0 < scale < 2e38:   # (times log2 e it must be a number of 32 bits: beyond 2.36e38 every result was NaN)
+        raise RuntimeError(f"packed_attention: scale must be a positive number below 2e38, got {scale}")
     if window is None:
         if sinks:
             raise RuntimeError("packed_attention: sinks without a window")
