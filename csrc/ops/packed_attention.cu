@@ -12,11 +12,9 @@
 // What bounds it: a block of 128 x 128 scores of 128 columns takes the tensor cores some 1024 clocks in both products, and its 16384 exponentials take the special
 // function units as long, behind which the threads of a tile have maxima, differences and conversions to do; two tiles in turn reach three quarters of the rate of a library
 // product (16381 tokens of 32 heads over 8 of 128: 1.73 ms, 1270 TFLOP/s; 2.0 ms where calls follow one another and the card's power is drawn).  A step of both tiles takes
-// 3400 clocks; per tile 200 until the scores are in registers, 500 for the maximum, 720 for each half of the exponentials, 1250 for the product with V and the next scores.  Measured on the way there:
-// the first version, two threads with products and a unit per block, 2.54 ms; products by one thread that waits once a step, and blocks that stay, 1.71; 8 texts of
-// 2048 tokens, 16 heads of 128: 190 us, with results by TMA 171.  Tried and slower: exponentials partly as polynomials, a second thread for the second tile's products
-// (both tiles then wait in step), the next unit's first scores ahead of the last products of the one before (1.75 -> 1.82 ms), two warps per row with half of the keys each (1.97 ms), the first half's
-// exponentials with the maximum so far while the block's own is found (1.76 ms).
+// 3400 clocks; per tile 200 until the scores are in registers, 500 for the maximum, 720 for each half of the exponentials, 1250 for the product with V and the next scores.
+// One thread with all products, which waits once a step, and blocks that stay: with two such threads and a unit per block 2.54 ms.  Results by TMA: 8 texts of 2048 tokens, 16
+// heads of 128, 171 us, 190 from registers.
 #include "packed_tiles.cuh"
 
 #include "smem_limit.hpp"
@@ -211,8 +209,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = *tmem_slot;
   pdl_trigger();
   // tensor memory: S of tile t in columns 128 t .. 128 t + 127, O in 256 + DP t .., P in 384 + 64 t .. where O leaves room for it.  Otherwise P is in the first 64
-  // columns of S, and the next scores are written behind its product: products of one shape (both 128 x 128 x 16) are carried out in the order they were issued
-  // in.  (Of different shapes they are not: 128 x 64 behind 128 x 128 overwrote weights that were still to be read.)
+  // columns of S, and the next scores are written there right behind the product that reads it.  What is promised is the order of products of one shape into one accumulator; these
+  // have one shape (128 x 128 x 16) and two accumulators, and that they too are carried out as they were issued is what has been seen: with a wait for the product with V in between
+  // 864 calls of 6 head dimensions gave the same bits, and 16381 x 32 heads over 8 took 2.16 ms instead of 1.99.  (Of different shapes they are not: 128 x 64 behind 128 x 128
+  // overwrote weights that were still to be read.)
   // Each role takes the units as they come; what they share in stages and phases goes on from one to the next, so that the loads and first products of a unit
   // are under way while the results of the one before are on their way out.
   if (warp >= 8) {

@@ -30,8 +30,9 @@ constexpr int kRowRegisters = 208, kOtherRegisters = 80;
 constexpr int kRoles = 8 + 3;       // warps that take a unit from the planning one
 
 // Where the 16-bit weights (or score gradients) of a tile are in tensor memory: in columns of their own where head_dim leaves room, otherwise in those of the scores,
-// each half of the threads in its own.  In the latter case the next scores are written behind the product that reads them: products of one shape, here 128 x 128
-// x 16, are carried out in the order they were issued in.
+// each half of the threads in its own.  In the latter case the next scores (dP) are written right behind the product that reads the weights (score gradients).  Promised is the order of
+// products of one shape into one accumulator; these have one shape, 128 x 128 x 16, and two accumulators, whose order is what has been seen: waits in between changed no bit of 432
+// calls of 6 head dimensions (and 8192 x 16 heads over 4 of 128 took 1268 us instead of 1185).
 template <int DP>
 constexpr int kApart = DP == 64 ? 32 : 64;
 

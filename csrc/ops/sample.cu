@@ -7,13 +7,13 @@
 //      and the few tokens in it are brought together and sorted (a step with too many is divided again, by logit and number, until it has few enough)
 //   3. sums of the kept weights per warp; the warp in whose part the random number falls goes through it once more
 // Where all tokens that min-p keeps do not fill the share of top-p, none of them lies behind its border: then the sums come with the counts, and nothing is searched
-// (64 x 128000 fp32 with settings per row: 69 -> 47 us).
+// (64 x 128000 fp32 with settings per row: 69 -> 47 us, 52 with the weights as exact as they are now).
 // Weights are whole numbers, exp((l - max) / T) 2^43 rounded, and their sums are exact: nothing depends on the order in which they are added, and the running
 // sum of 100000 tokens is off by 1e-11 of itself where sums of fp32 would be off by more than a token's weight.
 //
-// What bounds it: for one row the chain of passes and barriers (32000 tokens under top-k 50 and top-p 0.9: 11.5 us; maximum 1.1, barrier 0.6, counts 2.1, their sum over 8
-// blocks 1.5, border 0.9, list 1.7, the choice among 50 3), for many the instructions: some 60 per token with its weight, 10 us of 64 x 128000 for the pass itself, 8 for the
-// weights, 6 for the additions in shared memory.
+// What bounds it: for one row the chain of passes and barriers (32000 tokens under top-k 50 and top-p 0.9: 11.6 us; maximum 1.1, barrier 0.6, counts 2.1, their sum over 8
+// blocks 1.5, border 0.9, list 1.7, the choice among 50 3), for many the instructions: some 125 per token in all passes (64 x 128000 under top-p 0.95 and min-p
+// 0.01), at 58 % of the issue slots; 10 us of them for a pass itself, 13 for the weights, 6 for the additions in shared memory.
 #include "../core/launch.hpp"
 #include "half16.cuh"
 #include "ops.hpp"
@@ -61,7 +61,6 @@ struct Shared {
   u64 list[kList];
   u64 weights[kList];
   u64 best[kMost];                     // per block: the likeliest (composite key)
-  float least[kMost];
   int strange[kMost];
   u64 low[kMost], high[kMost];
   u64 total[kMost];
